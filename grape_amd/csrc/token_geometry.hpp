@@ -1,0 +1,135 @@
+// Which elements of a paged cache a call of the new tokens' kernels touches, and which calls are refused: the expressions that
+// the kernels and their entry points use, free of HIP so that a host build can walk over them.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+#include "../../include/grape_hip.h"
+
+#ifndef GRAPE_HD
+#ifdef __HIPCC__
+#define GRAPE_HD __host__ __device__ __forceinline__
+#else
+#define GRAPE_HD inline
+#endif
+#endif
+
+namespace grape {
+namespace token {
+
+// The positions lo <= t < hi that a sequence attends to.  False (and none) where its numbers do not fit the call.
+GRAPE_HD bool live_span(int32_t len, int32_t first, uint32_t max_len, uint32_t table_stride, uint32_t page_size, uint32_t& lo, uint32_t& hi) {
+    const bool ok = len >= 0 && first >= 0 && (uint32_t)len <= max_len && (uint64_t)len <= (uint64_t)table_stride * page_size;
+    lo = ok ? (uint32_t)first : 0;
+    hi = ok ? (uint32_t)len : 0;
+    if (lo > hi) lo = hi;
+    return ok;
+}
+
+// Offset of the first head of a page's token, or -1 where the page is outside the cache.
+GRAPE_HD int64_t token_offset(const grape_wit_cache& c, int32_t page, uint32_t in_page) {
+    if (page < 0 || (uint32_t)page >= c.pages) return -1;
+    return page * c.page_stride + (int64_t)in_page * c.token_stride;
+}
+
+// Whether a token with this slot and position is written at all (0), is padding (1) or is out of range (2).
+GRAPE_HD int append_kind(const grape_wit_cache& c, int64_t slot, int32_t position, uint32_t rot, uint32_t table_rows) {
+    if (slot < 0) return 1;
+    return slot < (int64_t)c.pages * c.page_size && (rot == 0 || (position >= 0 && (uint32_t)position < table_rows)) ? 0 : 2;
+}
+
+// Whether different slots, or heads of one, can share elements of the cache: axes in the order of their strides, each of which
+// has to step over all that the ones before it reach.
+inline bool cache_overlaps(const grape_wit_cache& c) {
+    uint64_t n[3] = {c.pages, c.page_size, c.heads}, st[3] = {(uint64_t)c.page_stride, (uint64_t)c.token_stride, (uint64_t)c.head_stride};
+    bool done[3] = {n[0] == 1, n[1] == 1, n[2] == 1};
+    unsigned __int128 extent = c.dim;
+    for (int step = 0; step < 3; step++) {
+        int at = -1;
+        for (int i = 0; i < 3; i++)
+            if (!done[i] && (at < 0 || st[i] < st[at])) at = i;
+        if (at < 0) break;
+        if (st[at] < extent) return true;
+        extent += (unsigned __int128)(n[at] - 1) * st[at];
+        done[at] = true;
+    }
+    return false;
+}
+
+#define GRAPE_REFUSE(cond, msg) \
+    if (cond) return msg
+
+inline const char* refuse_cache(const grape_wit_cache* c) {
+    GRAPE_REFUSE(!c, "cache is null");
+    GRAPE_REFUSE(!c->d_k || !c->d_v, "the cache's keys or values are null");
+    GRAPE_REFUSE(!c->pages || !c->page_size || !c->heads || !c->dim, "empty cache");
+    GRAPE_REFUSE((uint64_t)c->pages * c->page_size >= (uint64_t)1 << 31, "the cache has 2^31 slots or more");
+    GRAPE_REFUSE(c->heads > 65535 || c->dim > 16384, "at most 65535 heads of 16384 elements");
+    const int64_t most = (int64_t)1 << 40;
+    GRAPE_REFUSE(c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0, "negative stride");
+    GRAPE_REFUSE(c->page_stride >= most || c->token_stride >= most || c->head_stride >= most, "stride of 2^40 or more");
+    return nullptr;
+}
+
+// Units of work of one head and of one token of the append (see wit_append_kernel), pairs of `vec` elements each.
+GRAPE_HD uint32_t append_head_units(uint32_t dim, uint32_t rot, uint32_t vec) { return rot / (2 * vec) + (dim - rot + 2 * vec - 1) / (2 * vec); }
+
+inline const char* refuse_append(const grape_wit_rope_append_args* a, const grape_wit_cache* c) {
+    GRAPE_REFUSE(!a, "args is null");
+    if (const char* m = refuse_cache(c)) return m;
+    GRAPE_REFUSE(a->scale < 1 || a->scale > (int64_t)1 << 31, "scale must be in 1..2^31 (the remainder is stored as int32)");
+    GRAPE_REFUSE(a->rot % 2 || a->rot > c->dim, "rot must be even and at most dim");
+    GRAPE_REFUSE(a->heads > 65535, "at most 65535 heads");
+    GRAPE_REFUSE(cache_overlaps(*c), "different slots of the cache share elements");
+    GRAPE_REFUSE(a->q_stride < 0 || a->k_stride < 0 || a->v_stride < 0, "negative stride");
+    if (a->tokens == 0) return nullptr;
+    GRAPE_REFUSE(!a->d_k || !a->d_v || !a->d_slots, "d_k, d_v or d_slots is null");
+    GRAPE_REFUSE(a->heads && (!a->d_q || !a->d_q_out), "d_q or d_q_out is null");
+    GRAPE_REFUSE(a->rot && (!a->d_positions || !a->d_cos || !a->d_sin || !a->table_rows), "the positions or their tables are missing");
+    const uint64_t units = (uint64_t)(a->heads + 2 * c->heads) * append_head_units(c->dim, a->rot, 1);
+    GRAPE_REFUSE(units >= (uint64_t)1 << 31 || a->tokens * (unsigned __int128)units >= (uint64_t)1 << 38, "tensor too large");
+    return nullptr;
+}
+
+// Bytes of workspace, 0 where a call of these sizes is refused.
+inline size_t attention_workspace(uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len) {
+    if (!seqs || !heads || !cache_heads || !dim || heads > 65535 || seqs > 65535 || max_len >= (uint32_t)1 << 31) return 0;
+    if ((uint64_t)seqs * heads >= (uint64_t)1 << 38 || (unsigned __int128)((uint64_t)seqs * heads) * max_len >= (uint64_t)1 << 38) return 0;
+    return (size_t)12 * seqs * heads * max_len;
+}
+
+inline const char* refuse_attention(const grape_wit_attention_args* a, const grape_wit_cache* c) {
+    GRAPE_REFUSE(!a, "args is null");
+    if (const char* m = refuse_cache(c)) return m;
+    const int64_t most = (int64_t)1 << 31;
+    GRAPE_REFUSE(a->qk_scale < 1 || a->qk_scale > most || a->out_scale < 1 || a->out_scale > most || a->prob_scale < 1 || a->prob_scale > most / 2,
+                 "scales must be in 1..2^31, prob_scale in 1..2^30");
+    GRAPE_REFUSE(a->bit_shift < 1 || a->bit_shift > 30 || a->index_bits < 1 || a->index_bits > 30, "bit_shift and index_bits must be in 1..30");
+    GRAPE_REFUSE(a->heads < 1 || a->heads > 65535 || a->heads % c->heads, "heads must be a multiple of the cache's heads");
+    GRAPE_REFUSE(a->q_stride < 0, "negative stride");
+    if (a->seqs == 0) return nullptr;
+    GRAPE_REFUSE(a->seqs > 65535, "at most 65535 sequences");
+    GRAPE_REFUSE(a->max_len >= (uint32_t)1 << 31, "max_len must be below 2^31");
+    GRAPE_REFUSE(!a->d_q || !a->d_lens || !a->d_exp_table || !a->d_out, "d_q, d_lens, d_exp_table or d_out is null");
+    GRAPE_REFUSE(a->max_len && !a->d_block_table, "d_block_table is null");
+    GRAPE_REFUSE((unsigned __int128)((uint64_t)a->seqs * a->heads) * a->max_len >= (uint64_t)1 << 38, "tensor too large");
+    const size_t need = attention_workspace(a->seqs, a->heads, c->heads, c->dim, a->max_len);
+    GRAPE_REFUSE(a->workspace_bytes < need || (need && !a->d_workspace), "the workspace is too small");
+    GRAPE_REFUSE((uintptr_t)a->d_workspace & 15, "the workspace must be 16-byte aligned");
+    return nullptr;
+}
+
+inline const char* refuse_q4(const void* d_q, const void* d_x, int64_t x_stride, const void* d_w, int64_t w_stride, const void* d_scales,
+                             uint32_t tokens, uint32_t outputs, uint32_t inputs, uint32_t group, int64_t scale) {
+    GRAPE_REFUSE(scale < 1 || scale > (int64_t)1 << 31, "scale must be in 1..2^31 (the remainder is stored as int32)");
+    GRAPE_REFUSE(inputs < 1 || group < 1, "empty inner dimension or group");
+    GRAPE_REFUSE(inputs > (uint32_t)1 << 30, "at most 2^30 inputs");
+    GRAPE_REFUSE(x_stride < 0 || w_stride < 0, "negative stride");
+    if (!tokens || !outputs) return nullptr;
+    GRAPE_REFUSE(!d_q || !d_x || !d_w || !d_scales, "d_q, d_x, d_w or d_scales is null");
+    GRAPE_REFUSE((uint64_t)tokens * outputs >= (uint64_t)1 << 38, "tensor too large");
+    return nullptr;
+}
+#undef GRAPE_REFUSE
+
+}  // namespace token
+}  // namespace grape

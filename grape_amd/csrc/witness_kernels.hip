@@ -9,25 +9,9 @@
 // (quotients fit 32 bits) are recorded in a sticky device-side status word, read and cleared by
 // grape_wit_status().
 #include "common.hpp"
+#include "witness_device.hpp"
 
 namespace grape {
-
-enum WitFlag : uint32_t { kWitQuotient = 1, kWitIndex = 2, kWitSum = 4, kWitSquares = 8 };
-
-// floor((y + s/2) / s) and the centred remainder; s > 0, sh = log2(s) or -1 when s is no power of 2
-__device__ __forceinline__ void rescale64(int64_t y, int64_t s, int sh, int32_t& q, int32_t& r, uint32_t& bad) {
-    const int64_t t = y + (s >> 1);
-    int64_t qq;
-    if (sh >= 0) {
-        qq = t >> sh;                         // arithmetic shift floors
-    } else {
-        qq = t / s;
-        if ((t % s != 0) && (t < 0)) qq -= 1;  // C division truncates; floor wanted
-    }
-    bad |= (qq != (int64_t)(int32_t)qq) ? (uint32_t)kWitQuotient : 0u;
-    q = (int32_t)qq;
-    r = (int32_t)(y - qq * s);
-}
 
 // ------------------------------------------------------------------------------------------------
 // Y[l][n][m] = sum_k A[l][n][k] * B[l][m][k], rescaled.  Tile 128 x 128 x 32 per workgroup of 256
@@ -710,7 +694,7 @@ __global__ void wit_status_clear_kernel(uint32_t* status) { *status = 0; }
 
 static uint32_t* g_status[16] = {nullptr};
 
-static int status_word(uint32_t** out, hipStream_t s) {
+int wit_status_word(uint32_t** out, hipStream_t s) {
     int dev = 0;
     GRAPE_HIP_CHECK(hipGetDevice(&dev));
     GRAPE_REQUIRE(dev >= 0 && dev < 16, "device index out of range");
@@ -733,13 +717,6 @@ static int planes_for(uint32_t maxabs) {
     if (maxabs < (1u << 22)) return 3;
     if (maxabs < (1u << 30)) return 4;
     return 5;
-}
-
-static int log2_exact(int64_t s) {
-    if (s <= 0 || (s & (s - 1)) != 0) return -1;
-    int sh = 0;
-    while ((((int64_t)1) << sh) != s) sh++;
-    return sh;
 }
 
 }  // namespace grape
@@ -768,7 +745,7 @@ int grape_wit_matmul_rescale(int32_t* d_q, int32_t* d_r, const int32_t* d_a, con
     p.transpose_out = transpose_out ? 1 : 0;
     p.tiles_n = (N + kTM - 1) / kTM;
     p.tiles_m = (M + kTM - 1) / kTM;
-    int rc = status_word(&p.status, s);
+    int rc = wit_status_word(&p.status, s);
     if (rc) return rc;
     const bool aligned = (K % 4 == 0) && ((reinterpret_cast<uintptr_t>(d_a) | reinterpret_cast<uintptr_t>(d_b)) & 15) == 0;
     // matrix-core path: one batch, aligned rows, operands of at most three byte planes each.  The split into
@@ -863,7 +840,7 @@ int grape_wit_elemul_rescale(int32_t* d_q, int32_t* d_r, const int32_t* d_a, con
     CHECK_PTR(d_q); CHECK_PTR(d_a); CHECK_PTR(d_b);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = status_word(&status, s);
+    int rc = wit_status_word(&status, s);
     if (rc) return rc;
     wit_elemul_rescale_kernel<<<blocks_for(n), kBlock, 0, s>>>(d_q, d_r, d_a, d_b, n, scale, log2_exact(scale), status);
     GRAPE_LAUNCH_CHECK();
@@ -877,7 +854,7 @@ int grape_wit_table_lookup(int32_t* d_out, const int32_t* d_in, size_t n, int32_
     CHECK_PTR(d_out); CHECK_PTR(d_in); CHECK_PTR(d_table);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = status_word(&status, s);
+    int rc = wit_status_word(&status, s);
     if (rc) return rc;
     if (((reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(d_in)) & 15) == 0)
         wit_lookup_kernel<true><<<blocks_for((n + 3) / 4), kBlock, 0, s>>>(d_out, d_in, n, low, len, d_table, status);
@@ -907,7 +884,7 @@ int grape_wit_softmax(int32_t* d_max, int32_t* d_shifted, int32_t* d_exp, int32_
     CHECK_PTR(d_scores); CHECK_PTR(d_table);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = status_word(&status, s);
+    int rc = wit_status_word(&status, s);
     if (rc) return rc;
     wit_softmax_kernel<<<rows, kBlock, 0, s>>>(d_max, d_shifted, d_exp, d_sum, d_prob, d_query, d_scores, cols, d_table,
                                                (1u << bit_shift) - 1u, 1u << index_bits, scale, status);
@@ -922,7 +899,7 @@ int grape_wit_row_sumsq(uint64_t* d_out, const int32_t* d_x, uint32_t rows, uint
     CHECK_PTR(d_out); CHECK_PTR(d_x);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = status_word(&status, s);
+    int rc = wit_status_word(&status, s);
     if (rc) return rc;
     wit_row_sumsq_kernel<<<rows, kBlock, 0, s>>>(d_out, d_x, cols, status);
     GRAPE_LAUNCH_CHECK();
@@ -938,7 +915,7 @@ int grape_wit_rmsnorm_apply(int32_t* d_q_rmsw, int32_t* d_r_rmsw, int32_t* d_q_o
     CHECK_PTR(d_q_rmsw); CHECK_PTR(d_r_rmsw); CHECK_PTR(d_q_out); CHECK_PTR(d_r_out); CHECK_PTR(d_x); CHECK_PTR(d_rms); CHECK_PTR(d_w);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = status_word(&status, s);
+    int rc = wit_status_word(&status, s);
     if (rc) return rc;
     const size_t n = (size_t)rows * cols;
     wit_rmsnorm_apply_kernel<<<blocks_for(n), kBlock, 0, s>>>(d_q_rmsw, d_r_rmsw, d_q_out, d_r_out, d_x, d_rms, d_w, n, cols, scale,
@@ -952,7 +929,7 @@ int grape_wit_status(uint32_t* flags, grape_stream_t st) {
     CHECK_PTR(flags);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = status_word(&status, s);
+    int rc = wit_status_word(&status, s);
     if (rc) return rc;
     GRAPE_HIP_CHECK(hipMemcpyAsync(flags, status, sizeof(uint32_t), hipMemcpyDeviceToHost, s));
     GRAPE_HIP_CHECK(hipStreamSynchronize(s));

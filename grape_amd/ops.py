@@ -7,6 +7,8 @@ BLS12-381 and (n, 16) for BN254.  Host-side values travel as numpy uint64 arrays
 Every helper enqueues on torch's current stream.
 """
 import ctypes
+import struct
+
 import numpy as np
 import torch
 
@@ -727,6 +729,153 @@ def wit_rmsnorm_apply(x, rms, w, scale=1 << 16):
     _capi.check(lib.grape_wit_rmsnorm_apply(_p(outs[0]), _p(outs[1]), _p(outs[2]), _p(outs[3]), _p(x), _p(rms), _p(w), rows, cols,
                                             int(scale), _s()))
     return outs
+
+
+# ------------------------------------------------------------------ the witness of new tokens
+def _need(cond, msg):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _place():
+    return torch.device("cuda", torch.cuda.current_device())
+
+
+def _arr(t, name, shape, dev, dtype=torch.int32):
+    """address of a contiguous tensor of that shape and type on the current device; 0 for None"""
+    if t is None:
+        return 0
+    _need(t.dtype is dtype and t.device == dev and t.shape == shape and t.is_contiguous(),
+          "%s must be a contiguous %s tensor of shape %s on the current device" % (name, dtype, tuple(shape)))
+    return t.data_ptr()
+
+
+def _rows(t, name, shape, dev, dtype=torch.int32):
+    """the same for rows (all but the first axis) that are contiguous each; address and elements from row to row"""
+    _need(t.dtype is dtype and t.device == dev and t.shape == shape, "%s must be a %s tensor of shape %s on the current device" % (name, dtype, tuple(shape)))
+    if t.is_contiguous():
+        return t.data_ptr(), t.numel() // max(t.shape[0], 1)
+    step = 1
+    for n, s in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        _need(n == 1 or s == step, "the rows of %s must be contiguous" % name)
+        step *= n
+    return t.data_ptr(), t.stride(0)
+
+
+_CACHE = struct.Struct("<2Q4I3q")
+_APPEND = struct.Struct("<3Q3q7Q4Iq2i")
+_ATTEND = struct.Struct("<Qq16Q3q6I")
+
+
+def _cache(k_cache, v_cache, dev):
+    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(),
+          "the caches must be (pages, page size, heads, dim) tensors of the same shape and strides")
+    _need(k_cache.dtype is torch.int32 and v_cache.dtype is torch.int32 and k_cache.device == dev and v_cache.device == dev,
+          "the caches must be int32 tensors on the current device")
+    _need(k_cache.stride(3) == 1 or k_cache.shape[3] == 1, "the elements of a head must be contiguous")
+    pages, page, heads, dim = k_cache.shape
+    return _CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), pages, page, heads, dim, *k_cache.stride()[:3])
+
+
+def wit_rope_append(q, k, v, positions, slots, cos, sin, k_cache, v_cache, q_out=None, q_rem=None, k_rem=None, scale=1 << 16, interleaved=False):
+    """Rotates q (tokens, heads, dim) and k (tokens, cache heads, dim) by positions (int32) with the tables cos, sin (rows,
+    rot/2) at `scale`, and puts k and v into slots (int64: page * page size + offset; negative: padding, left out) of the caches
+    (pages, page size, cache heads, dim).  Tokens may be strided.  Returns q_out; remainders go to q_rem and k_rem if given.
+    q = None (with q_out None): keys and values only."""
+    lib = init()
+    dev = _place()
+    cache = _cache(k_cache, v_cache, dev)
+    heads_kv, dim = k_cache.shape[2:]
+    n = k.shape[0]
+    kp, ks = _rows(k, "k", (n, heads_kv, dim), dev)
+    vp, vs = _rows(v, "v", (n, heads_kv, dim), dev)
+    qp = qs = heads = 0
+    if q is not None:
+        _need(q.dim() == 3 and q.shape[1] >= 1, "q must be (tokens, heads, dim)")
+        heads = q.shape[1]
+        qp, qs = _rows(q, "q", (n, heads, dim), dev)
+        if q_out is None:
+            q_out = torch.zeros((n, heads, dim), dtype=torch.int32, device=dev)      # rows of padding are not written
+    else:
+        _need(q_out is None and q_rem is None, "q_out and q_rem need q")
+    _need(cos.dim() == 2 and cos.shape == sin.shape, "cos and sin must be (rows, rot / 2) tensors")
+    rows, half = cos.shape
+    args = _APPEND.pack(qp, kp, vp, qs, ks, vs, _arr(positions, "positions", (n,), dev), _arr(slots, "slots", (n,), dev, torch.int64),
+                        _arr(cos, "cos", (rows, half), dev), _arr(sin, "sin", (rows, half), dev),
+                        _arr(q_out, "q_out", (n, heads, dim), dev), _arr(q_rem, "q_rem", (n, heads, dim), dev),
+                        _arr(k_rem, "k_rem", (n, heads_kv, dim), dev), n, heads, 2 * half, rows, int(scale), 1 if interleaved else 0, 0)
+    _capi.check(lib.grape_wit_rope_append(args, cache, _s()))
+    return q_out
+
+
+# what a proof looks up of an attention, [seqs][heads][max_len] each, in the order of the C ABI's fields
+_PROOF_ROWS = ("scores", "scores_rem", "exp_input", "exp_output", "softmax_output", "softmax_lookup_query")
+
+
+def wit_paged_attention(q, k_cache, v_cache, block_table, lens, max_len, exp_table, first=None, bit_shift=20, index_bits=20,
+                        qk_scale=1 << 22, prob_scale=1 << 16, out_scale=1 << 16, out=None, proof=True, workspace=None):
+    """Attention of one token a sequence, q (seqs, heads, dim), over the positions first[b] <= t < lens[b] of the caches (pages,
+    page size, cache heads, dim) through block_table (seqs, pages of a sequence).  Returns a dict: "qkv" and "qkv_rem" (seqs,
+    heads, dim); for a proof also "max" and "exp_sum" (seqs, heads) and "scores", "scores_rem", "exp_input", "exp_output",
+    "softmax_output", "softmax_lookup_query" (seqs, heads, max_len), whose entries outside a sequence's positions are not
+    written.  `out`: such a dict of tensors to write to; "qkv" has to be there, the others may be left out.  `workspace`: a uint8
+    tensor of wit_paged_attention_workspace(...) bytes; without one the call makes its own."""
+    lib = init()
+    dev = _place()
+    cache = _cache(k_cache, v_cache, dev)
+    dim = k_cache.shape[3]
+    _need(q.dim() == 3, "q must be (seqs, heads, dim)")
+    n, heads = q.shape[:2]
+    qp, qs = _rows(q, "q", (n, heads, dim), dev)
+    _need(block_table.dim() == 2, "block_table must be (seqs, pages)")
+    width = block_table.shape[1]
+    _need(exp_table.shape == (1 << index_bits,), "the exponential table must have 2^index_bits entries")
+    _need(max_len >= 0, "max_len must not be negative")
+    if out is None:
+        out = {"qkv": _i32(n, heads, dim), "qkv_rem": _i32(n, heads, dim)}
+        if proof:
+            out["max"], out["exp_sum"] = _i32(n, heads), _i32(n, heads)
+            for name in _PROOF_ROWS:
+                out[name] = torch.zeros((n, heads, max_len), dtype=torch.int32, device=dev)
+    shapes = dict.fromkeys(_PROOF_ROWS, (n, heads, max_len))
+    shapes.update(max=(n, heads), exp_sum=(n, heads), qkv=(n, heads, dim), qkv_rem=(n, heads, dim))
+    _need("qkv" in out and not set(out) - set(shapes), "out must hold qkv, and may hold %s" % ", ".join(x for x in shapes if x != "qkv"))
+    at = [_arr(out.get(name), name, shape, dev) for name, shape in shapes.items()]
+    if workspace is None:
+        workspace = torch.empty(wit_paged_attention_workspace(n, heads, k_cache.shape[2], dim, max_len), dtype=torch.uint8, device=dev)
+    _need(workspace.dtype is torch.uint8 and workspace.device == dev and workspace.is_contiguous(), "the workspace must be a contiguous uint8 tensor")
+    args = _ATTEND.pack(qp, qs, _arr(block_table, "block_table", (n, width), dev), _arr(lens, "lens", (n,), dev), _arr(first, "first", (n,), dev),
+                        _arr(exp_table, "exp_table", exp_table.shape, dev), *at, workspace.data_ptr(), workspace.numel(),
+                        int(qk_scale), int(prob_scale), int(out_scale), n, heads, max_len, width, bit_shift, index_bits)
+    _capi.check(lib.grape_wit_paged_attention(args, cache, _s()))
+    return out
+
+
+def wit_paged_attention_workspace(seqs, heads, cache_heads, dim, max_len):
+    """bytes of workspace that wit_paged_attention needs"""
+    return init().grape_wit_paged_attention_workspace(seqs, heads, cache_heads, dim, max_len)
+
+
+def wit_matvec_q4(x, w, scales, group, zeros=None, scale=1 << 16, q=None, r=None, want_r=True):
+    """x (tokens, inputs) int32 times 4-bit weights w (outputs, ceil(inputs / 2)) uint8, the even input in the lower half, with
+    scales (outputs, ceil(inputs / group)) int32 and zero points (the same, uint8; None: all 8).  Returns quotient, remainder."""
+    lib = init()
+    dev = _place()
+    _need(x.dim() == 2 and w.dim() == 2 and group >= 1, "x must be (tokens, inputs), w (outputs, bytes), group positive")
+    n, k = x.shape
+    m = w.shape[0]
+    _need(k >= 1, "empty inner dimension")
+    groups = (k - 1) // group + 1
+    xp, xs = _rows(x, "x", (n, k), dev)
+    wp, ws = _rows(w, "w", (m, (k + 1) // 2), dev, torch.uint8)
+    if q is None:
+        q = _i32(n, m)
+    if r is None and want_r:
+        r = _i32(n, m)
+    _capi.check(lib.grape_wit_matvec_q4(_arr(q, "q", (n, m), dev), _arr(r, "r", (n, m), dev), xp, xs, wp, ws,
+                                        _arr(scales, "scales", (m, groups), dev), _arr(zeros, "zeros", (m, groups), dev, torch.uint8),
+                                        n, m, k, group, int(scale), _s()))
+    return q, r
 
 
 def wit_status():

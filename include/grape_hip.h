@@ -694,6 +694,80 @@ int grape_wit_row_sumsq(uint64_t *d_out, const int32_t *d_x, uint32_t rows, uint
 int grape_wit_rmsnorm_apply(int32_t *d_q_rmsw, int32_t *d_r_rmsw, int32_t *d_q_out, int32_t *d_r_out, const int32_t *d_x,
                             const int32_t *d_rms, const int32_t *d_w, uint32_t rows, uint32_t cols, int64_t scale,
                             grape_stream_t stream);
+/* The forms for new tokens.  The reference's generator takes whole prompts, with one head and no rotation (model.py:473-590);
+ * to prove an answer token by token a block needs the token's projections, its rotated key and its value behind those of
+ * the tokens before it, and its attention over them.  The rules of arithmetic are the ones above; no counterpart in the
+ * reference.  All of these are enqueued only, need no scratch of the stream's pool and record nothing but kernels.
+ *
+ * Keys and values of a cache stand in pages of page_size tokens each: element d of head h of the token at `offset` of page p
+ * is d_k[p*page_stride + offset*token_stride + h*head_stride + d] (strides in elements, the same for d_v).  A slot is
+ * p*page_size + offset.  At most 2^31 - 1 slots; sizes >= 1, strides >= 0. */
+typedef struct {
+    int32_t *d_k, *d_v;
+    uint32_t pages, page_size, heads, dim;
+    int64_t page_stride, token_stride, head_stride;
+} grape_wit_cache;
+/* Rotates the queries and keys of `tokens` tokens by their positions, appends keys and values to the cache and writes the
+ * rotated queries.  Token t's queries stand at d_q + t*q_stride as [heads][dim] and its keys and values at d_k + t*k_stride
+ * and d_v + t*v_stride as [cache heads][dim].  Of every head's first `rot` elements (even, at most dim) the pair j - elements
+ * (j, j + rot/2), or (2j, 2j + 1) with `interleaved` - becomes
+ *     x0*cos[pos][j] - x1*sin[pos][j]  and  x0*sin[pos][j] + x1*cos[pos][j],  both rescaled by `scale` (1..2^31),
+ * with cos and sin of table_rows x rot/2 elements; the others keep their value, with remainder 0.  Quotients go to
+ * d_q_out [tokens][heads][dim] and the cache, remainders to d_q_rem [tokens][heads][dim] and d_k_rem [tokens][cache
+ * heads][dim] (either may be NULL).  heads = 0 appends only.  d_q_out may be d_q itself where q_stride = heads*dim.
+ *
+ * A negative slot marks padding: nothing of that token is written.  A slot behind the cache's end or a position outside the
+ * tables sets GRAPE_WIT_INDEX, and nothing of that token is written either.  Where several tokens name one slot, the last of
+ * them has its rows there.  Different slots must not share elements of the cache (checked from the strides). */
+typedef struct {
+    const int32_t *d_q, *d_k, *d_v;
+    int64_t q_stride, k_stride, v_stride;
+    const int32_t *d_positions;
+    const int64_t *d_slots;
+    const int32_t *d_cos, *d_sin;
+    int32_t *d_q_out, *d_q_rem, *d_k_rem;
+    uint32_t tokens, heads, rot, table_rows;
+    int64_t scale;
+    int32_t interleaved, reserved;
+} grape_wit_rope_append_args;
+int grape_wit_rope_append(const grape_wit_rope_append_args *args, const grape_wit_cache *cache, grape_stream_t stream);
+/* Attention of one new token a sequence over the cache.  Sequence b attends to the positions first <= t < len (d_lens[b];
+ * d_first[b], or 0 where d_first is NULL), whose keys and values stand in page d_block_table[b*table_stride + t/page_size]
+ * at offset t % page_size.  Head h of `heads` (a multiple of the cache's) reads the cache's head h / (heads / cache heads):
+ *     scores = rescale(q . k_t, qk_scale), max over t, shifted = score - max, exp = d_exp_table[shifted + 2^bit_shift - 1]
+ *     (2^index_bits entries), sum of exp, prob = floor((exp*prob_scale + floor(sum/2)) / sum),
+ *     query = 2*prob_scale*exp - sum*(2*prob - 1), out = rescale(sum_t prob_t v_t, out_scale)
+ * - grape_wit_matmul_rescale, grape_wit_softmax and grape_wit_matmul_rescale again, with the same bits of status.
+ * The rows of a proof, [seqs][heads][max_len], d_scores, d_scores_rem, d_shifted, d_exp, d_prob and d_query, and
+ * d_max, d_sum [seqs][heads] and d_out_rem may each be NULL; d_out and d_out_rem are [seqs][heads][dim].  Positions outside
+ * first..len are left as they were; a row with no position has max, sum, out and remainder 0.
+ *
+ * max_len bounds every length.  A len above it or above table_stride*page_size, a negative len or first sets GRAPE_WIT_INDEX
+ * and makes the sequence's rows empty; a page outside the cache sets it too, and its keys and values count as zero.
+ * 1 <= scales <= 2^31 (prob_scale <= 2^30), dim <= 16384.
+ *
+ * d_workspace (16-byte aligned) holds what the launches hand on to each other, grape_wit_paged_attention_workspace(...) bytes;
+ * it needs no initial contents, and calls that may run at the same time, replays of captured ones among them, need one each. */
+typedef struct {
+    const int32_t *d_q;
+    int64_t q_stride;
+    const int32_t *d_block_table, *d_lens, *d_first, *d_exp_table;
+    int32_t *d_scores, *d_scores_rem, *d_shifted, *d_exp, *d_prob, *d_query, *d_max, *d_sum, *d_out, *d_out_rem;
+    void *d_workspace;
+    size_t workspace_bytes;
+    int64_t qk_scale, prob_scale, out_scale;
+    uint32_t seqs, heads, max_len, table_stride, bit_shift, index_bits;
+} grape_wit_attention_args;
+size_t grape_wit_paged_attention_workspace(uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len);
+int grape_wit_paged_attention(const grape_wit_attention_args *args, const grape_wit_cache *cache, grape_stream_t stream);
+/* Products with 4-bit weights: y[n][m] = sum_k x[n][k] * scale[m][k/group] * (w[m][k] - zero[m][k/group]), rescaled as
+ * grape_wit_matmul_rescale does it - its result for the weights written out as integers.  Token n's inputs stand at
+ * d_x + n*x_stride; row m of the weights at d_w + m*w_stride bytes, two to a byte, the even k in the lower half, (inputs + 1)/2
+ * bytes; scales int32 and zero points bytes (d_zeros NULL: all 8), ceil(inputs/group) a row; outputs [tokens][outputs], d_r
+ * may be NULL.  1 <= scale <= 2^31. */
+int grape_wit_matvec_q4(int32_t *d_q, int32_t *d_r, const int32_t *d_x, int64_t x_stride, const uint8_t *d_w, int64_t w_stride,
+                        const int32_t *d_scales, const uint8_t *d_zeros, uint32_t tokens, uint32_t outputs, uint32_t inputs,
+                        uint32_t group, int64_t scale, grape_stream_t stream);
 /* Synchronises, returns the status bits set since the last call and clears them: 1 = a quotient left
  * int32, 2 = a table index out of range (the reference's assertions, model.py:86-87, :137-138),
  * 4 = a softmax row summed to zero or met a negative table entry, 8 = a sum of squares left 64 bits. */

@@ -174,3 +174,83 @@ def layer(x, weights, tables, eps=NORM_EPS):
     out.update(feed_forward(n2["q_out"], weights["gate"], weights["down"], weights["up"], tables["silu"]))
     out["Q/output"] = (h.astype(np.int64) + out["Q/down_out"]).astype(np.int32)
     return out
+
+
+# ------------------------------------------------------------------ new tokens
+# The reference takes whole prompts with one head, no rotation and no cache (:473-590).  The forms for new tokens use its
+# rules of arithmetic; their definitions are those of include/grape_hip.h.
+def rotate(x, positions, cos, sin, interleaved, scale=SCALE):
+    """x (tokens, heads, dim), tables (rows, rot/2) -> quotient, remainder of the rotated elements"""
+    x = np.asarray(x, dtype=np.int64)
+    y = x * scale
+    half = cos.shape[1]
+    for j in range(half):
+        a, b = (2 * j, 2 * j + 1) if interleaved else (j, j + half)
+        c, s = (t[positions, j].astype(np.int64)[:, None] for t in (cos, sin))
+        y[:, :, a] = x[:, :, a] * c - x[:, :, b] * s
+        y[:, :, b] = x[:, :, a] * s + x[:, :, b] * c
+    return rescale(y, scale)
+
+
+def rope_append(q, k, v, positions, slots, cos, sin, k_cache, v_cache, q_out, q_rem, k_rem, interleaved, scale=SCALE):
+    """writes into the caches (pages, page size, heads, dim), q_out, q_rem and k_rem, token after token"""
+    live = [t for t in range(len(slots)) if slots[t] >= 0]
+    page = k_cache.shape[1]
+    at = np.asarray(positions)[live]
+    qq, qr = rotate(q[live], at, cos, sin, interleaved, scale)
+    kq, kr = rotate(k[live], at, cos, sin, interleaved, scale)
+    for i, t in enumerate(live):
+        q_out[t], q_rem[t], k_rem[t] = qq[i], qr[i], kr[i]
+        k_cache[slots[t] // page, slots[t] % page] = kq[i]
+        v_cache[slots[t] // page, slots[t] % page] = v[t]
+
+
+def paged_attention(q, k_cache, v_cache, block_table, lens, first, table, out, qk_scale=QK_SCALE, prob_scale=SCALE, out_scale=SCALE,
+                    bit_shift=EXP_BIT_SHIFT, index_bits=EXP_INDEX_BITS):
+    """q (seqs, heads, dim); writes the tensors of `out` (names of the softmax's tensors, scores, scores_rem, qkv, qkv_rem),
+    entries of positions outside first..len left as they are"""
+    seqs, heads, dim = q.shape
+    page, kv_heads = k_cache.shape[1:3]
+    for b in range(seqs):
+        at = np.arange(first[b], lens[b])
+        pages = np.asarray(block_table)[b, at // page]
+        inside = (pages >= 0) & (pages < k_cache.shape[0])
+        keys, values = (np.where(inside[:, None, None], c[np.where(inside, pages, 0), at % page], 0).astype(np.int64) for c in (k_cache, v_cache))
+        for h in range(heads):
+            kv = h // (heads // kv_heads)
+            one = {"max": 0, "exp_sum": 0, "qkv": 0, "qkv_rem": 0}
+            if len(at):
+                rows = {}
+                rows["scores"], rows["scores_rem"] = rescale((keys[:, kv] * q[b, h].astype(np.int64)).sum(1), qk_scale)
+                one["max"] = int(rows["scores"].max())
+                rows["exp_input"] = rows["scores"].astype(np.int64) - one["max"]
+                e = rows["exp_output"] = lut(rows["exp_input"], table, (1 << bit_shift) - 1, index_bits).astype(np.int64)
+                total = one["exp_sum"] = int(e.sum())
+                if total <= 0 or np.any(e < 0):
+                    raise ValueError("softmax row sums to zero")
+                p = rows["softmax_output"] = (e * prob_scale + total // 2) // total
+                rows["softmax_lookup_query"] = e * 2 * prob_scale - total * (2 * p - 1)
+                one["qkv"], one["qkv_rem"] = rescale((values[:, kv] * p[:, None]).sum(0), out_scale)
+                for name, x in rows.items():
+                    if name in out:
+                        out[name][b, h, first[b]:lens[b]] = np.asarray(x).astype(np.int64).astype(np.int32)
+            for name, x in one.items():
+                if name in out:
+                    out[name][b, h] = x
+
+
+def unpack_q4(w, inputs):
+    """(outputs, ceil(inputs / 2)) bytes -> (outputs, inputs) values 0..15, the even input in the lower half"""
+    w = np.asarray(w)
+    return np.stack((w & 15, w >> 4), axis=-1).reshape(w.shape[0], -1)[:, :inputs].astype(np.int64)
+
+
+def weights_q4(w, scales, group, zeros, inputs):
+    """the weights written out as integers: scale * (w - zero)"""
+    which = np.arange(inputs) // group
+    z = np.asarray(zeros)[:, which].astype(np.int64) if zeros is not None else 8
+    return np.asarray(scales)[:, which].astype(np.int64) * (unpack_q4(w, inputs) - z)
+
+
+def matvec_q4(x, w, scales, group, zeros, scale=SCALE):
+    return rescale(matmul_t(x, weights_q4(w, scales, group, zeros, x.shape[1])), scale)

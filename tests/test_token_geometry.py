@@ -1,0 +1,228 @@
+"""CPU checks of what the new tokens' entry points refuse, which positions and pages they touch, and how the Python helpers
+check and pack their arguments (the expressions of grape_amd/csrc/token_geometry.hpp, in a host build)."""
+import ctypes
+import os
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+from grape_amd import ops
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+SRC = os.path.join(HERE, "native", "token_geometry_host.cpp")
+LIB = os.path.join(HERE, "native", "libtoken_geometry_host.so")
+HDRS = (os.path.join(HERE, "..", "grape_amd", "csrc", "token_geometry.hpp"), os.path.join(HERE, "..", "include", "grape_hip.h"))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(LIB) or any(os.path.getmtime(d) > os.path.getmtime(LIB) for d in (SRC,) + HDRS):
+        subprocess.check_call(["g++", "-O1", "-std=c++17", "-Wall", "-fPIC", "-shared", "-o", LIB, SRC])
+    l = ctypes.CDLL(LIB)
+    p, u, i, q = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_int32, ctypes.c_int64
+    for name in ("refuse_append", "refuse_attention", "refuse_q4"):
+        getattr(l, name).restype = ctypes.c_char_p
+    l.refuse_append.argtypes = l.refuse_attention.argtypes = [p, p]
+    l.refuse_q4.argtypes = [p, p, q, p, q, p, u, u, u, u, q]
+    l.struct_bytes.restype = l.workspace.restype = ctypes.c_size_t
+    l.overlaps.argtypes = [p]
+    l.span.argtypes = [i, i, u, u, u, p]
+    l.offset_of.argtypes, l.offset_of.restype = [p, i, u], q
+    l.kind.argtypes = [p, q, i, u, u]
+    l.workspace.argtypes = [u] * 5
+    l.append_fields.argtypes = l.attention_fields.argtypes = l.cache_fields.argtypes = [p, p]
+    return l
+
+
+CACHE = dict(k=16, v=32, pages=10, page=16, heads=4, dim=64, ps=16 * 4 * 64, ts=4 * 64, hs=64)
+APPEND = dict(q=16, k=32, v=48, qs=512, ks=256, vs=256, pos=64, slots=80, cos=96, sin=112, qo=128, qr=0, kr=0, n=3, heads=8, rot=64, rows=100, scale=65536,
+              inter=0, res=0)
+ATTEND = dict(q=16, qs=512, table=32, lens=48, first=0, exp=64, s=0, sr=0, x=0, e=0, p=0, lq=0, mx=0, sm=0, o=80, r=0, ws=96, wb=1 << 30, qk=1 << 22, pr=1 << 16,
+              os=1 << 16, n=2, heads=8, max_len=100, ts=10, shift=20, bits=20)
+
+
+def cache(**kw):
+    return ops._CACHE.pack(*{**CACHE, **kw}.values())
+
+
+def append(**kw):
+    return ops._APPEND.pack(*{**APPEND, **kw}.values())
+
+
+def attend(**kw):
+    return ops._ATTEND.pack(*{**ATTEND, **kw}.values())
+
+
+def test_helpers_pack_the_structs_of_the_header(lib):
+    for which, s, fields in ((0, ops._CACHE, lib.cache_fields), (1, ops._APPEND, lib.append_fields), (2, ops._ATTEND, lib.attention_fields)):
+        assert lib.struct_bytes(which) == s.size
+        n = len(s.unpack(bytes(s.size)))
+        values = [i + 1 for i in range(n)]
+        out = (ctypes.c_int64 * n)()
+        fields(s.pack(*values), out)
+        assert list(out) == values
+
+
+@pytest.mark.parametrize("bad", [dict(k=0), dict(v=0), dict(pages=0), dict(page=0), dict(heads=0), dict(dim=0), dict(pages=1 << 27), dict(heads=65536),
+                                 dict(dim=16385), dict(ps=-1), dict(ts=-1), dict(hs=-1), dict(ps=1 << 40), dict(hs=1 << 40)])
+def test_bad_caches_are_refused(lib, bad):
+    assert lib.refuse_append(append(), cache()) is None and lib.refuse_attention(attend(), cache()) is None
+    assert lib.refuse_append(append(), cache(**bad)) and lib.refuse_attention(attend(), cache(**bad))
+    assert lib.refuse_append(append(), None) and lib.refuse_attention(attend(), None)
+    assert lib.refuse_append(None, cache()) and lib.refuse_attention(None, cache())
+
+
+@pytest.mark.parametrize("bad", [dict(scale=0), dict(scale=-1), dict(scale=(1 << 31) + 1), dict(rot=63), dict(rot=66), dict(heads=65536), dict(qs=-1), dict(ks=-1),
+                                 dict(vs=-1), dict(k=0), dict(v=0), dict(slots=0), dict(q=0), dict(qo=0), dict(pos=0), dict(cos=0), dict(sin=0), dict(rows=0),
+                                 dict(n=(1 << 32) - 1)])
+def test_bad_appends_are_refused(lib, bad):
+    assert lib.refuse_append(append(**bad), cache())
+
+
+def test_appends_that_are_taken(lib):
+    for ok in (dict(heads=0, q=0, qo=0), dict(rot=0, pos=0, cos=0, sin=0, rows=0), dict(n=0, k=0, v=0, slots=0), dict(scale=1), dict(scale=1 << 31), dict(qs=0)):
+        assert lib.refuse_append(append(**ok), cache()) is None
+
+
+@pytest.mark.parametrize("bad", [dict(qk=0), dict(qk=(1 << 31) + 1), dict(pr=0), dict(pr=(1 << 30) + 1), dict(os=0), dict(os=(1 << 31) + 1), dict(shift=0), dict(shift=31),
+                                 dict(bits=0), dict(bits=31), dict(heads=0), dict(heads=6), dict(heads=2), dict(heads=65536), dict(qs=-1), dict(n=65536), dict(max_len=1 << 31),
+                                 dict(q=0), dict(lens=0), dict(exp=0), dict(o=0), dict(table=0), dict(ws=0), dict(wb=10), dict(ws=100), dict(n=60000, heads=60000)])
+def test_bad_attentions_are_refused(lib, bad):
+    assert lib.refuse_attention(attend(**bad), cache())
+
+
+@pytest.mark.parametrize("bad", [dict(scale=0), dict(scale=(1 << 31) + 1), dict(k=0), dict(group=0), dict(k=(1 << 30) + 1), dict(xs=-1), dict(ws=-1), dict(q=0), dict(x=0), dict(w=0),
+                                 dict(sc=0), dict(n=1 << 20, m=1 << 20)])
+def test_bad_products_are_refused(lib, bad):
+    good = dict(q=16, x=16, xs=64, w=16, ws=32, sc=16, n=2, m=8, k=64, group=32, scale=65536)
+    assert lib.refuse_q4(*good.values()) is None
+    assert lib.refuse_q4(*{**good, "n": 0, "q": 0}.values()) is None
+    assert lib.refuse_q4(*{**good, **bad}.values())
+
+
+def test_overlapping_caches_are_found(lib):
+    """against the elements themselves"""
+    rng = np.random.default_rng(1)
+    seen = set()
+    for _ in range(3000):
+        n = [int(x) for x in rng.integers(1, 5, 4)]
+        st = [int(x) for x in rng.choice([0, 1, 2, 3, 4, 6, 8, 12, 16, 24, 48], 3)]
+        at = (np.arange(n[0])[:, None, None, None] * st[0] + np.arange(n[1])[:, None, None] * st[1] + np.arange(n[2])[:, None] * st[2] + np.arange(n[3])).reshape(-1)
+        found = bool(lib.overlaps(cache(pages=n[0], page=n[1], heads=n[2], dim=n[3], ps=st[0], ts=st[1], hs=st[2])))
+        seen.add(found)
+        if len(set(at.tolist())) < len(at):
+            assert found, (n, st)                         # never missed
+        if found:                                         # and nothing refused that is an ordinary tensor's layout in some order
+            order = sorted((s, m) for s, m in zip(st, n) if m > 1)
+            reach = n[3]
+            ordinary = True
+            for s, m in order:
+                ordinary = ordinary and s >= reach
+                reach = s * m if s >= reach else reach
+            assert not ordinary, (n, st)
+    assert seen == {False, True}
+
+
+def test_spans_and_pages(lib):
+    out = (ctypes.c_uint32 * 2)()
+    for len_, first, max_len, stride, page, ok, want in ((5, 0, 10, 2, 8, 1, (0, 5)), (5, 5, 10, 2, 8, 1, (5, 5)), (5, 9, 10, 2, 8, 1, (5, 5)), (16, 3, 16, 2, 8, 1, (3, 16)),
+                                                         (17, 0, 20, 2, 8, 0, (0, 0)), (11, 0, 10, 2, 8, 0, (0, 0)), (-1, 0, 10, 2, 8, 0, (0, 0)), (5, -1, 10, 2, 8, 0, (0, 0)),
+                                                         (-(1 << 31), 0, 10, 2, 8, 0, (0, 0)), (0, 0, 0, 0, 8, 1, (0, 0)), (1, 0, 1, 0, 8, 0, (0, 0)),
+                                                         ((1 << 31) - 1, 0, (1 << 31) - 1, 1 << 20, 1 << 20, 1, (0, (1 << 31) - 1))):
+        assert lib.span(len_, first, max_len, stride, page, out) == ok and tuple(out) == want
+    c = cache()
+    assert lib.offset_of(c, 9, 15) == 9 * 4096 + 15 * 256
+    assert lib.offset_of(c, 10, 0) == lib.offset_of(c, -1, 0) == lib.offset_of(c, (1 << 31) - 1, 3) == lib.offset_of(c, -(1 << 31), 3) == -1
+    big = cache(pages=1 << 20, page=1 << 10, ps=1 << 30, ts=1 << 20)
+    assert lib.offset_of(big, (1 << 20) - 1, 1023) == ((1 << 20) - 1 << 30) + (1023 << 20)             # offsets pass 32 bits
+    for slot, pos, rot, want in ((0, 0, 64, 0), (159, 99, 64, 0), (160, 0, 64, 2), (1 << 62, 0, 64, 2), (-1, 500, 64, 1), (-(1 << 63), 0, 64, 1), (3, 100, 64, 2), (3, -1, 64, 2), (3, -1, 0, 0)):
+        assert lib.kind(c, slot, pos, rot, 100) == want
+
+
+def test_workspace_sizes(lib):
+    assert lib.workspace(0, 8, 8, 64, 100) == 0 and lib.workspace(65536, 8, 8, 64, 100) == 0 and lib.workspace(60000, 60000, 1, 64, 100000) == 0
+    assert lib.workspace(1, 8, 2, 64, 1000) >= 4 * 8 * 1000
+
+
+# ------------------------------------------------------------------ the helpers' own checks
+
+
+@pytest.fixture
+def helpers(monkeypatch):
+    """the helpers on host tensors, in front of a library that takes every call"""
+    calls = []
+
+    class Library:
+        def __getattr__(self, name):
+            def call(*args):
+                calls.append((name, args))
+                return 64 if name.endswith("_workspace") else 0
+            return call
+    monkeypatch.setattr(ops, "init", lambda *a: Library())
+    monkeypatch.setattr(ops, "_place", lambda: torch.device("cpu"))
+    monkeypatch.setattr(ops, "_s", lambda: None)
+    monkeypatch.setattr(ops, "_i32", lambda *s: torch.empty(s, dtype=torch.int32))
+    return calls
+
+
+def i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def append_args():
+    return dict(q=i32(3, 8, 64), k=i32(3, 4, 64), v=i32(3, 4, 64), positions=i32(3), slots=torch.zeros(3, dtype=torch.int64), cos=i32(100, 32), sin=i32(100, 32),
+                k_cache=i32(10, 16, 4, 64), v_cache=i32(10, 16, 4, 64), q_out=i32(3, 8, 64), q_rem=i32(3, 8, 64), k_rem=i32(3, 4, 64))
+
+
+@pytest.mark.parametrize("bad", [dict(q=i32(3, 512)), dict(q=i32(2, 8, 64)), dict(q=i32(3, 8, 64).float()), dict(q=i32(3, 64, 8).transpose(1, 2)), dict(k=i32(3, 8, 64)),
+                                 dict(v=i32(3, 4, 63)), dict(positions=i32(4)), dict(positions=torch.zeros(3, dtype=torch.int64)), dict(slots=i32(3)),
+                                 dict(slots=torch.zeros(6, dtype=torch.int64)[::2]), dict(cos=i32(99, 32)), dict(sin=i32(100, 31)), dict(cos=i32(32, 100).t(), sin=i32(32, 100).t()),
+                                 dict(k_cache=i32(10, 16, 256)), dict(v_cache=i32(11, 16, 4, 64)), dict(k_cache=i32(10, 16, 64, 4).transpose(2, 3), v_cache=i32(10, 16, 64, 4).transpose(2, 3)),
+                                 dict(k_cache=i32(10, 16, 4, 64).long(), v_cache=i32(10, 16, 4, 64).long()), dict(q_out=i32(3, 8, 63)), dict(q_rem=i32(3, 4, 64)), dict(k_rem=i32(3, 8, 64)),
+                                 dict(q=None), dict(q=i32(3, 8, 64).to("meta"))])
+def test_append_helper_refuses(helpers, bad):
+    ops.wit_rope_append(**append_args())
+    with pytest.raises(ValueError):
+        ops.wit_rope_append(**{**append_args(), **bad})
+    assert len(helpers) == 1
+
+
+def attend_args():
+    return dict(q=i32(2, 8, 64), k_cache=i32(10, 16, 4, 64), v_cache=i32(10, 16, 4, 64), block_table=i32(2, 5), lens=i32(2), max_len=70, exp_table=i32(1 << 20))
+
+
+@pytest.mark.parametrize("bad", [dict(q=i32(2, 512)), dict(q=i32(2, 8, 60)), dict(block_table=i32(3, 5)), dict(block_table=i32(2, 10)[:, :5]), dict(block_table=i32(10)), dict(lens=i32(3)),
+                                 dict(first=i32(3)), dict(first=torch.zeros(2)), dict(exp_table=i32(1000)), dict(index_bits=19), dict(max_len=-1), dict(out={}), dict(out={"max": i32(2, 8)}),
+                                 dict(out={"qkv": i32(2, 8, 64), "score": i32(2, 8, 70)}), dict(out={"qkv": i32(2, 8, 64), "scores": i32(2, 8, 71)}), dict(out={"qkv": i32(2, 8, 64, 1)}),
+                                 dict(workspace=i32(1000)), dict(v_cache=i32(10, 16, 64, 4).transpose(2, 3))])
+def test_attention_helper_refuses(helpers, bad):
+    got = ops.wit_paged_attention(**attend_args())
+    assert got["scores"].shape == (2, 8, 70) and got["qkv"].shape == (2, 8, 64)
+    n = len(helpers)
+    with pytest.raises(ValueError):
+        ops.wit_paged_attention(**{**attend_args(), **bad})
+    assert not [c for c in helpers[n:] if not c[0].endswith("_workspace")]
+
+
+@pytest.mark.parametrize("bad", [dict(x=i32(64)), dict(x=i32(2, 64).long()), dict(x=i32(64, 2).t()), dict(w=i32(8, 32)), dict(w=torch.zeros((8, 33), dtype=torch.uint8)), dict(scales=i32(8, 3)),
+                                 dict(scales=i32(2, 8).t()), dict(zeros=i32(8, 2)), dict(group=0), dict(q=i32(2, 9)), dict(r=i32(3, 8)), dict(x=i32(2, 0), w=torch.zeros((8, 0), dtype=torch.uint8))])
+def test_q4_helper_refuses(helpers, bad):
+    good = dict(x=i32(2, 64), w=torch.zeros((8, 32), dtype=torch.uint8), scales=i32(8, 2), group=32)
+    assert ops.wit_matvec_q4(**good)[0].shape == (2, 8)
+    with pytest.raises(ValueError):
+        ops.wit_matvec_q4(**{**good, **bad})
+    assert len(helpers) == 1
+
+
+def test_helpers_hand_over_strides(helpers):
+    fused = i32(3, 16 * 64 + 4)
+    q, k, v = (fused[:, a * 64:b * 64].view(3, -1, 64) for a, b in ((0, 8), (8, 12), (12, 16)))
+    kc = i32(4, 10, 16, 70).permute(1, 2, 0, 3)[..., :64]
+    ops.wit_rope_append(**{**append_args(), "q": q, "k": k, "v": v, "k_cache": kc, "v_cache": kc})
+    args, c = helpers[0][1][:2]
+    assert ops._APPEND.unpack(args)[3:6] == (fused.stride(0),) * 3 and ops._CACHE.unpack(c)[2:] == (10, 16, 4, 64, 16 * 70, 70, 160 * 70)
+    x = i32(1, 64).expand(5, 64)
+    ops.wit_matvec_q4(x, torch.zeros((8, 40), dtype=torch.uint8)[:, 3:35], i32(8, 2), 32)
+    assert helpers[1][1][3] == 0 and helpers[1][1][5] == 40
