@@ -63,7 +63,7 @@ inline const char* refuse_cache(const grape_wit_cache* c) {
     GRAPE_REFUSE(!c->d_k || !c->d_v, "the cache's keys or values are null");
     GRAPE_REFUSE(!c->pages || !c->page_size || !c->heads || !c->dim, "empty cache");
     GRAPE_REFUSE((uint64_t)c->pages * c->page_size >= (uint64_t)1 << 31, "the cache has 2^31 slots or more");
-    GRAPE_REFUSE(c->heads > 65535 || c->dim > 16384, "at most 65535 heads of 16384 elements");
+    GRAPE_REFUSE(c->heads > 65535 || c->dim > 8192, "at most 65535 heads of 8192 elements");
     const int64_t most = (int64_t)1 << 40;
     GRAPE_REFUSE(c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0, "negative stride");
     GRAPE_REFUSE(c->page_stride >= most || c->token_stride >= most || c->head_stride >= most, "stride of 2^40 or more");
@@ -90,11 +90,82 @@ inline const char* refuse_append(const grape_wit_rope_append_args* a, const grap
     return nullptr;
 }
 
+// How an attention call is cut up.  A workgroup of the scores and of the values takes `rows` query heads of one cache head and a
+// chunk of the positions, one of the exponentials a query head and a chunk; with few sequences the chunks are short enough to
+// fill the chip (about 8 workgroups a CU), with many they are long.
+struct AttentionPlan {
+    uint32_t dim64;                    // blocks of 64 elements of a head
+    uint32_t rows, tiles;              // query heads of a workgroup, workgroups of a cache head
+    uint32_t score_chunk, score_chunks;
+    uint32_t exp_chunk, exp_chunks;
+    uint32_t blocks, groups;           // blocks of 64 elements of a values workgroup, workgroups of a head's elements
+    uint32_t value_chunk, value_chunks;
+    size_t at_scores, at_exp, at_max, at_sum, at_part, bytes;      // offsets in the workspace
+};
+constexpr uint32_t kTokenLds = 60 * 1024;      // of a workgroup
+constexpr uint32_t kWorkgroups = 2048;
+
+inline uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
+
+inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len, AttentionPlan& p) {
+    if (!seqs || !heads || !cache_heads || !dim || heads > 65535 || seqs > 65535 || heads % cache_heads || dim > 8192 || max_len >= (uint32_t)1 << 31) return false;
+    const uint64_t rows_all = (uint64_t)seqs * heads;
+    if ((unsigned __int128)rows_all * max_len >= (uint64_t)1 << 38) return false;
+    const uint32_t each = heads / cache_heads;
+    p.dim64 = ceil_div(dim, 64);
+    p.rows = kTokenLds / (5 * 64 * p.dim64);               // five planes of the queries' digits
+    p.rows = p.rows < 16 ? p.rows : 16;
+    p.rows = p.rows < each ? p.rows : each;
+    p.tiles = ceil_div(each, p.rows);
+    auto chunk = [&](uint64_t beside, uint32_t step, uint32_t most) {
+        const uint64_t want = beside >= kWorkgroups ? 1 : kWorkgroups / beside;
+        uint64_t c = (max_len + want - 1) / want;
+        c = (c + step - 1) / step * step;
+        c = c < step ? step : c;
+        return (uint32_t)(c < most ? c : most);
+    };
+    const uint64_t beside = (uint64_t)seqs * cache_heads * p.tiles;
+    p.score_chunk = chunk(beside, 64, (uint32_t)1 << 20);
+    p.score_chunks = ceil_div(max_len, p.score_chunk);
+    p.exp_chunk = chunk(rows_all, 1024, (uint32_t)1 << 20);
+    p.exp_chunks = ceil_div(max_len, p.exp_chunk);
+    p.blocks = p.dim64 % 4 == 0 ? 4 : p.dim64 % 2 == 0 ? 2 : 1;
+    p.groups = p.dim64 / p.blocks;
+    if ((uint64_t)cache_heads * p.tiles * p.groups > 65535) return false;          // a launch's second axis
+    const uint32_t step = 64 * (4 / p.blocks);
+    uint32_t most = kTokenLds / (4 * p.rows + 8) / step * step;
+    if (most > 1024) most = 1024;
+    p.value_chunk = chunk(beside * p.groups, step, most);
+    p.value_chunks = ceil_div(max_len, p.value_chunk);
+    const size_t row = (size_t)rows_all * max_len * 4;
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    p.at_scores = 0;
+    p.at_exp = up(row);
+    p.at_max = p.at_exp + up(row);
+    p.at_sum = p.at_max + up((size_t)rows_all * p.score_chunks * 4);
+    p.at_part = p.at_sum + up((size_t)rows_all * p.exp_chunks * 8);
+    p.bytes = p.at_part + (p.value_chunks > 1 ? (size_t)rows_all * p.value_chunks * dim * 8 : 0);
+    return true;
+}
+
 // Bytes of workspace, 0 where a call of these sizes is refused.
 inline size_t attention_workspace(uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len) {
-    if (!seqs || !heads || !cache_heads || !dim || heads > 65535 || seqs > 65535 || max_len >= (uint32_t)1 << 31) return 0;
-    if ((uint64_t)seqs * heads >= (uint64_t)1 << 38 || (unsigned __int128)((uint64_t)seqs * heads) * max_len >= (uint64_t)1 << 38) return 0;
-    return (size_t)12 * seqs * heads * max_len;
+    AttentionPlan p;
+    return attention_plan(seqs, heads, cache_heads, dim, max_len, p) ? p.bytes : 0;
+}
+
+// n / d for n below 2^31
+struct FastDiv {
+    uint32_t d, mul, shift;
+    GRAPE_HD uint32_t operator()(uint32_t n) const {
+        return d == 1 ? n : (uint32_t)(((uint64_t)n * mul) >> 32) >> shift;
+    }
+};
+inline FastDiv fast_div(uint32_t d) {
+    // the smallest l with 2^l >= d; mul = floor(2^(31 + l) / d) + 1 is off by at most d / 2^(31 + l) <= 2^-31 a unit of n
+    uint32_t l = 0;
+    while (((uint64_t)1 << l) < d) l++;
+    return FastDiv{d, d == 1 ? 0 : (uint32_t)((((uint64_t)1 << (31 + l)) / d) + 1), l - 1};
 }
 
 inline const char* refuse_attention(const grape_wit_attention_args* a, const grape_wit_cache* c) {
@@ -111,8 +182,9 @@ inline const char* refuse_attention(const grape_wit_attention_args* a, const gra
     GRAPE_REFUSE(a->max_len >= (uint32_t)1 << 31, "max_len must be below 2^31");
     GRAPE_REFUSE(!a->d_q || !a->d_lens || !a->d_exp_table || !a->d_out, "d_q, d_lens, d_exp_table or d_out is null");
     GRAPE_REFUSE(a->max_len && !a->d_block_table, "d_block_table is null");
-    GRAPE_REFUSE((unsigned __int128)((uint64_t)a->seqs * a->heads) * a->max_len >= (uint64_t)1 << 38, "tensor too large");
-    const size_t need = attention_workspace(a->seqs, a->heads, c->heads, c->dim, a->max_len);
+    AttentionPlan plan;
+    GRAPE_REFUSE(!attention_plan(a->seqs, a->heads, c->heads, c->dim, a->max_len, plan), "tensor too large");
+    const size_t need = plan.bytes;
     GRAPE_REFUSE(a->workspace_bytes < need || (need && !a->d_workspace), "the workspace is too small");
     GRAPE_REFUSE((uintptr_t)a->d_workspace & 15, "the workspace must be 16-byte aligned");
     return nullptr;

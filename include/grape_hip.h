@@ -744,7 +744,7 @@ int grape_wit_rope_append(const grape_wit_rope_append_args *args, const grape_wi
  *
  * max_len bounds every length.  A len above it or above table_stride*page_size, a negative len or first sets GRAPE_WIT_INDEX
  * and makes the sequence's rows empty; a page outside the cache sets it too, and its keys and values count as zero.
- * 1 <= scales <= 2^31 (prob_scale <= 2^30), dim <= 16384.
+ * 1 <= scales <= 2^31 (prob_scale <= 2^30), dim <= 8192.
  *
  * d_workspace (16-byte aligned) holds what the launches hand on to each other, grape_wit_paged_attention_workspace(...) bytes;
  * it needs no initial contents, and calls that may run at the same time, replays of captured ones among them, need one each. */

@@ -18,6 +18,16 @@ int span(int32_t len, int32_t first, uint32_t max_len, uint32_t stride, uint32_t
 int64_t offset_of(const grape_wit_cache* c, int32_t page, uint32_t in_page) { return token::token_offset(*c, page, in_page); }
 int kind(const grape_wit_cache* c, int64_t slot, int32_t pos, uint32_t rot, uint32_t rows) { return token::append_kind(*c, slot, pos, rot, rows); }
 size_t workspace(uint32_t s, uint32_t h, uint32_t hk, uint32_t d, uint32_t n) { return token::attention_workspace(s, h, hk, d, n); }
+uint32_t divided(uint32_t n, uint32_t d) { return token::fast_div(d)(n); }
+// the parts of a plan that bound what the kernels touch
+int plan_of(uint32_t s, uint32_t h, uint32_t hk, uint32_t d, uint32_t n, uint64_t* o) {
+    token::AttentionPlan p;
+    if (!token::attention_plan(s, h, hk, d, n, p)) return 0;
+    const uint64_t v[] = {p.dim64, p.rows, p.tiles, p.score_chunk, p.score_chunks, p.exp_chunk, p.exp_chunks, p.blocks, p.groups, p.value_chunk, p.value_chunks,
+                          p.at_scores, p.at_exp, p.at_max, p.at_sum, p.at_part, p.bytes};
+    std::memcpy(o, v, sizeof v);
+    return 1;
+}
 // every field of the structs, in the order in which the helpers pack them
 void append_fields(const grape_wit_rope_append_args* a, int64_t* o) {
     const int64_t v[] = {(int64_t)a->d_q, (int64_t)a->d_k, (int64_t)a->d_v, a->q_stride, a->k_stride, a->v_stride, (int64_t)a->d_positions, (int64_t)a->d_slots,

@@ -66,7 +66,7 @@ def test_helpers_pack_the_structs_of_the_header(lib):
 
 
 @pytest.mark.parametrize("bad", [dict(k=0), dict(v=0), dict(pages=0), dict(page=0), dict(heads=0), dict(dim=0), dict(pages=1 << 27), dict(heads=65536),
-                                 dict(dim=16385), dict(ps=-1), dict(ts=-1), dict(hs=-1), dict(ps=1 << 40), dict(hs=1 << 40)])
+                                 dict(dim=8193), dict(ps=-1), dict(ts=-1), dict(hs=-1), dict(ps=1 << 40), dict(hs=1 << 40)])
 def test_bad_caches_are_refused(lib, bad):
     assert lib.refuse_append(append(), cache()) is None and lib.refuse_attention(attend(), cache()) is None
     assert lib.refuse_append(append(), cache(**bad)) and lib.refuse_attention(attend(), cache(**bad))
@@ -139,6 +139,45 @@ def test_spans_and_pages(lib):
     assert lib.offset_of(big, (1 << 20) - 1, 1023) == ((1 << 20) - 1 << 30) + (1023 << 20)             # offsets pass 32 bits
     for slot, pos, rot, want in ((0, 0, 64, 0), (159, 99, 64, 0), (160, 0, 64, 2), (1 << 62, 0, 64, 2), (-1, 500, 64, 1), (-(1 << 63), 0, 64, 1), (3, 100, 64, 2), (3, -1, 64, 2), (3, -1, 0, 0)):
         assert lib.kind(c, slot, pos, rot, 100) == want
+
+
+def test_division_by_a_page_size(lib):
+    rng = np.random.default_rng(2)
+    lib.divided.restype = ctypes.c_uint32
+    for d in [1, 2, 3, 5, 7, 16, 17, 100, 255, 256, 257, 1 << 16, (1 << 16) + 1, 1 << 30, (1 << 31) - 1] + [int(x) for x in rng.integers(1, 1 << 31, 200)]:
+        for n in [0, 1, d - 1, d, d + 1, 2 * d - 1, 2 * d, (1 << 31) - 1, (1 << 31) // d * d, (1 << 31) // d * d - 1] + [int(x) for x in rng.integers(0, 1 << 31, 50)]:
+            if n < 1 << 31:
+                assert lib.divided(n, d) == n // d, (n, d)
+
+
+def test_plans_cover_every_position_within_their_limits(lib):
+    rng = np.random.default_rng(3)
+    names = "dim64 rows tiles score_chunk score_chunks exp_chunk exp_chunks blocks groups value_chunk value_chunks at_scores at_exp at_max at_sum at_part bytes".split()
+    out = (ctypes.c_uint64 * len(names))()
+    sizes = [(1, 32, 8, 128, 37), (1, 1, 1, 8192, 1 << 20), (64, 32, 8, 128, 2048), (1, 64, 1, 64, 131072), (65535, 1, 1, 1, 1), (1, 1, 1, 1, 0), (3, 48, 3, 192, 5000)]
+    for _ in range(2000):
+        hk = int(rng.integers(1, 20))
+        sizes.append((int(2 ** rng.uniform(0, 12)), hk * int(2 ** rng.uniform(0, 6)), hk, int(2 ** rng.uniform(0, 13)), int(2 ** rng.uniform(0, 22))))
+    taken = 0
+    for s, h, hk, d, n in sizes:
+        if not lib.plan_of(s, h, hk, d, n, out):
+            continue
+        taken += 1
+        p = dict(zip(names, out))
+        assert p["dim64"] * 64 >= d > (p["dim64"] - 1) * 64 and 1 <= p["rows"] <= 16 and p["rows"] * p["tiles"] >= h // hk > p["rows"] * (p["tiles"] - 1)
+        assert p["blocks"] * p["groups"] == p["dim64"] and p["blocks"] in (1, 2, 4)
+        for kind, step in (("score", 64), ("exp", 1024), ("value", 64 * 4 // p["blocks"])):
+            assert p[kind + "_chunk"] % step == 0 and p[kind + "_chunk"] * p[kind + "_chunks"] >= n and (p[kind + "_chunks"] == 0 or p[kind + "_chunk"] * (p[kind + "_chunks"] - 1) < n)
+        assert p["value_chunk"] <= 1024                                         # what the 32-bit sums of the planes' products hold
+        assert p["dim64"] * 64 * 5 * p["rows"] <= 61440                         # LDS
+        assert p["value_chunk"] * (p["rows"] * 4 + 8) <= 61440 and p["rows"] * p["blocks"] * 64 * 8 <= 61440
+        assert hk * p["tiles"] * p["groups"] <= 65535
+        rows = s * h
+        need = [rows * n * 4, rows * n * 4, rows * p["score_chunks"] * 4, rows * p["exp_chunks"] * 8, rows * p["value_chunks"] * d * 8 if p["value_chunks"] > 1 else 0]
+        at = [p[x] for x in ("at_scores", "at_exp", "at_max", "at_sum", "at_part", "bytes")]
+        assert at[0] == 0 and all(x % 16 == 0 for x in at[:5]) and all(b - a >= k for a, b, k in zip(at, at[1:], need))
+        assert lib.workspace(s, h, hk, d, n) == p["bytes"]
+    assert taken > 1000
 
 
 def test_workspace_sizes(lib):
