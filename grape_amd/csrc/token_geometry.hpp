@@ -3,6 +3,7 @@
 #pragma once
 #include <stddef.h>
 #include <stdint.h>
+#include <algorithm>
 #include "../../include/grape_hip.h"
 
 #ifndef GRAPE_HD
@@ -113,30 +114,36 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
     if ((unsigned __int128)rows_all * max_len >= (uint64_t)1 << 38) return false;
     const uint32_t each = heads / cache_heads;
     p.dim64 = ceil_div(dim, 64);
-    p.rows = kTokenLds / (5 * 64 * p.dim64);               // five planes of the queries' digits
+    p.rows = (kTokenLds - 4096) / (5 * 64 * p.dim64);      // five planes of the queries' digits
     p.rows = p.rows < 16 ? p.rows : 16;
     p.rows = p.rows < each ? p.rows : each;
     p.tiles = ceil_div(each, p.rows);
-    auto chunk = [&](uint64_t beside, uint32_t step, uint32_t most) {
-        const uint64_t want = beside >= kWorkgroups ? 1 : kWorkgroups / beside;
+    auto chunk = [&](uint64_t beside, uint32_t step, uint32_t most, uint32_t workgroups) {
+        const uint64_t want = beside >= workgroups ? 1 : workgroups / beside;
         uint64_t c = (max_len + want - 1) / want;
         c = (c + step - 1) / step * step;
         c = c < step ? step : c;
         return (uint32_t)(c < most ? c : most);
     };
     const uint64_t beside = (uint64_t)seqs * cache_heads * p.tiles;
-    p.score_chunk = chunk(beside, 64, (uint32_t)1 << 20);
+    // a score waits in LDS, 8 bytes, beside the positions' offsets and the queries' digits
+    const uint32_t left = kTokenLds - 5 * 64 * p.dim64 * p.rows;
+    uint32_t score_most = left / (8 * p.rows + 8) / 64 * 64;
+    if (score_most > 4096 / p.rows) score_most = 4096 / p.rows / 64 * 64;
+    if (score_most < 64) return false;
+    p.score_chunk = chunk(beside, 64, score_most, kWorkgroups);
     p.score_chunks = ceil_div(max_len, p.score_chunk);
-    p.exp_chunk = chunk(rows_all, 1024, (uint32_t)1 << 20);
+    p.exp_chunk = chunk(rows_all, 1024, (uint32_t)1 << 20, kWorkgroups);
     p.exp_chunks = ceil_div(max_len, p.exp_chunk);
     p.blocks = p.dim64 % 4 == 0 ? 4 : p.dim64 % 2 == 0 ? 2 : 1;
     p.groups = p.dim64 / p.blocks;
-    if ((uint64_t)cache_heads * p.tiles * p.groups > 65535) return false;          // a launch's second axis
     const uint32_t step = 64 * (4 / p.blocks);
     uint32_t most = kTokenLds / (4 * p.rows + 8) / step * step;
     if (most > 1024) most = 1024;
-    p.value_chunk = chunk(beside * p.groups, step, most);
+    p.value_chunk = chunk(beside * p.groups, step, most, kWorkgroups / 2);
     p.value_chunks = ceil_div(max_len, p.value_chunk);
+    // a launch's first axis, in threads
+    if ((uint64_t)cache_heads * p.tiles * std::max<uint64_t>(p.score_chunks, (uint64_t)p.value_chunks * p.groups) >= (uint64_t)1 << 23) return false;
     const size_t row = (size_t)rows_all * max_len * 4;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     p.at_scores = 0;

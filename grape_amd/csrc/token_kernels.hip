@@ -169,22 +169,31 @@ __device__ __forceinline__ v4i_t load4(const int32_t* x, uint32_t at, uint32_t n
 // 4 (l / 16) .. + 4 of position l % 16 that make up its operand of step s (any order of a step's elements will do, as long as
 // the queries' digits in LDS have the same), whole lines among the lanes.  Bound by reading the keys.
 template <bool VEC>
-__global__ void __launch_bounds__(256) wit_attend_scores_kernel(AttendArgs p) {
+__global__ void __launch_bounds__(256, 4) wit_attend_scores_kernel(AttendArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
-    __shared__ int32_t wave_max[4][16];
     __shared__ unsigned long long q_sum[16];
     __shared__ uint32_t over_any;
-    const uint32_t b = blockIdx.z, kv = blockIdx.y / p.plan.tiles, tile = blockIdx.y - kv * p.plan.tiles;
+    const uint32_t per_chunk = p.c.heads * p.plan.tiles, chunk = blockIdx.x / per_chunk, head_tile = blockIdx.x - chunk * per_chunk;
+    const uint32_t b = blockIdx.y, kv = head_tile / p.plan.tiles, tile = head_tile - kv * p.plan.tiles;
     const uint32_t each = p.a.heads / p.c.heads, h0 = kv * each + tile * p.plan.rows, R = min(p.plan.rows, each - tile * p.plan.rows);
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, kg = lane >> 4, dim = p.c.dim, steps = p.plan.dim64;
     uint32_t lo, hi, bad = 0;
     const bool fits = span_of(p, b, lo, hi);
-    if (!fits && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(p.status, (uint32_t)kWitIndex);
-    const uint64_t start = (uint64_t)lo + (uint64_t)blockIdx.x * p.plan.score_chunk;
+    if (!fits && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.status, (uint32_t)kWitIndex);
+    const uint64_t start = (uint64_t)lo + (uint64_t)chunk * p.plan.score_chunk;
     if (start >= hi) return;
     const uint32_t t0 = (uint32_t)start, t1 = min(hi, t0 + p.plan.score_chunk);
     if (threadIdx.x < 16) q_sum[threadIdx.x] = 0;
     if (threadIdx.x == 0) over_any = 0;
+    // behind the digits: the positions' offsets and the scores' 64-bit sums, so that nothing but the keys is read or written on
+    // the way (waiting for any other load or store would wait for all keys requested before it)
+    int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)5 * 16 * steps * p.plan.rows);
+    uint64_t* sums = reinterpret_cast<uint64_t*>(off + p.plan.score_chunk);            // [row][position]
+    const uint32_t n = t1 - t0;
+    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+        off[i] = token_at(p, b, t0 + i);
+        if (off[i] < 0) bad |= (uint32_t)kWitIndex;
+    }
     __syncthreads();
     // the queries' digits: [step][plane 0..4][lane group][row], 16 bytes each; plane 4 holds what a top digit of 128 carries
     for (uint32_t i = threadIdx.x; i < R * steps * 16; i += 256) {
@@ -205,78 +214,88 @@ __global__ void __launch_bounds__(256) wit_attend_scores_kernel(AttendArgs p) {
         for (uint32_t k = 0; k < 4; k++) o[k * 16 * R] = pl[k];
         o[4 * 16 * R] = carry;
         if (carry) over_any = 1;
-        atomicAdd(&q_sum[r], (unsigned long long)sum);
+        // sixteen neighbouring lanes are of one row
+#pragma unroll
+        for (int d = 8; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+        if ((i & 15u) == 0) atomicAdd(&q_sum[r], (unsigned long long)sum);
     }
     __syncthreads();
     const bool over = over_any != 0;
-    const uint32_t row = col < R ? col : R - 1;
-    int32_t mx[4] = {INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN};
-    for (uint32_t at = t0 + 16 * wave; at < t1; at += 64) {
-        const uint32_t t = at + col;
-        int64_t off = t < t1 ? token_at(p, b, t) : 0;
-        const bool outside = off < 0;
-        if (outside) off = 0, bad |= (uint32_t)kWitIndex;
-        const int32_t* k = p.c.d_k + off + (int64_t)kv * p.c.head_stride;
+    // row m of the product is query head 4 (m % 4) + m / 4: register i of lane l then holds head 4 i + l / 16 at position l % 16,
+    // and four heads need one register of every lane
+    const uint32_t head = 4 * (col & 3u) + (col >> 2), row = head < R ? head : R - 1;
+    const int32_t* keys = p.c.d_k + (int64_t)kv * p.c.head_stride;
+    for (uint32_t at = 16 * wave; at < n; at += 64) {
+        const int32_t* k = keys + max(off[min(at + col, n - 1)], (int64_t)0);
         v4i_t acc[8];
 #pragma unroll
         for (int g = 0; g < 8; g++) acc[g] = v4i_t{0, 0, 0, 0};
-#pragma unroll 2
-        for (uint32_t s = 0; s < steps; s++) {
-            v4i_t x[4], kb[4];
+        // two steps at a time: their keys are requested together, and other waves multiply meanwhile
+        for (uint32_t s = 0; s < steps; s += 2) {
+            v4i_t x[8];
 #pragma unroll
             for (uint32_t c = 0; c < 4; c++) x[c] = load4<VEC>(k, 64 * s + 16 * c + 4 * kg, dim);
+            if (s + 1 < steps) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t pl[4];
-                transpose4((uint32_t)x[c][0] ^ kByteTops, (uint32_t)x[c][1] ^ kByteTops, (uint32_t)x[c][2] ^ kByteTops, (uint32_t)x[c][3] ^ kByteTops, pl);
-#pragma unroll
-                for (int k2 = 0; k2 < 4; k2++) kb[k2][c] = (int)pl[k2];
+                for (uint32_t c = 4; c < 8; c++) x[c] = load4<VEC>(k, 64 * s + 16 * c + 4 * kg, dim);
             }
-            const v4i_t* qa = reinterpret_cast<const v4i_t*>(lds) + (s * 5 * 4 + kg) * R + row;
 #pragma unroll
-            for (int a = 0; a < 4; a++) {
-                const v4i_t f = qa[a * 4 * R];
+            for (uint32_t u = 0; u < 2; u++) {
+                if (s + u >= steps) break;
+                v4i_t kb[4];
 #pragma unroll
-                for (int k2 = 0; k2 < 4; k2++) acc[a + k2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, kb[k2], acc[a + k2], 0, 0, 0);
-            }
-            if (over) {
-                const v4i_t f = qa[4 * 4 * R];
+                for (int c = 0; c < 4; c++) {
+                    const v4i_t w = x[4 * u + c];
+                    uint32_t pl[4];
+                    transpose4((uint32_t)w[0] ^ kByteTops, (uint32_t)w[1] ^ kByteTops, (uint32_t)w[2] ^ kByteTops, (uint32_t)w[3] ^ kByteTops, pl);
 #pragma unroll
-                for (int k2 = 0; k2 < 4; k2++) acc[4 + k2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, kb[k2], acc[4 + k2], 0, 0, 0);
+                    for (int k2 = 0; k2 < 4; k2++) kb[k2][c] = (int)pl[k2];
+                }
+                const v4i_t* qa = reinterpret_cast<const v4i_t*>(lds) + ((s + u) * 5 * 4 + kg) * R + row;
+#pragma unroll
+                for (int a = 0; a < 4; a++) {
+                    const v4i_t f = qa[a * 4 * R];
+#pragma unroll
+                    for (int k2 = 0; k2 < 4; k2++) acc[a + k2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, kb[k2], acc[a + k2], 0, 0, 0);
+                }
+                if (over) {
+                    const v4i_t f = qa[4 * 4 * R];
+#pragma unroll
+                    for (int k2 = 0; k2 < 4; k2++) acc[4 + k2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, kb[k2], acc[4 + k2], 0, 0, 0);
+                }
             }
         }
-        // register i of a lane holds row 4 (l / 16) + i and position l % 16
+        if (at + col < n) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
-            const uint32_t r = 4 * kg + i;
-            if (i < R && r < R && t < t1) {
-                uint64_t y = 0;
+            for (uint32_t i = 0; i < 4; i++) {
+                const uint32_t r = 4 * i + kg;
+                if (4 * i < R && r < R) {
+                    uint64_t y = 0;
 #pragma unroll
-                for (int g = 7; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[g][i];
-                y += (uint64_t)kCacheOffset * q_sum[r];
-                if (outside) y = 0;
-                int32_t q, rem;
-                p.qk.apply((int64_t)y, q, rem, bad);
-                const size_t o = ((size_t)b * p.a.heads + h0 + r) * p.a.max_len + t;
-                p.a.d_scores[o] = q;
-                if (p.a.d_scores_rem) p.a.d_scores_rem[o] = rem;
-                mx[i] = max(mx[i], q);
+                    for (int g = 7; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[g][i];
+                    sums[r * p.plan.score_chunk + at + col] = y;
+                }
             }
         }
     }
+    __syncthreads();
+    for (uint32_t r = wave; r < R; r += 4) {
+        const size_t row = (size_t)b * p.a.heads + h0 + r, o = row * p.a.max_len + t0;
+        const uint64_t more = (uint64_t)kCacheOffset * q_sum[r];
+        int32_t mx = INT32_MIN;
+        for (uint32_t i = lane; i < n; i += 64) {
+            const int64_t y = off[i] < 0 ? 0 : (int64_t)(sums[r * p.plan.score_chunk + i] + more);          // a page outside: zero
+            int32_t q, rem;
+            p.qk.apply(y, q, rem, bad);
+            p.a.d_scores[o + i] = q;
+            if (p.a.d_scores_rem) p.a.d_scores_rem[o + i] = rem;
+            mx = max(mx, q);
+        }
 #pragma unroll
-    for (uint32_t i = 0; i < 4; i++) {
-#pragma unroll
-        for (int o = 8; o >= 1; o >>= 1) mx[i] = max(mx[i], __shfl_xor(mx[i], o, 64));
-        if (col == 0) wave_max[wave][4 * kg + i] = mx[i];
+        for (int d = 32; d >= 1; d >>= 1) mx = max(mx, __shfl_xor(mx, d, 64));
+        if (lane == 0) p.chunk_max[row * p.plan.score_chunks + chunk] = mx;
     }
     if (bad) atomicOr(p.status, bad);
-    __syncthreads();
-    if (threadIdx.x < R) {
-        const uint32_t r = threadIdx.x;
-        const int32_t m = max(max(wave_max[0][r], wave_max[1][r]), max(wave_max[2][r], wave_max[3][r]));
-        p.chunk_max[((size_t)b * p.a.heads + h0 + r) * p.plan.score_chunks + blockIdx.x] = m;
-    }
 }
 
 template <class T, class F>
@@ -293,7 +312,8 @@ __device__ __forceinline__ T block_all(T v, F f) {
     return v;
 }
 
-// Exponentials of a chunk of one row, and their sum.
+// Exponentials of a chunk of one row, and their sum.  Bound by the gathers' latency: four are under way a thread.
+constexpr uint32_t kExpAhead = 4;
 __global__ void __launch_bounds__(kBlock) wit_attend_exp_kernel(AttendArgs p) {
     const uint32_t h = blockIdx.y, b = blockIdx.z;
     const size_t row = (size_t)b * p.a.heads + h, o = row * p.a.max_len;
@@ -307,15 +327,26 @@ __global__ void __launch_bounds__(kBlock) wit_attend_exp_kernel(AttendArgs p) {
     mx = block_all(mx, [](int32_t x, int32_t y) { return max(x, y); });
     if (blockIdx.x == 0 && threadIdx.x == 0 && p.a.d_max) p.a.d_max[row] = mx;
     unsigned long long sum = 0;
-    for (uint32_t t = t0 + threadIdx.x; t < t1; t += kBlock) {
-        const int64_t d = (int64_t)p.a.d_scores[o + t] - mx, idx = d + (((int64_t)1 << p.a.bit_shift) - 1);
-        const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
-        const int32_t e = p.a.d_exp_table[ok ? idx : 0];
-        if (!ok) bad |= (uint32_t)kWitIndex;
-        if (e < 0) bad |= (uint32_t)kWitSum;
-        p.a.d_exp[o + t] = e;
-        if (p.a.d_shifted) p.a.d_shifted[o + t] = (int32_t)d;
-        sum += (unsigned long long)(e < 0 ? 0 : e);
+    for (uint32_t t = t0 + threadIdx.x; t < t1; t += kBlock * kExpAhead) {
+        int32_t x[kExpAhead], e[kExpAhead];
+#pragma unroll
+        for (uint32_t j = 0; j < kExpAhead; j++) x[j] = t + j * kBlock < t1 ? p.a.d_scores[o + t + j * kBlock] : mx;
+#pragma unroll
+        for (uint32_t j = 0; j < kExpAhead; j++) {
+            const int64_t idx = (int64_t)x[j] - mx + (((int64_t)1 << p.a.bit_shift) - 1);
+            const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
+            e[j] = p.a.d_exp_table[ok ? idx : 0];
+            if (!ok && t + j * kBlock < t1) bad |= (uint32_t)kWitIndex;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kExpAhead; j++) {
+            const uint32_t i = t + j * kBlock;
+            if (i >= t1) break;
+            if (e[j] < 0) bad |= (uint32_t)kWitSum;
+            p.a.d_exp[o + i] = e[j];
+            if (p.a.d_shifted) p.a.d_shifted[o + i] = (int32_t)((int64_t)x[j] - mx);
+            sum += (unsigned long long)(e[j] < 0 ? 0 : e[j]);
+        }
     }
     sum = block_all(sum, [](unsigned long long x, unsigned long long y) { return x + y; });
     if (threadIdx.x == 0) p.sums[row * p.plan.exp_chunks + blockIdx.x] = sum;
@@ -333,25 +364,25 @@ __device__ __forceinline__ uint32_t probability(uint32_t e, uint64_t scale, uint
 }
 
 // Probabilities of a chunk of the positions for `rows` query heads, and their products with 64 * blocks elements of the values.
-// A wave takes 64 positions x 64 elements: lane l reads the elements 4 (l % 16) .. + 4 of the positions 16 (l / 16) .. + 16,
-// 256 bytes in a row among 16 lanes, and turns four positions' words into the planes of four positions, in registers.  The
-// waves of a workgroup take different blocks of 64 elements, or every second or fourth step of 64 positions.  Bound by reading the values.
+// A wave reads 256 bytes in a row among 16 lanes and turns four positions' words into the planes of four positions, in registers.
+// The waves of a workgroup take different blocks of 64 elements, or every second or fourth step.  Bound by reading the values.
 template <bool VEC, int PP>          // PP: planes of the probabilities
 __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ unsigned long long p_sum[16];
-    const uint32_t b = blockIdx.z, group = blockIdx.y % p.plan.groups, head_tile = blockIdx.y / p.plan.groups;
+    const uint32_t per_chunk = p.c.heads * p.plan.tiles * p.plan.groups, chunk = blockIdx.x / per_chunk, within = blockIdx.x - chunk * per_chunk;
+    const uint32_t b = blockIdx.y, head_tile = within / p.plan.groups, group = within - head_tile * p.plan.groups;
     const uint32_t kv = head_tile / p.plan.tiles, tile = head_tile - kv * p.plan.tiles;
     const uint32_t each = p.a.heads / p.c.heads, h0 = kv * each + tile * p.plan.rows, R = min(p.plan.rows, each - tile * p.plan.rows);
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, kg = lane >> 4, dim = p.c.dim;
     uint32_t lo, hi, bad = 0;
     span_of(p, b, lo, hi);
-    const uint64_t start = (uint64_t)lo + (uint64_t)blockIdx.x * p.plan.value_chunk;
+    const uint64_t start = (uint64_t)lo + (uint64_t)chunk * p.plan.value_chunk;
     const bool direct = hi - lo <= p.plan.value_chunk;          // the whole row is this workgroup's
     const uint32_t e0 = group * p.plan.blocks * 64, width = p.plan.blocks * 64;
     const size_t row0 = (size_t)b * p.a.heads + h0;
     if (start >= hi) {
-        if (lo == hi && blockIdx.x == 0) {                      // nothing to attend to
+        if (lo == hi && chunk == 0) {                      // nothing to attend to
             for (uint32_t i = threadIdx.x; i < R * width; i += 256) {
                 const uint32_t r = i / width, e = e0 + i - r * width;
                 if (e >= dim) continue;
@@ -366,11 +397,25 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
         return;
     }
     const uint32_t t0 = (uint32_t)start, n = min(hi - t0, p.plan.value_chunk), steps = (n + 63) / 64;
-    // [step][plane][lane group][row] operands of 16 positions each, and the positions' offsets
+    // [step of 32][plane][lane group][row] operands of 8 positions each, and the positions' offsets
     int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)p.plan.value_chunk * R * PP / 4);
     if (threadIdx.x < 16) p_sum[threadIdx.x] = 0;
     for (uint32_t i = threadIdx.x; i < steps * 64; i += 256) off[i] = i < n ? token_at(p, b, t0 + i) : -1;
     __syncthreads();
+    // A wave takes 32 positions x 64 elements a step: lane l reads the elements 4 (l % 16) .. + 4 of the positions 8 (l / 16) ..
+    // + 8.  Its first step is on its way while the probabilities are computed, and each next one while this one multiplies.
+    const uint32_t block = wave % p.plan.blocks, apart = 4 / p.plan.blocks, e = e0 + 64 * block, halves = (n + 31) / 32;
+    const int32_t* v = p.c.d_v + (int64_t)kv * p.c.head_stride;
+    auto fetch = [&](v4i_t x[8], uint32_t s) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const int64_t at = off[s * 32 + kg * 8 + i];
+            x[i] = load4<VEC>(v + (at < 0 ? 0 : at), e + 4 * col, dim);
+        }
+    };
+    v4i_t next[8];
+    uint32_t s = wave / p.plan.blocks;
+    if (s < halves) fetch(next, s);
     const uint32_t quads = steps * 16, parts = (hi - lo - 1) / p.plan.exp_chunk + 1;
     for (uint32_t r = wave; r < R; r += 4) {
         const size_t row = row0 + r;
@@ -382,7 +427,7 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
             bad |= (uint32_t)kWitSum;
             sum = 1;
         }
-        if (blockIdx.x == 0 && group == 0 && lane == 0 && p.a.d_sum) p.a.d_sum[row] = (int32_t)sum;
+        if (chunk == 0 && group == 0 && lane == 0 && p.a.d_sum) p.a.d_sum[row] = (int32_t)sum;
         const double inv = 1.0 / (double)sum;
         unsigned long long mine = 0;
         for (uint32_t quad = lane; quad < quads; quad += 64) {
@@ -406,9 +451,9 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
                 w[j] = digits_of((int32_t)pr);
             }
             transpose4(w[0], w[1], w[2], w[3], pl);
-            uint32_t* o = lds + ((((quad >> 4) * PP * 4 + ((quad >> 2) & 3u)) * R + r) << 2) + (quad & 3u);
+            uint32_t* o = lds + ((((quad >> 3) * PP * 4 + ((quad >> 1) & 3u)) * R + r) << 1) + (quad & 1u);
 #pragma unroll
-            for (int k = 0; k < PP; k++) o[k * 16 * R] = pl[k];
+            for (int k = 0; k < PP; k++) o[k * 8 * R] = pl[k];
         }
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) mine += __shfl_xor(mine, o, 64);
@@ -421,33 +466,27 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
     for (int j = 0; j < 4; j++)
 #pragma unroll
         for (int g = 0; g < G; g++) acc[j][g] = v4i_t{0, 0, 0, 0};
-    const uint32_t block = wave % p.plan.blocks, apart = 4 / p.plan.blocks, e = e0 + 64 * block;
-    const int32_t* v = p.c.d_v + (int64_t)kv * p.c.head_stride;
-    const uint32_t row = col < R ? col : R - 1;
-    for (uint32_t s = wave / p.plan.blocks; s < steps; s += apart) {
-        v4i_t x[16];
+    // row m of the product is query head 4 (m % 4) + m / 4, as in the scores
+    const uint32_t head = 4 * (col & 3u) + (col >> 2), row = head < R ? head : R - 1;
+    for (; s < halves; s += apart) {
+        v4i_t x[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 16; i++) {
-            const int64_t at = off[s * 64 + kg * 16 + i];
-            x[i] = load4<VEC>(v + (at < 0 ? 0 : at), e + 4 * col, dim);
-        }
-        v4i_t pa[PP];
+        for (int i = 0; i < 8; i++) x[i] = next[i];
+        if (s + apart < halves) fetch(next, s + apart);
+        long pa[PP];
 #pragma unroll
-        for (int k = 0; k < PP; k++) pa[k] = reinterpret_cast<const v4i_t*>(lds)[((s * PP + k) * 4 + kg) * R + row];
+        for (int k = 0; k < PP; k++) pa[k] = reinterpret_cast<const long*>(lds)[((s * PP + k) * 4 + kg) * R + row];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            v4i_t vb[4];
+            uint32_t p0[4], p1[4];
+            transpose4((uint32_t)x[0][j] ^ kByteTops, (uint32_t)x[1][j] ^ kByteTops, (uint32_t)x[2][j] ^ kByteTops, (uint32_t)x[3][j] ^ kByteTops, p0);
+            transpose4((uint32_t)x[4][j] ^ kByteTops, (uint32_t)x[5][j] ^ kByteTops, (uint32_t)x[6][j] ^ kByteTops, (uint32_t)x[7][j] ^ kByteTops, p1);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t pl[4];
-                transpose4((uint32_t)x[4 * c][j] ^ kByteTops, (uint32_t)x[4 * c + 1][j] ^ kByteTops, (uint32_t)x[4 * c + 2][j] ^ kByteTops, (uint32_t)x[4 * c + 3][j] ^ kByteTops, pl);
+            for (int k2 = 0; k2 < 4; k2++) {
+                const long vb = (long)(((uint64_t)p1[k2] << 32) | p0[k2]);
 #pragma unroll
-                for (int k = 0; k < 4; k++) vb[k][c] = (int)pl[k];
+                for (int k = 0; k < PP; k++) acc[j][k + k2] = __builtin_amdgcn_mfma_i32_16x16x32_i8(pa[k], vb, acc[j][k + k2], 0, 0, 0);
             }
-#pragma unroll
-            for (int k = 0; k < PP; k++)
-#pragma unroll
-                for (int k2 = 0; k2 < 4; k2++) acc[j][k + k2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[k], vb[k2], acc[j][k + k2], 0, 0, 0);
         }
     }
     __syncthreads();
@@ -458,8 +497,8 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
     for (int j = 0; j < 4; j++)
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) {
-            const uint32_t r = 4 * kg + i;
-            if (i < R && r < R) {
+            const uint32_t r = 4 * i + kg;
+            if (4 * i < R && r < R) {
                 uint64_t y = 0;
 #pragma unroll
                 for (int g = G - 1; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[j][g][i];
@@ -476,15 +515,16 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
             p.a.d_out[(row0 + r) * dim + el] = q;
             if (p.a.d_out_rem) p.a.d_out_rem[(row0 + r) * dim + el] = rem;
         } else {
-            p.part[((row0 + r) * p.plan.value_chunks + blockIdx.x) * dim + el] = (int64_t)total[i];
+            p.part[((row0 + r) * p.plan.value_chunks + chunk) * dim + el] = (int64_t)total[i];
         }
     }
     if (bad) atomicOr(p.status, bad);
 }
 
-// The chunks' partial sums of 64 elements of one row, four threads an element.
-__global__ void __launch_bounds__(kBlock) wit_attend_join_kernel(AttendArgs p) {
-    __shared__ int64_t sh[kBlock];
+// The chunks' partial sums of 64 elements of one row, sixteen threads an element.
+constexpr uint32_t kJoinThreads = 1024;
+__global__ void __launch_bounds__(kJoinThreads) wit_attend_join_kernel(AttendArgs p) {
+    __shared__ int64_t sh[kJoinThreads];
     const uint32_t h = blockIdx.y, b = blockIdx.z, e = blockIdx.x * 64 + (threadIdx.x & 63u), dim = p.c.dim;
     const size_t row = (size_t)b * p.a.heads + h;
     uint32_t lo, hi, bad = 0;
@@ -492,13 +532,17 @@ __global__ void __launch_bounds__(kBlock) wit_attend_join_kernel(AttendArgs p) {
     if (hi - lo <= p.plan.value_chunk) return;
     const uint32_t parts = (hi - lo - 1) / p.plan.value_chunk + 1;
     int64_t y = 0;
-    if (e < dim)
-        for (uint32_t i = threadIdx.x >> 6; i < parts; i += kBlock / 64) y += p.part[(row * p.plan.value_chunks + i) * dim + e];
+    if (e < dim) {
+#pragma unroll 8
+        for (uint32_t i = threadIdx.x >> 6; i < parts; i += kJoinThreads / 64) y += p.part[(row * p.plan.value_chunks + i) * dim + e];
+    }
     sh[threadIdx.x] = y;
     __syncthreads();
     if (threadIdx.x < 64 && e < dim) {
+#pragma unroll
+        for (uint32_t i = 1; i < kJoinThreads / 64; i++) y += sh[threadIdx.x + 64 * i];
         int32_t q, r;
-        p.out.apply(sh[threadIdx.x] + sh[threadIdx.x + 64] + sh[threadIdx.x + 128] + sh[threadIdx.x + 192], q, r, bad);
+        p.out.apply(y, q, r, bad);
         p.a.d_out[row * dim + e] = q;
         if (p.a.d_out_rem) p.a.d_out_rem[row * dim + e] = r;
     }
@@ -842,9 +886,11 @@ int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_
     auto aligned = [&](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
     const bool vec = p.c.dim % 4 == 0 && ((p.c.page_stride | p.c.token_stride | p.c.head_stride) & 3) == 0 && aligned(p.c.d_k) && aligned(p.c.d_v);
     const int planes = a.prob_scale <= ((int64_t)1 << 22) ? 3 : 4;
-    const size_t score_lds = (size_t)pl.dim64 * 5 * 64 * pl.rows;
+    const size_t score_lds = (size_t)pl.dim64 * 5 * 64 * pl.rows + (size_t)pl.score_chunk * 8 * (pl.rows + 1);
     const size_t value_lds = std::max<size_t>((size_t)pl.value_chunk * (pl.rows * planes + 8), (size_t)pl.rows * pl.blocks * 64 * 8);
-    const dim3 score_grid(std::max(1u, pl.score_chunks), p.c.heads * pl.tiles, a.seqs), value_grid(std::max(1u, pl.value_chunks), p.c.heads * pl.tiles * pl.groups, a.seqs);
+    // the heads of one chunk are neighbours: they read the same tokens' lines of memory at the same time
+    const uint32_t head_tiles = p.c.heads * pl.tiles;
+    const dim3 score_grid(std::max(1u, pl.score_chunks) * head_tiles, a.seqs), value_grid(std::max(1u, pl.value_chunks) * head_tiles * pl.groups, a.seqs);
     if (vec) wit_attend_scores_kernel<true><<<score_grid, 256, score_lds, s>>>(p);
     else wit_attend_scores_kernel<false><<<score_grid, 256, score_lds, s>>>(p);
     GRAPE_LAUNCH_CHECK();
@@ -858,7 +904,7 @@ int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_
     else wit_attend_values_kernel<false, 4><<<value_grid, 256, value_lds, s>>>(p);
     GRAPE_LAUNCH_CHECK();
     if (pl.value_chunks > 1) {
-        wit_attend_join_kernel<<<dim3(pl.dim64, a.heads, a.seqs), kBlock, 0, s>>>(p);
+        wit_attend_join_kernel<<<dim3(pl.dim64, a.heads, a.seqs), kJoinThreads, 0, s>>>(p);
         GRAPE_LAUNCH_CHECK();
     }
     return GRAPE_OK;

@@ -169,9 +169,9 @@ def test_plans_cover_every_position_within_their_limits(lib):
         for kind, step in (("score", 64), ("exp", 1024), ("value", 64 * 4 // p["blocks"])):
             assert p[kind + "_chunk"] % step == 0 and p[kind + "_chunk"] * p[kind + "_chunks"] >= n and (p[kind + "_chunks"] == 0 or p[kind + "_chunk"] * (p[kind + "_chunks"] - 1) < n)
         assert p["value_chunk"] <= 1024                                         # what the 32-bit sums of the planes' products hold
-        assert p["dim64"] * 64 * 5 * p["rows"] <= 61440                         # LDS
+        assert p["dim64"] * 64 * 5 * p["rows"] + 8 * p["score_chunk"] * (p["rows"] + 1) <= 61440          # LDS
         assert p["value_chunk"] * (p["rows"] * 4 + 8) <= 61440 and p["rows"] * p["blocks"] * 64 * 8 <= 61440
-        assert hk * p["tiles"] * p["groups"] <= 65535
+        assert hk * p["tiles"] * max(p["score_chunks"], p["value_chunks"] * p["groups"]) * 256 < 1 << 31
         rows = s * h
         need = [rows * n * 4, rows * n * 4, rows * p["score_chunks"] * 4, rows * p["exp_chunks"] * 8, rows * p["value_chunks"] * d * 8 if p["value_chunks"] > 1 else 0]
         at = [p[x] for x in ("at_scores", "at_exp", "at_max", "at_sum", "at_part", "bytes")]
