@@ -99,12 +99,12 @@ struct AttentionPlan {
     uint32_t rows, tiles;              // query heads of a workgroup, workgroups of a cache head
     uint32_t score_chunk, score_chunks;
     uint32_t exp_chunk, exp_chunks;
-    uint32_t blocks, groups;           // blocks of 64 elements of a values workgroup, workgroups of a head's elements
+    uint32_t blocks, groups;           // blocks of 32 elements of a values workgroup, workgroups of a head's elements
     uint32_t value_chunk, value_chunks;
     size_t at_scores, at_exp, at_max, at_sum, at_part, bytes;      // offsets in the workspace
 };
 constexpr uint32_t kTokenLds = 60 * 1024;      // of a workgroup
-constexpr uint32_t kWorkgroups = 2048;
+constexpr uint32_t kWorkgroups = 4096;
 
 inline uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
 
@@ -133,14 +133,16 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
     if (score_most < 64) return false;
     p.score_chunk = chunk(beside, 64, score_most, kWorkgroups);
     p.score_chunks = ceil_div(max_len, p.score_chunk);
-    p.exp_chunk = chunk(rows_all, 1024, (uint32_t)1 << 20, kWorkgroups);
+    p.exp_chunk = chunk(rows_all, 1024, (uint32_t)1 << 20, kWorkgroups / 2);
     p.exp_chunks = ceil_div(max_len, p.exp_chunk);
-    p.blocks = p.dim64 % 4 == 0 ? 4 : p.dim64 % 2 == 0 ? 2 : 1;
-    p.groups = p.dim64 / p.blocks;
-    const uint32_t step = 64 * (4 / p.blocks);
+    // four waves share a workgroup's elements, 32 each; those that find none left take every second or fourth step instead
+    const uint32_t dim32 = ceil_div(dim, 32);
+    p.blocks = dim32 > 2 ? 4 : dim32;
+    p.groups = ceil_div(dim32, p.blocks);
+    const uint32_t step = 32 * (4 / p.blocks) < 64 ? 64 : 32 * (4 / p.blocks);
     uint32_t most = kTokenLds / (4 * p.rows + 8) / step * step;
     if (most > 1024) most = 1024;
-    p.value_chunk = chunk(beside * p.groups, step, most, kWorkgroups / 2);
+    p.value_chunk = chunk(beside * p.groups, step, most, kWorkgroups / 4);
     p.value_chunks = ceil_div(max_len, p.value_chunk);
     // a launch's first axis, in threads
     if ((uint64_t)cache_heads * p.tiles * std::max<uint64_t>(p.score_chunks, (uint64_t)p.value_chunks * p.groups) >= (uint64_t)1 << 23) return false;

@@ -147,10 +147,34 @@ __device__ __forceinline__ bool span_of(const AttendArgs& p, uint32_t b, uint32_
     return token::live_span(p.a.d_lens[b], p.a.d_first ? p.a.d_first[b] : 0, p.a.max_len, p.a.table_stride, p.c.page_size, lo, hi);
 }
 
-__device__ __forceinline__ int64_t token_at(const AttendArgs& p, uint32_t b, uint32_t t) {
-    const uint32_t pg = p.page(t);
-    return token::token_offset(p.c, p.a.d_block_table[(size_t)b * p.a.table_stride + pg], t - pg * p.c.page_size);
-}
+// The offsets of a chunk's positions t0 .. t0 + n, made by all 256 threads of a workgroup.  The first page of each thread is
+// requested before the sequence's length is known where it does not depend on it, so that the two loads are under way together.
+struct Offsets {
+    int32_t page = -1;
+    uint32_t t = 0;
+    bool early = false;
+    __device__ __forceinline__ int32_t load(const AttendArgs& p, uint32_t b, uint32_t pos) const {
+        return p.a.d_block_table[(size_t)b * p.a.table_stride + p.page(pos)];
+    }
+    __device__ __forceinline__ void request(const AttendArgs& p, uint32_t b, uint64_t start, uint32_t most) {
+        early = p.a.d_first == nullptr;
+        t = (uint32_t)start + threadIdx.x;
+        if (early && threadIdx.x < most && start + threadIdx.x < p.a.max_len && p.page(t) < p.a.table_stride) page = load(p, b, t);
+    }
+    __device__ __forceinline__ bool store(const AttendArgs& p, uint32_t b, uint32_t t0, uint32_t n, uint32_t filled, int64_t* off) const {
+        bool outside = false;
+        for (uint32_t i = threadIdx.x; i < filled; i += 256) {
+            int64_t o = -1;
+            if (i < n) {
+                const int32_t pg = early && i == threadIdx.x ? page : load(p, b, t0 + i);
+                o = token::token_offset(p.c, pg, t0 + i - p.page(t0 + i) * p.c.page_size);
+                outside |= o < 0;
+            }
+            off[i] = o;
+        }
+        return outside;
+    }
+};
 
 // four elements from x; those from `n` on are whatever comes first
 template <bool VEC>
@@ -161,6 +185,19 @@ __device__ __forceinline__ v4i_t load4(const int32_t* x, uint32_t at, uint32_t n
         v4i_t v;
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) v[j] = x[at + j < n ? at + j : 0];
+        return v;
+    }
+}
+
+typedef int v2i_t __attribute__((ext_vector_type(2)));
+template <bool VEC>
+__device__ __forceinline__ v2i_t load2(const int32_t* x, uint32_t at, uint32_t n) {
+    if constexpr (VEC) {
+        return *reinterpret_cast<const v2i_t*>(x + (at < n ? at : 0));
+    } else {
+        v2i_t v;
+#pragma unroll
+        for (uint32_t j = 0; j < 2; j++) v[j] = x[at + j < n ? at + j : 0];
         return v;
     }
 }
@@ -178,35 +215,42 @@ __global__ void __launch_bounds__(256, 4) wit_attend_scores_kernel(AttendArgs p)
     const uint32_t each = p.a.heads / p.c.heads, h0 = kv * each + tile * p.plan.rows, R = min(p.plan.rows, each - tile * p.plan.rows);
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, kg = lane >> 4, dim = p.c.dim, steps = p.plan.dim64;
     uint32_t lo, hi, bad = 0;
+    // what does not depend on the sequence's length is requested beside it
+    const uint32_t items = R * steps * 16;
+    auto query = [&](uint32_t i, int32_t v[4]) {
+        const uint32_t r = i / (steps * 16), quad = i - r * (steps * 16);
+        const int32_t* q = p.a.d_q + b * p.a.q_stride + (size_t)(h0 + r) * dim;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) v[j] = 4 * quad + j < dim ? q[4 * quad + j] : 0;
+    };
+    int32_t q4[4] = {0, 0, 0, 0};
+    if (threadIdx.x < items) query(threadIdx.x, q4);
+    Offsets offsets;
+    offsets.request(p, b, (uint64_t)chunk * p.plan.score_chunk, p.plan.score_chunk);
     const bool fits = span_of(p, b, lo, hi);
     if (!fits && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.status, (uint32_t)kWitIndex);
     const uint64_t start = (uint64_t)lo + (uint64_t)chunk * p.plan.score_chunk;
     if (start >= hi) return;
-    const uint32_t t0 = (uint32_t)start, t1 = min(hi, t0 + p.plan.score_chunk);
+    const uint32_t t0 = (uint32_t)start, n = min(hi - t0, p.plan.score_chunk);
     if (threadIdx.x < 16) q_sum[threadIdx.x] = 0;
     if (threadIdx.x == 0) over_any = 0;
     // behind the digits: the positions' offsets and the scores' 64-bit sums, so that nothing but the keys is read or written on
     // the way (waiting for any other load or store would wait for all keys requested before it)
     int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)5 * 16 * steps * p.plan.rows);
     uint64_t* sums = reinterpret_cast<uint64_t*>(off + p.plan.score_chunk);            // [row][position]
-    const uint32_t n = t1 - t0;
-    for (uint32_t i = threadIdx.x; i < n; i += 256) {
-        off[i] = token_at(p, b, t0 + i);
-        if (off[i] < 0) bad |= (uint32_t)kWitIndex;
-    }
+    if (offsets.store(p, b, t0, n, n, off)) bad |= (uint32_t)kWitIndex;
     __syncthreads();
     // the queries' digits: [step][plane 0..4][lane group][row], 16 bytes each; plane 4 holds what a top digit of 128 carries
-    for (uint32_t i = threadIdx.x; i < R * steps * 16; i += 256) {
+    for (uint32_t i = threadIdx.x; i < items; i += 256) {
         const uint32_t r = i / (steps * 16), quad = i - r * (steps * 16), s = quad >> 4, c = (quad >> 2) & 3u, g = quad & 3u;
-        const int32_t* q = p.a.d_q + b * p.a.q_stride + (size_t)(h0 + r) * dim;
+        if (i != threadIdx.x) query(i, q4);
         uint32_t w[4], pl[4], carry = 0;
         long long sum = 0;
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
-            const int32_t v = 4 * quad + j < dim ? q[4 * quad + j] : 0;
-            w[j] = digits_of(v);
-            sum += v;
-            carry |= v > kDigitTop ? 1u << (8 * j) : 0u;
+            w[j] = digits_of(q4[j]);
+            sum += q4[j];
+            carry |= q4[j] > kDigitTop ? 1u << (8 * j) : 0u;
         }
         transpose4(w[0], w[1], w[2], w[3], pl);
         uint32_t* o = lds + (((s * 5 * 4 + g) * R + r) << 2) + c;
@@ -312,8 +356,8 @@ __device__ __forceinline__ T block_all(T v, F f) {
     return v;
 }
 
-// Exponentials of a chunk of one row, and their sum.  Bound by the gathers' latency: four are under way a thread.
-constexpr uint32_t kExpAhead = 4;
+// Exponentials of a chunk of one row, and their sum.  Bound by the gathers' latency: eight are under way a thread.
+constexpr uint32_t kExpAhead = 8;
 __global__ void __launch_bounds__(kBlock) wit_attend_exp_kernel(AttendArgs p) {
     const uint32_t h = blockIdx.y, b = blockIdx.z;
     const size_t row = (size_t)b * p.a.heads + h, o = row * p.a.max_len;
@@ -363,11 +407,12 @@ __device__ __forceinline__ uint32_t probability(uint32_t e, uint64_t scale, uint
     return (uint32_t)q;
 }
 
-// Probabilities of a chunk of the positions for `rows` query heads, and their products with 64 * blocks elements of the values.
-// A wave reads 256 bytes in a row among 16 lanes and turns four positions' words into the planes of four positions, in registers.
+// Probabilities of a chunk of the positions for `rows` query heads, and their products with 32 * blocks elements of the values.
+// A wave reads a line among 16 lanes and turns four positions' words into the planes of four positions, in registers.
 // The waves of a workgroup take different blocks of 64 elements, or every second or fourth step.  Bound by reading the values.
+constexpr uint32_t kProbAhead = 2;   // four positions each under way a lane
 template <bool VEC, int PP>          // PP: planes of the probabilities
-__global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p) {
+__global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ unsigned long long p_sum[16];
     const uint32_t per_chunk = p.c.heads * p.plan.tiles * p.plan.groups, chunk = blockIdx.x / per_chunk, within = blockIdx.x - chunk * per_chunk;
@@ -376,10 +421,12 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
     const uint32_t each = p.a.heads / p.c.heads, h0 = kv * each + tile * p.plan.rows, R = min(p.plan.rows, each - tile * p.plan.rows);
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, kg = lane >> 4, dim = p.c.dim;
     uint32_t lo, hi, bad = 0;
+    Offsets offsets;
+    offsets.request(p, b, (uint64_t)chunk * p.plan.value_chunk, p.plan.value_chunk);
     span_of(p, b, lo, hi);
     const uint64_t start = (uint64_t)lo + (uint64_t)chunk * p.plan.value_chunk;
     const bool direct = hi - lo <= p.plan.value_chunk;          // the whole row is this workgroup's
-    const uint32_t e0 = group * p.plan.blocks * 64, width = p.plan.blocks * 64;
+    const uint32_t e0 = group * p.plan.blocks * 32, width = p.plan.blocks * 32;
     const size_t row0 = (size_t)b * p.a.heads + h0;
     if (start >= hi) {
         if (lo == hi && chunk == 0) {                      // nothing to attend to
@@ -400,20 +447,20 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
     // [step of 32][plane][lane group][row] operands of 8 positions each, and the positions' offsets
     int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)p.plan.value_chunk * R * PP / 4);
     if (threadIdx.x < 16) p_sum[threadIdx.x] = 0;
-    for (uint32_t i = threadIdx.x; i < steps * 64; i += 256) off[i] = i < n ? token_at(p, b, t0 + i) : -1;
+    offsets.store(p, b, t0, n, steps * 64, off);
     __syncthreads();
-    // A wave takes 32 positions x 64 elements a step: lane l reads the elements 4 (l % 16) .. + 4 of the positions 8 (l / 16) ..
+    // A wave takes 32 positions x 32 elements a step: lane l reads the elements 2 (l % 16), + 1 of the positions 8 (l / 16) ..
     // + 8.  Its first step is on its way while the probabilities are computed, and each next one while this one multiplies.
-    const uint32_t block = wave % p.plan.blocks, apart = 4 / p.plan.blocks, e = e0 + 64 * block, halves = (n + 31) / 32;
+    const uint32_t block = wave % p.plan.blocks, apart = 4 / p.plan.blocks, e = e0 + 32 * block, halves = e < dim ? (n + 31) / 32 : 0;
     const int32_t* v = p.c.d_v + (int64_t)kv * p.c.head_stride;
-    auto fetch = [&](v4i_t x[8], uint32_t s) {
+    auto fetch = [&](v2i_t x[8], uint32_t s) {
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
             const int64_t at = off[s * 32 + kg * 8 + i];
-            x[i] = load4<VEC>(v + (at < 0 ? 0 : at), e + 4 * col, dim);
+            x[i] = load2<VEC>(v + (at < 0 ? 0 : at), e + 2 * col, dim);
         }
     };
-    v4i_t next[8];
+    v2i_t next[8];
     uint32_t s = wave / p.plan.blocks;
     if (s < halves) fetch(next, s);
     const uint32_t quads = steps * 16, parts = (hi - lo - 1) / p.plan.exp_chunk + 1;
@@ -430,30 +477,42 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
         if (chunk == 0 && group == 0 && lane == 0 && p.a.d_sum) p.a.d_sum[row] = (int32_t)sum;
         const double inv = 1.0 / (double)sum;
         unsigned long long mine = 0;
-        for (uint32_t quad = lane; quad < quads; quad += 64) {
-            uint32_t w[4], pl[4];
+        for (uint32_t first = lane; first < quads; first += 64 * kProbAhead) {
+            int32_t ex[kProbAhead][4];
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t i = 4 * quad + j;
-                uint32_t pr = 0;
-                if (i < n) {
-                    const size_t o = row * p.a.max_len + t0 + i;
-                    const int32_t e = p.a.d_exp[o];
-                    const uint32_t ev = e < 0 ? 0 : (uint32_t)e;
-                    pr = probability(ev, (uint64_t)p.a.prob_scale, sum, inv);
-                    if (group == 0) {
-                        if (p.a.d_prob) p.a.d_prob[o] = (int32_t)pr;
-                        if (p.a.d_query) p.a.d_query[o] = (int32_t)((uint64_t)ev * 2 * (uint64_t)p.a.prob_scale - sum * (2 * (uint64_t)pr - 1));
-                    }
-                    if (off[i] < 0) pr = 0;                     // a page outside the cache
+            for (uint32_t a = 0; a < kProbAhead; a++)
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {
+                    const uint32_t i = 4 * (first + 64 * a) + j;
+                    ex[a][j] = i < n ? p.a.d_exp[row * p.a.max_len + t0 + i] : 0;
                 }
-                mine += pr;
-                w[j] = digits_of((int32_t)pr);
-            }
-            transpose4(w[0], w[1], w[2], w[3], pl);
-            uint32_t* o = lds + ((((quad >> 3) * PP * 4 + ((quad >> 1) & 3u)) * R + r) << 1) + (quad & 1u);
 #pragma unroll
-            for (int k = 0; k < PP; k++) o[k * 8 * R] = pl[k];
+            for (uint32_t a = 0; a < kProbAhead; a++) {
+                const uint32_t quad = first + 64 * a;
+                if (quad >= quads) break;
+                uint32_t w[4], pl[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {
+                    const uint32_t i = 4 * quad + j;
+                    uint32_t pr = 0;
+                    if (i < n) {
+                        const size_t o = row * p.a.max_len + t0 + i;
+                        const uint32_t ev = ex[a][j] < 0 ? 0 : (uint32_t)ex[a][j];
+                        pr = probability(ev, (uint64_t)p.a.prob_scale, sum, inv);
+                        if (group == 0) {
+                            if (p.a.d_prob) p.a.d_prob[o] = (int32_t)pr;
+                            if (p.a.d_query) p.a.d_query[o] = (int32_t)((uint64_t)ev * 2 * (uint64_t)p.a.prob_scale - sum * (2 * (uint64_t)pr - 1));
+                        }
+                        if (off[i] < 0) pr = 0;                     // a page outside the cache
+                    }
+                    mine += pr;
+                    w[j] = digits_of((int32_t)pr);
+                }
+                transpose4(w[0], w[1], w[2], w[3], pl);
+                uint32_t* o = lds + ((((quad >> 3) * PP * 4 + ((quad >> 1) & 3u)) * R + r) << 1) + (quad & 1u);
+#pragma unroll
+                for (int k = 0; k < PP; k++) o[k * 8 * R] = pl[k];
+            }
         }
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) mine += __shfl_xor(mine, o, 64);
@@ -461,15 +520,15 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
     }
     __syncthreads();
     constexpr int G = PP + 3;
-    v4i_t acc[4][G];
+    v4i_t acc[2][G];
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+    for (int j = 0; j < 2; j++)
 #pragma unroll
         for (int g = 0; g < G; g++) acc[j][g] = v4i_t{0, 0, 0, 0};
     // row m of the product is query head 4 (m % 4) + m / 4, as in the scores
     const uint32_t head = 4 * (col & 3u) + (col >> 2), row = head < R ? head : R - 1;
     for (; s < halves; s += apart) {
-        v4i_t x[8];
+        v2i_t x[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = next[i];
         if (s + apart < halves) fetch(next, s + apart);
@@ -477,7 +536,7 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
 #pragma unroll
         for (int k = 0; k < PP; k++) pa[k] = reinterpret_cast<const long*>(lds)[((s * PP + k) * 4 + kg) * R + row];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < 2; j++) {
             uint32_t p0[4], p1[4];
             transpose4((uint32_t)x[0][j] ^ kByteTops, (uint32_t)x[1][j] ^ kByteTops, (uint32_t)x[2][j] ^ kByteTops, (uint32_t)x[3][j] ^ kByteTops, p0);
             transpose4((uint32_t)x[4][j] ^ kByteTops, (uint32_t)x[5][j] ^ kByteTops, (uint32_t)x[6][j] ^ kByteTops, (uint32_t)x[7][j] ^ kByteTops, p1);
@@ -490,11 +549,11 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
         }
     }
     __syncthreads();
-    unsigned long long* total = reinterpret_cast<unsigned long long*>(lds);          // [rows][64 * blocks]
+    unsigned long long* total = reinterpret_cast<unsigned long long*>(lds);          // [rows][32 * blocks]
     for (uint32_t i = threadIdx.x; i < R * width; i += 256) total[i] = (unsigned long long)kCacheOffset * p_sum[i / width];
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+    for (int j = 0; j < 2; j++)
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) {
             const uint32_t r = 4 * i + kg;
@@ -502,7 +561,7 @@ __global__ void __launch_bounds__(256, 2) wit_attend_values_kernel(AttendArgs p)
                 uint64_t y = 0;
 #pragma unroll
                 for (int g = G - 1; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[j][g][i];
-                atomicAdd(&total[r * width + 64 * block + 4 * col + j], (unsigned long long)y);
+                atomicAdd(&total[r * width + 32 * block + 2 * col + j], (unsigned long long)y);
             }
         }
     __syncthreads();
@@ -887,7 +946,7 @@ int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_
     const bool vec = p.c.dim % 4 == 0 && ((p.c.page_stride | p.c.token_stride | p.c.head_stride) & 3) == 0 && aligned(p.c.d_k) && aligned(p.c.d_v);
     const int planes = a.prob_scale <= ((int64_t)1 << 22) ? 3 : 4;
     const size_t score_lds = (size_t)pl.dim64 * 5 * 64 * pl.rows + (size_t)pl.score_chunk * 8 * (pl.rows + 1);
-    const size_t value_lds = std::max<size_t>((size_t)pl.value_chunk * (pl.rows * planes + 8), (size_t)pl.rows * pl.blocks * 64 * 8);
+    const size_t value_lds = std::max<size_t>((size_t)pl.value_chunk * (pl.rows * planes + 8), (size_t)pl.rows * pl.blocks * 32 * 8);
     // the heads of one chunk are neighbours: they read the same tokens' lines of memory at the same time
     const uint32_t head_tiles = p.c.heads * pl.tiles;
     const dim3 score_grid(std::max(1u, pl.score_chunks) * head_tiles, a.seqs), value_grid(std::max(1u, pl.value_chunks) * head_tiles * pl.groups, a.seqs);

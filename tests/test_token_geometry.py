@@ -165,12 +165,12 @@ def test_plans_cover_every_position_within_their_limits(lib):
         taken += 1
         p = dict(zip(names, out))
         assert p["dim64"] * 64 >= d > (p["dim64"] - 1) * 64 and 1 <= p["rows"] <= 16 and p["rows"] * p["tiles"] >= h // hk > p["rows"] * (p["tiles"] - 1)
-        assert p["blocks"] * p["groups"] == p["dim64"] and p["blocks"] in (1, 2, 4)
-        for kind, step in (("score", 64), ("exp", 1024), ("value", 64 * 4 // p["blocks"])):
+        assert p["blocks"] * p["groups"] * 32 >= d and p["blocks"] * (p["groups"] - 1) * 32 < d and p["blocks"] in (1, 2, 4)
+        for kind, step in (("score", 64), ("exp", 1024), ("value", 64)):
             assert p[kind + "_chunk"] % step == 0 and p[kind + "_chunk"] * p[kind + "_chunks"] >= n and (p[kind + "_chunks"] == 0 or p[kind + "_chunk"] * (p[kind + "_chunks"] - 1) < n)
         assert p["value_chunk"] <= 1024                                         # what the 32-bit sums of the planes' products hold
         assert p["dim64"] * 64 * 5 * p["rows"] + 8 * p["score_chunk"] * (p["rows"] + 1) <= 61440          # LDS
-        assert p["value_chunk"] * (p["rows"] * 4 + 8) <= 61440 and p["rows"] * p["blocks"] * 64 * 8 <= 61440
+        assert p["value_chunk"] * (p["rows"] * 4 + 8) <= 61440 and p["rows"] * p["blocks"] * 32 * 8 <= 61440
         assert hk * p["tiles"] * max(p["score_chunks"], p["value_chunks"] * p["groups"]) * 256 < 1 << 31
         rows = s * h
         need = [rows * n * 4, rows * n * 4, rows * p["score_chunks"] * 4, rows * p["exp_chunks"] * 8, rows * p["value_chunks"] * d * 8 if p["value_chunks"] > 1 else 0]
