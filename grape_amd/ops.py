@@ -732,34 +732,38 @@ def wit_rmsnorm_apply(x, rms, w, scale=1 << 16):
 
 
 # ------------------------------------------------------------------ the witness of new tokens
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
-
-
+# These calls are small and many, so their checks are written to cost little: no message is made before it is needed.
 def _place():
-    return torch.device("cuda", torch.cuda.current_device())
+    return torch.cuda.current_device()
+
+
+def _stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _refuse(msg, *args):
+    raise ValueError(msg % args if args else msg)
 
 
 def _arr(t, name, shape, dev, dtype=torch.int32):
     """address of a contiguous tensor of that shape and type on the current device; 0 for None"""
     if t is None:
         return 0
-    _need(t.dtype is dtype and t.device == dev and t.shape == shape and t.is_contiguous(),
-          "%s must be a contiguous %s tensor of shape %s on the current device" % (name, dtype, tuple(shape)))
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        _refuse("%s must be a contiguous %s tensor of shape %s on the current device", name, dtype, tuple(shape))
     return t.data_ptr()
 
 
 def _rows(t, name, shape, dev, dtype=torch.int32):
     """the same for rows (all but the first axis) that are contiguous each; address and elements from row to row"""
-    _need(t.dtype is dtype and t.device == dev and t.shape == shape, "%s must be a %s tensor of shape %s on the current device" % (name, dtype, tuple(shape)))
-    if t.is_contiguous():
-        return t.data_ptr(), t.numel() // max(t.shape[0], 1)
-    step = 1
-    for n, s in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        _need(n == 1 or s == step, "the rows of %s must be contiguous" % name)
-        step *= n
-    return t.data_ptr(), t.stride(0)
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev:
+        _refuse("%s must be a %s tensor of shape %s on the current device", name, dtype, tuple(shape))
+    st, step = t.stride(), 1
+    for i in range(len(shape) - 1, 0, -1):
+        if st[i] != step and shape[i] > 1:
+            _refuse("the rows of %s must be contiguous", name)
+        step *= shape[i]
+    return t.data_ptr(), st[0]
 
 
 _CACHE = struct.Struct("<2Q4I3q")
@@ -768,13 +772,16 @@ _ATTEND = struct.Struct("<Qq16Q3q6I")
 
 
 def _cache(k_cache, v_cache, dev):
-    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(),
-          "the caches must be (pages, page size, heads, dim) tensors of the same shape and strides")
-    _need(k_cache.dtype is torch.int32 and v_cache.dtype is torch.int32 and k_cache.device == dev and v_cache.device == dev,
-          "the caches must be int32 tensors on the current device")
-    _need(k_cache.stride(3) == 1 or k_cache.shape[3] == 1, "the elements of a head must be contiguous")
-    pages, page, heads, dim = k_cache.shape
-    return _CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), pages, page, heads, dim, *k_cache.stride()[:3])
+    """the caches' struct, heads and elements of a head"""
+    shape, st = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != st:
+        _refuse("the caches must be (pages, page size, heads, dim) tensors of the same shape and strides")
+    if k_cache.dtype is not torch.int32 or v_cache.dtype is not torch.int32 or k_cache.get_device() != dev or v_cache.get_device() != dev:
+        _refuse("the caches must be int32 tensors on the current device")
+    pages, page, heads, dim = shape
+    if st[3] != 1 and dim > 1:
+        _refuse("the elements of a head must be contiguous")
+    return _CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), pages, page, heads, dim, st[0], st[1], st[2]), heads, dim
 
 
 def wit_rope_append(q, k, v, positions, slots, cos, sin, k_cache, v_cache, q_out=None, q_rem=None, k_rem=None, scale=1 << 16, interleaved=False):
@@ -784,32 +791,41 @@ def wit_rope_append(q, k, v, positions, slots, cos, sin, k_cache, v_cache, q_out
     q = None (with q_out None): keys and values only."""
     lib = init()
     dev = _place()
-    cache = _cache(k_cache, v_cache, dev)
-    heads_kv, dim = k_cache.shape[2:]
-    n = k.shape[0]
-    kp, ks = _rows(k, "k", (n, heads_kv, dim), dev)
-    vp, vs = _rows(v, "v", (n, heads_kv, dim), dev)
-    qp = qs = heads = 0
+    cache, heads_kv, dim = _cache(k_cache, v_cache, dev)
+    n = len(k)
+    kv_shape = (n, heads_kv, dim)
+    kp, ks = _rows(k, "k", kv_shape, dev)
+    vp, vs = _rows(v, "v", kv_shape, dev)
+    qp = qs = heads = qo = qr = 0
     if q is not None:
-        _need(q.dim() == 3 and q.shape[1] >= 1, "q must be (tokens, heads, dim)")
+        if q.dim() != 3 or q.shape[1] < 1:
+            _refuse("q must be (tokens, heads, dim)")
         heads = q.shape[1]
-        qp, qs = _rows(q, "q", (n, heads, dim), dev)
+        q_shape = (n, heads, dim)
+        qp, qs = _rows(q, "q", q_shape, dev)
         if q_out is None:
-            q_out = torch.zeros((n, heads, dim), dtype=torch.int32, device=dev)      # rows of padding are not written
-    else:
-        _need(q_out is None and q_rem is None, "q_out and q_rem need q")
-    _need(cos.dim() == 2 and cos.shape == sin.shape, "cos and sin must be (rows, rot / 2) tensors")
-    rows, half = cos.shape
+            q_out = torch.zeros(q_shape, dtype=torch.int32, device=q.device)      # rows of padding are not written
+        qo, qr = _arr(q_out, "q_out", q_shape, dev), _arr(q_rem, "q_rem", q_shape, dev)
+    elif q_out is not None or q_rem is not None:
+        _refuse("q_out and q_rem need q")
+    table = cos.shape
+    if len(table) != 2:
+        _refuse("cos and sin must be (rows, rot / 2) tensors")
     args = _APPEND.pack(qp, kp, vp, qs, ks, vs, _arr(positions, "positions", (n,), dev), _arr(slots, "slots", (n,), dev, torch.int64),
-                        _arr(cos, "cos", (rows, half), dev), _arr(sin, "sin", (rows, half), dev),
-                        _arr(q_out, "q_out", (n, heads, dim), dev), _arr(q_rem, "q_rem", (n, heads, dim), dev),
-                        _arr(k_rem, "k_rem", (n, heads_kv, dim), dev), n, heads, 2 * half, rows, int(scale), 1 if interleaved else 0, 0)
-    _capi.check(lib.grape_wit_rope_append(args, cache, _s()))
+                        _arr(cos, "cos", table, dev), _arr(sin, "sin", table, dev), qo, qr, _arr(k_rem, "k_rem", kv_shape, dev), n, heads,
+                        2 * table[1], table[0], scale, 1 if interleaved else 0, 0)
+    _check(lib.grape_wit_rope_append(args, cache, _stream(dev)))
     return q_out
+
+
+def _check(rc):
+    if rc:
+        _capi.check(rc)
 
 
 # what a proof looks up of an attention, [seqs][heads][max_len] each, in the order of the C ABI's fields
 _PROOF_ROWS = ("scores", "scores_rem", "exp_input", "exp_output", "softmax_output", "softmax_lookup_query")
+_NAMES = frozenset(_PROOF_ROWS + ("max", "exp_sum", "qkv", "qkv_rem"))
 
 
 def wit_paged_attention(q, k_cache, v_cache, block_table, lens, max_len, exp_table, first=None, bit_shift=20, index_bits=20,
@@ -822,32 +838,38 @@ def wit_paged_attention(q, k_cache, v_cache, block_table, lens, max_len, exp_tab
     tensor of wit_paged_attention_workspace(...) bytes; without one the call makes its own."""
     lib = init()
     dev = _place()
-    cache = _cache(k_cache, v_cache, dev)
-    dim = k_cache.shape[3]
-    _need(q.dim() == 3, "q must be (seqs, heads, dim)")
-    n, heads = q.shape[:2]
-    qp, qs = _rows(q, "q", (n, heads, dim), dev)
-    _need(block_table.dim() == 2, "block_table must be (seqs, pages)")
-    width = block_table.shape[1]
-    _need(exp_table.shape == (1 << index_bits,), "the exponential table must have 2^index_bits entries")
-    _need(max_len >= 0, "max_len must not be negative")
+    cache, heads_kv, dim = _cache(k_cache, v_cache, dev)
+    if q.dim() != 3:
+        _refuse("q must be (seqs, heads, dim)")
+    n, heads, _ = q.shape
+    rows, row, one = (n, heads, max_len), (n, heads, dim), (n, heads)
+    qp, qs = _rows(q, "q", row, dev)
+    width = block_table.shape
+    if len(width) != 2 or width[0] != n:
+        _refuse("block_table must be (seqs, pages)")
+    if exp_table.shape != (1 << index_bits,):
+        _refuse("the exponential table must have 2^index_bits entries")
+    if max_len < 0:
+        _refuse("max_len must not be negative")
     if out is None:
-        out = {"qkv": _i32(n, heads, dim), "qkv_rem": _i32(n, heads, dim)}
+        out = {"qkv": _i32(*row), "qkv_rem": _i32(*row)}
         if proof:
-            out["max"], out["exp_sum"] = _i32(n, heads), _i32(n, heads)
+            out["max"], out["exp_sum"] = _i32(*one), _i32(*one)
             for name in _PROOF_ROWS:
-                out[name] = torch.zeros((n, heads, max_len), dtype=torch.int32, device=dev)
-    shapes = dict.fromkeys(_PROOF_ROWS, (n, heads, max_len))
-    shapes.update(max=(n, heads), exp_sum=(n, heads), qkv=(n, heads, dim), qkv_rem=(n, heads, dim))
-    _need("qkv" in out and not set(out) - set(shapes), "out must hold qkv, and may hold %s" % ", ".join(x for x in shapes if x != "qkv"))
-    at = [_arr(out.get(name), name, shape, dev) for name, shape in shapes.items()]
+                out[name] = torch.zeros(rows, dtype=torch.int32, device=q.device)
+    get = out.get
+    if "qkv" not in out or not _NAMES.issuperset(out):
+        _refuse("out must hold qkv, and may hold %s", ", ".join(sorted(_NAMES)))
     if workspace is None:
-        workspace = torch.empty(wit_paged_attention_workspace(n, heads, k_cache.shape[2], dim, max_len), dtype=torch.uint8, device=dev)
-    _need(workspace.dtype is torch.uint8 and workspace.device == dev and workspace.is_contiguous(), "the workspace must be a contiguous uint8 tensor")
-    args = _ATTEND.pack(qp, qs, _arr(block_table, "block_table", (n, width), dev), _arr(lens, "lens", (n,), dev), _arr(first, "first", (n,), dev),
-                        _arr(exp_table, "exp_table", exp_table.shape, dev), *at, workspace.data_ptr(), workspace.numel(),
-                        int(qk_scale), int(prob_scale), int(out_scale), n, heads, max_len, width, bit_shift, index_bits)
-    _capi.check(lib.grape_wit_paged_attention(args, cache, _s()))
+        workspace = torch.empty(lib.grape_wit_paged_attention_workspace(n, heads, heads_kv, dim, max_len), dtype=torch.uint8, device=q.device)
+    elif workspace.dtype is not torch.uint8 or workspace.get_device() != dev or not workspace.is_contiguous():
+        _refuse("the workspace must be a contiguous uint8 tensor")
+    args = _ATTEND.pack(qp, qs, _arr(block_table, "block_table", width, dev), _arr(lens, "lens", (n,), dev), _arr(first, "first", (n,), dev),
+                        _arr(exp_table, "exp_table", exp_table.shape, dev), *[_arr(get(name), name, rows, dev) for name in _PROOF_ROWS],
+                        _arr(get("max"), "max", one, dev), _arr(get("exp_sum"), "exp_sum", one, dev), _arr(get("qkv"), "qkv", row, dev),
+                        _arr(get("qkv_rem"), "qkv_rem", row, dev), workspace.data_ptr(), workspace.numel(), qk_scale, prob_scale, out_scale, n,
+                        heads, max_len, width[1], bit_shift, index_bits)
+    _check(lib.grape_wit_paged_attention(args, cache, _stream(dev)))
     return out
 
 
@@ -861,20 +883,21 @@ def wit_matvec_q4(x, w, scales, group, zeros=None, scale=1 << 16, q=None, r=None
     scales (outputs, ceil(inputs / group)) int32 and zero points (the same, uint8; None: all 8).  Returns quotient, remainder."""
     lib = init()
     dev = _place()
-    _need(x.dim() == 2 and w.dim() == 2 and group >= 1, "x must be (tokens, inputs), w (outputs, bytes), group positive")
+    if x.dim() != 2 or w.dim() != 2 or group < 1:
+        _refuse("x must be (tokens, inputs), w (outputs, bytes), group positive")
     n, k = x.shape
-    m = w.shape[0]
-    _need(k >= 1, "empty inner dimension")
-    groups = (k - 1) // group + 1
+    m = len(w)
+    if k < 1:
+        _refuse("empty inner dimension")
+    groups = (m, (k - 1) // group + 1)
     xp, xs = _rows(x, "x", (n, k), dev)
     wp, ws = _rows(w, "w", (m, (k + 1) // 2), dev, torch.uint8)
     if q is None:
         q = _i32(n, m)
     if r is None and want_r:
         r = _i32(n, m)
-    _capi.check(lib.grape_wit_matvec_q4(_arr(q, "q", (n, m), dev), _arr(r, "r", (n, m), dev), xp, xs, wp, ws,
-                                        _arr(scales, "scales", (m, groups), dev), _arr(zeros, "zeros", (m, groups), dev, torch.uint8),
-                                        n, m, k, group, int(scale), _s()))
+    _check(lib.grape_wit_matvec_q4(_arr(q, "q", (n, m), dev), _arr(r, "r", (n, m), dev), xp, xs, wp, ws, _arr(scales, "scales", groups, dev),
+                                   _arr(zeros, "zeros", groups, dev, torch.uint8), n, m, k, group, scale, _stream(dev)))
     return q, r
 
 

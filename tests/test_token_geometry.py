@@ -200,8 +200,8 @@ def helpers(monkeypatch):
                 return 64 if name.endswith("_workspace") else 0
             return call
     monkeypatch.setattr(ops, "init", lambda *a: Library())
-    monkeypatch.setattr(ops, "_place", lambda: torch.device("cpu"))
-    monkeypatch.setattr(ops, "_s", lambda: None)
+    monkeypatch.setattr(ops, "_place", lambda: -1)          # what get_device() says of host tensors
+    monkeypatch.setattr(ops, "_stream", lambda dev: None)
     monkeypatch.setattr(ops, "_i32", lambda *s: torch.empty(s, dtype=torch.int32))
     return calls
 
@@ -220,12 +220,21 @@ def append_args():
                                  dict(slots=torch.zeros(6, dtype=torch.int64)[::2]), dict(cos=i32(99, 32)), dict(sin=i32(100, 31)), dict(cos=i32(32, 100).t(), sin=i32(32, 100).t()),
                                  dict(k_cache=i32(10, 16, 256)), dict(v_cache=i32(11, 16, 4, 64)), dict(k_cache=i32(10, 16, 64, 4).transpose(2, 3), v_cache=i32(10, 16, 64, 4).transpose(2, 3)),
                                  dict(k_cache=i32(10, 16, 4, 64).long(), v_cache=i32(10, 16, 4, 64).long()), dict(q_out=i32(3, 8, 63)), dict(q_rem=i32(3, 4, 64)), dict(k_rem=i32(3, 8, 64)),
-                                 dict(q=None), dict(q=i32(3, 8, 64).to("meta"))])
+                                 dict(q=None)])
 def test_append_helper_refuses(helpers, bad):
     ops.wit_rope_append(**append_args())
     with pytest.raises(ValueError):
         ops.wit_rope_append(**{**append_args(), **bad})
     assert len(helpers) == 1
+
+
+def test_helpers_refuse_tensors_of_another_device(helpers, monkeypatch):
+    monkeypatch.setattr(ops, "_place", lambda: 0)
+    for call, args in ((ops.wit_rope_append, append_args()), (ops.wit_paged_attention, attend_args()),
+                       (ops.wit_matvec_q4, dict(x=i32(2, 64), w=torch.zeros((8, 32), dtype=torch.uint8), scales=i32(8, 2), group=32))):
+        with pytest.raises(ValueError):
+            call(**args)
+    assert not helpers
 
 
 def attend_args():
