@@ -1,0 +1,745 @@
+// Attention of one new token a sequence over a paged cache of keys and values, with the tensors that a proof of it looks up.
+#include <algorithm>
+#include "token_device.hpp"
+
+namespace grape {
+
+// ------------------------------------------------------------------------------------------------
+// Attention of one token a sequence: scores, softmax through the table, products with the values.
+//
+// The softmax is the table's, rounded, so a running maximum cannot be corrected later by a factor: the maximum of the whole row
+// is needed before the first exponential and the sum of all before the first probability.  Hence three launches, each over
+// chunks of the positions, and a fourth that joins the values' partial sums.  Keys and values are read once; what goes between
+// the launches is 4 bytes a head and position.
+//
+// Both products run on the matrix cores: a cache element x is taken as x - c, c = 128 (1 + 2^8 + 2^16), whose balanced digits
+// are the bytes of x with three top bits turned over, and c times the sum of the other operand is added in the end.  The pairs
+// of planes with the same sum of exponents share an accumulator: 4 * 2^14 * 8192 elements (1024 positions) stay below 2^31.
+// ------------------------------------------------------------------------------------------------
+constexpr int64_t kCacheOffset = 0x808080;
+constexpr uint32_t kByteTops = 0x00808080;
+
+struct AttendArgs {
+    grape_wit_attention_args a;
+    grape_wit_cache c;
+    token::AttentionPlan plan;
+    token::FastDiv page;
+    Scaler qk, out;
+    int32_t* chunk_max;          // [seqs][heads][score chunks]
+    unsigned long long* sums;    // [seqs][heads][exp chunks]
+    int64_t* part;               // [seqs][heads][value chunks][dim]
+    uint32_t* status;
+};
+
+__device__ __forceinline__ bool span_of(const AttendArgs& p, uint32_t b, uint32_t& lo, uint32_t& hi) {
+    return token::live_span(p.a.d_lens[b], p.a.d_first ? p.a.d_first[b] : 0, p.a.max_len, p.a.table_stride, p.c.page_size, lo, hi);
+}
+
+// The offsets of a chunk's positions t0 .. t0 + n, made by all 256 threads of a workgroup.  The first page of each thread is
+// requested before the sequence's length is known where it does not depend on it, so that the two loads are under way together.
+struct Offsets {
+    int32_t page = -1;
+    uint32_t t = 0;
+    bool early = false;
+    __device__ __forceinline__ int32_t load(const AttendArgs& p, uint32_t b, uint32_t pos) const {
+        return p.a.d_block_table[(size_t)b * p.a.table_stride + p.page(pos)];
+    }
+    __device__ __forceinline__ void request(const AttendArgs& p, uint32_t b, uint64_t start, uint32_t most) {
+        early = p.a.d_first == nullptr;
+        t = (uint32_t)start + threadIdx.x;
+        if (early && threadIdx.x < most && start + threadIdx.x < p.a.max_len && p.page(t) < p.a.table_stride) page = load(p, b, t);
+    }
+    __device__ __forceinline__ bool store(const AttendArgs& p, uint32_t b, uint32_t t0, uint32_t n, uint32_t filled, int64_t* off) const {
+        bool outside = false;
+        for (uint32_t i = threadIdx.x; i < filled; i += 256) {
+            int64_t o = -1;
+            if (i < n) {
+                const int32_t pg = early && i == threadIdx.x ? page : load(p, b, t0 + i);
+                o = token::token_offset(p.c, pg, t0 + i - p.page(t0 + i) * p.c.page_size);
+                outside |= o < 0;
+            }
+            off[i] = o;
+        }
+        return outside;
+    }
+};
+
+// four elements from x; those from `n` on are whatever comes first
+template <bool VEC>
+__device__ __forceinline__ v4i_t load4(const int32_t* x, uint32_t at, uint32_t n) {
+    if constexpr (VEC) {
+        return *reinterpret_cast<const v4i_t*>(x + (at < n ? at : 0));          // n is a multiple of 4
+    } else {
+        v4i_t v;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) v[j] = x[at + j < n ? at + j : 0];
+        return v;
+    }
+}
+
+typedef int v2i_t __attribute__((ext_vector_type(2)));
+template <bool VEC>
+__device__ __forceinline__ v2i_t load2(const int32_t* x, uint32_t at, uint32_t n) {
+    if constexpr (VEC) {
+        return *reinterpret_cast<const v2i_t*>(x + (at < n ? at : 0));
+    } else {
+        v2i_t v;
+#pragma unroll
+        for (uint32_t j = 0; j < 2; j++) v[j] = x[at + j < n ? at + j : 0];
+        return v;
+    }
+}
+
+// The query heads of a workgroup: R heads from h0 of sequence b, which read the cache's head kv.
+struct Tile {
+    uint32_t b, kv, h0, R;
+    size_t row0;                 // of the rows [seqs][heads]
+    uint32_t lane, wave, col, kg;
+    __device__ __forceinline__ Tile(const AttendArgs& p, uint32_t b_, uint32_t head_tile) : b(b_) {
+        const uint32_t each = p.a.heads / p.c.heads;
+        kv = head_tile / p.plan.tiles;
+        const uint32_t tile = head_tile - kv * p.plan.tiles;
+        h0 = kv * each + tile * p.plan.rows;
+        R = min(p.plan.rows, each - tile * p.plan.rows);
+        row0 = (size_t)b * p.a.heads + h0;
+        lane = threadIdx.x & 63u;
+        wave = threadIdx.x >> 6;
+        col = lane & 15u;
+        kg = lane >> 4;
+    }
+    // Row m of a product is query head 4 (m % 4) + m / 4: register i of lane l then holds head 4 i + l / 16 at column l % 16, and
+    // four heads need one register of every lane.  Rows past the last head repeat it; nothing of them is kept.
+    __device__ __forceinline__ uint32_t row() const {
+        const uint32_t head = 4 * (col & 3u) + (col >> 2);
+        return head < R ? head : R - 1;
+    }
+};
+
+// The queries' digits in LDS, [step of 64][plane 0..4][lane group][row], 16 bytes each, with plane 4 what a top digit of 128
+// carries; and the queries' sums.  q4: this thread's first four elements, requested by first().
+struct Queries {
+    int32_t q4[4];
+    __device__ __forceinline__ void load(const AttendArgs& p, const Tile& w, uint32_t i) {
+        const uint32_t steps = p.plan.dim64, r = i / (steps * 16), quad = i - r * (steps * 16);
+        const int32_t* q = p.a.d_q + w.b * p.a.q_stride + (size_t)(w.h0 + r) * p.c.dim;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) q4[j] = 4 * quad + j < p.c.dim ? q[4 * quad + j] : 0;
+    }
+    __device__ __forceinline__ void first(const AttendArgs& p, const Tile& w) {
+        if (threadIdx.x < w.R * p.plan.dim64 * 16) load(p, w, threadIdx.x);
+    }
+    __device__ __forceinline__ void store(const AttendArgs& p, const Tile& w, uint32_t* digits, unsigned long long* q_sum, uint32_t* over_any) {
+        const uint32_t steps = p.plan.dim64;
+        for (uint32_t i = threadIdx.x; i < w.R * steps * 16; i += 256) {
+            const uint32_t r = i / (steps * 16), quad = i - r * (steps * 16), s = quad >> 4, c = (quad >> 2) & 3u, g = quad & 3u;
+            if (i != threadIdx.x) load(p, w, i);
+            uint32_t d[4], pl[4], carry = 0;
+            long long sum = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                d[j] = digits_of(q4[j]);
+                sum += q4[j];
+                carry |= q4[j] > kDigitTop ? 1u << (8 * j) : 0u;
+            }
+            transpose4(d[0], d[1], d[2], d[3], pl);
+            uint32_t* o = digits + (((s * 5 * 4 + g) * w.R + r) << 2) + c;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) o[k * 16 * w.R] = pl[k];
+            o[4 * 16 * w.R] = carry;
+            if (carry) *over_any = 1;
+            // sixteen neighbouring lanes are of one row
+#pragma unroll
+            for (int k = 8; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, 64);
+            if ((i & 15u) == 0) atomicAdd(&q_sum[r], (unsigned long long)sum);
+        }
+    }
+};
+
+// Products of the queries with n keys, as 64-bit sums [row][stride] in LDS (of the keys less their offset).  A wave takes 16
+// positions: lane l reads those elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16 that make up its operand of step s
+// (any order of a step's elements will do, as long as the queries' digits have the same), whole lines among the lanes.
+template <bool VEC>
+__device__ __forceinline__ void score_products(const AttendArgs& p, const Tile& w, uint32_t n, const int64_t* off, const uint32_t* digits, bool over,
+                                               uint64_t* sums, uint32_t stride) {
+    const uint32_t steps = p.plan.dim64, R = w.R, row = w.row(), dim = p.c.dim;
+    const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
+    for (uint32_t at = 16 * w.wave; at < n; at += 64) {
+        const int32_t* k = keys + max(off[min(at + w.col, n - 1)], (int64_t)0);
+        v4i_t acc[8];
+#pragma unroll
+        for (int g = 0; g < 8; g++) acc[g] = v4i_t{0, 0, 0, 0};
+        // two steps at a time: their keys are requested together, and other waves multiply meanwhile
+        for (uint32_t s = 0; s < steps; s += 2) {
+            v4i_t x[8];
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) x[c] = load4<VEC>(k, 64 * s + 16 * c + 4 * w.kg, dim);
+            if (s + 1 < steps) {
+#pragma unroll
+                for (uint32_t c = 4; c < 8; c++) x[c] = load4<VEC>(k, 64 * s + 16 * c + 4 * w.kg, dim);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < 2; u++) {
+                if (s + u >= steps) break;
+                v4i_t kb[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const v4i_t y = x[4 * u + c];
+                    uint32_t pl[4];
+                    transpose4((uint32_t)y[0] ^ kByteTops, (uint32_t)y[1] ^ kByteTops, (uint32_t)y[2] ^ kByteTops, (uint32_t)y[3] ^ kByteTops, pl);
+#pragma unroll
+                    for (int k2 = 0; k2 < 4; k2++) kb[k2][c] = (int)pl[k2];
+                }
+                const v4i_t* qa = reinterpret_cast<const v4i_t*>(digits) + ((s + u) * 5 * 4 + w.kg) * R + row;
+#pragma unroll
+                for (int a = 0; a < 4; a++) {
+                    const v4i_t f = qa[a * 4 * R];
+#pragma unroll
+                    for (int k2 = 0; k2 < 4; k2++) acc[a + k2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, kb[k2], acc[a + k2], 0, 0, 0);
+                }
+                if (over) {
+                    const v4i_t f = qa[4 * 4 * R];
+#pragma unroll
+                    for (int k2 = 0; k2 < 4; k2++) acc[4 + k2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, kb[k2], acc[4 + k2], 0, 0, 0);
+                }
+            }
+        }
+        if (at + w.col < n) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const uint32_t r = 4 * i + w.kg;
+                if (4 * i < R && r < R) {
+                    uint64_t y = 0;
+#pragma unroll
+                    for (int g = 7; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[g][i];
+                    sums[r * stride + at + w.col] = y;
+                }
+            }
+        }
+    }
+}
+
+// Those sums rescaled and written; the largest score of each row goes to largest(r, max).
+template <class F>
+__device__ __forceinline__ void score_rows(const AttendArgs& p, const Tile& w, uint32_t t0, uint32_t n, const int64_t* off, const uint64_t* sums, uint32_t stride,
+                                           const unsigned long long* q_sum, uint32_t& bad, F largest) {
+    for (uint32_t r = w.wave; r < w.R; r += 4) {
+        const size_t o = (w.row0 + r) * p.a.max_len + t0;
+        const uint64_t more = (uint64_t)kCacheOffset * q_sum[r];
+        int32_t mx = INT32_MIN;
+        for (uint32_t i = w.lane; i < n; i += 64) {
+            const int64_t y = off[i] < 0 ? 0 : (int64_t)(sums[r * stride + i] + more);          // a page outside: zero
+            int32_t q, rem;
+            p.qk.apply(y, q, rem, bad);
+            p.a.d_scores[o + i] = q;
+            if (p.a.d_scores_rem) p.a.d_scores_rem[o + i] = rem;
+            mx = max(mx, q);
+        }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) mx = max(mx, __shfl_xor(mx, d, 64));
+        if (w.lane == 0) largest(r, mx);
+    }
+}
+
+// Exponentials of the scores t0 + i of row `row`, i = from, from + step, ... below n, and their sum.  Bound by the gathers'
+// latency: eight are under way a thread.
+constexpr uint32_t kExpAhead = 8;
+__device__ __forceinline__ unsigned long long exponentials(const AttendArgs& p, size_t row, uint32_t t0, uint32_t from, uint32_t step, uint32_t n, int32_t mx, uint32_t& bad) {
+    const size_t o = row * p.a.max_len + t0;
+    unsigned long long sum = 0;
+    for (uint32_t t = from; t < n; t += step * kExpAhead) {
+        int32_t x[kExpAhead], e[kExpAhead];
+#pragma unroll
+        for (uint32_t j = 0; j < kExpAhead; j++) x[j] = t + j * step < n ? p.a.d_scores[o + t + j * step] : mx;
+#pragma unroll
+        for (uint32_t j = 0; j < kExpAhead; j++) {
+            const int64_t idx = (int64_t)x[j] - mx + (((int64_t)1 << p.a.bit_shift) - 1);
+            const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
+            e[j] = p.a.d_exp_table[ok ? idx : 0];
+            if (!ok && t + j * step < n) bad |= (uint32_t)kWitIndex;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kExpAhead; j++) {
+            const uint32_t i = t + j * step;
+            if (i >= n) break;
+            if (e[j] < 0) bad |= (uint32_t)kWitSum;
+            p.a.d_exp[o + i] = e[j];
+            if (p.a.d_shifted) p.a.d_shifted[o + i] = (int32_t)((int64_t)x[j] - mx);
+            sum += (unsigned long long)(e[j] < 0 ? 0 : e[j]);
+        }
+    }
+    return sum;
+}
+
+// floor((e * scale + sum / 2) / sum) for e <= sum: the quotient is at most `scale`, so one product in double precision is off by one at most
+__device__ __forceinline__ uint32_t probability(uint32_t e, uint64_t scale, uint64_t sum, double inv) {
+    const uint64_t num = e * scale + (sum >> 1);
+    uint64_t q = (uint64_t)((double)num * inv);
+    const int64_t rest = (int64_t)(num - q * sum);
+    if (rest < 0) q--;
+    else if (rest >= (int64_t)sum) q++;
+    return (uint32_t)q;
+}
+
+// Probabilities of n positions of row r from their exponentials, written if `write`, and their digits in LDS: [step of 32][plane]
+// [lane group][row], operands of 8 positions each, zero up to a whole number of 64 positions and for pages outside the cache.
+// A wave a row; returns the sum of the probabilities that the values are multiplied with.
+constexpr uint32_t kProbAhead = 2;   // four positions each under way a lane
+template <int PP>                    // planes of the probabilities
+__device__ __forceinline__ unsigned long long probabilities(const AttendArgs& p, const Tile& w, uint32_t r, uint32_t t0, uint32_t n, const int64_t* off,
+                                                            unsigned long long sum, bool write, uint32_t* digits) {
+    const size_t o = (w.row0 + r) * p.a.max_len + t0;
+    const double inv = 1.0 / (double)sum;
+    const uint32_t quads = (n + 63) / 64 * 16;
+    unsigned long long mine = 0;
+    for (uint32_t first = w.lane; first < quads; first += 64 * kProbAhead) {
+        int32_t ex[kProbAhead][4];
+#pragma unroll
+        for (uint32_t a = 0; a < kProbAhead; a++)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t i = 4 * (first + 64 * a) + j;
+                ex[a][j] = i < n ? p.a.d_exp[o + i] : 0;
+            }
+#pragma unroll
+        for (uint32_t a = 0; a < kProbAhead; a++) {
+            const uint32_t quad = first + 64 * a;
+            if (quad >= quads) break;
+            uint32_t d[4], pl[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t i = 4 * quad + j;
+                uint32_t pr = 0;
+                if (i < n) {
+                    const uint32_t ev = ex[a][j] < 0 ? 0 : (uint32_t)ex[a][j];
+                    pr = probability(ev, (uint64_t)p.a.prob_scale, sum, inv);
+                    if (write) {
+                        if (p.a.d_prob) p.a.d_prob[o + i] = (int32_t)pr;
+                        if (p.a.d_query) p.a.d_query[o + i] = (int32_t)((uint64_t)ev * 2 * (uint64_t)p.a.prob_scale - sum * (2 * (uint64_t)pr - 1));
+                    }
+                    if (off[i] < 0) pr = 0;
+                }
+                mine += pr;
+                d[j] = digits_of((int32_t)pr);
+            }
+            transpose4(d[0], d[1], d[2], d[3], pl);
+            uint32_t* out = digits + ((((quad >> 3) * PP * 4 + ((quad >> 1) & 3u)) * w.R + r) << 1) + (quad & 1u);
+#pragma unroll
+            for (int k = 0; k < PP; k++) out[k * 8 * w.R] = pl[k];
+        }
+    }
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) mine += __shfl_xor(mine, k, 64);
+    return mine;
+}
+
+// Products of the probabilities with 32 elements (from e) of n values.  A wave takes 32 positions a step: lane l reads the
+// elements 2 (l % 16), + 1 of the positions 8 (l / 16) .. + 8, a line among 16 lanes, and turns four positions' words into the
+// planes of four positions, in registers.  Every next step is on its way while this one multiplies.
+template <bool VEC, int PP>
+struct ValueProducts {
+    static constexpr int G = PP + 3;
+    v2i_t next[8];
+    v4i_t acc[2][G];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int g = 0; g < G; g++) acc[j][g] = v4i_t{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ void fetch(const AttendArgs& p, const Tile& w, const int64_t* off, uint32_t e, uint32_t s) {
+        const int32_t* v = p.c.d_v + (int64_t)w.kv * p.c.head_stride;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const int64_t at = off[s * 32 + w.kg * 8 + i];
+            next[i] = load2<VEC>(v + (at < 0 ? 0 : at), e + 2 * w.col, p.c.dim);
+        }
+    }
+    // steps s, s + apart, ... below `halves`; the first has been fetched
+    __device__ __forceinline__ void run(const AttendArgs& p, const Tile& w, const int64_t* off, const uint32_t* digits, uint32_t e, uint32_t s, uint32_t apart, uint32_t halves) {
+        const uint32_t row = w.row();
+        for (; s < halves; s += apart) {
+            v2i_t x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = next[i];
+            if (s + apart < halves) fetch(p, w, off, e, s + apart);
+            long pa[PP];
+#pragma unroll
+            for (int k = 0; k < PP; k++) pa[k] = reinterpret_cast<const long*>(digits)[((s * PP + k) * 4 + w.kg) * w.R + row];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                uint32_t p0[4], p1[4];
+                transpose4((uint32_t)x[0][j] ^ kByteTops, (uint32_t)x[1][j] ^ kByteTops, (uint32_t)x[2][j] ^ kByteTops, (uint32_t)x[3][j] ^ kByteTops, p0);
+                transpose4((uint32_t)x[4][j] ^ kByteTops, (uint32_t)x[5][j] ^ kByteTops, (uint32_t)x[6][j] ^ kByteTops, (uint32_t)x[7][j] ^ kByteTops, p1);
+#pragma unroll
+                for (int k2 = 0; k2 < 4; k2++) {
+                    const long vb = (long)(((uint64_t)p1[k2] << 32) | p0[k2]);
+#pragma unroll
+                    for (int k = 0; k < PP; k++) acc[j][k + k2] = __builtin_amdgcn_mfma_i32_16x16x32_i8(pa[k], vb, acc[j][k + k2], 0, 0, 0);
+                }
+            }
+        }
+    }
+    // added to 64-bit sums [row][width] in LDS, this wave's 32 elements from `at`, as far as they are within the width
+    __device__ __forceinline__ void add(const Tile& w, unsigned long long* total, uint32_t width, uint32_t at) {
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const uint32_t r = 4 * i + w.kg, el = at + 2 * w.col + j;
+                if (4 * i < w.R && r < w.R && el < width) {
+                    uint64_t y = 0;
+#pragma unroll
+                    for (int g = G - 1; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[j][g][i];
+                    atomicAdd(&total[r * width + el], (unsigned long long)y);
+                }
+            }
+    }
+};
+
+__device__ __forceinline__ void write_out(const AttendArgs& p, size_t row, uint32_t e, int64_t y, uint32_t& bad) {
+    int32_t q, rem;
+    p.out.apply(y, q, rem, bad);
+    p.a.d_out[row * p.c.dim + e] = q;
+    if (p.a.d_out_rem) p.a.d_out_rem[row * p.c.dim + e] = rem;
+}
+
+// Rows with nothing to attend to: elements e0 .. e0 + width of the output, and the maximum and sum if `rows`.
+__device__ __forceinline__ void write_empty(const AttendArgs& p, const Tile& w, uint32_t e0, uint32_t width, bool rows) {
+    for (uint32_t i = threadIdx.x; i < w.R * width; i += 256) {
+        const uint32_t r = i / width, e = e0 + i - r * width;
+        if (e >= p.c.dim) continue;
+        p.a.d_out[(w.row0 + r) * p.c.dim + e] = 0;
+        if (p.a.d_out_rem) p.a.d_out_rem[(w.row0 + r) * p.c.dim + e] = 0;
+    }
+    if (rows && threadIdx.x < w.R) {
+        if (p.a.d_max) p.a.d_max[w.row0 + threadIdx.x] = 0;
+        if (p.a.d_sum) p.a.d_sum[w.row0 + threadIdx.x] = 0;
+    }
+}
+
+// ---- the launches over chunks
+// Scores of `rows` query heads with a chunk of the keys.  Bound by reading the keys.
+template <bool VEC>
+__global__ void __launch_bounds__(256, 4) wit_attend_scores_kernel(AttendArgs p) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    __shared__ unsigned long long q_sum[16];
+    __shared__ uint32_t over_any;
+    const uint32_t per_chunk = p.c.heads * p.plan.tiles, chunk = blockIdx.x / per_chunk;
+    const Tile w(p, blockIdx.y, blockIdx.x - chunk * per_chunk);
+    uint32_t lo, hi, bad = 0;
+    // what does not depend on the sequence's length is requested beside it
+    Queries queries;
+    queries.first(p, w);
+    Offsets offsets;
+    offsets.request(p, w.b, (uint64_t)chunk * p.plan.score_chunk, p.plan.score_chunk);
+    const bool fits = span_of(p, w.b, lo, hi);
+    if (!fits && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.status, (uint32_t)kWitIndex);
+    const uint64_t start = (uint64_t)lo + (uint64_t)chunk * p.plan.score_chunk;
+    if (start >= hi) return;
+    const uint32_t t0 = (uint32_t)start, n = min(hi - t0, p.plan.score_chunk);
+    if (threadIdx.x < 16) q_sum[threadIdx.x] = 0;
+    if (threadIdx.x == 0) over_any = 0;
+    // behind the digits: the positions' offsets and the scores' 64-bit sums, so that nothing but the keys is read or written on
+    // the way (waiting for any other load or store would wait for all keys requested before it)
+    int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)5 * 16 * p.plan.dim64 * p.plan.rows);
+    uint64_t* sums = reinterpret_cast<uint64_t*>(off + p.plan.score_chunk);
+    if (offsets.store(p, w.b, t0, n, n, off)) bad |= (uint32_t)kWitIndex;
+    __syncthreads();
+    queries.store(p, w, lds, q_sum, &over_any);
+    __syncthreads();
+    score_products<VEC>(p, w, n, off, lds, over_any != 0, sums, p.plan.score_chunk);
+    __syncthreads();
+    score_rows(p, w, t0, n, off, sums, p.plan.score_chunk, q_sum, bad,
+               [&](uint32_t r, int32_t mx) { p.chunk_max[(w.row0 + r) * p.plan.score_chunks + chunk] = mx; });
+    if (bad) atomicOr(p.status, bad);
+}
+
+template <class T, class F>
+__device__ __forceinline__ T block_all(T v, F f) {
+    __shared__ T sh[kBlock / 64];
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) v = f(v, __shfl_xor(v, off, 64));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < kBlock / 64; w++) v = f(v, sh[w]);
+    __syncthreads();
+    return v;
+}
+
+// Exponentials of a chunk of one row, and their sum.
+__global__ void __launch_bounds__(kBlock) wit_attend_exp_kernel(AttendArgs p) {
+    const uint32_t b = blockIdx.z;
+    const size_t row = (size_t)b * p.a.heads + blockIdx.y;
+    uint32_t lo, hi, bad = 0;
+    span_of(p, b, lo, hi);
+    const uint64_t start = (uint64_t)lo + (uint64_t)blockIdx.x * p.plan.exp_chunk;
+    if (start >= hi) return;
+    const uint32_t t0 = (uint32_t)start, n = min(hi - t0, p.plan.exp_chunk), parts = (hi - lo - 1) / p.plan.score_chunk + 1;
+    int32_t mx = INT32_MIN;
+    for (uint32_t i = threadIdx.x; i < parts; i += kBlock) mx = max(mx, p.chunk_max[row * p.plan.score_chunks + i]);
+    mx = block_all(mx, [](int32_t x, int32_t y) { return max(x, y); });
+    if (blockIdx.x == 0 && threadIdx.x == 0 && p.a.d_max) p.a.d_max[row] = mx;
+    unsigned long long sum = exponentials(p, row, t0, threadIdx.x, kBlock, n, mx, bad);
+    sum = block_all(sum, [](unsigned long long x, unsigned long long y) { return x + y; });
+    if (threadIdx.x == 0) p.sums[row * p.plan.exp_chunks + blockIdx.x] = sum;
+    if (bad) atomicOr(p.status, bad);
+}
+
+// Probabilities of a chunk of the positions for `rows` query heads, and their products with 32 * blocks elements of the values.
+// The waves take different blocks of 32 elements, or every second or fourth step.  Bound by reading the values.
+template <bool VEC, int PP>
+__global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    __shared__ unsigned long long p_sum[16];
+    const uint32_t per_chunk = p.c.heads * p.plan.tiles * p.plan.groups, chunk = blockIdx.x / per_chunk, within = blockIdx.x - chunk * per_chunk;
+    const uint32_t group = within % p.plan.groups;
+    const Tile w(p, blockIdx.y, within / p.plan.groups);
+    uint32_t lo, hi, bad = 0;
+    Offsets offsets;
+    offsets.request(p, w.b, (uint64_t)chunk * p.plan.value_chunk, p.plan.value_chunk);
+    span_of(p, w.b, lo, hi);
+    const uint64_t start = (uint64_t)lo + (uint64_t)chunk * p.plan.value_chunk;
+    const bool direct = hi - lo <= p.plan.value_chunk;          // the whole row is this workgroup's
+    const uint32_t e0 = group * p.plan.blocks * 32, width = p.plan.blocks * 32, dim = p.c.dim;
+    if (start >= hi) {
+        if (lo == hi && chunk == 0) write_empty(p, w, e0, width, group == 0);
+        return;
+    }
+    const uint32_t t0 = (uint32_t)start, n = min(hi - t0, p.plan.value_chunk);
+    int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)p.plan.value_chunk * w.R * PP / 4);        // behind the digits
+    if (threadIdx.x < 16) p_sum[threadIdx.x] = 0;
+    offsets.store(p, w.b, t0, n, (n + 63) / 64 * 64, off);
+    __syncthreads();
+    const uint32_t block = w.wave % p.plan.blocks, apart = 4 / p.plan.blocks, e = e0 + 32 * block, halves = e < dim ? (n + 31) / 32 : 0, s = w.wave / p.plan.blocks;
+    ValueProducts<VEC, PP> products;
+    if (s < halves) products.fetch(p, w, off, e, s);            // under way while the probabilities are computed
+    const uint32_t parts = (hi - lo - 1) / p.plan.exp_chunk + 1;
+    for (uint32_t r = w.wave; r < w.R; r += 4) {
+        const size_t row = w.row0 + r;
+        unsigned long long sum = 0;
+        for (uint32_t i = w.lane; i < parts; i += 64) sum += p.sums[row * p.plan.exp_chunks + i];
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if (sum == 0) {
+            bad |= (uint32_t)kWitSum;
+            sum = 1;
+        }
+        if (chunk == 0 && group == 0 && w.lane == 0 && p.a.d_sum) p.a.d_sum[row] = (int32_t)sum;
+        const unsigned long long mine = probabilities<PP>(p, w, r, t0, n, off, sum, group == 0, lds);
+        if (w.lane == 0) p_sum[r] = mine;
+    }
+    __syncthreads();
+    products.clear();
+    products.run(p, w, off, lds, e, s, apart, halves);
+    __syncthreads();
+    unsigned long long* total = reinterpret_cast<unsigned long long*>(lds);          // [rows][32 * blocks]
+    for (uint32_t i = threadIdx.x; i < w.R * width; i += 256) total[i] = (unsigned long long)kCacheOffset * p_sum[i / width];
+    __syncthreads();
+    products.add(w, total, width, 32 * block);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < w.R * width; i += 256) {
+        const uint32_t r = i / width, el = e0 + i - r * width;
+        if (el >= dim) continue;
+        if (direct) write_out(p, w.row0 + r, el, (int64_t)total[i], bad);
+        else p.part[((w.row0 + r) * p.plan.value_chunks + chunk) * dim + el] = (int64_t)total[i];
+    }
+    if (bad) atomicOr(p.status, bad);
+}
+
+// The chunks' partial sums of 64 elements of one row, sixteen threads an element.
+constexpr uint32_t kJoinThreads = 1024;
+__global__ void __launch_bounds__(kJoinThreads) wit_attend_join_kernel(AttendArgs p) {
+    __shared__ int64_t sh[kJoinThreads];
+    const uint32_t h = blockIdx.y, b = blockIdx.z, e = blockIdx.x * 64 + (threadIdx.x & 63u), dim = p.c.dim;
+    const size_t row = (size_t)b * p.a.heads + h;
+    uint32_t lo, hi, bad = 0;
+    span_of(p, b, lo, hi);
+    if (hi - lo <= p.plan.value_chunk) return;
+    const uint32_t parts = (hi - lo - 1) / p.plan.value_chunk + 1;
+    int64_t y = 0;
+    if (e < dim) {
+#pragma unroll 8
+        for (uint32_t i = threadIdx.x >> 6; i < parts; i += kJoinThreads / 64) y += p.part[(row * p.plan.value_chunks + i) * dim + e];
+    }
+    sh[threadIdx.x] = y;
+    __syncthreads();
+    if (threadIdx.x < 64 && e < dim) {
+#pragma unroll
+        for (uint32_t i = 1; i < kJoinThreads / 64; i++) y += sh[threadIdx.x + 64 * i];
+        write_out(p, row, e, y, bad);
+    }
+    if (bad) atomicOr(p.status, bad);
+}
+
+// ---- the same in one launch, a workgroup for all positions of its query heads
+template <bool VEC, int PP>
+__global__ void __launch_bounds__(256, 3) wit_attend_whole_kernel(AttendArgs p) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    __shared__ unsigned long long q_sum[16], e_sum[16], p_sum[16];
+    __shared__ int32_t row_max[16];
+    __shared__ uint32_t over_any;
+    constexpr uint32_t C = token::kWholeChunk;
+    const Tile w(p, blockIdx.y, blockIdx.x);
+    const uint32_t dim = p.c.dim;
+    uint32_t lo, hi, bad = 0;
+    Queries queries;
+    queries.first(p, w);
+    Offsets offsets;
+    offsets.request(p, w.b, 0, C);
+    const bool fits = span_of(p, w.b, lo, hi);
+    if (!fits && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.status, (uint32_t)kWitIndex);
+    if (lo == hi) {
+        write_empty(p, w, 0, dim, true);
+        return;
+    }
+    const uint32_t n = hi - lo;
+    int64_t* off = reinterpret_cast<int64_t*>(lds);                                        // [C]
+    unsigned long long* total = reinterpret_cast<unsigned long long*>(off + C);            // [rows][dim]
+    // the scores' sums beside the queries' digits; later the probabilities' digits in the same place
+    uint32_t* digits = reinterpret_cast<uint32_t*>(total + ((size_t)w.R * dim + 1) / 2 * 2);
+    uint64_t* sums = reinterpret_cast<uint64_t*>(digits + (size_t)5 * 16 * p.plan.dim64 * w.R);
+    if (threadIdx.x < 16) {
+        q_sum[threadIdx.x] = e_sum[threadIdx.x] = p_sum[threadIdx.x] = 0;
+        row_max[threadIdx.x] = INT32_MIN;
+    }
+    if (threadIdx.x == 0) over_any = 0;
+    for (uint32_t i = threadIdx.x; i < w.R * dim; i += 256) total[i] = 0;
+    __syncthreads();
+    queries.store(p, w, digits, q_sum, &over_any);
+    for (uint32_t c = 0; c < n; c += C) {
+        const uint32_t m = min(C, n - c);
+        if (c) offsets.early = false;
+        if (offsets.store(p, w.b, lo + c, m, (m + 63) / 64 * 64, off)) bad |= (uint32_t)kWitIndex;
+        __syncthreads();
+        score_products<VEC>(p, w, m, off, digits, over_any != 0, sums, C);
+        __syncthreads();
+        score_rows(p, w, lo + c, m, off, sums, C, q_sum, bad, [&](uint32_t r, int32_t mx) { row_max[r] = max(row_max[r], mx); });     // a row is one wave's
+        __syncthreads();
+    }
+    // the values' first step, under way during the softmax: its positions' offsets are there unless there were more chunks
+    const uint32_t blocks = p.plan.blocks, groups = p.plan.groups, apart = 4 / blocks, block = w.wave % blocks, s = w.wave / blocks;
+    ValueProducts<VEC, PP> products;
+    const bool one = n <= C;
+    if (one && 32 * block < dim && s < (n + 31) / 32) products.fetch(p, w, off, 32 * block, s);
+    {
+        // the threads of a row: as many as are left for each
+        uint32_t each = 256;
+        while (each * w.R > 256) each >>= 1;
+        const uint32_t r = threadIdx.x / each;
+        if (r < w.R) {
+            unsigned long long sum = exponentials(p, w.row0 + r, lo, threadIdx.x - r * each, each, n, row_max[r], bad);
+            for (uint32_t o = min(each, 64u) / 2; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+            if (threadIdx.x % min(each, 64u) == 0) atomicAdd(&e_sum[r], sum);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < w.R) {
+        if (e_sum[threadIdx.x] == 0) {
+            bad |= (uint32_t)kWitSum;
+            e_sum[threadIdx.x] = 1;
+        }
+        if (p.a.d_max) p.a.d_max[w.row0 + threadIdx.x] = row_max[threadIdx.x];
+        if (p.a.d_sum) p.a.d_sum[w.row0 + threadIdx.x] = (int32_t)e_sum[threadIdx.x];
+    }
+    __syncthreads();
+    for (uint32_t c = 0; c < n; c += C) {
+        const uint32_t m = min(C, n - c), halves = (m + 31) / 32;
+        if (!one) {
+            offsets.early = false;
+            offsets.store(p, w.b, lo + c, m, (m + 63) / 64 * 64, off);
+            __syncthreads();
+            if (32 * block < dim && s < halves) products.fetch(p, w, off, 32 * block, s);
+        }
+        for (uint32_t r = w.wave; r < w.R; r += 4) {
+            const unsigned long long mine = probabilities<PP>(p, w, r, lo + c, m, off, e_sum[r], true, digits);
+            if (w.lane == 0) p_sum[r] += mine;
+        }
+        __syncthreads();
+        for (uint32_t g = 0; g < groups; g++) {
+            const uint32_t e = 32 * (g * blocks + block);
+            if (e >= dim || s >= halves) break;
+            if (g) products.fetch(p, w, off, e, s);
+            products.clear();
+            products.run(p, w, off, digits, e, s, apart, halves);
+            products.add(w, total, dim, e);
+        }
+        __syncthreads();
+    }
+    for (uint32_t i = threadIdx.x; i < w.R * dim; i += 256) {
+        const uint32_t r = i / dim;
+        write_out(p, w.row0 + r, i - r * dim, (int64_t)(total[i] + (unsigned long long)kCacheOffset * p_sum[r]), bad);
+    }
+    if (bad) atomicOr(p.status, bad);
+}
+
+}  // namespace grape
+
+using namespace grape;
+
+extern "C" {
+
+size_t grape_wit_paged_attention_workspace(uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len) {
+    return token::attention_workspace(seqs, heads, cache_heads, dim, max_len);
+}
+
+int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_wit_cache* cache, grape_stream_t st) {
+    GRAPE_REQUIRE(initialised(), "grape_init has not been called");
+    GRAPE_REFUSED_IF(token::refuse_attention(args, cache));
+    if (args->seqs == 0) return GRAPE_OK;
+    AttendArgs p;
+    p.a = *args;
+    p.c = *cache;
+    grape_wit_attention_args& a = p.a;
+    token::attention_plan(a.seqs, a.heads, p.c.heads, p.c.dim, a.max_len, p.plan);
+    const token::AttentionPlan& pl = p.plan;
+    uint8_t* ws = (uint8_t*)a.d_workspace;
+    if (!a.d_scores) a.d_scores = (int32_t*)(ws + pl.at_scores);
+    if (!a.d_exp) a.d_exp = (int32_t*)(ws + pl.at_exp);
+    p.chunk_max = (int32_t*)(ws + pl.at_max);
+    p.sums = (unsigned long long*)(ws + pl.at_sum);
+    p.part = (int64_t*)(ws + pl.at_part);
+    p.page = token::fast_div(p.c.page_size);
+    p.qk = scaler(a.qk_scale);
+    p.out = scaler(a.out_scale);
+    hipStream_t s = as_stream(st);
+    const int rc = wit_status_word(&p.status, s);
+    if (rc) return rc;
+    auto aligned = [&](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+    const bool vec = p.c.dim % 4 == 0 && ((p.c.page_stride | p.c.token_stride | p.c.head_stride) & 3) == 0 && aligned(p.c.d_k) && aligned(p.c.d_v);
+    const int planes = a.prob_scale <= ((int64_t)1 << 22) ? 3 : 4;
+    if (pl.whole) {
+        const dim3 grid(p.c.heads * pl.tiles, a.seqs);
+        if (vec && planes == 3) wit_attend_whole_kernel<true, 3><<<grid, 256, pl.whole_lds, s>>>(p);
+        else if (vec) wit_attend_whole_kernel<true, 4><<<grid, 256, pl.whole_lds, s>>>(p);
+        else if (planes == 3) wit_attend_whole_kernel<false, 3><<<grid, 256, pl.whole_lds, s>>>(p);
+        else wit_attend_whole_kernel<false, 4><<<grid, 256, pl.whole_lds, s>>>(p);
+        GRAPE_LAUNCH_CHECK();
+        return GRAPE_OK;
+    }
+    const size_t score_lds = (size_t)pl.dim64 * 5 * 64 * pl.rows + (size_t)pl.score_chunk * 8 * (pl.rows + 1);
+    const size_t value_lds = std::max<size_t>((size_t)pl.value_chunk * (pl.rows * planes + 8), (size_t)pl.rows * pl.blocks * 32 * 8);
+    // the heads of one chunk are neighbours: they read the same tokens' lines of memory at the same time
+    const uint32_t head_tiles = p.c.heads * pl.tiles;
+    const dim3 score_grid(std::max(1u, pl.score_chunks) * head_tiles, a.seqs), value_grid(std::max(1u, pl.value_chunks) * head_tiles * pl.groups, a.seqs);
+    if (vec) wit_attend_scores_kernel<true><<<score_grid, 256, score_lds, s>>>(p);
+    else wit_attend_scores_kernel<false><<<score_grid, 256, score_lds, s>>>(p);
+    GRAPE_LAUNCH_CHECK();
+    if (a.max_len) {
+        wit_attend_exp_kernel<<<dim3(pl.exp_chunks, a.heads, a.seqs), kBlock, 0, s>>>(p);
+        GRAPE_LAUNCH_CHECK();
+    }
+    if (vec && planes == 3) wit_attend_values_kernel<true, 3><<<value_grid, 256, value_lds, s>>>(p);
+    else if (vec) wit_attend_values_kernel<true, 4><<<value_grid, 256, value_lds, s>>>(p);
+    else if (planes == 3) wit_attend_values_kernel<false, 3><<<value_grid, 256, value_lds, s>>>(p);
+    else wit_attend_values_kernel<false, 4><<<value_grid, 256, value_lds, s>>>(p);
+    GRAPE_LAUNCH_CHECK();
+    if (pl.value_chunks > 1) {
+        wit_attend_join_kernel<<<dim3(pl.dim64, a.heads, a.seqs), kJoinThreads, 0, s>>>(p);
+        GRAPE_LAUNCH_CHECK();
+    }
+    return GRAPE_OK;
+}
+
+}  // extern "C"

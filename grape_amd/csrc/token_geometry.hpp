@@ -101,10 +101,13 @@ struct AttentionPlan {
     uint32_t exp_chunk, exp_chunks;
     uint32_t blocks, groups;           // blocks of 32 elements of a values workgroup, workgroups of a head's elements
     uint32_t value_chunk, value_chunks;
+    bool whole;                        // one launch, a workgroup for all positions
+    size_t whole_lds;
     size_t at_scores, at_exp, at_max, at_sum, at_part, bytes;      // offsets in the workspace
 };
 constexpr uint32_t kTokenLds = 60 * 1024;      // of a workgroup
 constexpr uint32_t kWorkgroups = 4096;
+constexpr uint32_t kWholeChunk = 256;         // positions that a workgroup of the one launch takes at a time
 
 inline uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
 
@@ -146,6 +149,10 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
     p.value_chunks = ceil_div(max_len, p.value_chunk);
     // a launch's first axis, in threads
     if ((uint64_t)cache_heads * p.tiles * std::max<uint64_t>(p.score_chunks, (uint64_t)p.value_chunks * p.groups) >= (uint64_t)1 << 23) return false;
+    // offsets, 64-bit sums of the output, and the queries' digits with the scores' sums or the probabilities' digits
+    const size_t one = (size_t)5 * 64 * p.dim64 * p.rows + (size_t)8 * kWholeChunk * p.rows, two = (size_t)4 * kWholeChunk * p.rows;
+    p.whole_lds = 8 * kWholeChunk + ((size_t)p.rows * dim + 1) / 2 * 16 + (one > two ? one : two);
+    p.whole = p.whole_lds <= kTokenLds && (max_len <= kWholeChunk);
     const size_t row = (size_t)rows_all * max_len * 4;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     p.at_scores = 0;
@@ -153,7 +160,7 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
     p.at_max = p.at_exp + up(row);
     p.at_sum = p.at_max + up((size_t)rows_all * p.score_chunks * 4);
     p.at_part = p.at_sum + up((size_t)rows_all * p.exp_chunks * 8);
-    p.bytes = p.at_part + (p.value_chunks > 1 ? (size_t)rows_all * p.value_chunks * dim * 8 : 0);
+    p.bytes = p.whole ? p.at_max : p.at_part + (p.value_chunks > 1 ? (size_t)rows_all * p.value_chunks * dim * 8 : 0);
     return true;
 }
 

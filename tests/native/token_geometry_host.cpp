@@ -24,7 +24,7 @@ int plan_of(uint32_t s, uint32_t h, uint32_t hk, uint32_t d, uint32_t n, uint64_
     token::AttentionPlan p;
     if (!token::attention_plan(s, h, hk, d, n, p)) return 0;
     const uint64_t v[] = {p.dim64, p.rows, p.tiles, p.score_chunk, p.score_chunks, p.exp_chunk, p.exp_chunks, p.blocks, p.groups, p.value_chunk, p.value_chunks,
-                          p.at_scores, p.at_exp, p.at_max, p.at_sum, p.at_part, p.bytes};
+                          p.at_scores, p.at_exp, p.at_max, p.at_sum, p.at_part, p.bytes, p.whole, p.whole_lds};
     std::memcpy(o, v, sizeof v);
     return 1;
 }

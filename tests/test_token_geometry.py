@@ -152,13 +152,13 @@ def test_division_by_a_page_size(lib):
 
 def test_plans_cover_every_position_within_their_limits(lib):
     rng = np.random.default_rng(3)
-    names = "dim64 rows tiles score_chunk score_chunks exp_chunk exp_chunks blocks groups value_chunk value_chunks at_scores at_exp at_max at_sum at_part bytes".split()
+    names = "dim64 rows tiles score_chunk score_chunks exp_chunk exp_chunks blocks groups value_chunk value_chunks at_scores at_exp at_max at_sum at_part bytes whole whole_lds".split()
     out = (ctypes.c_uint64 * len(names))()
     sizes = [(1, 32, 8, 128, 37), (1, 1, 1, 8192, 1 << 20), (64, 32, 8, 128, 2048), (1, 64, 1, 64, 131072), (65535, 1, 1, 1, 1), (1, 1, 1, 1, 0), (3, 48, 3, 192, 5000)]
     for _ in range(2000):
         hk = int(rng.integers(1, 20))
         sizes.append((int(2 ** rng.uniform(0, 12)), hk * int(2 ** rng.uniform(0, 6)), hk, int(2 ** rng.uniform(0, 13)), int(2 ** rng.uniform(0, 22))))
-    taken = 0
+    taken = split = 0
     for s, h, hk, d, n in sizes:
         if not lib.plan_of(s, h, hk, d, n, out):
             continue
@@ -174,10 +174,16 @@ def test_plans_cover_every_position_within_their_limits(lib):
         assert hk * p["tiles"] * max(p["score_chunks"], p["value_chunks"] * p["groups"]) * 256 < 1 << 31
         rows = s * h
         need = [rows * n * 4, rows * n * 4, rows * p["score_chunks"] * 4, rows * p["exp_chunks"] * 8, rows * p["value_chunks"] * d * 8 if p["value_chunks"] > 1 else 0]
+        if p["whole"]:
+            assert p["bytes"] >= 2 * rows * n * 4 and p["at_exp"] >= rows * n * 4
+            assert 61440 >= p["whole_lds"] >= 8 * 256 + 8 * p["rows"] * d + p["rows"] * max(5 * 64 * p["dim64"] + 8 * 256, 4 * 256)
+            assert lib.workspace(s, h, hk, d, n) == p["bytes"]
+            continue
+        split += 1
         at = [p[x] for x in ("at_scores", "at_exp", "at_max", "at_sum", "at_part", "bytes")]
         assert at[0] == 0 and all(x % 16 == 0 for x in at[:5]) and all(b - a >= k for a, b, k in zip(at, at[1:], need))
         assert lib.workspace(s, h, hk, d, n) == p["bytes"]
-    assert taken > 1000
+    assert taken > 1000 and split > 300
 
 
 def test_workspace_sizes(lib):
