@@ -155,21 +155,22 @@ struct Queries {
     }
 };
 
-// Products of the queries with n keys, as 64-bit sums [row][stride] in LDS (of the keys less their offset).  A wave takes 16
+// Products of the queries with n keys (less their offset): sink(row, position, whether there is one, 64-bit sum), called by all
+// lanes of a wave together, 16 neighbouring ones for one row.  A wave takes 16
 // positions: lane l reads those elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16 that make up its operand of step s
 // (any order of a step's elements will do, as long as the queries' digits have the same), whole lines among the lanes.
-template <bool VEC>
-__device__ __forceinline__ void score_products(const AttendArgs& p, const Tile& w, uint32_t n, const int64_t* off, const uint32_t* digits, bool over,
-                                               uint64_t* sums, uint32_t stride) {
+template <bool VEC, class F>
+__device__ __forceinline__ void score_products(const AttendArgs& p, const Tile& w, uint32_t n, const int64_t* off, const uint32_t* digits, bool over, bool apart, F sink) {
     const uint32_t steps = p.plan.dim64, R = w.R, row = w.row(), dim = p.c.dim;
     const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
-    for (uint32_t at = 16 * w.wave; at < n; at += 64) {
+    // the waves take different positions, or (apart) different steps of the same ones
+    for (uint32_t at = apart ? 0 : 16 * w.wave; at < n; at += apart ? 16 : 64) {
         const int32_t* k = keys + max(off[min(at + w.col, n - 1)], (int64_t)0);
         v4i_t acc[8];
 #pragma unroll
         for (int g = 0; g < 8; g++) acc[g] = v4i_t{0, 0, 0, 0};
         // two steps at a time: their keys are requested together, and other waves multiply meanwhile
-        for (uint32_t s = 0; s < steps; s += 2) {
+        for (uint32_t s = apart ? 2 * w.wave : 0; s < steps; s += apart ? 8 : 2) {
             v4i_t x[8];
 #pragma unroll
             for (uint32_t c = 0; c < 4; c++) x[c] = load4<VEC>(k, 64 * s + 16 * c + 4 * w.kg, dim);
@@ -203,22 +204,19 @@ __device__ __forceinline__ void score_products(const AttendArgs& p, const Tile& 
                 }
             }
         }
-        if (at + w.col < n) {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-                const uint32_t r = 4 * i + w.kg;
-                if (4 * i < R && r < R) {
-                    uint64_t y = 0;
+        for (uint32_t i = 0; i < 4; i++) {
+            if (4 * i >= R) break;
+            const uint32_t r = 4 * i + w.kg;
+            uint64_t y = 0;
 #pragma unroll
-                    for (int g = 7; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[g][i];
-                    sums[r * stride + at + w.col] = y;
-                }
-            }
+            for (int g = 7; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[g][i];
+            sink(r, at + w.col, r < R && at + w.col < n, y);
         }
     }
 }
 
-// Those sums rescaled and written; the largest score of each row goes to largest(r, max).
+// Such sums, [row][stride] in LDS, rescaled and written; the largest score of each row goes to largest(r, max).
 template <class F>
 __device__ __forceinline__ void score_rows(const AttendArgs& p, const Tile& w, uint32_t t0, uint32_t n, const int64_t* off, const uint64_t* sums, uint32_t stride,
                                            const unsigned long long* q_sum, uint32_t& bad, F largest) {
@@ -280,11 +278,25 @@ __device__ __forceinline__ uint32_t probability(uint32_t e, uint64_t scale, uint
     return (uint32_t)q;
 }
 
-// Probabilities of n positions of row r from their exponentials, written if `write`, and their digits in LDS: [step of 32][plane]
-// [lane group][row], operands of 8 positions each, zero up to a whole number of 64 positions and for pages outside the cache.
-// A wave a row; returns the sum of the probabilities that the values are multiplied with.
-constexpr uint32_t kProbAhead = 2;   // four positions each under way a lane
+// 2 * scale * e - sum * (2 * prob - 1), its low 32 bits
+__device__ __forceinline__ int32_t lookup_query(uint32_t e, int64_t scale, uint64_t sum, uint32_t prob) {
+    return (int32_t)((uint64_t)e * 2 * (uint64_t)scale - sum * (2 * (uint64_t)prob - 1));
+}
+
+// Digits of four positions' probabilities in LDS: [step of 32][plane][lane group][row], operands of 8 positions each.
 template <int PP>                    // planes of the probabilities
+__device__ __forceinline__ void store_probabilities(const uint32_t pr[4], uint32_t quad, uint32_t r, uint32_t R, uint32_t* digits) {
+    uint32_t pl[4];
+    transpose4(digits_of((int32_t)pr[0]), digits_of((int32_t)pr[1]), digits_of((int32_t)pr[2]), digits_of((int32_t)pr[3]), pl);
+    uint32_t* out = digits + ((((quad >> 3) * PP * 4 + ((quad >> 1) & 3u)) * R + r) << 1) + (quad & 1u);
+#pragma unroll
+    for (int k = 0; k < PP; k++) out[k * 8 * R] = pl[k];
+}
+
+// Probabilities of n positions of row r from their exponentials, written if `write`, and their digits in LDS, zero up to a whole
+// number of 64 positions and for pages outside the cache.  A wave a row; returns the sum of the probabilities that the values are multiplied with.
+constexpr uint32_t kProbAhead = 2;   // four positions each under way a lane
+template <int PP>
 __device__ __forceinline__ unsigned long long probabilities(const AttendArgs& p, const Tile& w, uint32_t r, uint32_t t0, uint32_t n, const int64_t* off,
                                                             unsigned long long sum, bool write, uint32_t* digits) {
     const size_t o = (w.row0 + r) * p.a.max_len + t0;
@@ -304,27 +316,23 @@ __device__ __forceinline__ unsigned long long probabilities(const AttendArgs& p,
         for (uint32_t a = 0; a < kProbAhead; a++) {
             const uint32_t quad = first + 64 * a;
             if (quad >= quads) break;
-            uint32_t d[4], pl[4];
+            uint32_t pr[4];
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
                 const uint32_t i = 4 * quad + j;
-                uint32_t pr = 0;
+                pr[j] = 0;
                 if (i < n) {
                     const uint32_t ev = ex[a][j] < 0 ? 0 : (uint32_t)ex[a][j];
-                    pr = probability(ev, (uint64_t)p.a.prob_scale, sum, inv);
+                    pr[j] = probability(ev, (uint64_t)p.a.prob_scale, sum, inv);
                     if (write) {
-                        if (p.a.d_prob) p.a.d_prob[o + i] = (int32_t)pr;
-                        if (p.a.d_query) p.a.d_query[o + i] = (int32_t)((uint64_t)ev * 2 * (uint64_t)p.a.prob_scale - sum * (2 * (uint64_t)pr - 1));
+                        if (p.a.d_prob) p.a.d_prob[o + i] = (int32_t)pr[j];
+                        if (p.a.d_query) p.a.d_query[o + i] = lookup_query(ev, p.a.prob_scale, sum, pr[j]);
                     }
-                    if (off[i] < 0) pr = 0;
+                    if (off[i] < 0) pr[j] = 0;
                 }
-                mine += pr;
-                d[j] = digits_of((int32_t)pr);
+                mine += pr[j];
             }
-            transpose4(d[0], d[1], d[2], d[3], pl);
-            uint32_t* out = digits + ((((quad >> 3) * PP * 4 + ((quad >> 1) & 3u)) * w.R + r) << 1) + (quad & 1u);
-#pragma unroll
-            for (int k = 0; k < PP; k++) out[k * 8 * w.R] = pl[k];
+            store_probabilities<PP>(pr, quad, r, w.R, digits);
         }
     }
 #pragma unroll
@@ -444,10 +452,18 @@ __global__ void __launch_bounds__(256, 4) wit_attend_scores_kernel(AttendArgs p)
     int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)5 * 16 * p.plan.dim64 * p.plan.rows);
     uint64_t* sums = reinterpret_cast<uint64_t*>(off + p.plan.score_chunk);
     if (offsets.store(p, w.b, t0, n, n, off)) bad |= (uint32_t)kWitIndex;
+    const bool apart = p.plan.score_apart;
+    if (apart)
+        for (uint32_t i = threadIdx.x; i < w.R * p.plan.score_chunk; i += 256) sums[i] = 0;
     __syncthreads();
     queries.store(p, w, lds, q_sum, &over_any);
     __syncthreads();
-    score_products<VEC>(p, w, n, off, lds, over_any != 0, sums, p.plan.score_chunk);
+    score_products<VEC>(p, w, n, off, lds, over_any != 0, apart, [&](uint32_t r, uint32_t i, bool there, uint64_t y) {
+        if (!there) return;
+        uint64_t* sum = &sums[r * p.plan.score_chunk + i];
+        if (apart) atomicAdd(reinterpret_cast<unsigned long long*>(sum), (unsigned long long)y);
+        else *sum = y;
+    });
     __syncthreads();
     score_rows(p, w, t0, n, off, sums, p.plan.score_chunk, q_sum, bad,
                [&](uint32_t r, int32_t mx) { p.chunk_max[(w.row0 + r) * p.plan.score_chunks + chunk] = mx; });
@@ -573,14 +589,15 @@ __global__ void __launch_bounds__(kJoinThreads) wit_attend_join_kernel(AttendArg
     if (bad) atomicOr(p.status, bad);
 }
 
-// ---- the same in one launch, a workgroup for all positions of its query heads
+// ---- the same in one launch, a workgroup for all positions of its query heads (at most kWholeMost): what goes from step to step
+// stays in LDS and registers, and the latencies of the loads that depend on each other are what is left.
 template <bool VEC, int PP>
 __global__ void __launch_bounds__(256, 3) wit_attend_whole_kernel(AttendArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ unsigned long long q_sum[16], e_sum[16], p_sum[16];
     __shared__ int32_t row_max[16];
     __shared__ uint32_t over_any;
-    constexpr uint32_t C = token::kWholeChunk;
+    constexpr uint32_t C = token::kWholeMost;
     const Tile w(p, blockIdx.y, blockIdx.x);
     const uint32_t dim = p.c.dim;
     uint32_t lo, hi, bad = 0;
@@ -597,9 +614,8 @@ __global__ void __launch_bounds__(256, 3) wit_attend_whole_kernel(AttendArgs p) 
     const uint32_t n = hi - lo;
     int64_t* off = reinterpret_cast<int64_t*>(lds);                                        // [C]
     unsigned long long* total = reinterpret_cast<unsigned long long*>(off + C);            // [rows][dim]
-    // the scores' sums beside the queries' digits; later the probabilities' digits in the same place
-    uint32_t* digits = reinterpret_cast<uint32_t*>(total + ((size_t)w.R * dim + 1) / 2 * 2);
-    uint64_t* sums = reinterpret_cast<uint64_t*>(digits + (size_t)5 * 16 * p.plan.dim64 * w.R);
+    int32_t* scores = reinterpret_cast<int32_t*>(total + ((size_t)w.R * dim + 1) / 2 * 2);  // [rows][C]
+    uint32_t* digits = reinterpret_cast<uint32_t*>(scores + w.R * C);                       // of the queries, then of the probabilities
     if (threadIdx.x < 16) {
         q_sum[threadIdx.x] = e_sum[threadIdx.x] = p_sum[threadIdx.x] = 0;
         row_max[threadIdx.x] = INT32_MIN;
@@ -607,69 +623,114 @@ __global__ void __launch_bounds__(256, 3) wit_attend_whole_kernel(AttendArgs p) 
     if (threadIdx.x == 0) over_any = 0;
     for (uint32_t i = threadIdx.x; i < w.R * dim; i += 256) total[i] = 0;
     __syncthreads();
+    if (offsets.store(p, w.b, lo, n, (n + 63) / 64 * 64, off)) bad |= (uint32_t)kWitIndex;
     queries.store(p, w, digits, q_sum, &over_any);
-    for (uint32_t c = 0; c < n; c += C) {
-        const uint32_t m = min(C, n - c);
-        if (c) offsets.early = false;
-        if (offsets.store(p, w.b, lo + c, m, (m + 63) / 64 * 64, off)) bad |= (uint32_t)kWitIndex;
-        __syncthreads();
-        score_products<VEC>(p, w, m, off, digits, over_any != 0, sums, C);
-        __syncthreads();
-        score_rows(p, w, lo + c, m, off, sums, C, q_sum, bad, [&](uint32_t r, int32_t mx) { row_max[r] = max(row_max[r], mx); });     // a row is one wave's
-        __syncthreads();
-    }
-    // the values' first step, under way during the softmax: its positions' offsets are there unless there were more chunks
-    const uint32_t blocks = p.plan.blocks, groups = p.plan.groups, apart = 4 / blocks, block = w.wave % blocks, s = w.wave / blocks;
+    __syncthreads();
+    score_products<VEC>(p, w, n, off, digits, over_any != 0, false, [&](uint32_t r, uint32_t i, bool there, uint64_t y) {
+        int32_t q = INT32_MIN, rem;
+        if (there) {
+            p.qk.apply(off[i] < 0 ? 0 : (int64_t)(y + (uint64_t)kCacheOffset * q_sum[r]), q, rem, bad);
+            const size_t o = (w.row0 + r) * p.a.max_len + lo + i;
+            if (p.a.d_scores) p.a.d_scores[o] = q;
+            if (p.a.d_scores_rem) p.a.d_scores_rem[o] = rem;
+            scores[r * C + i] = q;
+        }
+#pragma unroll
+        for (int d = 8; d >= 1; d >>= 1) q = max(q, __shfl_xor(q, d, 64));
+        if (w.col == 0 && r < w.R) atomicMax(&row_max[r], q);
+    });
+    // the values' first step is under way during the softmax
+    const uint32_t blocks = p.plan.blocks, apart = 4 / blocks, block = w.wave % blocks, s = w.wave / blocks, halves = (n + 31) / 32;
     ValueProducts<VEC, PP> products;
-    const bool one = n <= C;
-    if (one && 32 * block < dim && s < (n + 31) / 32) products.fetch(p, w, off, 32 * block, s);
-    {
-        // the threads of a row: as many as are left for each
-        uint32_t each = 256;
-        while (each * w.R > 256) each >>= 1;
-        const uint32_t r = threadIdx.x / each;
-        if (r < w.R) {
-            unsigned long long sum = exponentials(p, w.row0 + r, lo, threadIdx.x - r * each, each, n, row_max[r], bad);
-            for (uint32_t o = min(each, 64u) / 2; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-            if (threadIdx.x % min(each, 64u) == 0) atomicAdd(&e_sum[r], sum);
+    if (32 * block < dim && s < halves) products.fetch(p, w, off, 32 * block, s);
+    __syncthreads();
+    // 256 / 2^k threads a row, four positions each at a time; with 16 rows of 256 positions that is four times
+    uint32_t each = 256;
+    while (each * w.R > 256) each >>= 1;
+    const uint32_t r = threadIdx.x / each, quads = (n + 63) / 64 * 16, from = threadIdx.x - r * each;
+    const size_t o = (w.row0 + min(r, w.R - 1)) * p.a.max_len + lo;
+    uint32_t e[4][4];
+    if (r < w.R) {
+        const int32_t mx = row_max[r];
+        unsigned long long sum = 0;
+#pragma unroll
+        for (uint32_t a = 0; a < 4; a++) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t i = 4 * (from + a * each) + j;
+                e[a][j] = 0;
+                if (i < n) {
+                    const int64_t d = (int64_t)scores[r * C + i] - mx, idx = d + (((int64_t)1 << p.a.bit_shift) - 1);
+                    const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
+                    if (!ok) bad |= (uint32_t)kWitIndex;
+                    e[a][j] = (uint32_t)p.a.d_exp_table[ok ? idx : 0];
+                    if (p.a.d_shifted) p.a.d_shifted[o + i] = (int32_t)d;
+                }
+            }
         }
+#pragma unroll
+        for (uint32_t a = 0; a < 4; a++) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t i = 4 * (from + a * each) + j;
+                if (i < n && p.a.d_exp) p.a.d_exp[o + i] = (int32_t)e[a][j];
+                if ((int32_t)e[a][j] < 0) {
+                    bad |= (uint32_t)kWitSum;
+                    e[a][j] = 0;
+                }
+                sum += e[a][j];
+            }
+        }
+        for (uint32_t k = min(each, 64u) / 2; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, 64);
+        if (threadIdx.x % min(each, 64u) == 0) atomicAdd(&e_sum[r], sum);
     }
     __syncthreads();
-    if (threadIdx.x < w.R) {
-        if (e_sum[threadIdx.x] == 0) {
+    if (r < w.R) {
+        unsigned long long sum = e_sum[r], mine = 0;
+        if (sum == 0) {
             bad |= (uint32_t)kWitSum;
-            e_sum[threadIdx.x] = 1;
+            sum = 1;
         }
-        if (p.a.d_max) p.a.d_max[w.row0 + threadIdx.x] = row_max[threadIdx.x];
-        if (p.a.d_sum) p.a.d_sum[w.row0 + threadIdx.x] = (int32_t)e_sum[threadIdx.x];
+        if (from == 0) {
+            if (p.a.d_max) p.a.d_max[w.row0 + r] = row_max[r];
+            if (p.a.d_sum) p.a.d_sum[w.row0 + r] = (int32_t)sum;
+        }
+        const double inv = 1.0 / (double)sum;
+#pragma unroll
+        for (uint32_t a = 0; a < 4; a++) {
+            const uint32_t quad = from + a * each;
+            if (quad >= quads) break;
+            uint32_t pr[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t i = 4 * quad + j;
+                pr[j] = 0;
+                if (i < n) {
+                    pr[j] = probability(e[a][j], (uint64_t)p.a.prob_scale, sum, inv);
+                    if (p.a.d_prob) p.a.d_prob[o + i] = (int32_t)pr[j];
+                    if (p.a.d_query) p.a.d_query[o + i] = lookup_query(e[a][j], p.a.prob_scale, sum, pr[j]);
+                    if (off[i] < 0) pr[j] = 0;                     // a page outside the cache
+                }
+                mine += pr[j];
+            }
+            store_probabilities<PP>(pr, quad, r, w.R, digits);
+        }
+        for (uint32_t k = min(each, 64u) / 2; k >= 1; k >>= 1) mine += __shfl_xor(mine, k, 64);
+        if (threadIdx.x % min(each, 64u) == 0) atomicAdd(&p_sum[r], mine);
     }
     __syncthreads();
-    for (uint32_t c = 0; c < n; c += C) {
-        const uint32_t m = min(C, n - c), halves = (m + 31) / 32;
-        if (!one) {
-            offsets.early = false;
-            offsets.store(p, w.b, lo + c, m, (m + 63) / 64 * 64, off);
-            __syncthreads();
-            if (32 * block < dim && s < halves) products.fetch(p, w, off, 32 * block, s);
-        }
-        for (uint32_t r = w.wave; r < w.R; r += 4) {
-            const unsigned long long mine = probabilities<PP>(p, w, r, lo + c, m, off, e_sum[r], true, digits);
-            if (w.lane == 0) p_sum[r] += mine;
-        }
-        __syncthreads();
-        for (uint32_t g = 0; g < groups; g++) {
-            const uint32_t e = 32 * (g * blocks + block);
-            if (e >= dim || s >= halves) break;
-            if (g) products.fetch(p, w, off, e, s);
-            products.clear();
-            products.run(p, w, off, digits, e, s, apart, halves);
-            products.add(w, total, dim, e);
-        }
-        __syncthreads();
+    for (uint32_t g = 0; g < p.plan.groups; g++) {
+        const uint32_t el = 32 * (g * blocks + block);
+        if (el >= dim || s >= halves) break;
+        if (g) products.fetch(p, w, off, el, s);
+        products.clear();
+        products.run(p, w, off, digits, el, s, apart, halves);
+        products.add(w, total, dim, el);
     }
+    __syncthreads();
     for (uint32_t i = threadIdx.x; i < w.R * dim; i += 256) {
-        const uint32_t r = i / dim;
-        write_out(p, w.row0 + r, i - r * dim, (int64_t)(total[i] + (unsigned long long)kCacheOffset * p_sum[r]), bad);
+        const uint32_t row = i / dim;
+        write_out(p, w.row0 + row, i - row * dim, (int64_t)(total[i] + (unsigned long long)kCacheOffset * p_sum[row]), bad);
     }
     if (bad) atomicOr(p.status, bad);
 }
@@ -695,8 +756,8 @@ int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_
     token::attention_plan(a.seqs, a.heads, p.c.heads, p.c.dim, a.max_len, p.plan);
     const token::AttentionPlan& pl = p.plan;
     uint8_t* ws = (uint8_t*)a.d_workspace;
-    if (!a.d_scores) a.d_scores = (int32_t*)(ws + pl.at_scores);
-    if (!a.d_exp) a.d_exp = (int32_t*)(ws + pl.at_exp);
+    if (!pl.whole && !a.d_scores) a.d_scores = (int32_t*)(ws + pl.at_scores);
+    if (!pl.whole && !a.d_exp) a.d_exp = (int32_t*)(ws + pl.at_exp);
     p.chunk_max = (int32_t*)(ws + pl.at_max);
     p.sums = (unsigned long long*)(ws + pl.at_sum);
     p.part = (int64_t*)(ws + pl.at_part);

@@ -97,6 +97,7 @@ inline const char* refuse_append(const grape_wit_rope_append_args* a, const grap
 struct AttentionPlan {
     uint32_t dim64;                    // blocks of 64 elements of a head
     uint32_t rows, tiles;              // query heads of a workgroup, workgroups of a cache head
+    bool score_apart;
     uint32_t score_chunk, score_chunks;
     uint32_t exp_chunk, exp_chunks;
     uint32_t blocks, groups;           // blocks of 32 elements of a values workgroup, workgroups of a head's elements
@@ -107,7 +108,7 @@ struct AttentionPlan {
 };
 constexpr uint32_t kTokenLds = 60 * 1024;      // of a workgroup
 constexpr uint32_t kWorkgroups = 4096;
-constexpr uint32_t kWholeChunk = 256;         // positions that a workgroup of the one launch takes at a time
+constexpr uint32_t kWholeMost = 256;          // positions of the one launch
 
 inline uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
 
@@ -134,7 +135,10 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
     uint32_t score_most = left / (8 * p.rows + 8) / 64 * 64;
     if (score_most > 4096 / p.rows) score_most = 4096 / p.rows / 64 * 64;
     if (score_most < 64) return false;
-    p.score_chunk = chunk(beside, 64, score_most, kWorkgroups);
+    // with heads of 512 elements and more the waves share the elements of 16 positions instead of the positions: one sequence
+    // of 500 with a head of 4096 is 32 workgroups then and not 8
+    p.score_apart = p.dim64 >= 8;
+    p.score_chunk = chunk(beside, p.score_apart ? 16 : 64, score_most, kWorkgroups);
     p.score_chunks = ceil_div(max_len, p.score_chunk);
     p.exp_chunk = chunk(rows_all, 1024, (uint32_t)1 << 20, kWorkgroups / 2);
     p.exp_chunks = ceil_div(max_len, p.exp_chunk);
@@ -149,10 +153,10 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
     p.value_chunks = ceil_div(max_len, p.value_chunk);
     // a launch's first axis, in threads
     if ((uint64_t)cache_heads * p.tiles * std::max<uint64_t>(p.score_chunks, (uint64_t)p.value_chunks * p.groups) >= (uint64_t)1 << 23) return false;
-    // offsets, 64-bit sums of the output, and the queries' digits with the scores' sums or the probabilities' digits
-    const size_t one = (size_t)5 * 64 * p.dim64 * p.rows + (size_t)8 * kWholeChunk * p.rows, two = (size_t)4 * kWholeChunk * p.rows;
-    p.whole_lds = 8 * kWholeChunk + ((size_t)p.rows * dim + 1) / 2 * 16 + (one > two ? one : two);
-    p.whole = p.whole_lds <= kTokenLds && (max_len <= kWholeChunk);
+    // offsets, 64-bit sums of the output, scores, and the queries' digits or the probabilities' ones
+    const size_t one = (size_t)5 * 64 * p.dim64 * p.rows, two = (size_t)4 * kWholeMost * p.rows;
+    p.whole_lds = 8 * kWholeMost + ((size_t)p.rows * dim + 1) / 2 * 16 + (size_t)4 * kWholeMost * p.rows + (one > two ? one : two);
+    p.whole = p.whole_lds <= kTokenLds && max_len <= kWholeMost && dim <= 256;
     const size_t row = (size_t)rows_all * max_len * 4;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     p.at_scores = 0;
@@ -160,7 +164,7 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
     p.at_max = p.at_exp + up(row);
     p.at_sum = p.at_max + up((size_t)rows_all * p.score_chunks * 4);
     p.at_part = p.at_sum + up((size_t)rows_all * p.exp_chunks * 8);
-    p.bytes = p.whole ? p.at_max : p.at_part + (p.value_chunks > 1 ? (size_t)rows_all * p.value_chunks * dim * 8 : 0);
+    p.bytes = p.whole ? 0 : p.at_part + (p.value_chunks > 1 ? (size_t)rows_all * p.value_chunks * dim * 8 : 0);
     return true;
 }
 
