@@ -35,7 +35,7 @@ __device__ __forceinline__ bool span_of(const AttendArgs& p, uint32_t b, uint32_
     return token::live_span(p.a.d_lens[b], p.a.d_first ? p.a.d_first[b] : 0, p.a.max_len, p.a.table_stride, p.c.page_size, lo, hi);
 }
 
-// The offsets of a chunk's positions t0 .. t0 + n, made by all 256 threads of a workgroup.  The first page of each thread is
+// The offsets of a chunk's positions t0 .. t0 + n, made by all threads of a workgroup.  The first page of each thread is
 // requested before the sequence's length is known where it does not depend on it, so that the two loads are under way together.
 struct Offsets {
     int32_t page = -1;
@@ -51,7 +51,7 @@ struct Offsets {
     }
     __device__ __forceinline__ bool store(const AttendArgs& p, uint32_t b, uint32_t t0, uint32_t n, uint32_t filled, int64_t* off) const {
         bool outside = false;
-        for (uint32_t i = threadIdx.x; i < filled; i += 256) {
+        for (uint32_t i = threadIdx.x; i < filled; i += blockDim.x) {
             int64_t o = -1;
             if (i < n) {
                 const int32_t pg = early && i == threadIdx.x ? page : load(p, b, t0 + i);
@@ -130,7 +130,7 @@ struct Queries {
     }
     __device__ __forceinline__ void store(const AttendArgs& p, const Tile& w, uint32_t* digits, unsigned long long* q_sum, uint32_t* over_any) {
         const uint32_t steps = p.plan.dim64;
-        for (uint32_t i = threadIdx.x; i < w.R * steps * 16; i += 256) {
+        for (uint32_t i = threadIdx.x; i < w.R * steps * 16; i += blockDim.x) {
             const uint32_t r = i / (steps * 16), quad = i - r * (steps * 16), s = quad >> 4, c = (quad >> 2) & 3u, g = quad & 3u;
             if (i != threadIdx.x) load(p, w, i);
             uint32_t d[4], pl[4], carry = 0;
@@ -159,18 +159,18 @@ struct Queries {
 // lanes of a wave together, 16 neighbouring ones for one row.  A wave takes 16
 // positions: lane l reads those elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16 that make up its operand of step s
 // (any order of a step's elements will do, as long as the queries' digits have the same), whole lines among the lanes.
-template <bool VEC, class F>
+template <bool VEC, uint32_t WAVES, class F>
 __device__ __forceinline__ void score_products(const AttendArgs& p, const Tile& w, uint32_t n, const int64_t* off, const uint32_t* digits, bool over, bool apart, F sink) {
     const uint32_t steps = p.plan.dim64, R = w.R, row = w.row(), dim = p.c.dim;
     const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
     // the waves take different positions, or (apart) different steps of the same ones
-    for (uint32_t at = apart ? 0 : 16 * w.wave; at < n; at += apart ? 16 : 64) {
+    for (uint32_t at = apart ? 0 : 16 * w.wave; at < n; at += apart ? 16 : 16 * WAVES) {
         const int32_t* k = keys + max(off[min(at + w.col, n - 1)], (int64_t)0);
         v4i_t acc[8];
 #pragma unroll
         for (int g = 0; g < 8; g++) acc[g] = v4i_t{0, 0, 0, 0};
         // two steps at a time: their keys are requested together, and other waves multiply meanwhile
-        for (uint32_t s = apart ? 2 * w.wave : 0; s < steps; s += apart ? 8 : 2) {
+        for (uint32_t s = apart ? 2 * w.wave : 0; s < steps; s += apart ? 2 * WAVES : 2) {
             v4i_t x[8];
 #pragma unroll
             for (uint32_t c = 0; c < 4; c++) x[c] = load4<VEC>(k, 64 * s + 16 * c + 4 * w.kg, dim);
@@ -413,7 +413,7 @@ __device__ __forceinline__ void write_out(const AttendArgs& p, size_t row, uint3
 
 // Rows with nothing to attend to: elements e0 .. e0 + width of the output, and the maximum and sum if `rows`.
 __device__ __forceinline__ void write_empty(const AttendArgs& p, const Tile& w, uint32_t e0, uint32_t width, bool rows) {
-    for (uint32_t i = threadIdx.x; i < w.R * width; i += 256) {
+    for (uint32_t i = threadIdx.x; i < w.R * width; i += blockDim.x) {
         const uint32_t r = i / width, e = e0 + i - r * width;
         if (e >= p.c.dim) continue;
         p.a.d_out[(w.row0 + r) * p.c.dim + e] = 0;
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(256, 4) wit_attend_scores_kernel(AttendArgs p)
     __syncthreads();
     queries.store(p, w, lds, q_sum, &over_any);
     __syncthreads();
-    score_products<VEC>(p, w, n, off, lds, over_any != 0, apart, [&](uint32_t r, uint32_t i, bool there, uint64_t y) {
+    score_products<VEC, 4>(p, w, n, off, lds, over_any != 0, apart, [&](uint32_t r, uint32_t i, bool there, uint64_t y) {
         if (!there) return;
         uint64_t* sum = &sums[r * p.plan.score_chunk + i];
         if (apart) atomicAdd(reinterpret_cast<unsigned long long*>(sum), (unsigned long long)y);
@@ -590,9 +590,11 @@ __global__ void __launch_bounds__(kJoinThreads) wit_attend_join_kernel(AttendArg
 }
 
 // ---- the same in one launch, a workgroup for all positions of its query heads (at most kWholeMost): what goes from step to step
-// stays in LDS and registers, and the latencies of the loads that depend on each other are what is left.
+// stays on chip.  A few positions leave nothing but latencies - of loads that depend on each other, and of instructions that run
+// once - so eight waves share the positions, and the softmax takes one position a thread in short loops.
+constexpr uint32_t kWholeWaves = 8, kWholeThreads = 64 * kWholeWaves;
 template <bool VEC, int PP>
-__global__ void __launch_bounds__(256, 3) wit_attend_whole_kernel(AttendArgs p) {
+__global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(AttendArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ unsigned long long q_sum[16], e_sum[16], p_sum[16];
     __shared__ int32_t row_max[16];
@@ -613,80 +615,82 @@ __global__ void __launch_bounds__(256, 3) wit_attend_whole_kernel(AttendArgs p) 
     }
     const uint32_t n = hi - lo;
     int64_t* off = reinterpret_cast<int64_t*>(lds);                                        // [C]
-    unsigned long long* total = reinterpret_cast<unsigned long long*>(off + C);            // [rows][dim]
-    int32_t* scores = reinterpret_cast<int32_t*>(total + ((size_t)w.R * dim + 1) / 2 * 2);  // [rows][C]
-    uint32_t* digits = reinterpret_cast<uint32_t*>(scores + w.R * C);                       // of the queries, then of the probabilities
+    unsigned long long* total = reinterpret_cast<unsigned long long*>(off + C);            // the scores' sums [rows][C], then the output's [rows][dim]
+    uint32_t* scores = reinterpret_cast<uint32_t*>(total + (size_t)w.R * max(dim, C));      // [rows][C], then the exponentials
+    uint32_t* digits = scores + w.R * C;                                                    // of the queries, then of the probabilities
     if (threadIdx.x < 16) {
         q_sum[threadIdx.x] = e_sum[threadIdx.x] = p_sum[threadIdx.x] = 0;
         row_max[threadIdx.x] = INT32_MIN;
     }
     if (threadIdx.x == 0) over_any = 0;
-    for (uint32_t i = threadIdx.x; i < w.R * dim; i += 256) total[i] = 0;
     __syncthreads();
-    if (offsets.store(p, w.b, lo, n, (n + 63) / 64 * 64, off)) bad |= (uint32_t)kWitIndex;
+    const uint32_t filled = (n + 31) / 32 * 32;
+    if (offsets.store(p, w.b, lo, n, filled, off)) bad |= (uint32_t)kWitIndex;
     queries.store(p, w, digits, q_sum, &over_any);
     __syncthreads();
-    score_products<VEC>(p, w, n, off, digits, over_any != 0, false, [&](uint32_t r, uint32_t i, bool there, uint64_t y) {
-        int32_t q = INT32_MIN, rem;
-        if (there) {
-            p.qk.apply(off[i] < 0 ? 0 : (int64_t)(y + (uint64_t)kCacheOffset * q_sum[r]), q, rem, bad);
-            const size_t o = (w.row0 + r) * p.a.max_len + lo + i;
-            if (p.a.d_scores) p.a.d_scores[o] = q;
-            if (p.a.d_scores_rem) p.a.d_scores_rem[o] = rem;
-            scores[r * C + i] = q;
-        }
-#pragma unroll
-        for (int d = 8; d >= 1; d >>= 1) q = max(q, __shfl_xor(q, d, 64));
-        if (w.col == 0 && r < w.R) atomicMax(&row_max[r], q);
+    score_products<VEC, kWholeWaves>(p, w, n, off, digits, over_any != 0, false, [&](uint32_t r, uint32_t i, bool there, uint64_t y) {
+        if (there) total[r * C + i] = y;
     });
     // the values' first step is under way during the softmax
-    const uint32_t blocks = p.plan.blocks, apart = 4 / blocks, block = w.wave % blocks, s = w.wave / blocks, halves = (n + 31) / 32;
+    const uint32_t blocks = p.plan.blocks, apart = kWholeWaves / blocks, block = w.wave % blocks, s = w.wave / blocks, halves = (n + 31) / 32;
     ValueProducts<VEC, PP> products;
     if (32 * block < dim && s < halves) products.fetch(p, w, off, 32 * block, s);
     __syncthreads();
-    // 256 / 2^k threads a row, four positions each at a time; with 16 rows of 256 positions that is four times
-    uint32_t each = 256;
-    while (each * w.R > 256) each >>= 1;
-    const uint32_t r = threadIdx.x / each, quads = (n + 63) / 64 * 16, from = threadIdx.x - r * each;
+    // as many threads a row as there are for each, a power of two
+    uint32_t each = kWholeThreads;
+    while (each * w.R > kWholeThreads) each >>= 1;
+    const uint32_t r = threadIdx.x / each, from = threadIdx.x - r * each, lanes = min(each, 64u);
+    const bool mine = r < w.R, leads = threadIdx.x % lanes == 0;
     const size_t o = (w.row0 + min(r, w.R - 1)) * p.a.max_len + lo;
-    uint32_t e[4][4];
-    if (r < w.R) {
-        const int32_t mx = row_max[r];
-        unsigned long long sum = 0;
-#pragma unroll
-        for (uint32_t a = 0; a < 4; a++) {
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t i = 4 * (from + a * each) + j;
-                e[a][j] = 0;
-                if (i < n) {
-                    const int64_t d = (int64_t)scores[r * C + i] - mx, idx = d + (((int64_t)1 << p.a.bit_shift) - 1);
-                    const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
-                    if (!ok) bad |= (uint32_t)kWitIndex;
-                    e[a][j] = (uint32_t)p.a.d_exp_table[ok ? idx : 0];
-                    if (p.a.d_shifted) p.a.d_shifted[o + i] = (int32_t)d;
-                }
-            }
+    if (mine) {
+        const uint64_t more = (uint64_t)kCacheOffset * q_sum[r];
+        int32_t mx = INT32_MIN;
+#pragma unroll 1
+        for (uint32_t i = from; i < n; i += each) {
+            int32_t q, rem;
+            p.qk.apply(off[i] < 0 ? 0 : (int64_t)(total[r * C + i] + more), q, rem, bad);          // a page outside the cache: zero
+            if (p.a.d_scores) p.a.d_scores[o + i] = q;
+            if (p.a.d_scores_rem) p.a.d_scores_rem[o + i] = rem;
+            scores[r * C + i] = (uint32_t)q;
+            mx = max(mx, q);
         }
-#pragma unroll
-        for (uint32_t a = 0; a < 4; a++) {
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t i = 4 * (from + a * each) + j;
-                if (i < n && p.a.d_exp) p.a.d_exp[o + i] = (int32_t)e[a][j];
-                if ((int32_t)e[a][j] < 0) {
-                    bad |= (uint32_t)kWitSum;
-                    e[a][j] = 0;
-                }
-                sum += e[a][j];
-            }
-        }
-        for (uint32_t k = min(each, 64u) / 2; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, 64);
-        if (threadIdx.x % min(each, 64u) == 0) atomicAdd(&e_sum[r], sum);
+        for (uint32_t k = lanes / 2; k >= 1; k >>= 1) mx = max(mx, __shfl_xor(mx, k, 64));
+        if (leads) atomicMax(&row_max[r], mx);
     }
     __syncthreads();
-    if (r < w.R) {
-        unsigned long long sum = e_sum[r], mine = 0;
+    for (uint32_t i = threadIdx.x; i < w.R * dim; i += kWholeThreads) total[i] = 0;
+    if (mine) {
+        const int32_t mx = row_max[r];
+        unsigned long long sum = 0;
+#pragma unroll 1
+        for (uint32_t first = from; first < n; first += 4 * each) {          // four gathers under way a thread
+            int32_t e[4];
+#pragma unroll
+            for (uint32_t a = 0; a < 4; a++) {
+                const uint32_t i = first + a * each;
+                const int64_t idx = (int64_t)(int32_t)scores[r * C + min(i, n - 1)] - mx + (((int64_t)1 << p.a.bit_shift) - 1);
+                const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
+                if (!ok) bad |= (uint32_t)kWitIndex;
+                e[a] = p.a.d_exp_table[ok ? idx : 0];
+            }
+#pragma unroll
+            for (uint32_t a = 0; a < 4; a++) {
+                const uint32_t i = first + a * each;
+                if (i >= n) break;
+                if (p.a.d_shifted) p.a.d_shifted[o + i] = (int32_t)((int64_t)(int32_t)scores[r * C + i] - mx);
+                if (p.a.d_exp) p.a.d_exp[o + i] = e[a];
+                if (e[a] < 0) bad |= (uint32_t)kWitSum;
+                e[a] = max(e[a], 0);
+                scores[r * C + i] = (uint32_t)e[a];
+                sum += (uint32_t)e[a];
+            }
+        }
+        for (uint32_t k = lanes / 2; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, 64);
+        if (leads) atomicAdd(&e_sum[r], sum);
+    }
+    __syncthreads();
+    if (mine) {
+        unsigned long long sum = e_sum[r], all = 0;
         if (sum == 0) {
             bad |= (uint32_t)kWitSum;
             sum = 1;
@@ -696,27 +700,24 @@ __global__ void __launch_bounds__(256, 3) wit_attend_whole_kernel(AttendArgs p) 
             if (p.a.d_sum) p.a.d_sum[w.row0 + r] = (int32_t)sum;
         }
         const double inv = 1.0 / (double)sum;
-#pragma unroll
-        for (uint32_t a = 0; a < 4; a++) {
-            const uint32_t quad = from + a * each;
-            if (quad >= quads) break;
-            uint32_t pr[4];
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t i = 4 * quad + j;
-                pr[j] = 0;
-                if (i < n) {
-                    pr[j] = probability(e[a][j], (uint64_t)p.a.prob_scale, sum, inv);
-                    if (p.a.d_prob) p.a.d_prob[o + i] = (int32_t)pr[j];
-                    if (p.a.d_query) p.a.d_query[o + i] = lookup_query(e[a][j], p.a.prob_scale, sum, pr[j]);
-                    if (off[i] < 0) pr[j] = 0;                     // a page outside the cache
-                }
-                mine += pr[j];
+#pragma unroll 1
+        for (uint32_t i = from; i < filled; i += each) {
+            uint32_t pr = 0;
+            if (i < n) {
+                const uint32_t e = scores[r * C + i];
+                pr = probability(e, (uint64_t)p.a.prob_scale, sum, inv);
+                if (p.a.d_prob) p.a.d_prob[o + i] = (int32_t)pr;
+                if (p.a.d_query) p.a.d_query[o + i] = lookup_query(e, p.a.prob_scale, sum, pr);
+                if (off[i] < 0) pr = 0;
             }
-            store_probabilities<PP>(pr, quad, r, w.R, digits);
+            all += pr;
+            const uint32_t d = digits_of((int32_t)pr);
+            uint8_t* out = reinterpret_cast<uint8_t*>(digits) + ((((i >> 5) * PP * 4 + ((i >> 3) & 3u)) * w.R + r) << 3) + (i & 7u);
+#pragma unroll
+            for (int k = 0; k < PP; k++) out[k * 32 * w.R] = (uint8_t)(d >> (8 * k));
         }
-        for (uint32_t k = min(each, 64u) / 2; k >= 1; k >>= 1) mine += __shfl_xor(mine, k, 64);
-        if (threadIdx.x % min(each, 64u) == 0) atomicAdd(&p_sum[r], mine);
+        for (uint32_t k = lanes / 2; k >= 1; k >>= 1) all += __shfl_xor(all, k, 64);
+        if (leads) atomicAdd(&p_sum[r], all);
     }
     __syncthreads();
     for (uint32_t g = 0; g < p.plan.groups; g++) {
@@ -728,7 +729,7 @@ __global__ void __launch_bounds__(256, 3) wit_attend_whole_kernel(AttendArgs p) 
         products.add(w, total, dim, el);
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < w.R * dim; i += 256) {
+    for (uint32_t i = threadIdx.x; i < w.R * dim; i += kWholeThreads) {
         const uint32_t row = i / dim;
         write_out(p, w.row0 + row, i - row * dim, (int64_t)(total[i] + (unsigned long long)kCacheOffset * p_sum[row]), bad);
     }
@@ -772,10 +773,10 @@ int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_
     const int planes = a.prob_scale <= ((int64_t)1 << 22) ? 3 : 4;
     if (pl.whole) {
         const dim3 grid(p.c.heads * pl.tiles, a.seqs);
-        if (vec && planes == 3) wit_attend_whole_kernel<true, 3><<<grid, 256, pl.whole_lds, s>>>(p);
-        else if (vec) wit_attend_whole_kernel<true, 4><<<grid, 256, pl.whole_lds, s>>>(p);
-        else if (planes == 3) wit_attend_whole_kernel<false, 3><<<grid, 256, pl.whole_lds, s>>>(p);
-        else wit_attend_whole_kernel<false, 4><<<grid, 256, pl.whole_lds, s>>>(p);
+        if (vec && planes == 3) wit_attend_whole_kernel<true, 3><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
+        else if (vec) wit_attend_whole_kernel<true, 4><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
+        else if (planes == 3) wit_attend_whole_kernel<false, 3><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
+        else wit_attend_whole_kernel<false, 4><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
         GRAPE_LAUNCH_CHECK();
         return GRAPE_OK;
     }

@@ -106,7 +106,8 @@ struct AttentionPlan {
     size_t whole_lds;
     size_t at_scores, at_exp, at_max, at_sum, at_part, bytes;      // offsets in the workspace
 };
-constexpr uint32_t kTokenLds = 60 * 1024;      // of a workgroup
+constexpr uint32_t kTokenLds = 60 * 1024;      // of a workgroup; of one that takes all positions:
+constexpr size_t kWholeLds = 72 * 1024;
 constexpr uint32_t kWorkgroups = 4096;
 constexpr uint32_t kWholeMost = 256;          // positions of the one launch
 
@@ -153,10 +154,10 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
     p.value_chunks = ceil_div(max_len, p.value_chunk);
     // a launch's first axis, in threads
     if ((uint64_t)cache_heads * p.tiles * std::max<uint64_t>(p.score_chunks, (uint64_t)p.value_chunks * p.groups) >= (uint64_t)1 << 23) return false;
-    // offsets, 64-bit sums of the output, scores, and the queries' digits or the probabilities' ones
+    // offsets, 64-bit sums of the scores and then of the output, scores, and the queries' digits or the probabilities' ones
     const size_t one = (size_t)5 * 64 * p.dim64 * p.rows, two = (size_t)4 * kWholeMost * p.rows;
-    p.whole_lds = 8 * kWholeMost + ((size_t)p.rows * dim + 1) / 2 * 16 + (size_t)4 * kWholeMost * p.rows + (one > two ? one : two);
-    p.whole = p.whole_lds <= kTokenLds && max_len <= kWholeMost && dim <= 256;
+    p.whole_lds = 8 * kWholeMost + (size_t)8 * p.rows * (dim > kWholeMost ? dim : kWholeMost) + (size_t)4 * kWholeMost * p.rows + (one > two ? one : two);
+    p.whole = p.whole_lds <= kWholeLds && max_len <= kWholeMost && dim <= 256;
     const size_t row = (size_t)rows_all * max_len * 4;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     p.at_scores = 0;

@@ -176,7 +176,7 @@ def test_plans_cover_every_position_within_their_limits(lib):
         need = [rows * n * 4, rows * n * 4, rows * p["score_chunks"] * 4, rows * p["exp_chunks"] * 8, rows * p["value_chunks"] * d * 8 if p["value_chunks"] > 1 else 0]
         if p["whole"]:
             assert p["bytes"] == 0 and n <= 256
-            assert 61440 >= p["whole_lds"] >= 8 * 256 + 8 * p["rows"] * d + 4 * 256 * p["rows"] + p["rows"] * max(5 * 64 * p["dim64"], 4 * 256)
+            assert 73728 >= p["whole_lds"] >= 8 * 256 + 8 * p["rows"] * max(d, 256) + 4 * 256 * p["rows"] + p["rows"] * max(5 * 64 * p["dim64"], 4 * 256)
             assert lib.workspace(s, h, hk, d, n) == p["bytes"]
             continue
         split += 1
