@@ -6,63 +6,138 @@
 namespace grape {
 
 // ------------------------------------------------------------------------------------------------
-// Rotation and append.  A unit is one pair of a rotated head or two elements that only move; a token's units are those of its
-// query heads, its key heads and its value heads.
+// Rotation and append.  A unit is W pairs of a rotated head or 2 W elements that only move; a token's units are those of its
+// query heads, its key heads and its value heads.  W = 4: a unit is two 16-byte loads and two to four 16-byte stores.  Bound by
+// memory; with few tokens by two loads that depend on each other, the position and its row of the tables.
+//
+// Of several tokens with one slot the last one has to stay, whatever the order in which they are written: a workgroup looks for
+// its tokens' slots among those of the later tokens first.  It reads 8 bytes a later token for that, beside some hundred units of
+// 32 bytes and more each; with many tokens it asks a table of one bit a hash value before it compares.
 // ------------------------------------------------------------------------------------------------
+constexpr uint32_t kAppendTokens = 1024;     // tokens of a workgroup at most
+constexpr uint32_t kAppendFilter = 8;        // tokens from which the table of bits is used
 struct AppendArgs {
     grape_wit_rope_append_args a;
     grape_wit_cache c;
-    uint32_t units, head_units;   // of a token, of a head
+    uint32_t units, head_units, per;         // of a token, of a head, of a workgroup
     uint64_t total;
-    int shift;
+    token::FastDiv by_units, by_head, by_page;
+    Scaler scale;
     uint32_t* status;
 };
 
+template <int W>
+struct Elements {
+    int32_t v[W];
+    __device__ __forceinline__ void load(const int32_t* x) {
+        if constexpr (W == 4) *reinterpret_cast<v4i_t*>(v) = *reinterpret_cast<const v4i_t*>(x);
+        else v[0] = *x;
+    }
+    __device__ __forceinline__ void store(int32_t* x) const {
+        if constexpr (W == 4) *reinterpret_cast<v4i_t*>(x) = *reinterpret_cast<const v4i_t*>(v);
+        else *x = v[0];
+    }
+};
+
+template <int W>
 __global__ void __launch_bounds__(kBlock) wit_append_kernel(AppendArgs p) {
-    const uint64_t i = (uint64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (i >= p.total) return;
+    __shared__ uint32_t shadowed[kAppendTokens / 32], bits[2048];
     const grape_wit_rope_append_args& a = p.a;
     const grape_wit_cache& c = p.c;
-    const uint32_t t = (uint32_t)(i / p.units), u = (uint32_t)(i - (uint64_t)t * p.units);
-    const uint32_t hh = u / p.head_units, j = u - hh * p.head_units;
-    auto kind = [&](uint32_t tok) { return token::append_kind(c, a.d_slots[tok], a.rot ? a.d_positions[tok] : 0, a.rot, a.table_rows); };
-    const int64_t slot = a.d_slots[t];
-    const int k = kind(t);
-    if (k == 2 && u == 0) atomicOr(p.status, (uint32_t)kWitIndex);
-    if (k) return;
-    const bool is_q = hh < a.heads, is_k = !is_q && hh < a.heads + c.heads;
-    const uint32_t h = is_q ? hh : is_k ? hh - a.heads : hh - a.heads - c.heads;
-    const int32_t* x = is_q ? a.d_q + t * a.q_stride : is_k ? a.d_k + t * a.k_stride : a.d_v + t * a.v_stride;
-    x += (size_t)h * c.dim;
-    int32_t *q, *r = nullptr;
-    if (is_q) {
-        const size_t o = ((size_t)t * a.heads + h) * c.dim;
-        q = a.d_q_out + o;
-        if (a.d_q_rem) r = a.d_q_rem + o;
-    } else {
-        const int64_t pg = slot / c.page_size;
-        q = (is_k ? c.d_k : c.d_v) + token::token_offset(c, (int32_t)pg, (uint32_t)(slot - pg * c.page_size)) + h * c.head_stride;
-        if (is_k && a.d_k_rem) r = a.d_k_rem + ((size_t)t * c.heads + h) * c.dim;
-        for (uint32_t o = t + 1; o < a.tokens; o++)
-            if (a.d_slots[o] == slot && kind(o) == 0) {
-                q = nullptr;
-                break;
+    const uint64_t u0 = (uint64_t)blockIdx.x * p.per;
+    const uint32_t t0 = (uint32_t)(u0 / p.units), skip = (uint32_t)(u0 - (uint64_t)t0 * p.units), n = (uint32_t)min((uint64_t)p.per, p.total - u0);
+    const uint32_t tokens = (skip + n - 1) / p.units + 1;          // of this workgroup
+    auto kind = [&](int64_t slot, uint32_t tok) { return token::append_kind(c, slot, a.rot ? a.d_positions[tok] : 0, a.rot, a.table_rows); };
+    if (t0 + 1 < a.tokens) {
+        const bool filter = tokens > kAppendFilter;
+        for (uint32_t i = threadIdx.x; i < (tokens + 31) / 32; i += kBlock) shadowed[i] = 0;
+        auto hash = [](int64_t slot) { return ((uint32_t)slot * 2654435761u) >> 16; };
+        if (filter) {
+            for (uint32_t i = threadIdx.x; i < 2048; i += kBlock) bits[i] = 0;
+            __syncthreads();
+            for (uint32_t j = threadIdx.x; j < tokens; j += kBlock) {
+                const uint32_t h = hash(a.d_slots[t0 + j]);
+                atomicOr(&bits[h >> 5], 1u << (h & 31u));
             }
+        }
+        __syncthreads();
+        for (uint32_t o = t0 + 1 + threadIdx.x; o < a.tokens; o += kBlock) {
+            const int64_t slot = a.d_slots[o];
+            if (slot < 0) continue;
+            if (filter) {
+                const uint32_t h = hash(slot);
+                if (!((bits[h >> 5] >> (h & 31u)) & 1u)) continue;
+            }
+            for (uint32_t j = 0; j < tokens && t0 + j < o; j++)
+                if (a.d_slots[t0 + j] == slot && kind(slot, o) == 0) atomicOr(&shadowed[j >> 5], 1u << (j & 31u));
+        }
+        __syncthreads();
     }
+    const uint32_t half = a.rot / 2, rotated = a.rot / (2 * W);
     uint32_t bad = 0;
-    if ((is_q || is_k) && 2 * j < a.rot) {
-        const uint32_t half = a.rot / 2, e0 = a.interleaved ? 2 * j : j, e1 = a.interleaved ? 2 * j + 1 : j + half;
-        const size_t row = (size_t)a.d_positions[t] * half + j;
-        const int64_t x0 = x[e0], x1 = x[e1], cs = a.d_cos[row], sn = a.d_sin[row];
-        int32_t q0, r0, q1, r1;
-        rescale64(x0 * cs - x1 * sn, a.scale, p.shift, q0, r0, bad);
-        rescale64(x0 * sn + x1 * cs, a.scale, p.shift, q1, r1, bad);
-        if (q) q[e0] = q0, q[e1] = q1;
-        if (r) r[e0] = r0, r[e1] = r1;
-    } else {
-        for (uint32_t e = 2 * j; e < std::min(2 * j + 2, c.dim); e++) {
-            if (q) q[e] = x[e];
-            if (r) r[e] = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += kBlock) {
+        const uint32_t j = p.by_units(skip + i), t = t0 + j, u = skip + i - j * p.units, hh = p.by_head(u), m = u - hh * p.head_units;
+        const bool is_q = hh < a.heads, is_k = !is_q && hh < a.heads + c.heads, turns = (is_q || is_k) && m < rotated;
+        const uint32_t h = is_q ? hh : is_k ? hh - a.heads : hh - a.heads - c.heads;
+        const int32_t* x = (is_q ? a.d_q + t * a.q_stride : is_k ? a.d_k + t * a.k_stride : a.d_v + t * a.v_stride) + (size_t)h * c.dim;
+        // the unit's two parts: side by side, or half a rotation apart; the second may lie past the head's end
+        const bool halves = turns && !a.interleaved;
+        const uint32_t e0 = (halves ? W : 2 * W) * m, e1 = halves ? e0 + half : e0 + W;
+        const bool second = e1 < c.dim;
+        Elements<W> x0, x1;
+        x0.load(x + e0);
+        if (second) x1.load(x + e1);
+        const int64_t slot = a.d_slots[t];
+        if (slot < 0) continue;
+        const int k = kind(slot, t);
+        if (k) {
+            if (u == 0) bad |= (uint32_t)kWitIndex;
+            continue;
+        }
+        int32_t *q = nullptr, *r = nullptr;
+        if (is_q) {
+            const size_t o = ((size_t)t * a.heads + h) * c.dim;
+            q = a.d_q_out + o;
+            if (a.d_q_rem) r = a.d_q_rem + o;
+        } else {
+            if (t0 + 1 >= a.tokens || !((shadowed[j >> 5] >> (j & 31u)) & 1u)) {
+                const uint32_t pg = p.by_page((uint32_t)slot);
+                q = (is_k ? c.d_k : c.d_v) + token::token_offset(c, (int32_t)pg, (uint32_t)slot - pg * c.page_size) + h * c.head_stride;
+            }
+            if (is_k && a.d_k_rem) r = a.d_k_rem + ((size_t)t * c.heads + h) * c.dim;
+        }
+        Elements<W> r0, r1;
+#pragma unroll
+        for (int w = 0; w < W; w++) r0.v[w] = r1.v[w] = 0;
+        if (turns) {
+            const size_t row = (size_t)a.d_positions[t] * half + W * m;
+            Elements<W> cs, sn;
+            cs.load(a.d_cos + row);
+            sn.load(a.d_sin + row);
+            Elements<W> q0, q1;
+            auto turn = [&](int32_t y0, int32_t y1, int w, int32_t& o0, int32_t& s0, int32_t& o1, int32_t& s1) {
+                p.scale.apply((int64_t)y0 * cs.v[w] - (int64_t)y1 * sn.v[w], o0, s0, bad);
+                p.scale.apply((int64_t)y0 * sn.v[w] + (int64_t)y1 * cs.v[w], o1, s1, bad);
+            };
+            if (a.interleaved) {
+                // elements in the order of memory: pair w is elements 2 w and 2 w + 1 of the 2 W
+                auto at = [&](Elements<W>& y0, Elements<W>& y1, int e) -> int32_t& { return e < W ? y0.v[e] : y1.v[e - W]; };
+#pragma unroll
+                for (int w = 0; w < W; w++) turn(at(x0, x1, 2 * w), at(x0, x1, 2 * w + 1), w, at(q0, q1, 2 * w), at(r0, r1, 2 * w), at(q0, q1, 2 * w + 1), at(r0, r1, 2 * w + 1));
+            } else {
+#pragma unroll
+                for (int w = 0; w < W; w++) turn(x0.v[w], x1.v[w], w, q0.v[w], r0.v[w], q1.v[w], r1.v[w]);
+            }
+            x0 = q0;
+            x1 = q1;
+        }
+        if (q) {
+            x0.store(q + e0);
+            if (second) x1.store(q + e1);
+        }
+        if (r) {
+            r0.store(r + e0);
+            if (second) r1.store(r + e1);
         }
     }
     if (bad) atomicOr(p.status, bad);
@@ -358,14 +433,27 @@ int grape_wit_rope_append(const grape_wit_rope_append_args* args, const grape_wi
     p.a = *args;
     p.c = *cache;
     const grape_wit_rope_append_args& a = p.a;
-    p.head_units = token::append_head_units(p.c.dim, a.rot, 1);
+    auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+    const bool vec = p.c.dim % 4 == 0 && a.rot % 8 == 0 && ((a.q_stride | a.k_stride | a.v_stride | p.c.page_stride | p.c.token_stride | p.c.head_stride) & 3) == 0 &&
+                     aligned(a.d_q) && aligned(a.d_k) && aligned(a.d_v) && aligned(a.d_cos) && aligned(a.d_sin) && aligned(a.d_q_out) && aligned(a.d_q_rem) &&
+                     aligned(a.d_k_rem) && aligned(p.c.d_k) && aligned(p.c.d_v);
+    p.head_units = token::append_head_units(p.c.dim, a.rot, vec ? 4 : 1);
     p.units = (a.heads + 2 * p.c.heads) * p.head_units;
     p.total = (uint64_t)a.tokens * p.units;
-    p.shift = log2_exact(a.scale);
+    // one unit a thread as long as that fills the chip twice, then longer shares
+    uint64_t per = std::max<uint64_t>(kBlock, (p.total + 4095) / 4096);
+    per = std::min<uint64_t>((per + kBlock - 1) / kBlock * kBlock, (uint64_t)(kAppendTokens - 2) * p.units);
+    p.per = (uint32_t)per;
+    p.by_units = token::fast_div(p.units);
+    p.by_head = token::fast_div(p.head_units);
+    p.by_page = token::fast_div(p.c.page_size);
+    p.scale = scaler(a.scale);
     hipStream_t s = as_stream(st);
     const int rc = wit_status_word(&p.status, s);
     if (rc) return rc;
-    wit_append_kernel<<<blocks_for(p.total), kBlock, 0, s>>>(p);
+    const unsigned grid = (unsigned)((p.total + per - 1) / per);
+    if (vec) wit_append_kernel<4><<<grid, kBlock, 0, s>>>(p);
+    else wit_append_kernel<1><<<grid, kBlock, 0, s>>>(p);
     GRAPE_LAUNCH_CHECK();
     return GRAPE_OK;
 }
