@@ -440,8 +440,8 @@ int grape_wit_rope_append(const grape_wit_rope_append_args* args, const grape_wi
     p.head_units = token::append_head_units(p.c.dim, a.rot, vec ? 4 : 1);
     p.units = (a.heads + 2 * p.c.heads) * p.head_units;
     p.total = (uint64_t)a.tokens * p.units;
-    // one unit a thread as long as that fills the chip twice, then longer shares
-    uint64_t per = std::max<uint64_t>(kBlock, (p.total + 4095) / 4096);
+    // one unit a thread as long as that fills the chip, then longer shares (2048 tokens of a head of 4096: 80 us; in twice as many 83)
+    uint64_t per = std::max<uint64_t>(kBlock, (p.total + 2047) / 2048);
     per = std::min<uint64_t>((per + kBlock - 1) / kBlock * kBlock, (uint64_t)(kAppendTokens - 2) * p.units);
     p.per = (uint32_t)per;
     p.by_units = token::fast_div(p.units);
