@@ -146,7 +146,8 @@ SIGNATURES = {
     "grape_wit_paged_attention_workspace": [c_u32, c_u32, c_u32, c_u32, c_u32],
     "grape_wit_paged_attention": [c_void_p, c_void_p, c_void_p],
     "grape_wit_matvec_q4": [c_void_p, c_void_p, c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int64, c_void_p, c_void_p, c_u32, c_u32, c_u32,
-                            c_u32, ctypes.c_int64, c_void_p],
+                            c_u32, ctypes.c_int64, c_void_p, c_size_t, c_void_p],
+    "grape_wit_matvec_q4_workspace": [c_u32, c_u32, c_u32],
     "grape_wit_status": [ctypes.POINTER(c_u32), c_void_p],
     "grape_bench_copy": [c_void_p, c_void_p, c_size_t, c_int, ctypes.POINTER(ctypes.c_float), c_void_p],
     "grape_bench_copy_fr": [c_void_p, c_void_p, c_size_t, c_int, ctypes.POINTER(ctypes.c_float), c_void_p],
@@ -164,7 +165,7 @@ SIGNATURES = {
 }
 _RESTYPES = {"grape_last_error": ctypes.c_char_p, "grape_g1_wide_table_bytes": c_size_t, "grape_eq_pyramid_elems": c_size_t,
              "grape_wround2_partial_bytes": c_size_t, "grape_wround_partial_bytes": c_size_t, "grape_carried_partial_bytes": c_size_t, "grape_fr_fold_i32_elems": c_size_t,
-             "grape_wit_paged_attention_workspace": c_size_t}
+             "grape_wit_paged_attention_workspace": c_size_t, "grape_wit_matvec_q4_workspace": c_size_t}
 
 _lib = None
 

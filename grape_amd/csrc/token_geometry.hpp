@@ -211,15 +211,32 @@ inline const char* refuse_attention(const grape_wit_attention_args* a, const gra
     return nullptr;
 }
 
+// Products with 4-bit weights: up to this many tokens are taken apart by the workgroups that multiply them; more by a launch of its
+// own, into the workspace, in tiles of eight or sixteen, and one word a block of 2048 inputs of a token says what its digits lack.
+constexpr uint32_t kQ4Few = 4;
+inline uint32_t q4_tile_tokens(uint32_t tokens) { return tokens <= 8 ? 8 : 16; }
+inline size_t q4_digit_words(uint32_t tokens, uint32_t inputs) {
+    const uint32_t tile = q4_tile_tokens(tokens);
+    return (size_t)ceil_div(tokens, tile) * ceil_div(inputs, 128) * 32 * 4 * tile;
+}
+inline size_t q4_workspace(uint32_t tokens, uint32_t inputs, uint32_t group) {
+    if (tokens <= kQ4Few || !inputs || !group || group % 32) return 0;
+    return 4 * (q4_digit_words(tokens, inputs) + (size_t)tokens * ceil_div(ceil_div(inputs, 128) * 16, 256));
+}
+
 inline const char* refuse_q4(const void* d_q, const void* d_x, int64_t x_stride, const void* d_w, int64_t w_stride, const void* d_scales,
-                             uint32_t tokens, uint32_t outputs, uint32_t inputs, uint32_t group, int64_t scale) {
+                             uint32_t tokens, uint32_t outputs, uint32_t inputs, uint32_t group, int64_t scale, const void* d_workspace, size_t workspace_bytes) {
     GRAPE_REFUSE(scale < 1 || scale > (int64_t)1 << 31, "scale must be in 1..2^31 (the remainder is stored as int32)");
     GRAPE_REFUSE(inputs < 1 || group < 1, "empty inner dimension or group");
-    GRAPE_REFUSE(inputs > (uint32_t)1 << 30, "at most 2^30 inputs");
+    GRAPE_REFUSE(inputs > (uint32_t)1 << 30 || group > (uint32_t)1 << 30, "at most 2^30 inputs");
     GRAPE_REFUSE(x_stride < 0 || w_stride < 0, "negative stride");
     if (!tokens || !outputs) return nullptr;
     GRAPE_REFUSE(!d_q || !d_x || !d_w || !d_scales, "d_q, d_x, d_w or d_scales is null");
-    GRAPE_REFUSE((uint64_t)tokens * outputs >= (uint64_t)1 << 38, "tensor too large");
+    GRAPE_REFUSE(tokens > 65535, "at most 65535 tokens");
+    GRAPE_REFUSE(outputs > (uint32_t)1 << 24, "at most 2^24 outputs");
+    const size_t need = q4_workspace(tokens, inputs, group);
+    GRAPE_REFUSE(workspace_bytes < need || (need && !d_workspace), "the workspace is too small");
+    GRAPE_REFUSE(need && ((uintptr_t)d_workspace & 15), "the workspace must be 16-byte aligned");
     return nullptr;
 }
 #undef GRAPE_REFUSE

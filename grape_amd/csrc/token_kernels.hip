@@ -1,6 +1,7 @@
 // The witness of new tokens: rotation and append to a paged cache, and products with 4-bit weights (their attention is in
 // token_attention.hip).  The arithmetic is that of witness_kernels.hip: exact 64-bit products, rescaled.
 #include <algorithm>
+#include <type_traits>
 #include "token_device.hpp"
 
 namespace grape {
@@ -155,8 +156,10 @@ struct Q4Args {
     const int32_t* scales;
     const uint8_t* zeros;
     uint32_t tokens, outputs, inputs, group, groups;
+    token::FastDiv by_group;
     Scaler scale;
     uint32_t* status;
+    uint32_t *digits, *over;     // of the inputs, where a launch of its own makes them
 };
 
 // Any group: a wave a row and up to four tokens, its lanes over the row's bytes.
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(kBlock) wit_q4_any_kernel(Q4Args p) {
         for (uint32_t half = 0; half < 2; half++) {
             const uint32_t k = 2 * i + half;
             if (k >= p.inputs) break;
-            const size_t at = (size_t)m * p.groups + k / p.group;
+            const size_t at = (size_t)m * p.groups + p.by_group(k);
             const int64_t v = (int64_t)p.scales[at] * ((int32_t)((byte >> (4 * half)) & 15u) - (p.zeros ? (int32_t)p.zeros[at] : 8));
 #pragma unroll
             for (uint32_t n = 0; n < 4; n++)
@@ -194,229 +197,324 @@ __global__ void __launch_bounds__(kBlock) wit_q4_any_kernel(Q4Args p) {
     if (bad) atomicOr(p.status, bad);
 }
 
-// Groups of whole 32s, on the matrix cores.  The input x = sum_p d_p 256^p (balanced digits, four planes) gives four columns a
-// token, a tile of 16 columns holds four tokens, and a weight byte is one nibble of the packed byte moved to the upper half
-// with its top bit turned over: 16 (w - 8) as a signed byte.  A lane's 16 packed bytes are then 32 of the row's weights, the
-// even ones and the odd ones an operand each, with the digits laid out in the same order.  After each step (GS inputs, which
-// lie in one group) the 32-bit sums are scaled and added to 64-bit ones: 128 * 128 * 128 * 16 stays far below 2^31.  Zero
-// points other than 8 add (8 - z) * sum of digits, which one more product, with ones, gives in the same registers.
-// A workgroup takes 16 rows and its eight waves take the row's steps of 128 inputs in turn, so that 4096 rows fill the chip
-// and a wave's share is in flight at once; the digits, scales and zero points are staged in LDS meanwhile.
-constexpr int kQ4Waves = 8, kQ4Ahead = 4;
-constexpr uint32_t kQ4Lds = 60 * 1024;       // of digits, scales and zero points; a longer input goes through in pieces
+// Groups of whole 32s, on the matrix cores.  The input x = sum_p d_p 256^p (balanced digits, four planes) gives a token four rows of
+// the first operand, and a weight byte of the second is one nibble of the packed byte moved to the upper half with its top bit
+// turned over: 16 (w - 8) as a signed byte.  A lane's 16 packed bytes are 32 of the row's weights, the even ones and the odd ones an
+// operand each, with the digits laid out in the same order.  Lane l then holds the four planes of token l / 16 for weight row
+// l % 16, the row whose bytes it has read: one scale a lane.  After each step (GS inputs, which lie in one group) two planes at a
+// time are put together in 32 bits (128 * 128 * 8 * 257 and the zero points' part stay below 2^31), scaled and added in 64 bits.
+// Zero points other than 8 add (8 - z) * sum of digits; one more product, with ones, gives those sums in the same registers.
+// The eight waves of a workgroup take consecutive shares of a tile of 16 rows, so that 4096 rows fill the chip; what a wave needs
+// next is requested some units of 128 inputs ahead.
+constexpr int kQ4Waves = 8, kQ4Threads = 64 * kQ4Waves;
 
+// 128 inputs of a weight row, 64 bytes, in one lane group: its 16 bytes, and the scales and zero points of their groups
 template <int GS>
-__device__ __forceinline__ v4i_t q4_load(const uint8_t* row, uint32_t bytes, uint32_t unit, uint32_t kg) {
-    constexpr int CB = GS / 8;               // bytes of a lane's share of GS inputs
-    union { v4i_t v; uint8_t b[16]; uint32_t u[4]; uint2 d[2]; } o;
-    const uint32_t base = unit * 64;
-    if (base + 64 <= bytes) {
+struct Q4Unit {
+    static constexpr int STEPS = 128 / GS, CB = GS / 8;          // scalings of a unit, bytes of a lane's share of GS inputs
+    v4i_t w;
+    int32_t scale[STEPS];
+    int32_t zero[STEPS];
+    __device__ __forceinline__ void load(const Q4Args& p, uint32_t row, uint32_t unit, uint32_t kg) {
+        const uint8_t* s = p.w + row * p.w_stride;
+        const uint32_t bytes = (p.inputs + 1) / 2, base = unit * 64;
+        if (base + 64 <= bytes) {
+            union { v4i_t v; uint32_t u[4]; uint2 d[2]; } o;
 #pragma unroll
-        for (int c = 0; c < 16 / CB; c++) {
-            const uint8_t* s = row + base + c * (GS / 2) + kg * CB;
-            if constexpr (CB == 16) __builtin_memcpy(&o.v, s, 16);
-            else if constexpr (CB == 8) __builtin_memcpy(&o.d[c], s, 8);
-            else __builtin_memcpy(&o.u[c], s, 4);
-        }
-    } else {
-#pragma unroll
-        for (int c = 0; c < 16 / CB; c++)
-#pragma unroll
-            for (int i = 0; i < CB; i++) {
-                const uint32_t at = base + c * (GS / 2) + kg * CB + i;
-                o.b[c * CB + i] = at < bytes ? row[at] : 0x88;
+            for (int c = 0; c < 16 / CB; c++) {
+                const uint8_t* at = s + base + c * (GS / 2) + kg * CB;
+                if constexpr (CB == 16) __builtin_memcpy(&o.v, at, 16);
+                else if constexpr (CB == 8) __builtin_memcpy(&o.d[c], at, 8);
+                else __builtin_memcpy(&o.u[c], at, 4);
             }
+            w = o.v;
+        } else {
+            // the row's last bytes; what follows them meets digits of zero
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t word = 0;
+#pragma unroll 1
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t b = 4 * c + i, at = base + b / CB * (GS / 2) + kg * CB + b % CB;
+                    word |= (at < bytes ? (uint32_t)s[at] : 0u) << (8 * i);
+                }
+                w[c] = (int)word;
+            }
+        }
+        const size_t first = (size_t)row * p.groups;
+#pragma unroll
+        for (int st = 0; st < STEPS; st++) {
+            const uint32_t g = min(p.by_group(unit * 128 + st * GS), p.groups - 1);
+            scale[st] = p.scales[first + g];
+            zero[st] = p.zeros ? (int32_t)p.zeros[first + g] : 8;
+        }
     }
-    return o.v;
+};
+
+// Where the word of plane pl of token n (of `cols` / 4) and the inputs 8 e .. 8 e + 7 stands, in words, among the first operands:
+// [unit][operand][lane group][column] of 16 bytes (GS = 32: of 8, four operands a unit instead of two).  `odd`: the odd inputs' word.
+template <int GS>
+__device__ __forceinline__ size_t q4_word(uint32_t e, uint32_t n, uint32_t pl, uint32_t cols, uint32_t odd) {
+    const uint32_t in = e & 15u, col = 4 * n + pl;
+    const size_t unit = e >> 4;
+    if constexpr (GS == 128) return ((((unit * 2 + odd) * 4 + (in >> 2)) * cols + col) << 2) + (in & 3u);
+    else if constexpr (GS == 64) return ((((unit * 2 + (in >> 3)) * 4 + ((in >> 1) & 3u)) * cols + col) << 2) + 2 * odd + (in & 1u);
+    else return ((((unit * 4 + (in >> 2)) * 4 + (in & 3u)) * cols + col) << 1) + odd;
 }
 
-// Eight inputs' digits, x[0..7] from an even place: the even ones' bytes of plane p in lo[p], the odd ones' in hi[p].
-__device__ __forceinline__ bool q4_digits(const int32_t* x, uint32_t lo[4], uint32_t hi[4]) {
-    uint32_t d[8];
+// Digits of eight inputs of token n, from 8 e; true where one has a top digit of 128, which its byte holds as -128.
+template <int GS>
+__device__ __forceinline__ bool q4_digits(const Q4Args& p, uint32_t n, uint32_t e, uint32_t* out, uint32_t e_out, uint32_t n_out, uint32_t cols) {
+    const uint32_t k = 8 * e;
+    const int32_t* x = p.x + n * p.x_stride + k;
+    int32_t v[8];
+    if (k + 8 <= p.inputs) __builtin_memcpy(v, x, 32);
+    else
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = k + j < p.inputs ? x[j] : 0;
+    uint32_t d[8], lo[4], hi[4];
     bool over = false;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        d[i] = digits_of(x[i]);
-        over |= x[i] > kDigitTop;
+        d[i] = digits_of(v[i]);
+        over |= v[i] > kDigitTop;
     }
     transpose4(d[0], d[2], d[4], d[6], lo);
     transpose4(d[1], d[3], d[5], d[7], hi);
+#pragma unroll
+    for (int pl = 0; pl < 4; pl++) {
+        out[q4_word<GS>(e_out, n_out, pl, cols, 0)] = lo[pl];
+        out[q4_word<GS>(e_out, n_out, pl, cols, 1)] = hi[pl];
+    }
     return over;
 }
 
-// Where the word of plane p of token n (of `nt`) and the inputs 8 e .. 8 e + 7 stands, among the operands of the product: units
-// of 128 inputs, 2 operands of 16 bytes a lane group (GS = 128, 64) or 4 of 8 (GS = 32).  `odd`: the odd inputs' word.
-template <int GS>
-__device__ __forceinline__ uint32_t q4_word(uint32_t e, uint32_t n, uint32_t p, uint32_t nt, uint32_t odd) {
-    const uint32_t unit = e >> 4, in = e & 15u, cols = 4 * nt;
-    if constexpr (GS == 128) {               // lane group in / 4; operand = parity; word in % 4
-        return ((((unit * 2 + odd) * 4 + (in >> 2)) * cols + 4 * n + p) << 2) + (in & 3u);
-    } else if constexpr (GS == 64) {         // operand in / 8; lane group (in % 8) / 2; words: two even, two odd
-        return ((((unit * 2 + (in >> 3)) * 4 + ((in >> 1) & 3u)) * cols + 4 * n + p) << 2) + 2 * odd + (in & 1u);
-    } else {                                 // operand in / 4; lane group in % 4; words: even, odd
-        return ((((unit * 4 + (in >> 2)) * 4 + (in & 3u)) * cols + 4 * n + p) << 1) + odd;
+// One unit of 128 inputs: the sums of planes 0, 1 and of planes 2, 3 of NT tiles of four tokens.  operand(op, j): the digits.
+template <int GS, int NT, class F>
+__device__ __forceinline__ void q4_unit(const Q4Unit<GS>& x, bool zeros, int64_t (*y)[2], F operand) {
+    v4i_t even, odd;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const uint32_t w = (uint32_t)x.w[c] ^ 0x88888888u;
+        even[c] = (int)((w << 4) & 0xf0f0f0f0u);
+        odd[c] = (int)(w & 0xf0f0f0f0u);
+    }
+    const v4i_t none = {0, 0, 0, 0}, one = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
+#pragma unroll
+    for (int st = 0; st < 128 / GS; st++) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            v4i_t acc = none, ones = none;
+            if constexpr (GS == 32) {
+                const long d = operand(st, j);
+                const long w = (long)(((uint64_t)(uint32_t)odd[st] << 32) | (uint32_t)even[st]);
+                acc = __builtin_amdgcn_mfma_i32_16x16x32_i8(d, w, acc, 0, 0, 0);
+                if (zeros) ones = __builtin_amdgcn_mfma_i32_16x16x32_i8(d, 0x0101010101010101L, ones, 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int op = 0; op < GS / 64; op++) {
+                    const v4i_t d = operand(st + op, j);
+                    v4i_t w;
+                    if constexpr (GS == 128) w = op ? odd : even;
+                    else w = v4i_t{even[2 * st], even[2 * st + 1], odd[2 * st], odd[2 * st + 1]};
+                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(d, w, acc, 0, 0, 0);
+                    if (zeros) ones = __builtin_amdgcn_mfma_i32_16x16x64_i8(d, one, ones, 0, 0, 0);
+                }
+            }
+            const int32_t up = 8 - x.zero[st];
+            int32_t s[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[i] = (acc[i] >> 4) + (zeros ? up * ones[i] : 0);
+            y[j][0] += (int64_t)(s[0] + 256 * s[1]) * x.scale[st];
+            y[j][1] += (int64_t)(s[2] + 256 * s[3]) * x.scale[st];
+        }
     }
 }
 
-template <int GS, bool ZEROS, int NT>        // NT: tiles of four tokens
-__global__ void __launch_bounds__(64 * kQ4Waves) wit_q4_kernel(Q4Args p, uint32_t piece) {
+// What inputs above kDigitTop of token n are short of in row m: 2^32 of each.
+__device__ __forceinline__ uint64_t q4_over(const Q4Args& p, uint32_t n, uint32_t m) {
+    const int32_t* x = p.x + n * p.x_stride;
+    const uint8_t* w = p.w + m * p.w_stride;
+    uint64_t more = 0;
+    for (uint32_t k = 0; k < p.inputs; k++)
+        if (x[k] > kDigitTop) {
+            const size_t at = (size_t)m * p.groups + p.by_group(k);
+            more += (uint64_t)((int64_t)p.scales[at] * ((int32_t)((w[k >> 1] >> (4 * (k & 1u))) & 15u) - (p.zeros ? (int32_t)p.zeros[at] : 8)));
+        }
+    return more << 32;
+}
+
+__device__ __forceinline__ void q4_out(const Q4Args& p, uint32_t n, uint32_t m, int64_t y, uint32_t& bad) {
+    int32_t q, r;
+    p.scale.apply(y, q, r, bad);
+    const size_t o = (size_t)n * p.outputs + m;
+    p.q[o] = q;
+    if (p.r) p.r[o] = r;
+}
+
+// Up to four tokens: a workgroup makes their digits itself, in LDS, once for all of its tiles of 16 rows (a longer input goes
+// through in pieces, for each tile again).
+template <int GS>
+__global__ void __launch_bounds__(kQ4Threads, 4) wit_q4_few_kernel(Q4Args p, uint32_t piece) {
+    constexpr int kQ4Ahead = GS == 32 ? 3 : 4;              // units; more do not fit the registers with four scales each
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    __shared__ int64_t sum[2][kQ4Waves][64];
     __shared__ uint32_t over_any;
-    constexpr int OPS = GS == 32 ? 4 : 2, STEPS = 128 / GS;      // operands and scalings of a unit
+    constexpr int OPS = GS == 32 ? 4 : 2;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, kg = lane >> 4;
-    const uint32_t m0 = blockIdx.x * 16, n0 = blockIdx.y * 4 * NT, nt = min(4u * NT, p.tokens - n0), cols = 4 * nt;
-    const uint32_t row = min(m0 + col, p.outputs - 1), bytes = (p.inputs + 1) / 2, units = (p.inputs + 127) / 128;
-    const uint8_t* w = p.w + row * p.w_stride;
-    // columns past the tokens read the first ones' digits again; nothing of them is kept
-    uint32_t at_col[NT];
-#pragma unroll
-    for (int j = 0; j < NT; j++) at_col[j] = 16 * j + col < cols ? 16 * j + col : 0;
-    int64_t y[NT][4];
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) y[j][i] = 0;
-    uint32_t* sc = lds;                                          // [groups of the piece][20]: 16 rows' scales, 4 words of zero points
-    const uint32_t piece_groups = (min(piece, units) * 128 - 1) / p.group + 2;
-    uint32_t* xd = lds + ((piece_groups * 20 + 3) & ~3u);
+    const uint32_t nt = p.tokens, cols = 4 * nt, units = (p.inputs + 127) / 128, tiles = (p.outputs + 15) / 16;
+    const uint32_t at_col = col < cols ? col : 0;          // rows past the tokens' planes: nothing of them is kept
     if (threadIdx.x == 0) over_any = 0;
-    for (uint32_t u0 = 0; u0 < units; u0 += piece) {
-        const uint32_t u1 = min(units, u0 + piece);
-        v4i_t a[kQ4Ahead];
+    uint32_t bad = 0, turn = 0;
+    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1u) {
+        const uint32_t m0 = tile * 16, row = min(m0 + col, p.outputs - 1);
+        int64_t y[1][2] = {{0, 0}};
+        for (uint32_t u0 = 0; u0 < units; u0 += piece) {
+            const uint32_t un = min(units - u0, piece), share = (un + kQ4Waves - 1) / kQ4Waves;
+            const uint32_t first = min(wave * share, un), last = min(first + share, un);          // of this wave, in the piece
+            Q4Unit<GS> next[kQ4Ahead];
 #pragma unroll
-        for (int s = 0; s < kQ4Ahead; s++)
-            if (u0 + wave + s * kQ4Waves < u1) a[s] = q4_load<GS>(w, bytes, u0 + wave + s * kQ4Waves, kg);
-        __syncthreads();
-        // digits of the piece
-        const uint32_t eighths = (u1 - u0) * 16;
-        for (uint32_t i = threadIdx.x; i < eighths * nt; i += 64 * kQ4Waves) {
-            const uint32_t n = i / eighths, e = i - n * eighths, k = 8 * (u0 * 16 + e);
-            const int32_t* x = p.x + (n0 + n) * p.x_stride + k;
-            int32_t v[8];
-            if (k + 8 <= p.inputs) __builtin_memcpy(v, x, 32);
-            else
+            for (int s = 0; s < kQ4Ahead; s++)
+                if (first + s < last) next[s].load(p, row, u0 + first + s, kg);
+            if (tile == blockIdx.x || piece < units) {
+                __syncthreads();                                // the digits of the piece before are not needed any more
+                for (uint32_t i = threadIdx.x; i < un * 16 * nt; i += kQ4Threads) {
+                    const uint32_t n = i / (un * 16), e = i - n * (un * 16);
+                    if (q4_digits<GS>(p, n, u0 * 16 + e, lds, e, n, cols)) over_any = 1;
+                }
+                __syncthreads();
+            }
+#pragma unroll 1
+            for (uint32_t u = first; u < last; u++) {
+                const Q4Unit<GS> x = next[0];
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = k + j < p.inputs ? x[j] : 0;
-            uint32_t lo[4], hi[4];
-            if (q4_digits(v, lo, hi)) over_any = 1;
-#pragma unroll
-            for (int pl = 0; pl < 4; pl++) {
-                xd[q4_word<GS>(e, n, pl, nt, 0)] = lo[pl];
-                xd[q4_word<GS>(e, n, pl, nt, 1)] = hi[pl];
+                for (int s = 0; s + 1 < kQ4Ahead; s++) next[s] = next[s + 1];
+                if (u + kQ4Ahead < last) next[kQ4Ahead - 1].load(p, row, u0 + u + kQ4Ahead, kg);
+                q4_unit<GS, 1>(x, p.zeros != nullptr, y, [&](int op, int) {
+                    const uint32_t o = ((u * OPS + op) * 4 + kg) * cols + at_col;
+                    if constexpr (GS == 32) return reinterpret_cast<const long*>(lds)[o];
+                    else return reinterpret_cast<const v4i_t*>(lds)[o];
+                });
             }
         }
-        const uint32_t g0 = u0 * 128 / p.group, gn = (min(u1 * 128, p.inputs) - 1) / p.group - g0 + 1;
-        for (uint32_t i = threadIdx.x; i < gn * 16; i += 64 * kQ4Waves) {
-            const uint32_t r = i / gn, g = i - r * gn;
-            const size_t at = (size_t)min(m0 + r, p.outputs - 1) * p.groups + g0 + g;
-            sc[g * 20 + r] = (uint32_t)p.scales[at];
-            if (ZEROS) reinterpret_cast<uint8_t*>(sc + g * 20 + 16)[r] = p.zeros[at];
-        }
+        sum[turn][wave][lane] = y[0][0] + (int64_t)((uint64_t)y[0][1] << 16);
         __syncthreads();
-        for (uint32_t u = u0 + wave; u < u1; u += kQ4Waves * kQ4Ahead) {
+        if (wave == 0 && kg < nt && m0 + col < p.outputs) {
+            int64_t v = 0;
 #pragma unroll
-            for (int s = 0; s < kQ4Ahead; s++) {
-                const uint32_t unit = u + s * kQ4Waves;
-                if (unit < u1) {
-                    const v4i_t wv = a[s];
-                    if (unit + kQ4Ahead * kQ4Waves < u1) a[s] = q4_load<GS>(w, bytes, unit + kQ4Ahead * kQ4Waves, kg);
-                    v4i_t even, odd;
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const uint32_t x = (uint32_t)wv[c] ^ 0x88888888u;
-                        even[c] = (int)((x << 4) & 0xf0f0f0f0u);
-                        odd[c] = (int)(x & 0xf0f0f0f0u);
-                    }
-#pragma unroll
-                    for (int st = 0; st < STEPS; st++) {
-                        const uint32_t g = (unit * 128 + st * GS) / p.group - g0;
-                        if (unit * 128 + st * GS >= p.inputs) break;
-                        const v4i_t scale = *reinterpret_cast<const v4i_t*>(sc + g * 20 + 4 * kg);
-                        const uint32_t zero = ZEROS ? sc[g * 20 + 16 + kg] : 0;
-#pragma unroll
-                        for (int j = 0; j < NT; j++) {
-                            v4i_t acc = {0, 0, 0, 0}, ones = {0, 0, 0, 0};
-                            if constexpr (GS == 32) {
-                                const uint32_t o = (((unit - u0) * OPS + st) * 4 + kg) * cols + at_col[j];
-                                const long b = *reinterpret_cast<const long*>(xd + (o << 1));
-                                union { uint32_t u[2]; long l; } f = {{(uint32_t)even[st], (uint32_t)odd[st]}};
-                                acc = __builtin_amdgcn_mfma_i32_16x16x32_i8(f.l, b, acc, 0, 0, 0);
-                                if (ZEROS) ones = __builtin_amdgcn_mfma_i32_16x16x32_i8(0x0101010101010101L, b, ones, 0, 0, 0);
-                            } else {
-#pragma unroll
-                                for (int op = 0; op < OPS / STEPS; op++) {
-                                    const uint32_t o = (((unit - u0) * OPS + st + op) * 4 + kg) * cols + at_col[j];
-                                    const v4i_t b = *reinterpret_cast<const v4i_t*>(xd + (o << 2));
-                                    v4i_t f;
-                                    if constexpr (GS == 128) f = op ? odd : even;
-                                    else f = v4i_t{even[2 * st], even[2 * st + 1], odd[2 * st], odd[2 * st + 1]};
-                                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, b, acc, 0, 0, 0);
-                                    if (ZEROS) {
-                                        const v4i_t o1 = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
-                                        ones = __builtin_amdgcn_mfma_i32_16x16x64_i8(o1, b, ones, 0, 0, 0);
-                                    }
-                                }
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                int32_t v = acc[i] >> 4;
-                                if (ZEROS) v += (8 - (int32_t)((zero >> (8 * i)) & 255u)) * ones[i];
-                                y[j][i] += (int64_t)v * scale[i];
-                            }
-                        }
-                    }
-                }
-            }
+            for (int k = 0; k < kQ4Waves; k++) v += sum[turn][k][lane];
+            if (over_any) v += (int64_t)q4_over(p, kg, m0 + col);
+            q4_out(p, kg, m0 + col, v, bad);
         }
-    }
-    // planes of a token stand in four neighbouring columns; then the waves' sums
-    __syncthreads();
-    int64_t* sum = reinterpret_cast<int64_t*>(lds);              // [wave][16 rows][4 NT tokens]
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            int64_t v = (int64_t)((uint64_t)y[j][i] << (8 * (col & 3u)));
-            v += __shfl_xor((long long)v, 1, 64);
-            v += __shfl_xor((long long)v, 2, 64);
-            if ((col & 3u) == 0) sum[(wave * 16 + 4 * kg + i) * 4 * NT + 4 * j + (col >> 2)] = v;
-        }
-    __syncthreads();
-    uint32_t bad = 0;
-    for (uint32_t i = threadIdx.x; i < 16 * 4 * NT; i += 64 * kQ4Waves) {
-        const uint32_t r = i & 15u, n = i >> 4, m = m0 + r;
-        if (n >= nt || m >= p.outputs) continue;
-        int64_t v = 0;
-#pragma unroll
-        for (int wv = 0; wv < kQ4Waves; wv++) v += sum[(wv * 16 + r) * 4 * NT + n];
-        if (over_any) {
-            // inputs above kDigitTop: their top digit is 128, which the byte held as -128; 2^32 of each is missing
-            const int32_t* x = p.x + (n0 + n) * p.x_stride;
-            const uint8_t* wr = p.w + m * p.w_stride;
-            uint64_t more = 0;
-            for (uint32_t k = 0; k < p.inputs; k++)
-                if (x[k] > kDigitTop) {
-                    const size_t at = (size_t)m * p.groups + k / p.group;
-                    more += (uint64_t)((int64_t)p.scales[at] * ((int32_t)((wr[k >> 1] >> (4 * (k & 1u))) & 15u) - (p.zeros ? (int32_t)p.zeros[at] : 8)));
-                }
-            v += (int64_t)(more << 32);
-        }
-        int32_t q, rr;
-        p.scale.apply(v, q, rr, bad);
-        const size_t o = (size_t)(n0 + n) * p.outputs + m;
-        p.q[o] = q;
-        if (p.r) p.r[o] = rr;
     }
     if (bad) atomicOr(p.status, bad);
 }
 
-template <int GS, bool ZEROS>
-static void q4_launch(const Q4Args& p, hipStream_t s) {
-    const uint32_t nt = std::min(p.tokens, 4u), units = (p.inputs + 127) / 128;
-    const uint32_t piece = std::min(units, kQ4Lds / (512 * nt + 80 * std::max(1u, 128 / p.group)));
-    const uint32_t piece_groups = (uint32_t)(((uint64_t)piece * 128 - 1) / p.group) + 2;
-    const size_t bytes = std::max<size_t>(((piece_groups * 20 + 3) & ~3u) * 4 + (size_t)piece * 512 * nt, kQ4Waves * 16 * 4 * 8);
-    wit_q4_kernel<GS, ZEROS, 1><<<dim3((p.outputs + 15) / 16, (p.tokens + 3) / 4), 64 * kQ4Waves, bytes, s>>>(p, piece);
+// More tokens: their digits are made once, by a launch of its own, and read from L2 as operands, 4 NT tokens at a time for RT tiles
+// of 16 rows.
+template <int GS>
+__global__ void __launch_bounds__(kBlock) wit_q4_digits_kernel(Q4Args p, uint32_t tile_tokens) {
+    __shared__ uint32_t over;
+    const uint32_t units = (p.inputs + 127) / 128, n = blockIdx.y, e = blockIdx.x * kBlock + threadIdx.x, tile = n / tile_tokens, cols = 4 * tile_tokens;
+    if (threadIdx.x == 0) over = 0;
+    __syncthreads();
+    uint32_t* out = p.digits + (size_t)tile * units * 32 * cols;          // 128 inputs of a column are 32 words
+    if (e < units * 16 && q4_digits<GS>(p, n, e, out, e, n - tile * tile_tokens, cols)) over = 1;
+    __syncthreads();
+    if (threadIdx.x == 0) p.over[n * gridDim.x + blockIdx.x] = over;
+}
+
+template <int GS, int NT, int RT>
+__global__ void __launch_bounds__(kQ4Threads, 2) wit_q4_many_kernel(Q4Args p, uint32_t over_words) {
+    constexpr int kQ4ManyAhead = GS == 32 ? 1 : 2;
+    __shared__ int64_t sum[kQ4Waves][RT * NT * 64];
+    __shared__ uint32_t over_any;
+    constexpr int OPS = GS == 32 ? 4 : 2;
+    constexpr uint32_t COLS = 16 * NT;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, kg = lane >> 4;
+    const uint32_t units = (p.inputs + 127) / 128, m0 = blockIdx.x * 16 * RT, n0 = blockIdx.y * 4 * NT;
+    const uint32_t* digits = p.digits + (size_t)blockIdx.y * units * 32 * COLS;
+    if (threadIdx.x == 0) over_any = 0;
+    int64_t y[RT][NT][2];
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) y[t][j][0] = y[t][j][1] = 0;
+    const uint32_t share = (units + kQ4Waves - 1) / kQ4Waves, first = min(wave * share, units), last = min(first + share, units);
+    Q4Unit<GS> next[kQ4ManyAhead][RT];
+#pragma unroll
+    for (int s = 0; s < kQ4ManyAhead; s++)
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+            if (first + s < last) next[s][t].load(p, min(m0 + 16 * t + col, p.outputs - 1), first + s, kg);
+#pragma unroll 1
+    for (uint32_t u = first; u < last; u++) {
+        typedef typename std::conditional<GS == 32, long, v4i_t>::type operand_t;
+        operand_t d[OPS][NT];
+#pragma unroll
+        for (int op = 0; op < OPS; op++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) d[op][j] = reinterpret_cast<const operand_t*>(digits)[(((size_t)u * OPS + op) * 4 + kg) * COLS + 16 * j + col];
+        Q4Unit<GS> x[RT];
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            x[t] = next[0][t];
+#pragma unroll
+            for (int s = 0; s + 1 < kQ4ManyAhead; s++) next[s][t] = next[s + 1][t];
+            if (u + kQ4ManyAhead < last) next[kQ4ManyAhead - 1][t].load(p, min(m0 + 16 * t + col, p.outputs - 1), u + kQ4ManyAhead, kg);
+        }
+#pragma unroll
+        for (int t = 0; t < RT; t++) q4_unit<GS, NT>(x[t], p.zeros != nullptr, y[t], [&](int op, int j) { return d[op][j]; });
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) sum[wave][(t * NT + j) * 64 + lane] = y[t][j][0] + (int64_t)((uint64_t)y[t][j][1] << 16);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < over_words; i += kQ4Threads)
+        if (p.over[i]) over_any = 1;
+    __syncthreads();
+    uint32_t bad = 0;
+    for (uint32_t i = threadIdx.x; i < RT * NT * 64; i += kQ4Threads) {
+        const uint32_t m = m0 + 16 * (i / (64 * NT)) + (i & 15u), n = n0 + 4 * (i / 64 % NT) + ((i >> 4) & 3u);
+        if (m >= p.outputs || n >= p.tokens) continue;
+        int64_t v = 0;
+#pragma unroll
+        for (int k = 0; k < kQ4Waves; k++) v += sum[k][i];
+        if (over_any) v += (int64_t)q4_over(p, n, m);
+        q4_out(p, n, m, v, bad);
+    }
+    if (bad) atomicOr(p.status, bad);
+}
+
+template <int GS>
+static int q4_launch(const Q4Args& p, hipStream_t s) {
+    const uint32_t units = (p.inputs + 127) / 128, tiles = (p.outputs + 15) / 16;
+    if (p.tokens <= token::kQ4Few) {
+        const uint32_t piece = std::min(units, token::kTokenLds / (512 * p.tokens));
+        // as many tiles for each workgroup: two workgroups a CU
+        const uint32_t turns = (tiles + 2 * kNumCU - 1) / (2 * kNumCU), grid = (tiles + turns - 1) / turns;
+        wit_q4_few_kernel<GS><<<grid, kQ4Threads, (size_t)piece * 512 * p.tokens, s>>>(p, piece);
+        GRAPE_LAUNCH_CHECK();
+        return GRAPE_OK;
+    }
+    const uint32_t tile_tokens = token::q4_tile_tokens(p.tokens);
+    const dim3 makers((units * 16 + kBlock - 1) / kBlock, p.tokens);
+    wit_q4_digits_kernel<GS><<<makers, kBlock, 0, s>>>(p, tile_tokens);
+    GRAPE_LAUNCH_CHECK();
+    const uint32_t over_words = makers.x * p.tokens, token_tiles = (p.tokens + tile_tokens - 1) / tile_tokens;
+    // two tiles of rows share the digits where that still leaves a workgroup for each CU
+    const bool two = (uint64_t)(tiles + 1) / 2 * token_tiles >= (uint64_t)kNumCU;
+    const dim3 grid(two ? (tiles + 1) / 2 : tiles, token_tiles);
+    if (tile_tokens == 8) {
+        if (two) wit_q4_many_kernel<GS, 2, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+        else wit_q4_many_kernel<GS, 2, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+    } else {
+        if (two) wit_q4_many_kernel<GS, 4, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+        else wit_q4_many_kernel<GS, 4, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+    }
+    GRAPE_LAUNCH_CHECK();
+    return GRAPE_OK;
 }
 
 }  // namespace grape
@@ -458,26 +556,33 @@ int grape_wit_rope_append(const grape_wit_rope_append_args* args, const grape_wi
     return GRAPE_OK;
 }
 
+size_t grape_wit_matvec_q4_workspace(uint32_t tokens, uint32_t inputs, uint32_t group) {
+    return token::q4_workspace(tokens, inputs, group);
+}
+
 int grape_wit_matvec_q4(int32_t* d_q, int32_t* d_r, const int32_t* d_x, int64_t x_stride, const uint8_t* d_w, int64_t w_stride,
                         const int32_t* d_scales, const uint8_t* d_zeros, uint32_t tokens, uint32_t outputs, uint32_t inputs,
-                        uint32_t group, int64_t scale, grape_stream_t st) {
+                        uint32_t group, int64_t scale, void* d_workspace, size_t workspace_bytes, grape_stream_t st) {
     GRAPE_REQUIRE(initialised(), "grape_init has not been called");
-    GRAPE_REFUSED_IF(token::refuse_q4(d_q, d_x, x_stride, d_w, w_stride, d_scales, tokens, outputs, inputs, group, scale));
+    GRAPE_REFUSED_IF(token::refuse_q4(d_q, d_x, x_stride, d_w, w_stride, d_scales, tokens, outputs, inputs, group, scale, d_workspace, workspace_bytes));
     if (tokens == 0 || outputs == 0) return GRAPE_OK;
     Q4Args p;
     p.q = d_q; p.r = d_r; p.x = d_x; p.x_stride = x_stride; p.w = d_w; p.w_stride = w_stride; p.scales = d_scales; p.zeros = d_zeros;
     p.tokens = tokens; p.outputs = outputs; p.inputs = inputs; p.group = group;
     p.groups = (inputs - 1) / group + 1;
+    p.by_group = token::fast_div(group);
     p.scale = scaler(scale);
+    p.digits = (uint32_t*)d_workspace;
+    p.over = p.digits + token::q4_digit_words(tokens, inputs);
     hipStream_t s = as_stream(st);
-    int rc = wit_status_word(&p.status, s);
+    const int rc = wit_status_word(&p.status, s);
     if (rc) return rc;
-    if (group % 32) wit_q4_any_kernel<<<dim3((outputs + 3) / 4, (tokens + 3) / 4), kBlock, 0, s>>>(p);
-    else if (group % 64) d_zeros ? q4_launch<32, true>(p, s) : q4_launch<32, false>(p, s);
-    else if (group % 128) d_zeros ? q4_launch<64, true>(p, s) : q4_launch<64, false>(p, s);
-    else d_zeros ? q4_launch<128, true>(p, s) : q4_launch<128, false>(p, s);
-    GRAPE_LAUNCH_CHECK();
-    return GRAPE_OK;
+    if (group % 32) {
+        wit_q4_any_kernel<<<dim3((outputs + 3) / 4, (tokens + 3) / 4), kBlock, 0, s>>>(p);
+        GRAPE_LAUNCH_CHECK();
+        return GRAPE_OK;
+    }
+    return group % 64 ? q4_launch<32>(p, s) : group % 128 ? q4_launch<64>(p, s) : q4_launch<128>(p, s);
 }
 
 }  // extern "C"

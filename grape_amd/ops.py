@@ -784,6 +784,12 @@ def _cache(k_cache, v_cache, dev):
     return _CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), pages, page, heads, dim, st[0], st[1], st[2]), heads, dim
 
 
+def _space(workspace, dev):
+    if workspace.dtype is not torch.uint8 or workspace.get_device() != dev or not workspace.is_contiguous():
+        _refuse("the workspace must be a contiguous uint8 tensor on the current device")
+    return workspace.data_ptr(), workspace.numel()
+
+
 def wit_rope_append(q, k, v, positions, slots, cos, sin, k_cache, v_cache, q_out=None, q_rem=None, k_rem=None, scale=1 << 16, interleaved=False):
     """Rotates q (tokens, heads, dim) and k (tokens, cache heads, dim) by positions (int32) with the tables cos, sin (rows,
     rot/2) at `scale`, and puts k and v into slots (int64: page * page size + offset; negative: padding, left out) of the caches
@@ -861,13 +867,13 @@ def wit_paged_attention(q, k_cache, v_cache, block_table, lens, max_len, exp_tab
     if "qkv" not in out or not _NAMES.issuperset(out):
         _refuse("out must hold qkv, and may hold %s", ", ".join(sorted(_NAMES)))
     if workspace is None:
-        workspace = torch.empty(lib.grape_wit_paged_attention_workspace(n, heads, heads_kv, dim, max_len), dtype=torch.uint8, device=q.device)
-    elif workspace.dtype is not torch.uint8 or workspace.get_device() != dev or not workspace.is_contiguous():
-        _refuse("the workspace must be a contiguous uint8 tensor")
+        size = lib.grape_wit_paged_attention_workspace(n, heads, heads_kv, dim, max_len)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    space, size = _space(workspace, dev) if workspace is not None else (0, 0)
     args = _ATTEND.pack(qp, qs, _arr(block_table, "block_table", width, dev), _arr(lens, "lens", (n,), dev), _arr(first, "first", (n,), dev),
                         _arr(exp_table, "exp_table", exp_table.shape, dev), *[_arr(get(name), name, rows, dev) for name in _PROOF_ROWS],
                         _arr(get("max"), "max", one, dev), _arr(get("exp_sum"), "exp_sum", one, dev), _arr(get("qkv"), "qkv", row, dev),
-                        _arr(get("qkv_rem"), "qkv_rem", row, dev), workspace.data_ptr(), workspace.numel(), qk_scale, prob_scale, out_scale, n,
+                        _arr(get("qkv_rem"), "qkv_rem", row, dev), space, size, qk_scale, prob_scale, out_scale, n,
                         heads, max_len, width[1], bit_shift, index_bits)
     _check(lib.grape_wit_paged_attention(args, cache, _stream(dev)))
     return out
@@ -878,9 +884,15 @@ def wit_paged_attention_workspace(seqs, heads, cache_heads, dim, max_len):
     return init().grape_wit_paged_attention_workspace(seqs, heads, cache_heads, dim, max_len)
 
 
-def wit_matvec_q4(x, w, scales, group, zeros=None, scale=1 << 16, q=None, r=None, want_r=True):
+def wit_matvec_q4_workspace(tokens, inputs, group):
+    """bytes of workspace that wit_matvec_q4 needs"""
+    return init().grape_wit_matvec_q4_workspace(tokens, inputs, group)
+
+
+def wit_matvec_q4(x, w, scales, group, zeros=None, scale=1 << 16, q=None, r=None, want_r=True, workspace=None):
     """x (tokens, inputs) int32 times 4-bit weights w (outputs, ceil(inputs / 2)) uint8, the even input in the lower half, with
-    scales (outputs, ceil(inputs / group)) int32 and zero points (the same, uint8; None: all 8).  Returns quotient, remainder."""
+    scales (outputs, ceil(inputs / group)) int32 and zero points (the same, uint8; None: all 8).  Returns quotient, remainder.
+    `workspace`: a uint8 tensor of wit_matvec_q4_workspace(...) bytes; without one the call makes its own."""
     lib = init()
     dev = _place()
     if x.dim() != 2 or w.dim() != 2 or group < 1:
@@ -896,8 +908,14 @@ def wit_matvec_q4(x, w, scales, group, zeros=None, scale=1 << 16, q=None, r=None
         q = _i32(n, m)
     if r is None and want_r:
         r = _i32(n, m)
+    space = size = 0
+    if workspace is not None:
+        space, size = _space(workspace, dev)
+    elif n > 4:                                        # none for fewer
+        workspace = torch.empty(lib.grape_wit_matvec_q4_workspace(n, k, group), dtype=torch.uint8, device=x.device)
+        space, size = workspace.data_ptr(), workspace.numel()
     _check(lib.grape_wit_matvec_q4(_arr(q, "q", (n, m), dev), _arr(r, "r", (n, m), dev), xp, xs, wp, ws, _arr(scales, "scales", groups, dev),
-                                   _arr(zeros, "zeros", groups, dev, torch.uint8), n, m, k, group, scale, _stream(dev)))
+                                   _arr(zeros, "zeros", groups, dev, torch.uint8), n, m, k, group, scale, space, size, _stream(dev)))
     return q, r
 
 

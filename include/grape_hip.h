@@ -746,7 +746,8 @@ int grape_wit_rope_append(const grape_wit_rope_append_args *args, const grape_wi
  * and makes the sequence's rows empty; a page outside the cache sets it too, and its keys and values count as zero.
  * 1 <= scales <= 2^31 (prob_scale <= 2^30), dim <= 8192.
  *
- * d_workspace (16-byte aligned) holds what the launches hand on to each other, grape_wit_paged_attention_workspace(...) bytes;
+ * d_workspace (16-byte aligned) holds what the launches hand on to each other, grape_wit_paged_attention_workspace(...) bytes
+ * (none up to 256 positions of short heads);
  * it needs no initial contents, and calls that may run at the same time, replays of captured ones among them, need one each. */
 typedef struct {
     const int32_t *d_q;
@@ -764,10 +765,12 @@ int grape_wit_paged_attention(const grape_wit_attention_args *args, const grape_
  * grape_wit_matmul_rescale does it - its result for the weights written out as integers.  Token n's inputs stand at
  * d_x + n*x_stride; row m of the weights at d_w + m*w_stride bytes, two to a byte, the even k in the lower half, (inputs + 1)/2
  * bytes; scales int32 and zero points bytes (d_zeros NULL: all 8), ceil(inputs/group) a row; outputs [tokens][outputs], d_r
- * may be NULL.  1 <= scale <= 2^31. */
+ * may be NULL.  1 <= scale <= 2^31, tokens <= 65535, outputs <= 2^24, group and inputs <= 2^30.  Groups of whole 32s go through
+ * the matrix cores.  d_workspace as above, grape_wit_matvec_q4_workspace(...) bytes (none for up to 4 tokens). */
+size_t grape_wit_matvec_q4_workspace(uint32_t tokens, uint32_t inputs, uint32_t group);
 int grape_wit_matvec_q4(int32_t *d_q, int32_t *d_r, const int32_t *d_x, int64_t x_stride, const uint8_t *d_w, int64_t w_stride,
                         const int32_t *d_scales, const uint8_t *d_zeros, uint32_t tokens, uint32_t outputs, uint32_t inputs,
-                        uint32_t group, int64_t scale, grape_stream_t stream);
+                        uint32_t group, int64_t scale, void *d_workspace, size_t workspace_bytes, grape_stream_t stream);
 /* Synchronises, returns the status bits set since the last call and clears them: 1 = a quotient left
  * int32, 2 = a table index out of range (the reference's assertions, model.py:86-87, :137-138),
  * 4 = a softmax row summed to zero or met a negative table entry, 8 = a sum of squares left 64 bits. */

@@ -7,8 +7,9 @@ using namespace grape;
 extern "C" {
 const char* refuse_append(const grape_wit_rope_append_args* a, const grape_wit_cache* c) { return token::refuse_append(a, c); }
 const char* refuse_attention(const grape_wit_attention_args* a, const grape_wit_cache* c) { return token::refuse_attention(a, c); }
-const char* refuse_q4(const void* q, const void* x, int64_t xs, const void* w, int64_t ws, const void* sc, uint32_t n, uint32_t m, uint32_t k, uint32_t g, int64_t s) {
-    return token::refuse_q4(q, x, xs, w, ws, sc, n, m, k, g, s);
+const char* refuse_q4(const void* q, const void* x, int64_t xs, const void* w, int64_t ws, const void* sc, uint32_t n, uint32_t m, uint32_t k, uint32_t g, int64_t s,
+                      const void* sp, size_t sb) {
+    return token::refuse_q4(q, x, xs, w, ws, sc, n, m, k, g, s, sp, sb);
 }
 size_t struct_bytes(int which) { return which == 0 ? sizeof(grape_wit_cache) : which == 1 ? sizeof(grape_wit_rope_append_args) : sizeof(grape_wit_attention_args); }
 int overlaps(const grape_wit_cache* c) { return token::cache_overlaps(*c); }
@@ -17,6 +18,7 @@ int span(int32_t len, int32_t first, uint32_t max_len, uint32_t stride, uint32_t
 }
 int64_t offset_of(const grape_wit_cache* c, int32_t page, uint32_t in_page) { return token::token_offset(*c, page, in_page); }
 int kind(const grape_wit_cache* c, int64_t slot, int32_t pos, uint32_t rot, uint32_t rows) { return token::append_kind(*c, slot, pos, rot, rows); }
+size_t q4_workspace(uint32_t n, uint32_t k, uint32_t g) { return token::q4_workspace(n, k, g); }
 size_t workspace(uint32_t s, uint32_t h, uint32_t hk, uint32_t d, uint32_t n) { return token::attention_workspace(s, h, hk, d, n); }
 uint32_t divided(uint32_t n, uint32_t d) { return token::fast_div(d)(n); }
 // the parts of a plan that bound what the kernels touch

@@ -25,7 +25,8 @@ def lib():
     for name in ("refuse_append", "refuse_attention", "refuse_q4"):
         getattr(l, name).restype = ctypes.c_char_p
     l.refuse_append.argtypes = l.refuse_attention.argtypes = [p, p]
-    l.refuse_q4.argtypes = [p, p, q, p, q, p, u, u, u, u, q]
+    l.refuse_q4.argtypes = [p, p, q, p, q, p, u, u, u, u, q, p, ctypes.c_size_t]
+    l.q4_workspace.argtypes, l.q4_workspace.restype = [u] * 3, ctypes.c_size_t
     l.struct_bytes.restype = l.workspace.restype = ctypes.c_size_t
     l.overlaps.argtypes = [p]
     l.span.argtypes = [i, i, u, u, u, p]
@@ -94,11 +95,13 @@ def test_bad_attentions_are_refused(lib, bad):
 
 
 @pytest.mark.parametrize("bad", [dict(scale=0), dict(scale=(1 << 31) + 1), dict(k=0), dict(group=0), dict(k=(1 << 30) + 1), dict(xs=-1), dict(ws=-1), dict(q=0), dict(x=0), dict(w=0),
-                                 dict(sc=0), dict(n=1 << 20, m=1 << 20)])
+                                 dict(sc=0), dict(n=65536, sb=1 << 40), dict(m=(1 << 24) + 1), dict(group=(1 << 30) + 1), dict(n=5), dict(n=5, sp=64), dict(n=5, sp=72, sb=1 << 20)])
 def test_bad_products_are_refused(lib, bad):
-    good = dict(q=16, x=16, xs=64, w=16, ws=32, sc=16, n=2, m=8, k=64, group=32, scale=65536)
+    good = dict(q=16, x=16, xs=64, w=16, ws=32, sc=16, n=2, m=8, k=64, group=32, scale=65536, sp=0, sb=0)
     assert lib.refuse_q4(*good.values()) is None
     assert lib.refuse_q4(*{**good, "n": 0, "q": 0}.values()) is None
+    assert lib.refuse_q4(*{**good, "n": 5, "sp": 64, "sb": lib.q4_workspace(5, 64, 32)}.values()) is None
+    assert lib.refuse_q4(*{**good, "n": 5, "group": 20}.values()) is None               # no digits without the matrix cores
     assert lib.refuse_q4(*{**good, **bad}.values())
 
 
@@ -187,6 +190,11 @@ def test_plans_cover_every_position_within_their_limits(lib):
 
 
 def test_workspace_sizes(lib):
+    assert lib.q4_workspace(4, 4096, 128) == 0 and lib.q4_workspace(9, 4096, 100) == 0 and lib.q4_workspace(9, 0, 32) == 0
+    for n, k in ((5, 1), (8, 128), (9, 129), (16, 11008), (17, 2049), (40, 4095)):
+        tile = 8 if n <= 8 else 16
+        digits = -(-n // tile) * tile * 4 * -(-k // 128) * 128                            # a byte an input and plane, whole units
+        assert lib.q4_workspace(n, k, 32) == digits + 4 * n * -(-(-(-k // 128) * 16) // 256)
     assert lib.workspace(0, 8, 8, 64, 100) == 0 and lib.workspace(65536, 8, 8, 64, 100) == 0 and lib.workspace(60000, 60000, 1, 64, 100000) == 0
     assert lib.workspace(1, 8, 2, 64, 1000) >= 4 * 8 * 1000
 
@@ -277,6 +285,6 @@ def test_helpers_hand_over_strides(helpers):
     ops.wit_rope_append(**{**append_args(), "q": q, "k": k, "v": v, "k_cache": kc, "v_cache": kc})
     args, c = helpers[0][1][:2]
     assert ops._APPEND.unpack(args)[3:6] == (fused.stride(0),) * 3 and ops._CACHE.unpack(c)[2:] == (10, 16, 4, 64, 16 * 70, 70, 160 * 70)
-    x = i32(1, 64).expand(5, 64)
+    x = i32(1, 64).expand(4, 64)
     ops.wit_matvec_q4(x, torch.zeros((8, 40), dtype=torch.uint8)[:, 3:35], i32(8, 2), 32)
     assert helpers[1][1][3] == 0 and helpers[1][1][5] == 40
