@@ -204,9 +204,9 @@ __global__ void __launch_bounds__(kBlock) wit_q4_any_kernel(Q4Args p) {
 // l % 16, the row whose bytes it has read: one scale a lane.  After each step (GS inputs, which lie in one group) two planes at a
 // time are put together in 32 bits (128 * 128 * 8 * 257 and the zero points' part stay below 2^31), scaled and added in 64 bits.
 // Zero points other than 8 add (8 - z) * sum of digits; one more product, with ones, gives those sums in the same registers.
-// The eight waves of a workgroup take consecutive shares of a tile of 16 rows, so that 4096 rows fill the chip; what a wave needs
+// The waves of a workgroup take consecutive shares of a tile of 16 rows' inputs, so that 4096 rows fill the chip; what a wave needs
 // next is requested some units of 128 inputs ahead.
-constexpr int kQ4Waves = 8, kQ4Threads = 64 * kQ4Waves;
+constexpr int kQ4Waves = 8, kQ4Threads = 64 * kQ4Waves, kQ4MostWaves = 16;
 
 // 128 inputs of a weight row, 64 bytes, in one lane group: its 16 bytes, and the scales and zero points of their groups
 template <int GS>
@@ -242,6 +242,14 @@ struct Q4Unit {
             }
         }
         const size_t first = (size_t)row * p.groups;
+        if (p.group == GS && (unit + 1) * STEPS <= p.groups) {          // neighbours
+            __builtin_memcpy(scale, p.scales + first + unit * STEPS, 4 * STEPS);
+            uint8_t z[STEPS];
+            if (p.zeros) __builtin_memcpy(z, p.zeros + first + unit * STEPS, STEPS);
+#pragma unroll
+            for (int st = 0; st < STEPS; st++) zero[st] = p.zeros ? z[st] : 8;
+            return;
+        }
 #pragma unroll
         for (int st = 0; st < STEPS; st++) {
             const uint32_t g = min(p.by_group(unit * 128 + st * GS), p.groups - 1);
@@ -352,62 +360,56 @@ __device__ __forceinline__ void q4_out(const Q4Args& p, uint32_t n, uint32_t m, 
     if (p.r) p.r[o] = r;
 }
 
-// Up to four tokens: a workgroup makes their digits itself, in LDS, once for all of its tiles of 16 rows (a longer input goes
-// through in pieces, for each tile again).
+// Up to four tokens: a workgroup makes their digits itself, in LDS (a longer input goes through in pieces), while its first weights
+// are under way.  blockDim: as many waves as share a tile's inputs.
 template <int GS>
-__global__ void __launch_bounds__(kQ4Threads, 4) wit_q4_few_kernel(Q4Args p, uint32_t piece) {
+__global__ void __launch_bounds__(64 * kQ4MostWaves, 4) wit_q4_few_kernel(Q4Args p, uint32_t piece) {
     constexpr int kQ4Ahead = GS == 32 ? 3 : 4;              // units; more do not fit the registers with four scales each
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
-    __shared__ int64_t sum[2][kQ4Waves][64];
+    __shared__ int64_t sum[kQ4MostWaves][64];
     __shared__ uint32_t over_any;
     constexpr int OPS = GS == 32 ? 4 : 2;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, kg = lane >> 4;
-    const uint32_t nt = p.tokens, cols = 4 * nt, units = (p.inputs + 127) / 128, tiles = (p.outputs + 15) / 16;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, col = lane & 15u, kg = lane >> 4;
+    const uint32_t nt = p.tokens, cols = 4 * nt, units = (p.inputs + 127) / 128, m0 = blockIdx.x * 16, row = min(m0 + col, p.outputs - 1);
     const uint32_t at_col = col < cols ? col : 0;          // rows past the tokens' planes: nothing of them is kept
     if (threadIdx.x == 0) over_any = 0;
-    uint32_t bad = 0, turn = 0;
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1u) {
-        const uint32_t m0 = tile * 16, row = min(m0 + col, p.outputs - 1);
-        int64_t y[1][2] = {{0, 0}};
-        for (uint32_t u0 = 0; u0 < units; u0 += piece) {
-            const uint32_t un = min(units - u0, piece), share = (un + kQ4Waves - 1) / kQ4Waves;
-            const uint32_t first = min(wave * share, un), last = min(first + share, un);          // of this wave, in the piece
-            Q4Unit<GS> next[kQ4Ahead];
+    int64_t y[1][2] = {{0, 0}};
+    for (uint32_t u0 = 0; u0 < units; u0 += piece) {
+        const uint32_t un = min(units - u0, piece), share = (un + waves - 1) / waves;
+        const uint32_t first = min(wave * share, un), last = min(first + share, un);          // of this wave, in the piece
+        Q4Unit<GS> next[kQ4Ahead];
 #pragma unroll
-            for (int s = 0; s < kQ4Ahead; s++)
-                if (first + s < last) next[s].load(p, row, u0 + first + s, kg);
-            if (tile == blockIdx.x || piece < units) {
-                __syncthreads();                                // the digits of the piece before are not needed any more
-                for (uint32_t i = threadIdx.x; i < un * 16 * nt; i += kQ4Threads) {
-                    const uint32_t n = i / (un * 16), e = i - n * (un * 16);
-                    if (q4_digits<GS>(p, n, u0 * 16 + e, lds, e, n, cols)) over_any = 1;
-                }
-                __syncthreads();
-            }
-#pragma unroll 1
-            for (uint32_t u = first; u < last; u++) {
-                const Q4Unit<GS> x = next[0];
-#pragma unroll
-                for (int s = 0; s + 1 < kQ4Ahead; s++) next[s] = next[s + 1];
-                if (u + kQ4Ahead < last) next[kQ4Ahead - 1].load(p, row, u0 + u + kQ4Ahead, kg);
-                q4_unit<GS, 1>(x, p.zeros != nullptr, y, [&](int op, int) {
-                    const uint32_t o = ((u * OPS + op) * 4 + kg) * cols + at_col;
-                    if constexpr (GS == 32) return reinterpret_cast<const long*>(lds)[o];
-                    else return reinterpret_cast<const v4i_t*>(lds)[o];
-                });
-            }
+        for (int s = 0; s < kQ4Ahead; s++)
+            if (first + s < last) next[s].load(p, row, u0 + first + s, kg);
+        __syncthreads();                                    // the digits of the piece before are not needed any more
+        for (uint32_t i = threadIdx.x; i < un * 16 * nt; i += blockDim.x) {
+            const uint32_t n = i / (un * 16), e = i - n * (un * 16);
+            if (q4_digits<GS>(p, n, u0 * 16 + e, lds, e, n, cols)) over_any = 1;
         }
-        sum[turn][wave][lane] = y[0][0] + (int64_t)((uint64_t)y[0][1] << 16);
         __syncthreads();
-        if (wave == 0 && kg < nt && m0 + col < p.outputs) {
-            int64_t v = 0;
+#pragma unroll 1
+        for (uint32_t u = first; u < last; u++) {
+            const Q4Unit<GS> x = next[0];
 #pragma unroll
-            for (int k = 0; k < kQ4Waves; k++) v += sum[turn][k][lane];
-            if (over_any) v += (int64_t)q4_over(p, kg, m0 + col);
-            q4_out(p, kg, m0 + col, v, bad);
+            for (int s = 0; s + 1 < kQ4Ahead; s++) next[s] = next[s + 1];
+            if (u + kQ4Ahead < last) next[kQ4Ahead - 1].load(p, row, u0 + u + kQ4Ahead, kg);
+            q4_unit<GS, 1>(x, p.zeros != nullptr, y, [&](int op, int) {
+                const uint32_t o = ((u * OPS + op) * 4 + kg) * cols + at_col;
+                if constexpr (GS == 32) return reinterpret_cast<const long*>(lds)[o];
+                else return reinterpret_cast<const v4i_t*>(lds)[o];
+            });
         }
     }
-    if (bad) atomicOr(p.status, bad);
+    sum[wave][lane] = y[0][0] + (int64_t)((uint64_t)y[0][1] << 16);
+    __syncthreads();
+    if (wave == 0 && kg < nt && m0 + col < p.outputs) {
+        int64_t v = 0;
+        for (uint32_t k = 0; k < waves; k++) v += sum[k][lane];
+        if (over_any) v += (int64_t)q4_over(p, kg, m0 + col);
+        uint32_t bad = 0;
+        q4_out(p, kg, m0 + col, v, bad);
+        if (bad) atomicOr(p.status, bad);
+    }
 }
 
 // More tokens: their digits are made once, by a launch of its own, and read from L2 as operands, 4 NT tokens at a time for RT tiles
@@ -491,10 +493,10 @@ template <int GS>
 static int q4_launch(const Q4Args& p, hipStream_t s) {
     const uint32_t units = (p.inputs + 127) / 128, tiles = (p.outputs + 15) / 16;
     if (p.tokens <= token::kQ4Few) {
-        const uint32_t piece = std::min(units, token::kTokenLds / (512 * p.tokens));
-        // as many tiles for each workgroup: two workgroups a CU
-        const uint32_t turns = (tiles + 2 * kNumCU - 1) / (2 * kNumCU), grid = (tiles + turns - 1) / turns;
-        wit_q4_few_kernel<GS><<<grid, kQ4Threads, (size_t)piece * 512 * p.tokens, s>>>(p, piece);
+        const uint32_t piece = std::min(units, (token::kTokenLds - 8192) / (512 * p.tokens));
+        // about sixteen waves a CU, however many tiles there are
+        const uint32_t waves = tiles <= (uint32_t)kNumCU ? 16 : tiles <= 2u * kNumCU ? 8 : 4;
+        wit_q4_few_kernel<GS><<<tiles, 64 * waves, (size_t)piece * 512 * p.tokens, s>>>(p, piece);
         GRAPE_LAUNCH_CHECK();
         return GRAPE_OK;
     }
