@@ -208,56 +208,89 @@ __global__ void __launch_bounds__(kBlock) wit_q4_any_kernel(Q4Args p) {
 // next is requested some units of 128 inputs ahead.
 constexpr int kQ4Waves = 8, kQ4Threads = 64 * kQ4Waves, kQ4MostWaves = 16;
 
-// 128 inputs of a weight row, 64 bytes, in one lane group: its 16 bytes, and the scales and zero points of their groups
+// Four units of 128 inputs of 16 weight rows.  A wave reads 256 bytes in a row among 16 neighbouring lanes, then turns them over
+// through 4 KB of LDS of its own into the operands, where 16 neighbouring lanes hold 16 rows: read as operands in the first place,
+// every lane's 16 bytes would be a line of memory of their own, and so would the scales (22.5 MB of weights with scales and zero
+// points for each 64 took 17.7 us that way).  Scales and zero points are read by lane 4 r + s for row r and unit s.
 template <int GS>
-struct Q4Unit {
-    static constexpr int STEPS = 128 / GS, CB = GS / 8;          // scalings of a unit, bytes of a lane's share of GS inputs
-    v4i_t w;
+struct Q4Quad {
+    static constexpr int STEPS = 128 / GS;          // scalings of a unit
+    v4i_t w[4];
     int32_t scale[STEPS];
-    int32_t zero[STEPS];
-    __device__ __forceinline__ void load(const Q4Args& p, uint32_t row, uint32_t unit, uint32_t kg) {
-        const uint8_t* s = p.w + row * p.w_stride;
-        const uint32_t bytes = (p.inputs + 1) / 2, base = unit * 64;
-        if (base + 64 <= bytes) {
-            union { v4i_t v; uint32_t u[4]; uint2 d[2]; } o;
+    uint32_t zeros;                                 // a byte a step
+    __device__ __forceinline__ void load(const Q4Args& p, uint32_t m0, uint32_t unit, uint32_t lane) {
+        const uint32_t bytes = (p.inputs + 1) / 2, at = unit * 64 + 16 * (lane & 15u);
 #pragma unroll
-            for (int c = 0; c < 16 / CB; c++) {
-                const uint8_t* at = s + base + c * (GS / 2) + kg * CB;
-                if constexpr (CB == 16) __builtin_memcpy(&o.v, at, 16);
-                else if constexpr (CB == 8) __builtin_memcpy(&o.d[c], at, 8);
-                else __builtin_memcpy(&o.u[c], at, 4);
-            }
-            w = o.v;
-        } else {
-            // the row's last bytes; what follows them meets digits of zero
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t word = 0;
-#pragma unroll 1
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t b = 4 * c + i, at = base + b / CB * (GS / 2) + kg * CB + b % CB;
-                    word |= (at < bytes ? (uint32_t)s[at] : 0u) << (8 * i);
-                }
-                w[c] = (int)word;
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint8_t* s = p.w + min(m0 + 4 * i + (lane >> 4), p.outputs - 1) * p.w_stride;
+            if (at + 16 <= bytes) {
+                __builtin_memcpy(&w[i], s + at, 16);
+            } else {
+                // the row's last bytes; what follows them meets digits of zero
+                w[i] = v4i_t{0, 0, 0, 0};
+                uint8_t last[16] = {0};
+                for (uint32_t b = 0; at + b < bytes; b++) last[b] = s[at + b];
+                __builtin_memcpy(&w[i], last, 16);
             }
         }
+        const uint32_t row = min(m0 + (lane >> 2), p.outputs - 1), u = unit + (lane & 3u);
         const size_t first = (size_t)row * p.groups;
-        if (p.group == GS && (unit + 1) * STEPS <= p.groups) {          // neighbours
-            __builtin_memcpy(scale, p.scales + first + unit * STEPS, 4 * STEPS);
-            uint8_t z[STEPS];
-            if (p.zeros) __builtin_memcpy(z, p.zeros + first + unit * STEPS, STEPS);
-#pragma unroll
-            for (int st = 0; st < STEPS; st++) zero[st] = p.zeros ? z[st] : 8;
+        zeros = 0;
+        if (p.group == GS && (u + 1) * STEPS <= p.groups) {          // neighbours
+            __builtin_memcpy(scale, p.scales + first + u * STEPS, 4 * STEPS);
+            if (p.zeros) __builtin_memcpy(&zeros, p.zeros + first + u * STEPS, STEPS);
             return;
         }
 #pragma unroll
         for (int st = 0; st < STEPS; st++) {
-            const uint32_t g = min(p.by_group(unit * 128 + st * GS), p.groups - 1);
+            const uint32_t g = min(p.by_group(min(u * 128 + st * GS, p.inputs - 1)), p.groups - 1);
             scale[st] = p.scales[first + g];
-            zero[st] = p.zeros ? (int32_t)p.zeros[first + g] : 8;
+            if (p.zeros) zeros |= (uint32_t)p.zeros[first + g] << (8 * st);
+        }
+    }
+    // 16 bytes: chunk c of row r stands at 16 r + (c ^ r), so that the sixteen rows' equal chunks spread over the banks
+    __device__ __forceinline__ void store(uint8_t* lds, uint32_t lane) const {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t r = 4 * i + (lane >> 4), c = lane & 15u;
+            *reinterpret_cast<v4i_t*>(lds + 16 * (16 * r + (c ^ r))) = w[i];
         }
     }
 };
+
+// A lane's 16 bytes of unit s of its row, and its scales: GS / 2 bytes of a step lie among the four lane groups.
+template <int GS>
+struct Q4Unit {
+    static constexpr int STEPS = 128 / GS, CB = GS / 8;
+    v4i_t w;
+    int32_t scale[STEPS], zero[STEPS];
+    __device__ __forceinline__ void take(const Q4Quad<GS>& q, const uint8_t* lds, uint32_t s, uint32_t lane, bool zeros) {
+        const uint32_t r = lane & 15u, kg = lane >> 4;
+        union { v4i_t v; uint32_t u[4]; uint2 d[2]; } o;
+#pragma unroll
+        for (uint32_t c = 0; c < 16 / CB; c++) {
+            const uint32_t at = 64 * s + c * (GS / 2) + kg * CB, chunk = at >> 4;
+            const uint8_t* from = lds + 16 * (16 * r + (chunk ^ r)) + (at & 15u);
+            if constexpr (CB == 16) o.v = *reinterpret_cast<const v4i_t*>(from);
+            else if constexpr (CB == 8) o.d[c] = *reinterpret_cast<const uint2*>(from);
+            else o.u[c] = *reinterpret_cast<const uint32_t*>(from);
+        }
+        w = o.v;
+        const uint32_t z = zeros ? (uint32_t)__shfl((int)q.zeros, 4 * r + s, 64) : 0u;
+#pragma unroll
+        for (int st = 0; st < STEPS; st++) {
+            scale[st] = __shfl(q.scale[st], 4 * r + s, 64);
+            zero[st] = (int32_t)((z >> (8 * st)) & 255u);
+        }
+    }
+};
+
+// what one lane of a wave wrote to LDS is there for the others
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // Where the word of plane pl of token n (of `cols` / 4) and the inputs 8 e .. 8 e + 7 stands, in words, among the first operands:
 // [unit][operand][lane group][column] of 16 bytes (GS = 32: of 8, four operands a unit instead of two).  `odd`: the odd inputs' word.
@@ -361,26 +394,24 @@ __device__ __forceinline__ void q4_out(const Q4Args& p, uint32_t n, uint32_t m, 
 }
 
 // Up to four tokens: a workgroup makes their digits itself, in LDS (a longer input goes through in pieces), while its first weights
-// are under way.  blockDim: as many waves as share a tile's inputs.
+// are under way.  blockDim: as many waves as share a tile's inputs, 4 KB of LDS each behind the digits.
 template <int GS>
 __global__ void __launch_bounds__(64 * kQ4MostWaves, 4) wit_q4_few_kernel(Q4Args p, uint32_t piece) {
-    constexpr int kQ4Ahead = GS == 32 ? 3 : 4;              // units; more do not fit the registers with four scales each
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
-    __shared__ int64_t sum[kQ4MostWaves][64];
     __shared__ uint32_t over_any;
     constexpr int OPS = GS == 32 ? 4 : 2;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, col = lane & 15u, kg = lane >> 4;
-    const uint32_t nt = p.tokens, cols = 4 * nt, units = (p.inputs + 127) / 128, m0 = blockIdx.x * 16, row = min(m0 + col, p.outputs - 1);
+    const uint32_t nt = p.tokens, cols = 4 * nt, units = (p.inputs + 127) / 128, m0 = blockIdx.x * 16;
     const uint32_t at_col = col < cols ? col : 0;          // rows past the tokens' planes: nothing of them is kept
+    uint8_t* turned = reinterpret_cast<uint8_t*>(lds + (size_t)piece * 128 * nt) + 4096 * wave;
     if (threadIdx.x == 0) over_any = 0;
     int64_t y[1][2] = {{0, 0}};
     for (uint32_t u0 = 0; u0 < units; u0 += piece) {
-        const uint32_t un = min(units - u0, piece), share = (un + waves - 1) / waves;
+        // shares of whole fours
+        const uint32_t un = min(units - u0, piece), share = ((un + waves - 1) / waves + 3) / 4 * 4;
         const uint32_t first = min(wave * share, un), last = min(first + share, un);          // of this wave, in the piece
-        Q4Unit<GS> next[kQ4Ahead];
-#pragma unroll
-        for (int s = 0; s < kQ4Ahead; s++)
-            if (first + s < last) next[s].load(p, row, u0 + first + s, kg);
+        Q4Quad<GS> next;
+        if (first < last) next.load(p, m0, u0 + first, lane);
         __syncthreads();                                    // the digits of the piece before are not needed any more
         for (uint32_t i = threadIdx.x; i < un * 16 * nt; i += blockDim.x) {
             const uint32_t n = i / (un * 16), e = i - n * (un * 16);
@@ -388,23 +419,31 @@ __global__ void __launch_bounds__(64 * kQ4MostWaves, 4) wit_q4_few_kernel(Q4Args
         }
         __syncthreads();
 #pragma unroll 1
-        for (uint32_t u = first; u < last; u++) {
-            const Q4Unit<GS> x = next[0];
-#pragma unroll
-            for (int s = 0; s + 1 < kQ4Ahead; s++) next[s] = next[s + 1];
-            if (u + kQ4Ahead < last) next[kQ4Ahead - 1].load(p, row, u0 + u + kQ4Ahead, kg);
-            q4_unit<GS, 1>(x, p.zeros != nullptr, y, [&](int op, int) {
-                const uint32_t o = ((u * OPS + op) * 4 + kg) * cols + at_col;
-                if constexpr (GS == 32) return reinterpret_cast<const long*>(lds)[o];
-                else return reinterpret_cast<const v4i_t*>(lds)[o];
-            });
+        for (uint32_t u = first; u < last; u += 4) {
+            const Q4Quad<GS> quad = next;
+            if (u + 4 < last) next.load(p, m0, u0 + u + 4, lane);
+            wave_sync();
+            quad.store(turned, lane);
+            wave_sync();
+#pragma unroll 1
+            for (uint32_t s = 0; s < 4 && u + s < last; s++) {
+                Q4Unit<GS> x;
+                x.take(quad, turned, s, lane, p.zeros != nullptr);
+                q4_unit<GS, 1>(x, p.zeros != nullptr, y, [&](int op, int) {
+                    const uint32_t o = (((u + s) * OPS + op) * 4 + kg) * cols + at_col;
+                    if constexpr (GS == 32) return reinterpret_cast<const long*>(lds)[o];
+                    else return reinterpret_cast<const v4i_t*>(lds)[o];
+                });
+            }
         }
     }
-    sum[wave][lane] = y[0][0] + (int64_t)((uint64_t)y[0][1] << 16);
+    __syncthreads();
+    int64_t* sum = reinterpret_cast<int64_t*>(lds);          // [wave][lane]
+    sum[threadIdx.x] = y[0][0] + (int64_t)((uint64_t)y[0][1] << 16);
     __syncthreads();
     if (wave == 0 && kg < nt && m0 + col < p.outputs) {
         int64_t v = 0;
-        for (uint32_t k = 0; k < waves; k++) v += sum[k][lane];
+        for (uint32_t k = 0; k < waves; k++) v += sum[64 * k + lane];
         if (over_any) v += (int64_t)q4_over(p, kg, m0 + col);
         uint32_t bad = 0;
         q4_out(p, kg, m0 + col, v, bad);
@@ -428,51 +467,68 @@ __global__ void __launch_bounds__(kBlock) wit_q4_digits_kernel(Q4Args p, uint32_
 
 template <int GS, int NT, int RT>
 __global__ void __launch_bounds__(kQ4Threads, 2) wit_q4_many_kernel(Q4Args p, uint32_t over_words) {
-    constexpr int kQ4ManyAhead = GS == 32 ? 1 : 2;
-    __shared__ int64_t sum[kQ4Waves][RT * NT * 64];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kQ4Waves * RT * 4096];
     __shared__ uint32_t over_any;
     constexpr int OPS = GS == 32 ? 4 : 2;
     constexpr uint32_t COLS = 16 * NT;
+    static_assert(sizeof lds >= sizeof(int64_t) * kQ4Waves * RT * NT * 64, "the sums fit where the weights were turned over");
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, kg = lane >> 4;
     const uint32_t units = (p.inputs + 127) / 128, m0 = blockIdx.x * 16 * RT, n0 = blockIdx.y * 4 * NT;
     const uint32_t* digits = p.digits + (size_t)blockIdx.y * units * 32 * COLS;
+    uint8_t* turned = lds + wave * RT * 4096;
     if (threadIdx.x == 0) over_any = 0;
     int64_t y[RT][NT][2];
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
         for (int j = 0; j < NT; j++) y[t][j][0] = y[t][j][1] = 0;
-    const uint32_t share = (units + kQ4Waves - 1) / kQ4Waves, first = min(wave * share, units), last = min(first + share, units);
-    Q4Unit<GS> next[kQ4ManyAhead][RT];
+    const uint32_t share = ((units + kQ4Waves - 1) / kQ4Waves + 3) / 4 * 4, first = min(wave * share, units), last = min(first + share, units);
+    Q4Quad<GS> next[RT];
 #pragma unroll
-    for (int s = 0; s < kQ4ManyAhead; s++)
-#pragma unroll
-        for (int t = 0; t < RT; t++)
-            if (first + s < last) next[s][t].load(p, min(m0 + 16 * t + col, p.outputs - 1), first + s, kg);
-#pragma unroll 1
-    for (uint32_t u = first; u < last; u++) {
-        typedef typename std::conditional<GS == 32, long, v4i_t>::type operand_t;
-        operand_t d[OPS][NT];
+    for (int t = 0; t < RT; t++)
+        if (first < last) next[t].load(p, m0 + 16 * t, first, lane);
+    typedef typename std::conditional<GS == 32, long, v4i_t>::type operand_t;
+    operand_t d[OPS][NT];                                    // the next unit's digits
+    auto fetch = [&](uint32_t u) {
 #pragma unroll
         for (int op = 0; op < OPS; op++)
 #pragma unroll
             for (int j = 0; j < NT; j++) d[op][j] = reinterpret_cast<const operand_t*>(digits)[(((size_t)u * OPS + op) * 4 + kg) * COLS + 16 * j + col];
-        Q4Unit<GS> x[RT];
+    };
+    if (first < last) fetch(first);
+#pragma unroll 1
+    for (uint32_t u = first; u < last; u += 4) {
+        Q4Quad<GS> quad[RT];
+        wave_sync();
 #pragma unroll
         for (int t = 0; t < RT; t++) {
-            x[t] = next[0][t];
-#pragma unroll
-            for (int s = 0; s + 1 < kQ4ManyAhead; s++) next[s][t] = next[s + 1][t];
-            if (u + kQ4ManyAhead < last) next[kQ4ManyAhead - 1][t].load(p, min(m0 + 16 * t + col, p.outputs - 1), u + kQ4ManyAhead, kg);
+            quad[t] = next[t];
+            quad[t].store(turned + 4096 * t, lane);
+            if (u + 4 < last) next[t].load(p, m0 + 16 * t, u + 4, lane);
         }
+        wave_sync();
+#pragma unroll 1
+        for (uint32_t s = 0; s < 4 && u + s < last; s++) {
+            operand_t now[OPS][NT];
 #pragma unroll
-        for (int t = 0; t < RT; t++) q4_unit<GS, NT>(x[t], p.zeros != nullptr, y[t], [&](int op, int j) { return d[op][j]; });
+            for (int op = 0; op < OPS; op++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) now[op][j] = d[op][j];
+            if (u + s + 1 < last) fetch(u + s + 1);
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                Q4Unit<GS> x;
+                x.take(quad[t], turned + 4096 * t, s, lane, p.zeros != nullptr);
+                q4_unit<GS, NT>(x, p.zeros != nullptr, y[t], [&](int op, int j) { return now[op][j]; });
+            }
+        }
     }
+    __syncthreads();
+    int64_t(*sum)[RT * NT * 64] = reinterpret_cast<int64_t(*)[RT * NT * 64]>(lds);
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
         for (int j = 0; j < NT; j++) sum[wave][(t * NT + j) * 64 + lane] = y[t][j][0] + (int64_t)((uint64_t)y[t][j][1] << 16);
-    __syncthreads();
     for (uint32_t i = threadIdx.x; i < over_words; i += kQ4Threads)
         if (p.over[i]) over_any = 1;
     __syncthreads();
@@ -493,10 +549,10 @@ template <int GS>
 static int q4_launch(const Q4Args& p, hipStream_t s) {
     const uint32_t units = (p.inputs + 127) / 128, tiles = (p.outputs + 15) / 16;
     if (p.tokens <= token::kQ4Few) {
-        const uint32_t piece = std::min(units, (token::kTokenLds - 8192) / (512 * p.tokens));
-        // about sixteen waves a CU, however many tiles there are
-        const uint32_t waves = tiles <= (uint32_t)kNumCU ? 16 : tiles <= 2u * kNumCU ? 8 : 4;
-        wit_q4_few_kernel<GS><<<tiles, 64 * waves, (size_t)piece * 512 * p.tokens, s>>>(p, piece);
+        // a wave for each four units, and no more than fill the chip
+        const uint32_t waves = std::min((units + 3) / 4, tiles <= (uint32_t)kNumCU ? (uint32_t)kQ4MostWaves : 8u);
+        const uint32_t piece = std::min(units, token::kTokenLds / (512 * p.tokens) / 4 * 4);
+        wit_q4_few_kernel<GS><<<tiles, 64 * waves, (size_t)piece * 512 * p.tokens + 4096 * waves, s>>>(p, piece);
         GRAPE_LAUNCH_CHECK();
         return GRAPE_OK;
     }
