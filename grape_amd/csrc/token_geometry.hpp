@@ -214,14 +214,24 @@ inline const char* refuse_attention(const grape_wit_attention_args* a, const gra
 // Products with 4-bit weights: up to this many tokens are taken apart by the workgroups that multiply them; more by a launch of its
 // own, into the workspace, in tiles of eight or sixteen, and one word a block of 2048 inputs of a token says what its digits lack.
 constexpr uint32_t kQ4Few = 4;
-inline uint32_t q4_tile_tokens(uint32_t tokens) { return tokens <= 8 ? 8 : 16; }
-inline size_t q4_digit_words(uint32_t tokens, uint32_t inputs) {
-    const uint32_t tile = q4_tile_tokens(tokens);
-    return (size_t)ceil_div(tokens, tile) * ceil_div(inputs, 128) * 32 * 4 * tile;
+struct Q4Plan {
+    uint32_t tile_tokens, token_tiles;
+    uint32_t makers;                   // workgroups of one token that make digits
+    size_t at_over, bytes;
+};
+inline Q4Plan q4_plan(uint32_t tokens, uint32_t inputs) {
+    Q4Plan p;
+    const uint32_t units = ceil_div(inputs, 128);
+    p.tile_tokens = tokens <= 8 ? 8 : 16;
+    p.token_tiles = ceil_div(tokens, p.tile_tokens);
+    p.makers = ceil_div(units * 16, 256);
+    p.at_over = (size_t)p.token_tiles * units * 32 * 4 * p.tile_tokens * 4;
+    p.bytes = p.at_over + (size_t)4 * tokens * p.makers;
+    return p;
 }
 inline size_t q4_workspace(uint32_t tokens, uint32_t inputs, uint32_t group) {
-    if (tokens <= kQ4Few || !inputs || !group || group % 32) return 0;
-    return 4 * (q4_digit_words(tokens, inputs) + (size_t)tokens * ceil_div(ceil_div(inputs, 128) * 16, 256));
+    if (tokens <= kQ4Few || !inputs || !group || group % 32 || tokens > 65535 || inputs > (uint32_t)1 << 30) return 0;
+    return q4_plan(tokens, inputs).bytes;
 }
 
 inline const char* refuse_q4(const void* d_q, const void* d_x, int64_t x_stride, const void* d_w, int64_t w_stride, const void* d_scales,

@@ -206,7 +206,9 @@ __global__ void __launch_bounds__(kBlock) wit_q4_any_kernel(Q4Args p) {
 // Zero points other than 8 add (8 - z) * sum of digits; one more product, with ones, gives those sums in the same registers.
 // The waves of a workgroup take consecutive shares of a tile of 16 rows' inputs, so that 4096 rows fill the chip; what a wave needs
 // next is requested some units of 128 inputs ahead.
-constexpr int kQ4Waves = 8, kQ4Threads = 64 * kQ4Waves, kQ4MostWaves = 16;
+constexpr int kQ4Waves = 8, kQ4Threads = 64 * kQ4Waves;
+// waves of a workgroup for up to four tokens at most: four scales a lane need the registers of twice as many
+constexpr uint32_t q4_most_waves(int gs) { return gs == 32 ? 8 : 16; }
 
 // Four units of 128 inputs of 16 weight rows.  A wave reads 256 bytes in a row among 16 neighbouring lanes, then turns them over
 // through 4 KB of LDS of its own into the operands, where 16 neighbouring lanes hold 16 rows: read as operands in the first place,
@@ -227,10 +229,13 @@ struct Q4Quad {
                 __builtin_memcpy(&w[i], s + at, 16);
             } else {
                 // the row's last bytes; what follows them meets digits of zero
-                w[i] = v4i_t{0, 0, 0, 0};
-                uint8_t last[16] = {0};
-                for (uint32_t b = 0; at + b < bytes; b++) last[b] = s[at + b];
-                __builtin_memcpy(&w[i], last, 16);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {
+                    uint32_t word = 0;
+#pragma unroll 1
+                    for (uint32_t b = 0; b < 4; b++) word |= (at + 4 * j + b < bytes ? (uint32_t)s[at + 4 * j + b] : 0u) << (8 * b);
+                    w[i][j] = (int)word;
+                }
             }
         }
         const uint32_t row = min(m0 + (lane >> 2), p.outputs - 1), u = unit + (lane & 3u);
@@ -264,6 +269,50 @@ struct Q4Unit {
     static constexpr int STEPS = 128 / GS, CB = GS / 8;
     v4i_t w;
     int32_t scale[STEPS], zero[STEPS];
+    // straight from memory, every lane for itself
+    __device__ __forceinline__ void load(const Q4Args& p, uint32_t row, uint32_t unit, uint32_t kg) {
+        const uint8_t* s = p.w + row * p.w_stride;
+        const uint32_t bytes = (p.inputs + 1) / 2, base = unit * 64;
+        if (base + 64 <= bytes) {
+            union { v4i_t v; uint32_t u[4]; uint2 d[2]; } o;
+#pragma unroll
+            for (int c = 0; c < 16 / CB; c++) {
+                const uint8_t* at = s + base + c * (GS / 2) + kg * CB;
+                if constexpr (CB == 16) __builtin_memcpy(&o.v, at, 16);
+                else if constexpr (CB == 8) __builtin_memcpy(&o.d[c], at, 8);
+                else __builtin_memcpy(&o.u[c], at, 4);
+            }
+            w = o.v;
+        } else {
+            // the row's last bytes; what follows them meets digits of zero
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t word = 0;
+#pragma unroll 1
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t b = 4 * c + i, at = base + b / CB * (GS / 2) + kg * CB + b % CB;
+                    word |= (at < bytes ? (uint32_t)s[at] : 0u) << (8 * i);
+                }
+                w[c] = (int)word;
+            }
+        }
+        const size_t first = (size_t)row * p.groups;
+        if (p.group == GS && (unit + 1) * STEPS <= p.groups) {          // neighbours
+            __builtin_memcpy(scale, p.scales + first + unit * STEPS, 4 * STEPS);
+            uint8_t z[STEPS];
+            if (p.zeros) __builtin_memcpy(z, p.zeros + first + unit * STEPS, STEPS);
+#pragma unroll
+            for (int st = 0; st < STEPS; st++) zero[st] = p.zeros ? z[st] : 8;
+            return;
+        }
+#pragma unroll
+        for (int st = 0; st < STEPS; st++) {
+            const uint32_t g = min(p.by_group(unit * 128 + st * GS), p.groups - 1);
+            scale[st] = p.scales[first + g];
+            zero[st] = p.zeros ? (int32_t)p.zeros[first + g] : 8;
+        }
+    }
+    // from four units that have been turned over
     __device__ __forceinline__ void take(const Q4Quad<GS>& q, const uint8_t* lds, uint32_t s, uint32_t lane, bool zeros) {
         const uint32_t r = lane & 15u, kg = lane >> 4;
         union { v4i_t v; uint32_t u[4]; uint2 d[2]; } o;
@@ -343,29 +392,48 @@ __device__ __forceinline__ void q4_unit(const Q4Unit<GS>& x, bool zeros, int64_t
     const v4i_t none = {0, 0, 0, 0}, one = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
 #pragma unroll
     for (int st = 0; st < 128 / GS; st++) {
+        // all tiles' products before the first one's sums are looked at
+        v4i_t acc[NT], ones[NT];
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[j] = ones[j] = none;
+        if constexpr (GS == 32) {
+            const long w = (long)(((uint64_t)(uint32_t)odd[st] << 32) | (uint32_t)even[st]);
+            long d[NT];
+#pragma unroll
+            for (int j = 0; j < NT; j++) d[j] = operand(st, j);
+#pragma unroll
+            for (int j = 0; j < NT; j++) acc[j] = __builtin_amdgcn_mfma_i32_16x16x32_i8(d[j], w, acc[j], 0, 0, 0);
+            if (zeros) {
+#pragma unroll
+                for (int j = 0; j < NT; j++) ones[j] = __builtin_amdgcn_mfma_i32_16x16x32_i8(d[j], 0x0101010101010101L, ones[j], 0, 0, 0);
+            }
+        } else {
+            v4i_t d[GS / 64][NT];
+#pragma unroll
+            for (int op = 0; op < GS / 64; op++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) d[op][j] = operand(st + op, j);
+#pragma unroll
+            for (int op = 0; op < GS / 64; op++) {
+                v4i_t w;
+                if constexpr (GS == 128) w = op ? odd : even;
+                else w = v4i_t{even[2 * st], even[2 * st + 1], odd[2 * st], odd[2 * st + 1]};
+#pragma unroll
+                for (int j = 0; j < NT; j++) acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(d[op][j], w, acc[j], 0, 0, 0);
+            }
+            if (zeros) {
+#pragma unroll
+                for (int op = 0; op < GS / 64; op++)
+#pragma unroll
+                    for (int j = 0; j < NT; j++) ones[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(d[op][j], one, ones[j], 0, 0, 0);
+            }
+        }
+        const int32_t up = 8 - x.zero[st];
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-            v4i_t acc = none, ones = none;
-            if constexpr (GS == 32) {
-                const long d = operand(st, j);
-                const long w = (long)(((uint64_t)(uint32_t)odd[st] << 32) | (uint32_t)even[st]);
-                acc = __builtin_amdgcn_mfma_i32_16x16x32_i8(d, w, acc, 0, 0, 0);
-                if (zeros) ones = __builtin_amdgcn_mfma_i32_16x16x32_i8(d, 0x0101010101010101L, ones, 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int op = 0; op < GS / 64; op++) {
-                    const v4i_t d = operand(st + op, j);
-                    v4i_t w;
-                    if constexpr (GS == 128) w = op ? odd : even;
-                    else w = v4i_t{even[2 * st], even[2 * st + 1], odd[2 * st], odd[2 * st + 1]};
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(d, w, acc, 0, 0, 0);
-                    if (zeros) ones = __builtin_amdgcn_mfma_i32_16x16x64_i8(d, one, ones, 0, 0, 0);
-                }
-            }
-            const int32_t up = 8 - x.zero[st];
             int32_t s[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[i] = (acc[i] >> 4) + (zeros ? up * ones[i] : 0);
+            for (int i = 0; i < 4; i++) s[i] = (acc[j][i] >> 4) + (zeros ? __mul24(up, ones[j][i]) : 0);
             y[j][0] += (int64_t)(s[0] + 256 * s[1]) * x.scale[st];
             y[j][1] += (int64_t)(s[2] + 256 * s[3]) * x.scale[st];
         }
@@ -396,7 +464,7 @@ __device__ __forceinline__ void q4_out(const Q4Args& p, uint32_t n, uint32_t m, 
 // Up to four tokens: a workgroup makes their digits itself, in LDS (a longer input goes through in pieces), while its first weights
 // are under way.  blockDim: as many waves as share a tile's inputs, 4 KB of LDS each behind the digits.
 template <int GS>
-__global__ void __launch_bounds__(64 * kQ4MostWaves, 4) wit_q4_few_kernel(Q4Args p, uint32_t piece) {
+__global__ void __launch_bounds__(64 * q4_most_waves(GS), GS == 32 ? 2 : 4) wit_q4_few_kernel(Q4Args p, uint32_t piece) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ uint32_t over_any;
     constexpr int OPS = GS == 32 ? 4 : 2;
@@ -452,7 +520,9 @@ __global__ void __launch_bounds__(64 * kQ4MostWaves, 4) wit_q4_few_kernel(Q4Args
 }
 
 // More tokens: their digits are made once, by a launch of its own, and read from L2 as operands, 4 NT tokens at a time for RT tiles
-// of 16 rows.
+// of 16 rows.  For 16 tokens through 4096 x 11008 those are 180 MB at 12 TB/s, which bounds it (14.7 us, of which reading the weights
+// would take 5).  Digits in LDS for 128 rows at a time ask for 22 MB instead, but leave a workgroup a CU of which each waits for
+// its next weights, and sums to be joined: 14.8 and 3.9 us.
 template <int GS>
 __global__ void __launch_bounds__(kBlock) wit_q4_digits_kernel(Q4Args p, uint32_t tile_tokens) {
     __shared__ uint32_t over;
@@ -467,68 +537,51 @@ __global__ void __launch_bounds__(kBlock) wit_q4_digits_kernel(Q4Args p, uint32_
 
 template <int GS, int NT, int RT>
 __global__ void __launch_bounds__(kQ4Threads, 2) wit_q4_many_kernel(Q4Args p, uint32_t over_words) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kQ4Waves * RT * 4096];
+    constexpr int kQ4ManyAhead = GS == 32 ? 1 : 2;
+    __shared__ int64_t sum[kQ4Waves][RT * NT * 64];
     __shared__ uint32_t over_any;
     constexpr int OPS = GS == 32 ? 4 : 2;
     constexpr uint32_t COLS = 16 * NT;
-    static_assert(sizeof lds >= sizeof(int64_t) * kQ4Waves * RT * NT * 64, "the sums fit where the weights were turned over");
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, kg = lane >> 4;
     const uint32_t units = (p.inputs + 127) / 128, m0 = blockIdx.x * 16 * RT, n0 = blockIdx.y * 4 * NT;
     const uint32_t* digits = p.digits + (size_t)blockIdx.y * units * 32 * COLS;
-    uint8_t* turned = lds + wave * RT * 4096;
     if (threadIdx.x == 0) over_any = 0;
     int64_t y[RT][NT][2];
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
         for (int j = 0; j < NT; j++) y[t][j][0] = y[t][j][1] = 0;
-    const uint32_t share = ((units + kQ4Waves - 1) / kQ4Waves + 3) / 4 * 4, first = min(wave * share, units), last = min(first + share, units);
-    Q4Quad<GS> next[RT];
+    const uint32_t share = (units + kQ4Waves - 1) / kQ4Waves, first = min(wave * share, units), last = min(first + share, units);
+    Q4Unit<GS> next[kQ4ManyAhead][RT];
 #pragma unroll
-    for (int t = 0; t < RT; t++)
-        if (first < last) next[t].load(p, m0 + 16 * t, first, lane);
-    typedef typename std::conditional<GS == 32, long, v4i_t>::type operand_t;
-    operand_t d[OPS][NT];                                    // the next unit's digits
-    auto fetch = [&](uint32_t u) {
+    for (int s = 0; s < kQ4ManyAhead; s++)
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+            if (first + s < last) next[s][t].load(p, min(m0 + 16 * t + col, p.outputs - 1), first + s, kg);
+#pragma unroll 1
+    for (uint32_t u = first; u < last; u++) {
+        typedef typename std::conditional<GS == 32, long, v4i_t>::type operand_t;
+        operand_t d[OPS][NT];
 #pragma unroll
         for (int op = 0; op < OPS; op++)
 #pragma unroll
             for (int j = 0; j < NT; j++) d[op][j] = reinterpret_cast<const operand_t*>(digits)[(((size_t)u * OPS + op) * 4 + kg) * COLS + 16 * j + col];
-    };
-    if (first < last) fetch(first);
-#pragma unroll 1
-    for (uint32_t u = first; u < last; u += 4) {
-        Q4Quad<GS> quad[RT];
-        wave_sync();
+        Q4Unit<GS> x[RT];
 #pragma unroll
         for (int t = 0; t < RT; t++) {
-            quad[t] = next[t];
-            quad[t].store(turned + 4096 * t, lane);
-            if (u + 4 < last) next[t].load(p, m0 + 16 * t, u + 4, lane);
+            x[t] = next[0][t];
+#pragma unroll
+            for (int s = 0; s + 1 < kQ4ManyAhead; s++) next[s][t] = next[s + 1][t];
+            if (u + kQ4ManyAhead < last) next[kQ4ManyAhead - 1][t].load(p, min(m0 + 16 * t + col, p.outputs - 1), u + kQ4ManyAhead, kg);
         }
-        wave_sync();
-#pragma unroll 1
-        for (uint32_t s = 0; s < 4 && u + s < last; s++) {
-            operand_t now[OPS][NT];
 #pragma unroll
-            for (int op = 0; op < OPS; op++)
-#pragma unroll
-                for (int j = 0; j < NT; j++) now[op][j] = d[op][j];
-            if (u + s + 1 < last) fetch(u + s + 1);
-#pragma unroll
-            for (int t = 0; t < RT; t++) {
-                Q4Unit<GS> x;
-                x.take(quad[t], turned + 4096 * t, s, lane, p.zeros != nullptr);
-                q4_unit<GS, NT>(x, p.zeros != nullptr, y[t], [&](int op, int j) { return now[op][j]; });
-            }
-        }
+        for (int t = 0; t < RT; t++) q4_unit<GS, NT>(x[t], p.zeros != nullptr, y[t], [&](int op, int j) { return d[op][j]; });
     }
-    __syncthreads();
-    int64_t(*sum)[RT * NT * 64] = reinterpret_cast<int64_t(*)[RT * NT * 64]>(lds);
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
         for (int j = 0; j < NT; j++) sum[wave][(t * NT + j) * 64 + lane] = y[t][j][0] + (int64_t)((uint64_t)y[t][j][1] << 16);
+    __syncthreads();
     for (uint32_t i = threadIdx.x; i < over_words; i += kQ4Threads)
         if (p.over[i]) over_any = 1;
     __syncthreads();
@@ -549,28 +602,28 @@ template <int GS>
 static int q4_launch(const Q4Args& p, hipStream_t s) {
     const uint32_t units = (p.inputs + 127) / 128, tiles = (p.outputs + 15) / 16;
     if (p.tokens <= token::kQ4Few) {
-        // a wave for each four units, and no more than fill the chip
-        const uint32_t waves = std::min((units + 3) / 4, tiles <= (uint32_t)kNumCU ? (uint32_t)kQ4MostWaves : 8u);
+        // a wave for each four units of 128 inputs, and no more than sixteen a CU where that leaves four
+        uint32_t waves = std::min((units + 3) / 4, std::min(q4_most_waves(GS), std::max(4u, 16u * kNumCU / tiles)));
+        const uint32_t share = ((units + waves - 1) / waves + 3) / 4 * 4;
+        waves = (units + share - 1) / share;
         const uint32_t piece = std::min(units, token::kTokenLds / (512 * p.tokens) / 4 * 4);
         wit_q4_few_kernel<GS><<<tiles, 64 * waves, (size_t)piece * 512 * p.tokens + 4096 * waves, s>>>(p, piece);
         GRAPE_LAUNCH_CHECK();
         return GRAPE_OK;
     }
-    const uint32_t tile_tokens = token::q4_tile_tokens(p.tokens);
-    const dim3 makers((units * 16 + kBlock - 1) / kBlock, p.tokens);
-    wit_q4_digits_kernel<GS><<<makers, kBlock, 0, s>>>(p, tile_tokens);
+    const token::Q4Plan plan = token::q4_plan(p.tokens, p.inputs);
+    wit_q4_digits_kernel<GS><<<dim3(plan.makers, p.tokens), kBlock, 0, s>>>(p, plan.tile_tokens);
     GRAPE_LAUNCH_CHECK();
-    const uint32_t over_words = makers.x * p.tokens, token_tiles = (p.tokens + tile_tokens - 1) / tile_tokens;
-    // two tiles of rows share the digits where that still leaves a workgroup for each CU
-    const bool two = (uint64_t)(tiles + 1) / 2 * token_tiles >= (uint64_t)kNumCU;
-    const dim3 grid(two ? (tiles + 1) / 2 : tiles, token_tiles);
-    if (tile_tokens == 8) {
-        if (two) wit_q4_many_kernel<GS, 2, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
-        else wit_q4_many_kernel<GS, 2, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
-    } else {
-        if (two) wit_q4_many_kernel<GS, 4, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
-        else wit_q4_many_kernel<GS, 4, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+    const uint32_t over_words = plan.makers * p.tokens;
+    // two tiles of rows share the digits where that still leaves a workgroup for each CU (and the registers are enough)
+    const bool two = GS > 32 && (uint64_t)(tiles + 1) / 2 * plan.token_tiles >= (uint64_t)kNumCU;
+    const dim3 grid(two ? (tiles + 1) / 2 : tiles, plan.token_tiles);
+    if constexpr (GS > 32) {
+        if (two && plan.tile_tokens == 8) wit_q4_many_kernel<GS, 2, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+        else if (two) wit_q4_many_kernel<GS, 4, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
     }
+    if (!two && plan.tile_tokens == 8) wit_q4_many_kernel<GS, 2, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+    else if (!two) wit_q4_many_kernel<GS, 4, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
     GRAPE_LAUNCH_CHECK();
     return GRAPE_OK;
 }
@@ -631,7 +684,7 @@ int grape_wit_matvec_q4(int32_t* d_q, int32_t* d_r, const int32_t* d_x, int64_t 
     p.by_group = token::fast_div(group);
     p.scale = scaler(scale);
     p.digits = (uint32_t*)d_workspace;
-    p.over = p.digits + token::q4_digit_words(tokens, inputs);
+    p.over = (uint32_t*)((uint8_t*)d_workspace + token::q4_plan(tokens, inputs).at_over);
     hipStream_t s = as_stream(st);
     const int rc = wit_status_word(&p.status, s);
     if (rc) return rc;

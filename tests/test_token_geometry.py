@@ -191,10 +191,10 @@ def test_plans_cover_every_position_within_their_limits(lib):
 
 def test_workspace_sizes(lib):
     assert lib.q4_workspace(4, 4096, 128) == 0 and lib.q4_workspace(9, 4096, 100) == 0 and lib.q4_workspace(9, 0, 32) == 0
-    for n, k in ((5, 1), (8, 128), (9, 129), (16, 11008), (17, 2049), (40, 4095)):
-        tile = 8 if n <= 8 else 16
-        digits = -(-n // tile) * tile * 4 * -(-k // 128) * 128                            # a byte an input and plane, whole units
-        assert lib.q4_workspace(n, k, 32) == digits + 4 * n * -(-(-(-k // 128) * 16) // 256)
+    for n, k in ((5, 1), (8, 128), (9, 129), (16, 11008), (17, 2049), (40, 4095), (65535, 1 << 16)):
+        tile, units = 8 if n <= 8 else 16, -(-k // 128)
+        # a byte an input and plane, whole units and tiles of tokens, and a word a token and 2048 inputs
+        assert lib.q4_workspace(n, k, 32) == -(-n // tile) * tile * 4 * units * 128 + 4 * n * -(-units // 16)
     assert lib.workspace(0, 8, 8, 64, 100) == 0 and lib.workspace(65536, 8, 8, 64, 100) == 0 and lib.workspace(60000, 60000, 1, 64, 100000) == 0
     assert lib.workspace(1, 8, 2, 64, 1000) >= 4 * 8 * 1000
 
