@@ -283,61 +283,62 @@ __device__ __forceinline__ int32_t lookup_query(uint32_t e, int64_t scale, uint6
     return (int32_t)((uint64_t)e * 2 * (uint64_t)scale - sum * (2 * (uint64_t)prob - 1));
 }
 
-// Digits of four positions' probabilities in LDS: [step of 32][plane][lane group][row], operands of 8 positions each.
-template <int PP>                    // planes of the probabilities
-__device__ __forceinline__ void store_probabilities(const uint32_t pr[4], uint32_t quad, uint32_t r, uint32_t R, uint32_t* digits) {
-    uint32_t pl[4];
-    transpose4(digits_of((int32_t)pr[0]), digits_of((int32_t)pr[1]), digits_of((int32_t)pr[2]), digits_of((int32_t)pr[3]), pl);
-    uint32_t* out = digits + ((((quad >> 3) * PP * 4 + ((quad >> 1) & 3u)) * R + r) << 1) + (quad & 1u);
-#pragma unroll
-    for (int k = 0; k < PP; k++) out[k * 8 * R] = pl[k];
-}
+// The threads of a workgroup that share a query head: as many as there are for each, a power of two, in lanes side by side.
+struct RowThreads {
+    uint32_t each, r, from, lanes;
+    bool mine, leads;            // of a row that there is; the first of its lanes in a wave
+    __device__ __forceinline__ RowThreads(uint32_t threads, uint32_t R) {
+        each = threads;
+        while (each * R > threads) each >>= 1;
+        r = threadIdx.x / each;
+        from = threadIdx.x - r * each;
+        lanes = min(each, 64u);
+        mine = r < R;
+        leads = threadIdx.x % lanes == 0;
+    }
+    template <class T, class F>
+    __device__ __forceinline__ T all(T v, F f) const {
+        for (uint32_t k = lanes / 2; k >= 1; k >>= 1) v = f(v, __shfl_xor(v, k, 64));
+        return v;
+    }
+};
 
-// Probabilities of n positions of row r from their exponentials, written if `write`, and their digits in LDS, zero up to a whole
-// number of 64 positions and for pages outside the cache.  A wave a row; returns the sum of the probabilities that the values are multiplied with.
-constexpr uint32_t kProbAhead = 2;   // four positions each under way a lane
-template <int PP>
-__device__ __forceinline__ unsigned long long probabilities(const AttendArgs& p, const Tile& w, uint32_t r, uint32_t t0, uint32_t n, const int64_t* off,
-                                                            unsigned long long sum, bool write, uint32_t* digits) {
-    const size_t o = (w.row0 + r) * p.a.max_len + t0;
+// Probabilities of this thread's positions of its row, from load(position), its exponential; written if `write`, and their digits
+// in LDS: [step of 32][plane][lane group][row], operands of 8 positions each, zero up to a whole number of 32 positions and for
+// pages outside the cache.  Returns the sum of the probabilities that the values are multiplied with.
+template <int PP, uint32_t AHEAD, class F>          // planes of the probabilities, positions under way a thread
+__device__ __forceinline__ unsigned long long probabilities(const AttendArgs& p, const Tile& w, const RowThreads& row, uint32_t t0, uint32_t n, const int64_t* off,
+                                                            unsigned long long sum, bool write, uint32_t* digits, F load) {
+    const size_t o = (w.row0 + row.r) * p.a.max_len + t0;
     const double inv = 1.0 / (double)sum;
-    const uint32_t quads = (n + 63) / 64 * 16;
-    unsigned long long mine = 0;
-    for (uint32_t first = w.lane; first < quads; first += 64 * kProbAhead) {
-        int32_t ex[kProbAhead][4];
+    const uint32_t filled = (n + 31) / 32 * 32;
+    unsigned long long all = 0;
+#pragma unroll 1
+    for (uint32_t first = row.from; first < filled; first += AHEAD * row.each) {
+        uint32_t e[AHEAD];
 #pragma unroll
-        for (uint32_t a = 0; a < kProbAhead; a++)
+        for (uint32_t a = 0; a < AHEAD; a++) e[a] = first + a * row.each < n ? load(first + a * row.each) : 0;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t i = 4 * (first + 64 * a) + j;
-                ex[a][j] = i < n ? p.a.d_exp[o + i] : 0;
-            }
-#pragma unroll
-        for (uint32_t a = 0; a < kProbAhead; a++) {
-            const uint32_t quad = first + 64 * a;
-            if (quad >= quads) break;
-            uint32_t pr[4];
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t i = 4 * quad + j;
-                pr[j] = 0;
-                if (i < n) {
-                    const uint32_t ev = ex[a][j] < 0 ? 0 : (uint32_t)ex[a][j];
-                    pr[j] = probability(ev, (uint64_t)p.a.prob_scale, sum, inv);
-                    if (write) {
-                        if (p.a.d_prob) p.a.d_prob[o + i] = (int32_t)pr[j];
-                        if (p.a.d_query) p.a.d_query[o + i] = lookup_query(ev, p.a.prob_scale, sum, pr[j]);
-                    }
-                    if (off[i] < 0) pr[j] = 0;
+        for (uint32_t a = 0; a < AHEAD; a++) {
+            const uint32_t i = first + a * row.each;
+            if (i >= filled) break;
+            uint32_t pr = 0;
+            if (i < n) {
+                pr = probability(e[a], (uint64_t)p.a.prob_scale, sum, inv);
+                if (write) {
+                    if (p.a.d_prob) p.a.d_prob[o + i] = (int32_t)pr;
+                    if (p.a.d_query) p.a.d_query[o + i] = lookup_query(e[a], p.a.prob_scale, sum, pr);
                 }
-                mine += pr[j];
+                if (off[i] < 0) pr = 0;
             }
-            store_probabilities<PP>(pr, quad, r, w.R, digits);
+            all += pr;
+            const uint32_t d = digits_of((int32_t)pr);
+            uint8_t* out = reinterpret_cast<uint8_t*>(digits) + ((((i >> 5) * PP * 4 + ((i >> 3) & 3u)) * w.R + row.r) << 3) + (i & 7u);
+#pragma unroll
+            for (int k = 0; k < PP; k++) out[k * 32 * w.R] = (uint8_t)(d >> (8 * k));
         }
     }
-#pragma unroll
-    for (int k = 32; k >= 1; k >>= 1) mine += __shfl_xor(mine, k, 64);
-    return mine;
+    return row.all(all, [](unsigned long long x, unsigned long long y) { return x + y; });
 }
 
 // Products of the probabilities with 32 elements (from e) of n values.  A wave takes 32 positions a step: lane l reads the
@@ -505,10 +506,11 @@ __global__ void __launch_bounds__(kBlock) wit_attend_exp_kernel(AttendArgs p) {
 
 // Probabilities of a chunk of the positions for `rows` query heads, and their products with 32 * blocks elements of the values.
 // The waves take different blocks of 32 elements, or every second or fourth step.  Bound by reading the values.
+constexpr uint32_t kProbAhead = 4;
 template <bool VEC, int PP>
 __global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
-    __shared__ unsigned long long p_sum[16];
+    __shared__ unsigned long long e_sum[16], p_sum[16];
     const uint32_t per_chunk = p.c.heads * p.plan.tiles * p.plan.groups, chunk = blockIdx.x / per_chunk, within = blockIdx.x - chunk * per_chunk;
     const uint32_t group = within % p.plan.groups;
     const Tile w(p, blockIdx.y, within / p.plan.groups);
@@ -525,26 +527,32 @@ __global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p)
     }
     const uint32_t t0 = (uint32_t)start, n = min(hi - t0, p.plan.value_chunk);
     int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)p.plan.value_chunk * w.R * PP / 4);        // behind the digits
-    if (threadIdx.x < 16) p_sum[threadIdx.x] = 0;
+    if (threadIdx.x < 16) e_sum[threadIdx.x] = p_sum[threadIdx.x] = 0;
     offsets.store(p, w.b, t0, n, (n + 63) / 64 * 64, off);
     __syncthreads();
     const uint32_t block = w.wave % p.plan.blocks, apart = 4 / p.plan.blocks, e = e0 + 32 * block, halves = e < dim ? (n + 31) / 32 : 0, s = w.wave / p.plan.blocks;
     ValueProducts<VEC, PP> products;
     if (s < halves) products.fetch(p, w, off, e, s);            // under way while the probabilities are computed
     const uint32_t parts = (hi - lo - 1) / p.plan.exp_chunk + 1;
-    for (uint32_t r = w.wave; r < w.R; r += 4) {
-        const size_t row = w.row0 + r;
+    const RowThreads row(256, w.R);
+    const size_t at = w.row0 + min(row.r, w.R - 1);
+    if (row.mine) {
         unsigned long long sum = 0;
-        for (uint32_t i = w.lane; i < parts; i += 64) sum += p.sums[row * p.plan.exp_chunks + i];
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        for (uint32_t i = row.from; i < parts; i += row.each) sum += p.sums[at * p.plan.exp_chunks + i];
+        sum = row.all(sum, [](unsigned long long x, unsigned long long y) { return x + y; });
+        if (row.leads) atomicAdd(&e_sum[row.r], sum);
+    }
+    __syncthreads();
+    if (row.mine) {
+        unsigned long long sum = e_sum[row.r];
         if (sum == 0) {
             bad |= (uint32_t)kWitSum;
             sum = 1;
         }
-        if (chunk == 0 && group == 0 && w.lane == 0 && p.a.d_sum) p.a.d_sum[row] = (int32_t)sum;
-        const unsigned long long mine = probabilities<PP>(p, w, r, t0, n, off, sum, group == 0, lds);
-        if (w.lane == 0) p_sum[r] = mine;
+        if (chunk == 0 && group == 0 && row.from == 0 && p.a.d_sum) p.a.d_sum[at] = (int32_t)sum;
+        const int32_t* exps = p.a.d_exp + at * p.a.max_len + t0;
+        const unsigned long long mine = probabilities<PP, kProbAhead>(p, w, row, t0, n, off, sum, group == 0, lds, [&](uint32_t i) { return (uint32_t)max(exps[i], 0); });
+        if (row.leads) atomicAdd(&p_sum[row.r], mine);
     }
     __syncthreads();
     products.clear();
@@ -632,15 +640,13 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
         if (there) total[r * C + i] = y;
     });
     // the values' first step is under way during the softmax
-    const uint32_t blocks = p.plan.blocks, apart = kWholeWaves / blocks, block = w.wave % blocks, s = w.wave / blocks, halves = (n + 31) / 32;
+    const uint32_t dim32 = (dim + 31) / 32, blocks = dim32 > 4 ? 8 : dim32 > 2 ? 4 : dim32, apart = kWholeWaves / blocks, block = w.wave % blocks, s = w.wave / blocks, halves = (n + 31) / 32;
     ValueProducts<VEC, PP> products;
     if (32 * block < dim && s < halves) products.fetch(p, w, off, 32 * block, s);
     __syncthreads();
-    // as many threads a row as there are for each, a power of two
-    uint32_t each = kWholeThreads;
-    while (each * w.R > kWholeThreads) each >>= 1;
-    const uint32_t r = threadIdx.x / each, from = threadIdx.x - r * each, lanes = min(each, 64u);
-    const bool mine = r < w.R, leads = threadIdx.x % lanes == 0;
+    const RowThreads row(kWholeThreads, w.R);
+    const uint32_t r = row.r, from = row.from, each = row.each;
+    const bool mine = row.mine, leads = row.leads;
     const size_t o = (w.row0 + min(r, w.R - 1)) * p.a.max_len + lo;
     if (mine) {
         const uint64_t more = (uint64_t)kCacheOffset * q_sum[r];
@@ -654,7 +660,7 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
             scores[r * C + i] = (uint32_t)q;
             mx = max(mx, q);
         }
-        for (uint32_t k = lanes / 2; k >= 1; k >>= 1) mx = max(mx, __shfl_xor(mx, k, 64));
+        mx = row.all(mx, [](int32_t x, int32_t y) { return max(x, y); });
         if (leads) atomicMax(&row_max[r], mx);
     }
     __syncthreads();
@@ -685,12 +691,12 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
                 sum += (uint32_t)e[a];
             }
         }
-        for (uint32_t k = lanes / 2; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, 64);
+        sum = row.all(sum, [](unsigned long long x, unsigned long long y) { return x + y; });
         if (leads) atomicAdd(&e_sum[r], sum);
     }
     __syncthreads();
     if (mine) {
-        unsigned long long sum = e_sum[r], all = 0;
+        unsigned long long sum = e_sum[r];
         if (sum == 0) {
             bad |= (uint32_t)kWitSum;
             sum = 1;
@@ -699,31 +705,12 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
             if (p.a.d_max) p.a.d_max[w.row0 + r] = row_max[r];
             if (p.a.d_sum) p.a.d_sum[w.row0 + r] = (int32_t)sum;
         }
-        const double inv = 1.0 / (double)sum;
-#pragma unroll 1
-        for (uint32_t i = from; i < filled; i += each) {
-            uint32_t pr = 0;
-            if (i < n) {
-                const uint32_t e = scores[r * C + i];
-                pr = probability(e, (uint64_t)p.a.prob_scale, sum, inv);
-                if (p.a.d_prob) p.a.d_prob[o + i] = (int32_t)pr;
-                if (p.a.d_query) p.a.d_query[o + i] = lookup_query(e, p.a.prob_scale, sum, pr);
-                if (off[i] < 0) pr = 0;
-            }
-            all += pr;
-            const uint32_t d = digits_of((int32_t)pr);
-            uint8_t* out = reinterpret_cast<uint8_t*>(digits) + ((((i >> 5) * PP * 4 + ((i >> 3) & 3u)) * w.R + r) << 3) + (i & 7u);
-#pragma unroll
-            for (int k = 0; k < PP; k++) out[k * 32 * w.R] = (uint8_t)(d >> (8 * k));
-        }
-        for (uint32_t k = lanes / 2; k >= 1; k >>= 1) all += __shfl_xor(all, k, 64);
+        const unsigned long long all = probabilities<PP, 1>(p, w, row, lo, n, off, sum, true, digits, [&](uint32_t i) { return scores[r * C + i]; });
         if (leads) atomicAdd(&p_sum[r], all);
     }
     __syncthreads();
-    for (uint32_t g = 0; g < p.plan.groups; g++) {
-        const uint32_t el = 32 * (g * blocks + block);
-        if (el >= dim || s >= halves) break;
-        if (g) products.fetch(p, w, off, el, s);
+    for (uint32_t el = 32 * block; el < dim && s < halves; el += 32 * blocks) {
+        if (el != 32 * block) products.fetch(p, w, off, el, s);
         products.clear();
         products.run(p, w, off, digits, el, s, apart, halves);
         products.add(w, total, dim, el);
