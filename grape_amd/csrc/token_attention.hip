@@ -173,10 +173,9 @@ __device__ __forceinline__ void score_products(const AttendArgs& p, const Tile& 
         for (uint32_t s = apart ? 2 * w.wave : 0; s < steps; s += apart ? 2 * WAVES : 2) {
             v4i_t x[8];
 #pragma unroll
-            for (uint32_t c = 0; c < 4; c++) x[c] = load4<VEC>(k, 64 * s + 16 * c + 4 * w.kg, dim);
-            if (s + 1 < steps) {
-#pragma unroll
-                for (uint32_t c = 4; c < 8; c++) x[c] = load4<VEC>(k, 64 * s + 16 * c + 4 * w.kg, dim);
+            for (uint32_t c = 0; c < 8; c++) {
+                x[c] = v4i_t{0, 0, 0, 0};
+                if (64 * s + 16 * c < dim) x[c] = load4<VEC>(k, 64 * s + 16 * c + 4 * w.kg, dim);
             }
 #pragma unroll
             for (uint32_t u = 0; u < 2; u++) {
