@@ -733,8 +733,7 @@ def wit_rmsnorm_apply(x, rms, w, scale=1 << 16):
 
 # ------------------------------------------------------------------ the witness of new tokens
 # These calls are small and many, so their checks are written to cost little: no message is made before it is needed.
-def _place():
-    return torch.cuda.current_device()
+_place = torch.cuda.current_device
 
 
 def _stream(dev):
@@ -755,14 +754,12 @@ def _arr(t, name, shape, dev, dtype=torch.int32):
 
 
 def _rows(t, name, shape, dev, dtype=torch.int32):
-    """the same for rows (all but the first axis) that are contiguous each; address and elements from row to row"""
+    """the same for rows (all but the first of two or three axes) that are contiguous each; address and elements from row to row"""
     if t.dtype is not dtype or t.shape != shape or t.get_device() != dev:
         _refuse("%s must be a %s tensor of shape %s on the current device", name, dtype, tuple(shape))
-    st, step = t.stride(), 1
-    for i in range(len(shape) - 1, 0, -1):
-        if st[i] != step and shape[i] > 1:
-            _refuse("the rows of %s must be contiguous", name)
-        step *= shape[i]
+    st, last = t.stride(), shape[-1]
+    if (st[-1] != 1 and last > 1) or (len(st) == 3 and st[1] != last and shape[1] > 1):
+        _refuse("the rows of %s must be contiguous", name)
     return t.data_ptr(), st[0]
 
 
