@@ -17,7 +17,7 @@ namespace grape {
 // of planes with the same sum of exponents share an accumulator: 4 * 2^14 * 8192 elements (1024 positions) stay below 2^31.
 // ------------------------------------------------------------------------------------------------
 constexpr int64_t kCacheOffset = 0x808080;
-constexpr uint32_t kByteTops = 0x00808080;
+constexpr uint32_t kByteTops = 0x80808080;          // of a plane's four bytes
 
 struct AttendArgs {
     grape_wit_attention_args a;
@@ -174,8 +174,8 @@ __device__ __forceinline__ void score_products(const AttendArgs& p, const Tile& 
             v4i_t x[8];
 #pragma unroll
             for (uint32_t c = 0; c < 8; c++) {
-                x[c] = v4i_t{0, 0, 0, 0};
                 if (64 * s + 16 * c < dim) x[c] = load4<VEC>(k, 64 * s + 16 * c + 4 * w.kg, dim);
+                else x[c] = v4i_t{0, 0, 0, 0};
             }
 #pragma unroll
             for (uint32_t u = 0; u < 2; u++) {
@@ -185,9 +185,9 @@ __device__ __forceinline__ void score_products(const AttendArgs& p, const Tile& 
                 for (int c = 0; c < 4; c++) {
                     const v4i_t y = x[4 * u + c];
                     uint32_t pl[4];
-                    transpose4((uint32_t)y[0] ^ kByteTops, (uint32_t)y[1] ^ kByteTops, (uint32_t)y[2] ^ kByteTops, (uint32_t)y[3] ^ kByteTops, pl);
+                    transpose4((uint32_t)y[0], (uint32_t)y[1], (uint32_t)y[2], (uint32_t)y[3], pl);
 #pragma unroll
-                    for (int k2 = 0; k2 < 4; k2++) kb[k2][c] = (int)pl[k2];
+                    for (int k2 = 0; k2 < 4; k2++) kb[k2][c] = (int)(k2 < 3 ? pl[k2] ^ kByteTops : pl[k2]);
                 }
                 const v4i_t* qa = reinterpret_cast<const v4i_t*>(digits) + ((s + u) * 5 * 4 + w.kg) * R + row;
 #pragma unroll
@@ -376,8 +376,10 @@ struct ValueProducts {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 uint32_t p0[4], p1[4];
-                transpose4((uint32_t)x[0][j] ^ kByteTops, (uint32_t)x[1][j] ^ kByteTops, (uint32_t)x[2][j] ^ kByteTops, (uint32_t)x[3][j] ^ kByteTops, p0);
-                transpose4((uint32_t)x[4][j] ^ kByteTops, (uint32_t)x[5][j] ^ kByteTops, (uint32_t)x[6][j] ^ kByteTops, (uint32_t)x[7][j] ^ kByteTops, p1);
+                transpose4((uint32_t)x[0][j], (uint32_t)x[1][j], (uint32_t)x[2][j], (uint32_t)x[3][j], p0);
+                transpose4((uint32_t)x[4][j], (uint32_t)x[5][j], (uint32_t)x[6][j], (uint32_t)x[7][j], p1);
+#pragma unroll
+                for (int k2 = 0; k2 < 3; k2++) p0[k2] ^= kByteTops, p1[k2] ^= kByteTops;
 #pragma unroll
                 for (int k2 = 0; k2 < 4; k2++) {
                     const long vb = (long)(((uint64_t)p1[k2] << 32) | p0[k2]);
