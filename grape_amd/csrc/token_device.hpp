@@ -16,23 +16,24 @@ struct Scaler {
     double inv;
     int sh;
     __device__ __forceinline__ void apply(int64_t y, int32_t& q, int32_t& r, uint32_t& bad) const {
-        const int64_t t = y + (s >> 1);
+        const int64_t t = (int64_t)((uint64_t)y + (uint64_t)(s >> 1));
         int64_t qq;
         if (sh >= 0) {
             qq = t >> sh;
         } else {
+            auto left = [&]() { return (int64_t)((uint64_t)t - (uint64_t)qq * (uint64_t)s); };
             qq = (int64_t)floor((double)t * inv);
-            int64_t rest = t - qq * s;
+            int64_t rest = left();
             if (rest < 0 || rest >= s) {
                 qq += (int64_t)floor((double)rest * inv);
-                rest = t - qq * s;
+                rest = left();
                 if (rest < 0) qq--;
                 else if (rest >= s) qq++;
             }
         }
         bad |= (qq != (int64_t)(int32_t)qq) ? (uint32_t)kWitQuotient : 0u;
         q = (int32_t)qq;
-        r = (int32_t)(y - qq * s);
+        r = (int32_t)((uint64_t)y - (uint64_t)qq * (uint64_t)s);
     }
 };
 static Scaler scaler(int64_t s) { return Scaler{s, 1.0 / (double)s, log2_exact(s)}; }

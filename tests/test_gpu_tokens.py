@@ -400,6 +400,23 @@ def test_q4_of_the_largest_values(ops, k, group):
     assert ops.wit_status() == 1
 
 
+def test_rescaling_by_any_scale_is_exact_over_64_bits(ops):
+    """quotients far beyond 32 bits are reported; their low 32 bits and the remainders are those of the whole numbers"""
+    rng = np.random.default_rng(14)
+    m = 500
+    x = np.array([[(1 << 31) - 1], [-(1 << 31)], [1], [1 << 20]], dtype=np.int64).astype(np.int32)
+    w, zeros = rng.integers(0, 16, (m, 1)).astype(np.uint8), np.full((m, 1), 8, dtype=np.uint8)
+    scales = rng.integers(-(1 << 28), 1 << 28, (m, 1)).astype(np.int32)
+    scales[::3] = rng.integers(-50, 50, scales[::3].shape)
+    y = [[int(a[0]) * int(s[0]) * ((int(b[0]) & 15) - 8) for b, s in zip(w, scales)] for a in x]
+    for s in (3, 5, 7, 999, 999983, (1 << 31) - 1, 3 << 20):
+        q, r = ops.wit_matvec_q4(dev(x), dev(w), dev(scales), 1, zeros=dev(zeros), scale=s)
+        want = [[(v + s // 2) // s for v in row] for row in y]
+        assert host(r).tolist() == [[v - k * s for v, k in zip(row, ks)] for row, ks in zip(y, want)]
+        assert (host(q).astype(np.int64) % (1 << 32)).tolist() == [[k % (1 << 32) for k in ks] for ks in want]
+        assert ops.wit_status() == (1 if any(not -(1 << 31) <= k < 1 << 31 for ks in want for k in ks) else 0)
+
+
 def test_q4_of_strided_rows(ops):
     rng = np.random.default_rng(13)
     for n, m, k, group in ((3, 70, 256, 64), (2, 33, 77, 32), (1, 40, 1024, 128)):
@@ -427,6 +444,9 @@ def test_empty_calls_do_nothing(ops, exp_table):
     one = ops.wit_paged_attention(filled(1, 2, 8), kc, vc, torch.zeros((1, 0), dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"), 0,
                                   dev(exp_table))                            # no position anywhere
     assert bool((one["qkv"] == 0).all()) and bool((one["max"] == 0).all())
+    one = ops.wit_paged_attention(filled(2, 1, 300), filled(2, 4, 1, 300), filled(2, 4, 1, 300), torch.zeros((2, 0), dtype=torch.int32, device="cuda"),
+                                  torch.zeros(2, dtype=torch.int32, device="cuda"), 0, dev(exp_table))
+    assert bool((one["qkv"] == 0).all()) and bool((one["qkv_rem"] == 0).all()) and bool((one["exp_sum"] == 0).all())
     q, r = ops.wit_matvec_q4(filled(0, 16), torch.zeros((4, 8), dtype=torch.uint8, device="cuda"), filled(4, 1), 16)
     assert q.shape == (0, 4)
     q, r = ops.wit_matvec_q4(filled(2, 16), torch.zeros((0, 8), dtype=torch.uint8, device="cuda"), filled(0, 1), 16)
@@ -524,9 +544,11 @@ def test_the_last_token_of_a_prompt_sees_what_the_whole_prompt_kernels_compute(o
     assert ops.wit_status() == 0
 
 
-def test_captured_steps_replay(ops, exp_table):
-    """one captured step a model, two models' graphs replayed in turn and at once on two streams, with eager work between"""
-    a, b = (Decoder(ops, np.random.default_rng(s), 2, 4, 2, 64, 16, 24, exp_table) for s in (30, 31))
+@pytest.mark.parametrize("seqs,steps", [(2, 24), (6, 300)])
+def test_captured_steps_replay(ops, exp_table, seqs, steps):
+    """one captured step a model, two models' graphs replayed at once on two streams, with eager work between; two sequences in the
+    forms of one launch, six with workspaces"""
+    a, b = (Decoder(ops, np.random.default_rng(s), seqs, 4, 2, 64, 16, steps, exp_table) for s in (30, 31))
     graphs = []
     for d in (a, b):
         d.feed(0)
@@ -549,9 +571,9 @@ def test_captured_steps_replay(ops, exp_table):
                 g.replay()
         torch.cuda.synchronize()
         for d in (a, b):
-            assert all(np.array_equal(host(x)[..., :t + 1] if x.shape[-1] == 24 else host(x), w[..., :t + 1] if w.shape[-1] == 24 else w)
+            assert all(np.array_equal(host(x)[..., :t + 1] if x.shape[-1] == steps else host(x), w[..., :t + 1] if w.shape[-1] == steps else w)
                        for x, w in zip(d.outputs(), d.oracle(t)))
-        ops.wit_paged_attention(a.rot, a.kc, a.vc, a.dtable, a.lens, 24, a.dexp, qk_scale=a.scale)         # eager, its own workspace
+        ops.wit_paged_attention(a.rot, a.kc, a.vc, a.dtable, a.lens, steps, a.dexp, qk_scale=a.scale)         # eager, its own workspace
     assert ops.wit_status() == 0
 
 
