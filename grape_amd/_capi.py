@@ -147,7 +147,7 @@ SIGNATURES = {
     "grape_wit_paged_attention": [c_void_p, c_void_p, c_void_p],
     "grape_wit_matvec_q4": [c_void_p, c_void_p, c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int64, c_void_p, c_void_p, c_u32, c_u32, c_u32,
                             c_u32, ctypes.c_int64, c_void_p, c_size_t, c_void_p],
-    "grape_wit_matvec_q4_workspace": [c_u32, c_u32, c_u32],
+    "grape_wit_matvec_q4_workspace": [c_u32, c_u32, c_u32, c_u32],
     "grape_wit_status": [ctypes.POINTER(c_u32), c_void_p],
     "grape_bench_copy": [c_void_p, c_void_p, c_size_t, c_int, ctypes.POINTER(ctypes.c_float), c_void_p],
     "grape_bench_copy_fr": [c_void_p, c_void_p, c_size_t, c_int, ctypes.POINTER(ctypes.c_float), c_void_p],

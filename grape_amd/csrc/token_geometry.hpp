@@ -221,9 +221,14 @@ inline const char* refuse_attention(const grape_wit_attention_args* a, const gra
     return nullptr;
 }
 
-// Products with 4-bit weights: up to this many tokens are taken apart by the workgroups that multiply them; more by a launch of its
-// own, into the workspace, in tiles of eight or sixteen, and one word a block of 2048 inputs of a token says what its digits lack.
-constexpr uint32_t kQ4Few = 4;
+// Products with 4-bit weights.  One token is taken apart by the workgroups that multiply it, and so are up to four while that is
+// little work for them (4 tokens through 4096 x 4096: 8.3 us a call and not 11); more by a launch of its own, into the workspace, in
+// tiles of four, eight or sixteen (4 tokens through 16384 x 8192: 24 us and not 44).  One word a block of 2048 inputs of a token
+// says what its digits lack.
+inline bool q4_few(uint32_t tokens, uint32_t outputs, uint32_t inputs) {
+    const uint64_t tiles = ceil_div(outputs, 16) < 256 ? 256 : ceil_div(outputs, 16);
+    return tokens == 1 || (tokens <= 4 && tiles * tokens * ceil_div(inputs, 128) <= 40000);
+}
 struct Q4Plan {
     uint32_t tile_tokens, token_tiles;
     uint32_t makers;                   // workgroups of one token that make digits
@@ -232,15 +237,15 @@ struct Q4Plan {
 inline Q4Plan q4_plan(uint32_t tokens, uint32_t inputs) {
     Q4Plan p;
     const uint32_t units = ceil_div(inputs, 128);
-    p.tile_tokens = tokens <= 8 ? 8 : 16;
+    p.tile_tokens = tokens <= 4 ? 4 : tokens <= 8 ? 8 : 16;
     p.token_tiles = ceil_div(tokens, p.tile_tokens);
     p.makers = ceil_div(units * 16, 256);
     p.at_over = (size_t)p.token_tiles * units * 32 * 4 * p.tile_tokens * 4;
     p.bytes = p.at_over + (size_t)4 * tokens * p.makers;
     return p;
 }
-inline size_t q4_workspace(uint32_t tokens, uint32_t inputs, uint32_t group) {
-    if (tokens <= kQ4Few || !inputs || !group || group % 32 || tokens > 65535 || inputs > (uint32_t)1 << 30) return 0;
+inline size_t q4_workspace(uint32_t tokens, uint32_t outputs, uint32_t inputs, uint32_t group) {
+    if (!tokens || !outputs || !inputs || !group || group % 32 || tokens > 65535 || inputs > (uint32_t)1 << 30 || q4_few(tokens, outputs, inputs)) return 0;
     return q4_plan(tokens, inputs).bytes;
 }
 
@@ -254,7 +259,7 @@ inline const char* refuse_q4(const void* d_q, const void* d_x, int64_t x_stride,
     GRAPE_REFUSE(!d_q || !d_x || !d_w || !d_scales, "d_q, d_x, d_w or d_scales is null");
     GRAPE_REFUSE(tokens > 65535, "at most 65535 tokens");
     GRAPE_REFUSE(outputs > (uint32_t)1 << 24, "at most 2^24 outputs");
-    const size_t need = q4_workspace(tokens, inputs, group);
+    const size_t need = q4_workspace(tokens, outputs, inputs, group);
     GRAPE_REFUSE(workspace_bytes < need || (need && !d_workspace), "the workspace is too small");
     GRAPE_REFUSE(need && ((uintptr_t)d_workspace & 15), "the workspace must be 16-byte aligned");
     return nullptr;

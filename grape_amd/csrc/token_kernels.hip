@@ -535,13 +535,19 @@ __global__ void __launch_bounds__(kBlock) wit_q4_digits_kernel(Q4Args p, uint32_
     if (threadIdx.x == 0) p.over[n * gridDim.x + blockIdx.x] = over;
 }
 
+// Whether the weights go through LDS: with scales for each 64 or 32 the lanes of a row load short pieces, and many.  Four tokens
+// through 16384 x 8192: 39 us and not 55 with groups of 32, 33 and not 39 with groups of 64.  With sixteen the registers are not
+// enough for it (96 us and not 90).
+constexpr bool q4_turns(int gs, int nt) { return gs < 128 && nt < 4; }
 template <int GS, int NT, int RT>
 __global__ void __launch_bounds__(kQ4Threads, 2) wit_q4_many_kernel(Q4Args p, uint32_t over_words) {
-    constexpr int kQ4ManyAhead = GS == 32 ? 1 : 2;
-    __shared__ int64_t sum[kQ4Waves][RT * NT * 64];
-    __shared__ uint32_t over_any;
-    constexpr int OPS = GS == 32 ? 4 : 2;
+    constexpr int kQ4ManyAhead = 2, OPS = GS == 32 ? 4 : 2;
     constexpr uint32_t COLS = 16 * NT;
+    // the weights to be turned over, 4 KB a wave and tile, and in the end the waves' sums
+    constexpr bool kTurns = q4_turns(GS, NT);
+    constexpr size_t kTurned = kTurns ? kQ4Waves * RT * 4096 : 0, kSums = sizeof(int64_t) * kQ4Waves * RT * NT * 64;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kTurned > kSums ? kTurned : kSums];
+    __shared__ uint32_t over_any;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, kg = lane >> 4;
     const uint32_t units = (p.inputs + 127) / 128, m0 = blockIdx.x * 16 * RT, n0 = blockIdx.y * 4 * NT;
     const uint32_t* digits = p.digits + (size_t)blockIdx.y * units * 32 * COLS;
@@ -552,31 +558,76 @@ __global__ void __launch_bounds__(kQ4Threads, 2) wit_q4_many_kernel(Q4Args p, ui
 #pragma unroll
         for (int j = 0; j < NT; j++) y[t][j][0] = y[t][j][1] = 0;
     const uint32_t share = (units + kQ4Waves - 1) / kQ4Waves, first = min(wave * share, units), last = min(first + share, units);
-    Q4Unit<GS> next[kQ4ManyAhead][RT];
-#pragma unroll
-    for (int s = 0; s < kQ4ManyAhead; s++)
+    typedef typename std::conditional<GS == 32, long, v4i_t>::type operand_t;
+    if constexpr (kTurns) {
+        uint8_t* turned = lds + wave * RT * 4096;
+        Q4Quad<GS> next[RT];
 #pragma unroll
         for (int t = 0; t < RT; t++)
-            if (first + s < last) next[s][t].load(p, min(m0 + 16 * t + col, p.outputs - 1), first + s, kg);
+            if (first < last) next[t].load(p, m0 + 16 * t, first, lane);
+        operand_t d[OPS][NT];                                    // the next unit's digits
+        auto fetch = [&](uint32_t u) {
+#pragma unroll
+            for (int op = 0; op < OPS; op++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) d[op][j] = reinterpret_cast<const operand_t*>(digits)[(((size_t)u * OPS + op) * 4 + kg) * COLS + 16 * j + col];
+        };
+        if (first < last) fetch(first);
 #pragma unroll 1
-    for (uint32_t u = first; u < last; u++) {
-        typedef typename std::conditional<GS == 32, long, v4i_t>::type operand_t;
-        operand_t d[OPS][NT];
+        for (uint32_t u = first; u < last; u += 4) {
+            Q4Quad<GS> quad[RT];
+            wave_sync();
 #pragma unroll
-        for (int op = 0; op < OPS; op++)
+            for (int t = 0; t < RT; t++) {
+                quad[t] = next[t];
+                quad[t].store(turned + 4096 * t, lane);
+                if (u + 4 < last) next[t].load(p, m0 + 16 * t, u + 4, lane);
+            }
+            wave_sync();
+#pragma unroll 1
+            for (uint32_t s = 0; s < 4 && u + s < last; s++) {
+                operand_t now[OPS][NT];
 #pragma unroll
-            for (int j = 0; j < NT; j++) d[op][j] = reinterpret_cast<const operand_t*>(digits)[(((size_t)u * OPS + op) * 4 + kg) * COLS + 16 * j + col];
-        Q4Unit<GS> x[RT];
+                for (int op = 0; op < OPS; op++)
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            x[t] = next[0][t];
+                    for (int j = 0; j < NT; j++) now[op][j] = d[op][j];
+                if (u + s + 1 < last) fetch(u + s + 1);
 #pragma unroll
-            for (int s = 0; s + 1 < kQ4ManyAhead; s++) next[s][t] = next[s + 1][t];
-            if (u + kQ4ManyAhead < last) next[kQ4ManyAhead - 1][t].load(p, min(m0 + 16 * t + col, p.outputs - 1), u + kQ4ManyAhead, kg);
+                for (int t = 0; t < RT; t++) {
+                    Q4Unit<GS> x;
+                    x.take(quad[t], turned + 4096 * t, s, lane, p.zeros != nullptr);
+                    q4_unit<GS, NT>(x, p.zeros != nullptr, y[t], [&](int op, int j) { return now[op][j]; });
+                }
+            }
         }
+    } else {
+        Q4Unit<GS> next[kQ4ManyAhead][RT];
 #pragma unroll
-        for (int t = 0; t < RT; t++) q4_unit<GS, NT>(x[t], p.zeros != nullptr, y[t], [&](int op, int j) { return d[op][j]; });
+        for (int s = 0; s < kQ4ManyAhead; s++)
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+                if (first + s < last) next[s][t].load(p, min(m0 + 16 * t + col, p.outputs - 1), first + s, kg);
+#pragma unroll 1
+        for (uint32_t u = first; u < last; u++) {
+            operand_t d[OPS][NT];
+#pragma unroll
+            for (int op = 0; op < OPS; op++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) d[op][j] = reinterpret_cast<const operand_t*>(digits)[(((size_t)u * OPS + op) * 4 + kg) * COLS + 16 * j + col];
+            Q4Unit<GS> x[RT];
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                x[t] = next[0][t];
+#pragma unroll
+                for (int s = 0; s + 1 < kQ4ManyAhead; s++) next[s][t] = next[s + 1][t];
+                if (u + kQ4ManyAhead < last) next[kQ4ManyAhead - 1][t].load(p, min(m0 + 16 * t + col, p.outputs - 1), u + kQ4ManyAhead, kg);
+            }
+#pragma unroll
+            for (int t = 0; t < RT; t++) q4_unit<GS, NT>(x[t], p.zeros != nullptr, y[t], [&](int op, int j) { return d[op][j]; });
+        }
     }
+    __syncthreads();
+    int64_t(*sum)[RT * NT * 64] = reinterpret_cast<int64_t(*)[RT * NT * 64]>(lds);
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
@@ -601,7 +652,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2) wit_q4_many_kernel(Q4Args p, ui
 template <int GS>
 static int q4_launch(const Q4Args& p, hipStream_t s) {
     const uint32_t units = (p.inputs + 127) / 128, tiles = (p.outputs + 15) / 16;
-    if (p.tokens <= token::kQ4Few) {
+    if (token::q4_few(p.tokens, p.outputs, p.inputs)) {
         // a wave for each four units of 128 inputs, and no more than sixteen a CU where that leaves four
         uint32_t waves = std::min((units + 3) / 4, std::min(q4_most_waves(GS), std::max(4u, 16u * kNumCU / tiles)));
         const uint32_t share = ((units + waves - 1) / waves + 3) / 4 * 4;
@@ -616,13 +667,19 @@ static int q4_launch(const Q4Args& p, hipStream_t s) {
     GRAPE_LAUNCH_CHECK();
     const uint32_t over_words = plan.makers * p.tokens;
     // two tiles of rows share the digits where that still leaves a workgroup for each CU (and the registers are enough)
-    const bool two = GS > 32 && (uint64_t)(tiles + 1) / 2 * plan.token_tiles >= (uint64_t)kNumCU;
+    constexpr int kMost = GS == 32 ? 0 : GS == 64 ? 4 : 1;          // from which NT on
+    const uint32_t nt = plan.tile_tokens / 4;
+    const bool two = kMost && nt >= kMost && (uint64_t)(tiles + 1) / 2 * plan.token_tiles >= (uint64_t)kNumCU;
     const dim3 grid(two ? (tiles + 1) / 2 : tiles, plan.token_tiles);
-    if constexpr (GS > 32) {
-        if (two && plan.tile_tokens == 8) wit_q4_many_kernel<GS, 2, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
-        else if (two) wit_q4_many_kernel<GS, 4, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+    if constexpr (GS == 128) {
+        if (two && nt == 1) wit_q4_many_kernel<GS, 1, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+        else if (two && nt == 2) wit_q4_many_kernel<GS, 2, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
     }
-    if (!two && plan.tile_tokens == 8) wit_q4_many_kernel<GS, 2, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+    if constexpr (GS >= 64) {
+        if (two && nt == 4) wit_q4_many_kernel<GS, 4, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+    }
+    if (!two && nt == 1) wit_q4_many_kernel<GS, 1, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+    else if (!two && nt == 2) wit_q4_many_kernel<GS, 2, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
     else if (!two) wit_q4_many_kernel<GS, 4, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
     GRAPE_LAUNCH_CHECK();
     return GRAPE_OK;
@@ -667,8 +724,8 @@ int grape_wit_rope_append(const grape_wit_rope_append_args* args, const grape_wi
     return GRAPE_OK;
 }
 
-size_t grape_wit_matvec_q4_workspace(uint32_t tokens, uint32_t inputs, uint32_t group) {
-    return token::q4_workspace(tokens, inputs, group);
+size_t grape_wit_matvec_q4_workspace(uint32_t tokens, uint32_t outputs, uint32_t inputs, uint32_t group) {
+    return token::q4_workspace(tokens, outputs, inputs, group);
 }
 
 int grape_wit_matvec_q4(int32_t* d_q, int32_t* d_r, const int32_t* d_x, int64_t x_stride, const uint8_t* d_w, int64_t w_stride,

@@ -881,9 +881,9 @@ def wit_paged_attention_workspace(seqs, heads, cache_heads, dim, max_len):
     return init().grape_wit_paged_attention_workspace(seqs, heads, cache_heads, dim, max_len)
 
 
-def wit_matvec_q4_workspace(tokens, inputs, group):
+def wit_matvec_q4_workspace(tokens, outputs, inputs, group):
     """bytes of workspace that wit_matvec_q4 needs"""
-    return init().grape_wit_matvec_q4_workspace(tokens, inputs, group)
+    return init().grape_wit_matvec_q4_workspace(tokens, outputs, inputs, group)
 
 
 def wit_matvec_q4(x, w, scales, group, zeros=None, scale=1 << 16, q=None, r=None, want_r=True, workspace=None):
@@ -908,9 +908,11 @@ def wit_matvec_q4(x, w, scales, group, zeros=None, scale=1 << 16, q=None, r=None
     space = size = 0
     if workspace is not None:
         space, size = _space(workspace, dev)
-    elif n > 4:                                        # none for fewer
-        workspace = torch.empty(lib.grape_wit_matvec_q4_workspace(n, k, group), dtype=torch.uint8, device=x.device)
-        space, size = workspace.data_ptr(), workspace.numel()
+    elif n > 1:                                        # none for one
+        size = lib.grape_wit_matvec_q4_workspace(n, m, k, group)
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+            space = workspace.data_ptr()
     _check(lib.grape_wit_matvec_q4(_arr(q, "q", (n, m), dev), _arr(r, "r", (n, m), dev), xp, xs, wp, ws, _arr(scales, "scales", groups, dev),
                                    _arr(zeros, "zeros", groups, dev, torch.uint8), n, m, k, group, scale, space, size, _stream(dev)))
     return q, r

@@ -766,8 +766,8 @@ int grape_wit_paged_attention(const grape_wit_attention_args *args, const grape_
  * d_x + n*x_stride; row m of the weights at d_w + m*w_stride bytes, two to a byte, the even k in the lower half, (inputs + 1)/2
  * bytes; scales int32 and zero points bytes (d_zeros NULL: all 8), ceil(inputs/group) a row; outputs [tokens][outputs], d_r
  * may be NULL.  1 <= scale <= 2^31, tokens <= 65535, outputs <= 2^24, group and inputs <= 2^30.  Groups of whole 32s go through
- * the matrix cores.  d_workspace as above, grape_wit_matvec_q4_workspace(...) bytes (none for up to 4 tokens). */
-size_t grape_wit_matvec_q4_workspace(uint32_t tokens, uint32_t inputs, uint32_t group);
+ * the matrix cores.  d_workspace as above, grape_wit_matvec_q4_workspace(...) bytes (none for one token). */
+size_t grape_wit_matvec_q4_workspace(uint32_t tokens, uint32_t outputs, uint32_t inputs, uint32_t group);
 int grape_wit_matvec_q4(int32_t *d_q, int32_t *d_r, const int32_t *d_x, int64_t x_stride, const uint8_t *d_w, int64_t w_stride,
                         const int32_t *d_scales, const uint8_t *d_zeros, uint32_t tokens, uint32_t outputs, uint32_t inputs,
                         uint32_t group, int64_t scale, void *d_workspace, size_t workspace_bytes, grape_stream_t stream);

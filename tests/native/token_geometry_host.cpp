@@ -18,7 +18,7 @@ int span(int32_t len, int32_t first, uint32_t max_len, uint32_t stride, uint32_t
 }
 int64_t offset_of(const grape_wit_cache* c, int32_t page, uint32_t in_page) { return token::token_offset(*c, page, in_page); }
 int kind(const grape_wit_cache* c, int64_t slot, int32_t pos, uint32_t rot, uint32_t rows) { return token::append_kind(*c, slot, pos, rot, rows); }
-size_t q4_workspace(uint32_t n, uint32_t k, uint32_t g) { return token::q4_workspace(n, k, g); }
+size_t q4_workspace(uint32_t n, uint32_t m, uint32_t k, uint32_t g) { return token::q4_workspace(n, m, k, g); }
 size_t workspace(uint32_t s, uint32_t h, uint32_t hk, uint32_t d, uint32_t n) { return token::attention_workspace(s, h, hk, d, n); }
 uint32_t divided(uint32_t n, uint32_t d) { return token::fast_div(d)(n); }
 // the parts of a plan that bound what the kernels touch

@@ -344,7 +344,8 @@ Q4 = [
     # tokens, outputs, inputs, group
     (1, 1, 1, 1), (1, 3, 2, 1), (2, 5, 7, 3), (1, 64, 64, 32), (1, 4096, 4096, 128), (3, 100, 200, 64), (5, 33, 1000, 128), (1, 257, 96, 32),
     (16, 130, 11008, 128), (17, 65, 512, 256), (4, 777, 1001, 100), (40, 31, 320, 64), (2, 16, 8200, 8200), (1, 20, 130, 4096), (9, 48, 288, 96),
-    (7, 2049, 1024, 32), (24, 300, 160, 16)]
+    (7, 2049, 1024, 32), (24, 300, 160, 16),
+    (2, 1040, 40000, 128), (3, 8200, 2600, 64), (4, 9000, 2050, 96), (2, 65, 33000, 32), (6, 8200, 520, 32), (12, 8200, 200, 128)]
 
 
 def q4_case(rng, n, m, k, group, top=400):

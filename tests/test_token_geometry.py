@@ -26,7 +26,7 @@ def lib():
         getattr(l, name).restype = ctypes.c_char_p
     l.refuse_append.argtypes = l.refuse_attention.argtypes = [p, p]
     l.refuse_q4.argtypes = [p, p, q, p, q, p, u, u, u, u, q, p, ctypes.c_size_t]
-    l.q4_workspace.argtypes, l.q4_workspace.restype = [u] * 3, ctypes.c_size_t
+    l.q4_workspace.argtypes, l.q4_workspace.restype = [u] * 4, ctypes.c_size_t
     l.struct_bytes.restype = l.workspace.restype = ctypes.c_size_t
     l.overlaps.argtypes = [p]
     l.span.argtypes = [i, i, u, u, u, p]
@@ -100,7 +100,7 @@ def test_bad_products_are_refused(lib, bad):
     good = dict(q=16, x=16, xs=64, w=16, ws=32, sc=16, n=2, m=8, k=64, group=32, scale=65536, sp=0, sb=0)
     assert lib.refuse_q4(*good.values()) is None
     assert lib.refuse_q4(*{**good, "n": 0, "q": 0}.values()) is None
-    assert lib.refuse_q4(*{**good, "n": 5, "sp": 64, "sb": lib.q4_workspace(5, 64, 32)}.values()) is None
+    assert lib.refuse_q4(*{**good, "n": 5, "sp": 64, "sb": lib.q4_workspace(5, 8, 64, 32)}.values()) is None
     assert lib.refuse_q4(*{**good, "n": 5, "group": 20}.values()) is None               # no digits without the matrix cores
     assert lib.refuse_q4(*{**good, **bad}.values())
 
@@ -190,11 +190,12 @@ def test_plans_cover_every_position_within_their_limits(lib):
 
 
 def test_workspace_sizes(lib):
-    assert lib.q4_workspace(4, 4096, 128) == 0 and lib.q4_workspace(9, 4096, 100) == 0 and lib.q4_workspace(9, 0, 32) == 0
-    for n, k in ((5, 1), (8, 128), (9, 129), (16, 11008), (17, 2049), (40, 4095), (65535, 1 << 16)):
-        tile, units = 8 if n <= 8 else 16, -(-k // 128)
+    assert lib.q4_workspace(1, 1 << 20, 1 << 20, 128) == 0 and lib.q4_workspace(4, 4096, 4096, 128) == 0
+    assert lib.q4_workspace(9, 64, 4096, 100) == 0 and lib.q4_workspace(9, 64, 0, 32) == 0 and lib.q4_workspace(9, 0, 64, 32) == 0
+    for n, m, k in ((2, 16384, 8192), (4, 11008, 4096), (5, 1, 1), (8, 100, 128), (9, 1, 129), (16, 4096, 11008), (17, 5, 2049), (40, 3, 4095), (65535, 1, 1 << 16)):
+        tile, units = 4 if n <= 4 else 8 if n <= 8 else 16, -(-k // 128)
         # a byte an input and plane, whole units and tiles of tokens, and a word a token and 2048 inputs
-        assert lib.q4_workspace(n, k, 32) == -(-n // tile) * tile * 4 * units * 128 + 4 * n * -(-units // 16)
+        assert lib.q4_workspace(n, m, k, 32) == -(-n // tile) * tile * 4 * units * 128 + 4 * n * -(-units // 16)
     assert lib.workspace(0, 8, 8, 64, 100) == 0 and lib.workspace(65536, 8, 8, 64, 100) == 0 and lib.workspace(60000, 60000, 1, 64, 100000) == 0
     assert lib.workspace(1, 8, 2, 64, 1000) >= 4 * 8 * 1000
 
@@ -273,9 +274,10 @@ def test_attention_helper_refuses(helpers, bad):
 def test_q4_helper_refuses(helpers, bad):
     good = dict(x=i32(2, 64), w=torch.zeros((8, 32), dtype=torch.uint8), scales=i32(8, 2), group=32)
     assert ops.wit_matvec_q4(**good)[0].shape == (2, 8)
+    n = len(helpers)
     with pytest.raises(ValueError):
         ops.wit_matvec_q4(**{**good, **bad})
-    assert len(helpers) == 1
+    assert not [c for c in helpers[n:] if not c[0].endswith("_workspace")]
 
 
 def test_helpers_hand_over_strides(helpers):
@@ -287,4 +289,5 @@ def test_helpers_hand_over_strides(helpers):
     assert ops._APPEND.unpack(args)[3:6] == (fused.stride(0),) * 3 and ops._CACHE.unpack(c)[2:] == (10, 16, 4, 64, 16 * 70, 70, 160 * 70)
     x = i32(1, 64).expand(4, 64)
     ops.wit_matvec_q4(x, torch.zeros((8, 40), dtype=torch.uint8)[:, 3:35], i32(8, 2), 32)
-    assert helpers[1][1][3] == 0 and helpers[1][1][5] == 40
+    args = [c[1] for c in helpers if c[0] == "grape_wit_matvec_q4"][0]
+    assert args[3] == 0 and args[5] == 40
