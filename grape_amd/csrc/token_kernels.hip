@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(kBlock) wit_q4_digits_kernel(Q4Args p, uint32_
     uint32_t* out = p.digits + (size_t)tile * units * 32 * cols;          // 128 inputs of a column are 32 words
     if (e < units * 16 && q4_digits<GS>(p, n, e, out, e, n - tile * tile_tokens, cols)) over = 1;
     __syncthreads();
-    if (threadIdx.x == 0) p.over[n * gridDim.x + blockIdx.x] = over;
+    if (threadIdx.x == 0) p.over[(size_t)n * gridDim.x + blockIdx.x] = over;
 }
 
 // Whether the weights go through LDS: with scales for each 64 or 32 the lanes of a row load short pieces, and many.  Four tokens
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(kBlock) wit_q4_digits_kernel(Q4Args p, uint32_
 // enough for it (96 us and not 90).
 constexpr bool q4_turns(int gs, int nt) { return gs < 128 && nt < 4; }
 template <int GS, int NT, int RT>
-__global__ void __launch_bounds__(kQ4Threads, 2) wit_q4_many_kernel(Q4Args p, uint32_t over_words) {
+__global__ void __launch_bounds__(kQ4Threads, 2) wit_q4_many_kernel(Q4Args p, uint32_t makers) {
     constexpr int kQ4ManyAhead = 2, OPS = GS == 32 ? 4 : 2;
     constexpr uint32_t COLS = 16 * NT;
     // the weights to be turned over, 4 KB a wave and tile, and in the end the waves' sums
@@ -633,8 +633,9 @@ __global__ void __launch_bounds__(kQ4Threads, 2) wit_q4_many_kernel(Q4Args p, ui
 #pragma unroll
         for (int j = 0; j < NT; j++) sum[wave][(t * NT + j) * 64 + lane] = y[t][j][0] + (int64_t)((uint64_t)y[t][j][1] << 16);
     __syncthreads();
+    const uint32_t over_words = min(4u * NT, p.tokens - n0) * makers;
     for (uint32_t i = threadIdx.x; i < over_words; i += kQ4Threads)
-        if (p.over[i]) over_any = 1;
+        if (p.over[(size_t)n0 * makers + i]) over_any = 1;
     __syncthreads();
     uint32_t bad = 0;
     for (uint32_t i = threadIdx.x; i < RT * NT * 64; i += kQ4Threads) {
@@ -665,22 +666,21 @@ static int q4_launch(const Q4Args& p, hipStream_t s) {
     const token::Q4Plan plan = token::q4_plan(p.tokens, p.inputs);
     wit_q4_digits_kernel<GS><<<dim3(plan.makers, p.tokens), kBlock, 0, s>>>(p, plan.tile_tokens);
     GRAPE_LAUNCH_CHECK();
-    const uint32_t over_words = plan.makers * p.tokens;
     // two tiles of rows share the digits where that still leaves a workgroup for each CU (and the registers are enough)
     constexpr int kMost = GS == 32 ? 0 : GS == 64 ? 4 : 1;          // from which NT on
     const uint32_t nt = plan.tile_tokens / 4;
     const bool two = kMost && nt >= kMost && (uint64_t)(tiles + 1) / 2 * plan.token_tiles >= (uint64_t)kNumCU;
     const dim3 grid(two ? (tiles + 1) / 2 : tiles, plan.token_tiles);
     if constexpr (GS == 128) {
-        if (two && nt == 1) wit_q4_many_kernel<GS, 1, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
-        else if (two && nt == 2) wit_q4_many_kernel<GS, 2, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+        if (two && nt == 1) wit_q4_many_kernel<GS, 1, 2><<<grid, kQ4Threads, 0, s>>>(p, plan.makers);
+        else if (two && nt == 2) wit_q4_many_kernel<GS, 2, 2><<<grid, kQ4Threads, 0, s>>>(p, plan.makers);
     }
     if constexpr (GS >= 64) {
-        if (two && nt == 4) wit_q4_many_kernel<GS, 4, 2><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+        if (two && nt == 4) wit_q4_many_kernel<GS, 4, 2><<<grid, kQ4Threads, 0, s>>>(p, plan.makers);
     }
-    if (!two && nt == 1) wit_q4_many_kernel<GS, 1, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
-    else if (!two && nt == 2) wit_q4_many_kernel<GS, 2, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
-    else if (!two) wit_q4_many_kernel<GS, 4, 1><<<grid, kQ4Threads, 0, s>>>(p, over_words);
+    if (!two && nt == 1) wit_q4_many_kernel<GS, 1, 1><<<grid, kQ4Threads, 0, s>>>(p, plan.makers);
+    else if (!two && nt == 2) wit_q4_many_kernel<GS, 2, 1><<<grid, kQ4Threads, 0, s>>>(p, plan.makers);
+    else if (!two) wit_q4_many_kernel<GS, 4, 1><<<grid, kQ4Threads, 0, s>>>(p, plan.makers);
     GRAPE_LAUNCH_CHECK();
     return GRAPE_OK;
 }

@@ -763,6 +763,14 @@ def _rows(t, name, shape, dev, dtype=torch.int32):
     return t.data_ptr(), st[0]
 
 
+def _pack(form, *values):
+    """a struct of the C ABI; numbers that do not fit its fields are refused"""
+    try:
+        return form.pack(*values)
+    except struct.error as e:
+        raise ValueError("a size or scale is out of range: %s" % e) from None
+
+
 _CACHE = struct.Struct("<2Q4I3q")
 _APPEND = struct.Struct("<3Q3q7Q4Iq2i")
 _ATTEND = struct.Struct("<Qq16Q3q6I")
@@ -778,7 +786,7 @@ def _cache(k_cache, v_cache, dev):
     pages, page, heads, dim = shape
     if st[3] != 1 and dim > 1:
         _refuse("the elements of a head must be contiguous")
-    return _CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), pages, page, heads, dim, st[0], st[1], st[2]), heads, dim
+    return _pack(_CACHE, k_cache.data_ptr(), v_cache.data_ptr(), pages, page, heads, dim, st[0], st[1], st[2]), heads, dim
 
 
 def _space(workspace, dev):
@@ -814,7 +822,7 @@ def wit_rope_append(q, k, v, positions, slots, cos, sin, k_cache, v_cache, q_out
     table = cos.shape
     if len(table) != 2:
         _refuse("cos and sin must be (rows, rot / 2) tensors")
-    args = _APPEND.pack(qp, kp, vp, qs, ks, vs, _arr(positions, "positions", (n,), dev), _arr(slots, "slots", (n,), dev, torch.int64),
+    args = _pack(_APPEND, qp, kp, vp, qs, ks, vs, _arr(positions, "positions", (n,), dev), _arr(slots, "slots", (n,), dev, torch.int64),
                         _arr(cos, "cos", table, dev), _arr(sin, "sin", table, dev), qo, qr, _arr(k_rem, "k_rem", kv_shape, dev), n, heads,
                         2 * table[1], table[0], scale, 1 if interleaved else 0, 0)
     _check(lib.grape_wit_rope_append(args, cache, _stream(dev)))
@@ -852,8 +860,8 @@ def wit_paged_attention(q, k_cache, v_cache, block_table, lens, max_len, exp_tab
         _refuse("block_table must be (seqs, pages)")
     if exp_table.shape != (1 << index_bits,):
         _refuse("the exponential table must have 2^index_bits entries")
-    if max_len < 0:
-        _refuse("max_len must not be negative")
+    if max_len < 0 or max_len >> 31:
+        _refuse("max_len must be in 0..2^31 - 1")
     if out is None:
         out = {"qkv": _i32(*row), "qkv_rem": _i32(*row)}
         if proof:
@@ -867,7 +875,7 @@ def wit_paged_attention(q, k_cache, v_cache, block_table, lens, max_len, exp_tab
         size = lib.grape_wit_paged_attention_workspace(n, heads, heads_kv, dim, max_len)
         workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     space, size = _space(workspace, dev) if workspace is not None else (0, 0)
-    args = _ATTEND.pack(qp, qs, _arr(block_table, "block_table", width, dev), _arr(lens, "lens", (n,), dev), _arr(first, "first", (n,), dev),
+    args = _pack(_ATTEND, qp, qs, _arr(block_table, "block_table", width, dev), _arr(lens, "lens", (n,), dev), _arr(first, "first", (n,), dev),
                         _arr(exp_table, "exp_table", exp_table.shape, dev), *[_arr(get(name), name, rows, dev) for name in _PROOF_ROWS],
                         _arr(get("max"), "max", one, dev), _arr(get("exp_sum"), "exp_sum", one, dev), _arr(get("qkv"), "qkv", row, dev),
                         _arr(get("qkv_rem"), "qkv_rem", row, dev), space, size, qk_scale, prob_scale, out_scale, n,
@@ -877,12 +885,16 @@ def wit_paged_attention(q, k_cache, v_cache, block_table, lens, max_len, exp_tab
 
 
 def wit_paged_attention_workspace(seqs, heads, cache_heads, dim, max_len):
-    """bytes of workspace that wit_paged_attention needs"""
+    """bytes of workspace that wit_paged_attention needs; 0 for sizes that it refuses"""
+    if max(seqs, heads, cache_heads, dim, max_len) >> 31:
+        return 0
     return init().grape_wit_paged_attention_workspace(seqs, heads, cache_heads, dim, max_len)
 
 
 def wit_matvec_q4_workspace(tokens, outputs, inputs, group):
-    """bytes of workspace that wit_matvec_q4 needs"""
+    """bytes of workspace that wit_matvec_q4 needs; 0 for sizes that it refuses"""
+    if max(tokens, outputs, inputs, group) >> 31:
+        return 0
     return init().grape_wit_matvec_q4_workspace(tokens, outputs, inputs, group)
 
 
@@ -898,6 +910,8 @@ def wit_matvec_q4(x, w, scales, group, zeros=None, scale=1 << 16, q=None, r=None
     m = len(w)
     if k < 1:
         _refuse("empty inner dimension")
+    if n >> 31 or m >> 31 or k >> 31 or group >> 31 or scale >> 32:          # what ctypes would cut off
+        _refuse("a size or scale is out of range")
     groups = (m, (k - 1) // group + 1)
     xp, xs = _rows(x, "x", (n, k), dev)
     wp, ws = _rows(w, "w", (m, (k + 1) // 2), dev, torch.uint8)

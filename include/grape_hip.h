@@ -747,8 +747,8 @@ int grape_wit_rope_append(const grape_wit_rope_append_args *args, const grape_wi
  * 1 <= scales <= 2^31 (prob_scale <= 2^30), dim <= 8192.
  *
  * d_workspace (16-byte aligned) holds what the launches hand on to each other, grape_wit_paged_attention_workspace(...) bytes
- * (none up to 256 positions of short heads);
- * it needs no initial contents, and calls that may run at the same time, replays of captured ones among them, need one each. */
+ * (none up to 256 positions of heads up to 256 elements); it needs no initial contents, and calls that may run at the same time,
+ * replays of captured ones among them, need one each. */
 typedef struct {
     const int32_t *d_q;
     int64_t q_stride;
@@ -766,7 +766,8 @@ int grape_wit_paged_attention(const grape_wit_attention_args *args, const grape_
  * d_x + n*x_stride; row m of the weights at d_w + m*w_stride bytes, two to a byte, the even k in the lower half, (inputs + 1)/2
  * bytes; scales int32 and zero points bytes (d_zeros NULL: all 8), ceil(inputs/group) a row; outputs [tokens][outputs], d_r
  * may be NULL.  1 <= scale <= 2^31, tokens <= 65535, outputs <= 2^24, group and inputs <= 2^30.  Groups of whole 32s go through
- * the matrix cores.  d_workspace as above, grape_wit_matvec_q4_workspace(...) bytes (none for one token). */
+ * the matrix cores.  d_workspace as above, grape_wit_matvec_q4_workspace(...) bytes (none for one
+ * token, and for up to four where the weights are few). */
 size_t grape_wit_matvec_q4_workspace(uint32_t tokens, uint32_t outputs, uint32_t inputs, uint32_t group);
 int grape_wit_matvec_q4(int32_t *d_q, int32_t *d_r, const int32_t *d_x, int64_t x_stride, const uint8_t *d_w, int64_t w_stride,
                         const int32_t *d_scales, const uint8_t *d_zeros, uint32_t tokens, uint32_t outputs, uint32_t inputs,

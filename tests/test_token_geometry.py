@@ -291,3 +291,23 @@ def test_helpers_hand_over_strides(helpers):
     ops.wit_matvec_q4(x, torch.zeros((8, 40), dtype=torch.uint8)[:, 3:35], i32(8, 2), 32)
     args = [c[1] for c in helpers if c[0] == "grape_wit_matvec_q4"][0]
     assert args[3] == 0 and args[5] == 40
+
+
+@pytest.mark.parametrize("call, args, bad", [
+    (ops.wit_rope_append, append_args, dict(scale=1 << 63)), (ops.wit_rope_append, append_args, dict(scale=0.5)),
+    (ops.wit_paged_attention, attend_args, dict(max_len=1 << 32)), (ops.wit_paged_attention, attend_args, dict(qk_scale=1 << 64)),
+    (ops.wit_paged_attention, attend_args, dict(bit_shift=-1)), (ops.wit_paged_attention, attend_args, dict(bit_shift=1 << 32)),
+    (ops.wit_matvec_q4, lambda: dict(x=i32(2, 64), w=torch.zeros((8, 32), dtype=torch.uint8), scales=i32(8, 1), group=1 << 20), dict(group=(1 << 32) + 32)),
+    (ops.wit_matvec_q4, lambda: dict(x=i32(2, 64), w=torch.zeros((8, 32), dtype=torch.uint8), scales=i32(8, 1), group=1 << 20), dict(scale=(1 << 64) + 65536)),
+    (ops.wit_matvec_q4, lambda: dict(x=i32(2, 64), w=torch.zeros((8, 32), dtype=torch.uint8), scales=i32(8, 1), group=1 << 20), dict(x=i32(1, 64).expand((1 << 32) + 2, 64)))])
+def test_numbers_that_the_call_would_cut_off_are_refused(helpers, call, args, bad):
+    call(**args())
+    n = len(helpers)
+    with pytest.raises(ValueError):
+        call(**{**args(), **bad})
+    assert not [c for c in helpers[n:] if not c[0].endswith("_workspace")]
+
+
+def test_no_workspace_for_sizes_beyond_the_abi(helpers):
+    assert ops.wit_matvec_q4_workspace(2, (1 << 32) + 8, 64, 32) == 0 and ops.wit_paged_attention_workspace(1, 8, 8, 64, 1 << 32) == 0
+    assert not helpers
