@@ -156,9 +156,10 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
         p.value_chunk = max_len <= 64 ? 64 : ceil_div(max_len, 64) * 64;
     } else {
         p.groups = ceil_div(dim32, p.blocks);
-        // no longer than 256 while that leaves few parts to join: many of max_len's positions may be none (24 sequences with a window
-        // of 1024 of up to 5000, 4 heads of 80: 20 us of values in chunks of 512)
-        if (p.groups == 1 && beside * ceil_div(max_len, 256) <= kWorkgroups / 2 && most > 256) most = 256;
+        // no longer than 256 while that leaves few parts to join, as many of max_len's positions may be none (24 sequences with a
+        // window of 1024 of up to 5000, 4 heads of 80: 20 us of values in chunks of 512), and with several sequences, whose lengths
+        // differ (64 of up to 2048, 8 heads of 128: 161 us a call and not 170); but one of 131072 281 us and not 292 without
+        if (p.groups == 1 && (seqs >= 8 || beside * ceil_div(max_len, 256) <= kWorkgroups / 2) && most > 256) most = 256;
         p.value_chunk = chunk(beside * p.groups, p.blocks == 1 ? 128 : 64, most, kWorkgroups / 4);
     }
     p.value_chunks = ceil_div(max_len, p.value_chunk);
