@@ -428,7 +428,8 @@ __device__ __forceinline__ void write_empty(const AttendArgs& p, const Tile& w, 
 }
 
 // ---- the launches over chunks
-// Scores of `rows` query heads with a chunk of the keys.  Bound by reading the keys.
+// Scores of `rows` query heads with a chunk of the keys.  Bound by reading the keys: 131072 positions of 8 heads of 128 for 32 query
+// heads, 570 MB with what is written, 121 us, 4.7 TB/s, as a copy.
 template <bool VEC>
 __global__ void __launch_bounds__(256, 4) wit_attend_scores_kernel(AttendArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
@@ -486,7 +487,8 @@ __device__ __forceinline__ T block_all(T v, F f) {
     return v;
 }
 
-// Exponentials of a chunk of one row, and their sum.
+// Exponentials of a chunk of one row, and their sum.  Bound by the gathers: 32 rows of 131072, 31 us, 135 a nanosecond from a table
+// of 4 MB that the L2 of each die shares with the scores.
 __global__ void __launch_bounds__(kBlock) wit_attend_exp_kernel(AttendArgs p) {
     const uint32_t b = blockIdx.z;
     const size_t row = (size_t)b * p.a.heads + blockIdx.y;
@@ -506,7 +508,8 @@ __global__ void __launch_bounds__(kBlock) wit_attend_exp_kernel(AttendArgs p) {
 }
 
 // Probabilities of a chunk of the positions for `rows` query heads, and their products with 32 * blocks elements of the values.
-// The waves take different blocks of 32 elements, or every second or fourth step.  Bound by reading the values.
+// The waves take different blocks of 32 elements, or every second or fourth step.  Bound by reading the values: the
+// 131072 positions' 587 MB with probabilities and queries in 128 us, 4.6 TB/s.
 constexpr uint32_t kProbAhead = 4;
 template <bool VEC, int PP>
 __global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p) {
@@ -601,7 +604,8 @@ __global__ void __launch_bounds__(kJoinThreads) wit_attend_join_kernel(AttendArg
 
 // ---- the same in one launch, a workgroup for all positions of its query heads (at most kWholeMost): what goes from step to step
 // stays on chip.  A few positions leave nothing but latencies - of loads that depend on each other, and of instructions that run
-// once - so eight waves share the positions, and the softmax takes one position a thread in short loops.
+// once - so eight waves share the positions, and the softmax takes one position a thread in short loops.  37 positions of 32 heads of 128:
+// 10.2 us.
 constexpr uint32_t kWholeWaves = 8, kWholeThreads = 64 * kWholeWaves;
 template <bool VEC, int PP>
 __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(AttendArgs p) {

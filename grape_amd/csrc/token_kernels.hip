@@ -9,7 +9,8 @@ namespace grape {
 // ------------------------------------------------------------------------------------------------
 // Rotation and append.  A unit is W pairs of a rotated head or 2 W elements that only move; a token's units are those of its
 // query heads, its key heads and its value heads.  W = 4: a unit is two 16-byte loads and two to four 16-byte stores.  Bound by
-// memory; with few tokens by two loads that depend on each other, the position and its row of the tables.
+// memory (2048 tokens of one head of 4096 elements, 302 MB: 79 us, 3.8 TB/s; units of 16 bytes took 94); with few tokens by two
+// loads that depend on each other, the position and its row of the tables (one token: 3.4 us).
 //
 // Of several tokens with one slot the last one has to stay, whatever the order in which they are written: a workgroup looks for
 // its tokens' slots among those of the later tokens first.  It reads 8 bytes a later token for that, beside some hundred units of
@@ -462,7 +463,8 @@ __device__ __forceinline__ void q4_out(const Q4Args& p, uint32_t n, uint32_t m, 
 }
 
 // Up to four tokens: a workgroup makes their digits itself, in LDS (a longer input goes through in pieces), while its first weights
-// are under way.  blockDim: as many waves as share a tile's inputs, 4 KB of LDS each behind the digits.
+// are under way.  One token through 4096 x 4096, groups of 128: 5.7 us, as long as a launch and a chain of loads take; 11008 x 4096,
+// groups of 64 with zero points, 26 MB: 12.1 us, 2.1 TB/s, bound by what is under way and by the digits of each workgroup.  blockDim: as many waves as share a tile's inputs, 4 KB of LDS each behind the digits.
 template <int GS>
 __global__ void __launch_bounds__(64 * q4_most_waves(GS), GS == 32 ? 2 : 4) wit_q4_few_kernel(Q4Args p, uint32_t piece) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(64 * q4_most_waves(GS), GS == 32 ? 2 : 4) wit_
 }
 
 // More tokens: their digits are made once, by a launch of its own, and read from L2 as operands, 4 NT tokens at a time for RT tiles
-// of 16 rows.  For 16 tokens through 4096 x 11008 those are 180 MB at 12 TB/s, which bounds it (14.7 us, of which reading the weights
+// of 16 rows.  For 16 tokens through 4096 x 11008 those are 180 MB at 12 TB/s, which bounds it (14.3 us, of which reading the weights
 // would take 5).  Digits in LDS for 128 rows at a time ask for 22 MB instead, but leave a workgroup a CU of which each waits for
 // its next weights, and sums to be joined: 14.8 and 3.9 us.
 template <int GS>
