@@ -35,6 +35,42 @@ __device__ __forceinline__ bool span_of(const AttendArgs& p, uint32_t b, uint32_
     return token::live_span(p.a.d_lens[b], p.a.d_first ? p.a.d_first[b] : 0, p.a.max_len, p.a.table_stride, p.c.page_size, lo, hi);
 }
 
+// The sequence, the chunk of `size` positions and the positions that are number `index` when the sequences' chunks are counted, one
+// at least of each; false where there are fewer.  Where lengths differ, many of max_len's chunks are of no sequence: counted, their
+// workgroups come last, when all others are under way (64 sequences of up to 2048, 8 heads of 128: 147 us a call and not 156, 24 with
+// a window of 256 of up to 5000 29 and not 39).  It costs each workgroup a wait for the lengths (64 sequences of 1024 each: 153 and
+// not 149), so that few sequences keep the plain order.  All lanes of a wave together.
+__device__ __forceinline__ bool find_chunk(const AttendArgs& p, uint32_t index, uint32_t size, uint32_t& b, uint32_t& chunk, uint32_t& lo, uint32_t& hi, bool& fits) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < p.a.seqs; base += 64) {
+        uint32_t l = 0, h = 0, n = 0;
+        bool ok = true;
+        if (base + lane < p.a.seqs) {
+            ok = span_of(p, base + lane, l, h);
+            n = l < h ? (h - l - 1) / size + 1 : 1;
+        }
+        uint32_t sum = n;
+#pragma unroll
+        for (uint32_t d = 1; d < 64; d <<= 1) {
+            const uint32_t y = __shfl_up(sum, d, 64);
+            if (lane >= d) sum += y;
+        }
+        const unsigned long long past = __ballot(before + sum > index);
+        if (past) {
+            const int at = __ffsll(past) - 1;
+            b = base + (uint32_t)at;
+            chunk = index - before - (uint32_t)__builtin_amdgcn_readlane((int)(sum - n), at);
+            lo = (uint32_t)__builtin_amdgcn_readlane((int)l, at);
+            hi = (uint32_t)__builtin_amdgcn_readlane((int)h, at);
+            fits = __builtin_amdgcn_readlane((int)ok, at) != 0;
+            return true;
+        }
+        before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+    }
+    return false;
+}
+
 // The offsets of a chunk's positions t0 .. t0 + n, made by all threads of a workgroup.  The first page of each thread is
 // requested before the sequence's length is known where it does not depend on it, so that the two loads are under way together.
 struct Offsets {
@@ -435,16 +471,18 @@ __global__ void __launch_bounds__(256, 4) wit_attend_scores_kernel(AttendArgs p)
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ unsigned long long q_sum[16];
     __shared__ uint32_t over_any;
-    const uint32_t per_chunk = p.c.heads * p.plan.tiles, chunk = blockIdx.x / per_chunk;
-    const Tile w(p, blockIdx.y, blockIdx.x - chunk * per_chunk);
-    uint32_t lo, hi, bad = 0;
+    const uint32_t per_chunk = p.c.heads * p.plan.tiles, index = blockIdx.x / per_chunk, within = blockIdx.x - index * per_chunk;
+    uint32_t b = blockIdx.y, chunk = index, lo, hi, bad = 0;
+    bool fits;
+    if (p.plan.counted && !find_chunk(p, index, p.plan.score_chunk, b, chunk, lo, hi, fits)) return;
+    const Tile w(p, b, within);
     // what does not depend on the sequence's length is requested beside it
     Queries queries;
     queries.first(p, w);
     Offsets offsets;
     offsets.request(p, w.b, (uint64_t)chunk * p.plan.score_chunk, p.plan.score_chunk);
-    const bool fits = span_of(p, w.b, lo, hi);
-    if (!fits && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.status, (uint32_t)kWitIndex);
+    if (!p.plan.counted) fits = span_of(p, w.b, lo, hi);
+    if (!fits && chunk == 0 && within == 0 && threadIdx.x == 0) atomicOr(p.status, (uint32_t)kWitIndex);
     const uint64_t start = (uint64_t)lo + (uint64_t)chunk * p.plan.score_chunk;
     if (start >= hi) return;
     const uint32_t t0 = (uint32_t)start, n = min(hi - t0, p.plan.score_chunk);
@@ -515,13 +553,15 @@ template <bool VEC, int PP>
 __global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ unsigned long long e_sum[16], p_sum[16];
-    const uint32_t per_chunk = p.c.heads * p.plan.tiles * p.plan.groups, chunk = blockIdx.x / per_chunk, within = blockIdx.x - chunk * per_chunk;
+    const uint32_t per_chunk = p.c.heads * p.plan.tiles * p.plan.groups, index = blockIdx.x / per_chunk, within = blockIdx.x - index * per_chunk;
     const uint32_t group = within % p.plan.groups;
-    const Tile w(p, blockIdx.y, within / p.plan.groups);
-    uint32_t lo, hi, bad = 0;
+    uint32_t b = blockIdx.y, chunk = index, lo, hi, bad = 0;
+    bool fits;
+    if (p.plan.counted && !find_chunk(p, index, p.plan.value_chunk, b, chunk, lo, hi, fits)) return;
+    const Tile w(p, b, within / p.plan.groups);
     Offsets offsets;
     offsets.request(p, w.b, (uint64_t)chunk * p.plan.value_chunk, p.plan.value_chunk);
-    span_of(p, w.b, lo, hi);
+    if (!p.plan.counted) span_of(p, w.b, lo, hi);
     const uint64_t start = (uint64_t)lo + (uint64_t)chunk * p.plan.value_chunk;
     const bool direct = hi - lo <= p.plan.value_chunk;          // the whole row is this workgroup's
     const uint32_t e0 = group * p.plan.blocks * 32, width = p.plan.blocks * 32, dim = p.c.dim;
@@ -777,7 +817,8 @@ int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_
     const size_t value_lds = std::max<size_t>((size_t)pl.value_chunk * (pl.rows * planes + 8), (size_t)pl.rows * pl.blocks * 32 * 8);
     // the heads of one chunk are neighbours: they read the same tokens' lines of memory at the same time
     const uint32_t head_tiles = p.c.heads * pl.tiles;
-    const dim3 score_grid(std::max(1u, pl.score_chunks) * head_tiles, a.seqs), value_grid(std::max(1u, pl.value_chunks) * head_tiles * pl.groups, a.seqs);
+    const uint32_t along = pl.counted ? a.seqs : 1, across = pl.counted ? 1 : a.seqs;
+    const dim3 score_grid(std::max(1u, pl.score_chunks) * head_tiles * along, across), value_grid(std::max(1u, pl.value_chunks) * head_tiles * pl.groups * along, across);
     if (vec) wit_attend_scores_kernel<true><<<score_grid, 256, score_lds, s>>>(p);
     else wit_attend_scores_kernel<false><<<score_grid, 256, score_lds, s>>>(p);
     GRAPE_LAUNCH_CHECK();

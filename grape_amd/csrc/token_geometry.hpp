@@ -102,6 +102,7 @@ struct AttentionPlan {
     uint32_t exp_chunk, exp_chunks;
     uint32_t blocks, groups;           // blocks of 32 elements of a values workgroup, workgroups of a head's elements
     uint32_t value_chunk, value_chunks;
+    bool counted;                      // the scores' and the values' workgroups find their chunk by counting (see find_chunk)
     bool whole;                        // one launch, a workgroup for all positions
     size_t whole_lds;
     size_t at_scores, at_exp, at_max, at_sum, at_part, bytes;      // offsets in the workspace
@@ -110,6 +111,7 @@ constexpr uint32_t kTokenLds = 60 * 1024;      // of a workgroup; of one that ta
 constexpr size_t kWholeLds = 72 * 1024;
 constexpr uint32_t kWorkgroups = 4096;
 constexpr uint32_t kWholeMost = 256;          // positions of the one launch
+constexpr uint32_t kCountedMost = 256;        // sequences whose chunks are counted
 
 inline uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
 
@@ -156,15 +158,18 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
         p.value_chunk = max_len <= 64 ? 64 : ceil_div(max_len, 64) * 64;
     } else {
         p.groups = ceil_div(dim32, p.blocks);
-        // no longer than 256 while that leaves few parts to join, as many of max_len's positions may be none (24 sequences with a
-        // window of 1024 of up to 5000, 4 heads of 80: 20 us of values in chunks of 512), and with several sequences, whose lengths
-        // differ (64 of up to 2048, 8 heads of 128: 161 us a call and not 170); but one of 131072 281 us and not 292 without
+        // no longer than 256 while that leaves few parts to join, as many of max_len's positions may be none, and with several
+        // sequences, whose lengths differ (64 of up to 2048, 8 heads of 128: 147 us a call and not 152; 8 of up to 20000 with a
+        // window of 1024 39 and not 59); but one of 131072 281 us and not 292 without
         if (p.groups == 1 && (seqs >= 8 || beside * ceil_div(max_len, 256) <= kWorkgroups / 2) && most > 256) most = 256;
         p.value_chunk = chunk(beside * p.groups, p.blocks == 1 ? 128 : 64, most, kWorkgroups / 4);
     }
     p.value_chunks = ceil_div(max_len, p.value_chunk);
     // a launch's first axis, in threads
     if ((uint64_t)cache_heads * p.tiles * std::max<uint64_t>(p.score_chunks, (uint64_t)p.value_chunks * p.groups) >= (uint64_t)1 << 23) return false;
+    // lengths that differ (see find_chunk for both sides); more sequences would make each workgroup's count long
+    p.counted = seqs >= 8 && seqs <= kCountedMost &&
+                (uint64_t)seqs * cache_heads * p.tiles * std::max<uint64_t>(p.score_chunks, (uint64_t)p.value_chunks * p.groups) < (uint64_t)1 << 23;
     // offsets, 64-bit sums of the scores and then of the output, scores, and the queries' digits or the probabilities' ones
     const size_t one = (size_t)5 * 64 * p.dim64 * p.rows, two = (size_t)4 * kWholeMost * p.rows;
     p.whole_lds = 8 * kWholeMost + (size_t)8 * p.rows * (dim > kWholeMost ? dim : kWholeMost) + (size_t)4 * kWholeMost * p.rows + (one > two ? one : two);

@@ -30,6 +30,10 @@ int plan_of(uint32_t s, uint32_t h, uint32_t hk, uint32_t d, uint32_t n, uint64_
     std::memcpy(o, v, sizeof v);
     return 1;
 }
+int counted(uint32_t s, uint32_t h, uint32_t hk, uint32_t d, uint32_t n) {
+    token::AttentionPlan p;
+    return token::attention_plan(s, h, hk, d, n, p) ? p.counted : -1;
+}
 // every field of the structs, in the order in which the helpers pack them
 void append_fields(const grape_wit_rope_append_args* a, int64_t* o) {
     const int64_t v[] = {(int64_t)a->d_q, (int64_t)a->d_k, (int64_t)a->d_v, a->q_stride, a->k_stride, a->v_stride, (int64_t)a->d_positions, (int64_t)a->d_slots,

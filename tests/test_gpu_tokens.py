@@ -225,6 +225,33 @@ def test_attention_matches_the_oracle(ops, exp_table, lens, first, H, HK, D, pag
         assert ops.wit_status() == 0
 
 
+@pytest.mark.parametrize("seqs,longest,H,HK,D,page", [(7, 700, 4, 2, 64, 16), (8, 700, 4, 2, 64, 16), (63, 300, 2, 1, 40, 9), (64, 260, 2, 2, 32, 16), (65, 400, 3, 3, 16, 5),
+                                                     (130, 300, 2, 1, 20, 16), (256, 290, 1, 1, 16, 8), (257, 290, 1, 1, 16, 8), (9, 500, 1, 1, 1024, 16), (200, 2, 1, 1, 300, 1)])
+@pytest.mark.parametrize("windows", [False, True])
+def test_attention_of_many_sequences(ops, exp_table, seqs, longest, H, HK, D, page, windows):
+    """of every length, some of none, some refused"""
+    rng = np.random.default_rng(seqs + longest)
+    lens = [int(n) for n in rng.integers(0, longest + 1, seqs)]
+    lens[0], lens[seqs // 2], lens[-1] = 0, longest, 0
+    if seqs > 64:
+        lens[60:64] = [0] * 4
+    first = [int(rng.integers(0, n + 2)) for n in lens] if windows else None
+    table, kc, vc = paged(rng, lens, page, HK, D)
+    q = gauss(rng, (seqs, H, D))
+    full = run_attention(ops, q, kc, vc, table, lens, first, exp_table, longest, qk_scale=1 << 20)
+    assert ops.wit_status() == 0
+    full = {x: host(t).copy() for x, t in full.items()}
+    bad = np.array(lens)
+    wrong = [1, seqs // 2 - 1, seqs - 2]
+    bad[wrong] = [-1, longest + 1, -(1 << 31)]
+    got = {x: filled(*t.shape) for x, t in full.items()}
+    ops.wit_paged_attention(dev(q), dev(kc), dev(vc), dev(table), dev(bad), longest, dev(exp_table), first=None if first is None else dev(np.array(first)), out=got, qk_scale=1 << 20)
+    assert ops.wit_status() == 2
+    for x, t in full.items():
+        t[wrong] = UNTOUCHED if t.ndim == 3 and t.shape[2] == longest and x in PROOF else 0
+        assert np.array_equal(host(got[x]), t), x
+
+
 @pytest.mark.parametrize("prob_scale,out_scale", [(1 << 22, 1 << 22), (1 << 30, 1 << 31), (1, 1), (3000, 777), ((1 << 22) + 1, 1 << 20)])
 def test_attention_over_its_scales(ops, exp_table, prob_scale, out_scale):
     rng = np.random.default_rng(prob_scale % 1000)

@@ -189,6 +189,21 @@ def test_plans_cover_every_position_within_their_limits(lib):
     assert taken > 1000 and split > 300
 
 
+def test_counted_launches_fit_one_axis(lib):
+    names = "dim64 rows tiles score_chunk score_chunks exp_chunk exp_chunks blocks groups value_chunk value_chunks".split()
+    out = (ctypes.c_uint64 * 19)()
+    seen = set()
+    for s, h, hk, d, n in ((7, 8, 8, 64, 1000), (8, 8, 8, 64, 1000), (8, 8, 8, 64, 0), (256, 32, 8, 128, 2048), (257, 32, 8, 128, 2048), (256, 65535, 65535, 64, 64), (256, 512, 512, 128, 4096),
+                           (8, 65535, 65535, 8, 1000), (250, 16, 1, 8192, 100000), (256, 1, 1, 8192, 1 << 20)):
+        counted = lib.counted(s, h, hk, d, n)
+        if counted == 1:
+            lib.plan_of(s, h, hk, d, n, out)
+            p = dict(zip(names, out))
+            assert 8 <= s <= 256 and s * hk * p["tiles"] * max(p["score_chunks"], p["value_chunks"] * p["groups"], 1) * 256 < 1 << 31
+        seen.add(counted)
+    assert seen >= {0, 1} and lib.counted(64, 32, 8, 128, 2048) == 1 and lib.counted(1, 32, 8, 128, 131072) == 0
+
+
 def test_workspace_sizes(lib):
     assert lib.q4_workspace(1, 1 << 20, 1 << 20, 128) == 0 and lib.q4_workspace(4, 4096, 4096, 128) == 0
     assert lib.q4_workspace(9, 64, 4096, 100) == 0 and lib.q4_workspace(9, 64, 0, 32) == 0 and lib.q4_workspace(9, 0, 64, 32) == 0
