@@ -211,6 +211,33 @@ constexpr int kQ4Waves = 8, kQ4Threads = 64 * kQ4Waves;
 // waves of a workgroup for up to four tokens at most: four scales a lane need the registers of twice as many
 constexpr uint32_t q4_most_waves(int gs) { return gs == 32 ? 8 : 16; }
 
+// N bytes of a weight row of `bytes`, from `at`.  Where they pass the row's end, the row's last N are read and shifted instead (a
+// loop over bytes takes a load's latency for each: one token through 16384 x 1000 9.9 us a call and not 7.2, 4096 x 2033 9.4 and
+// not 7.2); what stands behind the end then meets digits of zero, whatever it is.
+template <int N>
+__device__ __forceinline__ void q4_bytes(const uint8_t* s, uint32_t at, uint32_t bytes, uint32_t* out) {
+    if (bytes >= N) {
+        const uint32_t from = min(at, bytes - N), past = at - from;
+        uint64_t v[2] = {0, 0};
+        __builtin_memcpy(v, s + from, N);
+        if (past) {
+            if (past & 8u) v[0] = v[1];
+            const uint32_t bits = 8 * (past & 7u);
+            v[0] >>= bits;
+            if (bits) v[0] |= v[1] << (64 - bits);
+            v[1] >>= bits;
+        }
+        __builtin_memcpy(out, v, N);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N / 4; j++) {
+            out[j] = 0;
+#pragma unroll 1
+            for (uint32_t b = 0; b < 4; b++) out[j] |= (at + 4 * j + b < bytes ? (uint32_t)s[at + 4 * j + b] : 0u) << (8 * b);
+        }
+    }
+}
+
 // Four units of 128 inputs of 16 weight rows.  A wave reads 256 bytes in a row among 16 neighbouring lanes, then turns them over
 // through 4 KB of LDS of its own into the operands, where 16 neighbouring lanes hold 16 rows: read as operands in the first place,
 // every lane's 16 bytes would be a line of memory of their own, and so would the scales (22.5 MB of weights with scales and zero
@@ -226,18 +253,7 @@ struct Q4Quad {
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) {
             const uint8_t* s = p.w + min(m0 + 4 * i + (lane >> 4), p.outputs - 1) * p.w_stride;
-            if (at + 16 <= bytes) {
-                __builtin_memcpy(&w[i], s + at, 16);
-            } else {
-                // the row's last bytes; what follows them meets digits of zero
-#pragma unroll
-                for (uint32_t j = 0; j < 4; j++) {
-                    uint32_t word = 0;
-#pragma unroll 1
-                    for (uint32_t b = 0; b < 4; b++) word |= (at + 4 * j + b < bytes ? (uint32_t)s[at + 4 * j + b] : 0u) << (8 * b);
-                    w[i][j] = (int)word;
-                }
-            }
+            q4_bytes<16>(s, at, bytes, reinterpret_cast<uint32_t*>(&w[i]));
         }
         const uint32_t row = min(m0 + (lane >> 2), p.outputs - 1), u = unit + (lane & 3u);
         const size_t first = (size_t)row * p.groups;
@@ -274,29 +290,15 @@ struct Q4Unit {
     __device__ __forceinline__ void load(const Q4Args& p, uint32_t row, uint32_t unit, uint32_t kg) {
         const uint8_t* s = p.w + row * p.w_stride;
         const uint32_t bytes = (p.inputs + 1) / 2, base = unit * 64;
-        if (base + 64 <= bytes) {
-            union { v4i_t v; uint32_t u[4]; uint2 d[2]; } o;
+        union { v4i_t v; uint32_t u[4]; } o;
+        if (CB < 16 && base + 64 <= bytes) {          // several shifts less
 #pragma unroll
-            for (int c = 0; c < 16 / CB; c++) {
-                const uint8_t* at = s + base + c * (GS / 2) + kg * CB;
-                if constexpr (CB == 16) __builtin_memcpy(&o.v, at, 16);
-                else if constexpr (CB == 8) __builtin_memcpy(&o.d[c], at, 8);
-                else __builtin_memcpy(&o.u[c], at, 4);
-            }
-            w = o.v;
+            for (int c = 0; c < 16 / CB; c++) __builtin_memcpy(o.u + c * CB / 4, s + base + c * (GS / 2) + kg * CB, CB);
         } else {
-            // the row's last bytes; what follows them meets digits of zero
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t word = 0;
-#pragma unroll 1
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t b = 4 * c + i, at = base + b / CB * (GS / 2) + kg * CB + b % CB;
-                    word |= (at < bytes ? (uint32_t)s[at] : 0u) << (8 * i);
-                }
-                w[c] = (int)word;
-            }
+            for (int c = 0; c < 16 / CB; c++) q4_bytes<CB>(s, base + c * (GS / 2) + kg * CB, bytes, o.u + c * CB / 4);
         }
+        w = o.v;
         const size_t first = (size_t)row * p.groups;
         if (p.group == GS && (unit + 1) * STEPS <= p.groups) {          // neighbours
             __builtin_memcpy(scale, p.scales + first + unit * STEPS, 4 * STEPS);
@@ -559,7 +561,9 @@ __global__ void __launch_bounds__(kQ4Threads, 2) wit_q4_many_kernel(Q4Args p, ui
     for (int t = 0; t < RT; t++)
 #pragma unroll
         for (int j = 0; j < NT; j++) y[t][j][0] = y[t][j][1] = 0;
-    const uint32_t share = (units + kQ4Waves - 1) / kQ4Waves, first = min(wave * share, units), last = min(first + share, units);
+    // shares of whole fours where the weights go through LDS, unless that leaves most waves without one
+    const uint32_t even = (units + kQ4Waves - 1) / kQ4Waves, share = kTurns && even > 2 ? (even + 3) / 4 * 4 : even;
+    const uint32_t first = min(wave * share, units), last = min(first + share, units);
     typedef typename std::conditional<GS == 32, long, v4i_t>::type operand_t;
     if constexpr (kTurns) {
         uint8_t* turned = lds + wave * RT * 4096;

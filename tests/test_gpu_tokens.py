@@ -394,6 +394,24 @@ def test_q4_matches_the_oracle(ops, n, m, k, group):
     assert ops.wit_status() == 0
 
 
+@pytest.mark.parametrize("n", [1, 3, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_q4_of_rows_that_end_anywhere(ops, n, group):
+    rng = np.random.default_rng(n + group)
+    for k in (1, 2, 7, 8, 9, 15, 31, 32, 33, 63, 65, 95, 127, 129, 160, 223, 255, 257, 500, 511, 513, 1000, 1025, 2047):
+        # two to four tokens through that many rows have their digits made beforehand, as more tokens always have
+        m = 16 * (40000 // (n * ((k + 127) // 128))) + 17 if 2 <= n <= 4 and k in (1000, 1025) else 17
+        x, w, scales, zeros = q4_case(rng, n, m, k, group)
+        want = wo.matvec_q4(x, w, scales, group, zeros)
+        # rows that stand at any byte, between others that hold anything
+        wide = dev(rng.integers(0, 256, (m, w.shape[1] + 5), dtype=np.uint8))
+        rows = wide[:, 3:3 + w.shape[1]]
+        rows.copy_(dev(w))
+        got = ops.wit_matvec_q4(dev(x), rows, dev(scales), group, zeros=dev(zeros))
+        assert np.array_equal(host(got[0]), want[0]) and np.array_equal(host(got[1]), want[1]), k
+    assert ops.wit_status() == 0
+
+
 def test_q4_equals_the_product_with_the_weights_written_out(ops):
     rng = np.random.default_rng(3)
     x, w, scales, zeros = q4_case(rng, 5, 300, 512, 64)
