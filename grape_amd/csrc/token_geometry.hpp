@@ -83,6 +83,7 @@ inline const char* refuse_append(const grape_wit_rope_append_args* a, const grap
     GRAPE_REFUSE(cache_overlaps(*c), "different slots of the cache share elements");
     GRAPE_REFUSE(a->q_stride < 0 || a->k_stride < 0 || a->v_stride < 0, "negative stride");
     if (a->tokens == 0) return nullptr;
+    GRAPE_REFUSE(a->tokens > (uint32_t)1 << 24, "at most 2^24 tokens");          // each workgroup looks through the later ones' slots
     GRAPE_REFUSE(!a->d_k || !a->d_v || !a->d_slots, "d_k, d_v or d_slots is null");
     GRAPE_REFUSE(a->heads && (!a->d_q || !a->d_q_out), "d_q or d_q_out is null");
     GRAPE_REFUSE(a->rot && (!a->d_positions || !a->d_cos || !a->d_sin || !a->table_rows), "the positions or their tables are missing");
@@ -231,6 +232,7 @@ inline const char* refuse_attention(const grape_wit_attention_args* a, const gra
 // little work for them (4 tokens through 4096 x 4096: 8.3 us a call and not 11); more by a launch of its own, into the workspace, in
 // tiles of four, eight or sixteen (4 tokens through 16384 x 8192: 24 us and not 44).  One word a block of 2048 inputs of a token
 // says what its digits lack.
+constexpr uint32_t kQ4Inputs = (uint32_t)1 << 24;          // a thread looks through a row's for those above the digits
 inline bool q4_few(uint32_t tokens, uint32_t outputs, uint32_t inputs) {
     const uint64_t tiles = ceil_div(outputs, 16) < 256 ? 256 : ceil_div(outputs, 16);
     return tokens == 1 || (tokens <= 4 && tiles * tokens * ceil_div(inputs, 128) <= 40000);
@@ -251,7 +253,7 @@ inline Q4Plan q4_plan(uint32_t tokens, uint32_t inputs) {
     return p;
 }
 inline size_t q4_workspace(uint32_t tokens, uint32_t outputs, uint32_t inputs, uint32_t group) {
-    if (!tokens || !outputs || !inputs || !group || group % 32 || tokens > 65535 || inputs > (uint32_t)1 << 30 || q4_few(tokens, outputs, inputs)) return 0;
+    if (!tokens || !outputs || !inputs || !group || group % 32 || tokens > 65535 || inputs > kQ4Inputs || q4_few(tokens, outputs, inputs)) return 0;
     return q4_plan(tokens, inputs).bytes;
 }
 
@@ -259,7 +261,7 @@ inline const char* refuse_q4(const void* d_q, const void* d_x, int64_t x_stride,
                              uint32_t tokens, uint32_t outputs, uint32_t inputs, uint32_t group, int64_t scale, const void* d_workspace, size_t workspace_bytes) {
     GRAPE_REFUSE(scale < 1 || scale > (int64_t)1 << 31, "scale must be in 1..2^31 (the remainder is stored as int32)");
     GRAPE_REFUSE(inputs < 1 || group < 1, "empty inner dimension or group");
-    GRAPE_REFUSE(inputs > (uint32_t)1 << 30 || group > (uint32_t)1 << 30, "at most 2^30 inputs");
+    GRAPE_REFUSE(inputs > kQ4Inputs || group > (uint32_t)1 << 30, "at most 2^24 inputs");
     GRAPE_REFUSE(x_stride < 0 || w_stride < 0, "negative stride");
     if (!tokens || !outputs) return nullptr;
     GRAPE_REFUSE(!d_q || !d_x || !d_w || !d_scales, "d_q, d_x, d_w or d_scales is null");

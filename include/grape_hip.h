@@ -718,7 +718,8 @@ typedef struct {
  *
  * A negative slot marks padding: nothing of that token is written.  A slot behind the cache's end or a position outside the
  * tables sets GRAPE_WIT_INDEX, and nothing of that token is written either.  Where several tokens name one slot, the last of
- * them has its rows there.  Different slots must not share elements of the cache (checked from the strides). */
+ * them has its rows there.  Different slots must not share elements of the cache (checked from the strides).  At most 2^24
+ * tokens a call. */
 typedef struct {
     const int32_t *d_q, *d_k, *d_v;
     int64_t q_stride, k_stride, v_stride;
@@ -765,7 +766,7 @@ int grape_wit_paged_attention(const grape_wit_attention_args *args, const grape_
  * grape_wit_matmul_rescale does it - its result for the weights written out as integers.  Token n's inputs stand at
  * d_x + n*x_stride; row m of the weights at d_w + m*w_stride bytes, two to a byte, the even k in the lower half, (inputs + 1)/2
  * bytes; scales int32 and zero points bytes (d_zeros NULL: all 8), ceil(inputs/group) a row; outputs [tokens][outputs], d_r
- * may be NULL.  1 <= scale <= 2^31, tokens <= 65535, outputs <= 2^24, group and inputs <= 2^30.  Groups of whole 32s go through
+ * may be NULL.  1 <= scale <= 2^31, tokens <= 65535, outputs and inputs <= 2^24, group <= 2^30.  Groups of whole 32s go through
  * the matrix cores.  d_workspace as above, grape_wit_matvec_q4_workspace(...) bytes (none for one
  * token, and for up to four where the weights are few). */
 size_t grape_wit_matvec_q4_workspace(uint32_t tokens, uint32_t outputs, uint32_t inputs, uint32_t group);

@@ -105,6 +105,18 @@ def test_bad_products_are_refused(lib, bad):
     assert lib.refuse_q4(*{**good, **bad}.values())
 
 
+def test_calls_whose_time_grows_with_a_square_are_bounded(lib):
+    """a workgroup of the append looks through all later slots, a product with an input above the digits through all of a row"""
+    few = cache(heads=1, dim=1, hs=1, ts=1, ps=16)
+    one = dict(heads=0, q=0, qo=0, rot=0, pos=0, cos=0, sin=0, rows=0)
+    assert lib.refuse_append(append(n=1 << 24, **one), few) is None
+    for n in ((1 << 24) + 1, 1 << 31, (1 << 32) - 200, (1 << 32) - 1):
+        assert lib.refuse_append(append(n=n, **one), few)
+    good = dict(q=16, x=16, xs=1 << 24, w=16, ws=1 << 23, sc=16, n=1, m=8, k=1 << 24, group=32, scale=65536, sp=0, sb=0)
+    assert lib.refuse_q4(*good.values()) is None
+    assert lib.refuse_q4(*{**good, "k": (1 << 24) + 1}.values()) and lib.q4_workspace(5, 8, (1 << 24) + 1, 32) == 0 < lib.q4_workspace(5, 8, 1 << 24, 32)
+
+
 def test_overlapping_caches_are_found(lib):
     """against the elements themselves"""
     rng = np.random.default_rng(1)
