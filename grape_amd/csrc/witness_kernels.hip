@@ -699,10 +699,16 @@ int wit_status_word(uint32_t** out, hipStream_t s) {
     GRAPE_HIP_CHECK(hipGetDevice(&dev));
     GRAPE_REQUIRE(dev >= 0 && dev < 16, "device index out of range");
     if (!g_status[dev]) {
-        GRAPE_HIP_CHECK(hipMalloc((void**)&g_status[dev], 256));
-        wit_status_clear_kernel<<<1, 1, 0, s>>>(g_status[dev]);
+        // grape_init has made that of its device; a first call on another must not be captured, as it allocates and waits
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        GRAPE_HIP_CHECK(hipStreamIsCapturing(s, &capture));
+        GRAPE_REQUIRE(capture == hipStreamCaptureStatusNone, "the first witness call on a device must not be captured");
+        uint32_t* word = nullptr;
+        GRAPE_HIP_CHECK(hipMalloc((void**)&word, 256));
+        wit_status_clear_kernel<<<1, 1, 0, s>>>(word);
         GRAPE_LAUNCH_CHECK();
         GRAPE_HIP_CHECK(hipStreamSynchronize(s));
+        g_status[dev] = word;
     }
     *out = g_status[dev];
     return GRAPE_OK;

@@ -641,3 +641,37 @@ def test_attention_on_two_streams_at_once(ops, exp_table):
         for x, y in zip(got, good):
             assert all(torch.equal(x[n], y[n]) for n in y)
     assert ops.wit_status() == 0
+
+
+FIRST_CALL_CAPTURED = """
+import numpy as np, torch
+from grape_amd import ops
+from oracle import witness_oracle as wo
+ops.init()
+rng = np.random.default_rng(1)
+x, w = rng.integers(-1000, 1000, (1, 100)).astype(np.int32), rng.integers(0, 256, (40, 50)).astype(np.uint8)
+scales = rng.integers(-400, 400, (40, 4)).astype(np.int32)
+dx, dw, ds = (torch.from_numpy(a).cuda() for a in (x, w, scales))
+q, r = torch.zeros((1, 40), dtype=torch.int32, device="cuda"), torch.zeros((1, 40), dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.wit_matvec_q4(dx, dw, ds, 32, q=q, r=r)
+for _ in range(3):
+    q.fill_(-1), r.fill_(-1)
+    graph.replay()
+    torch.cuda.synchronize()
+    want = wo.matvec_q4(x, w, scales, 32, None)
+    assert np.array_equal(q.cpu().numpy(), want[0]) and np.array_equal(r.cpu().numpy(), want[1])
+assert ops.wit_status() == 0
+print("captured")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], cwd=here, capture_output=True, text=True, timeout=100)
+    assert res.returncode == 0 and "captured" in res.stdout, res.stderr
