@@ -716,20 +716,21 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
         unsigned long long sum = 0;
 #pragma unroll 1
         for (uint32_t first = from; first < n; first += 4 * each) {          // four gathers under way a thread
-            int32_t e[4];
+            int32_t x[4], e[4];
 #pragma unroll
             for (uint32_t a = 0; a < 4; a++) {
                 const uint32_t i = first + a * each;
-                const int64_t idx = (int64_t)(int32_t)scores[r * C + min(i, n - 1)] - mx + (((int64_t)1 << p.a.bit_shift) - 1);
+                x[a] = i < n ? (int32_t)scores[r * C + i] : mx;          // its own positions only: the others' become exponentials meanwhile
+                const int64_t idx = (int64_t)x[a] - mx + (((int64_t)1 << p.a.bit_shift) - 1);
                 const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
-                if (!ok) bad |= (uint32_t)kWitIndex;
+                if (!ok && i < n) bad |= (uint32_t)kWitIndex;
                 e[a] = p.a.d_exp_table[ok ? idx : 0];
             }
 #pragma unroll
             for (uint32_t a = 0; a < 4; a++) {
                 const uint32_t i = first + a * each;
                 if (i >= n) break;
-                if (p.a.d_shifted) p.a.d_shifted[o + i] = (int32_t)((int64_t)(int32_t)scores[r * C + i] - mx);
+                if (p.a.d_shifted) p.a.d_shifted[o + i] = (int32_t)((int64_t)x[a] - mx);
                 if (p.a.d_exp) p.a.d_exp[o + i] = e[a];
                 if (e[a] < 0) bad |= (uint32_t)kWitSum;
                 e[a] = max(e[a], 0);
