@@ -313,9 +313,15 @@ __device__ __forceinline__ uint32_t probability(uint32_t e, uint64_t scale, uint
     return (uint32_t)q;
 }
 
-// 2 * scale * e - sum * (2 * prob - 1), its low 32 bits
-__device__ __forceinline__ int32_t lookup_query(uint32_t e, int64_t scale, uint64_t sum, uint32_t prob) {
-    return (int32_t)((uint64_t)e * 2 * (uint64_t)scale - sum * (2 * (uint64_t)prob - 1));
+// 2 * scale * e - sum * (2 * prob - 1), within 0 .. 2 sum: less than 2^63
+__device__ __forceinline__ uint64_t lookup_query(uint32_t e, int64_t scale, uint64_t sum, uint32_t prob) {
+    return (uint64_t)e * 2 * (uint64_t)scale - sum * (2 * (uint64_t)prob - 1);
+}
+
+// Where a tensor of the proof holds a sum or a query, its low 32 bits; the bit says that they are not all of it.
+__device__ __forceinline__ void store_sum(int32_t* to, uint64_t x, uint32_t& bad) {
+    bad |= x > (uint64_t)INT32_MAX ? (uint32_t)kWitSumWide : 0u;
+    *to = (int32_t)x;
 }
 
 // The threads of a workgroup that share a query head: as many as there are for each, a power of two, in lanes side by side.
@@ -343,7 +349,7 @@ struct RowThreads {
 // pages outside the cache.  Returns the sum of the probabilities that the values are multiplied with.
 template <int PP, uint32_t AHEAD, class F>          // planes of the probabilities, positions under way a thread
 __device__ __forceinline__ unsigned long long probabilities(const AttendArgs& p, const Tile& w, const RowThreads& row, uint32_t t0, uint32_t n, const int64_t* off,
-                                                            unsigned long long sum, bool write, uint32_t* digits, F load) {
+                                                            unsigned long long sum, bool write, uint32_t* digits, uint32_t& bad, F load) {
     const size_t o = (w.row0 + row.r) * p.a.max_len + t0;
     const double inv = 1.0 / (double)sum;
     const uint32_t filled = (n + 31) / 32 * 32;
@@ -362,7 +368,7 @@ __device__ __forceinline__ unsigned long long probabilities(const AttendArgs& p,
                 pr = probability(e[a], (uint64_t)p.a.prob_scale, sum, inv);
                 if (write) {
                     if (p.a.d_prob) p.a.d_prob[o + i] = (int32_t)pr;
-                    if (p.a.d_query) p.a.d_query[o + i] = lookup_query(e[a], p.a.prob_scale, sum, pr);
+                    if (p.a.d_query) store_sum(&p.a.d_query[o + i], lookup_query(e[a], p.a.prob_scale, sum, pr), bad);
                 }
                 if (off[i] < 0) pr = 0;
             }
@@ -593,9 +599,9 @@ __global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p)
             bad |= (uint32_t)kWitSum;
             sum = 1;
         }
-        if (chunk == 0 && group == 0 && row.from == 0 && p.a.d_sum) p.a.d_sum[at] = (int32_t)sum;
+        if (chunk == 0 && group == 0 && row.from == 0 && p.a.d_sum) store_sum(&p.a.d_sum[at], sum, bad);
         const int32_t* exps = p.a.d_exp + at * p.a.max_len + t0;
-        const unsigned long long mine = probabilities<PP, kProbAhead>(p, w, row, t0, n, off, sum, group == 0, lds, [&](uint32_t i) { return (uint32_t)max(exps[i], 0); });
+        const unsigned long long mine = probabilities<PP, kProbAhead>(p, w, row, t0, n, off, sum, group == 0, lds, bad, [&](uint32_t i) { return (uint32_t)max(exps[i], 0); });
         if (row.leads) atomicAdd(&p_sum[row.r], mine);
     }
     __syncthreads();
@@ -750,9 +756,9 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
         }
         if (from == 0) {
             if (p.a.d_max) p.a.d_max[w.row0 + r] = row_max[r];
-            if (p.a.d_sum) p.a.d_sum[w.row0 + r] = (int32_t)sum;
+            if (p.a.d_sum) store_sum(&p.a.d_sum[w.row0 + r], sum, bad);
         }
-        const unsigned long long all = probabilities<PP, 1>(p, w, row, lo, n, off, sum, true, digits, [&](uint32_t i) { return scores[r * C + i]; });
+        const unsigned long long all = probabilities<PP, 1>(p, w, row, lo, n, off, sum, true, digits, bad, [&](uint32_t i) { return scores[r * C + i]; });
         if (leads) atomicAdd(&p_sum[r], all);
     }
     __syncthreads();

@@ -845,7 +845,7 @@ def wit_paged_attention(q, k_cache, v_cache, block_table, lens, max_len, exp_tab
     page size, cache heads, dim) through block_table (seqs, pages of a sequence).  Returns a dict: "qkv" and "qkv_rem" (seqs,
     heads, dim); for a proof also "max" and "exp_sum" (seqs, heads) and "scores", "scores_rem", "exp_input", "exp_output",
     "softmax_output", "softmax_lookup_query" (seqs, heads, max_len), whose entries outside a sequence's positions are not
-    written.  `out`: such a dict of tensors to write to; "qkv" has to be there, the others may be left out.  `workspace`: a uint8
+    written; a sum or lookup query beyond int32 sets bit 16 of wit_status.  `out`: such a dict of tensors to write to; "qkv" has to be there, the others may be left out.  `workspace`: a uint8
     tensor of wit_paged_attention_workspace(...) bytes; without one the call makes its own."""
     lib = init()
     dev = _place()

@@ -738,7 +738,10 @@ int grape_wit_rope_append(const grape_wit_rope_append_args *args, const grape_wi
  *     scores = rescale(q . k_t, qk_scale), max over t, shifted = score - max, exp = d_exp_table[shifted + 2^bit_shift - 1]
  *     (2^index_bits entries), sum of exp, prob = floor((exp*prob_scale + floor(sum/2)) / sum),
  *     query = 2*prob_scale*exp - sum*(2*prob - 1), out = rescale(sum_t prob_t v_t, out_scale)
- * - grape_wit_matmul_rescale, grape_wit_softmax and grape_wit_matmul_rescale again, with the same bits of status.
+ * - grape_wit_matmul_rescale, grape_wit_softmax and grape_wit_matmul_rescale again, with the same bits of status.  Sums are held
+ * in 64 bits.  d_sum and d_query get the low 32 of a row's sum and of its queries, which lie in 0..2*sum: where one of them does
+ * not fit int32 (entries of 2^16: rows of some 16384 equal scores on) GRAPE_WIT_SUM_WIDE is set, and the row cannot be looked
+ * up from them.  All other outputs are exact there too.
  * The rows of a proof, [seqs][heads][max_len], d_scores, d_scores_rem, d_shifted, d_exp, d_prob and d_query, and
  * d_max, d_sum [seqs][heads] and d_out_rem may each be NULL; d_out and d_out_rem are [seqs][heads][dim].  Positions outside
  * first..len are left as they were; a row with no position has max, sum, out and remainder 0.
@@ -775,11 +778,13 @@ int grape_wit_matvec_q4(int32_t *d_q, int32_t *d_r, const int32_t *d_x, int64_t 
                         uint32_t group, int64_t scale, void *d_workspace, size_t workspace_bytes, grape_stream_t stream);
 /* Synchronises, returns the status bits set since the last call and clears them: 1 = a quotient left
  * int32, 2 = a table index out of range (the reference's assertions, model.py:86-87, :137-138),
- * 4 = a softmax row summed to zero or met a negative table entry, 8 = a sum of squares left 64 bits. */
+ * 4 = a softmax row summed to zero or met a negative table entry, 8 = a sum of squares left 64 bits,
+ * 16 = a sum of exponentials or a lookup query that grape_wit_paged_attention was asked for left int32. */
 #define GRAPE_WIT_QUOTIENT 1u
 #define GRAPE_WIT_INDEX 2u
 #define GRAPE_WIT_SUM 4u
 #define GRAPE_WIT_SQUARES 8u
+#define GRAPE_WIT_SUM_WIDE 16u
 int grape_wit_status(uint32_t *flags, grape_stream_t stream);
 
 /* ------------------------------------------------------------------ measurement -------------- */

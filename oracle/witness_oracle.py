@@ -236,7 +236,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lens, first, table, out, q
                         out[name][b, h, first[b]:lens[b]] = np.asarray(x).astype(np.int64).astype(np.int32)
             for name, x in one.items():
                 if name in out:
-                    out[name][b, h] = x
+                    out[name][b, h] = np.asarray(x).astype(np.int64).astype(np.int32)          # a sum's low 32 bits
 
 
 def unpack_q4(w, inputs):

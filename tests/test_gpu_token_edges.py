@@ -28,3 +28,50 @@ def test_equal_scores_set_no_bit(ops, exp_table, each, score):
         assert ops.wit_status() == 0
         assert bool((got["scores"][0] == score).all()) and bool((got["exp_output"][0] == 1 << 16).all())
         assert ops.wit_status() == 0
+
+
+# ------------------------------------------------------------------ sums and lookup queries that leave int32
+ROWS = ("scores", "scores_rem", "exp_input", "exp_output", "softmax_output")          # of a proof, in 32 bits whatever the sum is
+INT32 = range(-(1 << 31), 1 << 31)
+
+
+def attend_flat(ops, lens, exp, out, H=2, HK=1, D=8, page=64, **kw):
+    """rows of equal scores over caches of ordinary values; what the call gave, the oracle's outputs and the sums and queries as whole numbers"""
+    rng = np.random.default_rng(sum(lens))
+    table, kc, vc = paged(rng, lens, page, HK, D)
+    q = np.zeros((len(lens), H, D), dtype=np.int32)
+    shapes = {"qkv": (len(lens), H, D), "qkv_rem": (len(lens), H, D), "max": (len(lens), H), "exp_sum": (len(lens), H)}
+    got = {x: filled(*shapes.get(x, (len(lens), H, max(lens)))) for x in out}
+    want = {x: np.full(t.shape, -77, dtype=np.int32) for x, t in got.items()}
+    wo.paged_attention(q, kc, vc, table, lens, [0] * len(lens), exp, want, **kw)
+    ops.wit_paged_attention(dev(q), dev(kc), dev(vc), dev(table), dev(np.array(lens)), max(lens), dev(exp), out=got, **kw)
+    e = int(exp[(1 << 20) - 1])
+    sums = [n * e for n in lens if n]
+    prob = kw.get("prob_scale", 1 << 16)
+    queries = [2 * prob * e - s * (2 * ((e * prob + s // 2) // s) - 1) for s in sums]
+    return got, want, sums, queries
+
+
+@pytest.mark.parametrize("lens", [[16384], [32767], [32768], [65536, 100], [0, 40000, 3], [131072]])
+def test_sums_and_queries_beyond_32_bits_are_reported(ops, exp_table, lens):
+    """each entry is 2^16: a sum of 32768 and a query of some 16384 positions on leave int32, and 65536 positions' sum is 0 in 32 bits"""
+    for names, of in ((ROWS + ("max",), ()), (("exp_sum",), ("sum",)), (("softmax_lookup_query",), ("query",)), (("exp_sum", "softmax_lookup_query"), ("sum", "query")), ((), ())):
+        got, want, sums, queries = attend_flat(ops, lens, exp_table, ("qkv", "qkv_rem") + names)
+        wide = ("sum" in of and any(s not in INT32 for s in sums)) or ("query" in of and any(s not in INT32 for s in queries))
+        assert ops.wit_status() == (16 if wide else 0), (names, sums, queries)
+        for x in got:                                                             # the answer is exact, the low 32 bits are stored
+            assert np.array_equal(got[x].cpu().numpy(), want[x]), x
+
+
+@pytest.mark.parametrize("lens", [[200], [250, 1, 0], [900, 300]])
+@pytest.mark.parametrize("entry", [(1 << 31) // 250, (1 << 31) // 249, 1 << 30, (1 << 31) - 1])
+def test_sums_of_large_entries_are_reported(ops, lens, entry):
+    """the same up to 256 positions, where the call is one launch, with a table of larger entries"""
+    table = np.full(1 << 20, entry, dtype=np.int32)
+    for prob_scale in (1 << 16, 3000):
+        got, want, sums, queries = attend_flat(ops, lens, table, ("qkv", "qkv_rem", "exp_sum", "softmax_lookup_query") + ROWS, H=3, HK=3, prob_scale=prob_scale)
+        assert ops.wit_status() == (16 if any(s not in INT32 for s in sums + queries) else 0)
+        got2, _, _, _ = attend_flat(ops, lens, table, ("qkv",), H=3, HK=3, prob_scale=prob_scale)
+        assert ops.wit_status() == 0 and torch.equal(got2["qkv"], got["qkv"])
+        for x in got:
+            assert np.array_equal(got[x].cpu().numpy(), want[x]), x
