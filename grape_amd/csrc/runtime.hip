@@ -9,7 +9,6 @@
 #include <thread>
 #include <vector>
 #include "common.hpp"
-#include "witness_device.hpp"
 
 namespace grape {
 
@@ -311,15 +310,6 @@ int grape_init(int device) {
     }
     g_init = true;
     touch_exit_sentinel();
-    // the witness calls' status word, so that the first of them may be captured
-    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(nullptr, &capture) == hipSuccess && capture == hipStreamCaptureStatusNone) {
-        uint32_t* word;
-        const int rc = wit_status_word(&word, nullptr);
-        if (rc) return rc;
-    } else {
-        (void)hipGetLastError();
-    }
     return noalloc_setup();
 }
 const char* grape_last_error(void) { return g_err; }

@@ -806,7 +806,7 @@ int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_
     p.qk = scaler(a.qk_scale);
     p.out = scaler(a.out_scale);
     hipStream_t s = as_stream(st);
-    const int rc = wit_status_word(&p.status, s);
+    const int rc = wit_status_word(&p.status);
     if (rc) return rc;
     auto aligned = [&](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
     const bool vec = p.c.dim % 4 == 0 && ((p.c.page_stride | p.c.token_stride | p.c.head_stride) & 3) == 0 && aligned(p.c.d_k) && aligned(p.c.d_v);

@@ -721,7 +721,7 @@ int grape_wit_rope_append(const grape_wit_rope_append_args* args, const grape_wi
     p.by_page = token::fast_div(p.c.page_size);
     p.scale = scaler(a.scale);
     hipStream_t s = as_stream(st);
-    const int rc = wit_status_word(&p.status, s);
+    const int rc = wit_status_word(&p.status);
     if (rc) return rc;
     const unsigned grid = (unsigned)((p.total + per - 1) / per);
     if (vec) wit_append_kernel<4><<<grid, kBlock, 0, s>>>(p);
@@ -749,7 +749,7 @@ int grape_wit_matvec_q4(int32_t* d_q, int32_t* d_r, const int32_t* d_x, int64_t 
     p.digits = (uint32_t*)d_workspace;
     p.over = (uint32_t*)((uint8_t*)d_workspace + token::q4_plan(tokens, inputs).at_over);
     hipStream_t s = as_stream(st);
-    const int rc = wit_status_word(&p.status, s);
+    const int rc = wit_status_word(&p.status);
     if (rc) return rc;
     if (group % 32) {
         wit_q4_any_kernel<<<dim3((outputs + 3) / 4, (tokens + 3) / 4), kBlock, 0, s>>>(p);

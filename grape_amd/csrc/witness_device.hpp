@@ -29,7 +29,7 @@ static inline int log2_exact(int64_t s) {
     return sh;
 }
 
-// the current device's status word, made by grape_init or else on its first use (which waits for the stream and must not be captured)
-int wit_status_word(uint32_t** out, hipStream_t s);
+// the current device's status word
+int wit_status_word(uint32_t** out);
 
 }  // namespace grape

@@ -8,6 +8,7 @@
 // Conditions the reference asserts (table indices in range, model.py:86-87) or silently assumes
 // (quotients fit 32 bits) are recorded in a sticky device-side status word, read and cleared by
 // grape_wit_status().
+#include <atomic>
 #include "common.hpp"
 #include "witness_device.hpp"
 
@@ -692,25 +693,24 @@ __global__ void __launch_bounds__(kBlock) wit_rmsnorm_apply_kernel(int32_t* q_rm
 
 __global__ void wit_status_clear_kernel(uint32_t* status) { *status = 0; }
 
-static uint32_t* g_status[16] = {nullptr};
+// In the code object, which zeroes it as it is loaded: a first call neither allocates nor waits, so that it may be captured, on
+// any device.  Its address is looked up once a device.
+static __device__ __align__(256) uint32_t status_word[64];
+constexpr int kMaxDevices = 64;
+static std::atomic<uint32_t*> g_status[kMaxDevices];
 
-int wit_status_word(uint32_t** out, hipStream_t s) {
-    int dev = 0;
+int wit_status_word(uint32_t** out) {
+    int dev = -1;
     GRAPE_HIP_CHECK(hipGetDevice(&dev));
-    GRAPE_REQUIRE(dev >= 0 && dev < 16, "device index out of range");
-    if (!g_status[dev]) {
-        // grape_init has made that of its device; a first call on another must not be captured, as it allocates and waits
-        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-        GRAPE_HIP_CHECK(hipStreamIsCapturing(s, &capture));
-        GRAPE_REQUIRE(capture == hipStreamCaptureStatusNone, "the first witness call on a device must not be captured");
-        uint32_t* word = nullptr;
-        GRAPE_HIP_CHECK(hipMalloc((void**)&word, 256));
-        wit_status_clear_kernel<<<1, 1, 0, s>>>(word);
-        GRAPE_LAUNCH_CHECK();
-        GRAPE_HIP_CHECK(hipStreamSynchronize(s));
-        g_status[dev] = word;
+    GRAPE_REQUIRE(dev >= 0 && dev < kMaxDevices, "device index out of range");
+    *out = g_status[dev].load(std::memory_order_acquire);
+    if (!*out) {
+        void* word = nullptr;
+        GRAPE_HIP_CHECK(hipGetSymbolAddress(&word, HIP_SYMBOL(status_word)));
+        GRAPE_REQUIRE(word != nullptr, "no device address for the status word");
+        *out = (uint32_t*)word;
+        g_status[dev].store(*out, std::memory_order_release);
     }
-    *out = g_status[dev];
     return GRAPE_OK;
 }
 
@@ -751,7 +751,7 @@ int grape_wit_matmul_rescale(int32_t* d_q, int32_t* d_r, const int32_t* d_a, con
     p.transpose_out = transpose_out ? 1 : 0;
     p.tiles_n = (N + kTM - 1) / kTM;
     p.tiles_m = (M + kTM - 1) / kTM;
-    int rc = wit_status_word(&p.status, s);
+    int rc = wit_status_word(&p.status);
     if (rc) return rc;
     const bool aligned = (K % 4 == 0) && ((reinterpret_cast<uintptr_t>(d_a) | reinterpret_cast<uintptr_t>(d_b)) & 15) == 0;
     // matrix-core path: one batch, aligned rows, operands of at most three byte planes each.  The split into
@@ -846,7 +846,7 @@ int grape_wit_elemul_rescale(int32_t* d_q, int32_t* d_r, const int32_t* d_a, con
     CHECK_PTR(d_q); CHECK_PTR(d_a); CHECK_PTR(d_b);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = wit_status_word(&status, s);
+    int rc = wit_status_word(&status);
     if (rc) return rc;
     wit_elemul_rescale_kernel<<<blocks_for(n), kBlock, 0, s>>>(d_q, d_r, d_a, d_b, n, scale, log2_exact(scale), status);
     GRAPE_LAUNCH_CHECK();
@@ -860,7 +860,7 @@ int grape_wit_table_lookup(int32_t* d_out, const int32_t* d_in, size_t n, int32_
     CHECK_PTR(d_out); CHECK_PTR(d_in); CHECK_PTR(d_table);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = wit_status_word(&status, s);
+    int rc = wit_status_word(&status);
     if (rc) return rc;
     if (((reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(d_in)) & 15) == 0)
         wit_lookup_kernel<true><<<blocks_for((n + 3) / 4), kBlock, 0, s>>>(d_out, d_in, n, low, len, d_table, status);
@@ -890,7 +890,7 @@ int grape_wit_softmax(int32_t* d_max, int32_t* d_shifted, int32_t* d_exp, int32_
     CHECK_PTR(d_scores); CHECK_PTR(d_table);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = wit_status_word(&status, s);
+    int rc = wit_status_word(&status);
     if (rc) return rc;
     wit_softmax_kernel<<<rows, kBlock, 0, s>>>(d_max, d_shifted, d_exp, d_sum, d_prob, d_query, d_scores, cols, d_table,
                                                (1u << bit_shift) - 1u, 1u << index_bits, scale, status);
@@ -905,7 +905,7 @@ int grape_wit_row_sumsq(uint64_t* d_out, const int32_t* d_x, uint32_t rows, uint
     CHECK_PTR(d_out); CHECK_PTR(d_x);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = wit_status_word(&status, s);
+    int rc = wit_status_word(&status);
     if (rc) return rc;
     wit_row_sumsq_kernel<<<rows, kBlock, 0, s>>>(d_out, d_x, cols, status);
     GRAPE_LAUNCH_CHECK();
@@ -921,7 +921,7 @@ int grape_wit_rmsnorm_apply(int32_t* d_q_rmsw, int32_t* d_r_rmsw, int32_t* d_q_o
     CHECK_PTR(d_q_rmsw); CHECK_PTR(d_r_rmsw); CHECK_PTR(d_q_out); CHECK_PTR(d_r_out); CHECK_PTR(d_x); CHECK_PTR(d_rms); CHECK_PTR(d_w);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = wit_status_word(&status, s);
+    int rc = wit_status_word(&status);
     if (rc) return rc;
     const size_t n = (size_t)rows * cols;
     wit_rmsnorm_apply_kernel<<<blocks_for(n), kBlock, 0, s>>>(d_q_rmsw, d_r_rmsw, d_q_out, d_r_out, d_x, d_rms, d_w, n, cols, scale,
@@ -935,7 +935,7 @@ int grape_wit_status(uint32_t* flags, grape_stream_t st) {
     CHECK_PTR(flags);
     hipStream_t s = as_stream(st);
     uint32_t* status;
-    int rc = wit_status_word(&status, s);
+    int rc = wit_status_word(&status);
     if (rc) return rc;
     GRAPE_HIP_CHECK(hipMemcpyAsync(flags, status, sizeof(uint32_t), hipMemcpyDeviceToHost, s));
     GRAPE_HIP_CHECK(hipStreamSynchronize(s));
