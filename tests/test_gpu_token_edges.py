@@ -1,10 +1,11 @@
-"""GPU tests of the new tokens' calls at their edges: rows of equal scores, sums next to and beyond 32 bits.  The
+"""GPU tests of the new tokens' calls at their edges: rows of equal scores, sums next to and beyond 32 bits, forms of the
+kernels that need large products, odd heads with fine probabilities, or long heads with the largest values.  The
 helpers are those of test_gpu_tokens.py; every result is a whole number and is compared exactly with the numpy oracle."""
 import numpy as np
 import pytest
 import torch
 from oracle import witness_oracle as wo
-from test_gpu_tokens import dev, exp_table, filled, gauss, ops, paged, run_attention  # noqa: F401  (two of them are fixtures)
+from test_gpu_tokens import TOP, dev, exp_table, filled, gauss, host, ops, paged, q4_case, run_attention  # noqa: F401  (two of them are fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +76,55 @@ def test_sums_of_large_entries_are_reported(ops, lens, entry):
         assert ops.wit_status() == 0 and torch.equal(got2["qkv"], got["qkv"])
         for x in got:
             assert np.array_equal(got[x].cpu().numpy(), want[x]), x
+
+
+# ------------------------------------------------------------------ forms that few sizes choose
+@pytest.mark.parametrize("n,m,k,group", [(6, 8200, 520, 128), (8, 8161, 1030, 256), (12, 8200, 200, 64), (16, 8177, 300, 192), (20, 8200, 200, 128), (33, 4100, 130, 64), (37, 5000, 257, 128),
+                                         (20, 8200, 160, 32)])
+def test_q4_of_many_rows_and_tiles_of_tokens(ops, n, m, k, group):
+    """two tiles of rows a workgroup, of five to sixteen tokens and of more than one tile of tokens, with inputs above the digits"""
+    rng = np.random.default_rng(n * m + k)
+    x, w, scales, zeros = q4_case(rng, n, m, k, group, top=200)
+    x[n - 1, k - 1], x[0, 0] = TOP + 1, (1 << 31) - 1
+    for z in (None, zeros):
+        want = wo.matvec_q4(x, w, scales, group, z, 1 << 24)
+        q, r = ops.wit_matvec_q4(dev(x), dev(w), dev(scales), group, zeros=None if z is None else dev(z), scale=1 << 24)
+        assert np.array_equal(host(q), want[0]) and np.array_equal(host(r), want[1])
+    assert ops.wit_status() == 0
+
+
+@pytest.mark.parametrize("prob_scale,out_scale", [((1 << 22) + 1, 1 << 20), (1 << 30, 1 << 31)])
+@pytest.mark.parametrize("lens,H,HK,D,page", [([70, 200], 6, 2, 30, 9), ([256, 1], 5, 5, 50, 16), ([1500, 800], 4, 2, 30, 32), ([700], 34, 2, 50, 7), ([300, 299], 2, 1, 257, 16)])
+def test_fine_probabilities_of_heads_of_odd_sizes(ops, exp_table, lens, H, HK, D, page, prob_scale, out_scale):
+    """four planes of a probability, elements that are not read four at a time"""
+    rng = np.random.default_rng(D + len(lens))
+    table, kc, vc = paged(rng, lens, page, HK, D, sigma=20000.0)
+    for proof in (True, False):
+        run_attention(ops, gauss(rng, (len(lens), H, D)), kc, vc, table, lens, None, exp_table, max(lens), proof=proof, qk_scale=200000, prob_scale=prob_scale, out_scale=out_scale)
+    assert ops.wit_status() == 0
+
+
+@pytest.mark.parametrize("D", [512, 576, 1000, 1024, 4096])
+def test_long_heads_of_the_largest_values(ops, exp_table, D):
+    """queries above four planes of digits where the waves of a workgroup share a head's elements, an odd number of 64s among them"""
+    rng = np.random.default_rng(D)
+    H, HK, page, L = 2, 1, 16, 300
+    table, kc, vc = paged(rng, [L, L], page, HK, D, sigma=1000.0)
+    ends = np.array([-(1 << 31), (1 << 31) - 1, TOP, TOP + 1, -TOP - 1, 0], dtype=np.int64)
+    # products of the largest queries with the largest keys cancel, at both ends of a head and in its middle
+    q = rng.integers(-3, 4, (2, H, D)).astype(np.int32)
+    for a, b in ((0, 1), (D // 2, D // 2 + 1), (D - 2, D - 1)):
+        q[..., a] = q[..., b] = rng.choice(np.array([(1 << 31) - 1, TOP + 1, TOP, -(1 << 31)]), (2, H))
+        large = rng.integers(-(1 << 28), 1 << 28, kc.shape[:3])
+        kc[..., a], kc[..., b] = large, -large
+    vc[..., ::3] = rng.choice(ends, vc[..., ::3].shape)
+    run_attention(ops, q, kc, vc, table, [L, L - 7], None, exp_table, L, qk_scale=8)
+    # scores next to the ends of 32 bits
+    q = np.zeros((2, H, D), dtype=np.int32)
+    q[:, :, D - 1] = [(1 << 31) - 1, -(1 << 31)]
+    q[:, :, 3] = TOP + 5
+    kc[:] = 0
+    kc[..., D - 1] = rng.choice(np.array([TOP, TOP + 1, TOP + 7, TOP + 1000], dtype=np.int64), kc.shape[:3])
+    kc[..., 3] = rng.integers(-500, 500, kc.shape[:3])
+    run_attention(ops, q, kc, vc, table, [L, L - 3], None, exp_table, L, qk_scale=1 << 31)
+    assert ops.wit_status() == 0
