@@ -93,6 +93,19 @@ def test_q4_of_many_rows_and_tiles_of_tokens(ops, n, m, k, group):
     assert ops.wit_status() == 0
 
 
+@pytest.mark.parametrize("n,m,k,group", [(1, 4096, 11008, 128), (1, 70, 16384, 64), (1, 33, 40000, 32), (1, 16, 33001, 128), (2, 100, 9000, 128), (4, 33, 4900, 64)])
+def test_q4_of_few_tokens_with_long_inputs(ops, n, m, k, group):
+    """digits and turned weights of up to 124 KB a workgroup, inputs that go through in pieces"""
+    rng = np.random.default_rng(m + k)
+    x, w, scales, zeros = q4_case(rng, n, m, k, group, top=60)
+    x[0, [0, k // 2, k - 1]] = TOP + 1, -(1 << 31), (1 << 31) - 1
+    for z in (None, zeros):
+        want = wo.matvec_q4(x, w, scales, group, z, 1 << 20)
+        q, r = ops.wit_matvec_q4(dev(x), dev(w), dev(scales), group, zeros=None if z is None else dev(z), scale=1 << 20)
+        assert np.array_equal(host(q), want[0]) and np.array_equal(host(r), want[1])
+    assert ops.wit_status() == 0
+
+
 @pytest.mark.parametrize("prob_scale,out_scale", [((1 << 22) + 1, 1 << 20), (1 << 30, 1 << 31)])
 @pytest.mark.parametrize("lens,H,HK,D,page", [([70, 200], 6, 2, 30, 9), ([256, 1], 5, 5, 50, 16), ([1500, 800], 4, 2, 30, 32), ([700], 34, 2, 50, 7), ([300, 299], 2, 1, 257, 16)])
 def test_fine_probabilities_of_heads_of_odd_sizes(ops, exp_table, lens, H, HK, D, page, prob_scale, out_scale):
