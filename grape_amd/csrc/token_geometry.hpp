@@ -229,9 +229,10 @@ inline const char* refuse_attention(const grape_wit_attention_args* a, const gra
 }
 
 // Products with 4-bit weights.  One token is taken apart by the workgroups that multiply it, and so are up to four while that is
-// little work for them (4 tokens through 4096 x 4096: 8.3 us a call and not 11); more by a launch of its own, into the workspace, in
-// tiles of four, eight or sixteen (4 tokens through 16384 x 8192: 24 us and not 44).  One word a block of 2048 inputs of a token
-// says what its digits lack.
+// little work for them (two tokens through 4096 x 4096, groups of 128: 8.0 to 8.5 us a call and not 10.0, four 9.5 and not 10.4); more by
+// a launch of its own, into the workspace, in tiles of four, eight or sixteen (four tokens through 16384 x 8192, groups of 128: 24 us
+// and not 44, with zero points 30 and not 47).  One word a block of 2048 inputs of a token says whether one of them is above the digits;
+// any such word of a tile's tokens sends all of the tile's sums through their rows again.
 constexpr uint32_t kQ4Inputs = (uint32_t)1 << 24;          // a thread looks through a row's for those above the digits
 inline bool q4_few(uint32_t tokens, uint32_t outputs, uint32_t inputs) {
     const uint64_t tiles = ceil_div(outputs, 16) < 256 ? 256 : ceil_div(outputs, 16);

@@ -466,7 +466,10 @@ __device__ __forceinline__ void q4_out(const Q4Args& p, uint32_t n, uint32_t m, 
 
 // Up to four tokens: a workgroup makes their digits itself, in LDS (a longer input goes through in pieces), while its first weights
 // are under way.  One token through 4096 x 4096, groups of 128: 5.7 us, as long as a launch and a chain of loads take; 11008 x 4096,
-// groups of 64 with zero points, 26 MB: 12.1 us, 2.1 TB/s, bound by what is under way and by the digits of each workgroup.  blockDim: as many waves as share a tile's inputs, 4 KB of LDS each behind the digits.
+// groups of 64 with zero points, 26 MB: 12.1 us, 2.1 TB/s.  Not the memory bounds that (all 688 workgroups are resident, 11 MB requested at
+// the start) but the chain in each: inputs, digits, weights turned over, a second quad, the join; and the digits are made 688 times
+// and LDS waits 7.5e5 cycles for its banks in 2.1e5 instructions.  blockDim: as many waves as share a tile's inputs, 4 KB of LDS each
+// behind the digits.
 template <int GS>
 __global__ void __launch_bounds__(64 * q4_most_waves(GS), GS == 32 ? 2 : 4) wit_q4_few_kernel(Q4Args p, uint32_t piece) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
@@ -524,8 +527,9 @@ __global__ void __launch_bounds__(64 * q4_most_waves(GS), GS == 32 ? 2 : 4) wit_
 }
 
 // More tokens: their digits are made once, by a launch of its own, and read from L2 as operands, 4 NT tokens at a time for RT tiles
-// of 16 rows.  For 16 tokens through 4096 x 11008 those are 180 MB at 12 TB/s, which bounds it (14.3 us, of which reading the weights
-// would take 5).  Digits in LDS for 128 rows at a time ask for 22 MB instead, but leave a workgroup a CU of which each waits for
+// of 16 rows.  For 16 tokens through 4096 x 11008 (14.3 us, of which reading the weights would take 5) those are 180 MB, 12 TB/s: what a
+// chain reaches that requests a unit's digits when it multiplies them, with eight waves a CU; the rate of L2 itself was not measured.
+// 64 tokens 39 us a call, 256 142: weights and digits are read again for each sixteen.  Digits in LDS for 128 rows at a time ask for 22 MB instead, but leave a workgroup a CU of which each waits for
 // its next weights, and sums to be joined: 14.8 and 3.9 us.
 template <int GS>
 __global__ void __launch_bounds__(kBlock) wit_q4_digits_kernel(Q4Args p, uint32_t tile_tokens) {
@@ -540,8 +544,8 @@ __global__ void __launch_bounds__(kBlock) wit_q4_digits_kernel(Q4Args p, uint32_
 }
 
 // Whether the weights go through LDS: with scales for each 64 or 32 the lanes of a row load short pieces, and many.  Four tokens
-// through 16384 x 8192: 39 us and not 55 with groups of 32, 33 and not 39 with groups of 64.  With sixteen the registers are not
-// enough for it (96 us and not 90).
+// through 16384 x 8192, with zero points: 39 us and not 55 with groups of 32, 33 and not 39 with groups of 64.  With sixteen the registers
+// are not enough for it (96 us and not 90).
 constexpr bool q4_turns(int gs, int nt) { return gs < 128 && nt < 4; }
 template <int GS, int NT, int RT>
 __global__ void __launch_bounds__(kQ4Threads, 2) wit_q4_many_kernel(Q4Args p, uint32_t makers) {
