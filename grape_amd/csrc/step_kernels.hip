@@ -1,0 +1,389 @@
+// The step around new tokens: their pages, positions and slots from the requests' lengths, and the choice of the next token.
+#include <algorithm>
+#include "token_device.hpp"
+#include "step_geometry.hpp"
+
+namespace grape {
+
+// ------------------------------------------------------------------------------------------------
+// Pages and slots.  One launch: every workgroup makes the prefix sums of all sequences' tokens, pages and pages given back for
+// itself, in LDS, and then takes its share of the rows, the new pages and the ones given back, each of which finds its sequence by
+// halving.  Nothing that a workgroup reads is written by another one: the lengths and the ring's span go to places of their own,
+// entries of the table are read below the pages held and written above, and the ring is written behind its last entry alone.
+// ------------------------------------------------------------------------------------------------
+struct PageArgs {
+    grape_wit_page_step_args a;
+    token::FastDiv by_page;
+    uint32_t sink_pages;
+    uint32_t* status;
+};
+constexpr uint32_t kPageThreads = 256;
+
+// The sum of v over the threads before this one, and of all of them.
+__device__ __forceinline__ uint64_t before_me(uint64_t v, uint64_t& all) {
+    __shared__ uint64_t waves[kPageThreads / 64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint64_t sum = v;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint64_t y = __shfl_up(sum, d, 64);
+        if (lane >= d) sum += y;
+    }
+    __syncthreads();
+    if (lane == 63) waves[wave] = sum;
+    __syncthreads();
+    uint64_t base = 0;
+    all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kPageThreads / 64; w++) {
+        if (w < wave) base += waves[w];
+        all += waves[w];
+    }
+    return base + sum - v;
+}
+
+// The number of the n ascending sums that are at most `x`: the sequence that x belongs to.
+__device__ __forceinline__ uint32_t find_sequence(const uint32_t* sums, uint32_t n, uint32_t x) {
+    uint32_t lo = 0, hi = n;
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (sums[mid] <= x) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kPageThreads) wit_page_step_kernel(PageArgs p) {
+    extern __shared__ uint32_t lds[];
+    const grape_wit_page_step_args& a = p.a;
+    uint32_t *to_token = lds, *to_page = lds + a.seqs, *to_back = lds + 2 * a.seqs;          // sums up to and with each sequence
+    const uint32_t each = (a.seqs + kPageThreads - 1) / kPageThreads, b0 = min(threadIdx.x * each, a.seqs), b1 = min(b0 + each, a.seqs);
+    const uint64_t most = (uint64_t)a.page_size * a.table_stride;
+    uint32_t bad = 0;
+    uint32_t head = (uint32_t)a.d_span[0], count = (uint32_t)a.d_span[1];
+    const bool ring_ok = count <= a.ring && (head < a.ring || (head == 0 && a.ring == 0));
+    if (!ring_ok) {
+        head = count = 0;
+        bad |= (uint32_t)kWitIndex;
+    }
+    const uint32_t room = ring_ok ? a.ring - count : 0;
+    auto ask = [&](uint32_t b, step::Sequence& s) { return s.ask(a.d_lens[b], a.d_new[b], most, p.by_page); };
+    step::Sequence s;
+    uint64_t tokens = 0, pages = 0, all_tokens, all_pages;
+    for (uint32_t b = b0; b < b1; b++) {
+        if (!ask(b, s)) bad |= (uint32_t)kWitIndex;
+        tokens += s.tokens;
+        pages += s.taken;
+    }
+    tokens = before_me(tokens, all_tokens);
+    pages = before_me(pages, all_pages);
+    // sequences are served in their order until the rows or the free pages run out; from there on none is
+    uint64_t served_tokens = 0, served_pages = 0, back = 0, all_back;
+    for (uint32_t b = b0; b < b1; b++) {
+        ask(b, s);
+        tokens += s.tokens;
+        pages += s.taken;
+        const bool served = tokens <= a.rows && pages <= count;
+        if (!served) s.refuse();
+        else served_tokens = tokens, served_pages = pages;
+        s.give_back(a.window, p.sink_pages, p.by_page);
+        back += s.back;
+        to_token[b] = served ? (uint32_t)tokens : UINT32_MAX;
+        to_page[b] = served ? (uint32_t)pages : UINT32_MAX;
+    }
+    // the largest sums that were served
+    __shared__ uint32_t top[2];
+    if (threadIdx.x < 2) top[threadIdx.x] = 0;
+    back = before_me(back, all_back);
+    if (b0 < b1) {
+        atomicMax(&top[0], (uint32_t)served_tokens);
+        atomicMax(&top[1], (uint32_t)served_pages);
+    }
+    __syncthreads();
+    const uint32_t rows = top[0], taken = top[1], kept = (uint32_t)min(all_back, (uint64_t)room);
+    const bool mine = blockIdx.x == 0;          // of what is written once
+    for (uint32_t b = b0; b < b1; b++) {
+        ask(b, s);
+        const bool served = to_token[b] != UINT32_MAX;
+        if (!served) {
+            s.refuse();
+            to_token[b] = rows;
+            to_page[b] = taken;
+        }
+        s.give_back(a.window, p.sink_pages, p.by_page);
+        back += s.back;
+        to_back[b] = (uint32_t)back;
+        if (mine) {
+            a.d_starts[b + 1] = (int32_t)to_token[b];
+            a.d_lens_out[b] = !s.ok ? a.d_lens[b] : s.ended ? 0 : (int32_t)(s.len + s.tokens);
+        }
+    }
+    if (mine && threadIdx.x == 0) {
+        a.d_starts[0] = 0;
+        uint32_t at = head + taken;
+        a.d_span_out[0] = (int32_t)(ring_ok ? (at >= a.ring && a.ring ? at - a.ring : at) : (uint32_t)a.d_span[0]);
+        a.d_span_out[1] = (int32_t)(ring_ok ? count - taken + kept : (uint32_t)a.d_span[1]);
+        if (all_tokens > a.rows || all_pages > count || all_back > kept) bad |= (uint32_t)kWitPages;
+    }
+    __syncthreads();
+    auto ring_at = [&](uint32_t k) {
+        const uint32_t at = head + k;
+        return at >= a.ring ? at - a.ring : at;
+    };
+    // page number i of sequence b, whose first new page is number `first` of those taken
+    auto page_at = [&](uint32_t b, uint32_t i, uint32_t held, uint32_t first) {
+        return i < held ? a.d_block_table[(size_t)b * a.table_stride + i] : a.d_free[ring_at(first + i - held)];
+    };
+    const uint32_t stride = gridDim.x * kPageThreads, from = blockIdx.x * kPageThreads + threadIdx.x;
+    for (uint32_t r = from; r < a.rows; r += stride) {
+        int32_t pos = 0;
+        int64_t slot = -1;
+        if (r < rows) {
+            const uint32_t b = find_sequence(to_token, a.seqs, r);
+            ask(b, s);
+            const uint32_t at = s.len + (r - (b ? to_token[b - 1] : 0)), i = p.by_page(at);
+            const int32_t page = page_at(b, i, s.held, b ? to_page[b - 1] : 0);
+            pos = (int32_t)at;
+            if (page >= 0) slot = (int64_t)page * a.page_size + (at - i * a.page_size);
+            else bad |= (uint32_t)kWitIndex;
+        }
+        a.d_positions[r] = pos;
+        a.d_slots[r] = slot;
+    }
+    for (uint32_t k = from; k < taken; k += stride) {
+        const uint32_t b = find_sequence(to_page, a.seqs, k);
+        ask(b, s);
+        a.d_block_table[(size_t)b * a.table_stride + s.held + (k - (b ? to_page[b - 1] : 0))] = a.d_free[ring_at(k)];
+    }
+    for (uint32_t k = from; k < kept; k += stride) {
+        const uint32_t b = find_sequence(to_back, a.seqs, k);
+        ask(b, s);
+        if (b ? to_token[b] == to_token[b - 1] : to_token[b] == 0) s.refuse();
+        s.give_back(a.window, p.sink_pages, p.by_page);
+        const uint32_t i = s.back_page(k - (b ? to_back[b - 1] : 0));
+        const int32_t page = page_at(b, i, s.held, b ? to_page[b - 1] : 0);
+        if (page < 0) bad |= (uint32_t)kWitIndex;
+        a.d_free[ring_at(count + k)] = page;
+    }
+    if (bad) atomicOr(p.status, bad);
+}
+
+// ------------------------------------------------------------------------------------------------
+// The next token.  A workgroup counts a row's history for its chunk of the vocabulary in LDS, applies what the counts, biases and
+// mask ask for and keeps its largest logit; a second launch joins the chunks and writes how far each logit is below the row's largest.
+// Bound by memory: 4 bytes read a logit, up to 16 written, and 4 read again for the distances.
+// ------------------------------------------------------------------------------------------------
+constexpr int32_t kLowest = INT32_MIN;          // of a token that must not be chosen
+struct NextArgs {
+    grape_wit_next_token_args a;
+    step::NextPlan plan;
+    Scaler scale;
+    unsigned long long* part;          // [seqs][chunks]: the larger the logit, then the smaller the token, the larger the number
+    uint32_t* status;
+};
+
+__device__ __forceinline__ unsigned long long rank_of(int32_t z, uint32_t token) {
+    return ((unsigned long long)((uint32_t)z ^ 0x80000000u) << 32) | (uint32_t)~token;
+}
+__device__ __forceinline__ int32_t value_of(unsigned long long rank) { return (int32_t)((uint32_t)(rank >> 32) ^ 0x80000000u); }
+
+__device__ __forceinline__ unsigned long long block_largest(unsigned long long v) {
+    __shared__ unsigned long long sh[kBlock / 64];
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < kBlock / 64; w++) v = max(v, sh[w]);
+    return v;
+}
+
+template <bool VEC>
+__device__ __forceinline__ v4i_t row4(const int32_t* x, uint32_t at, uint32_t n) {
+    if constexpr (VEC) {
+        return *reinterpret_cast<const v4i_t*>(x + at);
+    } else {
+        v4i_t v = {0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+            if (at + j < n) v[j] = x[at + j];
+        return v;
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void put4(int32_t* x, uint32_t at, uint32_t n, v4i_t v) {
+    if constexpr (VEC) {
+        *reinterpret_cast<v4i_t*>(x + at) = v;
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+            if (at + j < n) x[at + j] = v[j];
+    }
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(kBlock) wit_next_adjust_kernel(NextArgs p) {
+    extern __shared__ uint32_t counts[];
+    const grape_wit_next_token_args& a = p.a;
+    const uint32_t b = blockIdx.y, v0 = blockIdx.x * p.plan.chunk, n = min(a.vocab - v0, p.plan.chunk);
+    uint32_t bad = 0;
+    for (uint32_t i = threadIdx.x; i < p.plan.chunk; i += kBlock) counts[i] = 0;
+    __syncthreads();
+    int32_t len = a.history ? a.d_history_lens[b] : 0;
+    if (len < 0 || (uint32_t)len > a.history) {
+        bad |= (uint32_t)kWitIndex;
+        len = len < 0 ? 0 : (int32_t)a.history;
+    }
+    const int32_t* history = a.d_history + (len ? b * a.history_stride : 0);
+    for (uint32_t i = threadIdx.x; i < (uint32_t)len; i += kBlock) {
+        const int32_t t = history[i];
+        if (t >= (int32_t)a.vocab) bad |= (uint32_t)kWitIndex;
+        const uint32_t at = (uint32_t)t - v0;
+        if (t >= 0 && at < n) atomicAdd(&counts[at], 1u);
+    }
+    int32_t repetition = 0;          // none
+    Scaler down{1, 1.0, 0};
+    if (a.d_repetition) {
+        repetition = a.d_repetition[b];
+        if (repetition < 1) {
+            bad |= (uint32_t)kWitIndex;
+            repetition = 0;
+        } else {
+            down = Scaler{repetition, 1.0 / (double)repetition, -1};
+        }
+    }
+    const int64_t presence = a.d_presence ? a.d_presence[b] : 0, frequency = a.d_frequency ? a.d_frequency[b] : 0;
+    const int32_t *logits = a.d_logits + b * a.logits_stride + v0, *bias = a.d_bias ? a.d_bias + b * a.bias_stride + v0 : nullptr;
+    const uint32_t* mask = a.d_mask ? reinterpret_cast<const uint32_t*>(a.d_mask) + b * a.mask_stride + v0 / 32 : nullptr;
+    const size_t o = (size_t)b * a.vocab + v0;
+    __syncthreads();
+    unsigned long long best = 0;
+    for (uint32_t i = 4 * threadIdx.x; i < n; i += 4 * kBlock) {
+        const v4i_t x = row4<VEC>(logits, i, n);
+        v4i_t more = {0, 0, 0, 0};
+        if (bias) more = row4<VEC>(bias, i, n);
+        const uint32_t allowed = mask ? mask[i / 32] >> (i & 31u) : 15u;
+        v4i_t z, rem, c;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            c[j] = (int32_t)counts[i + j];
+            int64_t y = x[j];
+            int32_t q, r = 0;
+            rem[j] = 0;
+            if (c[j]) {
+                if (repetition) {
+                    uint32_t wide = 0;          // a quotient beyond int32 is still one of 64 bits
+                    if (x[j] > 0) {
+                        down.apply((int64_t)x[j] * p.a.scale, q, r, wide);
+                        y = wide ? ((int64_t)x[j] * p.a.scale - r) / repetition : q;
+                    } else {
+                        p.scale.apply((int64_t)x[j] * repetition, q, r, wide);
+                        y = wide ? ((int64_t)x[j] * repetition - r) / p.a.scale : q;
+                    }
+                }
+                y -= presence + frequency * c[j];
+            }
+            y += more[j];
+            const bool chosen = ((allowed >> j) & 1u) && x[j] != kLowest && more[j] != kLowest;
+            if (chosen) {
+                if (y <= (int64_t)kLowest || y > (int64_t)INT32_MAX) {
+                    if (i + j < n) bad |= (uint32_t)kWitQuotient;
+                    y = y <= (int64_t)kLowest ? (int64_t)kLowest + 1 : (int64_t)INT32_MAX;
+                }
+                rem[j] = r;
+            }
+            z[j] = chosen ? (int32_t)y : kLowest;
+            if (i + j < n) best = max(best, rank_of(z[j], v0 + i + j));
+        }
+        if (a.d_out) put4<VEC>(a.d_out + o, i, n, z);
+        if (a.d_rem) put4<VEC>(a.d_rem + o, i, n, rem);
+        if (a.d_count) put4<VEC>(a.d_count + o, i, n, c);
+        if (a.d_gap) put4<VEC>(a.d_gap + o, i, n, z);          // the second launch takes it from the largest
+    }
+    best = block_largest(best);
+    if (threadIdx.x == 0) p.part[(size_t)b * p.plan.chunks + blockIdx.x] = best;
+    if (bad) atomicOr(p.status, bad);
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(kBlock) wit_next_choose_kernel(NextArgs p) {
+    const grape_wit_next_token_args& a = p.a;
+    const uint32_t b = blockIdx.y;
+    unsigned long long best = 0;
+    for (uint32_t i = threadIdx.x; i < p.plan.chunks; i += kBlock) best = max(best, p.part[(size_t)b * p.plan.chunks + i]);
+    best = block_largest(best);
+    const int32_t top = value_of(best);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        a.d_token[b] = top == kLowest ? -1 : (int32_t)~(uint32_t)best;
+        if (a.d_max) a.d_max[b] = top;
+    }
+    if (!a.d_gap) return;
+    const uint32_t v0 = blockIdx.x * p.plan.chunk, n = min(a.vocab - v0, p.plan.chunk);
+    int32_t* gap = a.d_gap + (size_t)b * a.vocab + v0;
+    uint32_t bad = 0;
+    for (uint32_t i = 4 * threadIdx.x; i < n; i += 4 * kBlock) {
+        v4i_t z = row4<VEC>(gap, i, n);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            const uint32_t below = z[j] == kLowest ? 0u : (uint32_t)top - (uint32_t)z[j];
+            if (below > (uint32_t)INT32_MAX && i + j < n) bad |= (uint32_t)kWitSumWide;
+            z[j] = (int32_t)below;
+        }
+        put4<VEC>(gap, i, n, z);
+    }
+    if (bad) atomicOr(p.status, bad);
+}
+
+}  // namespace grape
+
+using namespace grape;
+
+extern "C" {
+
+int grape_wit_page_step(const grape_wit_page_step_args* args, grape_stream_t st) {
+    GRAPE_REQUIRE(initialised(), "grape_init has not been called");
+    GRAPE_REFUSED_IF(step::refuse_pages(args));
+    PageArgs p;
+    p.a = *args;
+    p.by_page = token::fast_div(p.a.page_size);
+    p.sink_pages = p.a.window ? (uint32_t)(((uint64_t)p.a.sinks + p.a.page_size - 1) / p.a.page_size) : 0;
+    hipStream_t s = as_stream(st);
+    const int rc = wit_status_word(&p.status);
+    if (rc) return rc;
+    const uint32_t workgroups = std::min(256u, std::max(1u, token::ceil_div(std::max(p.a.rows, p.a.seqs), 4 * kPageThreads)));
+    wit_page_step_kernel<<<workgroups, kPageThreads, (size_t)12 * p.a.seqs, s>>>(p);
+    GRAPE_LAUNCH_CHECK();
+    return GRAPE_OK;
+}
+
+size_t grape_wit_next_token_workspace(uint32_t seqs, uint32_t vocab) { return step::next_workspace(seqs, vocab); }
+
+int grape_wit_next_token(const grape_wit_next_token_args* args, grape_stream_t st) {
+    GRAPE_REQUIRE(initialised(), "grape_init has not been called");
+    GRAPE_REFUSED_IF(step::refuse_next(args));
+    if (args->seqs == 0) return GRAPE_OK;
+    NextArgs p;
+    p.a = *args;
+    const grape_wit_next_token_args& a = p.a;
+    p.plan = step::next_plan(a.seqs, a.vocab);
+    p.scale = scaler(a.scale);
+    p.part = (unsigned long long*)a.d_workspace;
+    hipStream_t s = as_stream(st);
+    const int rc = wit_status_word(&p.status);
+    if (rc) return rc;
+    auto wide = [&](const void* x, int64_t stride) { return !x || ((reinterpret_cast<uintptr_t>(x) & 15) == 0 && stride % 4 == 0); };
+    const bool vec = a.vocab % 4 == 0 && wide(a.d_logits, a.logits_stride) && wide(a.d_bias, a.bias_stride) && wide(a.d_out, 0) && wide(a.d_rem, 0) && wide(a.d_count, 0) && wide(a.d_gap, 0);
+    const dim3 grid(p.plan.chunks, a.seqs);
+    const size_t lds = (size_t)4 * p.plan.chunk;
+    if (vec) wit_next_adjust_kernel<true><<<grid, kBlock, lds, s>>>(p);
+    else wit_next_adjust_kernel<false><<<grid, kBlock, lds, s>>>(p);
+    GRAPE_LAUNCH_CHECK();
+    const dim3 join(a.d_gap ? p.plan.chunks : 1, a.seqs);
+    if (vec) wit_next_choose_kernel<true><<<join, kBlock, 0, s>>>(p);
+    else wit_next_choose_kernel<false><<<join, kBlock, 0, s>>>(p);
+    GRAPE_LAUNCH_CHECK();
+    return GRAPE_OK;
+}
+
+}  // extern "C"

@@ -16,9 +16,6 @@ namespace grape {
 // are the bytes of x with three top bits turned over, and c times the sum of the other operand is added in the end.  The pairs
 // of planes with the same sum of exponents share an accumulator: 4 * 2^14 * 8192 elements (1024 positions) stay below 2^31.
 // ------------------------------------------------------------------------------------------------
-constexpr int64_t kCacheOffset = 0x808080;
-constexpr uint32_t kByteTops = 0x80808080;          // of a plane's four bytes
-
 struct AttendArgs {
     grape_wit_attention_args a;
     grape_wit_cache c;
@@ -99,19 +96,6 @@ struct Offsets {
         return outside;
     }
 };
-
-// four elements from x; those from `n` on are whatever comes first
-template <bool VEC>
-__device__ __forceinline__ v4i_t load4(const int32_t* x, uint32_t at, uint32_t n) {
-    if constexpr (VEC) {
-        return *reinterpret_cast<const v4i_t*>(x + (at < n ? at : 0));          // n is a multiple of 4
-    } else {
-        v4i_t v;
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++) v[j] = x[at + j < n ? at + j : 0];
-        return v;
-    }
-}
 
 typedef int v2i_t __attribute__((ext_vector_type(2)));
 template <bool VEC>
@@ -301,27 +285,6 @@ __device__ __forceinline__ unsigned long long exponentials(const AttendArgs& p, 
         }
     }
     return sum;
-}
-
-// floor((e * scale + sum / 2) / sum) for e <= sum: the quotient is at most `scale`, so one product in double precision is off by one at most
-__device__ __forceinline__ uint32_t probability(uint32_t e, uint64_t scale, uint64_t sum, double inv) {
-    const uint64_t num = e * scale + (sum >> 1);
-    uint64_t q = (uint64_t)((double)num * inv);
-    const int64_t rest = (int64_t)(num - q * sum);
-    if (rest < 0) q--;
-    else if (rest >= (int64_t)sum) q++;
-    return (uint32_t)q;
-}
-
-// 2 * scale * e - sum * (2 * prob - 1), within 0 .. 2 sum: less than 2^63
-__device__ __forceinline__ uint64_t lookup_query(uint32_t e, int64_t scale, uint64_t sum, uint32_t prob) {
-    return (uint64_t)e * 2 * (uint64_t)scale - sum * (2 * (uint64_t)prob - 1);
-}
-
-// Where a tensor of the proof holds a sum or a query, its low 32 bits; the bit says that they are not all of it.
-__device__ __forceinline__ void store_sum(int32_t* to, uint64_t x, uint32_t& bad) {
-    bad |= x > (uint64_t)INT32_MAX ? (uint32_t)kWitSumWide : 0u;
-    *to = (int32_t)x;
 }
 
 // The threads of a workgroup that share a query head: as many as there are for each, a power of two, in lanes side by side.

@@ -53,6 +53,44 @@ __device__ __forceinline__ void transpose4(uint32_t w0, uint32_t w1, uint32_t w2
     out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
+// A cache element x is taken as x - kCacheOffset, whose balanced digits are the bytes of x with the three lower top bits turned over.
+constexpr int64_t kCacheOffset = 0x808080;
+constexpr uint32_t kByteTops = 0x80808080;          // of a plane's four bytes
+
+// four elements from x; those from `n` on are whatever comes first
+template <bool VEC>
+__device__ __forceinline__ v4i_t load4(const int32_t* x, uint32_t at, uint32_t n) {
+    if constexpr (VEC) {
+        return *reinterpret_cast<const v4i_t*>(x + (at < n ? at : 0));          // n is a multiple of 4
+    } else {
+        v4i_t v;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) v[j] = x[at + j < n ? at + j : 0];
+        return v;
+    }
+}
+
+// floor((e * scale + sum / 2) / sum) for e <= sum: the quotient is at most `scale`, so one product in double precision is off by one at most
+__device__ __forceinline__ uint32_t probability(uint32_t e, uint64_t scale, uint64_t sum, double inv) {
+    const uint64_t num = e * scale + (sum >> 1);
+    uint64_t q = (uint64_t)((double)num * inv);
+    const int64_t rest = (int64_t)(num - q * sum);
+    if (rest < 0) q--;
+    else if (rest >= (int64_t)sum) q++;
+    return (uint32_t)q;
+}
+
+// 2 * scale * e - sum * (2 * prob - 1), within 0 .. 2 sum: less than 2^63
+__device__ __forceinline__ uint64_t lookup_query(uint32_t e, int64_t scale, uint64_t sum, uint32_t prob) {
+    return (uint64_t)e * 2 * (uint64_t)scale - sum * (2 * (uint64_t)prob - 1);
+}
+
+// Where a tensor of the proof holds a sum or a query, its low 32 bits; the bit says that they are not all of it.
+__device__ __forceinline__ void store_sum(int32_t* to, uint64_t x, uint32_t& bad) {
+    bad |= x > (uint64_t)INT32_MAX ? (uint32_t)kWitSumWide : 0u;
+    *to = (int32_t)x;
+}
+
 }  // namespace grape
 
 #define GRAPE_REFUSED_IF(expr)              \

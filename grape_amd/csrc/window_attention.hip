@@ -1,0 +1,609 @@
+// Attention of several new tokens a sequence over a paged cache - in their order, or behind a sliding window and a few first tokens -
+// with the tensors that a proof of it looks up.
+#include <algorithm>
+#include "token_device.hpp"
+#include "step_geometry.hpp"
+
+namespace grape {
+
+// ------------------------------------------------------------------------------------------------
+// Scores, softmax through the table, products with the values, for tiles of 64 rows: the query heads that read one cache head, token
+// after token, so that a key or a value that is read serves 64 rows.  The softmax is the table's, rounded: the row's maximum is
+// needed before the first exponential and the sum of all before the first probability, hence a launch for each of the three, and
+// a fourth that joins the values' partial sums where the positions are cut up.
+//
+// Both products run on the int8 matrix cores, exactly: an element x is taken as x - c, c = 128 (1 + 2^8 + 2^16), whose four balanced
+// digits are the bytes of x with the three lower top bits turned over, and sum q k = sum (q-c)(k-c) + c (sum (q-c) + sum (k-c)) + c^2 dim.
+// The pairs of planes with the same sum of exponents share an accumulator: 4 * 2^14 * 8192 elements stay below 2^31.
+// ------------------------------------------------------------------------------------------------
+using step::kRows;
+constexpr uint32_t kNoElement = 0x00808080;          // whose digits are all zero
+typedef int v4u_t __attribute__((ext_vector_type(4), aligned(4)));
+
+// rows of a tensor of the proof, or of the workspace, which holds the tiles that are seen side by side
+struct Rows {
+    int32_t* base;
+    size_t stride;
+    bool dense;
+    __device__ __forceinline__ int32_t* at(size_t row, uint32_t t, uint32_t v) const { return base + row * stride + (dense ? t : v * kRows + t % kRows); }
+};
+
+struct WindowArgs {
+    grape_wit_window_attention_args a;
+    grape_wit_cache c;
+    step::WindowPlan plan;
+    token::FastDiv page, by_each;
+    Scaler qk, out;
+    Rows scores, exps;
+    int32_t* chunk_max;          // [rows][heads][score chunks]
+    unsigned long long* sums;    // [rows][heads]
+    int64_t* part;               // [rows][heads][value chunks][dim]
+    uint32_t* status;
+    bool q_vec;
+};
+
+// A workgroup's rows: rows 64 * tile .. + R of the cache head kv of sequence b, whose n new tokens start at row `first` and position
+// `pos`.  Row r is query head r % each of token r / each.
+struct RowTile {
+    uint32_t b, kv, first, n, pos, at, R;
+    uint32_t lane, wave, col, kg;
+    __device__ __forceinline__ bool find(const WindowArgs& p, uint32_t index) {
+        lane = threadIdx.x & 63u;
+        wave = threadIdx.x >> 6;
+        col = lane & 15u;
+        kg = lane >> 4;
+        // the heads of one tile are neighbours, so that each die's L2 gets the keys of its own heads where there are eight; long rows first
+        kv = index % p.c.heads;
+        const uint32_t ti = p.plan.tiles - 1 - index / p.c.heads;
+        auto tile0 = [&](uint32_t s) { return (uint32_t)max(p.a.d_starts[s], 0) * (uint64_t)p.plan.each / kRows + s; };
+        // the last sequence whose tiles start at ti or before, 64 of them asked at a time
+        uint32_t lo = 0, left = p.a.seqs;
+        while (left > 1) {
+            const uint32_t step = (left + 63) / 64, probe = lane * step;
+            const unsigned long long before = __ballot(probe < left && tile0(lo + min(probe, left - 1)) <= ti);
+            const uint32_t last = before ? 63 - (uint32_t)__builtin_clzll(before) : 0;
+            lo += last * step;
+            left = min(step, left - last * step);
+        }
+        b = lo;
+        const int32_t s = p.a.d_starts[b];
+        if (!step::new_tokens(s, p.a.d_starts[b + 1], p.a.d_lens[b], p.a.rows, p.a.max_new, p.a.max_len, (uint64_t)p.a.table_stride * p.c.page_size, n, pos)) return false;
+        first = (uint32_t)s;
+        const uint64_t base = tile0(b);
+        if (ti < base) return false;
+        const uint64_t local = (uint64_t)(ti - base) * kRows, all = (uint64_t)n * p.plan.each;
+        if (local >= all) return false;
+        at = (uint32_t)local;
+        R = (uint32_t)min((uint64_t)kRows, all - local);
+        return true;
+    }
+    __device__ __forceinline__ uint32_t token(const WindowArgs& p, uint32_t r) const { return p.by_each(at + r); }
+    __device__ __forceinline__ uint32_t pos_of(const WindowArgs& p, uint32_t r) const { return pos + token(p, r); }
+    __device__ __forceinline__ size_t row(const WindowArgs& p, uint32_t r) const {
+        const uint32_t j = token(p, r);
+        return (size_t)(first + j) * p.a.heads + kv * p.plan.each + (at + r - j * p.plan.each);
+    }
+    __device__ __forceinline__ step::Seen seen(const WindowArgs& p) const { return step::Seen(pos_of(p, 0), pos_of(p, R - 1), p.a.window, p.a.sinks); }
+};
+
+// Offset of position t's token, -1 where its page is outside the cache, -2 where no row sees it.
+__device__ __forceinline__ int64_t offset_of(const WindowArgs& p, const RowTile& w, const step::Seen& seen, uint32_t t) {
+    if (!seen.any(t)) return -2;
+    const uint32_t pg = p.page(t);
+    return token::token_offset(p.c, p.a.d_block_table[(size_t)w.b * p.a.table_stride + pg], t - pg * p.c.page_size);
+}
+
+// The queries' digits of a block of 256 elements in LDS, [step of 64][plane][lane group][row], 16 bytes each; and their sums.
+constexpr uint32_t kBlockSteps = 4;
+__device__ __forceinline__ void stage_queries(const WindowArgs& p, const RowTile& w, uint32_t block, uint32_t* digits, unsigned long long* q_sum, bool sums) {
+    const uint32_t steps = min(p.plan.dim64 - kBlockSteps * block, kBlockSteps), e0 = 64 * kBlockSteps * block;
+    for (uint32_t i = threadIdx.x; i < kRows * steps * 16; i += blockDim.x) {
+        const uint32_t r = i / (steps * 16), quad = i - r * (steps * 16), s = quad >> 4, c = (quad >> 2) & 3u, g = quad & 3u, e = e0 + 4 * quad;
+        int32_t x[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) x[j] = (int32_t)kNoElement;
+        if (r < w.R && e < p.c.dim) {
+            const uint32_t tok = w.token(p, r);
+            const int32_t* q = p.a.d_q + (int64_t)(w.first + tok) * p.a.q_stride + (size_t)(w.kv * p.plan.each + (w.at + r - tok * p.plan.each)) * p.c.dim;
+            if (p.q_vec) {
+                *reinterpret_cast<v4i_t*>(x) = *reinterpret_cast<const v4i_t*>(q + e);
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++)
+                    if (e + j < p.c.dim) x[j] = q[e + j];
+            }
+        }
+        uint32_t pl[4];
+        long long sum = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) sum += e + j < p.c.dim && r < w.R ? (long long)x[j] - kCacheOffset : 0;
+        transpose4((uint32_t)x[0] ^ kNoElement, (uint32_t)x[1] ^ kNoElement, (uint32_t)x[2] ^ kNoElement, (uint32_t)x[3] ^ kNoElement, pl);
+        uint32_t* o = digits + (((s * 4 * 4 + g) * kRows + r) << 2) + c;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) o[k * 16 * kRows] = pl[k];
+        if (sums) {
+            // sixteen neighbouring lanes are of one row
+#pragma unroll
+            for (int k = 8; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, 64);
+            if ((i & 15u) == 0) atomicAdd(&q_sum[r], (unsigned long long)sum);
+        }
+    }
+}
+
+// Scores of 64 rows with a chunk of the positions.  A wave takes 16 positions of each tile of 64 and all rows; it reads its keys from
+// memory into the operand (lane l the elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16), the queries' digits from LDS.
+template <bool VEC>
+__global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    __shared__ unsigned long long q_sum[kRows];
+    __shared__ int32_t top[4][kRows];
+    uint32_t bad = 0;
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        uint32_t n, pos;
+        for (uint32_t b = threadIdx.x; b < p.a.seqs; b += 256)
+            if (!step::new_tokens(p.a.d_starts[b], p.a.d_starts[b + 1], p.a.d_lens[b], p.a.rows, p.a.max_new, p.a.max_len, (uint64_t)p.a.table_stride * p.c.page_size, n, pos))
+                atomicOr(p.status, (uint32_t)kWitIndex);
+    }
+    RowTile w;
+    if (!w.find(p, blockIdx.x)) return;
+    const step::Seen seen = w.seen(p);
+    const uint32_t v0 = blockIdx.y * p.plan.score_cols;
+    if (v0 >= seen.tiles) return;
+    const uint32_t tiles = min(p.plan.score_cols, seen.tiles - v0), steps = p.plan.dim64, dim = p.c.dim, blocks = (steps + kBlockSteps - 1) / kBlockSteps;
+    int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)min(steps, kBlockSteps) * 4 * 4 * kRows * 4);
+    if (threadIdx.x < kRows) q_sum[threadIdx.x] = 0;
+    for (uint32_t i = threadIdx.x; i < tiles * kRows; i += 256) {
+        const int64_t o = offset_of(p, w, seen, seen.tile(v0 + i / kRows) * kRows + i % kRows);
+        if (o == -1) bad |= (uint32_t)kWitIndex;
+        off[i] = o;
+    }
+    if (blockIdx.y == 0 && threadIdx.x < w.R) p.sums[w.row(p, threadIdx.x)] = 0;
+    __syncthreads();
+    if (blocks == 1) {
+        stage_queries(p, w, 0, lds, q_sum, true);
+        __syncthreads();
+    }
+    const uint32_t row_blocks = (w.R + 15) / 16;
+    const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
+    v4i_t x[4];
+    auto fetch = [&](uint32_t tile, uint32_t s) {
+        const int32_t* k = keys + max(off[tile * kRows + 16 * w.wave + w.col], (int64_t)0);
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++) {
+            const uint32_t e = 64 * s + 16 * c + 4 * w.kg;
+            v4i_t y = load4<VEC>(k, e, dim);
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) x[c][j] = e + j < dim ? y[j] : (int32_t)kNoElement;
+        }
+    };
+    fetch(0, 0);
+    int32_t mx[4] = {INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN};
+    for (uint32_t tile = 0; tile < tiles; tile++) {
+        v4i_t acc[4][7];
+        int32_t k_dot[4] = {0, 0, 0, 0};          // sums of the planes of this lane's part of its key
+#pragma unroll
+        for (int rb = 0; rb < 4; rb++)
+#pragma unroll
+            for (int g = 0; g < 7; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
+        for (uint32_t s = 0; s < steps; s++) {
+            if (blocks > 1 && s % kBlockSteps == 0) {
+                __syncthreads();
+                stage_queries(p, w, s / kBlockSteps, lds, q_sum, tile == 0);
+                __syncthreads();
+            }
+            v4i_t kb[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t pl[4];
+                transpose4((uint32_t)x[c][0], (uint32_t)x[c][1], (uint32_t)x[c][2], (uint32_t)x[c][3], pl);
+#pragma unroll
+                for (int k = 0; k < 4; k++) kb[k][c] = (int)(k < 3 ? pl[k] ^ kByteTops : pl[k]);
+            }
+            if (s + 1 < steps) fetch(tile, s + 1);
+            else if (tile + 1 < tiles) fetch(tile + 1, 0);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) k_dot[k] = __builtin_amdgcn_sdot4(kb[k][c], 0x01010101, k_dot[k], false);
+            const v4i_t* qa = reinterpret_cast<const v4i_t*>(lds) + ((s % kBlockSteps) * 16 + w.kg) * kRows + w.col;
+#pragma unroll
+            for (uint32_t rb = 0; rb < 4; rb++) {
+                if (rb >= row_blocks) break;
+#pragma unroll
+                for (int a = 0; a < 4; a++) {
+                    const v4i_t f = qa[a * 4 * kRows + 16 * rb];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[k], f, acc[rb][a + k], 0, 0, 0);
+                }
+            }
+        }
+        // register i of lane l: position 4 (l / 16) + i of the wave's 16, row l % 16 of a block
+        int64_t k_sum = 0;
+#pragma unroll
+        for (int k = 3; k >= 0; k--) k_sum = k_sum * 256 + k_dot[k];
+        k_sum += __shfl_xor(k_sum, 16, 64);
+        k_sum += __shfl_xor(k_sum, 32, 64);
+        uint64_t more[4];
+        int64_t o[4];
+        const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, t0 = seen.tile(v) * kRows + in_tile;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            more[i] = (uint64_t)kCacheOffset * (uint64_t)(__shfl(k_sum, (int)(4 * w.kg + i), 64) + kCacheOffset * dim);
+            o[i] = off[tile * kRows + in_tile + i];
+        }
+#pragma unroll
+        for (uint32_t rb = 0; rb < 4; rb++) {
+            const uint32_t r = 16 * rb + w.col;
+            if (r >= w.R) continue;
+            const uint64_t q_more = (uint64_t)kCacheOffset * q_sum[r];
+            const uint32_t pos = w.pos_of(p, r);
+            const size_t row = w.row(p, r);
+            v4u_t q, rem;
+            uint32_t there = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                uint64_t y = 0;
+#pragma unroll
+                for (int g = 6; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[rb][g][i];
+                y += more[i] + q_more;
+                uint32_t wide = 0;
+                int32_t qi, ri;
+                p.qk.apply(o[i] < 0 ? 0 : (int64_t)y, qi, ri, wide);          // a page outside: zero
+                q[i] = qi;
+                rem[i] = ri;
+                if (step::sees(pos, t0 + i, p.a.window, p.a.sinks)) {
+                    there |= 1u << i;
+                    bad |= wide;
+                    mx[rb] = max(mx[rb], qi);
+                }
+            }
+            int32_t* to = p.scores.at(row, t0, v);
+            int32_t* to_rem = p.a.d_scores_rem ? p.a.d_scores_rem + row * p.a.max_len + t0 : nullptr;
+            if (there == 15u) {
+                *reinterpret_cast<v4u_t*>(to) = q;
+                if (to_rem) *reinterpret_cast<v4u_t*>(to_rem) = rem;
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) {
+                    if (!((there >> i) & 1u)) continue;
+                    to[i] = q[i];
+                    if (to_rem) to_rem[i] = rem[i];
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int rb = 0; rb < 4; rb++) {
+        mx[rb] = max(mx[rb], __shfl_xor(mx[rb], 16, 64));
+        mx[rb] = max(mx[rb], __shfl_xor(mx[rb], 32, 64));
+        if (w.kg == 0) top[w.wave][16 * rb + w.col] = mx[rb];
+    }
+    __syncthreads();
+    if (threadIdx.x < w.R) {
+        int32_t m = top[0][threadIdx.x];
+#pragma unroll
+        for (int i = 1; i < 4; i++) m = max(m, top[i][threadIdx.x]);
+        p.chunk_max[w.row(p, threadIdx.x) * p.plan.score_chunks + blockIdx.y] = m;
+    }
+    if (bad) atomicOr(p.status, bad);
+}
+
+// Exponentials of 64 rows and a chunk of the positions, and the rows' sums, to which the chunks add.
+__global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
+    __shared__ int32_t top[kRows];
+    RowTile w;
+    if (!w.find(p, blockIdx.x)) return;
+    const step::Seen seen = w.seen(p);
+    const uint32_t v0 = blockIdx.y * p.plan.exp_cols;
+    if (v0 >= seen.tiles) return;
+    const uint32_t tiles = min(p.plan.exp_cols, seen.tiles - v0), parts = (seen.tiles - 1) / p.plan.score_cols + 1;
+    if (threadIdx.x < kRows) top[threadIdx.x] = INT32_MIN;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < parts * kRows; i += 256) {
+        const uint32_t r = i % kRows;
+        if (r < w.R) atomicMax(&top[r], p.chunk_max[w.row(p, r) * p.plan.score_chunks + i / kRows]);
+    }
+    __syncthreads();
+    if (blockIdx.y == 0 && p.a.d_max && threadIdx.x < w.R) p.a.d_max[w.row(p, threadIdx.x)] = top[threadIdx.x];
+    uint32_t bad = 0;
+    for (uint32_t r = w.wave; r < w.R; r += 4) {
+        const uint32_t pos = w.pos_of(p, r);
+        const size_t row = w.row(p, r);
+        const int32_t mx = top[r];
+        unsigned long long sum = 0;
+        for (uint32_t i = 4 * w.lane; i < tiles * kRows; i += 256) {
+            const uint32_t v = v0 + i / kRows, t = seen.tile(v) * kRows + i % kRows;
+            const int32_t* from = p.scores.at(row, t, v);
+            uint32_t there = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) there |= step::sees(pos, t + j, p.a.window, p.a.sinks) ? 1u << j : 0u;
+            if (!there) continue;
+            v4u_t x = {mx, mx, mx, mx}, e, shifted;
+            if (there == 15u) {
+                x = *reinterpret_cast<const v4u_t*>(from);
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++)
+                    if ((there >> j) & 1u) x[j] = from[j];
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const int64_t idx = (int64_t)x[j] - mx + (((int64_t)1 << p.a.bit_shift) - 1);
+                const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
+                e[j] = p.a.d_exp_table[ok ? idx : 0];
+                shifted[j] = (int32_t)((int64_t)x[j] - mx);
+                if ((there >> j) & 1u) {
+                    if (!ok) bad |= (uint32_t)kWitIndex;
+                    if (e[j] < 0) bad |= (uint32_t)kWitSum;
+                    sum += (unsigned long long)max(e[j], 0);
+                }
+            }
+            int32_t* to = p.exps.at(row, t, v);
+            int32_t* to_shifted = p.a.d_shifted ? p.a.d_shifted + row * p.a.max_len + t : nullptr;
+            if (there == 15u) {
+                *reinterpret_cast<v4u_t*>(to) = e;
+                if (to_shifted) *reinterpret_cast<v4u_t*>(to_shifted) = shifted;
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {
+                    if (!((there >> j) & 1u)) continue;
+                    to[j] = e[j];
+                    if (to_shifted) to_shifted[j] = shifted[j];
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+        if (w.lane == 0) atomicAdd(&p.sums[row], sum);
+    }
+    if (bad) atomicOr(p.status, bad);
+}
+
+// Probabilities of 64 rows and their products with 128 elements of the values, over a chunk of the positions.  Eight threads a row make
+// the digits of 64 positions in LDS while the waves multiply the 64 before them; a wave takes 16 elements and all rows, and turns
+// its values into operands in registers.
+constexpr uint32_t kValueThreads = 512;
+template <int PP>
+__global__ void __launch_bounds__(kValueThreads, 2) wit_window_values_kernel(WindowArgs p) {
+    __shared__ __attribute__((aligned(16))) uint32_t digits[2][PP * 4 * kRows * 4];
+    __shared__ int64_t off[step::kOffsetTiles * kRows];
+    __shared__ unsigned long long p_sum[kRows];
+    RowTile w;
+    if (!w.find(p, blockIdx.x)) return;
+    const step::Seen seen = w.seen(p);
+    const uint32_t group = blockIdx.y % p.plan.groups, chunk = blockIdx.y / p.plan.groups, v0 = chunk * p.plan.value_cols, dim = p.c.dim;
+    if (v0 >= seen.tiles) return;
+    const uint32_t tiles = min(p.plan.value_cols, seen.tiles - v0);
+    uint32_t bad = 0;
+    // of the probabilities: this thread's row and its eight positions of a tile
+    const uint32_t r = threadIdx.x >> 3, part = threadIdx.x & 7u;
+    const bool mine = r < w.R, write = group == 0;
+    const uint32_t rr = mine ? r : 0, pos = w.pos_of(p, rr);
+    const size_t row = w.row(p, rr);
+    unsigned long long sum = p.sums[row], all = 0;
+    if (sum == 0) {
+        if (mine) bad |= (uint32_t)kWitSum;
+        sum = 1;
+    }
+    if (mine && write && chunk == 0 && part == 0 && p.a.d_sum) store_sum(&p.a.d_sum[row], sum, bad);
+    const double inv = 1.0 / (double)sum;
+    int32_t e[8];
+    auto fetch_exps = [&](uint32_t tile) {
+        const uint32_t v = v0 + tile, t = seen.tile(v) * kRows + 8 * part;
+        const int32_t* from = p.exps.at(row, t, v);
+        uint32_t there = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) there |= mine && step::sees(pos, t + j, p.a.window, p.a.sinks) ? 1u << j : 0u;
+        if (there == 255u) {
+            *reinterpret_cast<v4u_t*>(e) = *reinterpret_cast<const v4u_t*>(from);
+            *reinterpret_cast<v4u_t*>(e + 4) = *reinterpret_cast<const v4u_t*>(from + 4);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) e[j] = (there >> j) & 1u ? from[j] : 0;
+        }
+    };
+    auto make_digits = [&](uint32_t tile) {
+        const uint32_t v = v0 + tile, t = seen.tile(v) * kRows + 8 * part;
+        uint32_t there = 0, d[8];
+        int32_t pr[8], query[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) {
+            there |= mine && step::sees(pos, t + j, p.a.window, p.a.sinks) ? 1u << j : 0u;
+            const uint32_t x = (uint32_t)max(e[j], 0);
+            uint32_t pj = probability(x, (uint64_t)p.a.prob_scale, sum, inv);
+            const bool seen_j = (there >> j) & 1u;
+            uint32_t wide = 0;
+            store_sum(&query[j], lookup_query(x, p.a.prob_scale, sum, pj), wide);
+            if (seen_j && write && p.a.d_query) bad |= wide;
+            pr[j] = (int32_t)pj;
+            if (!seen_j || off[(tile % step::kOffsetTiles) * kRows + 8 * part + j] < 0) pj = 0;
+            all += pj;
+            d[j] = digits_of((int32_t)pj);
+        }
+        if (write) {
+            const size_t o = row * p.a.max_len + t;
+            if (there == 255u) {
+                if (p.a.d_prob) {
+                    *reinterpret_cast<v4u_t*>(p.a.d_prob + o) = *reinterpret_cast<v4u_t*>(pr);
+                    *reinterpret_cast<v4u_t*>(p.a.d_prob + o + 4) = *reinterpret_cast<v4u_t*>(pr + 4);
+                }
+                if (p.a.d_query) {
+                    *reinterpret_cast<v4u_t*>(p.a.d_query + o) = *reinterpret_cast<v4u_t*>(query);
+                    *reinterpret_cast<v4u_t*>(p.a.d_query + o + 4) = *reinterpret_cast<v4u_t*>(query + 4);
+                }
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 8; j++) {
+                    if (!((there >> j) & 1u)) continue;
+                    if (p.a.d_prob) p.a.d_prob[o + j] = pr[j];
+                    if (p.a.d_query) p.a.d_query[o + j] = query[j];
+                }
+            }
+        }
+        uint32_t p0[4], p1[4];
+        transpose4(d[0], d[1], d[2], d[3], p0);
+        transpose4(d[4], d[5], d[6], d[7], p1);
+        uint64_t* to = reinterpret_cast<uint64_t*>(digits[tile & 1]) + ((part >> 1) * kRows + r) * 2 + (part & 1u);
+#pragma unroll
+        for (int k = 0; k < PP; k++) to[k * 4 * kRows * 2] = ((uint64_t)p1[k] << 32) | p0[k];
+    };
+    auto make_offsets = [&](uint32_t tile) {
+        const uint32_t n = min(step::kOffsetTiles, tiles - tile) * kRows;
+        for (uint32_t i = threadIdx.x; i < n; i += kValueThreads) off[i] = offset_of(p, w, seen, seen.tile(v0 + tile + i / kRows) * kRows + i % kRows);
+    };
+    const uint32_t e0 = group * step::kValueDims + 16 * w.wave, el = min(e0 + w.col, dim - 1), row_blocks = (w.R + 15) / 16;
+    const int32_t* values = p.c.d_v + (int64_t)w.kv * p.c.head_stride + el;
+    const bool multiplies = e0 < dim;
+    int32_t x[16];
+    auto fetch_values = [&](uint32_t tile) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16; j++) x[j] = values[max(off[(tile % step::kOffsetTiles) * kRows + 16 * w.kg + j], (int64_t)0)];
+    };
+    constexpr int G = PP + 3;
+    v4i_t acc[4][G];
+#pragma unroll
+    for (int rb = 0; rb < 4; rb++)
+#pragma unroll
+        for (int g = 0; g < G; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
+    fetch_exps(0);
+    for (uint32_t tile = 0; tile < tiles; tile++) {
+        if (tile % step::kOffsetTiles == 0) {
+            __syncthreads();          // nobody reads the offsets before any more
+            make_offsets(tile);
+            __syncthreads();
+        }
+        if (multiplies) fetch_values(tile);
+        make_digits(tile);
+        if (tile + 1 < tiles) fetch_exps(tile + 1);
+        __syncthreads();
+        if (!multiplies) continue;
+        v4i_t vb[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            uint32_t pl[4];
+            transpose4((uint32_t)x[4 * c], (uint32_t)x[4 * c + 1], (uint32_t)x[4 * c + 2], (uint32_t)x[4 * c + 3], pl);
+#pragma unroll
+            for (int k = 0; k < 4; k++) vb[k][c] = (int)(k < 3 ? pl[k] ^ kByteTops : pl[k]);
+        }
+        const v4i_t* pa = reinterpret_cast<const v4i_t*>(digits[tile & 1]) + w.kg * kRows + w.col;
+#pragma unroll
+        for (uint32_t rb = 0; rb < 4; rb++) {
+            if (rb >= row_blocks) break;
+#pragma unroll
+            for (int a = 0; a < PP; a++) {
+                const v4i_t f = pa[a * 4 * kRows + 16 * rb];
+#pragma unroll
+                for (int k = 0; k < 4; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[k], f, acc[rb][a + k], 0, 0, 0);
+            }
+        }
+    }
+    all += __shfl_xor(all, 1, 64);
+    all += __shfl_xor(all, 2, 64);
+    all += __shfl_xor(all, 4, 64);
+    if (part == 0) p_sum[r] = all;
+    __syncthreads();
+    const bool whole = seen.tiles <= p.plan.value_cols;          // all positions of the rows are this workgroup's
+    const uint32_t e1 = e0 + 4 * w.kg;
+#pragma unroll
+    for (uint32_t rb = 0; rb < 4; rb++) {
+        const uint32_t q_row = 16 * rb + w.col;
+        if (q_row >= w.R || e1 >= dim) continue;
+        const uint64_t more = (uint64_t)kCacheOffset * p_sum[q_row];
+        const size_t to = w.row(p, q_row);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            if (e1 + i >= dim) break;
+            uint64_t y = 0;
+#pragma unroll
+            for (int g = G - 1; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[rb][g][i];
+            y += more;
+            if (whole) {
+                int32_t q, rem;
+                p.out.apply((int64_t)y, q, rem, bad);
+                p.a.d_out[to * dim + e1 + i] = q;
+                if (p.a.d_out_rem) p.a.d_out_rem[to * dim + e1 + i] = rem;
+            } else {
+                p.part[(to * p.plan.value_chunks + chunk) * dim + e1 + i] = (int64_t)y;
+            }
+        }
+    }
+    if (bad) atomicOr(p.status, bad);
+}
+
+// The chunks' partial sums of 64 elements of 64 rows.
+__global__ void __launch_bounds__(256) wit_window_join_kernel(WindowArgs p) {
+    RowTile w;
+    if (!w.find(p, blockIdx.x)) return;
+    const step::Seen seen = w.seen(p);
+    if (seen.tiles <= p.plan.value_cols) return;
+    const uint32_t parts = (seen.tiles - 1) / p.plan.value_cols + 1, e = blockIdx.y * 64 + w.lane, dim = p.c.dim;
+    if (e >= dim) return;
+    uint32_t bad = 0;
+    for (uint32_t r = w.wave; r < w.R; r += 4) {
+        const size_t row = w.row(p, r);
+        int64_t y = 0;
+        for (uint32_t i = 0; i < parts; i++) y += p.part[(row * p.plan.value_chunks + i) * dim + e];
+        int32_t q, rem;
+        p.out.apply(y, q, rem, bad);
+        p.a.d_out[row * dim + e] = q;
+        if (p.a.d_out_rem) p.a.d_out_rem[row * dim + e] = rem;
+    }
+    if (bad) atomicOr(p.status, bad);
+}
+
+}  // namespace grape
+
+using namespace grape;
+
+extern "C" {
+
+size_t grape_wit_window_attention_workspace(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_new, uint32_t max_len, uint32_t window, uint32_t sinks) {
+    return step::window_workspace(rows, seqs, heads, cache_heads, dim, max_new, max_len, window, sinks);
+}
+
+int grape_wit_window_attention(const grape_wit_window_attention_args* args, const grape_wit_cache* cache, grape_stream_t st) {
+    GRAPE_REQUIRE(initialised(), "grape_init has not been called");
+    GRAPE_REFUSED_IF(step::refuse_window(args, cache));
+    if (!args->seqs || !args->rows || !args->max_new) return GRAPE_OK;
+    WindowArgs p;
+    p.a = *args;
+    p.c = *cache;
+    const grape_wit_window_attention_args& a = p.a;
+    step::window_plan(a.rows, a.seqs, a.heads, p.c.heads, p.c.dim, a.max_new, a.max_len, a.window, a.sinks, p.plan);
+    const step::WindowPlan& pl = p.plan;
+    uint8_t* ws = (uint8_t*)a.d_workspace;
+    const size_t cols = (size_t)pl.cols * kRows;
+    p.scores = a.d_scores ? Rows{a.d_scores, a.max_len, true} : Rows{(int32_t*)(ws + pl.at_scores), cols, false};
+    p.exps = a.d_exp ? Rows{a.d_exp, a.max_len, true} : Rows{(int32_t*)(ws + pl.at_exp), cols, false};
+    p.chunk_max = (int32_t*)(ws + pl.at_max);
+    p.sums = (unsigned long long*)(ws + pl.at_sum);
+    p.part = (int64_t*)(ws + pl.at_part);
+    p.page = token::fast_div(p.c.page_size);
+    p.by_each = token::fast_div(pl.each);
+    p.qk = scaler(a.qk_scale);
+    p.out = scaler(a.out_scale);
+    hipStream_t s = as_stream(st);
+    const int rc = wit_status_word(&p.status);
+    if (rc) return rc;
+    auto aligned = [&](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+    const bool vec = p.c.dim % 4 == 0 && ((p.c.page_stride | p.c.token_stride | p.c.head_stride) & 3) == 0 && aligned(p.c.d_k);
+    p.q_vec = p.c.dim % 4 == 0 && a.q_stride % 4 == 0 && aligned(a.d_q);
+    const uint32_t along = pl.tiles * p.c.heads;
+    const size_t score_lds = (size_t)std::min(pl.dim64, kBlockSteps) * 16 * kRows * 16 + (size_t)pl.score_cols * kRows * 8;
+    if (vec) wit_window_scores_kernel<true><<<dim3(along, pl.score_chunks), 256, score_lds, s>>>(p);
+    else wit_window_scores_kernel<false><<<dim3(along, pl.score_chunks), 256, score_lds, s>>>(p);
+    GRAPE_LAUNCH_CHECK();
+    wit_window_exp_kernel<<<dim3(along, pl.exp_chunks), 256, 0, s>>>(p);
+    GRAPE_LAUNCH_CHECK();
+    const dim3 values(along, pl.value_chunks * pl.groups);
+    if (a.prob_scale <= ((int64_t)1 << 22)) wit_window_values_kernel<3><<<values, kValueThreads, 0, s>>>(p);
+    else wit_window_values_kernel<4><<<values, kValueThreads, 0, s>>>(p);
+    GRAPE_LAUNCH_CHECK();
+    if (pl.value_chunks > 1) {
+        wit_window_join_kernel<<<dim3(along, pl.dim64), 256, 0, s>>>(p);
+        GRAPE_LAUNCH_CHECK();
+    }
+    return GRAPE_OK;
+}
+
+}  // extern "C"

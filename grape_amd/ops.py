@@ -932,6 +932,157 @@ def wit_matvec_q4(x, w, scales, group, zeros=None, scale=1 << 16, q=None, r=None
     return q, r
 
 
+# ------------------------------------------------------------------ the step around new tokens
+_PAGES = struct.Struct("<10Q8I")
+_WINDOW = struct.Struct("<Qq16Q3q10I")
+_NEXT = struct.Struct("<16Q5q4I")
+_PAGES_OUT = ("starts", "positions", "slots", "lens", "free_span")
+
+
+def wit_page_step(lens, new, block_table, free_pages, free_span, page_size, rows, window=0, sinks=0, out=None):
+    """The pages, positions and slots of a step's new tokens.  Sequence b has lens[b] tokens in the cache and gets new[b] more
+    (-1: its request is over); the pages that this takes come from the ring free_pages with free_span = (head, count) and go into
+    block_table (seqs, pages of a sequence); pages that a window of `window` tokens and the first `sinks` leave behind, or that
+    a request has left, go to the ring's end.  All int32.  Returns a dict of new tensors, or `out`, such a dict to write to: "starts" (seqs + 1),
+    "positions" (rows) and "slots" (rows, int64: -1 behind the last token) for wit_rope_append and wit_window_attention, "lens" and
+    "free_span" for the next step.  `rows` bounds the step's tokens; where they, the free pages or the ring's room do not suffice, bit 32 of
+    wit_status is set and the sequences from the first that does not fit get no tokens."""
+    lib = init()
+    dev = _place()
+    n = len(lens)
+    width = block_table.shape
+    if len(width) != 2 or width[0] != n:
+        _refuse("block_table must be (seqs, pages)")
+    if free_pages.dim() != 1:
+        _refuse("free_pages must have one axis")
+    if rows < 0 or rows >> 31:
+        _refuse("rows must be in 0..2^31 - 1")
+    if out is None:
+        out = {"starts": _i32(n + 1), "positions": _i32(rows), "slots": torch.empty(rows, dtype=torch.int64, device="cuda"), "lens": _i32(n), "free_span": _i32(2)}
+    elif set(out) != set(_PAGES_OUT):
+        _refuse("out must hold %s", ", ".join(_PAGES_OUT))
+    args = _pack(_PAGES, _arr(lens, "lens", (n,), dev), _arr(new, "new", (n,), dev), _arr(free_span, "free_span", (2,), dev),
+                 _arr(block_table, "block_table", width, dev), _arr(free_pages, "free_pages", free_pages.shape, dev),
+                 _arr(out["starts"], "starts", (n + 1,), dev), _arr(out["positions"], "positions", (rows,), dev),
+                 _arr(out["slots"], "slots", (rows,), dev, torch.int64), _arr(out["lens"], "lens", (n,), dev), _arr(out["free_span"], "free_span", (2,), dev),
+                 n, width[1], free_pages.shape[0], rows, page_size, window, sinks, 0)
+    _check(lib.grape_wit_page_step(args, _stream(dev)))
+    return out
+
+
+def wit_window_attention(q, k_cache, v_cache, block_table, starts, lens, max_new, max_len, exp_table, window=0, sinks=0, bit_shift=20, index_bits=20,
+                         qk_scale=1 << 22, prob_scale=1 << 16, out_scale=1 << 16, out=None, proof=True, workspace=None):
+    """wit_paged_attention for several new tokens a sequence: q (rows, heads, dim), of which starts[b]:starts[b + 1] are the last tokens of
+    sequence b with lens[b] tokens (themselves among them).  Each attends to what stands before it and to itself, with `window` > 0 only to the last
+    `window` of these and the first `sinks`.  max_new and max_len bound the sequences' new tokens and lengths.  Returns the dict of
+    wit_paged_attention, with rows in the place of seqs; positions that a token does not attend to and rows of no sequence are not
+    written (0 where the call makes the tensors).  `out` and `workspace` as there (wit_window_attention_workspace(...) bytes)."""
+    lib = init()
+    dev = _place()
+    cache, heads_kv, dim = _cache(k_cache, v_cache, dev)
+    if q.dim() != 3:
+        _refuse("q must be (rows, heads, dim)")
+    n, heads, _ = q.shape
+    seqs = len(lens)
+    rows, row, one = (n, heads, max_len), (n, heads, dim), (n, heads)
+    qp, qs = _rows(q, "q", row, dev)
+    width = block_table.shape
+    if len(width) != 2 or width[0] != seqs:
+        _refuse("block_table must be (seqs, pages)")
+    if exp_table.shape != (1 << index_bits,):
+        _refuse("the exponential table must have 2^index_bits entries")
+    if max_len < 0 or max_len >> 31 or max_new < 0 or max_new >> 31:
+        _refuse("max_len and max_new must be in 0..2^31 - 1")
+    if out is None:
+        out = {"qkv": torch.zeros(row, dtype=torch.int32, device=q.device), "qkv_rem": torch.zeros(row, dtype=torch.int32, device=q.device)}
+        if proof:
+            for name in ("max", "exp_sum"):
+                out[name] = torch.zeros(one, dtype=torch.int32, device=q.device)
+            for name in _PROOF_ROWS:
+                out[name] = torch.zeros(rows, dtype=torch.int32, device=q.device)
+    get = out.get
+    if "qkv" not in out or not _NAMES.issuperset(out):
+        _refuse("out must hold qkv, and may hold %s", ", ".join(sorted(_NAMES)))
+    if workspace is None:
+        size = wit_window_attention_workspace(n, seqs, heads, heads_kv, dim, max_new, max_len, window, sinks)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    space, size = _space(workspace, dev) if workspace is not None else (0, 0)
+    args = _pack(_WINDOW, qp, qs, _arr(block_table, "block_table", width, dev), _arr(starts, "starts", (seqs + 1,), dev), _arr(lens, "lens", (seqs,), dev),
+                 _arr(exp_table, "exp_table", exp_table.shape, dev), *[_arr(get(name), name, rows, dev) for name in _PROOF_ROWS],
+                 _arr(get("max"), "max", one, dev), _arr(get("exp_sum"), "exp_sum", one, dev), _arr(get("qkv"), "qkv", row, dev),
+                 _arr(get("qkv_rem"), "qkv_rem", row, dev), space, size, qk_scale, prob_scale, out_scale, n, seqs,
+                 heads, max_new, max_len, width[1], window, sinks, bit_shift, index_bits)
+    _check(lib.grape_wit_window_attention(args, cache, _stream(dev)))
+    return out
+
+
+def wit_window_attention_workspace(rows, seqs, heads, cache_heads, dim, max_new, max_len, window=0, sinks=0):
+    """bytes of workspace that wit_window_attention needs; 0 for sizes that it refuses"""
+    sizes = (rows, seqs, heads, cache_heads, dim, max_new, max_len, window, sinks)
+    if min(sizes) < 0 or max(sizes) >> 31:
+        return 0
+    return init().grape_wit_window_attention_workspace(*sizes)
+
+
+_NEXT_ROWS = ("logits", "rem", "count", "gap")
+
+
+def wit_next_token(logits, history=None, history_lens=None, repetition=None, presence=None, frequency=None, bias=None, mask=None, scale=1 << 16, out=None,
+                   proof=True, workspace=None):
+    """The choice of the next token from logits (seqs, vocab).  A token that occurs among the first history_lens[b] of history (seqs, tokens;
+    negative ones are skipped) has its logit divided (if positive) or multiplied (else) by repetition[b] / scale and lowered by presence[b] + frequency[b] for
+    each time; bias (vocab) or (seqs, vocab) is added; mask (seqs, ceil(vocab / 32)) or one row of it holds a bit for each token that may be
+    chosen, the first in a word's lowest.  All int32.  Returns a dict: "token" (seqs), the first with the largest logit or -1 where none may be chosen,
+    and "max" (seqs); for a proof also "logits", "rem", "count" and "gap" (seqs, vocab): the logits after all this, the divisions' remainders, how often each token
+    occurs, and how far each logit is below the largest.  `out`: such a dict to write to; "token" has to be there.  `workspace`: a uint8 tensor
+    of wit_next_token_workspace(...) bytes."""
+    lib = init()
+    dev = _place()
+    if logits.dim() != 2:
+        _refuse("logits must be (seqs, vocab)")
+    n, vocab = logits.shape
+    lp, ls = _rows(logits, "logits", (n, vocab), dev)
+    hp = hs = width = 0
+    if history is not None:
+        if history.dim() != 2 or history_lens is None:
+            _refuse("history must be (seqs, tokens), with history_lens")
+        width = history.shape[1]
+        hp, hs = _rows(history, "history", (n, width), dev)
+    elif history_lens is not None:
+        _refuse("history_lens needs history")
+    bp = bs = mp = ms = 0
+    if bias is not None:
+        bp, bs = _rows(bias, "bias", (n, vocab), dev) if bias.dim() == 2 else (_arr(bias, "bias", (vocab,), dev), 0)
+    if mask is not None:
+        words = (vocab + 31) // 32
+        mp, ms = _rows(mask, "mask", (n, words), dev) if mask.dim() == 2 else (_arr(mask, "mask", (words,), dev), 0)
+    if out is None:
+        out = {"token": _i32(n), "max": _i32(n)}
+        if proof:
+            for name in _NEXT_ROWS:
+                out[name] = _i32(n, vocab)
+    get = out.get
+    if "token" not in out or not set(out) <= {"token", "max", *_NEXT_ROWS}:
+        _refuse("out must hold token, and may hold max, %s", ", ".join(_NEXT_ROWS))
+    if workspace is None:
+        size = wit_next_token_workspace(n, vocab)
+        workspace = torch.empty(size, dtype=torch.uint8, device=logits.device) if size else None
+    space, size = _space(workspace, dev) if workspace is not None else (0, 0)
+    one, all_ = (n,), (n, vocab)
+    args = _pack(_NEXT, lp, hp, _arr(history_lens, "history_lens", one, dev), _arr(repetition, "repetition", one, dev), _arr(presence, "presence", one, dev),
+                 _arr(frequency, "frequency", one, dev), bp, mp, *[_arr(get(name), name, all_, dev) for name in _NEXT_ROWS],
+                 _arr(out["token"], "token", one, dev), _arr(get("max"), "max", one, dev), space, size, ls, hs, bs, ms, scale, n, vocab, width, 0)
+    _check(lib.grape_wit_next_token(args, _stream(dev)))
+    return out
+
+
+def wit_next_token_workspace(seqs, vocab):
+    """bytes of workspace that wit_next_token needs; 0 for sizes that it refuses"""
+    if min(seqs, vocab) < 0 or max(seqs, vocab) >> 31:
+        return 0
+    return init().grape_wit_next_token_workspace(seqs, vocab)
+
+
 def wit_status():
     """status bits set since the last call (synchronises and clears them)"""
     lib = init()

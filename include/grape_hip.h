@@ -776,15 +776,98 @@ size_t grape_wit_matvec_q4_workspace(uint32_t tokens, uint32_t outputs, uint32_t
 int grape_wit_matvec_q4(int32_t *d_q, int32_t *d_r, const int32_t *d_x, int64_t x_stride, const uint8_t *d_w, int64_t w_stride,
                         const int32_t *d_scales, const uint8_t *d_zeros, uint32_t tokens, uint32_t outputs, uint32_t inputs,
                         uint32_t group, int64_t scale, void *d_workspace, size_t workspace_bytes, grape_stream_t stream);
+/* The step around new tokens: where they stand, what they attend to, and which token comes next.  Enqueued only, nothing but
+ * kernels, no scratch of the stream's pool; no counterpart in the reference.
+ *
+ * Pages, positions and slots from the requests' lengths.  Sequence b has d_lens[b] tokens in the cache, in the pages
+ * d_block_table[b*table_stride + t/page_size], and gets d_new[b] more; d_new[b] = -1 says that its request is over.  Pages that
+ * this takes come from a ring of free ones, d_free[(head + k) % ring] for k < count, with d_span = {head, count}, in the order of the
+ * sequences, and their numbers go into the block table.  Behind the ring's last entry go, in the same order, pages that are not
+ * needed after this step: those of requests that are over, and with `window` > 0 those whose tokens all lie further back than the
+ * next token sees - it sees the last `window` tokens, itself among them, and the first `sinks`.  They are still read by this step's
+ * attention, and taken by a later step at the earliest; their entries in the block table keep their numbers and are not read
+ * again.  window and sinks must be those of the sequences' earlier steps.  A ring of twice as many entries as there are pages has
+ * room for everything.
+ *
+ * Writes d_starts[seqs + 1], the rows at which the sequences' tokens start (row after row, sequence after sequence);
+ * d_positions[rows] and d_slots[rows] (page*page_size + offset) of the tokens, 0 and -1 in rows behind the last; d_lens_out[seqs],
+ * the lengths after the step (0 where the request is over); d_span_out, the ring's head and count after it.  Outputs must
+ * not overlap each other or d_lens, d_new and d_span.
+ *
+ * Where the rows or the free pages do not suffice, GRAPE_WIT_PAGES is set and no sequence from the first one on that does not fit
+ * gets a token; the same bit says that the ring had no room for a page given back, which is lost then.  A negative length or one that leaves the table,
+ * d_new below -1 and a negative page set GRAPE_WIT_INDEX: such a sequence gets no token and keeps its length, a token of such a page slot -1.
+ * At most 4096 sequences; table_stride*page_size and seqs*table_stride below 2^31. */
+typedef struct {
+    const int32_t *d_lens, *d_new, *d_span;
+    int32_t *d_block_table, *d_free, *d_starts, *d_positions;
+    int64_t *d_slots;
+    int32_t *d_lens_out, *d_span_out;
+    uint32_t seqs, table_stride, ring, rows, page_size, window, sinks, reserved;
+} grape_wit_page_step_args;
+int grape_wit_page_step(const grape_wit_page_step_args *args, grape_stream_t stream);
+/* grape_wit_paged_attention for several new tokens a sequence: whole prompts, pieces of them, drafted tokens.  Sequence b's rows
+ * of the queries are d_starts[b] <= n < d_starts[b+1], its last tokens; d_lens[b] counts them too, and their keys and values stand in
+ * the cache already.  The token at position pos attends to the positions t <= pos, and with `window` > 0 only to those
+ * with t > pos - window or t < sinks.  Row n's queries stand at d_q + n*q_stride as [heads][dim].  The formulas, bits of status and
+ * outputs are those of grape_wit_paged_attention with [rows] in the place of [seqs]: the rows of a proof are
+ * [rows][heads][max_len], and positions that a token does not attend to, like rows of no sequence, are left as they were.
+ *
+ * max_new and max_len bound the sequences' new tokens and lengths.  A sequence outside these bounds, with fewer tokens than rows,
+ * or with more than table_stride*page_size, sets GRAPE_WIT_INDEX, and its rows are left as they were.  Pages that no token of
+ * the call sees are not read.  rows <= 2^24.  d_workspace as for grape_wit_paged_attention, grape_wit_window_attention_workspace(...)
+ * bytes. */
+typedef struct {
+    const int32_t *d_q;
+    int64_t q_stride;
+    const int32_t *d_block_table, *d_starts, *d_lens, *d_exp_table;
+    int32_t *d_scores, *d_scores_rem, *d_shifted, *d_exp, *d_prob, *d_query, *d_max, *d_sum, *d_out, *d_out_rem;
+    void *d_workspace;
+    size_t workspace_bytes;
+    int64_t qk_scale, prob_scale, out_scale;
+    uint32_t rows, seqs, heads, max_new, max_len, table_stride, window, sinks, bit_shift, index_bits;
+} grape_wit_window_attention_args;
+size_t grape_wit_window_attention_workspace(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim,
+                                            uint32_t max_new, uint32_t max_len, uint32_t window, uint32_t sinks);
+int grape_wit_window_attention(const grape_wit_window_attention_args *args, const grape_wit_cache *cache, grape_stream_t stream);
+/* The choice of the next token.  Row b's logits x stand at d_logits + b*logits_stride, and count[v] is how often v is among the
+ * first d_history_lens[b] tokens at d_history + b*history_stride (negative ones are skipped).  Where count > 0
+ *     x becomes floor((x*scale + floor(rep/2)) / rep) if x > 0, else floor((x*rep + floor(scale/2)) / scale), with rep = d_repetition[b],
+ *     and then loses d_presence[b] + d_frequency[b]*count;
+ * everywhere the bias at d_bias + b*bias_stride is added (stride 0: the same for all rows).  Token v is excluded where bit v % 32 of
+ * word v/32 at d_mask + b*mask_stride is 0, or where its logit or its bias is INT32_MIN; its logit becomes INT32_MIN.  Each of history (0),
+ * d_repetition, d_presence, d_frequency, d_bias and d_mask (NULL) may be left out.
+ *
+ * d_token[b] is the token with the largest logit, the first of several, or -1 where all are excluded; d_max[b] that logit.  For a
+ * proof, [seqs][vocab] each: d_out the logits, d_rem the division's remainders (0 where there was none), d_count, and d_gap, the
+ * largest logit less each (0 where excluded), to be looked up in a range.  All but d_token may be NULL; d_out may be d_logits where
+ * logits_stride = vocab, else outputs must not overlap each other or logits and biases.
+ *
+ * A logit beyond int32 sets GRAPE_WIT_QUOTIENT and becomes the nearest one that is not excluded; a gap beyond int32 sets
+ * GRAPE_WIT_SUM_WIDE, with its low 32 bits stored.  rep < 1 (taken as none), a history length outside 0..history (taken as the
+ * nearest) and a token of the history outside the vocabulary (skipped) set GRAPE_WIT_INDEX.  1 <= scale <= 2^31; vocab <= 2^24.
+ * d_workspace (16-byte aligned): grape_wit_next_token_workspace(...) bytes, one for each of the calls that may run at the same time. */
+typedef struct {
+    const int32_t *d_logits, *d_history, *d_history_lens, *d_repetition, *d_presence, *d_frequency, *d_bias, *d_mask;
+    int32_t *d_out, *d_rem, *d_count, *d_gap, *d_token, *d_max;
+    void *d_workspace;
+    size_t workspace_bytes;
+    int64_t logits_stride, history_stride, bias_stride, mask_stride, scale;
+    uint32_t seqs, vocab, history, reserved;
+} grape_wit_next_token_args;
+size_t grape_wit_next_token_workspace(uint32_t seqs, uint32_t vocab);
+int grape_wit_next_token(const grape_wit_next_token_args *args, grape_stream_t stream);
 /* Synchronises, returns the status bits set since the last call and clears them: 1 = a quotient left
  * int32, 2 = a table index out of range (the reference's assertions, model.py:86-87, :137-138),
  * 4 = a softmax row summed to zero or met a negative table entry, 8 = a sum of squares left 64 bits,
- * 16 = a sum of exponentials or a lookup query that grape_wit_paged_attention was asked for left int32. */
+ * 16 = a sum of exponentials or a lookup query that an attention was asked for, or a gap of grape_wit_next_token, left int32,
+ * 32 = grape_wit_page_step ran out of free pages, rows or room in the ring. */
 #define GRAPE_WIT_QUOTIENT 1u
 #define GRAPE_WIT_INDEX 2u
 #define GRAPE_WIT_SUM 4u
 #define GRAPE_WIT_SQUARES 8u
 #define GRAPE_WIT_SUM_WIDE 16u
+#define GRAPE_WIT_PAGES 32u
 int grape_wit_status(uint32_t *flags, grape_stream_t stream);
 
 /* ------------------------------------------------------------------ measurement -------------- */
