@@ -254,3 +254,95 @@ def weights_q4(w, scales, group, zeros, inputs):
 
 def matvec_q4(x, w, scales, group, zeros, scale=SCALE):
     return rescale(matmul_t(x, weights_q4(w, scales, group, zeros, x.shape[1])), scale)
+
+
+# ------------------------------------------------------------------ the step around new tokens
+def page_step(lens, new, block_table, ring, span, page, rows, window=0, sinks=0):
+    """Sequence after sequence, page after page.  Writes into block_table and ring; returns a dict of starts, positions, slots,
+    lens and free_span, and whether something ran out."""
+    ring_size, (head, count) = len(ring), span
+    most = page * block_table.shape[1]
+    starts, positions, slots, out_lens = [0], [0] * rows, [-1] * rows, []
+    taken, back, short, served = 0, [], False, True
+    # the last token that is not seen from position p on stands `window` before it
+    unseen = lambda i, p: window > 0 and i * page >= -(-sinks // page) * page and (i + 1) * page - 1 <= p - window  # noqa: E731
+    for b, (have, n) in enumerate(zip(lens, new)):
+        have, n = int(have), int(n)
+        ok = have >= 0 and n >= -1 and have + max(n, 0) <= most
+        more = max(n, 0) if ok else 0
+        need = -(-(have + more) // page) - -(-have // page) if ok else 0
+        if more and (starts[-1] + more > rows or taken + need > count):
+            served = False                       # and nobody behind it
+        if not served and more:
+            short, more, need = True, 0, 0
+        for k in range(need):
+            block_table[b, -(-have // page) + k] = ring[(head + taken + k) % ring_size]
+        taken += need
+        for j in range(more):
+            pg = int(block_table[b, (have + j) // page])
+            positions[starts[-1] + j] = have + j
+            slots[starts[-1] + j] = pg * page + (have + j) % page if pg >= 0 else -1
+        starts.append(starts[-1] + more)
+        over = ok and n == -1
+        out_lens.append(0 if over else have + more)
+        if ok:
+            back += [int(block_table[b, i]) for i in range(-(-(have + more) // page)) if (over or unseen(i, have + more)) and not unseen(i, have)]
+    room = ring_size - count
+    short |= len(back) > room
+    back = back[:room]
+    for k, p in enumerate(back):
+        ring[(head + count + k) % ring_size] = p
+    return {"starts": starts, "positions": positions, "slots": slots, "lens": out_lens,
+            "free_span": [(head + taken) % ring_size if ring_size else 0, count - taken + len(back)]}, short
+
+
+def window_attention(q, k_cache, v_cache, block_table, starts, lens, window, sinks, table, out, **kw):
+    """paged_attention of one token after the other, each over a cache of the positions that it sees"""
+    page = k_cache.shape[1]
+    for b in range(len(lens)):
+        n = int(starts[b + 1] - starts[b])
+        for j in range(n):
+            pos, row = int(lens[b]) - n + j, int(starts[b]) + j
+            sees = np.array([t for t in range(pos + 1) if not window or t > pos - window or t < sinks])
+            pages = np.asarray(block_table)[b, sees // page]
+            inside = (pages >= 0) & (pages < k_cache.shape[0])
+            own = [np.where(inside[:, None, None], c[np.where(inside, pages, 0), sees % page], 0)[:, None] for c in (k_cache, v_cache)]
+            one = {x: np.zeros((1, q.shape[1]) + ((len(sees),) if t.ndim == 3 and x not in ("qkv", "qkv_rem") else t.shape[2:]), dtype=np.int32) for x, t in out.items()}
+            paged_attention(q[row:row + 1], *own, np.arange(len(sees))[None], [len(sees)], [0], table, one, **kw)
+            for x, t in one.items():
+                if t.ndim == 3 and x not in ("qkv", "qkv_rem"):
+                    out[x][row][:, sees] = t[0]
+                else:
+                    out[x][row] = t[0]
+
+
+def next_token(logits, history=None, history_lens=None, repetition=None, presence=None, frequency=None, bias=None, mask=None, scale=SCALE):
+    """Returns the dict of token, max, logits, rem, count and gap (64-bit), and whether a logit left int32."""
+    lowest = -(1 << 31)
+    n, vocab = logits.shape
+    out = {x: np.zeros((n, vocab), dtype=np.int64) for x in ("logits", "rem", "count", "gap")} | {x: np.zeros(n, dtype=np.int64) for x in ("token", "max")}
+    left = False
+    for b in range(n):
+        count = np.zeros(vocab, dtype=np.int64)
+        if history is not None:
+            for t in np.asarray(history)[b, :history_lens[b]]:
+                if 0 <= t < vocab:
+                    count[t] += 1
+        z = np.full(vocab, lowest, dtype=np.int64)
+        for v in range(vocab):
+            x, extra = int(logits[b, v]), 0 if bias is None else int(np.asarray(bias)[b, v] if np.ndim(bias) == 2 else bias[v])
+            if x == lowest or extra == lowest or (mask is not None and not (int(np.asarray(mask)[b, v // 32] if np.ndim(mask) == 2 else mask[v // 32]) >> (v % 32)) & 1):
+                continue
+            if count[v]:
+                if repetition is not None:
+                    y, by = (x * scale, int(repetition[b])) if x > 0 else (x * int(repetition[b]), scale)
+                    x = (y + by // 2) // by
+                    out["rem"][b, v] = y - x * by
+                x -= (0 if presence is None else int(presence[b])) + (0 if frequency is None else int(frequency[b])) * int(count[v])
+            x += extra
+            left |= not lowest < x < 1 << 31
+            z[v] = min(max(x, lowest + 1), (1 << 31) - 1)
+        out["logits"][b], out["count"][b], out["max"][b] = z, count, z.max()
+        out["token"][b] = -1 if z.max() == lowest else z.argmax()
+        out["gap"][b] = np.where(z == lowest, 0, z.max() - z)
+    return out, left
