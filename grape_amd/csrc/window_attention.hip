@@ -12,12 +12,15 @@ namespace grape {
 // needed before the first exponential and the sum of all before the first probability, hence a launch for each of the three, and
 // a fourth that joins the values' partial sums where the positions are cut up.
 //
-// Both products run on the int8 matrix cores, exactly: an element x is taken as x - c, c = 128 (1 + 2^8 + 2^16), whose four balanced
-// digits are the bytes of x with the three lower top bits turned over, and sum q k = sum (q-c)(k-c) + c (sum (q-c) + sum (k-c)) + c^2 dim.
-// The pairs of planes with the same sum of exponents share an accumulator: 4 * 2^14 * 8192 elements stay below 2^31.
+// Both products run on the int8 matrix cores, exactly.  An element of magnitude below 2^23 is three balanced digits of base 256, the bytes
+// of x + 0x808080 with their top bits turned over, nine products of planes for a pair of operands and six where the probabilities
+// are small; pairs with the same sum of exponents share an accumulator (3 * 2^14 * 8192 elements stay below 2^31).  Where a larger
+// element turns up, the wave (or, for the values, the workgroup) takes its positions again with x - c, c = 128 (1 + 2^8 + 2^16), whose four
+// digits are the bytes of x with the three lower top bits turned over: sum q k = sum (q-c)(k-c) + c (sum (q-c) + sum (k-c)) + c^2 dim.
 // ------------------------------------------------------------------------------------------------
 using step::kRows;
-constexpr uint32_t kNoElement = 0x00808080;          // whose digits are all zero
+constexpr uint32_t kNoElement = 0x00808080;          // whose four digits are all zero
+constexpr uint32_t kThreeDigits = 0x00808080;        // added to an element, leaves 24 bits of it where three digits hold it
 typedef int v4u_t __attribute__((ext_vector_type(4), aligned(4)));
 
 // rows of a tensor of the proof, or of the workspace, which holds the tiles that are seen side by side
@@ -40,7 +43,31 @@ struct WindowArgs {
     int64_t* part;               // [rows][heads][value chunks][dim]
     uint32_t* status;
     bool q_vec;
+    double limit;                // of a score's product that is rescaled in double precision
+    double* factors;             // of the exponential table, see wit_window_table_kernel; null where it is not looked into
+    uint32_t* differs;
 };
+
+// the three planes of four elements; `over` gathers bits above the 24
+__device__ __forceinline__ void three_planes(v4i_t x, uint32_t out[3], uint32_t& over) {
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) u[j] = (uint32_t)x[j] + kThreeDigits;
+    over |= (u[0] | u[1]) | (u[2] | u[3]);
+    const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), b = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(u[1], u[0], 0x07030602u), d = __builtin_amdgcn_perm(u[3], u[2], 0x07030602u);
+    out[0] = __builtin_amdgcn_perm(b, a, 0x05040100u) ^ kByteTops;
+    out[1] = __builtin_amdgcn_perm(b, a, 0x07060302u) ^ kByteTops;
+    out[2] = __builtin_amdgcn_perm(d, c, 0x05040100u) ^ kByteTops;
+}
+constexpr uint32_t kOver = 0xff000000;
+
+// the four planes of x - kCacheOffset
+__device__ __forceinline__ void four_planes(v4i_t x, uint32_t out[4]) {
+    transpose4((uint32_t)x[0], (uint32_t)x[1], (uint32_t)x[2], (uint32_t)x[3], out);
+#pragma unroll
+    for (int k = 0; k < 3; k++) out[k] ^= kByteTops;
+}
 
 // A workgroup's rows: rows 64 * tile .. + R of the cache head kv of sequence b, whose n new tokens start at row `first` and position
 // `pos`.  Row r is query head r % each of token r / each.
@@ -93,50 +120,145 @@ __device__ __forceinline__ int64_t offset_of(const WindowArgs& p, const RowTile&
     return token::token_offset(p.c, p.a.d_block_table[(size_t)w.b * p.a.table_stride + pg], t - pg * p.c.page_size);
 }
 
-// The queries' digits of a block of 256 elements in LDS, [step of 64][plane][lane group][row], 16 bytes each; and their sums.
+// The queries' digits of a block of 256 elements in LDS, [step of 64][plane][lane group][row], 16 bytes each.
 constexpr uint32_t kBlockSteps = 4;
-__device__ __forceinline__ void stage_queries(const WindowArgs& p, const RowTile& w, uint32_t block, uint32_t* digits, unsigned long long* q_sum, bool sums) {
+__device__ __forceinline__ const int32_t* query_of(const WindowArgs& p, const RowTile& w, uint32_t r) {
+    const uint32_t tok = w.token(p, r);
+    return p.a.d_q + (int64_t)(w.first + tok) * p.a.q_stride + (size_t)(w.kv * p.plan.each + (w.at + r - tok * p.plan.each)) * p.c.dim;
+}
+// four elements of a row, `pad` where there is none
+__device__ __forceinline__ v4i_t elements(const int32_t* x, uint32_t e, uint32_t dim, bool vec, int32_t pad) {
+    v4i_t y = {pad, pad, pad, pad};
+    if (vec) {
+        if (e < dim) y = *reinterpret_cast<const v4i_t*>(x + e);
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+            if (e + j < dim) y[j] = x[e + j];
+    }
+    return y;
+}
+__device__ __forceinline__ void stage_queries(const WindowArgs& p, const RowTile& w, uint32_t block, uint32_t* digits, uint32_t& over) {
     const uint32_t steps = min(p.plan.dim64 - kBlockSteps * block, kBlockSteps), e0 = 64 * kBlockSteps * block;
     for (uint32_t i = threadIdx.x; i < kRows * steps * 16; i += blockDim.x) {
-        const uint32_t r = i / (steps * 16), quad = i - r * (steps * 16), s = quad >> 4, c = (quad >> 2) & 3u, g = quad & 3u, e = e0 + 4 * quad;
-        int32_t x[4];
+        const uint32_t r = i / (steps * 16), quad = i - r * (steps * 16), s = quad >> 4, c = (quad >> 2) & 3u, g = quad & 3u;
+        v4i_t x = {0, 0, 0, 0};
+        if (r < w.R) x = elements(query_of(p, w, r), e0 + 4 * quad, p.c.dim, p.q_vec, 0);
+        uint32_t pl[3];
+        three_planes(x, pl, over);
+        uint32_t* o = digits + (((s * 3 * 4 + g) * kRows + r) << 2) + c;
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++) x[j] = (int32_t)kNoElement;
-        if (r < w.R && e < p.c.dim) {
-            const uint32_t tok = w.token(p, r);
-            const int32_t* q = p.a.d_q + (int64_t)(w.first + tok) * p.a.q_stride + (size_t)(w.kv * p.plan.each + (w.at + r - tok * p.plan.each)) * p.c.dim;
-            if (p.q_vec) {
-                *reinterpret_cast<v4i_t*>(x) = *reinterpret_cast<const v4i_t*>(q + e);
-            } else {
+        for (uint32_t k = 0; k < 3; k++) o[k * 16 * kRows] = pl[k];
+    }
+}
+
+__device__ __forceinline__ uint32_t seen_of_four(const WindowArgs& p, uint32_t pos, uint32_t t) {
+    uint32_t there = 0;
 #pragma unroll
-                for (uint32_t j = 0; j < 4; j++)
-                    if (e + j < p.c.dim) x[j] = q[e + j];
+    for (uint32_t i = 0; i < 4; i++) there |= step::sees(pos, t + i, p.a.window, p.a.sinks) ? 1u << i : 0u;
+    return there;
+}
+__device__ __forceinline__ void store_four(int32_t* to, v4u_t x, uint32_t there) {
+    if (there == 15u) {
+        *reinterpret_cast<v4u_t*>(to) = x;
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+            if ((there >> i) & 1u) to[i] = x[i];
+    }
+}
+
+// The scores of a wave's positions with operands of any size, both from memory: sixteen rows at a time, four planes each.
+__device__ __forceinline__ void wide_scores(const WindowArgs& p, const RowTile& w, const step::Seen& seen, uint32_t v0, uint32_t tiles, const int64_t* off, int32_t mx[4], uint32_t& bad) {
+    const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
+    const uint32_t dim = p.c.dim;
+#pragma unroll 1
+    for (uint32_t tile = 0; tile < tiles; tile++) {
+        const int32_t* k_row = keys + max(off[tile * kRows + 16 * w.wave + w.col], (int64_t)0);
+        const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, t0 = seen.tile(v) * kRows + in_tile;
+#pragma unroll 1
+        for (uint32_t rb = 0; 16 * rb < w.R; rb++) {
+            const uint32_t r = min(16 * rb + w.col, w.R - 1);
+            const int32_t* q_row = query_of(p, w, r);
+            v4i_t acc[7];
+            int32_t k_dot[4] = {0, 0, 0, 0}, q_dot[4] = {0, 0, 0, 0};          // sums of the planes of this lane's parts
+#pragma unroll
+            for (int g = 0; g < 7; g++) acc[g] = v4i_t{0, 0, 0, 0};
+#pragma unroll 1
+            for (uint32_t s = 0; s < p.plan.dim64; s++) {
+                v4i_t kb[4], qb[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const uint32_t e = 64 * s + 16 * c + 4 * w.kg;
+                    uint32_t pl[4];
+                    four_planes(elements(k_row, e, dim, false, (int32_t)kNoElement), pl);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) kb[k][c] = (int)pl[k];
+                    four_planes(elements(q_row, e, dim, false, (int32_t)kNoElement), pl);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) qb[k][c] = (int)pl[k];
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        k_dot[k] = __builtin_amdgcn_sdot4(kb[k][c], 0x01010101, k_dot[k], false);
+                        q_dot[k] = __builtin_amdgcn_sdot4(qb[k][c], 0x01010101, q_dot[k], false);
+                    }
+#pragma unroll
+                    for (int a = 0; a < 4; a++) acc[a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[k], qb[a], acc[a + k], 0, 0, 0);
+                }
             }
-        }
-        uint32_t pl[4];
-        long long sum = 0;
+            int64_t k_sum = 0, q_sum = 0;
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++) sum += e + j < p.c.dim && r < w.R ? (long long)x[j] - kCacheOffset : 0;
-        transpose4((uint32_t)x[0] ^ kNoElement, (uint32_t)x[1] ^ kNoElement, (uint32_t)x[2] ^ kNoElement, (uint32_t)x[3] ^ kNoElement, pl);
-        uint32_t* o = digits + (((s * 4 * 4 + g) * kRows + r) << 2) + c;
+            for (int k = 3; k >= 0; k--) {
+                k_sum = k_sum * 256 + k_dot[k];
+                q_sum = q_sum * 256 + q_dot[k];
+            }
 #pragma unroll
-        for (uint32_t k = 0; k < 4; k++) o[k * 16 * kRows] = pl[k];
-        if (sums) {
-            // sixteen neighbouring lanes are of one row
+            for (int d = 16; d <= 32; d <<= 1) {
+                k_sum += __shfl_xor(k_sum, d, 64);
+                q_sum += __shfl_xor(q_sum, d, 64);
+            }
+            const uint32_t there = 16 * rb + w.col < w.R ? seen_of_four(p, w.pos_of(p, r), t0) : 0;
+            v4u_t q, rem;
 #pragma unroll
-            for (int k = 8; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, 64);
-            if ((i & 15u) == 0) atomicAdd(&q_sum[r], (unsigned long long)sum);
+            for (uint32_t i = 0; i < 4; i++) {
+                const int64_t k_of = __shfl(k_sum, (int)(4 * w.kg + i), 64);
+                uint64_t y = 0;
+#pragma unroll
+                for (int g = 6; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[g][i];
+                y += (uint64_t)kCacheOffset * (uint64_t)(k_of + q_sum + kCacheOffset * dim);
+                uint32_t wide = 0;
+                int32_t qi, ri;
+                p.qk.apply(off[tile * kRows + in_tile + i] < 0 ? 0 : (int64_t)y, qi, ri, wide);          // a page outside: zero
+                q[i] = qi;
+                rem[i] = ri;
+                if ((there >> i) & 1u) {
+                    bad |= wide;
+                    if (rb == 0) mx[0] = max(mx[0], qi);
+                    else if (rb == 1) mx[1] = max(mx[1], qi);
+                    else if (rb == 2) mx[2] = max(mx[2], qi);
+                    else mx[3] = max(mx[3], qi);
+                }
+            }
+            const size_t row = w.row(p, r);
+            store_four(p.scores.at(row, t0, v), q, there);
+            if (p.a.d_scores_rem) store_four(p.a.d_scores_rem + row * p.a.max_len + t0, rem, there);
         }
     }
 }
 
 // Scores of 64 rows with a chunk of the positions.  A wave takes 16 positions of each tile of 64 and all rows; it reads its keys from
-// memory into the operand (lane l the elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16), the queries' digits from LDS.
+// memory into the operand (lane l the elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16), the queries' digits from LDS.  The
+// instructions behind the products - 64 scores a lane for 128 elements' 288 matrix instructions a wave - are what it is short of:
+// five accumulators become a sum in double precision, exact below 2^53, and below 2^50 the quotient of (y + s/2 + 1/2) / s needs no
+// second look: it is no nearer than 1 / (2 s) to a whole number, and the product with 1 / s off by at most 2^-52 of itself.
 template <bool VEC>
-__global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p) {
+__global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
-    __shared__ unsigned long long q_sum[kRows];
     __shared__ int32_t top[4][kRows];
+    __shared__ uint32_t q_over;
     uint32_t bad = 0;
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         uint32_t n, pos;
@@ -150,127 +272,118 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
     const uint32_t v0 = blockIdx.y * p.plan.score_cols;
     if (v0 >= seen.tiles) return;
     const uint32_t tiles = min(p.plan.score_cols, seen.tiles - v0), steps = p.plan.dim64, dim = p.c.dim, blocks = (steps + kBlockSteps - 1) / kBlockSteps;
-    int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)min(steps, kBlockSteps) * 4 * 4 * kRows * 4);
-    if (threadIdx.x < kRows) q_sum[threadIdx.x] = 0;
+    int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)min(steps, kBlockSteps) * 3 * 4 * kRows * 4);
+    if (threadIdx.x == 0) q_over = 0;
     for (uint32_t i = threadIdx.x; i < tiles * kRows; i += 256) {
         const int64_t o = offset_of(p, w, seen, seen.tile(v0 + i / kRows) * kRows + i % kRows);
         if (o == -1) bad |= (uint32_t)kWitIndex;
         off[i] = o;
     }
     if (blockIdx.y == 0 && threadIdx.x < w.R) p.sums[w.row(p, threadIdx.x)] = 0;
+    uint32_t over = 0;
     __syncthreads();
     if (blocks == 1) {
-        stage_queries(p, w, 0, lds, q_sum, true);
+        stage_queries(p, w, 0, lds, over);
         __syncthreads();
     }
     const uint32_t row_blocks = (w.R + 15) / 16;
     const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
     v4i_t x[4];
     auto fetch = [&](uint32_t tile, uint32_t s) {
-        const int32_t* k = keys + max(off[tile * kRows + 16 * w.wave + w.col], (int64_t)0);
+        const int32_t* k = keys + max(off[tile * kRows + 16 * w.wave + w.col], (int64_t)0) + 64 * s + 4 * w.kg;
+        if (VEC && 64 * s + 64 <= dim) {
 #pragma unroll
-        for (uint32_t c = 0; c < 4; c++) {
-            const uint32_t e = 64 * s + 16 * c + 4 * w.kg;
-            v4i_t y = load4<VEC>(k, e, dim);
+            for (uint32_t c = 0; c < 4; c++) x[c] = *reinterpret_cast<const v4i_t*>(k + 16 * c);
+        } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) x[c][j] = e + j < dim ? y[j] : (int32_t)kNoElement;
+            for (uint32_t c = 0; c < 4; c++) {
+                const uint32_t e = 64 * s + 16 * c + 4 * w.kg;
+                x[c] = elements(k + 16 * c - e, e, dim, VEC, 0);
+            }
         }
     };
     fetch(0, 0);
     int32_t mx[4] = {INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN};
+    uint32_t pos[4];
+    size_t row[4];
+#pragma unroll
+    for (uint32_t rb = 0; rb < 4; rb++) {
+        const uint32_t r = min(16 * rb + w.col, w.R - 1);
+        pos[rb] = w.pos_of(p, r);
+        row[rb] = w.row(p, r);
+    }
+    const uint32_t first_pos = w.pos_of(p, 0), last_pos = w.pos_of(p, w.R - 1);
+    const double scale = (double)p.qk.s, inv = p.qk.inv, half = (double)(p.qk.s >> 1) + 0.5, limit = p.limit;
+    bool large = false;
+#pragma unroll 1
     for (uint32_t tile = 0; tile < tiles; tile++) {
-        v4i_t acc[4][7];
-        int32_t k_dot[4] = {0, 0, 0, 0};          // sums of the planes of this lane's part of its key
+        v4i_t acc[4][5];
+        uint32_t k_over = 0;
 #pragma unroll
         for (int rb = 0; rb < 4; rb++)
 #pragma unroll
-            for (int g = 0; g < 7; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
+            for (int g = 0; g < 5; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
+#pragma unroll 1
         for (uint32_t s = 0; s < steps; s++) {
             if (blocks > 1 && s % kBlockSteps == 0) {
                 __syncthreads();
-                stage_queries(p, w, s / kBlockSteps, lds, q_sum, tile == 0);
+                stage_queries(p, w, s / kBlockSteps, lds, over);
                 __syncthreads();
             }
-            v4i_t kb[4];
+            v4i_t kb[3];
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                uint32_t pl[4];
-                transpose4((uint32_t)x[c][0], (uint32_t)x[c][1], (uint32_t)x[c][2], (uint32_t)x[c][3], pl);
+                uint32_t pl[3];
+                three_planes(x[c], pl, k_over);
 #pragma unroll
-                for (int k = 0; k < 4; k++) kb[k][c] = (int)(k < 3 ? pl[k] ^ kByteTops : pl[k]);
+                for (int k = 0; k < 3; k++) kb[k][c] = (int)pl[k];
             }
             if (s + 1 < steps) fetch(tile, s + 1);
             else if (tile + 1 < tiles) fetch(tile + 1, 0);
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) k_dot[k] = __builtin_amdgcn_sdot4(kb[k][c], 0x01010101, k_dot[k], false);
-            const v4i_t* qa = reinterpret_cast<const v4i_t*>(lds) + ((s % kBlockSteps) * 16 + w.kg) * kRows + w.col;
+            const v4i_t* qa = reinterpret_cast<const v4i_t*>(lds) + ((s % kBlockSteps) * 12 + w.kg) * kRows + w.col;
 #pragma unroll
             for (uint32_t rb = 0; rb < 4; rb++) {
                 if (rb >= row_blocks) break;
 #pragma unroll
-                for (int a = 0; a < 4; a++) {
+                for (int a = 0; a < 3; a++) {
                     const v4i_t f = qa[a * 4 * kRows + 16 * rb];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[k], f, acc[rb][a + k], 0, 0, 0);
+                    for (int k = 0; k < 3; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[k], f, acc[rb][a + k], 0, 0, 0);
                 }
             }
         }
         // register i of lane l: position 4 (l / 16) + i of the wave's 16, row l % 16 of a block
-        int64_t k_sum = 0;
+        const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, k0 = seen.tile(v) * kRows, t0 = k0 + in_tile;
+        const bool all = k0 + kRows - 1 <= first_pos && (!p.a.window || k0 + p.a.window > last_pos || k0 + kRows <= p.a.sinks);
 #pragma unroll
-        for (int k = 3; k >= 0; k--) k_sum = k_sum * 256 + k_dot[k];
-        k_sum += __shfl_xor(k_sum, 16, 64);
-        k_sum += __shfl_xor(k_sum, 32, 64);
-        uint64_t more[4];
-        int64_t o[4];
-        const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, t0 = seen.tile(v) * kRows + in_tile;
-#pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
-            more[i] = (uint64_t)kCacheOffset * (uint64_t)(__shfl(k_sum, (int)(4 * w.kg + i), 64) + kCacheOffset * dim);
-            o[i] = off[tile * kRows + in_tile + i];
-        }
+        for (uint32_t i = 0; i < 4; i++) large |= off[tile * kRows + in_tile + i] == -1;          // wide_scores knows what to do with them
+        large |= (k_over & kOver) && off[tile * kRows + 16 * w.wave + w.col] >= 0;
 #pragma unroll
         for (uint32_t rb = 0; rb < 4; rb++) {
-            const uint32_t r = 16 * rb + w.col;
-            if (r >= w.R) continue;
-            const uint64_t q_more = (uint64_t)kCacheOffset * q_sum[r];
-            const uint32_t pos = w.pos_of(p, r);
-            const size_t row = w.row(p, r);
+            if (rb >= row_blocks) break;
             v4u_t q, rem;
-            uint32_t there = 0;
+            const uint32_t there = 16 * rb + w.col >= w.R ? 0 : all ? 15u : seen_of_four(p, pos[rb], t0);
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
-                uint64_t y = 0;
+                double y = (double)acc[rb][4][i];
 #pragma unroll
-                for (int g = 6; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[rb][g][i];
-                y += more[i] + q_more;
-                uint32_t wide = 0;
-                int32_t qi, ri;
-                p.qk.apply(o[i] < 0 ? 0 : (int64_t)y, qi, ri, wide);          // a page outside: zero
-                q[i] = qi;
-                rem[i] = ri;
-                if (step::sees(pos, t0 + i, p.a.window, p.a.sinks)) {
-                    there |= 1u << i;
-                    bad |= wide;
-                    mx[rb] = max(mx[rb], qi);
-                }
+                for (int g = 3; g >= 0; g--) y = __builtin_fma(y, 256.0, (double)acc[rb][g][i]);
+                const double t = y + half, quotient = __builtin_floor(t * inv);
+                large |= ((there >> i) & 1u) && __builtin_fabs(t) >= limit;
+                q[i] = (int32_t)quotient;
+                rem[i] = (int32_t)__builtin_fma(-quotient, scale, y);
+                mx[rb] = max(mx[rb], (there >> i) & 1u ? q[i] : INT32_MIN);
             }
-            int32_t* to = p.scores.at(row, t0, v);
-            int32_t* to_rem = p.a.d_scores_rem ? p.a.d_scores_rem + row * p.a.max_len + t0 : nullptr;
-            if (there == 15u) {
-                *reinterpret_cast<v4u_t*>(to) = q;
-                if (to_rem) *reinterpret_cast<v4u_t*>(to_rem) = rem;
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i++) {
-                    if (!((there >> i) & 1u)) continue;
-                    to[i] = q[i];
-                    if (to_rem) to_rem[i] = rem[i];
-                }
-            }
+            store_four(p.scores.at(row[rb], t0, v), q, there);
+            if (p.a.d_scores_rem) store_four(p.a.d_scores_rem + row[rb] * p.a.max_len + t0, rem, there);
         }
+    }
+    if (__any((over & kOver) != 0) && w.lane == 0) q_over = 1;          // the queries' digits were made by all threads
+    __syncthreads();
+    if (q_over || __any(large)) {
+#pragma unroll
+        for (int rb = 0; rb < 4; rb++) mx[rb] = INT32_MIN;
+        wide_scores(p, w, seen, v0, tiles, off, mx, bad);
     }
 #pragma unroll
     for (int rb = 0; rb < 4; rb++) {
@@ -582,6 +695,7 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     p.by_each = token::fast_div(pl.each);
     p.qk = scaler(a.qk_scale);
     p.out = scaler(a.out_scale);
+    p.limit = std::min(0x1p50, 2147483647.0 * (double)a.qk_scale);
     hipStream_t s = as_stream(st);
     const int rc = wit_status_word(&p.status);
     if (rc) return rc;
@@ -589,7 +703,7 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     const bool vec = p.c.dim % 4 == 0 && ((p.c.page_stride | p.c.token_stride | p.c.head_stride) & 3) == 0 && aligned(p.c.d_k);
     p.q_vec = p.c.dim % 4 == 0 && a.q_stride % 4 == 0 && aligned(a.d_q);
     const uint32_t along = pl.tiles * p.c.heads;
-    const size_t score_lds = (size_t)std::min(pl.dim64, kBlockSteps) * 16 * kRows * 16 + (size_t)pl.score_cols * kRows * 8;
+    const size_t score_lds = (size_t)std::min(pl.dim64, kBlockSteps) * 12 * kRows * 16 + (size_t)pl.score_cols * kRows * 8;
     if (vec) wit_window_scores_kernel<true><<<dim3(along, pl.score_chunks), 256, score_lds, s>>>(p);
     else wit_window_scores_kernel<false><<<dim3(along, pl.score_chunks), 256, score_lds, s>>>(p);
     GRAPE_LAUNCH_CHECK();
