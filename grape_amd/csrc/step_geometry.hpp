@@ -147,8 +147,10 @@ struct WindowPlan {
     uint32_t score_cols, score_chunks;         // of a workgroup of the scores, and workgroups along the positions
     uint32_t exp_cols, exp_chunks;
     uint32_t value_cols, value_chunks, groups;          // and workgroups along a head's elements
-    size_t at_scores, at_exp, at_max, at_sum, at_part, bytes;
+    bool factors;                              // the exponential table's entries are computed, see wit_window_table_kernel
+    size_t at_scores, at_exp, at_max, at_sum, at_factors, at_part, bytes;
 };
+constexpr size_t kFactorBytes = 2 * 1024 * 8 + 64 * 4;
 constexpr uint32_t kValueDims = 128;
 constexpr uint32_t kOffsetTiles = 16;          // tiles of positions whose offsets a values workgroup holds
 
@@ -174,7 +176,8 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     };
     p.score_cols = chunk(2048, 8, 1);
     p.score_chunks = token::ceil_div(p.cols, p.score_cols);
-    p.exp_cols = 4;
+    p.exp_cols = 8;
+    p.factors = rows_all * cols >= (uint64_t)1 << 16;
     p.exp_chunks = token::ceil_div(p.cols, p.exp_cols);
     p.groups = token::ceil_div(dim, kValueDims);
     const uint64_t want = beside * p.groups >= 512 ? 1 : 1024 / (beside * p.groups);
@@ -187,7 +190,8 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     p.at_exp = up(row);
     p.at_max = p.at_exp + up(row);
     p.at_sum = p.at_max + up((size_t)rows_all * p.score_chunks * 4);
-    p.at_part = p.at_sum + up((size_t)rows_all * 8);
+    p.at_factors = p.at_sum + up((size_t)rows_all * 8);
+    p.at_part = p.at_factors + (p.factors ? up(kFactorBytes) : 0);
     p.bytes = p.at_part + (p.value_chunks > 1 ? (size_t)rows_all * p.value_chunks * dim * 8 : 0);
     return true;
 }

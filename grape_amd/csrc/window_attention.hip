@@ -401,9 +401,41 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
     if (bad) atomicOr(p.status, bad);
 }
 
-// Exponentials of 64 rows and a chunk of the positions, and the rows' sums, to which the chunks add.
+// A table of exponentials need not be looked into where it is one: entry 2^bit_shift - 1 - d is then round(S exp(-d / S)) with S the
+// entry of d = 0.  Written as d = 1024 a + b that is the product of two factors of a thousand each, 16 KB in all, which LDS holds.  This
+// launch makes the factors and compares every entry that a score can meet; where one differs, the entries are read.
+constexpr uint32_t kFactors = 1024, kTableGroups = 64;
+__global__ void __launch_bounds__(kBlock) wit_window_table_kernel(WindowArgs p) {
+    __shared__ double factors[2 * kFactors];
+    __shared__ uint32_t differs;
+    const int64_t last = ((int64_t)1 << p.a.bit_shift) - 1;
+    const int32_t top = p.a.d_exp_table[last];
+    const double scale = (double)max(top, 1);
+    if (threadIdx.x == 0) differs = top < 1;
+    for (uint32_t i = threadIdx.x; i < kFactors; i += kBlock) {
+        factors[i] = scale * exp(-(double)(i * kFactors) / scale);
+        factors[kFactors + i] = exp(-(double)i / scale);
+    }
+    __syncthreads();
+    const uint32_t each = (uint32_t)(last / kTableGroups + 1), from = blockIdx.x * each;
+    bool other = false;
+    for (uint32_t i = threadIdx.x; i < each && from + i <= last; i += kBlock) {
+        const uint32_t d = from + i;
+        other |= p.a.d_exp_table[last - d] != (int32_t)__builtin_rint(factors[d / kFactors] * factors[kFactors + d % kFactors]);
+    }
+    if (other) differs = 1;
+    __syncthreads();
+    if (threadIdx.x == 0) p.differs[blockIdx.x] = differs;
+    if (blockIdx.x == 0)
+        for (uint32_t i = threadIdx.x; i < 2 * kFactors; i += kBlock) p.factors[i] = factors[i];
+}
+
+// Exponentials of 64 rows and a chunk of the positions, and the rows' sums, to which the chunks add.  The table's entries are 4 MB,
+// of which a wave asks for 64 lines at a time: reading them is bound by L2.
+template <bool FACTORS>
 __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
     __shared__ int32_t top[kRows];
+    __shared__ double factors[FACTORS ? 2 * kFactors : 1];
     RowTile w;
     if (!w.find(p, blockIdx.x)) return;
     const step::Seen seen = w.seen(p);
@@ -411,6 +443,12 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
     if (v0 >= seen.tiles) return;
     const uint32_t tiles = min(p.plan.exp_cols, seen.tiles - v0), parts = (seen.tiles - 1) / p.plan.score_cols + 1;
     if (threadIdx.x < kRows) top[threadIdx.x] = INT32_MIN;
+    bool computed = false;
+    if constexpr (FACTORS) {
+        computed = !__any(p.differs[w.lane] != 0);
+        if (computed)
+            for (uint32_t i = threadIdx.x; i < 2 * kFactors; i += 256) factors[i] = p.factors[i];
+    }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < parts * kRows; i += 256) {
         const uint32_t r = i % kRows;
@@ -419,18 +457,18 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
     __syncthreads();
     if (blockIdx.y == 0 && p.a.d_max && threadIdx.x < w.R) p.a.d_max[w.row(p, threadIdx.x)] = top[threadIdx.x];
     uint32_t bad = 0;
+    const uint32_t last = ((uint32_t)1 << p.a.bit_shift) - 1, first_pos = w.pos_of(p, 0), last_pos = w.pos_of(p, w.R - 1);
     for (uint32_t r = w.wave; r < w.R; r += 4) {
         const uint32_t pos = w.pos_of(p, r);
         const size_t row = w.row(p, r);
         const int32_t mx = top[r];
         unsigned long long sum = 0;
         for (uint32_t i = 4 * w.lane; i < tiles * kRows; i += 256) {
-            const uint32_t v = v0 + i / kRows, t = seen.tile(v) * kRows + i % kRows;
-            const int32_t* from = p.scores.at(row, t, v);
-            uint32_t there = 0;
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) there |= step::sees(pos, t + j, p.a.window, p.a.sinks) ? 1u << j : 0u;
+            const uint32_t v = v0 + i / kRows, k0 = seen.tile(v) * kRows, t = k0 + i % kRows;
+            const bool all = k0 + kRows - 1 <= first_pos && (!p.a.window || k0 + p.a.window > last_pos || k0 + kRows <= p.a.sinks);
+            const uint32_t there = all ? 15u : seen_of_four(p, pos, t);
             if (!there) continue;
+            const int32_t* from = p.scores.at(row, t, v);
             v4u_t x = {mx, mx, mx, mx}, e, shifted;
             if (there == 15u) {
                 x = *reinterpret_cast<const v4u_t*>(from);
@@ -439,31 +477,31 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
                 for (uint32_t j = 0; j < 4; j++)
                     if ((there >> j) & 1u) x[j] = from[j];
             }
+            if (computed) {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const int64_t idx = (int64_t)x[j] - mx + (((int64_t)1 << p.a.bit_shift) - 1);
-                const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
-                e[j] = p.a.d_exp_table[ok ? idx : 0];
-                shifted[j] = (int32_t)((int64_t)x[j] - mx);
-                if ((there >> j) & 1u) {
-                    if (!ok) bad |= (uint32_t)kWitIndex;
-                    if (e[j] < 0) bad |= (uint32_t)kWitSum;
-                    sum += (unsigned long long)max(e[j], 0);
+                for (uint32_t j = 0; j < 4; j++) {
+                    const uint32_t below = (uint32_t)mx - (uint32_t)x[j], d = min(below, last);          // entry 0 stands in for those before it
+                    shifted[j] = (int32_t)(0 - below);
+                    e[j] = (int32_t)__builtin_rint(factors[d / kFactors] * factors[kFactors + d % kFactors]);
+                    sum += (uint32_t)((there >> j) & 1u ? e[j] : 0);
+                    if (below > last) bad |= (uint32_t)kWitIndex;          // only positions that are there have a score below the maximum
                 }
-            }
-            int32_t* to = p.exps.at(row, t, v);
-            int32_t* to_shifted = p.a.d_shifted ? p.a.d_shifted + row * p.a.max_len + t : nullptr;
-            if (there == 15u) {
-                *reinterpret_cast<v4u_t*>(to) = e;
-                if (to_shifted) *reinterpret_cast<v4u_t*>(to_shifted) = shifted;
             } else {
 #pragma unroll
                 for (uint32_t j = 0; j < 4; j++) {
-                    if (!((there >> j) & 1u)) continue;
-                    to[j] = e[j];
-                    if (to_shifted) to_shifted[j] = shifted[j];
+                    const int64_t idx = (int64_t)x[j] - mx + last;
+                    const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
+                    e[j] = p.a.d_exp_table[ok ? idx : 0];
+                    shifted[j] = (int32_t)((int64_t)x[j] - mx);
+                    if ((there >> j) & 1u) {
+                        if (!ok) bad |= (uint32_t)kWitIndex;
+                        if (e[j] < 0) bad |= (uint32_t)kWitSum;
+                        sum += (unsigned long long)max(e[j], 0);
+                    }
                 }
             }
+            store_four(p.exps.at(row, t, v), e, there);
+            if (p.a.d_shifted) store_four(p.a.d_shifted + row * p.a.max_len + t, shifted, there);
         }
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
@@ -474,13 +512,64 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
 
 // Probabilities of 64 rows and their products with 128 elements of the values, over a chunk of the positions.  Eight threads a row make
 // the digits of 64 positions in LDS while the waves multiply the 64 before them; a wave takes 16 elements and all rows, and turns
-// its values into operands in registers.
+// its values into operands in registers.  A probability is floor((e P + floor(S/2)) / S) from one product in double precision, as the
+// scores' quotients are, where S is below 2^28 and P at most 2^22; the remainder of the division gives the lookup's query.
 constexpr uint32_t kValueThreads = 512;
+constexpr uint64_t kPlainSum = (uint64_t)1 << 28;
+template <int PP, bool WIDE>
+struct Values {
+    static constexpr int VP = WIDE ? 4 : 3, G = PP + VP - 1;
+    v4i_t acc[4][G];
+    int32_t x[16];
+    uint32_t over = 0;
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int rb = 0; rb < 4; rb++)
+#pragma unroll
+            for (int g = 0; g < G; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ void fetch(const int32_t* values, const int64_t* off) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16; j++) x[j] = values[max(off[j], (int64_t)0)];
+    }
+    // the planes of the probabilities' digits below `planes`, from LDS
+    __device__ __forceinline__ void multiply(const v4i_t* digits, uint32_t row_blocks, int planes) {
+        v4i_t vb[VP];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const v4i_t y = {x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
+            uint32_t pl[4];
+            if constexpr (WIDE) four_planes(y, pl);
+            else three_planes(y, pl, over);
+#pragma unroll
+            for (int k = 0; k < VP; k++) vb[k][c] = (int)pl[k];
+        }
+#pragma unroll
+        for (uint32_t rb = 0; rb < 4; rb++) {
+            if (rb >= row_blocks) break;
+#pragma unroll
+            for (int a = 0; a < PP; a++) {
+                if (a >= planes) break;
+                const v4i_t f = digits[a * 4 * kRows + 16 * rb];
+#pragma unroll
+                for (int k = 0; k < VP; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[k], f, acc[rb][a + k], 0, 0, 0);
+            }
+        }
+    }
+    __device__ __forceinline__ uint64_t sum(uint32_t rb, uint32_t i) const {
+        uint64_t y = 0;
+#pragma unroll
+        for (int g = G - 1; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[rb][g][i];
+        return y;
+    }
+};
+
 template <int PP>
 __global__ void __launch_bounds__(kValueThreads, 2) wit_window_values_kernel(WindowArgs p) {
     __shared__ __attribute__((aligned(16))) uint32_t digits[2][PP * 4 * kRows * 4];
     __shared__ int64_t off[step::kOffsetTiles * kRows];
     __shared__ unsigned long long p_sum[kRows];
+    __shared__ uint32_t third[2], wide_any;          // the last tile with digits in the third plane (and 1), for odd and even ones
     RowTile w;
     if (!w.find(p, blockIdx.x)) return;
     const step::Seen seen = w.seen(p);
@@ -488,10 +577,11 @@ __global__ void __launch_bounds__(kValueThreads, 2) wit_window_values_kernel(Win
     if (v0 >= seen.tiles) return;
     const uint32_t tiles = min(p.plan.value_cols, seen.tiles - v0);
     uint32_t bad = 0;
+    if (threadIdx.x == 0) third[0] = third[1] = wide_any = 0;
     // of the probabilities: this thread's row and its eight positions of a tile
     const uint32_t r = threadIdx.x >> 3, part = threadIdx.x & 7u;
     const bool mine = r < w.R, write = group == 0;
-    const uint32_t rr = mine ? r : 0, pos = w.pos_of(p, rr);
+    const uint32_t rr = mine ? r : 0, pos = w.pos_of(p, rr), first_pos = w.pos_of(p, 0), last_pos = w.pos_of(p, w.R - 1);
     const size_t row = w.row(p, rr);
     unsigned long long sum = p.sums[row], all = 0;
     if (sum == 0) {
@@ -499,14 +589,20 @@ __global__ void __launch_bounds__(kValueThreads, 2) wit_window_values_kernel(Win
         sum = 1;
     }
     if (mine && write && chunk == 0 && part == 0 && p.a.d_sum) store_sum(&p.a.d_sum[row], sum, bad);
-    const double inv = 1.0 / (double)sum;
+    const double inv = 1.0 / (double)sum, scale = (double)p.a.prob_scale, half = (double)(sum >> 1) + 0.5, whole_sum = (double)sum, odd = (double)(sum & 1) - 1.0;
+    const bool plain = PP == 3 && __all(sum < kPlainSum);
     int32_t e[8];
+    auto seen_of_eight = [&](uint32_t tile, uint32_t& t) {
+        const uint32_t k0 = seen.tile(v0 + tile) * kRows;
+        t = k0 + 8 * part;
+        if (!mine) return 0u;
+        if (k0 + kRows - 1 <= first_pos && (!p.a.window || k0 + p.a.window > last_pos || k0 + kRows <= p.a.sinks)) return 255u;
+        return seen_of_four(p, pos, t) | seen_of_four(p, pos, t + 4) << 4;
+    };
     auto fetch_exps = [&](uint32_t tile) {
-        const uint32_t v = v0 + tile, t = seen.tile(v) * kRows + 8 * part;
-        const int32_t* from = p.exps.at(row, t, v);
-        uint32_t there = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < 8; j++) there |= mine && step::sees(pos, t + j, p.a.window, p.a.sinks) ? 1u << j : 0u;
+        uint32_t t;
+        const uint32_t there = seen_of_eight(tile, t);
+        const int32_t* from = p.exps.at(row, t, v0 + tile);
         if (there == 255u) {
             *reinterpret_cast<v4u_t*>(e) = *reinterpret_cast<const v4u_t*>(from);
             *reinterpret_cast<v4u_t*>(e + 4) = *reinterpret_cast<const v4u_t*>(from + 4);
@@ -515,130 +611,127 @@ __global__ void __launch_bounds__(kValueThreads, 2) wit_window_values_kernel(Win
             for (uint32_t j = 0; j < 8; j++) e[j] = (there >> j) & 1u ? from[j] : 0;
         }
     };
-    auto make_digits = [&](uint32_t tile) {
-        const uint32_t v = v0 + tile, t = seen.tile(v) * kRows + 8 * part;
-        uint32_t there = 0, d[8];
-        int32_t pr[8], query[8];
+    auto make_digits = [&](uint32_t tile, bool writes) {
+        uint32_t t;
+        const uint32_t there = seen_of_eight(tile, t);
+        v4u_t pr[2], query[2];
+        if (plain) {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) {
+                const double num = __builtin_fma((double)max(e[j], 0), scale, half), q = __builtin_floor(num * inv);
+                pr[j / 4][j % 4] = (int32_t)q;
+                query[j / 4][j % 4] = (int32_t)__builtin_fma(2.0, __builtin_fma(-q, whole_sum, num), odd);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) {
+                const uint32_t x = (uint32_t)max(e[j], 0), pj = probability(x, (uint64_t)p.a.prob_scale, sum, inv);
+                uint32_t wide = 0;
+                int32_t qj;
+                store_sum(&qj, lookup_query(x, p.a.prob_scale, sum, pj), wide);
+                pr[j / 4][j % 4] = (int32_t)pj;
+                query[j / 4][j % 4] = qj;
+                if (((there >> j) & 1u) && write && p.a.d_query) bad |= wide;
+            }
+        }
+        if (writes) {
+            const size_t o = row * p.a.max_len + t;
+            if (p.a.d_prob) {
+                store_four(p.a.d_prob + o, pr[0], there & 15u);
+                store_four(p.a.d_prob + o + 4, pr[1], there >> 4);
+            }
+            if (p.a.d_query) {
+                store_four(p.a.d_query + o, query[0], there & 15u);
+                store_four(p.a.d_query + o + 4, query[1], there >> 4);
+            }
+        }
+        v4i_t d[2];
+        uint32_t large = 0;
 #pragma unroll
         for (uint32_t j = 0; j < 8; j++) {
-            there |= mine && step::sees(pos, t + j, p.a.window, p.a.sinks) ? 1u << j : 0u;
-            const uint32_t x = (uint32_t)max(e[j], 0);
-            uint32_t pj = probability(x, (uint64_t)p.a.prob_scale, sum, inv);
-            const bool seen_j = (there >> j) & 1u;
-            uint32_t wide = 0;
-            store_sum(&query[j], lookup_query(x, p.a.prob_scale, sum, pj), wide);
-            if (seen_j && write && p.a.d_query) bad |= wide;
-            pr[j] = (int32_t)pj;
-            if (!seen_j || off[(tile % step::kOffsetTiles) * kRows + 8 * part + j] < 0) pj = 0;
-            all += pj;
-            d[j] = digits_of((int32_t)pj);
+            const bool used = ((there >> j) & 1u) && off[(tile % step::kOffsetTiles) * kRows + 8 * part + j] >= 0;          // a page outside: no value
+            d[j / 4][j % 4] = used ? pr[j / 4][j % 4] : 0;
+            large |= (uint32_t)d[j / 4][j % 4] + 0x8080u;
         }
-        if (write) {
-            const size_t o = row * p.a.max_len + t;
-            if (there == 255u) {
-                if (p.a.d_prob) {
-                    *reinterpret_cast<v4u_t*>(p.a.d_prob + o) = *reinterpret_cast<v4u_t*>(pr);
-                    *reinterpret_cast<v4u_t*>(p.a.d_prob + o + 4) = *reinterpret_cast<v4u_t*>(pr + 4);
-                }
-                if (p.a.d_query) {
-                    *reinterpret_cast<v4u_t*>(p.a.d_query + o) = *reinterpret_cast<v4u_t*>(query);
-                    *reinterpret_cast<v4u_t*>(p.a.d_query + o + 4) = *reinterpret_cast<v4u_t*>(query + 4);
-                }
-            } else {
+        uint32_t pl[2][4];
+        if constexpr (PP == 3) {
+            uint32_t none = 0;
+            three_planes(d[0], pl[0], none);
+            three_planes(d[1], pl[1], none);
+        } else {
 #pragma unroll
-                for (uint32_t j = 0; j < 8; j++) {
-                    if (!((there >> j) & 1u)) continue;
-                    if (p.a.d_prob) p.a.d_prob[o + j] = pr[j];
-                    if (p.a.d_query) p.a.d_query[o + j] = query[j];
-                }
-            }
+            for (uint32_t h = 0; h < 2; h++) transpose4(digits_of(d[h][0]), digits_of(d[h][1]), digits_of(d[h][2]), digits_of(d[h][3]), pl[h]);
         }
-        uint32_t p0[4], p1[4];
-        transpose4(d[0], d[1], d[2], d[3], p0);
-        transpose4(d[4], d[5], d[6], d[7], p1);
+        if (__any(large >> 16) && w.lane == 0) third[tile & 1] = tile + 1;
         uint64_t* to = reinterpret_cast<uint64_t*>(digits[tile & 1]) + ((part >> 1) * kRows + r) * 2 + (part & 1u);
 #pragma unroll
-        for (int k = 0; k < PP; k++) to[k * 4 * kRows * 2] = ((uint64_t)p1[k] << 32) | p0[k];
+        for (int k = 0; k < PP; k++) to[k * 4 * kRows * 2] = ((uint64_t)pl[1][k] << 32) | pl[0][k];
+        return d[0][0] + (uint64_t)d[0][1] + d[0][2] + d[0][3] + d[1][0] + d[1][1] + d[1][2] + d[1][3];
     };
-    auto make_offsets = [&](uint32_t tile) {
-        const uint32_t n = min(step::kOffsetTiles, tiles - tile) * kRows;
-        for (uint32_t i = threadIdx.x; i < n; i += kValueThreads) off[i] = offset_of(p, w, seen, seen.tile(v0 + tile + i / kRows) * kRows + i % kRows);
-    };
-    const uint32_t e0 = group * step::kValueDims + 16 * w.wave, el = min(e0 + w.col, dim - 1), row_blocks = (w.R + 15) / 16;
-    const int32_t* values = p.c.d_v + (int64_t)w.kv * p.c.head_stride + el;
+    const uint32_t e0 = group * step::kValueDims + 16 * w.wave, row_blocks = (w.R + 15) / 16;
+    const int32_t* values = p.c.d_v + (int64_t)w.kv * p.c.head_stride + min(e0 + w.col, dim - 1);
     const bool multiplies = e0 < dim;
-    int32_t x[16];
-    auto fetch_values = [&](uint32_t tile) {
-#pragma unroll
-        for (uint32_t j = 0; j < 16; j++) x[j] = values[max(off[(tile % step::kOffsetTiles) * kRows + 16 * w.kg + j], (int64_t)0)];
-    };
-    constexpr int G = PP + 3;
-    v4i_t acc[4][G];
-#pragma unroll
-    for (int rb = 0; rb < 4; rb++)
-#pragma unroll
-        for (int g = 0; g < G; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
-    fetch_exps(0);
-    for (uint32_t tile = 0; tile < tiles; tile++) {
-        if (tile % step::kOffsetTiles == 0) {
-            __syncthreads();          // nobody reads the offsets before any more
-            make_offsets(tile);
-            __syncthreads();
-        }
-        if (multiplies) fetch_values(tile);
-        make_digits(tile);
-        if (tile + 1 < tiles) fetch_exps(tile + 1);
-        __syncthreads();
-        if (!multiplies) continue;
-        v4i_t vb[4];
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            uint32_t pl[4];
-            transpose4((uint32_t)x[4 * c], (uint32_t)x[4 * c + 1], (uint32_t)x[4 * c + 2], (uint32_t)x[4 * c + 3], pl);
-#pragma unroll
-            for (int k = 0; k < 4; k++) vb[k][c] = (int)(k < 3 ? pl[k] ^ kByteTops : pl[k]);
-        }
-        const v4i_t* pa = reinterpret_cast<const v4i_t*>(digits[tile & 1]) + w.kg * kRows + w.col;
-#pragma unroll
-        for (uint32_t rb = 0; rb < 4; rb++) {
-            if (rb >= row_blocks) break;
-#pragma unroll
-            for (int a = 0; a < PP; a++) {
-                const v4i_t f = pa[a * 4 * kRows + 16 * rb];
-#pragma unroll
-                for (int k = 0; k < 4; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[k], f, acc[rb][a + k], 0, 0, 0);
+    auto run = [&](auto& products, bool writes) {
+        products.clear();
+        fetch_exps(0);
+#pragma unroll 1
+        for (uint32_t tile = 0; tile < tiles; tile++) {
+            if (tile % step::kOffsetTiles == 0) {
+                __syncthreads();          // nobody reads the offsets before any more
+                const uint32_t n = min(step::kOffsetTiles, tiles - tile) * kRows;
+                for (uint32_t i = threadIdx.x; i < n; i += kValueThreads) off[i] = offset_of(p, w, seen, seen.tile(v0 + tile + i / kRows) * kRows + i % kRows);
+                __syncthreads();
             }
+            const int64_t* o = off + (tile % step::kOffsetTiles) * kRows + 16 * w.kg;
+            if (multiplies) products.fetch(values, o);
+            all += make_digits(tile, writes);
+            if (tile + 1 < tiles) fetch_exps(tile + 1);
+            __syncthreads();
+            if (multiplies) products.multiply(reinterpret_cast<const v4i_t*>(digits[tile & 1]) + w.kg * kRows + w.col, row_blocks, PP == 3 && third[tile & 1] != tile + 1 ? 2 : PP);
         }
-    }
-    all += __shfl_xor(all, 1, 64);
-    all += __shfl_xor(all, 2, 64);
-    all += __shfl_xor(all, 4, 64);
-    if (part == 0) p_sum[r] = all;
-    __syncthreads();
+    };
     const bool whole = seen.tiles <= p.plan.value_cols;          // all positions of the rows are this workgroup's
     const uint32_t e1 = e0 + 4 * w.kg;
+    auto put = [&](auto& products, bool offset) {
 #pragma unroll
-    for (uint32_t rb = 0; rb < 4; rb++) {
-        const uint32_t q_row = 16 * rb + w.col;
-        if (q_row >= w.R || e1 >= dim) continue;
-        const uint64_t more = (uint64_t)kCacheOffset * p_sum[q_row];
-        const size_t to = w.row(p, q_row);
+        for (uint32_t rb = 0; rb < 4; rb++) {
+            const uint32_t q_row = 16 * rb + w.col;
+            if (q_row >= w.R || e1 >= dim) continue;
+            const size_t to = w.row(p, q_row);
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
-            if (e1 + i >= dim) break;
-            uint64_t y = 0;
-#pragma unroll
-            for (int g = G - 1; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[rb][g][i];
-            y += more;
-            if (whole) {
-                int32_t q, rem;
-                p.out.apply((int64_t)y, q, rem, bad);
-                p.a.d_out[to * dim + e1 + i] = q;
-                if (p.a.d_out_rem) p.a.d_out_rem[to * dim + e1 + i] = rem;
-            } else {
-                p.part[(to * p.plan.value_chunks + chunk) * dim + e1 + i] = (int64_t)y;
+            for (uint32_t i = 0; i < 4; i++) {
+                if (e1 + i >= dim) break;
+                const uint64_t y = products.sum(rb, i) + (offset ? (uint64_t)kCacheOffset * p_sum[q_row] : 0);
+                if (whole) {
+                    int32_t q, rem;
+                    p.out.apply((int64_t)y, q, rem, bad);
+                    p.a.d_out[to * dim + e1 + i] = q;
+                    if (p.a.d_out_rem) p.a.d_out_rem[to * dim + e1 + i] = rem;
+                } else {
+                    p.part[(to * p.plan.value_chunks + chunk) * dim + e1 + i] = (int64_t)y;
+                }
             }
         }
+    };
+    bool wide;
+    {
+        Values<PP, false> products;
+        run(products, write);
+        if (__any((products.over & kOver) != 0) && w.lane == 0) wide_any = 1;
+        __syncthreads();
+        wide = wide_any != 0;
+        if (!wide) put(products, false);
+    }
+    if (wide) {
+        all = 0;
+        Values<PP, true> products;
+        run(products, false);
+        all += __shfl_xor(all, 1, 64);
+        all += __shfl_xor(all, 2, 64);
+        all += __shfl_xor(all, 4, 64);
+        if (part == 0) p_sum[r] = all;
+        __syncthreads();
+        put(products, true);
     }
     if (bad) atomicOr(p.status, bad);
 }
@@ -707,7 +800,15 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     if (vec) wit_window_scores_kernel<true><<<dim3(along, pl.score_chunks), 256, score_lds, s>>>(p);
     else wit_window_scores_kernel<false><<<dim3(along, pl.score_chunks), 256, score_lds, s>>>(p);
     GRAPE_LAUNCH_CHECK();
-    wit_window_exp_kernel<<<dim3(along, pl.exp_chunks), 256, 0, s>>>(p);
+    if (pl.factors && a.bit_shift <= 20 && a.index_bits >= a.bit_shift) {
+        p.factors = (double*)(ws + pl.at_factors);
+        p.differs = (uint32_t*)(p.factors + 2 * kFactors);
+        wit_window_table_kernel<<<kTableGroups, kBlock, 0, s>>>(p);
+        GRAPE_LAUNCH_CHECK();
+        wit_window_exp_kernel<true><<<dim3(along, pl.exp_chunks), 256, 0, s>>>(p);
+    } else {
+        wit_window_exp_kernel<false><<<dim3(along, pl.exp_chunks), 256, 0, s>>>(p);
+    }
     GRAPE_LAUNCH_CHECK();
     const dim3 values(along, pl.value_chunks * pl.groups);
     if (a.prob_scale <= ((int64_t)1 << 22)) wit_window_values_kernel<3><<<values, kValueThreads, 0, s>>>(p);
