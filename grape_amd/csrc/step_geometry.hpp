@@ -136,9 +136,9 @@ inline const char* refuse_next(const grape_wit_next_token_args* a) {
 
 // ---- attention of several tokens a sequence
 // A workgroup takes kRows rows of one cache head - the query heads of a token that read it side by side, token after token - and
-// positions in tiles of kRows.  Sequence b's tiles of rows are numbered from starts[b] * each / kRows + b on, which leaves none to two
+// positions in tiles of kCols.  Sequence b's tiles of rows are numbered from starts[b] * each / kRows + b on, which leaves none to two
 // sequences whatever the lengths are: no workgroup has to know more than its own sequence.
-constexpr uint32_t kRows = 64;
+constexpr uint32_t kRows = 32, kCols = 64;
 
 struct WindowPlan {
     uint32_t each, dim64;
@@ -147,7 +147,7 @@ struct WindowPlan {
     uint32_t score_cols, score_chunks;         // of a workgroup of the scores, and workgroups along the positions
     uint32_t exp_cols, exp_chunks;
     uint32_t value_cols, value_chunks, groups;          // and workgroups along a head's elements
-    bool factors;                              // the exponential table's entries are computed, see wit_window_table_kernel
+    bool factors;                              // the exponential table's entries are computed, see make_factors
     size_t at_scores, at_exp, at_max, at_sum, at_factors, at_part, bytes;
 };
 constexpr size_t kFactorBytes = 2 * 1024 * 8 + 64 * 4;
@@ -162,30 +162,30 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     p.dim64 = token::ceil_div(dim, 64);
     const uint64_t rows_all = (uint64_t)rows * heads, tiles = (uint64_t)rows * p.each / kRows + seqs;
     if ((unsigned __int128)rows_all * max_len >= (uint64_t)1 << 38) return false;
-    uint64_t cols = token::ceil_div(max_len, kRows);
-    if (window) cols = std::min<uint64_t>(cols, ((uint64_t)window + 2 * kRows - 1) / kRows + 1 + ((uint64_t)sinks + kRows - 1) / kRows);
+    uint64_t cols = token::ceil_div(max_len, kCols);
+    if (window) cols = std::min<uint64_t>(cols, ((uint64_t)window + kRows + kCols - 1) / kCols + 1 + ((uint64_t)sinks + kCols - 1) / kCols);
     p.tiles = (uint32_t)tiles;
     p.cols = (uint32_t)cols;
     // a launch's first axis in workgroups, the others' limits
     if (tiles * cache_heads >= (uint64_t)1 << 22) return false;
-    const uint64_t beside = std::max<uint64_t>(1, std::min<uint64_t>((uint64_t)rows * p.each / kRows + 1, tiles) * cache_heads);
-    auto chunk = [&](uint64_t workgroups, uint32_t most, uint32_t least) {
+    // tiles of rows that are surely there, and as many workgroups as fill the chip
+    const uint64_t beside = std::max<uint64_t>((uint64_t)rows * p.each / kRows, std::min(seqs, rows)) * cache_heads;
+    auto chunk = [&](uint64_t workgroups, uint64_t most) {
         const uint64_t want = beside >= workgroups ? 1 : workgroups / beside;
-        const uint64_t c = (cols + want - 1) / want;
-        return (uint32_t)std::max<uint64_t>(least, std::min<uint64_t>(most, c));
+        return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, (cols + want - 1) / want));
     };
-    p.score_cols = chunk(2048, 8, 1);
+    p.score_cols = chunk(4096, 8);
     p.score_chunks = token::ceil_div(p.cols, p.score_cols);
     p.exp_cols = 8;
     p.factors = rows_all * cols >= (uint64_t)1 << 16;
     p.exp_chunks = token::ceil_div(p.cols, p.exp_cols);
     p.groups = token::ceil_div(dim, kValueDims);
-    const uint64_t want = beside * p.groups >= 512 ? 1 : 1024 / (beside * p.groups);
+    const uint64_t want = beside * p.groups >= 512 ? 1 : 512 / (beside * p.groups);
     p.value_cols = (uint32_t)((cols + want - 1) / want);
     p.value_chunks = token::ceil_div(p.cols, p.value_cols);
     if (p.score_chunks > 65535 || p.exp_chunks > 65535 || (uint64_t)p.value_chunks * p.groups > 65535) return false;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-    const size_t row = (size_t)rows_all * p.cols * kRows * 4;
+    const size_t row = (size_t)rows_all * p.cols * kCols * 4;
     p.at_scores = 0;
     p.at_exp = up(row);
     p.at_max = p.at_exp + up(row);
@@ -218,10 +218,10 @@ struct Seen {
         hi = pos1 + 1;
         lo = window && pos0 + 1 > window ? pos0 + 1 - window : 0;
         sinks = sinks_ < lo ? sinks_ : lo;
-        from = lo / kRows;
-        sink_tiles = (sinks + kRows - 1) / kRows;
+        from = lo / kCols;
+        sink_tiles = (sinks + kCols - 1) / kCols;
         if (sink_tiles > from) sink_tiles = from;
-        tiles = sink_tiles + (hi + kRows - 1) / kRows - from;
+        tiles = sink_tiles + (hi + kCols - 1) / kCols - from;
     }
     GRAPE_HD uint32_t tile(uint32_t v) const { return v < sink_tiles ? v : v - sink_tiles + from; }
     GRAPE_HD bool any(uint32_t t) const { return t < hi && (t >= lo || t < sinks); }

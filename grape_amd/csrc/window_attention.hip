@@ -7,8 +7,8 @@
 namespace grape {
 
 // ------------------------------------------------------------------------------------------------
-// Scores, softmax through the table, products with the values, for tiles of 64 rows: the query heads that read one cache head, token
-// after token, so that a key or a value that is read serves 64 rows.  The softmax is the table's, rounded: the row's maximum is
+// Scores, softmax through the table, products with the values, for tiles of 32 rows: the query heads that read one cache head, token
+// after token, so that a key or a value that is read serves 32 rows.  The softmax is the table's, rounded: the row's maximum is
 // needed before the first exponential and the sum of all before the first probability, hence a launch for each of the three, and
 // a fourth that joins the values' partial sums where the positions are cut up.
 //
@@ -18,6 +18,7 @@ namespace grape {
 // element turns up, the wave (or, for the values, the workgroup) takes its positions again with x - c, c = 128 (1 + 2^8 + 2^16), whose four
 // digits are the bytes of x with the three lower top bits turned over: sum q k = sum (q-c)(k-c) + c (sum (q-c) + sum (k-c)) + c^2 dim.
 // ------------------------------------------------------------------------------------------------
+using step::kCols;
 using step::kRows;
 constexpr uint32_t kNoElement = 0x00808080;          // whose four digits are all zero
 constexpr uint32_t kThreeDigits = 0x00808080;        // added to an element, leaves 24 bits of it where three digits hold it
@@ -28,7 +29,7 @@ struct Rows {
     int32_t* base;
     size_t stride;
     bool dense;
-    __device__ __forceinline__ int32_t* at(size_t row, uint32_t t, uint32_t v) const { return base + row * stride + (dense ? t : v * kRows + t % kRows); }
+    __device__ __forceinline__ int32_t* at(size_t row, uint32_t t, uint32_t v) const { return base + row * stride + (dense ? t : v * kCols + t % kCols); }
 };
 
 struct WindowArgs {
@@ -44,7 +45,8 @@ struct WindowArgs {
     uint32_t* status;
     bool q_vec;
     double limit;                // of a score's product that is rescaled in double precision
-    double* factors;             // of the exponential table, see wit_window_table_kernel; null where it is not looked into
+    uint32_t along;              // workgroups of a launch's first axis
+    double* factors;             // of the exponential table, see make_factors; null where it is read
     uint32_t* differs;
 };
 
@@ -69,14 +71,14 @@ __device__ __forceinline__ void four_planes(v4i_t x, uint32_t out[4]) {
     for (int k = 0; k < 3; k++) out[k] ^= kByteTops;
 }
 
-// A workgroup's rows: rows 64 * tile .. + R of the cache head kv of sequence b, whose n new tokens start at row `first` and position
+// A workgroup's rows: rows `at` .. + R of the cache head kv of sequence b, whose n new tokens start at row `first` and position
 // `pos`.  Row r is query head r % each of token r / each.
 struct RowTile {
-    uint32_t b, kv, first, n, pos, at, R;
+    uint32_t b, kv, first, n, pos, at, R, first_pos, last_pos;
     uint32_t lane, wave, col, kg;
     __device__ __forceinline__ bool find(const WindowArgs& p, uint32_t index) {
         lane = threadIdx.x & 63u;
-        wave = threadIdx.x >> 6;
+        wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
         col = lane & 15u;
         kg = lane >> 4;
         // the heads of one tile are neighbours, so that each die's L2 gets the keys of its own heads where there are eight; long rows first
@@ -102,6 +104,8 @@ struct RowTile {
         if (local >= all) return false;
         at = (uint32_t)local;
         R = (uint32_t)min((uint64_t)kRows, all - local);
+        first_pos = pos_of(p, 0);
+        last_pos = pos_of(p, R - 1);
         return true;
     }
     __device__ __forceinline__ uint32_t token(const WindowArgs& p, uint32_t r) const { return p.by_each(at + r); }
@@ -110,7 +114,11 @@ struct RowTile {
         const uint32_t j = token(p, r);
         return (size_t)(first + j) * p.a.heads + kv * p.plan.each + (at + r - j * p.plan.each);
     }
-    __device__ __forceinline__ step::Seen seen(const WindowArgs& p) const { return step::Seen(pos_of(p, 0), pos_of(p, R - 1), p.a.window, p.a.sinks); }
+    __device__ __forceinline__ step::Seen seen(const WindowArgs& p) const { return step::Seen(first_pos, last_pos, p.a.window, p.a.sinks); }
+    // whether there are kRows rows and all of them see the kCols positions from k0 on
+    __device__ __forceinline__ bool all_see(const WindowArgs& p, uint32_t k0) const {
+        return R == kRows && k0 + kCols - 1 <= first_pos && (!p.a.window || k0 + p.a.window > last_pos || k0 + kCols <= p.a.sinks);
+    }
 };
 
 // Offset of position t's token, -1 where its page is outside the cache, -2 where no row sees it.
@@ -120,8 +128,8 @@ __device__ __forceinline__ int64_t offset_of(const WindowArgs& p, const RowTile&
     return token::token_offset(p.c, p.a.d_block_table[(size_t)w.b * p.a.table_stride + pg], t - pg * p.c.page_size);
 }
 
-// The queries' digits of a block of 256 elements in LDS, [step of 64][plane][lane group][row], 16 bytes each.
-constexpr uint32_t kBlockSteps = 4;
+// The queries' digits of a block of 512 elements in LDS, [step of 64][plane][lane group][row], 16 bytes each.
+constexpr uint32_t kBlockSteps = 8;
 __device__ __forceinline__ const int32_t* query_of(const WindowArgs& p, const RowTile& w, uint32_t r) {
     const uint32_t tok = w.token(p, r);
     return p.a.d_q + (int64_t)(w.first + tok) * p.a.q_stride + (size_t)(w.kv * p.plan.each + (w.at + r - tok * p.plan.each)) * p.c.dim;
@@ -169,13 +177,13 @@ __device__ __forceinline__ void store_four(int32_t* to, v4u_t x, uint32_t there)
 }
 
 // The scores of a wave's positions with operands of any size, both from memory: sixteen rows at a time, four planes each.
-__device__ __forceinline__ void wide_scores(const WindowArgs& p, const RowTile& w, const step::Seen& seen, uint32_t v0, uint32_t tiles, const int64_t* off, int32_t mx[4], uint32_t& bad) {
+__device__ __forceinline__ void wide_scores(const WindowArgs& p, const RowTile& w, const step::Seen& seen, uint32_t v0, uint32_t tiles, const int64_t* off, int32_t mx[2], uint32_t& bad) {
     const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
     const uint32_t dim = p.c.dim;
 #pragma unroll 1
     for (uint32_t tile = 0; tile < tiles; tile++) {
-        const int32_t* k_row = keys + max(off[tile * kRows + 16 * w.wave + w.col], (int64_t)0);
-        const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, t0 = seen.tile(v) * kRows + in_tile;
+        const int32_t* k_row = keys + max(off[tile * kCols + 16 * w.wave + w.col], (int64_t)0);
+        const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, t0 = seen.tile(v) * kCols + in_tile;
 #pragma unroll 1
         for (uint32_t rb = 0; 16 * rb < w.R; rb++) {
             const uint32_t r = min(16 * rb + w.col, w.R - 1);
@@ -231,15 +239,13 @@ __device__ __forceinline__ void wide_scores(const WindowArgs& p, const RowTile& 
                 y += (uint64_t)kCacheOffset * (uint64_t)(k_of + q_sum + kCacheOffset * dim);
                 uint32_t wide = 0;
                 int32_t qi, ri;
-                p.qk.apply(off[tile * kRows + in_tile + i] < 0 ? 0 : (int64_t)y, qi, ri, wide);          // a page outside: zero
+                p.qk.apply(off[tile * kCols + in_tile + i] < 0 ? 0 : (int64_t)y, qi, ri, wide);          // a page outside: zero
                 q[i] = qi;
                 rem[i] = ri;
                 if ((there >> i) & 1u) {
                     bad |= wide;
                     if (rb == 0) mx[0] = max(mx[0], qi);
-                    else if (rb == 1) mx[1] = max(mx[1], qi);
-                    else if (rb == 2) mx[2] = max(mx[2], qi);
-                    else mx[3] = max(mx[3], qi);
+                    else mx[1] = max(mx[1], qi);
                 }
             }
             const size_t row = w.row(p, r);
@@ -249,17 +255,49 @@ __device__ __forceinline__ void wide_scores(const WindowArgs& p, const RowTile& 
     }
 }
 
-// Scores of 64 rows with a chunk of the positions.  A wave takes 16 positions of each tile of 64 and all rows; it reads its keys from
-// memory into the operand (lane l the elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16), the queries' digits from LDS.  The
-// instructions behind the products - 64 scores a lane for 128 elements' 288 matrix instructions a wave - are what it is short of:
-// five accumulators become a sum in double precision, exact below 2^53, and below 2^50 the quotient of (y + s/2 + 1/2) / s needs no
+// A table of exponentials need not be looked into where it is one: entry 2^bit_shift - 1 - d is then round(S exp(-d / S)) with S the
+// entry of d = 0.  Written as d = 1024 a + b that is the product of two factors of a thousand each, 16 KB in all, which LDS holds.  These
+// workgroups make the factors and compare every entry that a score can meet; where one differs, the entries are read.
+constexpr uint32_t kFactors = 1024, kTableGroups = 64;
+__device__ __forceinline__ void make_factors(const WindowArgs& p, uint32_t group, double* factors, uint32_t& differs) {
+    const uint32_t last = ((uint32_t)1 << p.a.bit_shift) - 1;
+    const int32_t top = p.a.d_exp_table[last];
+    const double scale = (double)max(top, 1);
+    if (threadIdx.x == 0) differs = top < 1;
+    for (uint32_t i = threadIdx.x; i < kFactors; i += kBlock) {
+        factors[i] = scale * exp(-(double)(i * kFactors) / scale);
+        factors[kFactors + i] = exp(-(double)i / scale);
+    }
+    __syncthreads();
+    const uint32_t each = last / kTableGroups + 1, from = group * each, to = min(from + each, last + 1);
+    bool other = false;
+#pragma unroll 8
+    for (uint32_t d = from + threadIdx.x; d < to; d += kBlock) other |= p.a.d_exp_table[last - d] != (int32_t)__builtin_rint(factors[d / kFactors] * factors[kFactors + d % kFactors]);
+    if (other) differs = 1;
+    __syncthreads();
+    if (threadIdx.x == 0) p.differs[group] = differs;
+    if (group == 0)
+        for (uint32_t i = threadIdx.x; i < 2 * kFactors; i += kBlock) p.factors[i] = factors[i];
+}
+
+// Loads of the next positions are issued before this one's stores, so that waiting for them does not wait for the stores; that holds
+// where the number of stores is known, so a tile that all rows see in full goes straight, and others wait for everything in the end.
+__device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }          // vmcnt 0
+
+// Scores of 32 rows with a chunk of the positions.  A wave takes 16 positions of each tile of 64 and all rows; it reads its keys from
+// memory into the operand (lane l the elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16), the queries' digits from LDS.
+// Five accumulators become a sum in double precision, exact below 2^53, and below 2^50 the quotient of (y + s/2 + 1/2) / s needs no
 // second look: it is no nearer than 1 / (2 s) to a whole number, and the product with 1 / s off by at most 2^-52 of itself.
-template <bool VEC>
+template <bool VEC, bool REM>
 __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ int32_t top[4][kRows];
     __shared__ uint32_t q_over;
     uint32_t bad = 0;
+    if (blockIdx.x >= p.along) {
+        if (blockIdx.y == 0) make_factors(p, blockIdx.x - p.along, reinterpret_cast<double*>(lds), q_over);
+        return;
+    }
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         uint32_t n, pos;
         for (uint32_t b = threadIdx.x; b < p.a.seqs; b += 256)
@@ -274,8 +312,8 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
     const uint32_t tiles = min(p.plan.score_cols, seen.tiles - v0), steps = p.plan.dim64, dim = p.c.dim, blocks = (steps + kBlockSteps - 1) / kBlockSteps;
     int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)min(steps, kBlockSteps) * 3 * 4 * kRows * 4);
     if (threadIdx.x == 0) q_over = 0;
-    for (uint32_t i = threadIdx.x; i < tiles * kRows; i += 256) {
-        const int64_t o = offset_of(p, w, seen, seen.tile(v0 + i / kRows) * kRows + i % kRows);
+    for (uint32_t i = threadIdx.x; i < tiles * kCols; i += 256) {
+        const int64_t o = offset_of(p, w, seen, seen.tile(v0 + i / kCols) * kCols + i % kCols);
         if (o == -1) bad |= (uint32_t)kWitIndex;
         off[i] = o;
     }
@@ -290,7 +328,7 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
     const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
     v4i_t x[4];
     auto fetch = [&](uint32_t tile, uint32_t s) {
-        const int32_t* k = keys + max(off[tile * kRows + 16 * w.wave + w.col], (int64_t)0) + 64 * s + 4 * w.kg;
+        const int32_t* k = keys + max(off[tile * kCols + 16 * w.wave + w.col], (int64_t)0) + 64 * s + 4 * w.kg;
         if (VEC && 64 * s + 64 <= dim) {
 #pragma unroll
             for (uint32_t c = 0; c < 4; c++) x[c] = *reinterpret_cast<const v4i_t*>(k + 16 * c);
@@ -303,24 +341,23 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
         }
     };
     fetch(0, 0);
-    int32_t mx[4] = {INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN};
-    uint32_t pos[4];
-    size_t row[4];
+    int32_t mx[2] = {INT32_MIN, INT32_MIN};
+    uint32_t pos[2];
+    size_t row[2];
 #pragma unroll
-    for (uint32_t rb = 0; rb < 4; rb++) {
+    for (uint32_t rb = 0; rb < 2; rb++) {
         const uint32_t r = min(16 * rb + w.col, w.R - 1);
         pos[rb] = w.pos_of(p, r);
         row[rb] = w.row(p, r);
     }
-    const uint32_t first_pos = w.pos_of(p, 0), last_pos = w.pos_of(p, w.R - 1);
     const double scale = (double)p.qk.s, inv = p.qk.inv, half = (double)(p.qk.s >> 1) + 0.5, limit = p.limit;
     bool large = false;
 #pragma unroll 1
     for (uint32_t tile = 0; tile < tiles; tile++) {
-        v4i_t acc[4][5];
+        v4i_t acc[2][5];
         uint32_t k_over = 0;
 #pragma unroll
-        for (int rb = 0; rb < 4; rb++)
+        for (int rb = 0; rb < 2; rb++)
 #pragma unroll
             for (int g = 0; g < 5; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
 #pragma unroll 1
@@ -342,7 +379,7 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
             else if (tile + 1 < tiles) fetch(tile + 1, 0);
             const v4i_t* qa = reinterpret_cast<const v4i_t*>(lds) + ((s % kBlockSteps) * 12 + w.kg) * kRows + w.col;
 #pragma unroll
-            for (uint32_t rb = 0; rb < 4; rb++) {
+            for (uint32_t rb = 0; rb < 2; rb++) {
                 if (rb >= row_blocks) break;
 #pragma unroll
                 for (int a = 0; a < 3; a++) {
@@ -353,40 +390,55 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
             }
         }
         // register i of lane l: position 4 (l / 16) + i of the wave's 16, row l % 16 of a block
-        const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, k0 = seen.tile(v) * kRows, t0 = k0 + in_tile;
-        const bool all = k0 + kRows - 1 <= first_pos && (!p.a.window || k0 + p.a.window > last_pos || k0 + kRows <= p.a.sinks);
+        const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, k0 = seen.tile(v) * kCols, t0 = k0 + in_tile;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) large |= off[tile * kRows + in_tile + i] == -1;          // wide_scores knows what to do with them
-        large |= (k_over & kOver) && off[tile * kRows + 16 * w.wave + w.col] >= 0;
-#pragma unroll
-        for (uint32_t rb = 0; rb < 4; rb++) {
-            if (rb >= row_blocks) break;
-            v4u_t q, rem;
-            const uint32_t there = 16 * rb + w.col >= w.R ? 0 : all ? 15u : seen_of_four(p, pos[rb], t0);
+        for (uint32_t i = 0; i < 4; i++) large |= off[tile * kCols + in_tile + i] == -1;          // wide_scores knows what to do with them
+        large |= (k_over & kOver) && off[tile * kCols + 16 * w.wave + w.col] >= 0;
+        auto rescale = [&](uint32_t rb, uint32_t there, v4u_t& q, v4u_t& rem) {
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
                 double y = (double)acc[rb][4][i];
 #pragma unroll
                 for (int g = 3; g >= 0; g--) y = __builtin_fma(y, 256.0, (double)acc[rb][g][i]);
                 const double t = y + half, quotient = __builtin_floor(t * inv);
-                large |= ((there >> i) & 1u) && __builtin_fabs(t) >= limit;
+                const bool here = (there >> i) & 1u;
+                large |= here && __builtin_fabs(t) >= limit;
                 q[i] = (int32_t)quotient;
-                rem[i] = (int32_t)__builtin_fma(-quotient, scale, y);
-                mx[rb] = max(mx[rb], (there >> i) & 1u ? q[i] : INT32_MIN);
+                if constexpr (REM) rem[i] = (int32_t)__builtin_fma(-quotient, scale, y);
+                mx[rb] = max(mx[rb], here ? q[i] : INT32_MIN);
             }
-            store_four(p.scores.at(row[rb], t0, v), q, there);
-            if (p.a.d_scores_rem) store_four(p.a.d_scores_rem + row[rb] * p.a.max_len + t0, rem, there);
+        };
+        if (w.all_see(p, k0)) {
+#pragma unroll
+            for (uint32_t rb = 0; rb < 2; rb++) {
+                v4u_t q, rem;
+                __builtin_amdgcn_sched_barrier(0);          // one block's numbers in registers at a time
+                rescale(rb, 15u, q, rem);
+                *reinterpret_cast<v4u_t*>(p.scores.at(row[rb], t0, v)) = q;
+                if constexpr (REM) *reinterpret_cast<v4u_t*>(p.a.d_scores_rem + row[rb] * p.a.max_len + t0) = rem;
+            }
+        } else {
+#pragma unroll 1
+            for (uint32_t rb = 0; rb < row_blocks; rb++) {
+                const uint32_t there = 16 * rb + w.col >= w.R ? 0 : seen_of_four(p, rb ? pos[1] : pos[0], t0);
+                const size_t to = rb ? row[1] : row[0];
+                v4u_t q, rem;
+                if (rb) rescale(1, there, q, rem);
+                else rescale(0, there, q, rem);
+                store_four(p.scores.at(to, t0, v), q, there);
+                if constexpr (REM) store_four(p.a.d_scores_rem + to * p.a.max_len + t0, rem, there);
+            }
+            wait_for_memory();
         }
     }
     if (__any((over & kOver) != 0) && w.lane == 0) q_over = 1;          // the queries' digits were made by all threads
     __syncthreads();
     if (q_over || __any(large)) {
-#pragma unroll
-        for (int rb = 0; rb < 4; rb++) mx[rb] = INT32_MIN;
+        mx[0] = mx[1] = INT32_MIN;
         wide_scores(p, w, seen, v0, tiles, off, mx, bad);
     }
 #pragma unroll
-    for (int rb = 0; rb < 4; rb++) {
+    for (int rb = 0; rb < 2; rb++) {
         mx[rb] = max(mx[rb], __shfl_xor(mx[rb], 16, 64));
         mx[rb] = max(mx[rb], __shfl_xor(mx[rb], 32, 64));
         if (w.kg == 0) top[w.wave][16 * rb + w.col] = mx[rb];
@@ -401,38 +453,9 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
     if (bad) atomicOr(p.status, bad);
 }
 
-// A table of exponentials need not be looked into where it is one: entry 2^bit_shift - 1 - d is then round(S exp(-d / S)) with S the
-// entry of d = 0.  Written as d = 1024 a + b that is the product of two factors of a thousand each, 16 KB in all, which LDS holds.  This
-// launch makes the factors and compares every entry that a score can meet; where one differs, the entries are read.
-constexpr uint32_t kFactors = 1024, kTableGroups = 64;
-__global__ void __launch_bounds__(kBlock) wit_window_table_kernel(WindowArgs p) {
-    __shared__ double factors[2 * kFactors];
-    __shared__ uint32_t differs;
-    const int64_t last = ((int64_t)1 << p.a.bit_shift) - 1;
-    const int32_t top = p.a.d_exp_table[last];
-    const double scale = (double)max(top, 1);
-    if (threadIdx.x == 0) differs = top < 1;
-    for (uint32_t i = threadIdx.x; i < kFactors; i += kBlock) {
-        factors[i] = scale * exp(-(double)(i * kFactors) / scale);
-        factors[kFactors + i] = exp(-(double)i / scale);
-    }
-    __syncthreads();
-    const uint32_t each = (uint32_t)(last / kTableGroups + 1), from = blockIdx.x * each;
-    bool other = false;
-    for (uint32_t i = threadIdx.x; i < each && from + i <= last; i += kBlock) {
-        const uint32_t d = from + i;
-        other |= p.a.d_exp_table[last - d] != (int32_t)__builtin_rint(factors[d / kFactors] * factors[kFactors + d % kFactors]);
-    }
-    if (other) differs = 1;
-    __syncthreads();
-    if (threadIdx.x == 0) p.differs[blockIdx.x] = differs;
-    if (blockIdx.x == 0)
-        for (uint32_t i = threadIdx.x; i < 2 * kFactors; i += kBlock) p.factors[i] = factors[i];
-}
-
-// Exponentials of 64 rows and a chunk of the positions, and the rows' sums, to which the chunks add.  The table's entries are 4 MB,
-// of which a wave asks for 64 lines at a time: reading them is bound by L2.
-template <bool FACTORS>
+// Exponentials of 32 rows and a chunk of the positions, and the rows' sums, to which the chunks add.  A wave takes 256 positions of a row
+// at a time.  The table's entries are 4 MB, of which a wave asks for 64 lines at a time: reading them is bound by L2.
+template <bool FACTORS, bool SHIFTED>
 __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
     __shared__ int32_t top[kRows];
     __shared__ double factors[FACTORS ? 2 * kFactors : 1];
@@ -457,303 +480,330 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
     __syncthreads();
     if (blockIdx.y == 0 && p.a.d_max && threadIdx.x < w.R) p.a.d_max[w.row(p, threadIdx.x)] = top[threadIdx.x];
     uint32_t bad = 0;
-    const uint32_t last = ((uint32_t)1 << p.a.bit_shift) - 1, first_pos = w.pos_of(p, 0), last_pos = w.pos_of(p, w.R - 1);
-    for (uint32_t r = w.wave; r < w.R; r += 4) {
-        const uint32_t pos = w.pos_of(p, r);
-        const size_t row = w.row(p, r);
-        const int32_t mx = top[r];
-        unsigned long long sum = 0;
-        for (uint32_t i = 4 * w.lane; i < tiles * kRows; i += 256) {
-            const uint32_t v = v0 + i / kRows, k0 = seen.tile(v) * kRows, t = k0 + i % kRows;
-            const bool all = k0 + kRows - 1 <= first_pos && (!p.a.window || k0 + p.a.window > last_pos || k0 + kRows <= p.a.sinks);
-            const uint32_t there = all ? 15u : seen_of_four(p, pos, t);
-            if (!there) continue;
-            const int32_t* from = p.scores.at(row, t, v);
-            v4u_t x = {mx, mx, mx, mx}, e, shifted;
-            if (there == 15u) {
-                x = *reinterpret_cast<const v4u_t*>(from);
-            } else {
+    const uint32_t last = ((uint32_t)1 << p.a.bit_shift) - 1, groups = (tiles + 3) / 4, items = w.wave < w.R ? ((w.R - 1 - w.wave) / 4 + 1) * groups : 0;
+    // item `it`: 256 positions of tiles 4 g .. of row r
+    struct Place {
+        uint32_t r, v, t, there;
+        bool full;
+        size_t row;
+    };
+    auto place = [&](uint32_t it) {
+        Place a;
+        const uint32_t k = it / groups, g = it - k * groups;
+        a.r = w.wave + 4 * k;
+        a.row = w.row(p, a.r);
+        a.full = 4 * g + 4 <= tiles;
+        if (a.full) {
 #pragma unroll
-                for (uint32_t j = 0; j < 4; j++)
-                    if ((there >> j) & 1u) x[j] = from[j];
-            }
-            if (computed) {
-#pragma unroll
-                for (uint32_t j = 0; j < 4; j++) {
-                    const uint32_t below = (uint32_t)mx - (uint32_t)x[j], d = min(below, last);          // entry 0 stands in for those before it
-                    shifted[j] = (int32_t)(0 - below);
-                    e[j] = (int32_t)__builtin_rint(factors[d / kFactors] * factors[kFactors + d % kFactors]);
-                    sum += (uint32_t)((there >> j) & 1u ? e[j] : 0);
-                    if (below > last) bad |= (uint32_t)kWitIndex;          // only positions that are there have a score below the maximum
-                }
-            } else {
-#pragma unroll
-                for (uint32_t j = 0; j < 4; j++) {
-                    const int64_t idx = (int64_t)x[j] - mx + last;
-                    const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
-                    e[j] = p.a.d_exp_table[ok ? idx : 0];
-                    shifted[j] = (int32_t)((int64_t)x[j] - mx);
-                    if ((there >> j) & 1u) {
-                        if (!ok) bad |= (uint32_t)kWitIndex;
-                        if (e[j] < 0) bad |= (uint32_t)kWitSum;
-                        sum += (unsigned long long)max(e[j], 0);
-                    }
-                }
-            }
-            store_four(p.exps.at(row, t, v), e, there);
-            if (p.a.d_shifted) store_four(p.a.d_shifted + row * p.a.max_len + t, shifted, there);
+            for (uint32_t j = 0; j < 4; j++) a.full = a.full && w.all_see(p, seen.tile(v0 + 4 * g + j) * kCols);
         }
+        a.v = v0 + 4 * g + w.lane / 16;
+        a.t = seen.tile(a.v) * kCols + 4 * w.lane % kCols;
+        a.there = a.full ? 15u : a.v < v0 + tiles ? seen_of_four(p, w.pos_of(p, a.r), a.t) : 0;
+        return a;
+    };
+    auto load = [&](const Place& a, v4u_t& x) {
+        const int32_t* from = p.scores.at(a.row, a.t, a.v);
+        if (a.full) {
+            x = *reinterpret_cast<const v4u_t*>(from);
+        } else {
 #pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
-        if (w.lane == 0) atomicAdd(&p.sums[row], sum);
+            for (uint32_t j = 0; j < 4; j++) x[j] = (a.there >> j) & 1u ? from[j] : INT32_MIN;
+        }
+    };
+    Place at, next;
+    v4u_t x, x_next;
+    unsigned long long sum = 0;
+    if (items) {
+        next = place(0);
+        load(next, x_next);
+    }
+#pragma unroll 1
+    for (uint32_t it = 0; it < items; it++) {
+        at = next;
+        x = x_next;
+        if (it + 1 < items) {
+            next = place(it + 1);
+            load(next, x_next);
+        }
+        const int32_t mx = top[at.r];
+        v4u_t e, shifted;
+        if (computed) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t below = (uint32_t)mx - (uint32_t)x[j], d = min(below, last);          // entry 0 stands in for those before it
+                shifted[j] = (int32_t)(0 - below);
+                e[j] = (int32_t)__builtin_rint(factors[d / kFactors] * factors[kFactors + d % kFactors]);
+                const bool here = (at.there >> j) & 1u;
+                sum += (uint32_t)(here ? e[j] : 0);
+                if (here && below > last) bad |= (uint32_t)kWitIndex;
+            }
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const int64_t idx = (int64_t)x[j] - mx + last;
+                const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
+                e[j] = p.a.d_exp_table[ok ? idx : 0];
+                shifted[j] = (int32_t)((int64_t)x[j] - mx);
+                if ((at.there >> j) & 1u) {
+                    if (!ok) bad |= (uint32_t)kWitIndex;
+                    if (e[j] < 0) bad |= (uint32_t)kWitSum;
+                    sum += (unsigned long long)max(e[j], 0);
+                }
+            }
+        }
+        int32_t* to = p.exps.at(at.row, at.t, at.v);
+        if (at.full) {
+            *reinterpret_cast<v4u_t*>(to) = e;
+            if constexpr (SHIFTED) *reinterpret_cast<v4u_t*>(p.a.d_shifted + at.row * p.a.max_len + at.t) = shifted;
+        } else {
+            store_four(to, e, at.there);
+            if constexpr (SHIFTED) store_four(p.a.d_shifted + at.row * p.a.max_len + at.t, shifted, at.there);
+            wait_for_memory();
+        }
+        if (it + 1 == items || next.r != at.r) {
+#pragma unroll
+            for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+            if (w.lane == 0) atomicAdd(&p.sums[at.row], sum);
+            sum = 0;
+        }
     }
     if (bad) atomicOr(p.status, bad);
 }
 
-// Probabilities of 64 rows and their products with 128 elements of the values, over a chunk of the positions.  Eight threads a row make
+// Probabilities of 32 rows and their products with 128 elements of the values, over a chunk of the positions.  Sixteen threads a row make
 // the digits of 64 positions in LDS while the waves multiply the 64 before them; a wave takes 16 elements and all rows, and turns
 // its values into operands in registers.  A probability is floor((e P + floor(S/2)) / S) from one product in double precision, as the
 // scores' quotients are, where S is below 2^28 and P at most 2^22; the remainder of the division gives the lookup's query.
 constexpr uint32_t kValueThreads = 512;
 constexpr uint64_t kPlainSum = (uint64_t)1 << 28;
-template <int PP, bool WIDE>
-struct Values {
-    static constexpr int VP = WIDE ? 4 : 3, G = PP + VP - 1;
-    v4i_t acc[4][G];
-    int32_t x[16];
-    uint32_t over = 0;
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int rb = 0; rb < 4; rb++)
-#pragma unroll
-            for (int g = 0; g < G; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
-    }
-    __device__ __forceinline__ void fetch(const int32_t* values, const int64_t* off) {
-#pragma unroll
-        for (uint32_t j = 0; j < 16; j++) x[j] = values[max(off[j], (int64_t)0)];
-    }
-    // the planes of the probabilities' digits below `planes`, from LDS
-    __device__ __forceinline__ void multiply(const v4i_t* digits, uint32_t row_blocks, int planes) {
-        v4i_t vb[VP];
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const v4i_t y = {x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
-            uint32_t pl[4];
-            if constexpr (WIDE) four_planes(y, pl);
-            else three_planes(y, pl, over);
-#pragma unroll
-            for (int k = 0; k < VP; k++) vb[k][c] = (int)pl[k];
-        }
-#pragma unroll
-        for (uint32_t rb = 0; rb < 4; rb++) {
-            if (rb >= row_blocks) break;
-#pragma unroll
-            for (int a = 0; a < PP; a++) {
-                if (a >= planes) break;
-                const v4i_t f = digits[a * 4 * kRows + 16 * rb];
-#pragma unroll
-                for (int k = 0; k < VP; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[k], f, acc[rb][a + k], 0, 0, 0);
-            }
-        }
-    }
-    __device__ __forceinline__ uint64_t sum(uint32_t rb, uint32_t i) const {
-        uint64_t y = 0;
-#pragma unroll
-        for (int g = G - 1; g >= 0; g--) y = (y << 8) + (uint64_t)(int64_t)acc[rb][g][i];
-        return y;
-    }
-};
+enum Written { kNone, kBoth, kSome };          // of the probabilities and queries
 
 template <int PP>
-__global__ void __launch_bounds__(kValueThreads, 2) wit_window_values_kernel(WindowArgs p) {
-    __shared__ __attribute__((aligned(16))) uint32_t digits[2][PP * 4 * kRows * 4];
-    __shared__ int64_t off[step::kOffsetTiles * kRows];
-    __shared__ unsigned long long p_sum[kRows];
-    __shared__ uint32_t third[2], wide_any;          // the last tile with digits in the third plane (and 1), for odd and even ones
-    RowTile w;
-    if (!w.find(p, blockIdx.x)) return;
-    const step::Seen seen = w.seen(p);
-    const uint32_t group = blockIdx.y % p.plan.groups, chunk = blockIdx.y / p.plan.groups, v0 = chunk * p.plan.value_cols, dim = p.c.dim;
-    if (v0 >= seen.tiles) return;
-    const uint32_t tiles = min(p.plan.value_cols, seen.tiles - v0);
-    uint32_t bad = 0;
-    if (threadIdx.x == 0) third[0] = third[1] = wide_any = 0;
-    // of the probabilities: this thread's row and its eight positions of a tile
-    const uint32_t r = threadIdx.x >> 3, part = threadIdx.x & 7u;
-    const bool mine = r < w.R, write = group == 0;
-    const uint32_t rr = mine ? r : 0, pos = w.pos_of(p, rr), first_pos = w.pos_of(p, 0), last_pos = w.pos_of(p, w.R - 1);
+struct ValueLds {
+    uint32_t digits[2][PP * 4 * kRows * 4];
+    int64_t off[2][step::kOffsetTiles * kCols];
+    unsigned long long p_sum[kRows];
+    uint32_t third[2], wide;          // the last tile with digits in the third plane (and 1), of even and odd ones
+};
+
+template <int PP, bool WIDE, Written W>
+__device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile& w, const step::Seen& seen, ValueLds<PP>& lds, uint32_t group, uint32_t chunk, uint32_t& bad) {
+    constexpr int VP = WIDE ? 4 : 3, G = PP + VP - 1;
+    constexpr uint32_t K = step::kOffsetTiles;
+    const uint32_t v0 = chunk * p.plan.value_cols, tiles = min(p.plan.value_cols, seen.tiles - v0), dim = p.c.dim;
+    // of the probabilities: this thread's row and its four positions of a tile
+    const uint32_t r = threadIdx.x >> 4, part = threadIdx.x & 15u, rr = min(r, w.R - 1), pos = w.pos_of(p, rr);
+    const bool mine = r < w.R;
     const size_t row = w.row(p, rr);
     unsigned long long sum = p.sums[row], all = 0;
     if (sum == 0) {
         if (mine) bad |= (uint32_t)kWitSum;
         sum = 1;
     }
-    if (mine && write && chunk == 0 && part == 0 && p.a.d_sum) store_sum(&p.a.d_sum[row], sum, bad);
+    if (!WIDE && mine && group == 0 && chunk == 0 && part == 0 && p.a.d_sum) store_sum(&p.a.d_sum[row], sum, bad);
     const double inv = 1.0 / (double)sum, scale = (double)p.a.prob_scale, half = (double)(sum >> 1) + 0.5, whole_sum = (double)sum, odd = (double)(sum & 1) - 1.0;
     const bool plain = PP == 3 && __all(sum < kPlainSum);
-    int32_t e[8];
-    auto seen_of_eight = [&](uint32_t tile, uint32_t& t) {
-        const uint32_t k0 = seen.tile(v0 + tile) * kRows;
-        t = k0 + 8 * part;
-        if (!mine) return 0u;
-        if (k0 + kRows - 1 <= first_pos && (!p.a.window || k0 + p.a.window > last_pos || k0 + kRows <= p.a.sinks)) return 255u;
-        return seen_of_four(p, pos, t) | seen_of_four(p, pos, t + 4) << 4;
-    };
-    auto fetch_exps = [&](uint32_t tile) {
-        uint32_t t;
-        const uint32_t there = seen_of_eight(tile, t);
-        const int32_t* from = p.exps.at(row, t, v0 + tile);
-        if (there == 255u) {
-            *reinterpret_cast<v4u_t*>(e) = *reinterpret_cast<const v4u_t*>(from);
-            *reinterpret_cast<v4u_t*>(e + 4) = *reinterpret_cast<const v4u_t*>(from + 4);
-        } else {
-#pragma unroll
-            for (uint32_t j = 0; j < 8; j++) e[j] = (there >> j) & 1u ? from[j] : 0;
-        }
-    };
-    auto make_digits = [&](uint32_t tile, bool writes) {
-        uint32_t t;
-        const uint32_t there = seen_of_eight(tile, t);
-        v4u_t pr[2], query[2];
-        if (plain) {
-#pragma unroll
-            for (uint32_t j = 0; j < 8; j++) {
-                const double num = __builtin_fma((double)max(e[j], 0), scale, half), q = __builtin_floor(num * inv);
-                pr[j / 4][j % 4] = (int32_t)q;
-                query[j / 4][j % 4] = (int32_t)__builtin_fma(2.0, __builtin_fma(-q, whole_sum, num), odd);
-            }
-        } else {
-#pragma unroll
-            for (uint32_t j = 0; j < 8; j++) {
-                const uint32_t x = (uint32_t)max(e[j], 0), pj = probability(x, (uint64_t)p.a.prob_scale, sum, inv);
-                uint32_t wide = 0;
-                int32_t qj;
-                store_sum(&qj, lookup_query(x, p.a.prob_scale, sum, pj), wide);
-                pr[j / 4][j % 4] = (int32_t)pj;
-                query[j / 4][j % 4] = qj;
-                if (((there >> j) & 1u) && write && p.a.d_query) bad |= wide;
-            }
-        }
-        if (writes) {
-            const size_t o = row * p.a.max_len + t;
-            if (p.a.d_prob) {
-                store_four(p.a.d_prob + o, pr[0], there & 15u);
-                store_four(p.a.d_prob + o + 4, pr[1], there >> 4);
-            }
-            if (p.a.d_query) {
-                store_four(p.a.d_query + o, query[0], there & 15u);
-                store_four(p.a.d_query + o + 4, query[1], there >> 4);
-            }
-        }
-        v4i_t d[2];
-        uint32_t large = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < 8; j++) {
-            const bool used = ((there >> j) & 1u) && off[(tile % step::kOffsetTiles) * kRows + 8 * part + j] >= 0;          // a page outside: no value
-            d[j / 4][j % 4] = used ? pr[j / 4][j % 4] : 0;
-            large |= (uint32_t)d[j / 4][j % 4] + 0x8080u;
-        }
-        uint32_t pl[2][4];
-        if constexpr (PP == 3) {
-            uint32_t none = 0;
-            three_planes(d[0], pl[0], none);
-            three_planes(d[1], pl[1], none);
-        } else {
-#pragma unroll
-            for (uint32_t h = 0; h < 2; h++) transpose4(digits_of(d[h][0]), digits_of(d[h][1]), digits_of(d[h][2]), digits_of(d[h][3]), pl[h]);
-        }
-        if (__any(large >> 16) && w.lane == 0) third[tile & 1] = tile + 1;
-        uint64_t* to = reinterpret_cast<uint64_t*>(digits[tile & 1]) + ((part >> 1) * kRows + r) * 2 + (part & 1u);
-#pragma unroll
-        for (int k = 0; k < PP; k++) to[k * 4 * kRows * 2] = ((uint64_t)pl[1][k] << 32) | pl[0][k];
-        return d[0][0] + (uint64_t)d[0][1] + d[0][2] + d[0][3] + d[1][0] + d[1][1] + d[1][2] + d[1][3];
-    };
     const uint32_t e0 = group * step::kValueDims + 16 * w.wave, row_blocks = (w.R + 15) / 16;
     const int32_t* values = p.c.d_v + (int64_t)w.kv * p.c.head_stride + min(e0 + w.col, dim - 1);
     const bool multiplies = e0 < dim;
-    auto run = [&](auto& products, bool writes) {
-        products.clear();
-        fetch_exps(0);
-#pragma unroll 1
-        for (uint32_t tile = 0; tile < tiles; tile++) {
-            if (tile % step::kOffsetTiles == 0) {
-                __syncthreads();          // nobody reads the offsets before any more
-                const uint32_t n = min(step::kOffsetTiles, tiles - tile) * kRows;
-                for (uint32_t i = threadIdx.x; i < n; i += kValueThreads) off[i] = offset_of(p, w, seen, seen.tile(v0 + tile + i / kRows) * kRows + i % kRows);
-                __syncthreads();
-            }
-            const int64_t* o = off + (tile % step::kOffsetTiles) * kRows + 16 * w.kg;
-            if (multiplies) products.fetch(values, o);
-            all += make_digits(tile, writes);
-            if (tile + 1 < tiles) fetch_exps(tile + 1);
-            __syncthreads();
-            if (multiplies) products.multiply(reinterpret_cast<const v4i_t*>(digits[tile & 1]) + w.kg * kRows + w.col, row_blocks, PP == 3 && third[tile & 1] != tile + 1 ? 2 : PP);
+    auto make_offsets = [&](uint32_t tile) {
+        const uint32_t n = min(K, tiles - tile) * kCols;
+        for (uint32_t i = threadIdx.x; i < n; i += kValueThreads) lds.off[(tile / K) & 1][i] = offset_of(p, w, seen, seen.tile(v0 + tile + i / kCols) * kCols + i % kCols);
+    };
+    auto offsets = [&](uint32_t tile) { return lds.off[(tile / K) & 1] + (tile % K) * kCols; };
+    int32_t x[16];
+    v4u_t e;
+    auto fetch = [&](uint32_t tile) {
+        const int64_t* o = offsets(tile) + 16 * w.kg;
+        if (multiplies) {
+#pragma unroll
+            for (uint32_t j = 0; j < 16; j++) x[j] = values[max(o[j], (int64_t)0)];
+        }
+        const uint32_t k0 = seen.tile(v0 + tile) * kCols, t = k0 + 4 * part;
+        const int32_t* from = p.exps.at(row, t, v0 + tile);
+        if (w.all_see(p, k0)) {
+            e = *reinterpret_cast<const v4u_t*>(from);
+        } else {
+            const uint32_t there = mine ? seen_of_four(p, pos, t) : 0;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) e[j] = (there >> j) & 1u ? from[j] : 0;
         }
     };
-    const bool whole = seen.tiles <= p.plan.value_cols;          // all positions of the rows are this workgroup's
-    const uint32_t e1 = e0 + 4 * w.kg;
-    auto put = [&](auto& products, bool offset) {
+    v4i_t acc[2][G];
 #pragma unroll
-        for (uint32_t rb = 0; rb < 4; rb++) {
-            const uint32_t q_row = 16 * rb + w.col;
-            if (q_row >= w.R || e1 >= dim) continue;
-            const size_t to = w.row(p, q_row);
+    for (int rb = 0; rb < 2; rb++)
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-                if (e1 + i >= dim) break;
-                const uint64_t y = products.sum(rb, i) + (offset ? (uint64_t)kCacheOffset * p_sum[q_row] : 0);
-                if (whole) {
-                    int32_t q, rem;
-                    p.out.apply((int64_t)y, q, rem, bad);
-                    p.a.d_out[to * dim + e1 + i] = q;
-                    if (p.a.d_out_rem) p.a.d_out_rem[to * dim + e1 + i] = rem;
-                } else {
-                    p.part[(to * p.plan.value_chunks + chunk) * dim + e1 + i] = (int64_t)y;
+        for (int g = 0; g < G; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
+    uint32_t over = 0;
+    __syncthreads();
+    make_offsets(0);
+    if (threadIdx.x < 2) lds.third[threadIdx.x] = 0;
+    __syncthreads();
+    fetch(0);
+#pragma unroll 1
+    for (uint32_t tile = 0; tile < tiles; tile++) {
+        // operands and probabilities first, then the next tile's loads, then this one's stores
+        v4i_t vb[VP];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const v4i_t y = {x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
+            uint32_t v[4];
+            if constexpr (WIDE) four_planes(y, v);
+            else three_planes(y, v, over);
+#pragma unroll
+            for (int k = 0; k < VP; k++) vb[k][c] = (int)v[k];
+        }
+        const uint32_t k0 = seen.tile(v0 + tile) * kCols, t = k0 + 4 * part;
+        const bool full = w.all_see(p, k0);
+        const uint32_t there = full ? 15u : mine ? seen_of_four(p, pos, t) : 0;
+        v4u_t pr, query;
+        if (plain) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const double num = __builtin_fma((double)max(e[j], 0), scale, half), q = __builtin_floor(num * inv);
+                pr[j] = (int32_t)q;
+                if constexpr (W != kNone) query[j] = (int32_t)__builtin_fma(2.0, __builtin_fma(-q, whole_sum, num), odd);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t ej = (uint32_t)max(e[j], 0), pj = probability(ej, (uint64_t)p.a.prob_scale, sum, inv);
+                pr[j] = (int32_t)pj;
+                if constexpr (W != kNone) {
+                    uint32_t wide = 0;
+                    int32_t qj;
+                    store_sum(&qj, lookup_query(ej, p.a.prob_scale, sum, pj), wide);
+                    query[j] = qj;
+                    if (((there >> j) & 1u) && p.a.d_query) bad |= wide;
                 }
             }
         }
-    };
+        if (tile + 1 < tiles) {
+            if ((tile + 1) % K == 0) {
+                make_offsets(tile + 1);
+                __syncthreads();
+            }
+            fetch(tile + 1);
+        }
+        if constexpr (W != kNone) {
+            const size_t o = row * p.a.max_len + t;
+            if (W == kBoth && full) {
+                *reinterpret_cast<v4u_t*>(p.a.d_prob + o) = pr;
+                *reinterpret_cast<v4u_t*>(p.a.d_query + o) = query;
+            } else {
+                if (W == kBoth || p.a.d_prob) store_four(p.a.d_prob + o, pr, there);
+                if (W == kBoth || p.a.d_query) store_four(p.a.d_query + o, query, there);
+                wait_for_memory();
+            }
+        }
+        v4i_t d;
+        uint32_t large = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            const bool used = ((there >> j) & 1u) && offsets(tile)[4 * part + j] >= 0;          // a page outside: no value
+            d[j] = used ? pr[j] : 0;
+            large |= (uint32_t)d[j] + 0x8080u;
+            if constexpr (WIDE) all += (uint32_t)d[j];
+        }
+        uint32_t pl[4];
+        if constexpr (PP == 3) {
+            uint32_t none = 0;
+            three_planes(d, pl, none);
+            if (__any(large >> 16) && w.lane == 0) lds.third[tile & 1] = tile + 1;
+        } else {
+            transpose4(digits_of(d[0]), digits_of(d[1]), digits_of(d[2]), digits_of(d[3]), pl);
+        }
+        uint32_t* to = lds.digits[tile & 1] + (((part >> 2) * kRows + r) << 2) + (part & 3u);
+#pragma unroll
+        for (int k = 0; k < PP; k++) to[k * 16 * kRows] = pl[k];
+        __syncthreads();
+        if (!multiplies) continue;
+        const v4i_t* pa = reinterpret_cast<const v4i_t*>(lds.digits[tile & 1]) + w.kg * kRows + w.col;
+        const int planes = PP == 3 && lds.third[tile & 1] != tile + 1 ? 2 : PP;
+#pragma unroll
+        for (uint32_t rb = 0; rb < 2; rb++) {
+            if (rb >= row_blocks) break;
+#pragma unroll
+            for (int a = 0; a < PP; a++) {
+                if (a >= planes) break;
+                const v4i_t f = pa[a * 4 * kRows + 16 * rb];
+#pragma unroll
+                for (int k = 0; k < VP; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[k], f, acc[rb][a + k], 0, 0, 0);
+            }
+        }
+    }
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int k = 8; k >= 1; k >>= 1) all += __shfl_xor(all, k, 64);
+        if (part == 0) lds.p_sum[r] = all;
+    } else {
+        if (__any((over & kOver) != 0) && w.lane == 0) lds.wide = 1;
+    }
+    __syncthreads();
+    if (!WIDE && lds.wide) return true;
+    const bool whole = seen.tiles <= p.plan.value_cols;          // all positions of the rows are this workgroup's
+    const uint32_t e1 = e0 + 4 * w.kg;
+#pragma unroll
+    for (uint32_t rb = 0; rb < 2; rb++) {
+        const uint32_t q_row = 16 * rb + w.col;
+        if (q_row >= w.R || e1 >= dim) continue;
+        const size_t at = w.row(p, q_row);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            if (e1 + i >= dim) break;
+            uint64_t y = WIDE ? (uint64_t)kCacheOffset * lds.p_sum[q_row] : 0, z = 0;
+#pragma unroll
+            for (int g = G - 1; g >= 0; g--) z = (z << 8) + (uint64_t)(int64_t)acc[rb][g][i];
+            y += z;
+            if (whole) {
+                int32_t q, rem;
+                p.out.apply((int64_t)y, q, rem, bad);
+                p.a.d_out[at * dim + e1 + i] = q;
+                if (p.a.d_out_rem) p.a.d_out_rem[at * dim + e1 + i] = rem;
+            } else {
+                p.part[(at * p.plan.value_chunks + chunk) * dim + e1 + i] = (int64_t)y;
+            }
+        }
+    }
+    return false;
+}
+
+template <int PP>
+__global__ void __launch_bounds__(kValueThreads, 4) wit_window_values_kernel(WindowArgs p) {
+    __shared__ __attribute__((aligned(16))) ValueLds<PP> lds;
+    RowTile w;
+    if (!w.find(p, blockIdx.x)) return;
+    const step::Seen seen = w.seen(p);
+    const uint32_t group = blockIdx.y % p.plan.groups, chunk = blockIdx.y / p.plan.groups;
+    if (chunk * p.plan.value_cols >= seen.tiles) return;
+    uint32_t bad = 0;
+    if (threadIdx.x == 0) lds.wide = 0;
     bool wide;
-    {
-        Values<PP, false> products;
-        run(products, write);
-        if (__any((products.over & kOver) != 0) && w.lane == 0) wide_any = 1;
-        __syncthreads();
-        wide = wide_any != 0;
-        if (!wide) put(products, false);
-    }
-    if (wide) {
-        all = 0;
-        Values<PP, true> products;
-        run(products, false);
-        all += __shfl_xor(all, 1, 64);
-        all += __shfl_xor(all, 2, 64);
-        all += __shfl_xor(all, 4, 64);
-        if (part == 0) p_sum[r] = all;
-        __syncthreads();
-        put(products, true);
-    }
+    if (group || (!p.a.d_prob && !p.a.d_query)) wide = window_values<PP, false, kNone>(p, w, seen, lds, group, chunk, bad);
+    else if (p.a.d_prob && p.a.d_query) wide = window_values<PP, false, kBoth>(p, w, seen, lds, group, chunk, bad);
+    else wide = window_values<PP, false, kSome>(p, w, seen, lds, group, chunk, bad);
+    if (wide) window_values<PP, true, kNone>(p, w, seen, lds, group, chunk, bad);
     if (bad) atomicOr(p.status, bad);
 }
 
-// The chunks' partial sums of 64 elements of 64 rows.
+// The chunks' partial sums of 64 elements of a row, a wave each.
 __global__ void __launch_bounds__(256) wit_window_join_kernel(WindowArgs p) {
     RowTile w;
     if (!w.find(p, blockIdx.x)) return;
     const step::Seen seen = w.seen(p);
-    if (seen.tiles <= p.plan.value_cols) return;
-    const uint32_t parts = (seen.tiles - 1) / p.plan.value_cols + 1, e = blockIdx.y * 64 + w.lane, dim = p.c.dim;
-    if (e >= dim) return;
+    const uint32_t r = blockIdx.z * 4 + w.wave, e = blockIdx.y * 64 + w.lane, dim = p.c.dim;
+    if (seen.tiles <= p.plan.value_cols || r >= w.R || e >= dim) return;
+    const uint32_t parts = (seen.tiles - 1) / p.plan.value_cols + 1;
     uint32_t bad = 0;
-    for (uint32_t r = w.wave; r < w.R; r += 4) {
-        const size_t row = w.row(p, r);
-        int64_t y = 0;
-        for (uint32_t i = 0; i < parts; i++) y += p.part[(row * p.plan.value_chunks + i) * dim + e];
-        int32_t q, rem;
-        p.out.apply(y, q, rem, bad);
-        p.a.d_out[row * dim + e] = q;
-        if (p.a.d_out_rem) p.a.d_out_rem[row * dim + e] = rem;
-    }
+    const size_t row = w.row(p, r);
+    int64_t y = 0;
+#pragma unroll 8
+    for (uint32_t i = 0; i < parts; i++) y += p.part[(row * p.plan.value_chunks + i) * dim + e];
+    int32_t q, rem;
+    p.out.apply(y, q, rem, bad);
+    p.a.d_out[row * dim + e] = q;
+    if (p.a.d_out_rem) p.a.d_out_rem[row * dim + e] = rem;
     if (bad) atomicOr(p.status, bad);
 }
 
@@ -778,7 +828,7 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     step::window_plan(a.rows, a.seqs, a.heads, p.c.heads, p.c.dim, a.max_new, a.max_len, a.window, a.sinks, p.plan);
     const step::WindowPlan& pl = p.plan;
     uint8_t* ws = (uint8_t*)a.d_workspace;
-    const size_t cols = (size_t)pl.cols * kRows;
+    const size_t cols = (size_t)pl.cols * kCols;
     p.scores = a.d_scores ? Rows{a.d_scores, a.max_len, true} : Rows{(int32_t*)(ws + pl.at_scores), cols, false};
     p.exps = a.d_exp ? Rows{a.d_exp, a.max_len, true} : Rows{(int32_t*)(ws + pl.at_exp), cols, false};
     p.chunk_max = (int32_t*)(ws + pl.at_max);
@@ -795,27 +845,29 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     auto aligned = [&](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
     const bool vec = p.c.dim % 4 == 0 && ((p.c.page_stride | p.c.token_stride | p.c.head_stride) & 3) == 0 && aligned(p.c.d_k);
     p.q_vec = p.c.dim % 4 == 0 && a.q_stride % 4 == 0 && aligned(a.d_q);
-    const uint32_t along = pl.tiles * p.c.heads;
-    const size_t score_lds = (size_t)std::min(pl.dim64, kBlockSteps) * 12 * kRows * 16 + (size_t)pl.score_cols * kRows * 8;
-    if (vec) wit_window_scores_kernel<true><<<dim3(along, pl.score_chunks), 256, score_lds, s>>>(p);
-    else wit_window_scores_kernel<false><<<dim3(along, pl.score_chunks), 256, score_lds, s>>>(p);
-    GRAPE_LAUNCH_CHECK();
+    p.along = pl.tiles * p.c.heads;
+    p.factors = nullptr;
     if (pl.factors && a.bit_shift <= 20 && a.index_bits >= a.bit_shift) {
         p.factors = (double*)(ws + pl.at_factors);
         p.differs = (uint32_t*)(p.factors + 2 * kFactors);
-        wit_window_table_kernel<<<kTableGroups, kBlock, 0, s>>>(p);
-        GRAPE_LAUNCH_CHECK();
-        wit_window_exp_kernel<true><<<dim3(along, pl.exp_chunks), 256, 0, s>>>(p);
-    } else {
-        wit_window_exp_kernel<false><<<dim3(along, pl.exp_chunks), 256, 0, s>>>(p);
     }
+    const size_t score_lds = std::max<size_t>((size_t)std::min(pl.dim64, kBlockSteps) * 12 * kRows * 16 + (size_t)pl.score_cols * kCols * 8, p.factors ? 2 * kFactors * sizeof(double) : 0);
+    const dim3 scores(p.along + (p.factors ? kTableGroups : 0), pl.score_chunks), exps(p.along, pl.exp_chunks), values(p.along, pl.value_chunks * pl.groups);
+    if (vec && a.d_scores_rem) wit_window_scores_kernel<true, true><<<scores, 256, score_lds, s>>>(p);
+    else if (vec) wit_window_scores_kernel<true, false><<<scores, 256, score_lds, s>>>(p);
+    else if (a.d_scores_rem) wit_window_scores_kernel<false, true><<<scores, 256, score_lds, s>>>(p);
+    else wit_window_scores_kernel<false, false><<<scores, 256, score_lds, s>>>(p);
     GRAPE_LAUNCH_CHECK();
-    const dim3 values(along, pl.value_chunks * pl.groups);
+    if (p.factors && a.d_shifted) wit_window_exp_kernel<true, true><<<exps, 256, 0, s>>>(p);
+    else if (p.factors) wit_window_exp_kernel<true, false><<<exps, 256, 0, s>>>(p);
+    else if (a.d_shifted) wit_window_exp_kernel<false, true><<<exps, 256, 0, s>>>(p);
+    else wit_window_exp_kernel<false, false><<<exps, 256, 0, s>>>(p);
+    GRAPE_LAUNCH_CHECK();
     if (a.prob_scale <= ((int64_t)1 << 22)) wit_window_values_kernel<3><<<values, kValueThreads, 0, s>>>(p);
     else wit_window_values_kernel<4><<<values, kValueThreads, 0, s>>>(p);
     GRAPE_LAUNCH_CHECK();
     if (pl.value_chunks > 1) {
-        wit_window_join_kernel<<<dim3(along, pl.dim64), 256, 0, s>>>(p);
+        wit_window_join_kernel<<<dim3(p.along, pl.dim64, kRows / 4), 256, 0, s>>>(p);
         GRAPE_LAUNCH_CHECK();
     }
     return GRAPE_OK;
