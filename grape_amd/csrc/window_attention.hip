@@ -1,6 +1,7 @@
 // Attention of several new tokens a sequence over a paged cache - in their order, or behind a sliding window and a few first tokens -
 // with the tensors that a proof of it looks up.
 #include <algorithm>
+#include <type_traits>
 #include "token_device.hpp"
 #include "step_geometry.hpp"
 
@@ -288,7 +289,7 @@ __device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0
 // memory into the operand (lane l the elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16), the queries' digits from LDS.
 // Five accumulators become a sum in double precision, exact below 2^53, and below 2^50 the quotient of (y + s/2 + 1/2) / s needs no
 // second look: it is no nearer than 1 / (2 s) to a whole number, and the product with 1 / s off by at most 2^-52 of itself.
-template <bool VEC, bool REM>
+template <int STEPS, bool VEC, bool REM>
 __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ int32_t top[4][kRows];
@@ -326,21 +327,39 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
     }
     const uint32_t row_blocks = (w.R + 15) / 16;
     const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
-    v4i_t x[4];
-    auto fetch = [&](uint32_t tile, uint32_t s) {
-        const int32_t* k = keys + max(off[tile * kCols + 16 * w.wave + w.col], (int64_t)0) + 64 * s + 4 * w.kg;
-        if (VEC && 64 * s + 64 <= dim) {
+    const int64_t* my_off = off + 16 * w.wave + w.col;
+    const v4i_t* q_digits = reinterpret_cast<const v4i_t*>(lds) + w.kg * kRows + w.col;
+    // STEPS > 0: of the last step, quads that lie behind a head's end read its last one and count as zero
+    constexpr int S = STEPS ? STEPS : 1;
+    v4i_t x[S][4];
+    int32_t last_e[4], last_mask[4];
+    auto key_of = [&](uint32_t tile) { return keys + max(my_off[tile * kCols], (int64_t)0); };
+    auto fetch_step = [&](const int32_t* k, int s) {
+        if (s + 1 < STEPS) {
 #pragma unroll
-            for (uint32_t c = 0; c < 4; c++) x[c] = *reinterpret_cast<const v4i_t*>(k + 16 * c);
+            for (int c = 0; c < 4; c++) x[s][c] = *reinterpret_cast<const v4i_t*>(k + 64 * s + 16 * c + 4 * w.kg);
         } else {
 #pragma unroll
-            for (uint32_t c = 0; c < 4; c++) {
-                const uint32_t e = 64 * s + 16 * c + 4 * w.kg;
-                x[c] = elements(k + 16 * c - e, e, dim, VEC, 0);
-            }
+            for (int c = 0; c < 4; c++) x[s][c] = *reinterpret_cast<const v4i_t*>(k + last_e[c]);
         }
     };
-    fetch(0, 0);
+    auto fetch = [&](uint32_t tile, uint32_t s) {
+        const int32_t* k = key_of(tile);
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++) x[0][c] = elements(k, 64 * s + 16 * c + 4 * w.kg, dim, VEC, 0);
+    };
+    if constexpr (STEPS > 0) {
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++) {
+            const uint32_t e = 64 * (STEPS - 1) + 16 * c + 4 * w.kg;
+            last_e[c] = (int32_t)min(e, dim - 4);
+            last_mask[c] = e < dim ? -1 : 0;
+        }
+#pragma unroll
+        for (int s2 = 0; s2 < STEPS; s2++) fetch_step(key_of(0), s2);
+    } else {
+        fetch(0, 0);
+    }
     int32_t mx[2] = {INT32_MIN, INT32_MIN};
     uint32_t pos[2];
     size_t row[2];
@@ -360,32 +379,58 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
         for (int rb = 0; rb < 2; rb++)
 #pragma unroll
             for (int g = 0; g < 5; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
-#pragma unroll 1
-        for (uint32_t s = 0; s < steps; s++) {
-            if (blocks > 1 && s % kBlockSteps == 0) {
-                __syncthreads();
-                stage_queries(p, w, s / kBlockSteps, lds, over);
-                __syncthreads();
-            }
-            v4i_t kb[3];
+        auto planes_of = [&](const v4i_t (&y)[4], v4i_t (&kb)[3]) {
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 uint32_t pl[3];
-                three_planes(x[c], pl, k_over);
+                three_planes(y[c], pl, k_over);
 #pragma unroll
                 for (int k = 0; k < 3; k++) kb[k][c] = (int)pl[k];
             }
-            if (s + 1 < steps) fetch(tile, s + 1);
-            else if (tile + 1 < tiles) fetch(tile + 1, 0);
-            const v4i_t* qa = reinterpret_cast<const v4i_t*>(lds) + ((s % kBlockSteps) * 12 + w.kg) * kRows + w.col;
+        };
+        if constexpr (STEPS > 0) {
+            const int32_t* next = key_of(min(tile + 1, tiles - 1));
 #pragma unroll
-            for (uint32_t rb = 0; rb < 2; rb++) {
-                if (rb >= row_blocks) break;
+            for (int s = 0; s < STEPS; s++) {
+                v4i_t kb[3], f[3][2];
 #pragma unroll
-                for (int a = 0; a < 3; a++) {
-                    const v4i_t f = qa[a * 4 * kRows + 16 * rb];
+                for (int a = 0; a < 3; a++)
 #pragma unroll
-                    for (int k = 0; k < 3; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[k], f, acc[rb][a + k], 0, 0, 0);
+                    for (int rb = 0; rb < 2; rb++) f[a][rb] = q_digits[(s * 12 + a * 4) * kRows + 16 * rb];
+                if (s == STEPS - 1) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) x[s][c] &= last_mask[c];
+                }
+                planes_of(x[s], kb);
+                fetch_step(next, s);
+#pragma unroll
+                for (int a = 0; a < 3; a++)
+#pragma unroll
+                    for (int k = 0; k < 3; k++)
+#pragma unroll
+                        for (int rb = 0; rb < 2; rb++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[k], f[a][rb], acc[rb][a + k], 0, 0, 0);
+            }
+        } else {
+#pragma unroll 1
+            for (uint32_t s = 0; s < steps; s++) {
+                if (blocks > 1 && s % kBlockSteps == 0) {
+                    __syncthreads();
+                    stage_queries(p, w, s / kBlockSteps, lds, over);
+                    __syncthreads();
+                }
+                v4i_t kb[3];
+                planes_of(x[0], kb);
+                if (s + 1 < steps) fetch(tile, s + 1);
+                else if (tile + 1 < tiles) fetch(tile + 1, 0);
+#pragma unroll
+                for (uint32_t rb = 0; rb < 2; rb++) {
+                    if (rb >= row_blocks) break;
+#pragma unroll
+                    for (int a = 0; a < 3; a++) {
+                        const v4i_t f = q_digits[((s % kBlockSteps) * 12 + a * 4) * kRows + 16 * rb];
+#pragma unroll
+                        for (int k = 0; k < 3; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[k], f, acc[rb][a + k], 0, 0, 0);
+                    }
                 }
             }
         }
@@ -853,10 +898,18 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     }
     const size_t score_lds = std::max<size_t>((size_t)std::min(pl.dim64, kBlockSteps) * 12 * kRows * 16 + (size_t)pl.score_cols * kCols * 8, p.factors ? 2 * kFactors * sizeof(double) : 0);
     const dim3 scores(p.along + (p.factors ? kTableGroups : 0), pl.score_chunks), exps(p.along, pl.exp_chunks), values(p.along, pl.value_chunks * pl.groups);
-    if (vec && a.d_scores_rem) wit_window_scores_kernel<true, true><<<scores, 256, score_lds, s>>>(p);
-    else if (vec) wit_window_scores_kernel<true, false><<<scores, 256, score_lds, s>>>(p);
-    else if (a.d_scores_rem) wit_window_scores_kernel<false, true><<<scores, 256, score_lds, s>>>(p);
-    else wit_window_scores_kernel<false, false><<<scores, 256, score_lds, s>>>(p);
+    auto launch_scores = [&](auto kernel) { kernel<<<scores, 256, score_lds, s>>>(p); };
+    auto scores_of = [&](auto steps, auto by_four) {
+        if (a.d_scores_rem) launch_scores(wit_window_scores_kernel<decltype(steps)::value, decltype(by_four)::value, true>);
+        else launch_scores(wit_window_scores_kernel<decltype(steps)::value, decltype(by_four)::value, false>);
+    };
+    using std::integral_constant;
+    if (vec && pl.dim64 == 1) scores_of(integral_constant<int, 1>{}, std::true_type{});
+    else if (vec && pl.dim64 == 2) scores_of(integral_constant<int, 2>{}, std::true_type{});
+    else if (vec && pl.dim64 == 3) scores_of(integral_constant<int, 3>{}, std::true_type{});
+    else if (vec && pl.dim64 == 4) scores_of(integral_constant<int, 4>{}, std::true_type{});
+    else if (vec) scores_of(integral_constant<int, 0>{}, std::true_type{});
+    else scores_of(integral_constant<int, 0>{}, std::false_type{});
     GRAPE_LAUNCH_CHECK();
     if (p.factors && a.d_shifted) wit_window_exp_kernel<true, true><<<exps, 256, 0, s>>>(p);
     else if (p.factors) wit_window_exp_kernel<true, false><<<exps, 256, 0, s>>>(p);
