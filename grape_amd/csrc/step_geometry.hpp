@@ -174,9 +174,9 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
         const uint64_t want = beside >= workgroups ? 1 : workgroups / beside;
         return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, (cols + want - 1) / want));
     };
-    p.score_cols = chunk(4096, 8);
+    p.score_cols = chunk(p.dim64 > 8 ? 4096 : 768, 32);
     p.score_chunks = token::ceil_div(p.cols, p.score_cols);
-    p.exp_cols = 8;
+    p.exp_cols = std::max(4u, chunk(2048, 32));
     p.factors = rows_all * cols >= (uint64_t)1 << 16;
     p.exp_chunks = token::ceil_div(p.cols, p.exp_cols);
     p.groups = token::ceil_div(dim, kValueDims);
@@ -195,7 +195,18 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     p.bytes = p.at_part + (p.value_chunks > 1 ? (size_t)rows_all * p.value_chunks * dim * 8 : 0);
     return true;
 }
+// Single tokens go the way of attention_plan, with at most this many positions each.
+GRAPE_HD uint32_t seen_most(uint32_t max_len, uint32_t window, uint32_t sinks) {
+    return window && (uint64_t)window + sinks < max_len ? window + sinks : max_len;
+}
+inline bool single_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len, uint32_t window, uint32_t sinks, token::AttentionPlan& p) {
+    return rows && max_len && token::attention_plan(seqs, heads, cache_heads, dim, seen_most(max_len, window, sinks), p, max_len, rows);
+}
 inline size_t window_workspace(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_new, uint32_t max_len, uint32_t window, uint32_t sinks) {
+    if (max_new == 1) {
+        token::AttentionPlan one;
+        return single_plan(rows, seqs, heads, cache_heads, dim, max_len, window, sinks, one) ? one.bytes : 0;
+    }
     WindowPlan p;
     return window_plan(rows, seqs, heads, cache_heads, dim, max_new, max_len, window, sinks, p) ? p.bytes : 0;
 }
@@ -244,9 +255,13 @@ inline const char* refuse_window(const grape_wit_window_attention_args* a, const
     if (!a->seqs || !a->rows || !a->max_new) return nullptr;
     GRAPE_REFUSE(a->seqs > 65535, "at most 65535 sequences");
     GRAPE_REFUSE(!a->d_q || !a->d_starts || !a->d_lens || !a->d_exp_table || !a->d_out || !a->d_block_table, "d_q, d_starts, d_lens, d_exp_table, d_block_table or d_out is null");
+    GRAPE_REFUSE(a->rows > (uint32_t)1 << 24, "at most 2^24 rows");
     WindowPlan p;
-    GRAPE_REFUSE(!window_plan(a->rows, a->seqs, a->heads, c->heads, c->dim, a->max_new, a->max_len, a->window, a->sinks, p), "tensor too large");
-    GRAPE_REFUSE(a->workspace_bytes < p.bytes || !a->d_workspace, "the workspace is too small");
+    token::AttentionPlan one;
+    GRAPE_REFUSE(a->max_new == 1 ? !single_plan(a->rows, a->seqs, a->heads, c->heads, c->dim, a->max_len, a->window, a->sinks, one)
+                                 : !window_plan(a->rows, a->seqs, a->heads, c->heads, c->dim, a->max_new, a->max_len, a->window, a->sinks, p), "tensor too large");
+    const size_t need = a->max_new == 1 ? one.bytes : p.bytes;
+    GRAPE_REFUSE(a->workspace_bytes < need || (need && !a->d_workspace), "the workspace is too small");
     GRAPE_REFUSE((uintptr_t)a->d_workspace & 15, "the workspace must be 16-byte aligned");
     return nullptr;
 }

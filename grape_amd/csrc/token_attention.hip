@@ -1,6 +1,8 @@
 // Attention of one new token a sequence over a paged cache of keys and values, with the tensors that a proof of it looks up.
 #include <algorithm>
 #include "token_device.hpp"
+#include "step_geometry.hpp"
+#include "token_attention.hpp"
 
 namespace grape {
 
@@ -26,26 +28,52 @@ struct AttendArgs {
     unsigned long long* sums;    // [seqs][heads][exp chunks]
     int64_t* part;               // [seqs][heads][value chunks][dim]
     uint32_t* status;
+    const int32_t* d_starts;     // of a call with a window, see Span
+    uint32_t rows, window, sinks;
 };
 
-__device__ __forceinline__ bool span_of(const AttendArgs& p, uint32_t b, uint32_t& lo, uint32_t& hi) {
-    return token::live_span(p.a.d_lens[b], p.a.d_first ? p.a.d_first[b] : 0, p.a.max_len, p.a.table_stride, p.c.page_size, lo, hi);
-}
+// The positions lo <= t < hi that a sequence attends to, and its row.  With a window (WINDOW) and first tokens that stay visible the
+// positions are numbered as if these stood right before the window: the numbers lo .. first - 1 are the positions 0 .. first - 1 - gap.
+template <bool WINDOW>
+struct Span {
+    uint32_t lo, hi, first = 0, gap = 0, row;
+    bool fits, there = true;
+    __device__ __forceinline__ Span() {}
+    __device__ __forceinline__ Span(const AttendArgs& p, uint32_t b) {
+        if constexpr (WINDOW) {
+            uint32_t n, pos;
+            const int32_t s = p.d_starts[b];
+            fits = step::new_tokens(s, p.d_starts[b + 1], p.a.d_lens[b], p.rows, 1, p.a.max_len, (uint64_t)p.a.table_stride * p.c.page_size, n, pos);
+            there = n == 1;
+            row = there ? (uint32_t)s : 0;
+            hi = there ? pos + 1 : 0;
+            first = p.window && hi > p.window ? hi - p.window : 0;
+            lo = gap = first - min(p.sinks, first);
+        } else {
+            fits = token::live_span(p.a.d_lens[b], p.a.d_first ? p.a.d_first[b] : 0, p.a.max_len, p.a.table_stride, p.c.page_size, lo, hi);
+            row = b;
+        }
+    }
+    __device__ __forceinline__ uint32_t at(uint32_t t) const { return WINDOW && t < first ? t - gap : t; }
+};
 
 // The sequence, the chunk of `size` positions and the positions that are number `index` when the sequences' chunks are counted, one
 // at least of each; false where there are fewer.  Where lengths differ, many of max_len's chunks are of no sequence: counted, their
 // workgroups come last, when all others are under way (64 sequences of up to 2048, 8 heads of 128: 147 us a call and not 156, 24 with
 // a window of 256 of up to 5000 29 and not 39).  It costs each workgroup a wait for the lengths (64 sequences of 1024 each: 153 and
 // not 149), so that few sequences keep the plain order.  All lanes of a wave together.
-__device__ __forceinline__ bool find_chunk(const AttendArgs& p, uint32_t index, uint32_t size, uint32_t& b, uint32_t& chunk, uint32_t& lo, uint32_t& hi, bool& fits) {
+template <bool WINDOW>
+__device__ __forceinline__ bool find_chunk(const AttendArgs& p, uint32_t index, uint32_t size, uint32_t& b, uint32_t& chunk, Span<WINDOW>& span) {
     const uint32_t lane = threadIdx.x & 63u;
     uint32_t before = 0;
     for (uint32_t base = 0; base < p.a.seqs; base += 64) {
-        uint32_t l = 0, h = 0, n = 0;
-        bool ok = true;
+        uint32_t n = 0;
+        Span<WINDOW> mine;
+        mine.lo = mine.hi = mine.row = 0;
+        mine.fits = true;
         if (base + lane < p.a.seqs) {
-            ok = span_of(p, base + lane, l, h);
-            n = l < h ? (h - l - 1) / size + 1 : 1;
+            mine = Span<WINDOW>(p, base + lane);
+            n = mine.lo < mine.hi ? (mine.hi - mine.lo - 1) / size + 1 : 1;
         }
         uint32_t sum = n;
 #pragma unroll
@@ -56,11 +84,19 @@ __device__ __forceinline__ bool find_chunk(const AttendArgs& p, uint32_t index, 
         const unsigned long long past = __ballot(before + sum > index);
         if (past) {
             const int at = __ffsll(past) - 1;
+            auto of = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, at); };
             b = base + (uint32_t)at;
-            chunk = index - before - (uint32_t)__builtin_amdgcn_readlane((int)(sum - n), at);
-            lo = (uint32_t)__builtin_amdgcn_readlane((int)l, at);
-            hi = (uint32_t)__builtin_amdgcn_readlane((int)h, at);
-            fits = __builtin_amdgcn_readlane((int)ok, at) != 0;
+            chunk = index - before - of(sum - n);
+            span.lo = of(mine.lo);
+            span.hi = of(mine.hi);
+            span.fits = of(mine.fits) != 0;
+            span.row = b;
+            if constexpr (WINDOW) {
+                span.first = of(mine.first);
+                span.gap = of(mine.gap);
+                span.row = of(mine.row);
+                span.there = of(mine.there) != 0;
+            }
             return true;
         }
         before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
@@ -82,13 +118,15 @@ struct Offsets {
         t = (uint32_t)start + threadIdx.x;
         if (early && threadIdx.x < most && start + threadIdx.x < p.a.max_len && p.page(t) < p.a.table_stride) page = load(p, b, t);
     }
-    __device__ __forceinline__ bool store(const AttendArgs& p, uint32_t b, uint32_t t0, uint32_t n, uint32_t filled, int64_t* off) const {
+    template <bool WINDOW>
+    __device__ __forceinline__ bool store(const AttendArgs& p, uint32_t b, const Span<WINDOW>& span, uint32_t t0, uint32_t n, uint32_t filled, int64_t* off) const {
         bool outside = false;
         for (uint32_t i = threadIdx.x; i < filled; i += blockDim.x) {
             int64_t o = -1;
             if (i < n) {
-                const int32_t pg = early && i == threadIdx.x ? page : load(p, b, t0 + i);
-                o = token::token_offset(p.c, pg, t0 + i - p.page(t0 + i) * p.c.page_size);
+                const uint32_t pos = span.at(t0 + i);
+                const int32_t pg = early && i == threadIdx.x ? page : load(p, b, pos);
+                o = token::token_offset(p.c, pg, pos - p.page(pos) * p.c.page_size);
                 outside |= o < 0;
             }
             off[i] = o;
@@ -112,20 +150,24 @@ __device__ __forceinline__ v2i_t load2(const int32_t* x, uint32_t at, uint32_t n
 
 // The query heads of a workgroup: R heads from h0 of sequence b, which read the cache's head kv.
 struct Tile {
-    uint32_t b, kv, h0, R;
+    uint32_t b, kv, h0, R, q_row;
     size_t row0;                 // of the rows [seqs][heads]
     uint32_t lane, wave, col, kg;
-    __device__ __forceinline__ Tile(const AttendArgs& p, uint32_t b_, uint32_t head_tile) : b(b_) {
+    __device__ __forceinline__ Tile(const AttendArgs& p, uint32_t b_, uint32_t head_tile, uint32_t row = 0) : b(b_) {
         const uint32_t each = p.a.heads / p.c.heads;
         kv = head_tile / p.plan.tiles;
         const uint32_t tile = head_tile - kv * p.plan.tiles;
         h0 = kv * each + tile * p.plan.rows;
         R = min(p.plan.rows, each - tile * p.plan.rows);
-        row0 = (size_t)b * p.a.heads + h0;
+        place(p, row);
         lane = threadIdx.x & 63u;
         wave = threadIdx.x >> 6;
         col = lane & 15u;
         kg = lane >> 4;
+    }
+    __device__ __forceinline__ void place(const AttendArgs& p, uint32_t row) {
+        q_row = row;
+        row0 = (size_t)row * p.a.heads + h0;
     }
     // Row m of a product is query head 4 (m % 4) + m / 4: register i of lane l then holds head 4 i + l / 16 at column l % 16, and
     // four heads need one register of every lane.  Rows past the last head repeat it; nothing of them is kept.
@@ -141,7 +183,7 @@ struct Queries {
     int32_t q4[4];
     __device__ __forceinline__ void load(const AttendArgs& p, const Tile& w, uint32_t i) {
         const uint32_t steps = p.plan.dim64, r = i / (steps * 16), quad = i - r * (steps * 16);
-        const int32_t* q = p.a.d_q + w.b * p.a.q_stride + (size_t)(w.h0 + r) * p.c.dim;
+        const int32_t* q = p.a.d_q + w.q_row * p.a.q_stride + (size_t)(w.h0 + r) * p.c.dim;
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) q4[j] = 4 * quad + j < p.c.dim ? q[4 * quad + j] : 0;
     }
@@ -236,19 +278,20 @@ __device__ __forceinline__ void score_products(const AttendArgs& p, const Tile& 
 }
 
 // Such sums, [row][stride] in LDS, rescaled and written; the largest score of each row goes to largest(r, max).
-template <class F>
-__device__ __forceinline__ void score_rows(const AttendArgs& p, const Tile& w, uint32_t t0, uint32_t n, const int64_t* off, const uint64_t* sums, uint32_t stride,
+template <bool WINDOW, class F>
+__device__ __forceinline__ void score_rows(const AttendArgs& p, const Tile& w, const Span<WINDOW>& span, uint32_t t0, uint32_t n, const int64_t* off, const uint64_t* sums, uint32_t stride,
                                            const unsigned long long* q_sum, uint32_t& bad, F largest) {
     for (uint32_t r = w.wave; r < w.R; r += 4) {
-        const size_t o = (w.row0 + r) * p.a.max_len + t0;
+        const size_t o = (w.row0 + r) * p.a.max_len;
         const uint64_t more = (uint64_t)kCacheOffset * q_sum[r];
         int32_t mx = INT32_MIN;
         for (uint32_t i = w.lane; i < n; i += 64) {
             const int64_t y = off[i] < 0 ? 0 : (int64_t)(sums[r * stride + i] + more);          // a page outside: zero
+            const size_t to = o + span.at(t0 + i);
             int32_t q, rem;
             p.qk.apply(y, q, rem, bad);
-            p.a.d_scores[o + i] = q;
-            if (p.a.d_scores_rem) p.a.d_scores_rem[o + i] = rem;
+            p.a.d_scores[to] = q;
+            if (p.a.d_scores_rem) p.a.d_scores_rem[to] = rem;
             mx = max(mx, q);
         }
 #pragma unroll
@@ -260,13 +303,14 @@ __device__ __forceinline__ void score_rows(const AttendArgs& p, const Tile& w, u
 // Exponentials of the scores t0 + i of row `row`, i = from, from + step, ... below n, and their sum.  Bound by the gathers'
 // latency: eight are under way a thread.
 constexpr uint32_t kExpAhead = 8;
-__device__ __forceinline__ unsigned long long exponentials(const AttendArgs& p, size_t row, uint32_t t0, uint32_t from, uint32_t step, uint32_t n, int32_t mx, uint32_t& bad) {
-    const size_t o = row * p.a.max_len + t0;
+template <bool WINDOW>
+__device__ __forceinline__ unsigned long long exponentials(const AttendArgs& p, size_t row, const Span<WINDOW>& span, uint32_t t0, uint32_t from, uint32_t step, uint32_t n, int32_t mx, uint32_t& bad) {
+    const size_t o = row * p.a.max_len;
     unsigned long long sum = 0;
     for (uint32_t t = from; t < n; t += step * kExpAhead) {
         int32_t x[kExpAhead], e[kExpAhead];
 #pragma unroll
-        for (uint32_t j = 0; j < kExpAhead; j++) x[j] = t + j * step < n ? p.a.d_scores[o + t + j * step] : mx;
+        for (uint32_t j = 0; j < kExpAhead; j++) x[j] = t + j * step < n ? p.a.d_scores[o + span.at(t0 + t + j * step)] : mx;
 #pragma unroll
         for (uint32_t j = 0; j < kExpAhead; j++) {
             const int64_t idx = (int64_t)x[j] - mx + (((int64_t)1 << p.a.bit_shift) - 1);
@@ -279,8 +323,9 @@ __device__ __forceinline__ unsigned long long exponentials(const AttendArgs& p, 
             const uint32_t i = t + j * step;
             if (i >= n) break;
             if (e[j] < 0) bad |= (uint32_t)kWitSum;
-            p.a.d_exp[o + i] = e[j];
-            if (p.a.d_shifted) p.a.d_shifted[o + i] = (int32_t)((int64_t)x[j] - mx);
+            const size_t to = o + span.at(t0 + i);
+            p.a.d_exp[to] = e[j];
+            if (p.a.d_shifted) p.a.d_shifted[to] = (int32_t)((int64_t)x[j] - mx);
             sum += (unsigned long long)(e[j] < 0 ? 0 : e[j]);
         }
     }
@@ -310,10 +355,10 @@ struct RowThreads {
 // Probabilities of this thread's positions of its row, from load(position), its exponential; written if `write`, and their digits
 // in LDS: [step of 32][plane][lane group][row], operands of 8 positions each, zero up to a whole number of 32 positions and for
 // pages outside the cache.  Returns the sum of the probabilities that the values are multiplied with.
-template <int PP, uint32_t AHEAD, class F>          // planes of the probabilities, positions under way a thread
-__device__ __forceinline__ unsigned long long probabilities(const AttendArgs& p, const Tile& w, const RowThreads& row, uint32_t t0, uint32_t n, const int64_t* off,
+template <int PP, uint32_t AHEAD, bool WINDOW, class F>          // planes of the probabilities, positions under way a thread
+__device__ __forceinline__ unsigned long long probabilities(const AttendArgs& p, const Tile& w, const RowThreads& row, const Span<WINDOW>& span, uint32_t t0, uint32_t n, const int64_t* off,
                                                             unsigned long long sum, bool write, uint32_t* digits, uint32_t& bad, F load) {
-    const size_t o = (w.row0 + row.r) * p.a.max_len + t0;
+    const size_t o = (w.row0 + row.r) * p.a.max_len;
     const double inv = 1.0 / (double)sum;
     const uint32_t filled = (n + 31) / 32 * 32;
     unsigned long long all = 0;
@@ -330,8 +375,9 @@ __device__ __forceinline__ unsigned long long probabilities(const AttendArgs& p,
             if (i < n) {
                 pr = probability(e[a], (uint64_t)p.a.prob_scale, sum, inv);
                 if (write) {
-                    if (p.a.d_prob) p.a.d_prob[o + i] = (int32_t)pr;
-                    if (p.a.d_query) store_sum(&p.a.d_query[o + i], lookup_query(e[a], p.a.prob_scale, sum, pr), bad);
+                    const size_t to = o + span.at(t0 + i);
+                    if (p.a.d_prob) p.a.d_prob[to] = (int32_t)pr;
+                    if (p.a.d_query) store_sum(&p.a.d_query[to], lookup_query(e[a], p.a.prob_scale, sum, pr), bad);
                 }
                 if (off[i] < 0) pr = 0;
             }
@@ -435,33 +481,34 @@ __device__ __forceinline__ void write_empty(const AttendArgs& p, const Tile& w, 
 // ---- the launches over chunks
 // Scores of `rows` query heads with a chunk of the keys.  Bound by reading the keys: 131072 positions of 8 heads of 128 for 32 query
 // heads, 570 MB with what is written, 121 us, 4.7 TB/s, as a copy.
-template <bool VEC>
+template <bool VEC, bool WINDOW>
 __global__ void __launch_bounds__(256, 4) wit_attend_scores_kernel(AttendArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ unsigned long long q_sum[16];
     __shared__ uint32_t over_any;
     const uint32_t per_chunk = p.c.heads * p.plan.tiles, index = blockIdx.x / per_chunk, within = blockIdx.x - index * per_chunk;
-    uint32_t b = blockIdx.y, chunk = index, lo, hi, bad = 0;
-    bool fits;
-    if (p.plan.counted && !find_chunk(p, index, p.plan.score_chunk, b, chunk, lo, hi, fits)) return;
-    const Tile w(p, b, within);
+    uint32_t b = blockIdx.y, chunk = index, bad = 0;
+    Span<WINDOW> span;
+    if (p.plan.counted && !find_chunk(p, index, p.plan.score_chunk, b, chunk, span)) return;
+    if (WINDOW && !p.plan.counted) span = Span<WINDOW>(p, b);
+    Tile w(p, b, within, WINDOW ? span.row : b);
     // what does not depend on the sequence's length is requested beside it
     Queries queries;
     queries.first(p, w);
     Offsets offsets;
-    offsets.request(p, w.b, (uint64_t)chunk * p.plan.score_chunk, p.plan.score_chunk);
-    if (!p.plan.counted) fits = span_of(p, w.b, lo, hi);
-    if (!fits && chunk == 0 && within == 0 && threadIdx.x == 0) atomicOr(p.status, (uint32_t)kWitIndex);
-    const uint64_t start = (uint64_t)lo + (uint64_t)chunk * p.plan.score_chunk;
-    if (start >= hi) return;
-    const uint32_t t0 = (uint32_t)start, n = min(hi - t0, p.plan.score_chunk);
+    if constexpr (!WINDOW) offsets.request(p, w.b, (uint64_t)chunk * p.plan.score_chunk, p.plan.score_chunk);
+    if (!WINDOW && !p.plan.counted) span = Span<WINDOW>(p, b);
+    if (!span.fits && chunk == 0 && within == 0 && threadIdx.x == 0) atomicOr(p.status, (uint32_t)kWitIndex);
+    const uint64_t start = (uint64_t)span.lo + (uint64_t)chunk * p.plan.score_chunk;
+    if (start >= span.hi) return;
+    const uint32_t t0 = (uint32_t)start, n = min(span.hi - t0, p.plan.score_chunk);
     if (threadIdx.x < 16) q_sum[threadIdx.x] = 0;
     if (threadIdx.x == 0) over_any = 0;
     // behind the digits: the positions' offsets and the scores' 64-bit sums, so that nothing but the keys is read or written on
     // the way (waiting for any other load or store would wait for all keys requested before it)
     int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)5 * 16 * p.plan.dim64 * p.plan.rows);
     uint64_t* sums = reinterpret_cast<uint64_t*>(off + p.plan.score_chunk);
-    if (offsets.store(p, w.b, t0, n, n, off)) bad |= (uint32_t)kWitIndex;
+    if (offsets.store(p, w.b, span, t0, n, n, off)) bad |= (uint32_t)kWitIndex;
     const bool apart = p.plan.score_apart;
     if (apart)
         for (uint32_t i = threadIdx.x; i < w.R * p.plan.score_chunk; i += 256) sums[i] = 0;
@@ -475,7 +522,7 @@ __global__ void __launch_bounds__(256, 4) wit_attend_scores_kernel(AttendArgs p)
         else *sum = y;
     });
     __syncthreads();
-    score_rows(p, w, t0, n, off, sums, p.plan.score_chunk, q_sum, bad,
+    score_rows(p, w, span, t0, n, off, sums, p.plan.score_chunk, q_sum, bad,
                [&](uint32_t r, int32_t mx) { p.chunk_max[(w.row0 + r) * p.plan.score_chunks + chunk] = mx; });
     if (bad) atomicOr(p.status, bad);
 }
@@ -496,19 +543,20 @@ __device__ __forceinline__ T block_all(T v, F f) {
 
 // Exponentials of a chunk of one row, and their sum.  Bound by the gathers: 32 rows of 131072, 31 us, 135 a nanosecond from a table
 // of 4 MB that the L2 of each die shares with the scores.
+template <bool WINDOW>
 __global__ void __launch_bounds__(kBlock) wit_attend_exp_kernel(AttendArgs p) {
     const uint32_t b = blockIdx.z;
-    const size_t row = (size_t)b * p.a.heads + blockIdx.y;
-    uint32_t lo, hi, bad = 0;
-    span_of(p, b, lo, hi);
-    const uint64_t start = (uint64_t)lo + (uint64_t)blockIdx.x * p.plan.exp_chunk;
-    if (start >= hi) return;
-    const uint32_t t0 = (uint32_t)start, n = min(hi - t0, p.plan.exp_chunk), parts = (hi - lo - 1) / p.plan.score_chunk + 1;
+    const Span<WINDOW> span(p, b);
+    const size_t row = (size_t)span.row * p.a.heads + blockIdx.y;
+    uint32_t bad = 0;
+    const uint64_t start = (uint64_t)span.lo + (uint64_t)blockIdx.x * p.plan.exp_chunk;
+    if (start >= span.hi) return;
+    const uint32_t t0 = (uint32_t)start, n = min(span.hi - t0, p.plan.exp_chunk), parts = (span.hi - span.lo - 1) / p.plan.score_chunk + 1;
     int32_t mx = INT32_MIN;
     for (uint32_t i = threadIdx.x; i < parts; i += kBlock) mx = max(mx, p.chunk_max[row * p.plan.score_chunks + i]);
     mx = block_all(mx, [](int32_t x, int32_t y) { return max(x, y); });
     if (blockIdx.x == 0 && threadIdx.x == 0 && p.a.d_max) p.a.d_max[row] = mx;
-    unsigned long long sum = exponentials(p, row, t0, threadIdx.x, kBlock, n, mx, bad);
+    unsigned long long sum = exponentials(p, row, span, t0, threadIdx.x, kBlock, n, mx, bad);
     sum = block_all(sum, [](unsigned long long x, unsigned long long y) { return x + y; });
     if (threadIdx.x == 0) p.sums[row * p.plan.exp_chunks + blockIdx.x] = sum;
     if (bad) atomicOr(p.status, bad);
@@ -518,19 +566,24 @@ __global__ void __launch_bounds__(kBlock) wit_attend_exp_kernel(AttendArgs p) {
 // The waves take different blocks of 32 elements, or every second or fourth step.  Bound by reading the values: the
 // 131072 positions' 587 MB with probabilities and queries in 128 us, 4.6 TB/s.
 constexpr uint32_t kProbAhead = 4;
-template <bool VEC, int PP>
+template <bool VEC, int PP, bool WINDOW>
 __global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ unsigned long long e_sum[16], p_sum[16];
     const uint32_t per_chunk = p.c.heads * p.plan.tiles * p.plan.groups, index = blockIdx.x / per_chunk, within = blockIdx.x - index * per_chunk;
     const uint32_t group = within % p.plan.groups;
-    uint32_t b = blockIdx.y, chunk = index, lo, hi, bad = 0;
-    bool fits;
-    if (p.plan.counted && !find_chunk(p, index, p.plan.value_chunk, b, chunk, lo, hi, fits)) return;
-    const Tile w(p, b, within / p.plan.groups);
+    uint32_t b = blockIdx.y, chunk = index, bad = 0;
+    Span<WINDOW> span;
+    if (p.plan.counted && !find_chunk(p, index, p.plan.value_chunk, b, chunk, span)) return;
+    Tile w(p, b, within / p.plan.groups, b);
     Offsets offsets;
-    offsets.request(p, w.b, (uint64_t)chunk * p.plan.value_chunk, p.plan.value_chunk);
-    if (!p.plan.counted) span_of(p, w.b, lo, hi);
+    if constexpr (!WINDOW) offsets.request(p, w.b, (uint64_t)chunk * p.plan.value_chunk, p.plan.value_chunk);
+    if (!p.plan.counted) span = Span<WINDOW>(p, b);
+    if constexpr (WINDOW) {
+        if (!span.there) return;
+        w.place(p, span.row);
+    }
+    const uint32_t lo = span.lo, hi = span.hi;
     const uint64_t start = (uint64_t)lo + (uint64_t)chunk * p.plan.value_chunk;
     const bool direct = hi - lo <= p.plan.value_chunk;          // the whole row is this workgroup's
     const uint32_t e0 = group * p.plan.blocks * 32, width = p.plan.blocks * 32, dim = p.c.dim;
@@ -541,7 +594,7 @@ __global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p)
     const uint32_t t0 = (uint32_t)start, n = min(hi - t0, p.plan.value_chunk);
     int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)p.plan.value_chunk * w.R * PP / 4);        // behind the digits
     if (threadIdx.x < 16) e_sum[threadIdx.x] = p_sum[threadIdx.x] = 0;
-    offsets.store(p, w.b, t0, n, (n + 63) / 64 * 64, off);
+    offsets.store(p, w.b, span, t0, n, (n + 63) / 64 * 64, off);
     __syncthreads();
     const uint32_t block = w.wave % p.plan.blocks, apart = 4 / p.plan.blocks, e = e0 + 32 * block, halves = e < dim ? (n + 31) / 32 : 0, s = w.wave / p.plan.blocks;
     ValueProducts<VEC, PP> products;
@@ -563,8 +616,8 @@ __global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p)
             sum = 1;
         }
         if (chunk == 0 && group == 0 && row.from == 0 && p.a.d_sum) store_sum(&p.a.d_sum[at], sum, bad);
-        const int32_t* exps = p.a.d_exp + at * p.a.max_len + t0;
-        const unsigned long long mine = probabilities<PP, kProbAhead>(p, w, row, t0, n, off, sum, group == 0, lds, bad, [&](uint32_t i) { return (uint32_t)max(exps[i], 0); });
+        const int32_t* exps = p.a.d_exp + at * p.a.max_len;
+        const unsigned long long mine = probabilities<PP, kProbAhead>(p, w, row, span, t0, n, off, sum, group == 0, lds, bad, [&](uint32_t i) { return (uint32_t)max(exps[span.at(t0 + i)], 0); });
         if (row.leads) atomicAdd(&p_sum[row.r], mine);
     }
     __syncthreads();
@@ -588,12 +641,14 @@ __global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p)
 // The chunks' partial sums of 64 elements of one row.  A wave for each four chunks, at most sixteen: with few of them the rows are
 // many, and more waves would only stand in line (64 sequences of 32 heads of 128 and 8 chunks: 5.2 us, with sixteen waves 11.2).
 constexpr uint32_t kJoinThreads = 1024;
+template <bool WINDOW>
 __global__ void __launch_bounds__(kJoinThreads) wit_attend_join_kernel(AttendArgs p) {
     __shared__ int64_t sh[kJoinThreads];
     const uint32_t h = blockIdx.y, b = blockIdx.z, e = blockIdx.x * 64 + (threadIdx.x & 63u), dim = p.c.dim;
-    const size_t row = (size_t)b * p.a.heads + h;
-    uint32_t lo, hi, bad = 0;
-    span_of(p, b, lo, hi);
+    const Span<WINDOW> span(p, b);
+    const size_t row = (size_t)span.row * p.a.heads + h;
+    const uint32_t lo = span.lo, hi = span.hi;
+    uint32_t bad = 0;
     if (hi - lo <= p.plan.value_chunk) return;
     const uint32_t parts = (hi - lo - 1) / p.plan.value_chunk + 1;
     const uint32_t waves = blockDim.x >> 6;
@@ -616,22 +671,31 @@ __global__ void __launch_bounds__(kJoinThreads) wit_attend_join_kernel(AttendArg
 // once - so eight waves share the positions, and the softmax takes one position a thread in short loops.  37 positions of 32 heads of 128:
 // 10.2 us.
 constexpr uint32_t kWholeWaves = 8, kWholeThreads = 64 * kWholeWaves;
-template <bool VEC, int PP>
+template <bool VEC, int PP, bool WINDOW>
 __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(AttendArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ unsigned long long q_sum[16], e_sum[16], p_sum[16];
     __shared__ int32_t row_max[16];
     __shared__ uint32_t over_any;
     constexpr uint32_t C = token::kWholeMost;
-    const Tile w(p, blockIdx.y, blockIdx.x);
+    Tile w(p, blockIdx.y, blockIdx.x, blockIdx.y);
     const uint32_t dim = p.c.dim;
-    uint32_t lo, hi, bad = 0;
+    uint32_t bad = 0;
+    Span<WINDOW> span;
+    if constexpr (WINDOW) {
+        span = Span<WINDOW>(p, w.b);
+        w.place(p, span.row);
+    }
     Queries queries;
     queries.first(p, w);
     Offsets offsets;
-    offsets.request(p, w.b, 0, C);
-    const bool fits = span_of(p, w.b, lo, hi);
-    if (!fits && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.status, (uint32_t)kWitIndex);
+    if constexpr (!WINDOW) {
+        offsets.request(p, w.b, 0, C);
+        span = Span<WINDOW>(p, w.b);
+    }
+    const uint32_t lo = span.lo, hi = span.hi;
+    if (!span.fits && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.status, (uint32_t)kWitIndex);
+    if (WINDOW && !span.there) return;
     if (lo == hi) {
         write_empty(p, w, 0, dim, true);
         return;
@@ -648,7 +712,7 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
     if (threadIdx.x == 0) over_any = 0;
     __syncthreads();
     const uint32_t filled = (n + 31) / 32 * 32;
-    if (offsets.store(p, w.b, lo, n, filled, off)) bad |= (uint32_t)kWitIndex;
+    if (offsets.store(p, w.b, span, lo, n, filled, off)) bad |= (uint32_t)kWitIndex;
     queries.store(p, w, digits, q_sum, &over_any);
     __syncthreads();
     score_products<VEC, kWholeWaves>(p, w, n, off, digits, over_any != 0, false, [&](uint32_t r, uint32_t i, bool there, uint64_t y) {
@@ -662,7 +726,7 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
     const RowThreads row(kWholeThreads, w.R);
     const uint32_t r = row.r, from = row.from, each = row.each;
     const bool mine = row.mine, leads = row.leads;
-    const size_t o = (w.row0 + min(r, w.R - 1)) * p.a.max_len + lo;
+    const size_t o = (w.row0 + min(r, w.R - 1)) * p.a.max_len;
     if (mine) {
         const uint64_t more = (uint64_t)kCacheOffset * q_sum[r];
         int32_t mx = INT32_MIN;
@@ -670,8 +734,9 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
         for (uint32_t i = from; i < n; i += each) {
             int32_t q, rem;
             p.qk.apply(off[i] < 0 ? 0 : (int64_t)(total[r * C + i] + more), q, rem, bad);          // a page outside the cache: zero
-            if (p.a.d_scores) p.a.d_scores[o + i] = q;
-            if (p.a.d_scores_rem) p.a.d_scores_rem[o + i] = rem;
+            const size_t to = o + span.at(lo + i);
+            if (p.a.d_scores) p.a.d_scores[to] = q;
+            if (p.a.d_scores_rem) p.a.d_scores_rem[to] = rem;
             scores[r * C + i] = (uint32_t)q;
             mx = max(mx, q);
         }
@@ -699,8 +764,9 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
             for (uint32_t a = 0; a < 4; a++) {
                 const uint32_t i = first + a * each;
                 if (i >= n) break;
-                if (p.a.d_shifted) p.a.d_shifted[o + i] = (int32_t)((int64_t)x[a] - mx);
-                if (p.a.d_exp) p.a.d_exp[o + i] = e[a];
+                const size_t to = o + span.at(lo + i);
+                if (p.a.d_shifted) p.a.d_shifted[to] = (int32_t)((int64_t)x[a] - mx);
+                if (p.a.d_exp) p.a.d_exp[to] = e[a];
                 if (e[a] < 0) bad |= (uint32_t)kWitSum;
                 e[a] = max(e[a], 0);
                 scores[r * C + i] = (uint32_t)e[a];
@@ -721,7 +787,7 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
             if (p.a.d_max) p.a.d_max[w.row0 + r] = row_max[r];
             if (p.a.d_sum) store_sum(&p.a.d_sum[w.row0 + r], sum, bad);
         }
-        const unsigned long long all = probabilities<PP, 1>(p, w, row, lo, n, off, sum, true, digits, bad, [&](uint32_t i) { return scores[r * C + i]; });
+        const unsigned long long all = probabilities<PP, 1>(p, w, row, span, lo, n, off, sum, true, digits, bad, [&](uint32_t i) { return scores[r * C + i]; });
         if (leads) atomicAdd(&p_sum[r], all);
     }
     __syncthreads();
@@ -739,25 +805,10 @@ __global__ void __launch_bounds__(kWholeThreads, 4) wit_attend_whole_kernel(Atte
     if (bad) atomicOr(p.status, bad);
 }
 
-}  // namespace grape
-
-using namespace grape;
-
-extern "C" {
-
-size_t grape_wit_paged_attention_workspace(uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len) {
-    return token::attention_workspace(seqs, heads, cache_heads, dim, max_len);
-}
-
-int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_wit_cache* cache, grape_stream_t st) {
-    GRAPE_REQUIRE(initialised(), "grape_init has not been called");
-    GRAPE_REFUSED_IF(token::refuse_attention(args, cache));
-    if (args->seqs == 0) return GRAPE_OK;
-    AttendArgs p;
-    p.a = *args;
-    p.c = *cache;
+// The launches of a call whose plan and arguments are set.
+template <bool WINDOW>
+static int attend(AttendArgs& p, grape_stream_t st) {
     grape_wit_attention_args& a = p.a;
-    token::attention_plan(a.seqs, a.heads, p.c.heads, p.c.dim, a.max_len, p.plan);
     const token::AttentionPlan& pl = p.plan;
     uint8_t* ws = (uint8_t*)a.d_workspace;
     if (!pl.whole && !a.d_scores) a.d_scores = (int32_t*)(ws + pl.at_scores);
@@ -776,10 +827,10 @@ int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_
     const int planes = a.prob_scale <= ((int64_t)1 << 22) ? 3 : 4;
     if (pl.whole) {
         const dim3 grid(p.c.heads * pl.tiles, a.seqs);
-        if (vec && planes == 3) wit_attend_whole_kernel<true, 3><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
-        else if (vec) wit_attend_whole_kernel<true, 4><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
-        else if (planes == 3) wit_attend_whole_kernel<false, 3><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
-        else wit_attend_whole_kernel<false, 4><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
+        if (vec && planes == 3) wit_attend_whole_kernel<true, 3, WINDOW><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
+        else if (vec) wit_attend_whole_kernel<true, 4, WINDOW><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
+        else if (planes == 3) wit_attend_whole_kernel<false, 3, WINDOW><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
+        else wit_attend_whole_kernel<false, 4, WINDOW><<<grid, kWholeThreads, pl.whole_lds, s>>>(p);
         GRAPE_LAUNCH_CHECK();
         return GRAPE_OK;
     }
@@ -789,24 +840,59 @@ int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_
     const uint32_t head_tiles = p.c.heads * pl.tiles;
     const uint32_t along = pl.counted ? a.seqs : 1, across = pl.counted ? 1 : a.seqs;
     const dim3 score_grid(std::max(1u, pl.score_chunks) * head_tiles * along, across), value_grid(std::max(1u, pl.value_chunks) * head_tiles * pl.groups * along, across);
-    if (vec) wit_attend_scores_kernel<true><<<score_grid, 256, score_lds, s>>>(p);
-    else wit_attend_scores_kernel<false><<<score_grid, 256, score_lds, s>>>(p);
+    if (vec) wit_attend_scores_kernel<true, WINDOW><<<score_grid, 256, score_lds, s>>>(p);
+    else wit_attend_scores_kernel<false, WINDOW><<<score_grid, 256, score_lds, s>>>(p);
     GRAPE_LAUNCH_CHECK();
     if (a.max_len) {
-        wit_attend_exp_kernel<<<dim3(pl.exp_chunks, a.heads, a.seqs), kBlock, 0, s>>>(p);
+        wit_attend_exp_kernel<WINDOW><<<dim3(pl.exp_chunks, a.heads, a.seqs), kBlock, 0, s>>>(p);
         GRAPE_LAUNCH_CHECK();
     }
-    if (vec && planes == 3) wit_attend_values_kernel<true, 3><<<value_grid, 256, value_lds, s>>>(p);
-    else if (vec) wit_attend_values_kernel<true, 4><<<value_grid, 256, value_lds, s>>>(p);
-    else if (planes == 3) wit_attend_values_kernel<false, 3><<<value_grid, 256, value_lds, s>>>(p);
-    else wit_attend_values_kernel<false, 4><<<value_grid, 256, value_lds, s>>>(p);
+    if (vec && planes == 3) wit_attend_values_kernel<true, 3, WINDOW><<<value_grid, 256, value_lds, s>>>(p);
+    else if (vec) wit_attend_values_kernel<true, 4, WINDOW><<<value_grid, 256, value_lds, s>>>(p);
+    else if (planes == 3) wit_attend_values_kernel<false, 3, WINDOW><<<value_grid, 256, value_lds, s>>>(p);
+    else wit_attend_values_kernel<false, 4, WINDOW><<<value_grid, 256, value_lds, s>>>(p);
     GRAPE_LAUNCH_CHECK();
     if (pl.value_chunks > 1) {
         const uint32_t waves = std::min(kJoinThreads / 64, (pl.value_chunks + 3) / 4);
-        wit_attend_join_kernel<<<dim3(pl.dim64, a.heads, a.seqs), 64 * waves, 0, s>>>(p);
+        wit_attend_join_kernel<WINDOW><<<dim3(pl.dim64, a.heads, a.seqs), 64 * waves, 0, s>>>(p);
         GRAPE_LAUNCH_CHECK();
     }
     return GRAPE_OK;
+}
+
+// grape_wit_window_attention of at most one token a sequence, whose arguments have been looked over.
+int attend_single(const grape_wit_window_attention_args& w, const grape_wit_cache& cache, grape_stream_t st) {
+    AttendArgs p{};
+    p.c = cache;
+    p.a = grape_wit_attention_args{w.d_q, w.q_stride, w.d_block_table, w.d_lens, nullptr, w.d_exp_table, w.d_scores, w.d_scores_rem, w.d_shifted, w.d_exp, w.d_prob, w.d_query, w.d_max, w.d_sum,
+                                   w.d_out, w.d_out_rem, w.d_workspace, w.workspace_bytes, w.qk_scale, w.prob_scale, w.out_scale, w.seqs, w.heads, w.max_len, w.table_stride, w.bit_shift, w.index_bits};
+    p.d_starts = w.d_starts;
+    p.rows = w.rows;
+    p.window = w.window;
+    p.sinks = w.sinks;
+    step::single_plan(w.rows, w.seqs, w.heads, cache.heads, cache.dim, w.max_len, w.window, w.sinks, p.plan);
+    return attend<true>(p, st);
+}
+
+}  // namespace grape
+
+using namespace grape;
+
+extern "C" {
+
+size_t grape_wit_paged_attention_workspace(uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len) {
+    return token::attention_workspace(seqs, heads, cache_heads, dim, max_len);
+}
+
+int grape_wit_paged_attention(const grape_wit_attention_args* args, const grape_wit_cache* cache, grape_stream_t st) {
+    GRAPE_REQUIRE(initialised(), "grape_init has not been called");
+    GRAPE_REFUSED_IF(token::refuse_attention(args, cache));
+    if (args->seqs == 0) return GRAPE_OK;
+    AttendArgs p{};
+    p.a = *args;
+    p.c = *cache;
+    token::attention_plan(p.a.seqs, p.a.heads, p.c.heads, p.c.dim, p.a.max_len, p.plan);
+    return attend<false>(p, st);
 }
 
 }  // extern "C"

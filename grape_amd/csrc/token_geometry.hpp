@@ -116,7 +116,8 @@ constexpr uint32_t kCountedMost = 256;        // sequences whose chunks are coun
 
 inline uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
 
-inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len, AttentionPlan& p) {
+// `row_len`, `rows`: entries of a row of scores, and rows, where they are other than max_len positions and one of each sequence
+inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len, AttentionPlan& p, uint32_t row_len = 0, uint32_t rows = 0) {
     if (!seqs || !heads || !cache_heads || !dim || heads > 65535 || seqs > 65535 || heads % cache_heads || dim > 8192 || max_len >= (uint32_t)1 << 31) return false;
     const uint64_t rows_all = (uint64_t)seqs * heads;
     if ((unsigned __int128)rows_all * max_len >= (uint64_t)1 << 38) return false;
@@ -175,14 +176,17 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
     const size_t one = (size_t)5 * 64 * p.dim64 * p.rows, two = (size_t)4 * kWholeMost * p.rows;
     p.whole_lds = 8 * kWholeMost + (size_t)8 * p.rows * (dim > kWholeMost ? dim : kWholeMost) + (size_t)4 * kWholeMost * p.rows + (one > two ? one : two);
     p.whole = p.whole_lds <= kWholeLds && max_len <= kWholeMost && dim <= 256;
-    const size_t row = (size_t)rows_all * max_len * 4;
+    const uint64_t rows_held = (uint64_t)std::max(seqs, rows) * heads;
+    const uint32_t row_held = std::max(max_len, row_len);
+    if ((unsigned __int128)rows_held * row_held >= (uint64_t)1 << 38) return false;
+    const size_t row = (size_t)rows_held * row_held * 4;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     p.at_scores = 0;
     p.at_exp = up(row);
     p.at_max = p.at_exp + up(row);
-    p.at_sum = p.at_max + up((size_t)rows_all * p.score_chunks * 4);
-    p.at_part = p.at_sum + up((size_t)rows_all * p.exp_chunks * 8);
-    p.bytes = p.whole ? 0 : p.at_part + (p.value_chunks > 1 ? (size_t)rows_all * p.value_chunks * dim * 8 : 0);
+    p.at_sum = p.at_max + up((size_t)rows_held * p.score_chunks * 4);
+    p.at_part = p.at_sum + up((size_t)rows_held * p.exp_chunks * 8);
+    p.bytes = p.whole ? 0 : p.at_part + (p.value_chunks > 1 ? (size_t)rows_held * p.value_chunks * dim * 8 : 0);
     return true;
 }
 

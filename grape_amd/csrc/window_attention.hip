@@ -4,6 +4,7 @@
 #include <type_traits>
 #include "token_device.hpp"
 #include "step_geometry.hpp"
+#include "token_attention.hpp"
 
 namespace grape {
 
@@ -866,6 +867,7 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     GRAPE_REQUIRE(initialised(), "grape_init has not been called");
     GRAPE_REFUSED_IF(step::refuse_window(args, cache));
     if (!args->seqs || !args->rows || !args->max_new) return GRAPE_OK;
+    if (args->max_new == 1) return attend_single(*args, *cache, st);          // heads by sixteen and not rows by 32, one launch for few positions
     WindowArgs p;
     p.a = *args;
     p.c = *cache;
