@@ -90,7 +90,7 @@ struct NextPlan {
     uint32_t chunk, chunks;
     size_t bytes;
 };
-constexpr uint32_t kNextLeast = 1024, kNextMost = 8192;
+constexpr uint32_t kNextLeast = 1024, kNextMost = 4096;
 
 inline NextPlan next_plan(uint32_t seqs, uint32_t vocab) {
     NextPlan p;

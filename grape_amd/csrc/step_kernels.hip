@@ -199,114 +199,156 @@ __device__ __forceinline__ unsigned long long block_largest(unsigned long long v
     return v;
 }
 
-template <bool VEC>
+// four entries of a row, wherever it starts; those from n on are 0 and left as they were
+typedef int v4u_t __attribute__((ext_vector_type(4), aligned(4)));
 __device__ __forceinline__ v4i_t row4(const int32_t* x, uint32_t at, uint32_t n) {
-    if constexpr (VEC) {
-        return *reinterpret_cast<const v4i_t*>(x + at);
-    } else {
-        v4i_t v = {0, 0, 0, 0};
+    if (at + 4 <= n) return *reinterpret_cast<const v4u_t*>(x + at);
+    v4i_t v = {0, 0, 0, 0};
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++)
-            if (at + j < n) v[j] = x[at + j];
-        return v;
-    }
+    for (uint32_t j = 0; j < 3; j++)
+        if (at + j < n) v[j] = x[at + j];
+    return v;
 }
-template <bool VEC>
 __device__ __forceinline__ void put4(int32_t* x, uint32_t at, uint32_t n, v4i_t v) {
-    if constexpr (VEC) {
-        *reinterpret_cast<v4i_t*>(x + at) = v;
+    if (at + 4 <= n) {
+        *reinterpret_cast<v4u_t*>(x + at) = v;
     } else {
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++)
+        for (uint32_t j = 0; j < 3; j++)
             if (at + j < n) x[at + j] = v[j];
     }
 }
 
-template <bool VEC>
+// One way of the repetition's division, x * mul / by: in double precision where every product stays below 2^50 (see Penalty).
+struct Division {
+    double mul, by, inv, half;
+    Division() = default;
+    __device__ __forceinline__ Division(int64_t mul_, int64_t by_) : mul((double)mul_), by((double)by_), inv(1.0 / (double)by_), half((double)(by_ >> 1) + 0.5) {}
+};
+
+// What a token that occurs in the history loses.  With `scale` and the repetition's factor up to 2^18 a product of int32 stays below 2^50, and
+// the quotient of (y + by/2 + 1/2) / by is no nearer than 1 / (2 by) to a whole number while its product with 1 / by is off by at most 2^-52 of
+// itself: one product gives it.  Sums that leave 2^53 are no longer exact, and far outside int32.
+struct Penalty {
+    Division up, down;                         // of logits above zero, and of the others
+    Scaler wide_up, wide_down;
+    int64_t scale, repetition;
+    double presence, frequency;
+    bool divides, plain;
+    __device__ __forceinline__ void apply(int32_t x, uint32_t count, double& y, int32_t& rem) const {
+        y = (double)x;
+        rem = 0;
+        if (divides) {
+            if (plain) {
+                const double t = __builtin_fma(y, x > 0 ? up.mul : down.mul, x > 0 ? up.half : down.half), q = __builtin_floor(t * (x > 0 ? up.inv : down.inv));
+                rem = (int32_t)(__builtin_fma(-q, x > 0 ? up.by : down.by, t) - (x > 0 ? up.half : down.half));
+                y = q;
+            } else {
+                const int64_t product = (int64_t)x * (x > 0 ? scale : repetition), by = x > 0 ? repetition : scale;
+                int32_t q;
+                uint32_t beyond = 0;          // a quotient beyond int32 is still one of 64 bits
+                if (x > 0) wide_up.apply(product, q, rem, beyond);
+                else wide_down.apply(product, q, rem, beyond);
+                y = beyond ? (double)((product - rem) / by) : (double)q;
+            }
+        }
+        y -= __builtin_fma(frequency, (double)count, presence);
+    }
+};
+
 __global__ void __launch_bounds__(kBlock) wit_next_adjust_kernel(NextArgs p) {
-    extern __shared__ uint32_t counts[];
+    extern __shared__ __attribute__((aligned(16))) uint32_t counts[];
     const grape_wit_next_token_args& a = p.a;
     const uint32_t b = blockIdx.y, v0 = blockIdx.x * p.plan.chunk, n = min(a.vocab - v0, p.plan.chunk);
-    uint32_t bad = 0;
-    for (uint32_t i = threadIdx.x; i < p.plan.chunk; i += kBlock) counts[i] = 0;
-    __syncthreads();
+    const int32_t *logits = a.d_logits + b * a.logits_stride + v0, *bias = a.d_bias ? a.d_bias + b * a.bias_stride + v0 : nullptr;
+    const uint32_t* mask = a.d_mask ? reinterpret_cast<const uint32_t*>(a.d_mask) + b * a.mask_stride + v0 / 32 : nullptr;
+    uint32_t bad = 0, i = 4 * threadIdx.x;
+    // the first logits are under way while the history is counted, each next ones while these are worked on
+    v4i_t x = {0, 0, 0, 0}, more = {0, 0, 0, 0}, x_next = x, more_next = more;
+    uint32_t allowed = ~0u, allowed_next = ~0u;
+    auto fetch = [&](uint32_t at) {
+        if (at >= n) return;
+        x_next = row4(logits, at, n);
+        if (bias) more_next = row4(bias, at, n);
+        if (mask) allowed_next = mask[at / 32];
+    };
+    fetch(i);
+    for (uint32_t k = threadIdx.x; k < p.plan.chunk / 4; k += kBlock) reinterpret_cast<v4i_t*>(counts)[k] = v4i_t{0, 0, 0, 0};
     int32_t len = a.history ? a.d_history_lens[b] : 0;
     if (len < 0 || (uint32_t)len > a.history) {
         bad |= (uint32_t)kWitIndex;
         len = len < 0 ? 0 : (int32_t)a.history;
     }
+    Penalty penalty;
+    penalty.scale = a.scale;
+    penalty.repetition = a.d_repetition ? a.d_repetition[b] : a.scale;
+    if (penalty.repetition < 1) bad |= (uint32_t)kWitIndex;
+    penalty.divides = a.d_repetition && penalty.repetition >= 1;
+    penalty.plain = a.scale <= (1 << 18) && penalty.repetition <= (1 << 18);
+    if (penalty.divides) {
+        penalty.up = Division(a.scale, penalty.repetition);
+        penalty.down = Division(penalty.repetition, a.scale);
+        penalty.wide_up = Scaler{penalty.repetition, penalty.up.inv, -1};
+        penalty.wide_down = p.scale;
+    }
+    penalty.presence = a.d_presence ? (double)a.d_presence[b] : 0.0;
+    penalty.frequency = a.d_frequency ? (double)a.d_frequency[b] : 0.0;
+    __syncthreads();
     const int32_t* history = a.d_history + (len ? b * a.history_stride : 0);
-    for (uint32_t i = threadIdx.x; i < (uint32_t)len; i += kBlock) {
-        const int32_t t = history[i];
+#pragma unroll 4
+    for (uint32_t k = threadIdx.x; k < (uint32_t)len; k += kBlock) {
+        const int32_t t = history[k];
         if (t >= (int32_t)a.vocab) bad |= (uint32_t)kWitIndex;
         const uint32_t at = (uint32_t)t - v0;
         if (t >= 0 && at < n) atomicAdd(&counts[at], 1u);
     }
-    int32_t repetition = 0;          // none
-    Scaler down{1, 1.0, 0};
-    if (a.d_repetition) {
-        repetition = a.d_repetition[b];
-        if (repetition < 1) {
-            bad |= (uint32_t)kWitIndex;
-            repetition = 0;
-        } else {
-            down = Scaler{repetition, 1.0 / (double)repetition, -1};
-        }
-    }
-    const int64_t presence = a.d_presence ? a.d_presence[b] : 0, frequency = a.d_frequency ? a.d_frequency[b] : 0;
-    const int32_t *logits = a.d_logits + b * a.logits_stride + v0, *bias = a.d_bias ? a.d_bias + b * a.bias_stride + v0 : nullptr;
-    const uint32_t* mask = a.d_mask ? reinterpret_cast<const uint32_t*>(a.d_mask) + b * a.mask_stride + v0 / 32 : nullptr;
     const size_t o = (size_t)b * a.vocab + v0;
     __syncthreads();
-    unsigned long long best = 0;
-    for (uint32_t i = 4 * threadIdx.x; i < n; i += 4 * kBlock) {
-        const v4i_t x = row4<VEC>(logits, i, n);
-        v4i_t more = {0, 0, 0, 0};
-        if (bias) more = row4<VEC>(bias, i, n);
-        const uint32_t allowed = mask ? mask[i / 32] >> (i & 31u) : 15u;
-        v4i_t z, rem, c;
+    int32_t best = kLowest;
+    uint32_t best_at = 0;
+    for (; i < n; i += 4 * kBlock) {
+        x = x_next;
+        more = more_next;
+        allowed = allowed_next >> (i & 31u);
+        fetch(i + 4 * kBlock);
+        const v4i_t c = *reinterpret_cast<const v4i_t*>(counts + i);
+        v4i_t z, rem = {0, 0, 0, 0};
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
-            c[j] = (int32_t)counts[i + j];
-            int64_t y = x[j];
-            int32_t q, r = 0;
-            rem[j] = 0;
+            const bool in = i + j < n, chosen = ((allowed >> j) & 1u) && x[j] != kLowest && more[j] != kLowest;
+            int32_t zj;
+            bool beyond;
             if (c[j]) {
-                if (repetition) {
-                    uint32_t wide = 0;          // a quotient beyond int32 is still one of 64 bits
-                    if (x[j] > 0) {
-                        down.apply((int64_t)x[j] * p.a.scale, q, r, wide);
-                        y = wide ? ((int64_t)x[j] * p.a.scale - r) / repetition : q;
-                    } else {
-                        p.scale.apply((int64_t)x[j] * repetition, q, r, wide);
-                        y = wide ? ((int64_t)x[j] * repetition - r) / p.a.scale : q;
-                    }
-                }
-                y -= presence + frequency * c[j];
+                double y;
+                int32_t r;
+                penalty.apply(x[j], (uint32_t)c[j], y, r);
+                y += (double)more[j];
+                beyond = y <= (double)kLowest || y > (double)INT32_MAX;
+                zj = beyond ? (y < 0.0 ? kLowest + 1 : INT32_MAX) : (int32_t)y;
+                if (chosen) rem[j] = r;
+            } else {
+                beyond = __builtin_add_overflow(x[j], more[j], &zj);
+                if (beyond) zj = more[j] < 0 ? kLowest : INT32_MAX;
+                beyond |= zj == kLowest;
+                zj = max(zj, kLowest + 1);
             }
-            y += more[j];
-            const bool chosen = ((allowed >> j) & 1u) && x[j] != kLowest && more[j] != kLowest;
-            if (chosen) {
-                if (y <= (int64_t)kLowest || y > (int64_t)INT32_MAX) {
-                    if (i + j < n) bad |= (uint32_t)kWitQuotient;
-                    y = y <= (int64_t)kLowest ? (int64_t)kLowest + 1 : (int64_t)INT32_MAX;
-                }
-                rem[j] = r;
+            if (chosen && in && beyond) bad |= (uint32_t)kWitQuotient;
+            z[j] = chosen ? zj : kLowest;
+            if (in && z[j] > best) {
+                best = z[j];
+                best_at = v0 + i + j;
             }
-            z[j] = chosen ? (int32_t)y : kLowest;
-            if (i + j < n) best = max(best, rank_of(z[j], v0 + i + j));
         }
-        if (a.d_out) put4<VEC>(a.d_out + o, i, n, z);
-        if (a.d_rem) put4<VEC>(a.d_rem + o, i, n, rem);
-        if (a.d_count) put4<VEC>(a.d_count + o, i, n, c);
-        if (a.d_gap) put4<VEC>(a.d_gap + o, i, n, z);          // the second launch takes it from the largest
+        if (a.d_out) put4(a.d_out + o, i, n, z);
+        if (a.d_rem) put4(a.d_rem + o, i, n, rem);
+        if (a.d_count) put4(a.d_count + o, i, n, c);
+        if (a.d_gap) put4(a.d_gap + o, i, n, z);          // the second launch takes it from the largest
     }
-    best = block_largest(best);
-    if (threadIdx.x == 0) p.part[(size_t)b * p.plan.chunks + blockIdx.x] = best;
+    const unsigned long long largest = block_largest(rank_of(best, best_at));
+    if (threadIdx.x == 0) p.part[(size_t)b * p.plan.chunks + blockIdx.x] = largest;
     if (bad) atomicOr(p.status, bad);
 }
 
-template <bool VEC>
 __global__ void __launch_bounds__(kBlock) wit_next_choose_kernel(NextArgs p) {
     const grape_wit_next_token_args& a = p.a;
     const uint32_t b = blockIdx.y;
@@ -323,14 +365,14 @@ __global__ void __launch_bounds__(kBlock) wit_next_choose_kernel(NextArgs p) {
     int32_t* gap = a.d_gap + (size_t)b * a.vocab + v0;
     uint32_t bad = 0;
     for (uint32_t i = 4 * threadIdx.x; i < n; i += 4 * kBlock) {
-        v4i_t z = row4<VEC>(gap, i, n);
+        v4i_t z = row4(gap, i, n);
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
             const uint32_t below = z[j] == kLowest ? 0u : (uint32_t)top - (uint32_t)z[j];
             if (below > (uint32_t)INT32_MAX && i + j < n) bad |= (uint32_t)kWitSumWide;
             z[j] = (int32_t)below;
         }
-        put4<VEC>(gap, i, n, z);
+        put4(gap, i, n, z);
     }
     if (bad) atomicOr(p.status, bad);
 }
@@ -372,16 +414,12 @@ int grape_wit_next_token(const grape_wit_next_token_args* args, grape_stream_t s
     hipStream_t s = as_stream(st);
     const int rc = wit_status_word(&p.status);
     if (rc) return rc;
-    auto wide = [&](const void* x, int64_t stride) { return !x || ((reinterpret_cast<uintptr_t>(x) & 15) == 0 && stride % 4 == 0); };
-    const bool vec = a.vocab % 4 == 0 && wide(a.d_logits, a.logits_stride) && wide(a.d_bias, a.bias_stride) && wide(a.d_out, 0) && wide(a.d_rem, 0) && wide(a.d_count, 0) && wide(a.d_gap, 0);
     const dim3 grid(p.plan.chunks, a.seqs);
     const size_t lds = (size_t)4 * p.plan.chunk;
-    if (vec) wit_next_adjust_kernel<true><<<grid, kBlock, lds, s>>>(p);
-    else wit_next_adjust_kernel<false><<<grid, kBlock, lds, s>>>(p);
+    wit_next_adjust_kernel<<<grid, kBlock, lds, s>>>(p);
     GRAPE_LAUNCH_CHECK();
     const dim3 join(a.d_gap ? p.plan.chunks : 1, a.seqs);
-    if (vec) wit_next_choose_kernel<true><<<join, kBlock, 0, s>>>(p);
-    else wit_next_choose_kernel<false><<<join, kBlock, 0, s>>>(p);
+    wit_next_choose_kernel<<<join, kBlock, 0, s>>>(p);
     GRAPE_LAUNCH_CHECK();
     return GRAPE_OK;
 }
