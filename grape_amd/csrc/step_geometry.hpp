@@ -90,12 +90,12 @@ struct NextPlan {
     uint32_t chunk, chunks;
     size_t bytes;
 };
-constexpr uint32_t kNextLeast = 1024, kNextMost = 4096;
+constexpr uint32_t kNextLeast = 2048, kNextMost = 8192;
 
 inline NextPlan next_plan(uint32_t seqs, uint32_t vocab) {
     NextPlan p;
     p.chunk = kNextMost;
-    while (p.chunk > kNextLeast && (uint64_t)seqs * token::ceil_div(vocab, p.chunk) < 1024) p.chunk /= 2;
+    while (p.chunk > kNextLeast && (uint64_t)seqs * token::ceil_div(vocab, p.chunk) < 512) p.chunk /= 2;
     p.chunks = token::ceil_div(vocab, p.chunk);
     p.bytes = (size_t)8 * seqs * p.chunks;
     return p;

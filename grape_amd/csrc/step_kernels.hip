@@ -187,15 +187,16 @@ __device__ __forceinline__ unsigned long long rank_of(int32_t z, uint32_t token)
 }
 __device__ __forceinline__ int32_t value_of(unsigned long long rank) { return (int32_t)((uint32_t)(rank >> 32) ^ 0x80000000u); }
 
+constexpr uint32_t kNextThreads = 512, kNextAhead = 4;          // of a workgroup; tokens of the history asked for at once by a thread
 __device__ __forceinline__ unsigned long long block_largest(unsigned long long v) {
-    __shared__ unsigned long long sh[kBlock / 64];
+    __shared__ unsigned long long sh[kNextThreads / 64];
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
     __syncthreads();
     v = sh[0];
 #pragma unroll
-    for (int w = 1; w < kBlock / 64; w++) v = max(v, sh[w]);
+    for (uint32_t w = 1; w < kNextThreads / 64; w++) v = max(v, sh[w]);
     return v;
 }
 
@@ -256,25 +257,33 @@ struct Penalty {
     }
 };
 
-__global__ void __launch_bounds__(kBlock) wit_next_adjust_kernel(NextArgs p) {
+__global__ void __launch_bounds__(kNextThreads, 6) wit_next_adjust_kernel(NextArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t counts[];
     const grape_wit_next_token_args& a = p.a;
     const uint32_t b = blockIdx.y, v0 = blockIdx.x * p.plan.chunk, n = min(a.vocab - v0, p.plan.chunk);
     const int32_t *logits = a.d_logits + b * a.logits_stride + v0, *bias = a.d_bias ? a.d_bias + b * a.bias_stride + v0 : nullptr;
     const uint32_t* mask = a.d_mask ? reinterpret_cast<const uint32_t*>(a.d_mask) + b * a.mask_stride + v0 / 32 : nullptr;
-    uint32_t bad = 0, i = 4 * threadIdx.x;
-    // the first logits are under way while the history is counted, each next ones while these are worked on
-    v4i_t x = {0, 0, 0, 0}, more = {0, 0, 0, 0}, x_next = x, more_next = more;
-    uint32_t allowed = ~0u, allowed_next = ~0u;
-    auto fetch = [&](uint32_t at) {
-        if (at >= n) return;
-        x_next = row4(logits, at, n);
-        if (bias) more_next = row4(bias, at, n);
-        if (mask) allowed_next = mask[at / 32];
-    };
-    fetch(i);
-    for (uint32_t k = threadIdx.x; k < p.plan.chunk / 4; k += kBlock) reinterpret_cast<v4i_t*>(counts)[k] = v4i_t{0, 0, 0, 0};
+    uint32_t bad = 0;
+    // a thread's logits are all under way while the history is counted
+    constexpr uint32_t kFours = step::kNextMost / (4 * kNextThreads);
+    v4i_t x[kFours];
+#pragma unroll
+    for (uint32_t k = 0; k < kFours; k++) {
+        const uint32_t i = 4 * (threadIdx.x + k * kNextThreads);
+        x[k] = i < n ? row4(logits, i, n) : v4i_t{0, 0, 0, 0};
+    }
     int32_t len = a.history ? a.d_history_lens[b] : 0;
+    const int32_t* history = a.history ? a.d_history + b * a.history_stride : nullptr;
+    int32_t seen[kNextAhead];
+    auto fetch = [&](uint32_t from) {
+#pragma unroll
+        for (uint32_t k = 0; k < kNextAhead; k++) {
+            const uint32_t at = from + threadIdx.x + k * kNextThreads;
+            seen[k] = at < a.history ? history[at] : -1;
+        }
+    };
+    fetch(0);
+    for (uint32_t k = threadIdx.x; k < p.plan.chunk / 4; k += kNextThreads) reinterpret_cast<v4i_t*>(counts)[k] = v4i_t{0, 0, 0, 0};
     if (len < 0 || (uint32_t)len > a.history) {
         bad |= (uint32_t)kWitIndex;
         len = len < 0 ? 0 : (int32_t)a.history;
@@ -294,50 +303,60 @@ __global__ void __launch_bounds__(kBlock) wit_next_adjust_kernel(NextArgs p) {
     penalty.presence = a.d_presence ? (double)a.d_presence[b] : 0.0;
     penalty.frequency = a.d_frequency ? (double)a.d_frequency[b] : 0.0;
     __syncthreads();
-    const int32_t* history = a.d_history + (len ? b * a.history_stride : 0);
-#pragma unroll 4
-    for (uint32_t k = threadIdx.x; k < (uint32_t)len; k += kBlock) {
-        const int32_t t = history[k];
-        if (t >= (int32_t)a.vocab) bad |= (uint32_t)kWitIndex;
-        const uint32_t at = (uint32_t)t - v0;
-        if (t >= 0 && at < n) atomicAdd(&counts[at], 1u);
+    for (uint32_t from = 0; from < (uint32_t)len; from += kNextAhead * kNextThreads) {
+        if (from) fetch(from);
+#pragma unroll
+        for (uint32_t k = 0; k < kNextAhead; k++) {
+            const int32_t t = seen[k];
+            if (from + threadIdx.x + k * kNextThreads >= (uint32_t)len) break;
+            if (t >= (int32_t)a.vocab) bad |= (uint32_t)kWitIndex;
+            const uint32_t at = (uint32_t)t - v0;
+            if (t >= 0 && at < n) atomicAdd(&counts[at], 1u);
+        }
     }
     const size_t o = (size_t)b * a.vocab + v0;
     __syncthreads();
     int32_t best = kLowest;
     uint32_t best_at = 0;
-    for (; i < n; i += 4 * kBlock) {
-        x = x_next;
-        more = more_next;
-        allowed = allowed_next >> (i & 31u);
-        fetch(i + 4 * kBlock);
+#pragma unroll
+    for (uint32_t k = 0; k < kFours; k++) {
+        const uint32_t i = 4 * (threadIdx.x + k * kNextThreads);
+        if (i >= n) break;
+        const v4i_t more = bias ? row4(bias, i, n) : v4i_t{0, 0, 0, 0};
+        const uint32_t allowed = mask ? mask[i / 32] >> (i & 31u) : ~0u;
         const v4i_t c = *reinterpret_cast<const v4i_t*>(counts + i);
         v4i_t z, rem = {0, 0, 0, 0};
+        // a sum at either end of int32 may have left it, or stand where excluded tokens do
+        uint32_t edge = ~0u;
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
-            const bool in = i + j < n, chosen = ((allowed >> j) & 1u) && x[j] != kLowest && more[j] != kLowest;
-            int32_t zj;
-            bool beyond;
-            if (c[j]) {
-                double y;
-                int32_t r;
-                penalty.apply(x[j], (uint32_t)c[j], y, r);
+            const bool chosen = ((allowed >> j) & 1u) && min(x[k][j], more[j]) != kLowest;
+            const int32_t sum = __builtin_elementwise_add_sat((int)x[k][j], (int)more[j]);
+            edge = min(edge, ((uint32_t)sum ^ 0x80000000u) + 1u);
+            z[j] = chosen ? sum : kLowest;
+        }
+        if ((c[0] | c[1] | c[2] | c[3]) || edge < 2) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                if (!(c[j] || edge < 2) || !((allowed >> j) & 1u) || min(x[k][j], more[j]) == kLowest || i + j >= n) continue;
+                double y = (double)x[k][j];
+                int32_t r = 0;
+                if (c[j]) penalty.apply(x[k][j], (uint32_t)c[j], y, r);
+                rem[j] = r;
                 y += (double)more[j];
-                beyond = y <= (double)kLowest || y > (double)INT32_MAX;
-                zj = beyond ? (y < 0.0 ? kLowest + 1 : INT32_MAX) : (int32_t)y;
-                if (chosen) rem[j] = r;
-            } else {
-                beyond = __builtin_add_overflow(x[j], more[j], &zj);
-                if (beyond) zj = more[j] < 0 ? kLowest : INT32_MAX;
-                beyond |= zj == kLowest;
-                zj = max(zj, kLowest + 1);
+                const bool beyond = y <= (double)kLowest || y > (double)INT32_MAX;
+                if (beyond) bad |= (uint32_t)kWitQuotient;
+                z[j] = beyond ? (y < 0.0 ? kLowest + 1 : INT32_MAX) : (int32_t)y;
             }
-            if (chosen && in && beyond) bad |= (uint32_t)kWitQuotient;
-            z[j] = chosen ? zj : kLowest;
-            if (in && z[j] > best) {
-                best = z[j];
-                best_at = v0 + i + j;
-            }
+        }
+        if (i + 4 > n) {
+#pragma unroll
+            for (uint32_t j = 1; j < 4; j++) z[j] = i + j < n ? z[j] : kLowest;
+        }
+        const int32_t most = max(max(z[0], z[1]), max(z[2], z[3]));
+        if (most > best) {
+            best = most;
+            best_at = v0 + i + (z[0] == most ? 0 : z[1] == most ? 1 : z[2] == most ? 2 : 3);
         }
         if (a.d_out) put4(a.d_out + o, i, n, z);
         if (a.d_rem) put4(a.d_rem + o, i, n, rem);
@@ -349,11 +368,11 @@ __global__ void __launch_bounds__(kBlock) wit_next_adjust_kernel(NextArgs p) {
     if (bad) atomicOr(p.status, bad);
 }
 
-__global__ void __launch_bounds__(kBlock) wit_next_choose_kernel(NextArgs p) {
+__global__ void __launch_bounds__(kNextThreads) wit_next_choose_kernel(NextArgs p) {
     const grape_wit_next_token_args& a = p.a;
     const uint32_t b = blockIdx.y;
     unsigned long long best = 0;
-    for (uint32_t i = threadIdx.x; i < p.plan.chunks; i += kBlock) best = max(best, p.part[(size_t)b * p.plan.chunks + i]);
+    for (uint32_t i = threadIdx.x; i < p.plan.chunks; i += kNextThreads) best = max(best, p.part[(size_t)b * p.plan.chunks + i]);
     best = block_largest(best);
     const int32_t top = value_of(best);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -364,7 +383,7 @@ __global__ void __launch_bounds__(kBlock) wit_next_choose_kernel(NextArgs p) {
     const uint32_t v0 = blockIdx.x * p.plan.chunk, n = min(a.vocab - v0, p.plan.chunk);
     int32_t* gap = a.d_gap + (size_t)b * a.vocab + v0;
     uint32_t bad = 0;
-    for (uint32_t i = 4 * threadIdx.x; i < n; i += 4 * kBlock) {
+    for (uint32_t i = 4 * threadIdx.x; i < n; i += 4 * kNextThreads) {
         v4i_t z = row4(gap, i, n);
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
@@ -416,10 +435,10 @@ int grape_wit_next_token(const grape_wit_next_token_args* args, grape_stream_t s
     if (rc) return rc;
     const dim3 grid(p.plan.chunks, a.seqs);
     const size_t lds = (size_t)4 * p.plan.chunk;
-    wit_next_adjust_kernel<<<grid, kBlock, lds, s>>>(p);
+    wit_next_adjust_kernel<<<grid, kNextThreads, lds, s>>>(p);
     GRAPE_LAUNCH_CHECK();
     const dim3 join(a.d_gap ? p.plan.chunks : 1, a.seqs);
-    wit_next_choose_kernel<<<join, kBlock, 0, s>>>(p);
+    wit_next_choose_kernel<<<join, kNextThreads, 0, s>>>(p);
     GRAPE_LAUNCH_CHECK();
     return GRAPE_OK;
 }
