@@ -17,29 +17,30 @@ struct PageArgs {
     uint32_t sink_pages;
     uint32_t* status;
 };
-constexpr uint32_t kPageThreads = 256;
-
-// The sum of v over the threads before this one, and of all of them.
-__device__ __forceinline__ uint64_t before_me(uint64_t v, uint64_t& all) {
-    __shared__ uint64_t waves[kPageThreads / 64];
+struct Two {
+    uint64_t a, b;
+};
+// The sums of v over the threads before this one, and of all of them.
+template <uint32_t THREADS>
+__device__ __forceinline__ Two before_me(Two v, Two& all, Two* waves) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    uint64_t sum = v;
+    Two sum = v;
 #pragma unroll
     for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint64_t y = __shfl_up(sum, d, 64);
-        if (lane >= d) sum += y;
+        const uint64_t x = __shfl_up(sum.a, d, 64), y = __shfl_up(sum.b, d, 64);
+        if (lane >= d) sum.a += x, sum.b += y;
     }
-    __syncthreads();
     if (lane == 63) waves[wave] = sum;
     __syncthreads();
-    uint64_t base = 0;
-    all = 0;
+    Two base{sum.a - v.a, sum.b - v.b};
+    all = Two{0, 0};
 #pragma unroll
-    for (uint32_t w = 0; w < kPageThreads / 64; w++) {
-        if (w < wave) base += waves[w];
-        all += waves[w];
+    for (uint32_t w = 0; w < THREADS / 64; w++) {
+        if (w < wave) base.a += waves[w].a, base.b += waves[w].b;
+        all.a += waves[w].a;
+        all.b += waves[w].b;
     }
-    return base + sum - v;
+    return base;
 }
 
 // The number of the n ascending sums that are at most `x`: the sequence that x belongs to.
@@ -53,117 +54,119 @@ __device__ __forceinline__ uint32_t find_sequence(const uint32_t* sums, uint32_t
     return lo;
 }
 
-__global__ void __launch_bounds__(kPageThreads) wit_page_step_kernel(PageArgs p) {
+template <uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS) wit_page_step_kernel(PageArgs p) {
     extern __shared__ uint32_t lds[];
+    __shared__ Two waves[2][THREADS / 64];
+    __shared__ uint32_t top[2];
     const grape_wit_page_step_args& a = p.a;
     uint32_t *to_token = lds, *to_page = lds + a.seqs, *to_back = lds + 2 * a.seqs;          // sums up to and with each sequence
-    const uint32_t each = (a.seqs + kPageThreads - 1) / kPageThreads, b0 = min(threadIdx.x * each, a.seqs), b1 = min(b0 + each, a.seqs);
+    int32_t *lens = reinterpret_cast<int32_t*>(lds + 3 * a.seqs), *news = lens + a.seqs;
     const uint64_t most = (uint64_t)a.page_size * a.table_stride;
     uint32_t bad = 0;
-    uint32_t head = (uint32_t)a.d_span[0], count = (uint32_t)a.d_span[1];
-    const bool ring_ok = count <= a.ring && (head < a.ring || (head == 0 && a.ring == 0));
-    if (!ring_ok) {
-        head = count = 0;
-        bad |= (uint32_t)kWitIndex;
+    for (uint32_t b = threadIdx.x; b < a.seqs; b += THREADS) {
+        lens[b] = a.d_lens[b];
+        news[b] = a.d_new[b];
     }
-    const uint32_t room = ring_ok ? a.ring - count : 0;
-    auto ask = [&](uint32_t b, step::Sequence& s) { return s.ask(a.d_lens[b], a.d_new[b], most, p.by_page); };
+    const uint32_t head_in = (uint32_t)a.d_span[0], count_in = (uint32_t)a.d_span[1];
+    const bool ring_ok = count_in <= a.ring && (head_in < a.ring || (head_in == 0 && a.ring == 0));
+    const uint32_t head = ring_ok ? head_in : 0, count = ring_ok ? count_in : 0, room = ring_ok ? a.ring - count : 0;
+    if (!ring_ok) bad |= (uint32_t)kWitIndex;
+    if (threadIdx.x < 2) top[threadIdx.x] = 0;
+    __syncthreads();
+    const uint32_t each = (a.seqs + THREADS - 1) / THREADS, b0 = min(threadIdx.x * each, a.seqs), b1 = min(b0 + each, a.seqs);
     step::Sequence s;
-    uint64_t tokens = 0, pages = 0, all_tokens, all_pages;
+    auto ask = [&](uint32_t b) { return s.ask(lens[b], news[b], most, p.by_page); };
+    Two wanted{0, 0}, all, back{0, 0}, all_back;          // tokens and pages; pages given back
     for (uint32_t b = b0; b < b1; b++) {
-        if (!ask(b, s)) bad |= (uint32_t)kWitIndex;
-        tokens += s.tokens;
-        pages += s.taken;
+        if (!ask(b)) bad |= (uint32_t)kWitIndex;
+        wanted.a += s.tokens;
+        wanted.b += s.taken;
     }
-    tokens = before_me(tokens, all_tokens);
-    pages = before_me(pages, all_pages);
+    wanted = before_me<THREADS>(wanted, all, waves[0]);
     // sequences are served in their order until the rows or the free pages run out; from there on none is
-    uint64_t served_tokens = 0, served_pages = 0, back = 0, all_back;
+    uint32_t served_tokens = 0, served_pages = 0;
     for (uint32_t b = b0; b < b1; b++) {
-        ask(b, s);
-        tokens += s.tokens;
-        pages += s.taken;
-        const bool served = tokens <= a.rows && pages <= count;
-        if (!served) s.refuse();
-        else served_tokens = tokens, served_pages = pages;
+        ask(b);
+        wanted.a += s.tokens;
+        wanted.b += s.taken;
+        const bool served = wanted.a <= a.rows && wanted.b <= count;
+        if (served) served_tokens = (uint32_t)wanted.a, served_pages = (uint32_t)wanted.b;
+        else s.refuse();
         s.give_back(a.window, p.sink_pages, p.by_page);
-        back += s.back;
-        to_token[b] = served ? (uint32_t)tokens : UINT32_MAX;
-        to_page[b] = served ? (uint32_t)pages : UINT32_MAX;
+        back.a += s.back;
+        to_token[b] = served ? (uint32_t)wanted.a : UINT32_MAX;
+        to_page[b] = (uint32_t)wanted.b;
+        to_back[b] = s.back;
     }
     // the largest sums that were served
-    __shared__ uint32_t top[2];
-    if (threadIdx.x < 2) top[threadIdx.x] = 0;
-    back = before_me(back, all_back);
-    if (b0 < b1) {
-        atomicMax(&top[0], (uint32_t)served_tokens);
-        atomicMax(&top[1], (uint32_t)served_pages);
-    }
-    __syncthreads();
-    const uint32_t rows = top[0], taken = top[1], kept = (uint32_t)min(all_back, (uint64_t)room);
+    if (served_tokens) atomicMax(&top[0], served_tokens);
+    if (served_pages) atomicMax(&top[1], served_pages);
+    back = before_me<THREADS>(back, all_back, waves[1]);
+    const uint32_t rows = top[0], taken = top[1], kept = (uint32_t)min(all_back.a, (uint64_t)room);
     const bool mine = blockIdx.x == 0;          // of what is written once
     for (uint32_t b = b0; b < b1; b++) {
-        ask(b, s);
         const bool served = to_token[b] != UINT32_MAX;
         if (!served) {
-            s.refuse();
             to_token[b] = rows;
             to_page[b] = taken;
         }
-        s.give_back(a.window, p.sink_pages, p.by_page);
-        back += s.back;
-        to_back[b] = (uint32_t)back;
+        back.a += to_back[b];
+        to_back[b] = (uint32_t)back.a;
         if (mine) {
+            const bool ok = ask(b);
             a.d_starts[b + 1] = (int32_t)to_token[b];
-            a.d_lens_out[b] = !s.ok ? a.d_lens[b] : s.ended ? 0 : (int32_t)(s.len + s.tokens);
+            a.d_lens_out[b] = !ok ? lens[b] : s.ended ? 0 : (int32_t)(s.len + (served ? s.tokens : 0));
         }
     }
     if (mine && threadIdx.x == 0) {
         a.d_starts[0] = 0;
-        uint32_t at = head + taken;
-        a.d_span_out[0] = (int32_t)(ring_ok ? (at >= a.ring && a.ring ? at - a.ring : at) : (uint32_t)a.d_span[0]);
-        a.d_span_out[1] = (int32_t)(ring_ok ? count - taken + kept : (uint32_t)a.d_span[1]);
-        if (all_tokens > a.rows || all_pages > count || all_back > kept) bad |= (uint32_t)kWitPages;
+        const uint32_t at = head + taken;
+        a.d_span_out[0] = (int32_t)(ring_ok ? (at >= a.ring && a.ring ? at - a.ring : at) : head_in);
+        a.d_span_out[1] = (int32_t)(ring_ok ? count - taken + kept : count_in);
+        if (all.a > a.rows || all.b > count || all_back.a > kept) bad |= (uint32_t)kWitPages;
     }
     __syncthreads();
     auto ring_at = [&](uint32_t k) {
         const uint32_t at = head + k;
         return at >= a.ring ? at - a.ring : at;
     };
-    // page number i of sequence b, whose first new page is number `first` of those taken
+    // page number i of sequence b, which held `held` and whose first new one is number `first` of those taken
     auto page_at = [&](uint32_t b, uint32_t i, uint32_t held, uint32_t first) {
         return i < held ? a.d_block_table[(size_t)b * a.table_stride + i] : a.d_free[ring_at(first + i - held)];
     };
-    const uint32_t stride = gridDim.x * kPageThreads, from = blockIdx.x * kPageThreads + threadIdx.x;
-    for (uint32_t r = from; r < a.rows; r += stride) {
-        int32_t pos = 0;
-        int64_t slot = -1;
-        if (r < rows) {
-            const uint32_t b = find_sequence(to_token, a.seqs, r);
-            ask(b, s);
-            const uint32_t at = s.len + (r - (b ? to_token[b - 1] : 0)), i = p.by_page(at);
-            const int32_t page = page_at(b, i, s.held, b ? to_page[b - 1] : 0);
-            pos = (int32_t)at;
-            if (page >= 0) slot = (int64_t)page * a.page_size + (at - i * a.page_size);
-            else bad |= (uint32_t)kWitIndex;
+    // rows, new pages and pages given back, each from a wave of its own on, so that none waits for the loads of another kind
+    auto up = [](uint64_t x) { return (x + 63) / 64 * 64; };
+    const uint64_t page0 = up(a.rows), back0 = page0 + up(taken), end = back0 + kept;
+    for (uint64_t at = (uint64_t)blockIdx.x * THREADS + threadIdx.x; at < end; at += (uint64_t)gridDim.x * THREADS) {
+        if (at < page0) {
+            const uint32_t r = (uint32_t)at;
+            if (r >= a.rows) continue;
+            int32_t pos = 0;
+            int64_t slot = -1;
+            if (r < rows) {
+                const uint32_t b = find_sequence(to_token, a.seqs, r), had = (uint32_t)lens[b], t = had + (r - (b ? to_token[b - 1] : 0)), i = p.by_page(t);
+                const int32_t page = page_at(b, i, step::pages_of(had, p.by_page), b ? to_page[b - 1] : 0);
+                pos = (int32_t)t;
+                if (page >= 0) slot = (int64_t)page * a.page_size + (t - i * a.page_size);
+                else bad |= (uint32_t)kWitIndex;
+            }
+            a.d_positions[r] = pos;
+            a.d_slots[r] = slot;
+        } else if (at < back0) {
+            const uint32_t k = (uint32_t)(at - page0);
+            if (k >= taken) continue;
+            const uint32_t b = find_sequence(to_page, a.seqs, k);
+            a.d_block_table[(size_t)b * a.table_stride + step::pages_of((uint32_t)lens[b], p.by_page) + (k - (b ? to_page[b - 1] : 0))] = a.d_free[ring_at(k)];
+        } else {
+            const uint32_t k = (uint32_t)(at - back0), b = find_sequence(to_back, a.seqs, k);
+            ask(b);
+            if (b ? to_token[b] == to_token[b - 1] : to_token[b] == 0) s.refuse();
+            s.give_back(a.window, p.sink_pages, p.by_page);
+            const int32_t page = page_at(b, s.back_page(k - (b ? to_back[b - 1] : 0)), s.held, b ? to_page[b - 1] : 0);
+            if (page < 0) bad |= (uint32_t)kWitIndex;
+            a.d_free[ring_at(count + k)] = page;
         }
-        a.d_positions[r] = pos;
-        a.d_slots[r] = slot;
-    }
-    for (uint32_t k = from; k < taken; k += stride) {
-        const uint32_t b = find_sequence(to_page, a.seqs, k);
-        ask(b, s);
-        a.d_block_table[(size_t)b * a.table_stride + s.held + (k - (b ? to_page[b - 1] : 0))] = a.d_free[ring_at(k)];
-    }
-    for (uint32_t k = from; k < kept; k += stride) {
-        const uint32_t b = find_sequence(to_back, a.seqs, k);
-        ask(b, s);
-        if (b ? to_token[b] == to_token[b - 1] : to_token[b] == 0) s.refuse();
-        s.give_back(a.window, p.sink_pages, p.by_page);
-        const uint32_t i = s.back_page(k - (b ? to_back[b - 1] : 0));
-        const int32_t page = page_at(b, i, s.held, b ? to_page[b - 1] : 0);
-        if (page < 0) bad |= (uint32_t)kWitIndex;
-        a.d_free[ring_at(count + k)] = page;
     }
     if (bad) atomicOr(p.status, bad);
 }
@@ -412,8 +415,11 @@ int grape_wit_page_step(const grape_wit_page_step_args* args, grape_stream_t st)
     hipStream_t s = as_stream(st);
     const int rc = wit_status_word(&p.status);
     if (rc) return rc;
-    const uint32_t workgroups = std::min(256u, std::max(1u, token::ceil_div(std::max(p.a.rows, p.a.seqs), 4 * kPageThreads)));
-    wit_page_step_kernel<<<workgroups, kPageThreads, (size_t)12 * p.a.seqs, s>>>(p);
+    // every workgroup makes the sums, of a sequence a thread or up to four
+    const uint32_t threads = p.a.seqs <= 256 ? 256 : 1024, workgroups = std::min(256u, token::ceil_div(p.a.rows, threads) + token::ceil_div(p.a.seqs, 128));
+    const size_t lds = (size_t)20 * p.a.seqs;
+    if (threads == 256) wit_page_step_kernel<256><<<std::max(1u, workgroups), 256, lds, s>>>(p);
+    else wit_page_step_kernel<1024><<<std::max(1u, workgroups), 1024, lds, s>>>(p);
     GRAPE_LAUNCH_CHECK();
     return GRAPE_OK;
 }
