@@ -236,6 +236,14 @@ struct Seen {
     }
     GRAPE_HD uint32_t tile(uint32_t v) const { return v < sink_tiles ? v : v - sink_tiles + from; }
     GRAPE_HD bool any(uint32_t t) const { return t < hi && (t >= lo || t < sinks); }
+    // the tiles from <= v < to of v0 .. v0 + n, counted from v0, whose positions all rows see (tokens pos0 .. pos1); sinks' tiles are not counted
+    GRAPE_HD void full(uint32_t pos0, uint32_t pos1, uint32_t window, uint32_t v0, uint32_t n, uint32_t& first, uint32_t& last) const {
+        const uint32_t lowest = window && pos1 + 1 > window ? (pos1 - window) / kCols + 1 : 0, end = (pos0 + 1) / kCols;
+        const uint32_t a = sink_tiles + (lowest > from ? lowest - from : 0), b = end > from ? sink_tiles + end - from : 0;
+        first = a > v0 ? (a - v0 < n ? a - v0 : n) : 0;
+        last = b > v0 ? (b - v0 < n ? b - v0 : n) : 0;
+        if (last < first) last = first;
+    }
 };
 // whether the token at `pos` sees position t
 GRAPE_HD bool sees(uint32_t pos, uint32_t t, uint32_t window, uint32_t sinks) { return t <= pos && (!window || t + window > pos || t < sinks); }

@@ -74,7 +74,8 @@ __device__ __forceinline__ void four_planes(v4i_t x, uint32_t out[4]) {
 }
 
 // A workgroup's rows: rows `at` .. + R of the cache head kv of sequence b, whose n new tokens start at row `first` and position
-// `pos`.  Row r is query head r % each of token r / each.
+// `pos`.  Row r is query head r % each of token r / each.  Where there are fewer than kRows, the last one stands in for those that are
+// missing: what is written for it is written several times, and the same.
 struct RowTile {
     uint32_t b, kv, first, n, pos, at, R, first_pos, last_pos;
     uint32_t lane, wave, col, kg;
@@ -117,9 +118,9 @@ struct RowTile {
         return (size_t)(first + j) * p.a.heads + kv * p.plan.each + (at + r - j * p.plan.each);
     }
     __device__ __forceinline__ step::Seen seen(const WindowArgs& p) const { return step::Seen(first_pos, last_pos, p.a.window, p.a.sinks); }
-    // whether there are kRows rows and all of them see the kCols positions from k0 on
-    __device__ __forceinline__ bool all_see(const WindowArgs& p, uint32_t k0) const {
-        return R == kRows && k0 + kCols - 1 <= first_pos && (!p.a.window || k0 + p.a.window > last_pos || k0 + kCols <= p.a.sinks);
+    // the tiles first <= v < last of v0 .. v0 + n whose positions all rows see
+    __device__ __forceinline__ void full(const WindowArgs& p, const step::Seen& seen, uint32_t v0, uint32_t n, uint32_t& first, uint32_t& last) const {
+        seen.full(first_pos, last_pos, p.a.window, v0, n, first, last);
     }
 };
 
@@ -152,8 +153,7 @@ __device__ __forceinline__ void stage_queries(const WindowArgs& p, const RowTile
     const uint32_t steps = min(p.plan.dim64 - kBlockSteps * block, kBlockSteps), e0 = 64 * kBlockSteps * block;
     for (uint32_t i = threadIdx.x; i < kRows * steps * 16; i += blockDim.x) {
         const uint32_t r = i / (steps * 16), quad = i - r * (steps * 16), s = quad >> 4, c = (quad >> 2) & 3u, g = quad & 3u;
-        v4i_t x = {0, 0, 0, 0};
-        if (r < w.R) x = elements(query_of(p, w, r), e0 + 4 * quad, p.c.dim, p.q_vec, 0);
+        const v4i_t x = elements(query_of(p, w, min(r, w.R - 1)), e0 + 4 * quad, p.c.dim, p.q_vec, 0);
         uint32_t pl[3];
         three_planes(x, pl, over);
         uint32_t* o = digits + (((s * 3 * 4 + g) * kRows + r) << 2) + c;
@@ -282,8 +282,9 @@ __device__ __forceinline__ void make_factors(const WindowArgs& p, uint32_t group
         for (uint32_t i = threadIdx.x; i < 2 * kFactors; i += kBlock) p.factors[i] = factors[i];
 }
 
-// Loads of the next positions are issued before this one's stores, so that waiting for them does not wait for the stores; that holds
-// where the number of stores is known, so a tile that all rows see in full goes straight, and others wait for everything in the end.
+// Loads of the next positions are issued before this one's stores, so that waiting for them does not wait for the stores; the compiler can
+// count on that where every way through a loop has the same number of stores.  Tiles that all rows see in full therefore have a loop of
+// their own, and the other ones wait for everything in the end.
 __device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }          // vmcnt 0
 
 // Scores of 32 rows with a chunk of the positions.  A wave takes 16 positions of each tile of 64 and all rows; it reads its keys from
@@ -326,7 +327,6 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
         stage_queries(p, w, 0, lds, over);
         __syncthreads();
     }
-    const uint32_t row_blocks = (w.R + 15) / 16;
     const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
     const int64_t* my_off = off + 16 * w.wave + w.col;
     const v4i_t* q_digits = reinterpret_cast<const v4i_t*>(lds) + w.kg * kRows + w.col;
@@ -372,15 +372,20 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
     }
     const double scale = (double)p.qk.s, inv = p.qk.inv, half = (double)(p.qk.s >> 1) + 0.5, limit = p.limit;
     bool large = false;
-#pragma unroll 1
-    for (uint32_t tile = 0; tile < tiles; tile++) {
+    auto body = [&](uint32_t tile, auto all_see) {
+        constexpr bool FULL = decltype(all_see)::value;
         v4i_t acc[2][5];
         uint32_t k_over = 0;
 #pragma unroll
         for (int rb = 0; rb < 2; rb++)
 #pragma unroll
             for (int g = 0; g < 5; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
-        auto planes_of = [&](const v4i_t (&y)[4], v4i_t (&kb)[3]) {
+        auto multiply = [&](const v4i_t (&y)[4], int step, auto&& then) {
+            v4i_t kb[3], f[3][2];
+#pragma unroll
+            for (int a = 0; a < 3; a++)
+#pragma unroll
+                for (int rb = 0; rb < 2; rb++) f[a][rb] = q_digits[(step * 12 + a * 4) * kRows + 16 * rb];
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 uint32_t pl[3];
@@ -388,28 +393,25 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
 #pragma unroll
                 for (int k = 0; k < 3; k++) kb[k][c] = (int)pl[k];
             }
+            then();
+            __builtin_amdgcn_sched_barrier(0);          // the loads that this frees registers for go first
+#pragma unroll
+            for (int a = 0; a < 3; a++)
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+#pragma unroll
+                    for (int rb = 0; rb < 2; rb++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[k], f[a][rb], acc[rb][a + k], 0, 0, 0);
         };
+        const uint32_t next_tile = min(tile + 1, tiles - 1);
         if constexpr (STEPS > 0) {
-            const int32_t* next = key_of(min(tile + 1, tiles - 1));
+            const int32_t* next = key_of(next_tile);
 #pragma unroll
             for (int s = 0; s < STEPS; s++) {
-                v4i_t kb[3], f[3][2];
-#pragma unroll
-                for (int a = 0; a < 3; a++)
-#pragma unroll
-                    for (int rb = 0; rb < 2; rb++) f[a][rb] = q_digits[(s * 12 + a * 4) * kRows + 16 * rb];
                 if (s == STEPS - 1) {
 #pragma unroll
                     for (int c = 0; c < 4; c++) x[s][c] &= last_mask[c];
                 }
-                planes_of(x[s], kb);
-                fetch_step(next, s);
-#pragma unroll
-                for (int a = 0; a < 3; a++)
-#pragma unroll
-                    for (int k = 0; k < 3; k++)
-#pragma unroll
-                        for (int rb = 0; rb < 2; rb++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[k], f[a][rb], acc[rb][a + k], 0, 0, 0);
+                multiply(x[s], s, [&]() { fetch_step(next, s); });
             }
         } else {
 #pragma unroll 1
@@ -419,28 +421,18 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
                     stage_queries(p, w, s / kBlockSteps, lds, over);
                     __syncthreads();
                 }
-                v4i_t kb[3];
-                planes_of(x[0], kb);
-                if (s + 1 < steps) fetch(tile, s + 1);
-                else if (tile + 1 < tiles) fetch(tile + 1, 0);
-#pragma unroll
-                for (uint32_t rb = 0; rb < 2; rb++) {
-                    if (rb >= row_blocks) break;
-#pragma unroll
-                    for (int a = 0; a < 3; a++) {
-                        const v4i_t f = q_digits[((s % kBlockSteps) * 12 + a * 4) * kRows + 16 * rb];
-#pragma unroll
-                        for (int k = 0; k < 3; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[k], f, acc[rb][a + k], 0, 0, 0);
-                    }
-                }
+                multiply(x[0], (int)(s % kBlockSteps), [&]() { fetch(s + 1 < steps ? tile : next_tile, s + 1 < steps ? s + 1 : 0); });
             }
         }
         // register i of lane l: position 4 (l / 16) + i of the wave's 16, row l % 16 of a block
-        const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, k0 = seen.tile(v) * kCols, t0 = k0 + in_tile;
+        const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, t0 = seen.tile(v) * kCols + in_tile;
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) large |= off[tile * kCols + in_tile + i] == -1;          // wide_scores knows what to do with them
         large |= (k_over & kOver) && off[tile * kCols + 16 * w.wave + w.col] >= 0;
-        auto rescale = [&](uint32_t rb, uint32_t there, v4u_t& q, v4u_t& rem) {
+#pragma unroll
+        for (uint32_t rb = 0; rb < 2; rb++) {
+            const uint32_t there = FULL ? 15u : seen_of_four(p, pos[rb], t0);
+            v4u_t q, rem;
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
                 double y = (double)acc[rb][4][i];
@@ -453,30 +445,25 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
                 if constexpr (REM) rem[i] = (int32_t)__builtin_fma(-quotient, scale, y);
                 mx[rb] = max(mx[rb], here ? q[i] : INT32_MIN);
             }
-        };
-        if (w.all_see(p, k0)) {
-#pragma unroll
-            for (uint32_t rb = 0; rb < 2; rb++) {
-                v4u_t q, rem;
-                __builtin_amdgcn_sched_barrier(0);          // one block's numbers in registers at a time
-                rescale(rb, 15u, q, rem);
-                *reinterpret_cast<v4u_t*>(p.scores.at(row[rb], t0, v)) = q;
-                if constexpr (REM) *reinterpret_cast<v4u_t*>(p.a.d_scores_rem + row[rb] * p.a.max_len + t0) = rem;
+            int32_t* to = p.scores.at(row[rb], t0, v);
+            if constexpr (FULL) *reinterpret_cast<v4u_t*>(to) = q;
+            else store_four(to, q, there);
+            if constexpr (REM) {
+                int32_t* to_rem = p.a.d_scores_rem + row[rb] * p.a.max_len + t0;
+                if constexpr (FULL) *reinterpret_cast<v4u_t*>(to_rem) = rem;
+                else store_four(to_rem, rem, there);
             }
-        } else {
-#pragma unroll 1
-            for (uint32_t rb = 0; rb < row_blocks; rb++) {
-                const uint32_t there = 16 * rb + w.col >= w.R ? 0 : seen_of_four(p, rb ? pos[1] : pos[0], t0);
-                const size_t to = rb ? row[1] : row[0];
-                v4u_t q, rem;
-                if (rb) rescale(1, there, q, rem);
-                else rescale(0, there, q, rem);
-                store_four(p.scores.at(to, t0, v), q, there);
-                if constexpr (REM) store_four(p.a.d_scores_rem + to * p.a.max_len + t0, rem, there);
-            }
-            wait_for_memory();
         }
-    }
+        if constexpr (!FULL) wait_for_memory();
+    };
+    uint32_t full0, full1, tile = 0;
+    w.full(p, seen, v0, tiles, full0, full1);
+#pragma unroll 1
+    for (; tile < full0; tile++) body(tile, std::false_type{});
+#pragma unroll 1
+    for (; tile < full1; tile++) body(tile, std::true_type{});
+#pragma unroll 1
+    for (; tile < tiles; tile++) body(tile, std::false_type{});
     if (__any((over & kOver) != 0) && w.lane == 0) q_over = 1;          // the queries' digits were made by all threads
     __syncthreads();
     if (q_over || __any(large)) {
@@ -504,6 +491,7 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
 template <bool FACTORS, bool SHIFTED>
 __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
     __shared__ int32_t top[kRows];
+    __shared__ unsigned long long sums[kRows];
     __shared__ double factors[FACTORS ? 2 * kFactors : 1];
     RowTile w;
     if (!w.find(p, blockIdx.x)) return;
@@ -511,7 +499,10 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
     const uint32_t v0 = blockIdx.y * p.plan.exp_cols;
     if (v0 >= seen.tiles) return;
     const uint32_t tiles = min(p.plan.exp_cols, seen.tiles - v0), parts = (seen.tiles - 1) / p.plan.score_cols + 1;
-    if (threadIdx.x < kRows) top[threadIdx.x] = INT32_MIN;
+    if (threadIdx.x < kRows) {
+        top[threadIdx.x] = INT32_MIN;
+        sums[threadIdx.x] = 0;
+    }
     bool computed = false;
     if constexpr (FACTORS) {
         computed = !__any(p.differs[w.lane] != 0);
@@ -526,94 +517,104 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
     __syncthreads();
     if (blockIdx.y == 0 && p.a.d_max && threadIdx.x < w.R) p.a.d_max[w.row(p, threadIdx.x)] = top[threadIdx.x];
     uint32_t bad = 0;
-    const uint32_t last = ((uint32_t)1 << p.a.bit_shift) - 1, groups = (tiles + 3) / 4, items = w.wave < w.R ? ((w.R - 1 - w.wave) / 4 + 1) * groups : 0;
-    // item `it`: 256 positions of tiles 4 g .. of row r
-    struct Place {
-        uint32_t r, v, t, there;
-        bool full;
-        size_t row;
+    const uint32_t last = ((uint32_t)1 << p.a.bit_shift) - 1, groups = (tiles + 3) / 4, mine = w.wave < w.R ? (w.R - 1 - w.wave) / 4 + 1 : 0;          // rows of the wave
+    uint32_t full0, full1;
+    w.full(p, seen, v0, tiles, full0, full1);
+    full0 = (full0 + 3) / 4;          // in groups of four tiles, of which a lane takes four positions
+    full1 = computed && full1 / 4 > full0 ? full1 / 4 : full0;
+    auto entry = [&](uint32_t below, uint32_t d) { return (int32_t)__builtin_rint(factors[d / kFactors] * factors[kFactors + d % kFactors]); };
+    auto add = [&](uint32_t r, unsigned long long sum) {
+        sum += __shfl_xor(sum, 1, 64);
+        sum += __shfl_xor(sum, 2, 64);
+        if ((w.lane & 3u) == 0) atomicAdd(&sums[r], sum);
     };
-    auto place = [&](uint32_t it) {
-        Place a;
-        const uint32_t k = it / groups, g = it - k * groups;
-        a.r = w.wave + 4 * k;
-        a.row = w.row(p, a.r);
-        a.full = 4 * g + 4 <= tiles;
-        if (a.full) {
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) a.full = a.full && w.all_see(p, seen.tile(v0 + 4 * g + j) * kCols);
-        }
-        a.v = v0 + 4 * g + w.lane / 16;
-        a.t = seen.tile(a.v) * kCols + 4 * w.lane % kCols;
-        a.there = a.full ? 15u : a.v < v0 + tiles ? seen_of_four(p, w.pos_of(p, a.r), a.t) : 0;
-        return a;
-    };
-    auto load = [&](const Place& a, v4u_t& x) {
-        const int32_t* from = p.scores.at(a.row, a.t, a.v);
-        if (a.full) {
-            x = *reinterpret_cast<const v4u_t*>(from);
-        } else {
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) x[j] = (a.there >> j) & 1u ? from[j] : INT32_MIN;
-        }
-    };
-    Place at, next;
-    v4u_t x, x_next;
-    unsigned long long sum = 0;
+    const uint32_t count = full1 - full0, items = mine * count;
     if (items) {
-        next = place(0);
-        load(next, x_next);
-    }
-#pragma unroll 1
-    for (uint32_t it = 0; it < items; it++) {
-        at = next;
-        x = x_next;
-        if (it + 1 < items) {
-            next = place(it + 1);
-            load(next, x_next);
-        }
-        const int32_t mx = top[at.r];
-        v4u_t e, shifted;
-        if (computed) {
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t below = (uint32_t)mx - (uint32_t)x[j], d = min(below, last);          // entry 0 stands in for those before it
-                shifted[j] = (int32_t)(0 - below);
-                e[j] = (int32_t)__builtin_rint(factors[d / kFactors] * factors[kFactors + d % kFactors]);
-                const bool here = (at.there >> j) & 1u;
-                sum += (uint32_t)(here ? e[j] : 0);
-                if (here && below > last) bad |= (uint32_t)kWitIndex;
+        // item i: group full0 + i % count of the wave's row i / count; two at a time, each in registers of its own
+        struct Item {
+            uint32_t r, t, v;
+            size_t row;
+        };
+        uint32_t k = 0, g = 0;
+        auto next_item = [&]() {
+            Item a;
+            a.r = w.wave + 4 * k;
+            a.row = w.row(p, a.r);
+            a.v = v0 + 4 * (full0 + g) + w.lane / 16;
+            a.t = seen.tile(a.v) * kCols + 4 * w.lane % kCols;
+            if (++g == count) {
+                g = 0;
+                if (k + 1 < mine) k++;
             }
-        } else {
+            return a;
+        };
+        auto load = [&](const Item& a) { return *reinterpret_cast<const v4u_t*>(p.scores.at(a.row, a.t, a.v)); };
+        auto work = [&](const Item& a, const v4u_t& x) {
+            const int32_t mx = top[a.r];
+            v4u_t e, shifted;
+            unsigned long long sum = 0;
+            uint32_t most = 0;
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
-                const int64_t idx = (int64_t)x[j] - mx + last;
+                const uint32_t below = (uint32_t)mx - (uint32_t)x[j];
+                most = max(most, below);
+                shifted[j] = (int32_t)(0 - below);
+                e[j] = entry(below, min(below, last));          // entry 0 stands in for those before it
+                sum += (uint32_t)e[j];
+            }
+            if (most > last) bad |= (uint32_t)kWitIndex;
+            *reinterpret_cast<v4u_t*>(p.exps.at(a.row, a.t, a.v)) = e;
+            if constexpr (SHIFTED) *reinterpret_cast<v4u_t*>(p.a.d_shifted + a.row * p.a.max_len + a.t) = shifted;
+            add(a.r, sum);
+        };
+        Item a = next_item();
+        v4u_t x = load(a);
+        uint32_t it = 0;
+#pragma unroll 1
+        for (; it + 2 <= items; it += 2) {
+            const Item b = next_item();
+            const v4u_t y = load(b);
+            __builtin_amdgcn_sched_barrier(0);
+            work(a, x);
+            a = next_item();
+            x = load(a);
+            __builtin_amdgcn_sched_barrier(0);
+            work(b, y);
+        }
+        if (it < items) work(a, x);
+    }
+    for (uint32_t k = 0; k < mine; k++) {
+        const uint32_t r = w.wave + 4 * k, pos = w.pos_of(p, r);
+        const size_t row = w.row(p, r);
+        const int32_t mx = top[r];
+        unsigned long long sum = 0;
+        for (uint32_t g = full0 > 0 ? 0 : full1; g < groups; g = g + 1 == full0 ? full1 : g + 1) {
+            const uint32_t v = v0 + 4 * g + w.lane / 16, t = seen.tile(v) * kCols + 4 * w.lane % kCols, there = v < v0 + tiles ? seen_of_four(p, pos, t) : 0;
+            if (!there) continue;
+            const int32_t* from = p.scores.at(row, t, v);
+            v4u_t x, e, shifted;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) x[j] = (there >> j) & 1u ? from[j] : mx;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t below = (uint32_t)mx - (uint32_t)x[j];
+                const int64_t idx = (int64_t)last - below;
                 const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
-                e[j] = p.a.d_exp_table[ok ? idx : 0];
-                shifted[j] = (int32_t)((int64_t)x[j] - mx);
-                if ((at.there >> j) & 1u) {
+                e[j] = computed ? entry(below, min(below, last)) : p.a.d_exp_table[ok ? idx : 0];
+                shifted[j] = (int32_t)(0 - below);
+                if ((there >> j) & 1u) {
                     if (!ok) bad |= (uint32_t)kWitIndex;
                     if (e[j] < 0) bad |= (uint32_t)kWitSum;
                     sum += (unsigned long long)max(e[j], 0);
                 }
             }
+            store_four(p.exps.at(row, t, v), e, there);
+            if constexpr (SHIFTED) store_four(p.a.d_shifted + row * p.a.max_len + t, shifted, there);
         }
-        int32_t* to = p.exps.at(at.row, at.t, at.v);
-        if (at.full) {
-            *reinterpret_cast<v4u_t*>(to) = e;
-            if constexpr (SHIFTED) *reinterpret_cast<v4u_t*>(p.a.d_shifted + at.row * p.a.max_len + at.t) = shifted;
-        } else {
-            store_four(to, e, at.there);
-            if constexpr (SHIFTED) store_four(p.a.d_shifted + at.row * p.a.max_len + at.t, shifted, at.there);
-            wait_for_memory();
-        }
-        if (it + 1 == items || next.r != at.r) {
-#pragma unroll
-            for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
-            if (w.lane == 0) atomicAdd(&p.sums[at.row], sum);
-            sum = 0;
-        }
+        add(r, sum);
     }
+    __syncthreads();
+    if (threadIdx.x < w.R) atomicAdd(&p.sums[w.row(p, threadIdx.x)], sums[threadIdx.x]);
     if (bad) atomicOr(p.status, bad);
 }
 
@@ -630,7 +631,7 @@ struct ValueLds {
     uint32_t digits[2][PP * 4 * kRows * 4];
     int64_t off[2][step::kOffsetTiles * kCols];
     unsigned long long p_sum[kRows];
-    uint32_t third[2], wide;          // the last tile with digits in the third plane (and 1), of even and odd ones
+    uint32_t third[2], wide, outside;          // the last tile with digits in the third plane (and 1), of even and odd ones; whether a page is outside the cache
 };
 
 template <int PP, bool WIDE, Written W>
@@ -640,38 +641,40 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     const uint32_t v0 = chunk * p.plan.value_cols, tiles = min(p.plan.value_cols, seen.tiles - v0), dim = p.c.dim;
     // of the probabilities: this thread's row and its four positions of a tile
     const uint32_t r = threadIdx.x >> 4, part = threadIdx.x & 15u, rr = min(r, w.R - 1), pos = w.pos_of(p, rr);
-    const bool mine = r < w.R;
     const size_t row = w.row(p, rr);
     unsigned long long sum = p.sums[row], all = 0;
     if (sum == 0) {
-        if (mine) bad |= (uint32_t)kWitSum;
+        bad |= (uint32_t)kWitSum;
         sum = 1;
     }
-    if (!WIDE && mine && group == 0 && chunk == 0 && part == 0 && p.a.d_sum) store_sum(&p.a.d_sum[row], sum, bad);
+    if (!WIDE && r < w.R && group == 0 && chunk == 0 && part == 0 && p.a.d_sum) store_sum(&p.a.d_sum[row], sum, bad);
     const double inv = 1.0 / (double)sum, scale = (double)p.a.prob_scale, half = (double)(sum >> 1) + 0.5, whole_sum = (double)sum, odd = (double)(sum & 1) - 1.0;
     const bool plain = PP == 3 && __all(sum < kPlainSum);
-    const uint32_t e0 = group * step::kValueDims + 16 * w.wave, row_blocks = (w.R + 15) / 16;
-    const int32_t* values = p.c.d_v + (int64_t)w.kv * p.c.head_stride + min(e0 + w.col, dim - 1);
-    const bool multiplies = e0 < dim;
+    const uint32_t e0 = group * step::kValueDims + 16 * w.wave;
+    const int32_t* values = p.c.d_v + (int64_t)w.kv * p.c.head_stride + min(e0 + w.col, dim - 1);          // waves behind the last element take it again
     auto make_offsets = [&](uint32_t tile) {
         const uint32_t n = min(K, tiles - tile) * kCols;
-        for (uint32_t i = threadIdx.x; i < n; i += kValueThreads) lds.off[(tile / K) & 1][i] = offset_of(p, w, seen, seen.tile(v0 + tile + i / kCols) * kCols + i % kCols);
+        for (uint32_t i = threadIdx.x; i < n; i += kValueThreads) {
+            const int64_t o = offset_of(p, w, seen, seen.tile(v0 + tile + i / kCols) * kCols + i % kCols);
+            lds.off[(tile / K) & 1][i] = o;
+            if (o == -1) lds.outside = 1;
+        }
     };
     auto offsets = [&](uint32_t tile) { return lds.off[(tile / K) & 1] + (tile % K) * kCols; };
     int32_t x[16];
     v4u_t e;
-    auto fetch = [&](uint32_t tile) {
+    auto fetch_values = [&](uint32_t tile) {
         const int64_t* o = offsets(tile) + 16 * w.kg;
-        if (multiplies) {
 #pragma unroll
-            for (uint32_t j = 0; j < 16; j++) x[j] = values[max(o[j], (int64_t)0)];
-        }
-        const uint32_t k0 = seen.tile(v0 + tile) * kCols, t = k0 + 4 * part;
+        for (uint32_t j = 0; j < 16; j++) x[j] = values[max(o[j], (int64_t)0)];
+    };
+    auto fetch_exps = [&](uint32_t tile, auto all_see) {
+        const uint32_t t = seen.tile(v0 + tile) * kCols + 4 * part;
         const int32_t* from = p.exps.at(row, t, v0 + tile);
-        if (w.all_see(p, k0)) {
+        if constexpr (decltype(all_see)::value) {
             e = *reinterpret_cast<const v4u_t*>(from);
         } else {
-            const uint32_t there = mine ? seen_of_four(p, pos, t) : 0;
+            const uint32_t there = seen_of_four(p, pos, t);
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) e[j] = (there >> j) & 1u ? from[j] : 0;
         }
@@ -682,13 +685,9 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
 #pragma unroll
         for (int g = 0; g < G; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
     uint32_t over = 0;
-    __syncthreads();
-    make_offsets(0);
-    if (threadIdx.x < 2) lds.third[threadIdx.x] = 0;
-    __syncthreads();
-    fetch(0);
-#pragma unroll 1
-    for (uint32_t tile = 0; tile < tiles; tile++) {
+    // a tile and, if it is not the last one, the loads of the next; FULL: all rows see this tile's positions and the next one's
+    auto body = [&](uint32_t tile, auto all_see) {
+        constexpr bool FULL = decltype(all_see)::value;
         // operands and probabilities first, then the next tile's loads, then this one's stores
         v4i_t vb[VP];
 #pragma unroll
@@ -700,9 +699,7 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
 #pragma unroll
             for (int k = 0; k < VP; k++) vb[k][c] = (int)v[k];
         }
-        const uint32_t k0 = seen.tile(v0 + tile) * kCols, t = k0 + 4 * part;
-        const bool full = w.all_see(p, k0);
-        const uint32_t there = full ? 15u : mine ? seen_of_four(p, pos, t) : 0;
+        const uint32_t t = seen.tile(v0 + tile) * kCols + 4 * part, there = FULL ? 15u : seen_of_four(p, pos, t);
         v4u_t pr, query;
         if (plain) {
 #pragma unroll
@@ -725,16 +722,18 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
                 }
             }
         }
-        if (tile + 1 < tiles) {
+        if (FULL || tile + 1 < tiles) {
             if ((tile + 1) % K == 0) {
                 make_offsets(tile + 1);
                 __syncthreads();
             }
-            fetch(tile + 1);
+            fetch_values(tile + 1);
+            fetch_exps(tile + 1, all_see);
+            __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (W != kNone) {
             const size_t o = row * p.a.max_len + t;
-            if (W == kBoth && full) {
+            if constexpr (W == kBoth && FULL) {
                 *reinterpret_cast<v4u_t*>(p.a.d_prob + o) = pr;
                 *reinterpret_cast<v4u_t*>(p.a.d_query + o) = query;
             } else {
@@ -744,11 +743,16 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
             }
         }
         v4i_t d;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) d[j] = (there >> j) & 1u ? pr[j] : 0;
+        if (lds.outside) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++)
+                if (offsets(tile)[4 * part + j] < 0) d[j] = 0;          // a page outside: no value
+        }
         uint32_t large = 0;
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
-            const bool used = ((there >> j) & 1u) && offsets(tile)[4 * part + j] >= 0;          // a page outside: no value
-            d[j] = used ? pr[j] : 0;
             large |= (uint32_t)d[j] + 0x8080u;
             if constexpr (WIDE) all += (uint32_t)d[j];
         }
@@ -764,21 +768,38 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
 #pragma unroll
         for (int k = 0; k < PP; k++) to[k * 16 * kRows] = pl[k];
         __syncthreads();
-        if (!multiplies) continue;
         const v4i_t* pa = reinterpret_cast<const v4i_t*>(lds.digits[tile & 1]) + w.kg * kRows + w.col;
-        const int planes = PP == 3 && lds.third[tile & 1] != tile + 1 ? 2 : PP;
+        auto multiply = [&](auto a) {
+            v4i_t f[2];
 #pragma unroll
-        for (uint32_t rb = 0; rb < 2; rb++) {
-            if (rb >= row_blocks) break;
+            for (uint32_t rb = 0; rb < 2; rb++) f[rb] = pa[decltype(a)::value * 4 * kRows + 16 * rb];
 #pragma unroll
-            for (int a = 0; a < PP; a++) {
-                if (a >= planes) break;
-                const v4i_t f = pa[a * 4 * kRows + 16 * rb];
+            for (int k = 0; k < VP; k++)
 #pragma unroll
-                for (int k = 0; k < VP; k++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[k], f, acc[rb][a + k], 0, 0, 0);
-            }
-        }
-    }
+                for (uint32_t rb = 0; rb < 2; rb++) acc[rb][decltype(a)::value + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[k], f[rb], acc[rb][decltype(a)::value + k], 0, 0, 0);
+        };
+        multiply(std::integral_constant<int, 0>{});
+        multiply(std::integral_constant<int, 1>{});
+        if (PP > 3 || lds.third[tile & 1] == tile + 1) multiply(std::integral_constant<int, 2>{});
+        if constexpr (PP > 3) multiply(std::integral_constant<int, 3>{});
+    };
+    __syncthreads();
+    if (threadIdx.x < 2) lds.third[threadIdx.x] = 0;
+    if (threadIdx.x == 0) lds.outside = 0;
+    __syncthreads();
+    make_offsets(0);
+    __syncthreads();
+    fetch_values(0);
+    fetch_exps(0, std::false_type{});
+    wait_for_memory();
+    uint32_t full0, full1, tile = 0;
+    w.full(p, seen, v0, tiles, full0, full1);
+#pragma unroll 1
+    for (; tile < full0; tile++) body(tile, std::false_type{});
+#pragma unroll 1
+    for (; tile + 1 < full1; tile++) body(tile, std::true_type{});
+#pragma unroll 1
+    for (; tile < tiles; tile++) body(tile, std::false_type{});
     if constexpr (WIDE) {
 #pragma unroll
         for (int k = 8; k >= 1; k >>= 1) all += __shfl_xor(all, k, 64);
