@@ -283,8 +283,8 @@ __device__ __forceinline__ void make_factors(const WindowArgs& p, uint32_t group
 }
 
 // Loads of the next positions are issued before this one's stores, so that waiting for them does not wait for the stores; the compiler can
-// count on that where every way through a loop has the same number of stores.  Tiles that all rows see in full therefore have a loop of
-// their own, and the other ones wait for everything in the end.
+// count on that where every way to the wait has the same number of stores behind the loads.  Tiles that all rows see in full therefore have a
+// loop of their own, nothing is under way when it begins, and the other tiles wait for everything in the end.
 __device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }          // vmcnt 0
 
 // Scores of 32 rows with a chunk of the positions.  A wave takes 16 positions of each tile of 64 and all rows; it reads its keys from
@@ -292,7 +292,7 @@ __device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0
 // Five accumulators become a sum in double precision, exact below 2^53, and below 2^50 the quotient of (y + s/2 + 1/2) / s needs no
 // second look: it is no nearer than 1 / (2 s) to a whole number, and the product with 1 / s off by at most 2^-52 of itself.
 template <int STEPS, bool VEC, bool REM>
-__global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p) {
+__global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ int32_t top[4][kRows];
     __shared__ uint32_t q_over;
@@ -394,7 +394,6 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
                 for (int k = 0; k < 3; k++) kb[k][c] = (int)pl[k];
             }
             then();
-            __builtin_amdgcn_sched_barrier(0);          // the loads that this frees registers for go first
 #pragma unroll
             for (int a = 0; a < 3; a++)
 #pragma unroll
@@ -431,6 +430,7 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
         large |= (k_over & kOver) && off[tile * kCols + 16 * w.wave + w.col] >= 0;
 #pragma unroll
         for (uint32_t rb = 0; rb < 2; rb++) {
+            __builtin_amdgcn_sched_barrier(0);
             const uint32_t there = FULL ? 15u : seen_of_four(p, pos[rb], t0);
             v4u_t q, rem;
 #pragma unroll
@@ -460,6 +460,7 @@ __global__ void __launch_bounds__(256, 3) wit_window_scores_kernel(WindowArgs p)
     w.full(p, seen, v0, tiles, full0, full1);
 #pragma unroll 1
     for (; tile < full0; tile++) body(tile, std::false_type{});
+    wait_for_memory();
 #pragma unroll 1
     for (; tile < full1; tile++) body(tile, std::true_type{});
 #pragma unroll 1
@@ -517,59 +518,63 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
     __syncthreads();
     if (blockIdx.y == 0 && p.a.d_max && threadIdx.x < w.R) p.a.d_max[w.row(p, threadIdx.x)] = top[threadIdx.x];
     uint32_t bad = 0;
-    const uint32_t last = ((uint32_t)1 << p.a.bit_shift) - 1, groups = (tiles + 3) / 4, mine = w.wave < w.R ? (w.R - 1 - w.wave) / 4 + 1 : 0;          // rows of the wave
+    const uint32_t last = ((uint32_t)1 << p.a.bit_shift) - 1, mine = w.wave < w.R ? (w.R - 1 - w.wave) / 4 + 1 : 0;          // rows of the wave
     uint32_t full0, full1;
     w.full(p, seen, v0, tiles, full0, full1);
-    full0 = (full0 + 3) / 4;          // in groups of four tiles, of which a lane takes four positions
-    full1 = computed && full1 / 4 > full0 ? full1 / 4 : full0;
-    auto entry = [&](uint32_t below, uint32_t d) { return (int32_t)__builtin_rint(factors[d / kFactors] * factors[kFactors + d % kFactors]); };
-    auto add = [&](uint32_t r, unsigned long long sum) {
-        sum += __shfl_xor(sum, 1, 64);
-        sum += __shfl_xor(sum, 2, 64);
-        if ((w.lane & 3u) == 0) atomicAdd(&sums[r], sum);
-    };
-    const uint32_t count = full1 - full0, items = mine * count;
+    if (!computed) full1 = full0;
+    auto entry = [&](uint32_t d) { return (int32_t)__builtin_rint(factors[d / kFactors] * factors[kFactors + d % kFactors]); };
+    const uint32_t groups = (full1 - full0 + 3) / 4, items = mine * groups;
     if (items) {
-        // item i: group full0 + i % count of the wave's row i / count; two at a time, each in registers of its own
+        // item i: four tiles, group i % groups, of the wave's row i / groups; two items at a time, each in registers of its own.  Lanes behind
+        // the last tile take it again, and leave it out of the sum.
         struct Item {
-            uint32_t r, t, v;
+            uint32_t r, g, t, v;
             size_t row;
         };
         uint32_t k = 0, g = 0;
         auto next_item = [&]() {
             Item a;
             a.r = w.wave + 4 * k;
+            a.g = g;
             a.row = w.row(p, a.r);
-            a.v = v0 + 4 * (full0 + g) + w.lane / 16;
+            a.v = v0 + min(full0 + 4 * g + w.lane / 16, full1 - 1);
             a.t = seen.tile(a.v) * kCols + 4 * w.lane % kCols;
-            if (++g == count) {
+            if (++g == groups) {
                 g = 0;
                 if (k + 1 < mine) k++;
             }
             return a;
         };
         auto load = [&](const Item& a) { return *reinterpret_cast<const v4u_t*>(p.scores.at(a.row, a.t, a.v)); };
+        unsigned long long sum = 0;
         auto work = [&](const Item& a, const v4u_t& x) {
             const int32_t mx = top[a.r];
             v4u_t e, shifted;
-            unsigned long long sum = 0;
+            unsigned long long four = 0;
             uint32_t most = 0;
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
                 const uint32_t below = (uint32_t)mx - (uint32_t)x[j];
                 most = max(most, below);
                 shifted[j] = (int32_t)(0 - below);
-                e[j] = entry(below, min(below, last));          // entry 0 stands in for those before it
-                sum += (uint32_t)e[j];
+                e[j] = entry(min(below, last));          // entry 0 stands in for those before it
+                four += (uint32_t)e[j];
             }
             if (most > last) bad |= (uint32_t)kWitIndex;
             *reinterpret_cast<v4u_t*>(p.exps.at(a.row, a.t, a.v)) = e;
             if constexpr (SHIFTED) *reinterpret_cast<v4u_t*>(p.a.d_shifted + a.row * p.a.max_len + a.t) = shifted;
-            add(a.r, sum);
+            sum += full0 + 4 * a.g + w.lane / 16 < full1 ? four : 0;
+            if (a.g + 1 == groups) {
+#pragma unroll
+                for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+                if (w.lane == 0) sums[a.r] = sum;
+                sum = 0;
+            }
         };
         Item a = next_item();
         v4u_t x = load(a);
         uint32_t it = 0;
+        wait_for_memory();
 #pragma unroll 1
         for (; it + 2 <= items; it += 2) {
             const Item b = next_item();
@@ -583,35 +588,43 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
         }
         if (it < items) work(a, x);
     }
-    for (uint32_t k = 0; k < mine; k++) {
-        const uint32_t r = w.wave + 4 * k, pos = w.pos_of(p, r);
-        const size_t row = w.row(p, r);
-        const int32_t mx = top[r];
-        unsigned long long sum = 0;
-        for (uint32_t g = full0 > 0 ? 0 : full1; g < groups; g = g + 1 == full0 ? full1 : g + 1) {
-            const uint32_t v = v0 + 4 * g + w.lane / 16, t = seen.tile(v) * kCols + 4 * w.lane % kCols, there = v < v0 + tiles ? seen_of_four(p, pos, t) : 0;
-            if (!there) continue;
-            const int32_t* from = p.scores.at(row, t, v);
-            v4u_t x, e, shifted;
+    __syncthreads();
+    // the other tiles, four rows of one at a time
+    const uint32_t others = tiles - (full1 - full0), quads = (w.R + 3) / 4;
+    for (uint32_t i = w.wave; i < others * quads; i += 4) {
+        const uint32_t j = i / quads, r = 4 * (i - j * quads) + w.lane / 16, v = v0 + (j < full0 ? j : j - full0 + full1), t = seen.tile(v) * kCols + 4 * w.col;
+        const uint32_t rr = min(r, w.R - 1), there = r < w.R ? seen_of_four(p, w.pos_of(p, rr), t) : 0;
+        const size_t row = w.row(p, rr);
+        const int32_t mx = top[rr];
+        const int32_t* from = p.scores.at(row, t, v);
+        v4u_t x = {mx, mx, mx, mx}, e, shifted;
+        if (there == 15u) {
+            x = *reinterpret_cast<const v4u_t*>(from);
+        } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) x[j] = (there >> j) & 1u ? from[j] : mx;
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t below = (uint32_t)mx - (uint32_t)x[j];
-                const int64_t idx = (int64_t)last - below;
-                const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
-                e[j] = computed ? entry(below, min(below, last)) : p.a.d_exp_table[ok ? idx : 0];
-                shifted[j] = (int32_t)(0 - below);
-                if ((there >> j) & 1u) {
-                    if (!ok) bad |= (uint32_t)kWitIndex;
-                    if (e[j] < 0) bad |= (uint32_t)kWitSum;
-                    sum += (unsigned long long)max(e[j], 0);
-                }
-            }
-            store_four(p.exps.at(row, t, v), e, there);
-            if constexpr (SHIFTED) store_four(p.a.d_shifted + row * p.a.max_len + t, shifted, there);
+            for (uint32_t m = 0; m < 3; m++)
+                if ((there >> m) & 1u) x[m] = from[m];
+            if (there >> 3) x[3] = from[3];
         }
-        add(r, sum);
+        unsigned long long sum = 0;
+#pragma unroll
+        for (uint32_t m = 0; m < 4; m++) {
+            const uint32_t below = (uint32_t)mx - (uint32_t)x[m];
+            const int64_t idx = (int64_t)last - below;
+            const bool ok = idx >= 0 && idx < ((int64_t)1 << p.a.index_bits);
+            e[m] = computed ? entry(min(below, last)) : p.a.d_exp_table[ok ? idx : 0];
+            shifted[m] = (int32_t)(0 - below);
+            if ((there >> m) & 1u) {
+                if (!ok) bad |= (uint32_t)kWitIndex;
+                if (e[m] < 0) bad |= (uint32_t)kWitSum;
+                sum += (unsigned long long)max(e[m], 0);
+            }
+        }
+        store_four(p.exps.at(row, t, v), e, there);
+        if constexpr (SHIFTED) store_four(p.a.d_shifted + row * p.a.max_len + t, shifted, there);
+#pragma unroll
+        for (int d = 8; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+        if (w.col == 0 && r < w.R) atomicAdd(&sums[r], sum);
     }
     __syncthreads();
     if (threadIdx.x < w.R) atomicAdd(&p.sums[w.row(p, threadIdx.x)], sums[threadIdx.x]);
@@ -729,7 +742,6 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
             }
             fetch_values(tile + 1);
             fetch_exps(tile + 1, all_see);
-            __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (W != kNone) {
             const size_t o = row * p.a.max_len + t;
@@ -796,6 +808,7 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     w.full(p, seen, v0, tiles, full0, full1);
 #pragma unroll 1
     for (; tile < full0; tile++) body(tile, std::false_type{});
+    wait_for_memory();
 #pragma unroll 1
     for (; tile + 1 < full1; tile++) body(tile, std::true_type{});
 #pragma unroll 1
