@@ -124,9 +124,10 @@ struct RowTile {
     }
 };
 
-// Offset of position t's token, -1 where its page is outside the cache, -2 where no row sees it.
+// Offset of position t's token; of the last one that is seen where no row sees t, so that nothing is read but what is there.  -1 where the
+// page is outside the cache.
 __device__ __forceinline__ int64_t offset_of(const WindowArgs& p, const RowTile& w, const step::Seen& seen, uint32_t t) {
-    if (!seen.any(t)) return -2;
+    if (!seen.any(t)) t = seen.hi - 1;
     const uint32_t pg = p.page(t);
     return token::token_offset(p.c, p.a.d_block_table[(size_t)w.b * p.a.table_stride + pg], t - pg * p.c.page_size);
 }
@@ -179,13 +180,14 @@ __device__ __forceinline__ void store_four(int32_t* to, v4u_t x, uint32_t there)
 }
 
 // The scores of a wave's positions with operands of any size, both from memory: sixteen rows at a time, four planes each.
-__device__ __forceinline__ void wide_scores(const WindowArgs& p, const RowTile& w, const step::Seen& seen, uint32_t v0, uint32_t tiles, const int64_t* off, int32_t mx[2], uint32_t& bad) {
+__device__ __forceinline__ void wide_scores(const WindowArgs& p, const RowTile& w, const step::Seen& seen, uint32_t v0, uint32_t tiles, int32_t mx[2], uint32_t& bad) {
     const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
     const uint32_t dim = p.c.dim;
 #pragma unroll 1
     for (uint32_t tile = 0; tile < tiles; tile++) {
-        const int32_t* k_row = keys + max(off[tile * kCols + 16 * w.wave + w.col], (int64_t)0);
         const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, t0 = seen.tile(v) * kCols + in_tile;
+        const int64_t k_off = offset_of(p, w, seen, seen.tile(v) * kCols + 16 * w.wave + w.col);
+        const int32_t* k_row = keys + max(k_off, (int64_t)0);
 #pragma unroll 1
         for (uint32_t rb = 0; 16 * rb < w.R; rb++) {
             const uint32_t r = min(16 * rb + w.col, w.R - 1);
@@ -241,7 +243,7 @@ __device__ __forceinline__ void wide_scores(const WindowArgs& p, const RowTile& 
                 y += (uint64_t)kCacheOffset * (uint64_t)(k_of + q_sum + kCacheOffset * dim);
                 uint32_t wide = 0;
                 int32_t qi, ri;
-                p.qk.apply(off[tile * kCols + in_tile + i] < 0 ? 0 : (int64_t)y, qi, ri, wide);          // a page outside: zero
+                p.qk.apply(__shfl(k_off < 0 ? 1 : 0, (int)(4 * w.kg + i), 64) ? 0 : (int64_t)y, qi, ri, wide);          // a page outside: zero
                 q[i] = qi;
                 rem[i] = ri;
                 if ((there >> i) & 1u) {
@@ -315,11 +317,13 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
     const uint32_t tiles = min(p.plan.score_cols, seen.tiles - v0), steps = p.plan.dim64, dim = p.c.dim, blocks = (steps + kBlockSteps - 1) / kBlockSteps;
     int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)min(steps, kBlockSteps) * 3 * 4 * kRows * 4);
     if (threadIdx.x == 0) q_over = 0;
+    bool outside = false;
     for (uint32_t i = threadIdx.x; i < tiles * kCols; i += 256) {
         const int64_t o = offset_of(p, w, seen, seen.tile(v0 + i / kCols) * kCols + i % kCols);
-        if (o == -1) bad |= (uint32_t)kWitIndex;
-        off[i] = o;
+        outside |= o < 0;
+        off[i] = max(o, (int64_t)0);
     }
+    if (outside) bad |= (uint32_t)kWitIndex;
     if (blockIdx.y == 0 && threadIdx.x < w.R) p.sums[w.row(p, threadIdx.x)] = 0;
     uint32_t over = 0;
     __syncthreads();
@@ -334,7 +338,7 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
     constexpr int S = STEPS ? STEPS : 1;
     v4i_t x[S][4];
     int32_t last_e[4], last_mask[4];
-    auto key_of = [&](uint32_t tile) { return keys + max(my_off[tile * kCols], (int64_t)0); };
+    auto key_of = [&](uint32_t tile) { return keys + my_off[tile * kCols]; };
     auto fetch_step = [&](const int32_t* k, int s) {
         if (s + 1 < STEPS) {
 #pragma unroll
@@ -372,10 +376,10 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
     }
     const double scale = (double)p.qk.s, inv = p.qk.inv, half = (double)(p.qk.s >> 1) + 0.5, limit = p.limit;
     bool large = false;
+    uint32_t k_over = 0;
     auto body = [&](uint32_t tile, auto all_see) {
         constexpr bool FULL = decltype(all_see)::value;
         v4i_t acc[2][5];
-        uint32_t k_over = 0;
 #pragma unroll
         for (int rb = 0; rb < 2; rb++)
 #pragma unroll
@@ -426,18 +430,21 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
         // register i of lane l: position 4 (l / 16) + i of the wave's 16, row l % 16 of a block
         const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, t0 = seen.tile(v) * kCols + in_tile;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) large |= off[tile * kCols + in_tile + i] == -1;          // wide_scores knows what to do with them
-        large |= (k_over & kOver) && off[tile * kCols + 16 * w.wave + w.col] >= 0;
-#pragma unroll
         for (uint32_t rb = 0; rb < 2; rb++) {
             __builtin_amdgcn_sched_barrier(0);
             const uint32_t there = FULL ? 15u : seen_of_four(p, pos[rb], t0);
             v4u_t q, rem;
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
-                double y = (double)acc[rb][4][i];
+                double y;
+                if constexpr (STEPS > 0 && STEPS < 4) {          // two of the sums fit 32 bits: 2 * 2^14 * 192 * 2^8 and 2^14 * 192
+                    const int32_t low = (acc[rb][1][i] << 8) + acc[rb][0][i], high = (acc[rb][4][i] << 8) + acc[rb][3][i];
+                    y = __builtin_fma((double)high, 0x1p24, __builtin_fma((double)acc[rb][2][i], 0x1p16, (double)low));
+                } else {
+                    y = (double)acc[rb][4][i];
 #pragma unroll
-                for (int g = 3; g >= 0; g--) y = __builtin_fma(y, 256.0, (double)acc[rb][g][i]);
+                    for (int g = 3; g >= 0; g--) y = __builtin_fma(y, 256.0, (double)acc[rb][g][i]);
+                }
                 const double t = y + half, quotient = __builtin_floor(t * inv);
                 const bool here = (there >> i) & 1u;
                 large |= here && __builtin_fabs(t) >= limit;
@@ -465,11 +472,12 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
     for (; tile < full1; tile++) body(tile, std::true_type{});
 #pragma unroll 1
     for (; tile < tiles; tile++) body(tile, std::false_type{});
-    if (__any((over & kOver) != 0) && w.lane == 0) q_over = 1;          // the queries' digits were made by all threads
+    if (__any((over & kOver) != 0 || outside) && w.lane == 0) q_over = 1;          // what all threads made for all waves
+    large |= (k_over & kOver) != 0;
     __syncthreads();
     if (q_over || __any(large)) {
         mx[0] = mx[1] = INT32_MIN;
-        wide_scores(p, w, seen, v0, tiles, off, mx, bad);
+        wide_scores(p, w, seen, v0, tiles, mx, bad);
     }
 #pragma unroll
     for (int rb = 0; rb < 2; rb++) {
@@ -669,8 +677,8 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
         const uint32_t n = min(K, tiles - tile) * kCols;
         for (uint32_t i = threadIdx.x; i < n; i += kValueThreads) {
             const int64_t o = offset_of(p, w, seen, seen.tile(v0 + tile + i / kCols) * kCols + i % kCols);
-            lds.off[(tile / K) & 1][i] = o;
-            if (o == -1) lds.outside = 1;
+            lds.off[(tile / K) & 1][i] = max(o, (int64_t)0);
+            if (o < 0) lds.outside = 1;
         }
     };
     auto offsets = [&](uint32_t tile) { return lds.off[(tile / K) & 1] + (tile % K) * kCols; };
@@ -679,7 +687,7 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     auto fetch_values = [&](uint32_t tile) {
         const int64_t* o = offsets(tile) + 16 * w.kg;
 #pragma unroll
-        for (uint32_t j = 0; j < 16; j++) x[j] = values[max(o[j], (int64_t)0)];
+        for (uint32_t j = 0; j < 16; j++) x[j] = values[o[j]];
     };
     auto fetch_exps = [&](uint32_t tile, auto all_see) {
         const uint32_t t = seen.tile(v0 + tile) * kCols + 4 * part;
@@ -714,7 +722,7 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
         }
         const uint32_t t = seen.tile(v0 + tile) * kCols + 4 * part, there = FULL ? 15u : seen_of_four(p, pos, t);
         v4u_t pr, query;
-        if (plain) {
+        if (FULL || plain) {
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
                 const double num = __builtin_fma((double)max(e[j], 0), scale, half), q = __builtin_floor(num * inv);
@@ -757,22 +765,17 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
         v4i_t d;
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) d[j] = (there >> j) & 1u ? pr[j] : 0;
-        if (lds.outside) {
+        if (!FULL && lds.outside) {
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++)
-                if (offsets(tile)[4 * part + j] < 0) d[j] = 0;          // a page outside: no value
+                if (offset_of(p, w, seen, t + j) < 0) d[j] = 0;          // a page outside: no value
         }
-        uint32_t large = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
-            large |= (uint32_t)d[j] + 0x8080u;
-            if constexpr (WIDE) all += (uint32_t)d[j];
-        }
+        if constexpr (WIDE) all += (uint64_t)(uint32_t)d[0] + (uint32_t)d[1] + (uint32_t)d[2] + (uint32_t)d[3];
         uint32_t pl[4];
         if constexpr (PP == 3) {
             uint32_t none = 0;
             three_planes(d, pl, none);
-            if (__any(large >> 16) && w.lane == 0) lds.third[tile & 1] = tile + 1;
+            if (__any(pl[2] != 0) && w.lane == 0) lds.third[tile & 1] = tile + 1;
         } else {
             transpose4(digits_of(d[0]), digits_of(d[1]), digits_of(d[2]), digits_of(d[3]), pl);
         }
@@ -810,7 +813,7 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     for (; tile < full0; tile++) body(tile, std::false_type{});
     wait_for_memory();
 #pragma unroll 1
-    for (; tile + 1 < full1; tile++) body(tile, std::true_type{});
+    for (; plain && tile + 1 < full1 && !lds.outside; tile++) body(tile, std::true_type{});
 #pragma unroll 1
     for (; tile < tiles; tile++) body(tile, std::false_type{});
     if constexpr (WIDE) {
