@@ -639,13 +639,14 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
     if (bad) atomicOr(p.status, bad);
 }
 
-// Probabilities of 32 rows and their products with 128 elements of the values, over a chunk of the positions.  Sixteen threads a row make
-// the digits of 64 positions in LDS while the waves multiply the 64 before them; a wave takes 16 elements and all rows, and turns
-// its values into operands in registers.  A probability is floor((e P + floor(S/2)) / S) from one product in double precision, as the
-// scores' quotients are, where S is below 2^28 and P at most 2^22; the remainder of the division gives the lookup's query.
-constexpr uint32_t kValueThreads = 512;
+// Probabilities of 32 rows and their products with 128 elements of the values, over a chunk of the positions.  Eight threads a row make
+// the digits of 64 positions in LDS; a wave takes 32 elements and all rows, and turns its values into operands in registers.  A
+// probability is floor((e P + floor(S/2)) / S) from one product in double precision, as the scores' quotients are, where S is below 2^28 and P
+// at most 2^22; the remainder of the division gives the lookup's query.
+constexpr uint32_t kValueThreads = 256;
 constexpr uint64_t kPlainSum = (uint64_t)1 << 28;
 enum Written { kNone, kBoth, kSome };          // of the probabilities and queries
+typedef int v2u_t __attribute__((ext_vector_type(2), aligned(4)));
 
 template <int PP>
 struct ValueLds {
@@ -660,8 +661,8 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     constexpr int VP = WIDE ? 4 : 3, G = PP + VP - 1;
     constexpr uint32_t K = step::kOffsetTiles;
     const uint32_t v0 = chunk * p.plan.value_cols, tiles = min(p.plan.value_cols, seen.tiles - v0), dim = p.c.dim;
-    // of the probabilities: this thread's row and its four positions of a tile
-    const uint32_t r = threadIdx.x >> 4, part = threadIdx.x & 15u, rr = min(r, w.R - 1), pos = w.pos_of(p, rr);
+    // of the probabilities: this thread's row and its eight positions of a tile
+    const uint32_t r = threadIdx.x >> 3, part = threadIdx.x & 7u, rr = min(r, w.R - 1), pos = w.pos_of(p, rr);
     const size_t row = w.row(p, rr);
     unsigned long long sum = p.sums[row], all = 0;
     if (sum == 0) {
@@ -671,8 +672,11 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     if (!WIDE && r < w.R && group == 0 && chunk == 0 && part == 0 && p.a.d_sum) store_sum(&p.a.d_sum[row], sum, bad);
     const double inv = 1.0 / (double)sum, scale = (double)p.a.prob_scale, half = (double)(sum >> 1) + 0.5, whole_sum = (double)sum, odd = (double)(sum & 1) - 1.0;
     const bool plain = PP == 3 && __all(sum < kPlainSum);
-    const uint32_t e0 = group * step::kValueDims + 16 * w.wave;
-    const int32_t* values = p.c.d_v + (int64_t)w.kv * p.c.head_stride + min(e0 + w.col, dim - 1);          // waves behind the last element take it again
+    // of the values: elements e0 + 2 col, + 1; lanes behind the last element take it again
+    const uint32_t e0 = group * step::kValueDims + 32 * w.wave, el = e0 + 2 * w.col;
+    const bool pairs = dim % 2 == 0;
+    const int32_t* values = p.c.d_v + (int64_t)w.kv * p.c.head_stride;
+    const int32_t *value0 = values + (pairs ? min(el, dim - 2) : min(el, dim - 1)), *value1 = values + min(el + 1, dim - 1);
     auto make_offsets = [&](uint32_t tile) {
         const uint32_t n = min(K, tiles - tile) * kCols;
         for (uint32_t i = threadIdx.x; i < n; i += kValueThreads) {
@@ -682,63 +686,80 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
         }
     };
     auto offsets = [&](uint32_t tile) { return lds.off[(tile / K) & 1] + (tile % K) * kCols; };
-    int32_t x[16];
-    v4u_t e;
+    v2u_t x[16];
+    v4u_t e[2];
     auto fetch_values = [&](uint32_t tile) {
         const int64_t* o = offsets(tile) + 16 * w.kg;
+        if (pairs) {
 #pragma unroll
-        for (uint32_t j = 0; j < 16; j++) x[j] = values[o[j]];
-    };
-    auto fetch_exps = [&](uint32_t tile, auto all_see) {
-        const uint32_t t = seen.tile(v0 + tile) * kCols + 4 * part;
-        const int32_t* from = p.exps.at(row, t, v0 + tile);
-        if constexpr (decltype(all_see)::value) {
-            e = *reinterpret_cast<const v4u_t*>(from);
+            for (uint32_t j = 0; j < 16; j++) x[j] = *reinterpret_cast<const v2u_t*>(value0 + o[j]);
         } else {
-            const uint32_t there = seen_of_four(p, pos, t);
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) e[j] = (there >> j) & 1u ? from[j] : 0;
+            for (uint32_t j = 0; j < 16; j++) x[j] = v2u_t{value0[o[j]], value1[o[j]]};
         }
     };
-    v4i_t acc[2][G];
+    auto fetch_exps = [&](uint32_t tile, auto all_see) {
+        const uint32_t t = seen.tile(v0 + tile) * kCols + 8 * part;
+        const int32_t* from = p.exps.at(row, t, v0 + tile);
+        if constexpr (decltype(all_see)::value) {
+            e[0] = *reinterpret_cast<const v4u_t*>(from);
+            e[1] = *reinterpret_cast<const v4u_t*>(from + 4);
+        } else {
 #pragma unroll
-    for (int rb = 0; rb < 2; rb++)
+            for (uint32_t h = 0; h < 2; h++) {
+                const uint32_t there = seen_of_four(p, pos, t + 4 * h);
+                if (there == 15u) {
+                    e[h] = *reinterpret_cast<const v4u_t*>(from + 4 * h);
+                } else {
 #pragma unroll
-        for (int g = 0; g < G; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
+                    for (uint32_t j = 0; j < 4; j++) e[h][j] = (there >> j) & 1u ? from[4 * h + j] : 0;
+                }
+            }
+        }
+    };
+    v4i_t acc[2][2][G];          // [element of a pair][block of rows][exponent]
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+            for (int g = 0; g < G; g++) acc[j][rb][g] = v4i_t{0, 0, 0, 0};
     uint32_t over = 0;
     // a tile and, if it is not the last one, the loads of the next; FULL: all rows see this tile's positions and the next one's
     auto body = [&](uint32_t tile, auto all_see) {
         constexpr bool FULL = decltype(all_see)::value;
         // operands and probabilities first, then the next tile's loads, then this one's stores
-        v4i_t vb[VP];
+        v4i_t vb[2][VP];
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const v4i_t y = {x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
-            uint32_t v[4];
-            if constexpr (WIDE) four_planes(y, v);
-            else three_planes(y, v, over);
+        for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int k = 0; k < VP; k++) vb[k][c] = (int)v[k];
-        }
-        const uint32_t t = seen.tile(v0 + tile) * kCols + 4 * part, there = FULL ? 15u : seen_of_four(p, pos, t);
-        v4u_t pr, query;
+            for (int c = 0; c < 4; c++) {
+                const v4i_t y = {x[4 * c][j], x[4 * c + 1][j], x[4 * c + 2][j], x[4 * c + 3][j]};
+                uint32_t v[4];
+                if constexpr (WIDE) four_planes(y, v);
+                else three_planes(y, v, over);
+#pragma unroll
+                for (int k = 0; k < VP; k++) vb[j][k][c] = (int)v[k];
+            }
+        const uint32_t t = seen.tile(v0 + tile) * kCols + 8 * part, there = FULL ? 255u : seen_of_four(p, pos, t) | seen_of_four(p, pos, t + 4) << 4;
+        v4u_t pr[2], query[2];
         if (FULL || plain) {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const double num = __builtin_fma((double)max(e[j], 0), scale, half), q = __builtin_floor(num * inv);
-                pr[j] = (int32_t)q;
-                if constexpr (W != kNone) query[j] = (int32_t)__builtin_fma(2.0, __builtin_fma(-q, whole_sum, num), odd);
+            for (uint32_t j = 0; j < 8; j++) {
+                const double num = __builtin_fma((double)max(e[j / 4][j % 4], 0), scale, half), q = __builtin_floor(num * inv);
+                pr[j / 4][j % 4] = (int32_t)q;
+                if constexpr (W != kNone) query[j / 4][j % 4] = (int32_t)__builtin_fma(2.0, __builtin_fma(-q, whole_sum, num), odd);
             }
         } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t ej = (uint32_t)max(e[j], 0), pj = probability(ej, (uint64_t)p.a.prob_scale, sum, inv);
-                pr[j] = (int32_t)pj;
+            for (uint32_t j = 0; j < 8; j++) {
+                const uint32_t ej = (uint32_t)max(e[j / 4][j % 4], 0), pj = probability(ej, (uint64_t)p.a.prob_scale, sum, inv);
+                pr[j / 4][j % 4] = (int32_t)pj;
                 if constexpr (W != kNone) {
                     uint32_t wide = 0;
                     int32_t qj;
                     store_sum(&qj, lookup_query(ej, p.a.prob_scale, sum, pj), wide);
-                    query[j] = qj;
+                    query[j / 4][j % 4] = qj;
                     if (((there >> j) & 1u) && p.a.d_query) bad |= wide;
                 }
             }
@@ -754,44 +775,54 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
         if constexpr (W != kNone) {
             const size_t o = row * p.a.max_len + t;
             if constexpr (W == kBoth && FULL) {
-                *reinterpret_cast<v4u_t*>(p.a.d_prob + o) = pr;
-                *reinterpret_cast<v4u_t*>(p.a.d_query + o) = query;
+#pragma unroll
+                for (uint32_t h = 0; h < 2; h++) {
+                    *reinterpret_cast<v4u_t*>(p.a.d_prob + o + 4 * h) = pr[h];
+                    *reinterpret_cast<v4u_t*>(p.a.d_query + o + 4 * h) = query[h];
+                }
             } else {
-                if (W == kBoth || p.a.d_prob) store_four(p.a.d_prob + o, pr, there);
-                if (W == kBoth || p.a.d_query) store_four(p.a.d_query + o, query, there);
+#pragma unroll
+                for (uint32_t h = 0; h < 2; h++) {
+                    if (W == kBoth || p.a.d_prob) store_four(p.a.d_prob + o + 4 * h, pr[h], (there >> (4 * h)) & 15u);
+                    if (W == kBoth || p.a.d_query) store_four(p.a.d_query + o + 4 * h, query[h], (there >> (4 * h)) & 15u);
+                }
                 wait_for_memory();
             }
         }
-        v4i_t d;
+        uint32_t pl[2][4];
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++) d[j] = (there >> j) & 1u ? pr[j] : 0;
-        if (!FULL && lds.outside) {
+        for (uint32_t h = 0; h < 2; h++) {
+            v4i_t d;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++)
-                if (offset_of(p, w, seen, t + j) < 0) d[j] = 0;          // a page outside: no value
+            for (uint32_t j = 0; j < 4; j++) {
+                d[j] = (there >> (4 * h + j)) & 1u ? pr[h][j] : 0;
+                if (!FULL && lds.outside && offset_of(p, w, seen, t + 4 * h + j) < 0) d[j] = 0;          // a page outside: no value
+                if constexpr (WIDE) all += (uint32_t)d[j];
+            }
+            if constexpr (PP == 3) {
+                uint32_t none = 0;
+                three_planes(d, pl[h], none);
+            } else {
+                transpose4(digits_of(d[0]), digits_of(d[1]), digits_of(d[2]), digits_of(d[3]), pl[h]);
+            }
         }
-        if constexpr (WIDE) all += (uint64_t)(uint32_t)d[0] + (uint32_t)d[1] + (uint32_t)d[2] + (uint32_t)d[3];
-        uint32_t pl[4];
-        if constexpr (PP == 3) {
-            uint32_t none = 0;
-            three_planes(d, pl, none);
-            if (__any(pl[2] != 0) && w.lane == 0) lds.third[tile & 1] = tile + 1;
-        } else {
-            transpose4(digits_of(d[0]), digits_of(d[1]), digits_of(d[2]), digits_of(d[3]), pl);
-        }
-        uint32_t* to = lds.digits[tile & 1] + (((part >> 2) * kRows + r) << 2) + (part & 3u);
+        if (PP == 3 && __any((pl[0][2] | pl[1][2]) != 0) && w.lane == 0) lds.third[tile & 1] = tile + 1;
+        uint64_t* to = reinterpret_cast<uint64_t*>(lds.digits[tile & 1]) + ((part >> 1) * kRows + r) * 2 + (part & 1u);
 #pragma unroll
-        for (int k = 0; k < PP; k++) to[k * 16 * kRows] = pl[k];
+        for (int k = 0; k < PP; k++) to[k * 8 * kRows] = ((uint64_t)pl[1][k] << 32) | pl[0][k];
         __syncthreads();
         const v4i_t* pa = reinterpret_cast<const v4i_t*>(lds.digits[tile & 1]) + w.kg * kRows + w.col;
         auto multiply = [&](auto a) {
+            constexpr int A = decltype(a)::value;
             v4i_t f[2];
 #pragma unroll
-            for (uint32_t rb = 0; rb < 2; rb++) f[rb] = pa[decltype(a)::value * 4 * kRows + 16 * rb];
+            for (uint32_t rb = 0; rb < 2; rb++) f[rb] = pa[A * 4 * kRows + 16 * rb];
 #pragma unroll
             for (int k = 0; k < VP; k++)
 #pragma unroll
-                for (uint32_t rb = 0; rb < 2; rb++) acc[rb][decltype(a)::value + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[k], f[rb], acc[rb][decltype(a)::value + k], 0, 0, 0);
+                for (uint32_t rb = 0; rb < 2; rb++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) acc[j][rb][A + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[j][k], f[rb], acc[j][rb][A + k], 0, 0, 0);
         };
         multiply(std::integral_constant<int, 0>{});
         multiply(std::integral_constant<int, 1>{});
@@ -818,7 +849,7 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     for (; tile < tiles; tile++) body(tile, std::false_type{});
     if constexpr (WIDE) {
 #pragma unroll
-        for (int k = 8; k >= 1; k >>= 1) all += __shfl_xor(all, k, 64);
+        for (int k = 4; k >= 1; k >>= 1) all += __shfl_xor(all, k, 64);
         if (part == 0) lds.p_sum[r] = all;
     } else {
         if (__any((over & kOver) != 0) && w.lane == 0) lds.wide = 1;
@@ -826,18 +857,18 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     __syncthreads();
     if (!WIDE && lds.wide) return true;
     const bool whole = seen.tiles <= p.plan.value_cols;          // all positions of the rows are this workgroup's
-    const uint32_t e1 = e0 + 4 * w.kg;
+    const uint32_t e1 = e0 + 8 * w.kg;
 #pragma unroll
     for (uint32_t rb = 0; rb < 2; rb++) {
         const uint32_t q_row = 16 * rb + w.col;
         if (q_row >= w.R || e1 >= dim) continue;
         const size_t at = w.row(p, q_row);
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
+        for (uint32_t i = 0; i < 8; i++) {
             if (e1 + i >= dim) break;
             uint64_t y = WIDE ? (uint64_t)kCacheOffset * lds.p_sum[q_row] : 0, z = 0;
 #pragma unroll
-            for (int g = G - 1; g >= 0; g--) z = (z << 8) + (uint64_t)(int64_t)acc[rb][g][i];
+            for (int g = G - 1; g >= 0; g--) z = (z << 8) + (uint64_t)(int64_t)acc[i % 2][rb][g][i / 2];
             y += z;
             if (whole) {
                 int32_t q, rem;
@@ -852,20 +883,19 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     return false;
 }
 
-template <int PP>
-__global__ void __launch_bounds__(kValueThreads, 4) wit_window_values_kernel(WindowArgs p) {
+template <int PP, Written W, bool GROUPS>          // what the first group of elements writes; whether there are others
+__global__ void __launch_bounds__(kValueThreads, 2) wit_window_values_kernel(WindowArgs p) {
     __shared__ __attribute__((aligned(16))) ValueLds<PP> lds;
     RowTile w;
     if (!w.find(p, blockIdx.x)) return;
     const step::Seen seen = w.seen(p);
-    const uint32_t group = blockIdx.y % p.plan.groups, chunk = blockIdx.y / p.plan.groups;
+    const uint32_t group = GROUPS ? blockIdx.y % p.plan.groups : 0, chunk = GROUPS ? blockIdx.y / p.plan.groups : blockIdx.y;
     if (chunk * p.plan.value_cols >= seen.tiles) return;
     uint32_t bad = 0;
     if (threadIdx.x == 0) lds.wide = 0;
     bool wide;
-    if (group || (!p.a.d_prob && !p.a.d_query)) wide = window_values<PP, false, kNone>(p, w, seen, lds, group, chunk, bad);
-    else if (p.a.d_prob && p.a.d_query) wide = window_values<PP, false, kBoth>(p, w, seen, lds, group, chunk, bad);
-    else wide = window_values<PP, false, kSome>(p, w, seen, lds, group, chunk, bad);
+    if (W != kNone && GROUPS && group) wide = window_values<PP, false, kNone>(p, w, seen, lds, group, chunk, bad);
+    else wide = window_values<PP, false, W>(p, w, seen, lds, group, chunk, bad);
     if (wide) window_values<PP, true, kNone>(p, w, seen, lds, group, chunk, bad);
     if (bad) atomicOr(p.status, bad);
 }
@@ -955,8 +985,19 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     else if (a.d_shifted) wit_window_exp_kernel<false, true><<<exps, 256, 0, s>>>(p);
     else wit_window_exp_kernel<false, false><<<exps, 256, 0, s>>>(p);
     GRAPE_LAUNCH_CHECK();
-    if (a.prob_scale <= ((int64_t)1 << 22)) wit_window_values_kernel<3><<<values, kValueThreads, 0, s>>>(p);
-    else wit_window_values_kernel<4><<<values, kValueThreads, 0, s>>>(p);
+    auto values_of = [&](auto planes, auto written) {
+        constexpr int PP = decltype(planes)::value;
+        constexpr Written W = decltype(written)::value;
+        if (pl.groups > 1) wit_window_values_kernel<PP, W, true><<<values, kValueThreads, 0, s>>>(p);
+        else wit_window_values_kernel<PP, W, false><<<values, kValueThreads, 0, s>>>(p);
+    };
+    auto values_by = [&](auto planes) {
+        if (a.d_prob && a.d_query) values_of(planes, integral_constant<Written, kBoth>{});
+        else if (a.d_prob || a.d_query) values_of(planes, integral_constant<Written, kSome>{});
+        else values_of(planes, integral_constant<Written, kNone>{});
+    };
+    if (a.prob_scale <= ((int64_t)1 << 22)) values_by(integral_constant<int, 3>{});
+    else values_by(integral_constant<int, 4>{});
     GRAPE_LAUNCH_CHECK();
     if (pl.value_chunks > 1) {
         wit_window_join_kernel<<<dim3(p.along, pl.dim64, kRows / 4), 256, 0, s>>>(p);
