@@ -148,10 +148,15 @@ struct WindowPlan {
     uint32_t exp_cols, exp_chunks;
     uint32_t value_cols, value_chunks, groups;          // and workgroups along a head's elements
     bool factors;                              // the exponential table's entries are computed, see make_factors
+    bool packed;                               // operands are made beforehand, see wit_window_pack_kernel:
+    uint32_t steps, all_cols, splits;          // steps of 64 elements of theirs, tiles of positions that a sequence's rows see, workgroups of a tile's elements
+    size_t at_keys, at_values, at_queries, at_over, at_query_over;
     size_t at_scores, at_exp, at_max, at_sum, at_factors, at_part, bytes;
 };
 constexpr size_t kFactorBytes = 2 * 1024 * 8 + 64 * 4;
 constexpr uint32_t kValueDims = 128;
+constexpr uint32_t kPackTiles = 8, kPackSteps = 4;          // tiles of rows that operands made beforehand serve at least; steps of a workgroup
+constexpr size_t kKeyStepBytes = 3 * kCols * 64, kQueryStepBytes = 3 * kRows * 64, kValueStepBytes = 3 * kCols * 64;
 constexpr uint32_t kOffsetTiles = 16;          // tiles of positions whose offsets a values workgroup holds
 
 inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_new, uint32_t max_len, uint32_t window, uint32_t sinks,
@@ -185,6 +190,18 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     p.value_chunks = token::ceil_div(p.cols, p.value_cols);
     if (p.score_chunks > 65535 || p.exp_chunks > 65535 || (uint64_t)p.value_chunks * p.groups > 65535) return false;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    // Operands are made beforehand where that is little beside the products: each key and value then serves kPackTiles tiles of rows and
+    // more (both sides: see the kernels), and they take no more than a few GiB.
+    p.steps = p.dim64 == 1 ? 1 : (p.dim64 + 1) / 2 * 2;
+    uint64_t all = token::ceil_div(max_len, kCols);
+    if (window) all = std::min<uint64_t>(all, ((uint64_t)window + max_new + kCols - 1) / kCols + 1 + ((uint64_t)sinks + kCols - 1) / kCols);
+    p.all_cols = (uint32_t)all;
+    p.splits = token::ceil_div(p.dim64, kPackSteps);
+    const uint64_t cache_tiles = (uint64_t)seqs * p.all_cols * cache_heads;
+    const unsigned __int128 key_bytes = (unsigned __int128)cache_tiles * p.steps * kKeyStepBytes, value_bytes = (unsigned __int128)cache_tiles * p.dim64 * kValueStepBytes;
+    const uint64_t query_bytes = tiles * cache_heads * p.steps * kQueryStepBytes;
+    p.packed = (uint64_t)rows * p.each >= (uint64_t)kPackTiles * kRows * seqs && key_bytes + value_bytes + query_bytes <= (uint64_t)4 << 30 &&
+               (cache_tiles + tiles * cache_heads) * p.splits < (uint64_t)1 << 22;
     const size_t row = (size_t)rows_all * p.cols * kCols * 4;
     p.at_scores = 0;
     p.at_exp = up(row);
@@ -192,7 +209,12 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     p.at_sum = p.at_max + up((size_t)rows_all * p.score_chunks * 4);
     p.at_factors = p.at_sum + up((size_t)rows_all * 8);
     p.at_part = p.at_factors + (p.factors ? up(kFactorBytes) : 0);
-    p.bytes = p.at_part + (p.value_chunks > 1 ? (size_t)rows_all * p.value_chunks * dim * 8 : 0);
+    p.at_keys = p.at_part + up(p.value_chunks > 1 ? (size_t)rows_all * p.value_chunks * dim * 8 : 0);
+    p.at_values = p.at_keys + (p.packed ? up((size_t)key_bytes) : 0);
+    p.at_queries = p.at_values + (p.packed ? up((size_t)value_bytes) : 0);
+    p.at_over = p.at_queries + (p.packed ? up((size_t)query_bytes) : 0);
+    p.at_query_over = p.at_over + (p.packed ? up((size_t)cache_tiles * p.splits * 4) : 0);
+    p.bytes = p.at_query_over + (p.packed ? up((size_t)tiles * cache_heads * p.splits * 4) : 0);
     return true;
 }
 // Single tokens go the way of attention_plan, with at most this many positions each.
@@ -235,6 +257,8 @@ struct Seen {
         tiles = sink_tiles + (hi + kCols - 1) / kCols - from;
     }
     GRAPE_HD uint32_t tile(uint32_t v) const { return v < sink_tiles ? v : v - sink_tiles + from; }
+    // and back: the number of a tile that is one of these
+    GRAPE_HD uint32_t number(uint32_t tile) const { return tile < sink_tiles ? tile : tile - from + sink_tiles; }
     GRAPE_HD bool any(uint32_t t) const { return t < hi && (t >= lo || t < sinks); }
     // the tiles from <= v < to of v0 .. v0 + n, counted from v0, whose positions all rows see (tokens pos0 .. pos1); sinks' tiles are not counted
     GRAPE_HD void full(uint32_t pos0, uint32_t pos1, uint32_t window, uint32_t v0, uint32_t n, uint32_t& first, uint32_t& last) const {

@@ -45,11 +45,15 @@ struct WindowArgs {
     unsigned long long* sums;    // [rows][heads]
     int64_t* part;               // [rows][heads][value chunks][dim]
     uint32_t* status;
-    bool q_vec;
+    bool q_vec, k_vec;           // rows of the queries and of the keys that can be read by four elements
     double limit;                // of a score's product that is rescaled in double precision
     uint32_t along;              // workgroups of a launch's first axis
     double* factors;             // of the exponential table, see make_factors; null where it is read
     uint32_t* differs;
+    // operands made beforehand (see wit_window_pack_kernel), and whether an element did not fit
+    uint8_t *keys, *values, *queries;
+    uint32_t *over, *query_over;
+    __device__ __forceinline__ size_t tile_of(uint32_t b, uint32_t kv, uint32_t number) const { return ((size_t)b * c.heads + kv) * plan.all_cols + number; }
 };
 
 // the three planes of four elements; `over` gathers bits above the 24
@@ -117,6 +121,8 @@ struct RowTile {
         const uint32_t j = token(p, r);
         return (size_t)(first + j) * p.a.heads + kv * p.plan.each + (at + r - j * p.plan.each);
     }
+    // what all of the sequence's rows see, by which the operands made beforehand are numbered
+    __device__ __forceinline__ step::Seen all_seen(const WindowArgs& p) const { return step::Seen(pos, pos + n - 1, p.a.window, p.a.sinks); }
     __device__ __forceinline__ step::Seen seen(const WindowArgs& p) const { return step::Seen(first_pos, last_pos, p.a.window, p.a.sinks); }
     // the tiles first <= v < last of v0 .. v0 + n whose positions all rows see
     __device__ __forceinline__ void full(const WindowArgs& p, const step::Seen& seen, uint32_t v0, uint32_t n, uint32_t& first, uint32_t& last) const {
@@ -126,10 +132,10 @@ struct RowTile {
 
 // Offset of position t's token; of the last one that is seen where no row sees t, so that nothing is read but what is there.  -1 where the
 // page is outside the cache.
-__device__ __forceinline__ int64_t offset_of(const WindowArgs& p, const RowTile& w, const step::Seen& seen, uint32_t t) {
+__device__ __forceinline__ int64_t offset_of(const WindowArgs& p, uint32_t b, const step::Seen& seen, uint32_t t) {
     if (!seen.any(t)) t = seen.hi - 1;
     const uint32_t pg = p.page(t);
-    return token::token_offset(p.c, p.a.d_block_table[(size_t)w.b * p.a.table_stride + pg], t - pg * p.c.page_size);
+    return token::token_offset(p.c, p.a.d_block_table[(size_t)b * p.a.table_stride + pg], t - pg * p.c.page_size);
 }
 
 // The queries' digits of a block of 512 elements in LDS, [step of 64][plane][lane group][row], 16 bytes each.
@@ -186,7 +192,7 @@ __device__ __forceinline__ void wide_scores(const WindowArgs& p, const RowTile& 
 #pragma unroll 1
     for (uint32_t tile = 0; tile < tiles; tile++) {
         const uint32_t in_tile = 16 * w.wave + 4 * w.kg, v = v0 + tile, t0 = seen.tile(v) * kCols + in_tile;
-        const int64_t k_off = offset_of(p, w, seen, seen.tile(v) * kCols + 16 * w.wave + w.col);
+        const int64_t k_off = offset_of(p, w.b, seen, seen.tile(v) * kCols + 16 * w.wave + w.col);
         const int32_t* k_row = keys + max(k_off, (int64_t)0);
 #pragma unroll 1
         for (uint32_t rb = 0; 16 * rb < w.R; rb++) {
@@ -289,17 +295,116 @@ __device__ __forceinline__ void make_factors(const WindowArgs& p, uint32_t group
 // loop of their own, nothing is under way when it begins, and the other tiles wait for everything in the end.
 __device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }          // vmcnt 0
 
-// Scores of 32 rows with a chunk of the positions.  A wave takes 16 positions of each tile of 64 and all rows; it reads its keys from
-// memory into the operand (lane l the elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16), the queries' digits from LDS.
+// The operands of a call with many rows, made once: turning an element into digits costs as much as its products with 32 rows.  Keys of a
+// tile of 64 positions: [step][plane][16 positions][lane group][position], queries of a tile of rows: [step][plane][lane group][row], values of a
+// tile of 64 positions: [16 elements][plane][lane group][element] - 16 bytes each, what a lane of a product takes.  Positions that nobody sees and
+// pages outside the cache are zero.  A workgroup takes 256 elements.
+__global__ void __launch_bounds__(256) wit_window_pack_kernel(WindowArgs p) {
+    __shared__ double factors[2 * kFactors];
+    __shared__ int64_t off[kCols];
+    __shared__ uint32_t word[2];
+    uint32_t index = blockIdx.x, bad = 0;
+    if (p.factors) {
+        if (index < kTableGroups) return make_factors(p, index, factors, word[0]);
+        index -= kTableGroups;
+    }
+    if (threadIdx.x < 2) word[threadIdx.x] = 0;
+    const uint32_t dim = p.c.dim;
+    uint32_t over = 0;
+    const uint32_t split = index % p.plan.splits, s0 = split * step::kPackSteps;
+    index /= p.plan.splits;
+    if (index < p.along) {
+        RowTile w;
+        if (!w.find(p, index)) return;
+        __syncthreads();
+        const uint32_t g = threadIdx.x & 3u, r = (threadIdx.x >> 2) % kRows;          // two steps at a time
+        const int32_t* q = query_of(p, w, min(r, w.R - 1));
+        uint8_t* to = p.queries + (size_t)index * p.plan.steps * step::kQueryStepBytes + (g * kRows + r) * 16;
+        for (uint32_t s = s0 + threadIdx.x / (4 * kRows); s < min(s0 + step::kPackSteps, p.plan.steps); s += 2) {
+            uint32_t pl[4][3];
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) three_planes(elements(q, 64 * s + 16 * c + 4 * g, dim, p.q_vec, 0), pl[c], over);
+#pragma unroll
+            for (uint32_t k = 0; k < 3; k++)
+                *reinterpret_cast<v4i_t*>(to + (s * 3 + k) * 64 * kRows) = v4i_t{(int)pl[0][k], (int)pl[1][k], (int)pl[2][k], (int)pl[3][k]};
+        }
+        if (over & kOver) word[0] = 1;
+        __syncthreads();
+        if (threadIdx.x == 0) p.query_over[(size_t)index * p.plan.splits + split] = word[0];
+        return;
+    }
+    index -= p.along;
+    const uint32_t kv = index % p.c.heads, rest = index / p.c.heads, number = rest % p.plan.all_cols, b = rest / p.plan.all_cols;
+    uint32_t n, pos;
+    if (!step::new_tokens(p.a.d_starts[b], p.a.d_starts[b + 1], p.a.d_lens[b], p.a.rows, p.a.max_new, p.a.max_len, (uint64_t)p.a.table_stride * p.c.page_size, n, pos) || n == 0) return;
+    const step::Seen seen(pos, pos + n - 1, p.a.window, p.a.sinks);
+    if (number >= seen.tiles) return;
+    const uint32_t k0 = seen.tile(number) * kCols;
+    if (threadIdx.x < kCols) {
+        const uint32_t t = k0 + threadIdx.x;
+        const int64_t o = seen.any(t) ? offset_of(p, b, seen, t) : -2;
+        if (o == -1) bad |= (uint32_t)kWitIndex;
+        off[threadIdx.x] = o;
+    }
+    __syncthreads();
+    const size_t at = p.tile_of(b, kv, number);
+    {
+        const uint32_t key = threadIdx.x >> 2, g = threadIdx.x & 3u;
+        const int64_t o = off[key];
+        const int32_t* k = p.c.d_k + (int64_t)kv * p.c.head_stride + max(o, (int64_t)0);
+        uint8_t* to = p.keys + at * p.plan.steps * step::kKeyStepBytes + (((key >> 4) * 4 + g) * 16 + (key & 15u)) * 16;
+        for (uint32_t s = s0; s < min(s0 + step::kPackSteps, p.plan.steps); s++) {
+            uint32_t pl[4][3];
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) {
+                v4i_t x = {0, 0, 0, 0};
+                if (o >= 0) x = elements(k, 64 * s + 16 * c + 4 * g, dim, p.k_vec, 0);
+                three_planes(x, pl[c], over);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 3; j++)
+                *reinterpret_cast<v4i_t*>(to + (size_t)(s * 3 + j) * kCols * 64) = v4i_t{(int)pl[0][j], (int)pl[1][j], (int)pl[2][j], (int)pl[3][j]};
+        }
+        if (over & kOver) word[0] = 1;
+    }
+    over = 0;
+    {
+        const uint32_t g = threadIdx.x >> 6;
+        const int32_t* values = p.c.d_v + (int64_t)kv * p.c.head_stride;
+        uint8_t* to = p.values + at * p.plan.dim64 * step::kValueStepBytes;
+        for (uint32_t s = s0; s < min(s0 + step::kPackSteps, p.plan.dim64); s++) {
+            const uint32_t e = 64 * s + (threadIdx.x & 63u);
+            int32_t x[16];
+#pragma unroll
+            for (uint32_t j = 0; j < 16; j++) {
+                const int64_t o = off[16 * g + j];
+                x[j] = o >= 0 && e < dim ? values[o + e] : 0;
+            }
+            uint32_t pl[4][3];
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) three_planes(v4i_t{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]}, pl[c], over);
+#pragma unroll
+            for (uint32_t k = 0; k < 3; k++)
+                *reinterpret_cast<v4i_t*>(to + ((size_t)((e >> 4) * 3 + k) * 64 + g * 16 + (e & 15u)) * 16) = v4i_t{(int)pl[0][k], (int)pl[1][k], (int)pl[2][k], (int)pl[3][k]};
+        }
+        if (over & kOver) word[1] = 1;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) p.over[at * p.plan.splits + split] = word[0] | word[1] << 1;
+    if (bad) atomicOr(p.status, bad);
+}
+
+// Scores of 32 rows with a chunk of the positions.  A wave takes 16 positions of each tile of 64 and all rows.  Its keys come as operands
+// (PACKED), or from the cache into the operand (lane l the elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16); the queries' digits from LDS.
 // Five accumulators become a sum in double precision, exact below 2^53, and below 2^50 the quotient of (y + s/2 + 1/2) / s needs no
 // second look: it is no nearer than 1 / (2 s) to a whole number, and the product with 1 / s off by at most 2^-52 of itself.
-template <int STEPS, bool VEC, bool REM>
+template <bool PACKED, bool VEC, bool REM>
 __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ int32_t top[4][kRows];
     __shared__ uint32_t q_over;
     uint32_t bad = 0;
-    if (blockIdx.x >= p.along) {
+    if (!PACKED && blockIdx.x >= p.along) {
         if (blockIdx.y == 0) make_factors(p, blockIdx.x - p.along, reinterpret_cast<double*>(lds), q_over);
         return;
     }
@@ -312,56 +417,61 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
     RowTile w;
     if (!w.find(p, blockIdx.x)) return;
     const step::Seen seen = w.seen(p);
+    const step::Seen made = w.all_seen(p);
     const uint32_t v0 = blockIdx.y * p.plan.score_cols;
     if (v0 >= seen.tiles) return;
-    const uint32_t tiles = min(p.plan.score_cols, seen.tiles - v0), steps = p.plan.dim64, dim = p.c.dim, blocks = (steps + kBlockSteps - 1) / kBlockSteps;
+    const uint32_t tiles = min(p.plan.score_cols, seen.tiles - v0), steps = PACKED ? p.plan.steps : p.plan.dim64, dim = p.c.dim, blocks = (steps + kBlockSteps - 1) / kBlockSteps;
     int64_t* off = reinterpret_cast<int64_t*>(lds + (size_t)min(steps, kBlockSteps) * 3 * 4 * kRows * 4);
     if (threadIdx.x == 0) q_over = 0;
     bool outside = false;
-    for (uint32_t i = threadIdx.x; i < tiles * kCols; i += 256) {
-        const int64_t o = offset_of(p, w, seen, seen.tile(v0 + i / kCols) * kCols + i % kCols);
-        outside |= o < 0;
-        off[i] = max(o, (int64_t)0);
+    if constexpr (PACKED) {
+        __syncthreads();
+        bool over = false;
+        for (uint32_t i = threadIdx.x; i < tiles * p.plan.splits; i += 256) over |= p.over[p.tile_of(w.b, w.kv, made.number(seen.tile(v0 + i / p.plan.splits))) * p.plan.splits + i % p.plan.splits] & 1u;
+        for (uint32_t i = threadIdx.x; i < p.plan.splits; i += 256) over |= p.query_over[(size_t)blockIdx.x * p.plan.splits + i] != 0;
+        if (over) q_over = 1;
+    } else {
+        for (uint32_t i = threadIdx.x; i < tiles * kCols; i += 256) {
+            const int64_t o = offset_of(p, w.b, seen, seen.tile(v0 + i / kCols) * kCols + i % kCols);
+            outside |= o < 0;
+            off[i] = max(o, (int64_t)0);
+        }
+        if (outside) bad |= (uint32_t)kWitIndex;
     }
-    if (outside) bad |= (uint32_t)kWitIndex;
     if (blockIdx.y == 0 && threadIdx.x < w.R) p.sums[w.row(p, threadIdx.x)] = 0;
     uint32_t over = 0;
+    auto stage = [&](uint32_t block) {
+        if constexpr (PACKED) {
+            const uint32_t n = min(steps - kBlockSteps * block, kBlockSteps) * (uint32_t)(step::kQueryStepBytes / 16);
+            const v4i_t* from = reinterpret_cast<const v4i_t*>(p.queries + ((size_t)blockIdx.x * steps + kBlockSteps * block) * step::kQueryStepBytes);
+#pragma unroll 4
+            for (uint32_t i = threadIdx.x; i < n; i += 256) reinterpret_cast<v4i_t*>(lds)[i] = from[i];
+        } else {
+            stage_queries(p, w, block, lds, over);
+        }
+    };
     __syncthreads();
     if (blocks == 1) {
-        stage_queries(p, w, 0, lds, over);
+        stage(0);
         __syncthreads();
     }
-    const int32_t* keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
-    const int64_t* my_off = off + 16 * w.wave + w.col;
     const v4i_t* q_digits = reinterpret_cast<const v4i_t*>(lds) + w.kg * kRows + w.col;
-    // STEPS > 0: of the last step, quads that lie behind a head's end read its last one and count as zero
-    constexpr int S = STEPS ? STEPS : 1;
-    v4i_t x[S][4];
-    int32_t last_e[4], last_mask[4];
-    auto key_of = [&](uint32_t tile) { return keys + my_off[tile * kCols]; };
-    auto fetch_step = [&](const int32_t* k, int s) {
-        if (s + 1 < STEPS) {
+    // PACKED: operands of two steps, each next pair requested as the one before it has been used
+    v4i_t x[4], keys[2][3];
+    auto request = [&](int half, uint32_t tile, uint32_t s) {
+        const uint8_t* from = p.keys + (p.tile_of(w.b, w.kv, made.number(seen.tile(v0 + tile))) * steps + s) * step::kKeyStepBytes + (w.wave * 64 + w.lane) * 16;
 #pragma unroll
-            for (int c = 0; c < 4; c++) x[s][c] = *reinterpret_cast<const v4i_t*>(k + 64 * s + 16 * c + 4 * w.kg);
-        } else {
-#pragma unroll
-            for (int c = 0; c < 4; c++) x[s][c] = *reinterpret_cast<const v4i_t*>(k + last_e[c]);
-        }
+        for (int k = 0; k < 3; k++) keys[half][k] = *reinterpret_cast<const v4i_t*>(from + k * kCols * 64);
     };
+    const int32_t* cache_keys = p.c.d_k + (int64_t)w.kv * p.c.head_stride;
     auto fetch = [&](uint32_t tile, uint32_t s) {
-        const int32_t* k = key_of(tile);
+        const int32_t* k = cache_keys + off[tile * kCols + 16 * w.wave + w.col];
 #pragma unroll
-        for (uint32_t c = 0; c < 4; c++) x[0][c] = elements(k, 64 * s + 16 * c + 4 * w.kg, dim, VEC, 0);
+        for (uint32_t c = 0; c < 4; c++) x[c] = elements(k, 64 * s + 16 * c + 4 * w.kg, dim, VEC, 0);
     };
-    if constexpr (STEPS > 0) {
-#pragma unroll
-        for (uint32_t c = 0; c < 4; c++) {
-            const uint32_t e = 64 * (STEPS - 1) + 16 * c + 4 * w.kg;
-            last_e[c] = (int32_t)min(e, dim - 4);
-            last_mask[c] = e < dim ? -1 : 0;
-        }
-#pragma unroll
-        for (int s2 = 0; s2 < STEPS; s2++) fetch_step(key_of(0), s2);
+    if constexpr (PACKED) {
+        request(0, 0, 0);
+        if (steps > 1) request(1, 0, 1);
     } else {
         fetch(0, 0);
     }
@@ -384,20 +494,12 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
         for (int rb = 0; rb < 2; rb++)
 #pragma unroll
             for (int g = 0; g < 5; g++) acc[rb][g] = v4i_t{0, 0, 0, 0};
-        auto multiply = [&](const v4i_t (&y)[4], int step, auto&& then) {
-            v4i_t kb[3], f[3][2];
+        auto multiply = [&](const v4i_t (&kb)[3], uint32_t step) {
+            v4i_t f[3][2];
 #pragma unroll
             for (int a = 0; a < 3; a++)
 #pragma unroll
                 for (int rb = 0; rb < 2; rb++) f[a][rb] = q_digits[(step * 12 + a * 4) * kRows + 16 * rb];
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t pl[3];
-                three_planes(y[c], pl, k_over);
-#pragma unroll
-                for (int k = 0; k < 3; k++) kb[k][c] = (int)pl[k];
-            }
-            then();
 #pragma unroll
             for (int a = 0; a < 3; a++)
 #pragma unroll
@@ -406,25 +508,42 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
                     for (int rb = 0; rb < 2; rb++) acc[rb][a + k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[k], f[a][rb], acc[rb][a + k], 0, 0, 0);
         };
         const uint32_t next_tile = min(tile + 1, tiles - 1);
-        if constexpr (STEPS > 0) {
-            const int32_t* next = key_of(next_tile);
-#pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                if (s == STEPS - 1) {
-#pragma unroll
-                    for (int c = 0; c < 4; c++) x[s][c] &= last_mask[c];
+        auto next_block = [&](uint32_t s) {
+            if (blocks > 1 && s % kBlockSteps == 0) {
+                __syncthreads();
+                stage(s / kBlockSteps);
+                __syncthreads();
+            }
+        };
+        if constexpr (PACKED) {
+            if (steps == 1) {
+                multiply(keys[0], 0);
+                request(0, next_tile, 0);
+            } else {
+#pragma unroll 1
+                for (uint32_t s = 0; s < steps; s += 2) {
+                    next_block(s);
+                    const bool more = s + 2 < steps;
+                    multiply(keys[0], s % kBlockSteps);
+                    request(0, more ? tile : next_tile, more ? s + 2 : 0);
+                    multiply(keys[1], s % kBlockSteps + 1);
+                    request(1, more ? tile : next_tile, more ? s + 3 : 1);
                 }
-                multiply(x[s], s, [&]() { fetch_step(next, s); });
             }
         } else {
 #pragma unroll 1
             for (uint32_t s = 0; s < steps; s++) {
-                if (blocks > 1 && s % kBlockSteps == 0) {
-                    __syncthreads();
-                    stage_queries(p, w, s / kBlockSteps, lds, over);
-                    __syncthreads();
+                next_block(s);
+                v4i_t kb[3];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t pl[3];
+                    three_planes(x[c], pl, k_over);
+#pragma unroll
+                    for (int k = 0; k < 3; k++) kb[k][c] = (int)pl[k];
                 }
-                multiply(x[0], (int)(s % kBlockSteps), [&]() { fetch(s + 1 < steps ? tile : next_tile, s + 1 < steps ? s + 1 : 0); });
+                fetch(s + 1 < steps ? tile : next_tile, s + 1 < steps ? s + 1 : 0);
+                multiply(kb, s % kBlockSteps);
             }
         }
         // register i of lane l: position 4 (l / 16) + i of the wave's 16, row l % 16 of a block
@@ -437,7 +556,7 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
                 double y;
-                if constexpr (STEPS > 0 && STEPS < 4) {          // two of the sums fit 32 bits: 2 * 2^14 * 192 * 2^8 and 2^14 * 192
+                if (steps < 4) {          // two of the sums fit 32 bits: 2 * 2^14 * 192 * 2^8 + 2^14 * 192
                     const int32_t low = (acc[rb][1][i] << 8) + acc[rb][0][i], high = (acc[rb][4][i] << 8) + acc[rb][3][i];
                     y = __builtin_fma((double)high, 0x1p24, __builtin_fma((double)acc[rb][2][i], 0x1p16, (double)low));
                 } else {
@@ -656,10 +775,11 @@ struct ValueLds {
     uint32_t third[2], wide, outside;          // the last tile with digits in the third plane (and 1), of even and odd ones; whether a page is outside the cache
 };
 
-template <int PP, bool WIDE, Written W>
+template <int PP, bool WIDE, Written W, bool PACKED>
 __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile& w, const step::Seen& seen, ValueLds<PP>& lds, uint32_t group, uint32_t chunk, uint32_t& bad) {
     constexpr int VP = WIDE ? 4 : 3, G = PP + VP - 1;
     constexpr uint32_t K = step::kOffsetTiles;
+    const step::Seen made = w.all_seen(p);
     const uint32_t v0 = chunk * p.plan.value_cols, tiles = min(p.plan.value_cols, seen.tiles - v0), dim = p.c.dim;
     // of the probabilities: this thread's row and its eight positions of a tile
     const uint32_t r = threadIdx.x >> 3, part = threadIdx.x & 7u, rr = min(r, w.R - 1), pos = w.pos_of(p, rr);
@@ -680,7 +800,7 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     auto make_offsets = [&](uint32_t tile) {
         const uint32_t n = min(K, tiles - tile) * kCols;
         for (uint32_t i = threadIdx.x; i < n; i += kValueThreads) {
-            const int64_t o = offset_of(p, w, seen, seen.tile(v0 + tile + i / kCols) * kCols + i % kCols);
+            const int64_t o = offset_of(p, w.b, seen, seen.tile(v0 + tile + i / kCols) * kCols + i % kCols);
             lds.off[(tile / K) & 1][i] = max(o, (int64_t)0);
             if (o < 0) lds.outside = 1;
         }
@@ -688,6 +808,16 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     auto offsets = [&](uint32_t tile) { return lds.off[(tile / K) & 1] + (tile % K) * kCols; };
     v2u_t x[16];
     v4u_t e[2];
+    v4i_t vb[2][VP];          // the tile's operands, of the elements 2 col, + 1 or (PACKED) col, 16 + col
+    auto request = [&](uint32_t tile) {
+#pragma unroll
+        for (uint32_t j = 0; j < 2; j++) {
+            const uint32_t block = min(e0 / 16 + j, 4 * p.plan.dim64 - 1);
+            const uint8_t* from = p.values + p.tile_of(w.b, w.kv, made.number(seen.tile(v0 + tile))) * p.plan.dim64 * step::kValueStepBytes + (size_t)block * 3 * 1024 + w.lane * 16;
+#pragma unroll
+            for (int k = 0; k < 3; k++) vb[j][k] = *reinterpret_cast<const v4i_t*>(from + k * 1024);
+        }
+    };
     auto fetch_values = [&](uint32_t tile) {
         const int64_t* o = offsets(tile) + 16 * w.kg;
         if (pairs) {
@@ -729,18 +859,19 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     auto body = [&](uint32_t tile, auto all_see) {
         constexpr bool FULL = decltype(all_see)::value;
         // operands and probabilities first, then the next tile's loads, then this one's stores
-        v4i_t vb[2][VP];
+        if constexpr (!PACKED) {
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const v4i_t y = {x[4 * c][j], x[4 * c + 1][j], x[4 * c + 2][j], x[4 * c + 3][j]};
-                uint32_t v[4];
-                if constexpr (WIDE) four_planes(y, v);
-                else three_planes(y, v, over);
+                for (int c = 0; c < 4; c++) {
+                    const v4i_t y = {x[4 * c][j], x[4 * c + 1][j], x[4 * c + 2][j], x[4 * c + 3][j]};
+                    uint32_t v[4];
+                    if constexpr (WIDE) four_planes(y, v);
+                    else three_planes(y, v, over);
 #pragma unroll
-                for (int k = 0; k < VP; k++) vb[j][k][c] = (int)v[k];
-            }
+                    for (int k = 0; k < VP; k++) vb[j][k][c] = (int)v[k];
+                }
+        }
         const uint32_t t = seen.tile(v0 + tile) * kCols + 8 * part, there = FULL ? 255u : seen_of_four(p, pos, t) | seen_of_four(p, pos, t + 4) << 4;
         v4u_t pr[2], query[2];
         if (FULL || plain) {
@@ -765,11 +896,13 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
             }
         }
         if (FULL || tile + 1 < tiles) {
-            if ((tile + 1) % K == 0) {
-                make_offsets(tile + 1);
-                __syncthreads();
+            if constexpr (!PACKED) {
+                if ((tile + 1) % K == 0) {
+                    make_offsets(tile + 1);
+                    __syncthreads();
+                }
+                fetch_values(tile + 1);
             }
-            fetch_values(tile + 1);
             fetch_exps(tile + 1, all_see);
         }
         if constexpr (W != kNone) {
@@ -796,7 +929,7 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
                 d[j] = (there >> (4 * h + j)) & 1u ? pr[h][j] : 0;
-                if (!FULL && lds.outside && offset_of(p, w, seen, t + 4 * h + j) < 0) d[j] = 0;          // a page outside: no value
+                if (!PACKED && !FULL && lds.outside && offset_of(p, w.b, seen, t + 4 * h + j) < 0) d[j] = 0;          // a page outside: no value
                 if constexpr (WIDE) all += (uint32_t)d[j];
             }
             if constexpr (PP == 3) {
@@ -828,14 +961,21 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
         multiply(std::integral_constant<int, 1>{});
         if (PP > 3 || lds.third[tile & 1] == tile + 1) multiply(std::integral_constant<int, 2>{});
         if constexpr (PP > 3) multiply(std::integral_constant<int, 3>{});
+        if constexpr (PACKED) request(FULL ? tile + 1 : min(tile + 1, tiles - 1));
     };
     __syncthreads();
     if (threadIdx.x < 2) lds.third[threadIdx.x] = 0;
     if (threadIdx.x == 0) lds.outside = 0;
     __syncthreads();
-    make_offsets(0);
-    __syncthreads();
-    fetch_values(0);
+    if constexpr (PACKED) {
+        for (uint32_t i = threadIdx.x; i < tiles * p.plan.splits; i += kValueThreads)
+            if (p.over[p.tile_of(w.b, w.kv, made.number(seen.tile(v0 + i / p.plan.splits))) * p.plan.splits + i % p.plan.splits] & 2u) over = kOver;
+        request(0);
+    } else {
+        make_offsets(0);
+        __syncthreads();
+        fetch_values(0);
+    }
     fetch_exps(0, std::false_type{});
     wait_for_memory();
     uint32_t full0, full1, tile = 0;
@@ -857,33 +997,33 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     __syncthreads();
     if (!WIDE && lds.wide) return true;
     const bool whole = seen.tiles <= p.plan.value_cols;          // all positions of the rows are this workgroup's
-    const uint32_t e1 = e0 + 8 * w.kg;
 #pragma unroll
     for (uint32_t rb = 0; rb < 2; rb++) {
         const uint32_t q_row = 16 * rb + w.col;
-        if (q_row >= w.R || e1 >= dim) continue;
+        if (q_row >= w.R) continue;
         const size_t at = w.row(p, q_row);
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
-            if (e1 + i >= dim) break;
+            const uint32_t j = PACKED ? i / 4 : i % 2, m = PACKED ? i % 4 : i / 2, e1 = PACKED ? e0 + 16 * j + 4 * w.kg + m : e0 + 8 * w.kg + i;
+            if (e1 >= dim) break;
             uint64_t y = WIDE ? (uint64_t)kCacheOffset * lds.p_sum[q_row] : 0, z = 0;
 #pragma unroll
-            for (int g = G - 1; g >= 0; g--) z = (z << 8) + (uint64_t)(int64_t)acc[i % 2][rb][g][i / 2];
+            for (int g = G - 1; g >= 0; g--) z = (z << 8) + (uint64_t)(int64_t)acc[j][rb][g][m];
             y += z;
             if (whole) {
                 int32_t q, rem;
                 p.out.apply((int64_t)y, q, rem, bad);
-                p.a.d_out[at * dim + e1 + i] = q;
-                if (p.a.d_out_rem) p.a.d_out_rem[at * dim + e1 + i] = rem;
+                p.a.d_out[at * dim + e1] = q;
+                if (p.a.d_out_rem) p.a.d_out_rem[at * dim + e1] = rem;
             } else {
-                p.part[(at * p.plan.value_chunks + chunk) * dim + e1 + i] = (int64_t)y;
+                p.part[(at * p.plan.value_chunks + chunk) * dim + e1] = (int64_t)y;
             }
         }
     }
     return false;
 }
 
-template <int PP, Written W, bool GROUPS>          // what the first group of elements writes; whether there are others
+template <int PP, Written W, bool GROUPS, bool PACKED>          // what the first group of elements writes; whether there are others
 __global__ void __launch_bounds__(kValueThreads, 2) wit_window_values_kernel(WindowArgs p) {
     __shared__ __attribute__((aligned(16))) ValueLds<PP> lds;
     RowTile w;
@@ -894,9 +1034,9 @@ __global__ void __launch_bounds__(kValueThreads, 2) wit_window_values_kernel(Win
     uint32_t bad = 0;
     if (threadIdx.x == 0) lds.wide = 0;
     bool wide;
-    if (W != kNone && GROUPS && group) wide = window_values<PP, false, kNone>(p, w, seen, lds, group, chunk, bad);
-    else wide = window_values<PP, false, W>(p, w, seen, lds, group, chunk, bad);
-    if (wide) window_values<PP, true, kNone>(p, w, seen, lds, group, chunk, bad);
+    if (W != kNone && GROUPS && group) wide = window_values<PP, false, kNone, PACKED>(p, w, seen, lds, group, chunk, bad);
+    else wide = window_values<PP, false, W, PACKED>(p, w, seen, lds, group, chunk, bad);
+    if (wide) window_values<PP, true, kNone, false>(p, w, seen, lds, group, chunk, bad);
     if (bad) atomicOr(p.status, bad);
 }
 
@@ -948,6 +1088,11 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     p.chunk_max = (int32_t*)(ws + pl.at_max);
     p.sums = (unsigned long long*)(ws + pl.at_sum);
     p.part = (int64_t*)(ws + pl.at_part);
+    p.keys = ws + pl.at_keys;
+    p.values = ws + pl.at_values;
+    p.queries = ws + pl.at_queries;
+    p.over = (uint32_t*)(ws + pl.at_over);
+    p.query_over = (uint32_t*)(ws + pl.at_query_over);
     p.page = token::fast_div(p.c.page_size);
     p.by_each = token::fast_div(pl.each);
     p.qk = scaler(a.qk_scale);
@@ -957,7 +1102,7 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     const int rc = wit_status_word(&p.status);
     if (rc) return rc;
     auto aligned = [&](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
-    const bool vec = p.c.dim % 4 == 0 && ((p.c.page_stride | p.c.token_stride | p.c.head_stride) & 3) == 0 && aligned(p.c.d_k);
+    p.k_vec = p.c.dim % 4 == 0 && ((p.c.page_stride | p.c.token_stride | p.c.head_stride) & 3) == 0 && aligned(p.c.d_k);
     p.q_vec = p.c.dim % 4 == 0 && a.q_stride % 4 == 0 && aligned(a.d_q);
     p.along = pl.tiles * p.c.heads;
     p.factors = nullptr;
@@ -965,20 +1110,23 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
         p.factors = (double*)(ws + pl.at_factors);
         p.differs = (uint32_t*)(p.factors + 2 * kFactors);
     }
-    const size_t score_lds = std::max<size_t>((size_t)std::min(pl.dim64, kBlockSteps) * 12 * kRows * 16 + (size_t)pl.score_cols * kCols * 8, p.factors ? 2 * kFactors * sizeof(double) : 0);
-    const dim3 scores(p.along + (p.factors ? kTableGroups : 0), pl.score_chunks), exps(p.along, pl.exp_chunks), values(p.along, pl.value_chunks * pl.groups);
-    auto launch_scores = [&](auto kernel) { kernel<<<scores, 256, score_lds, s>>>(p); };
-    auto scores_of = [&](auto steps, auto by_four) {
-        if (a.d_scores_rem) launch_scores(wit_window_scores_kernel<decltype(steps)::value, decltype(by_four)::value, true>);
-        else launch_scores(wit_window_scores_kernel<decltype(steps)::value, decltype(by_four)::value, false>);
-    };
+    const size_t score_lds = std::max<size_t>((size_t)std::min(pl.packed ? pl.steps : pl.dim64, kBlockSteps) * 12 * kRows * 16 + (pl.packed ? 0 : (size_t)pl.score_cols * kCols * 8), p.factors ? 2 * kFactors * sizeof(double) : 0);
+    const dim3 scores(p.along + (p.factors && !pl.packed ? kTableGroups : 0), pl.score_chunks), exps(p.along, pl.exp_chunks), values(p.along, pl.value_chunks * pl.groups);
     using std::integral_constant;
-    if (vec && pl.dim64 == 1) scores_of(integral_constant<int, 1>{}, std::true_type{});
-    else if (vec && pl.dim64 == 2) scores_of(integral_constant<int, 2>{}, std::true_type{});
-    else if (vec && pl.dim64 == 3) scores_of(integral_constant<int, 3>{}, std::true_type{});
-    else if (vec && pl.dim64 == 4) scores_of(integral_constant<int, 4>{}, std::true_type{});
-    else if (vec) scores_of(integral_constant<int, 0>{}, std::true_type{});
-    else scores_of(integral_constant<int, 0>{}, std::false_type{});
+    auto scores_of = [&](auto packed, auto by_four) {
+        constexpr bool P = decltype(packed)::value, V = decltype(by_four)::value;
+        if (a.d_scores_rem) wit_window_scores_kernel<P, V, true><<<scores, 256, score_lds, s>>>(p);
+        else wit_window_scores_kernel<P, V, false><<<scores, 256, score_lds, s>>>(p);
+    };
+    if (pl.packed) {
+        wit_window_pack_kernel<<<(p.factors ? kTableGroups : 0) + (p.along + a.seqs * pl.all_cols * p.c.heads) * pl.splits, 256, 0, s>>>(p);
+        GRAPE_LAUNCH_CHECK();
+        scores_of(std::true_type{}, std::true_type{});
+    } else if (p.k_vec) {
+        scores_of(std::false_type{}, std::true_type{});
+    } else {
+        scores_of(std::false_type{}, std::false_type{});
+    }
     GRAPE_LAUNCH_CHECK();
     if (p.factors && a.d_shifted) wit_window_exp_kernel<true, true><<<exps, 256, 0, s>>>(p);
     else if (p.factors) wit_window_exp_kernel<true, false><<<exps, 256, 0, s>>>(p);
@@ -988,8 +1136,10 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     auto values_of = [&](auto planes, auto written) {
         constexpr int PP = decltype(planes)::value;
         constexpr Written W = decltype(written)::value;
-        if (pl.groups > 1) wit_window_values_kernel<PP, W, true><<<values, kValueThreads, 0, s>>>(p);
-        else wit_window_values_kernel<PP, W, false><<<values, kValueThreads, 0, s>>>(p);
+        if (pl.packed && pl.groups > 1) wit_window_values_kernel<PP, W, true, true><<<values, kValueThreads, 0, s>>>(p);
+        else if (pl.packed) wit_window_values_kernel<PP, W, false, true><<<values, kValueThreads, 0, s>>>(p);
+        else if (pl.groups > 1) wit_window_values_kernel<PP, W, true, false><<<values, kValueThreads, 0, s>>>(p);
+        else wit_window_values_kernel<PP, W, false, false><<<values, kValueThreads, 0, s>>>(p);
     };
     auto values_by = [&](auto planes) {
         if (a.d_prob && a.d_query) values_of(planes, integral_constant<Written, kBoth>{});
