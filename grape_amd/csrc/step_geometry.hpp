@@ -181,7 +181,7 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     };
     p.score_cols = chunk(p.dim64 > 8 ? 4096 : 768, 32);
     p.score_chunks = token::ceil_div(p.cols, p.score_cols);
-    p.exp_cols = std::max(4u, chunk(2048, 32));
+    p.exp_cols = std::max(4u, chunk(2048, 16));
     p.factors = rows_all * cols >= (uint64_t)1 << 16;
     p.exp_chunks = token::ceil_div(p.cols, p.exp_cols);
     p.groups = token::ceil_div(dim, kValueDims);

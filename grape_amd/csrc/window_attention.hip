@@ -175,6 +175,8 @@ __device__ __forceinline__ uint32_t seen_of_four(const WindowArgs& p, uint32_t p
     for (uint32_t i = 0; i < 4; i++) there |= step::sees(pos, t + i, p.a.window, p.a.sinks) ? 1u << i : 0u;
     return there;
 }
+// Four elements of a tensor of the proof that no later launch of the call reads, which then does not push out of the caches what the next one does.
+__device__ __forceinline__ void store_last(int32_t* to, v4u_t x) { __builtin_nontemporal_store(x, reinterpret_cast<v4u_t*>(to)); }
 __device__ __forceinline__ void store_four(int32_t* to, v4u_t x, uint32_t there) {
     if (there == 15u) {
         *reinterpret_cast<v4u_t*>(to) = x;
@@ -576,7 +578,7 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
             else store_four(to, q, there);
             if constexpr (REM) {
                 int32_t* to_rem = p.a.d_scores_rem + row[rb] * p.a.max_len + t0;
-                if constexpr (FULL) *reinterpret_cast<v4u_t*>(to_rem) = rem;
+                if constexpr (FULL) store_last(to_rem, rem);
                 else store_four(to_rem, rem, there);
             }
         }
@@ -688,8 +690,9 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
                 four += (uint32_t)e[j];
             }
             if (most > last) bad |= (uint32_t)kWitIndex;
-            *reinterpret_cast<v4u_t*>(p.exps.at(a.row, a.t, a.v)) = e;
-            if constexpr (SHIFTED) *reinterpret_cast<v4u_t*>(p.a.d_shifted + a.row * p.a.max_len + a.t) = shifted;
+            if constexpr (SHIFTED) store_last(p.exps.at(a.row, a.t, a.v), e);          // 240 -> 221 us; not so a workspace's, which stays in the caches (47, values 57 -> 53)
+            else *reinterpret_cast<v4u_t*>(p.exps.at(a.row, a.t, a.v)) = e;
+            if constexpr (SHIFTED) store_last(p.a.d_shifted + a.row * p.a.max_len + a.t, shifted);
             sum += full0 + 4 * a.g + w.lane / 16 < full1 ? four : 0;
             if (a.g + 1 == groups) {
 #pragma unroll
