@@ -147,7 +147,6 @@ struct WindowPlan {
     uint32_t score_cols, score_chunks;         // of a workgroup of the scores, and workgroups along the positions
     uint32_t exp_cols, exp_chunks;
     uint32_t value_cols, value_chunks, groups;          // and workgroups along a head's elements
-    bool factors;                              // the exponential table's entries are computed, see make_factors
     bool packed;                               // operands are made beforehand, see wit_window_pack_kernel:
     uint32_t steps, all_cols, splits;          // steps of 64 elements of theirs, tiles of positions that a sequence's rows see, workgroups of a tile's elements
     size_t at_keys, at_values, at_queries, at_over, at_query_over;
@@ -155,7 +154,9 @@ struct WindowPlan {
 };
 constexpr size_t kFactorBytes = 2 * 1024 * 8 + 64 * 4;
 constexpr uint32_t kValueDims = 128;
+constexpr uint32_t kValueMost = 511;          // tiles of positions: four products of digits each, 4 * 2^14 * 64 * 511, fit 32 bits
 constexpr uint32_t kPackTiles = 8, kPackSteps = 4;          // tiles of rows that operands made beforehand serve at least; steps of a workgroup
+constexpr uint64_t kPackProducts = (uint64_t)1 << 30;
 constexpr size_t kKeyStepBytes = 3 * kCols * 64, kQueryStepBytes = 3 * kRows * 64, kValueStepBytes = 3 * kCols * 64;
 constexpr uint32_t kOffsetTiles = 16;          // tiles of positions whose offsets a values workgroup holds
 
@@ -182,16 +183,16 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     p.score_cols = chunk(p.dim64 > 8 ? 4096 : 768, 32);
     p.score_chunks = token::ceil_div(p.cols, p.score_cols);
     p.exp_cols = std::max(4u, chunk(2048, 16));
-    p.factors = rows_all * cols >= (uint64_t)1 << 16;
     p.exp_chunks = token::ceil_div(p.cols, p.exp_cols);
     p.groups = token::ceil_div(dim, kValueDims);
     const uint64_t want = beside * p.groups >= 512 ? 1 : 512 / (beside * p.groups);
-    p.value_cols = (uint32_t)((cols + want - 1) / want);
+    p.value_cols = (uint32_t)std::min<uint64_t>((cols + want - 1) / want, kValueMost);
     p.value_chunks = token::ceil_div(p.cols, p.value_cols);
     if (p.score_chunks > 65535 || p.exp_chunks > 65535 || (uint64_t)p.value_chunks * p.groups > 65535) return false;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-    // Operands are made beforehand where that is little beside the products: each key and value then serves kPackTiles tiles of rows and
-    // more (both sides: see the kernels), and they take no more than a few GiB.
+    // Operands are made beforehand where each key and value then serves eight tiles of rows or more (24 sequences of 2000 positions, 32 heads of 128
+    // over 8: 32 new tokens 674 us from the cache and 706 so, 12 of 64 tokens 671 and 627), in calls of 2^30 products or more (one such sequence:
+    // 64 tokens of 1000 64 and 68 us, 128 of 2000 135 and 127, 512 of 4000 698 and 556), and where they take no more than a few GiB.
     p.steps = p.dim64 == 1 ? 1 : (p.dim64 + 1) / 2 * 2;
     uint64_t all = token::ceil_div(max_len, kCols);
     if (window) all = std::min<uint64_t>(all, ((uint64_t)window + max_new + kCols - 1) / kCols + 1 + ((uint64_t)sinks + kCols - 1) / kCols);
@@ -200,7 +201,7 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     const uint64_t cache_tiles = (uint64_t)seqs * p.all_cols * cache_heads;
     const unsigned __int128 key_bytes = (unsigned __int128)cache_tiles * p.steps * kKeyStepBytes, value_bytes = (unsigned __int128)cache_tiles * p.dim64 * kValueStepBytes;
     const uint64_t query_bytes = tiles * cache_heads * p.steps * kQueryStepBytes;
-    p.packed = (uint64_t)rows * p.each >= (uint64_t)kPackTiles * kRows * seqs && key_bytes + value_bytes + query_bytes <= (uint64_t)4 << 30 &&
+    p.packed = (uint64_t)rows * p.each >= (uint64_t)kPackTiles * kRows * seqs && (unsigned __int128)rows_all * p.cols * kCols * dim >= kPackProducts && key_bytes + value_bytes + query_bytes <= (uint64_t)4 << 30 &&
                (cache_tiles + tiles * cache_heads) * p.splits < (uint64_t)1 << 22;
     const size_t row = (size_t)rows_all * p.cols * kCols * 4;
     p.at_scores = 0;
@@ -208,7 +209,7 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     p.at_max = p.at_exp + up(row);
     p.at_sum = p.at_max + up((size_t)rows_all * p.score_chunks * 4);
     p.at_factors = p.at_sum + up((size_t)rows_all * 8);
-    p.at_part = p.at_factors + (p.factors ? up(kFactorBytes) : 0);
+    p.at_part = p.at_factors + up(kFactorBytes);
     p.at_keys = p.at_part + up(p.value_chunks > 1 ? (size_t)rows_all * p.value_chunks * dim * 8 : 0);
     p.at_values = p.at_keys + (p.packed ? up((size_t)key_bytes) : 0);
     p.at_queries = p.at_values + (p.packed ? up((size_t)value_bytes) : 0);

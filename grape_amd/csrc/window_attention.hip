@@ -269,7 +269,8 @@ __device__ __forceinline__ void wide_scores(const WindowArgs& p, const RowTile& 
 
 // A table of exponentials need not be looked into where it is one: entry 2^bit_shift - 1 - d is then round(S exp(-d / S)) with S the
 // entry of d = 0.  Written as d = 1024 a + b that is the product of two factors of a thousand each, 16 KB in all, which LDS holds.  These
-// workgroups make the factors and compare every entry that a score can meet; where one differs, the entries are read.
+// workgroups make the factors and compare every entry that a score can meet; where one differs, the entries are read.  That pays from the smallest
+// calls on, since it runs beside another launch: 2 new tokens behind 64 positions 24 us either way, 64 behind 1000 (32 heads) 67 us, and 75 read.
 constexpr uint32_t kFactors = 1024, kTableGroups = 64;
 __device__ __forceinline__ void make_factors(const WindowArgs& p, uint32_t group, double* factors, uint32_t& differs) {
     const uint32_t last = ((uint32_t)1 << p.a.bit_shift) - 1;
@@ -1109,7 +1110,7 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     p.q_vec = p.c.dim % 4 == 0 && a.q_stride % 4 == 0 && aligned(a.d_q);
     p.along = pl.tiles * p.c.heads;
     p.factors = nullptr;
-    if (pl.factors && a.bit_shift <= 20 && a.index_bits >= a.bit_shift) {
+    if (a.bit_shift <= 20 && a.index_bits >= a.bit_shift) {
         p.factors = (double*)(ws + pl.at_factors);
         p.differs = (uint32_t*)(p.factors + 2 * kFactors);
     }

@@ -364,6 +364,158 @@ def test_window_attention_with_some_outputs_and_a_kept_workspace(ops, exp_table,
     assert ops.wit_status() == 0
 
 
+# ---- calls with many rows, whose queries, keys and values are turned into digits once
+def alone(ops, q, kc, vc, table, starts, lens, exp_table, max_len, window=0, sinks=0, **kw):
+    """each token as a sequence of its own, one new token long"""
+    new = np.diff(starts)
+    seq = np.repeat(np.arange(len(new)), new)
+    ends = np.concatenate([np.arange(n - m + 1, n + 1) for n, m in zip(lens, new)]).astype(np.int64)
+    rows = slice(int(starts[0]), int(starts[-1]))
+    return ops.wit_window_attention(dev(q[rows]), kc, vc, dev(table[seq]), dev(np.arange(len(seq) + 1)), dev(ends), 1, max_len, dev(exp_table), window=window, sinks=sinks, **kw)
+
+
+MANY = [
+    # new tokens, lengths, heads, cache heads, dim, page, window, sinks: 256 rows of a cache head and more for each sequence, 2^30 products and more
+    ([300], [640], 8, 1, 1024, 16, 0, 0), ([520], [1000], 8, 2, 260, 17, 0, 0), ([400], [500], 2, 1, 4096, 7, 100, 70), ([300, 0, 261], [900, 5, 261], 16, 2, 128, 16, 0, 0),
+    ([512], [2049], 16, 2, 64, 100, 0, 0), ([700], [1700], 16, 2, 128, 16, 700, 4), ([1100], [1100], 30, 10, 33, 16, 0, 0), ([600, 400], [700, 777], 8, 2, 183, 32, 640, 130),
+    ([513], [513], 16, 16, 255, 16, 0, 0), ([300], [2000], 4, 1, 515, 64, 0, 0)]
+
+
+@pytest.mark.parametrize("new,lens,H,HK,D,page,window,sinks", MANY)
+def test_window_attention_of_many_rows(ops, exp_table, new, lens, H, HK, D, page, window, sinks):
+    rng = np.random.default_rng(sum(lens) + H + D)
+    table, kc, vc = paged(rng, lens, page, HK, D)
+    starts, L, scale = starts_of(new), max(lens), int(round(65536 * D ** 0.5))
+    q, k, v = gauss(rng, (int(starts[-1]), H, D)), dev(kc), dev(vc)
+    args = (dev(q), k, v, dev(table), dev(starts), dev(np.array(lens)), max(new), L, dev(exp_table))
+    want = alone(ops, q, k, v, table, starts, lens, exp_table, L, window, sinks, qk_scale=scale)
+    got = ops.wit_window_attention(*args, window=window, sinks=sinks, qk_scale=scale)
+    assert set(got) == set(want)
+    for x in want:
+        assert torch.equal(got[x], want[x]), x
+    for keep in (("qkv",), ("qkv", "softmax_output"), ("qkv", "qkv_rem", "exp_output", "softmax_lookup_query")):
+        some = ops.wit_window_attention(*args, window=window, sinks=sinks, qk_scale=scale, out={x: torch.zeros_like(want[x]) for x in keep})
+        assert all(torch.equal(some[x], want[x]) for x in keep), keep
+    assert ops.wit_status() == 0
+
+
+def test_window_attention_of_many_rows_matches_the_oracle(ops, exp_table):
+    rng = np.random.default_rng(30)
+    table, kc, vc = paged(rng, [600], 16, 1, 2048)
+    run_window(ops, gauss(rng, (129, 8, 2048)), kc, vc, table, [0, 129], [600], exp_table, 129, 600, 0, 0, qk_scale=65536 * 45)
+    assert ops.wit_status() == 0
+
+
+@pytest.mark.parametrize("where", ["queries", "keys", "values", "all", "one"])
+def test_window_attention_of_many_rows_with_the_largest_values(ops, exp_table, where):
+    rng = np.random.default_rng(31)
+    H, HK, D, page, new, lens = 8, 1, 700, 16, [300], [640]
+    ends = np.array([-(1 << 31), (1 << 31) - 1, TOP, TOP + 1, -TOP - 1, 0x7F7F7F, 0x7F7F80, -0x808080, -0x808081, 0], dtype=np.int64)
+    table, kc, vc = paged(rng, lens, page, HK, D)
+    q = rng.integers(-3, 4, (300, H, D)).astype(np.int32)
+    kc[:] = gauss(rng, kc.shape, 1000.0)
+    kc[..., 2] = rng.integers(0, 1 << 19, kc.shape[:3])
+    q[..., 0], q[..., 1], q[..., 2] = 1, -1, 1
+    if where in ("keys", "all"):
+        kc[..., 0] = kc[..., 1] = rng.choice(ends, kc.shape[:3])
+    if where in ("queries", "all"):
+        q[..., 3] = q[..., 4] = rng.choice(ends, q.shape[:2])
+        kc[..., 3] = rng.integers(-100, 100, kc.shape[:3])
+        kc[..., 4] = -kc[..., 3]
+    if where in ("values", "all"):
+        vc[..., ::3] = rng.choice(ends, vc[..., ::3].shape)
+    if where == "one":                                  # one element of one row, of the last key and of the first value
+        q[299, 7, 699], kc[table[0, 639 // page], 639 % page, 0, 699], vc[table[0, 0], 0, 0, 0] = 1 << 23, 1, -(1 << 31)
+    want = alone(ops, q, dev(kc), dev(vc), table, [0, 300], lens, exp_table, 640, 600, 5, qk_scale=2)
+    # 2^23 times a key's element of about 1000 is beyond 2^31 after a rescaling by 2, and further from the maximum than the table is long
+    status = 3 if where == "one" else 0
+    assert ops.wit_status() == status
+    got = ops.wit_window_attention(dev(q), dev(kc), dev(vc), dev(table), dev(np.array([0, 300])), dev(np.array(lens)), 300, 640, dev(exp_table), window=600, sinks=5, qk_scale=2)
+    assert all(torch.equal(got[x], want[x]) for x in want) and ops.wit_status() == status
+
+
+def test_window_attention_of_many_rows_reports(ops, exp_table):
+    """a page outside the cache counts as zero, a sequence whose numbers do not fit is left out, and neither reaches another one's rows"""
+    rng = np.random.default_rng(32)
+    new, lens, H, HK, D, page = [300, 260, 280], [800, 700, 280], 16, 2, 128, 16
+    table, kc, vc = paged(rng, lens, page, HK, D)
+    starts, k, v = starts_of(new), dev(kc), dev(vc)
+    q = gauss(rng, (int(starts[-1]), H, D))
+    for bad in (-1, kc.shape[0], (1 << 31) - 1, -(1 << 31)):
+        t = table.copy()
+        t[0, 3], t[1, 40] = bad, bad
+        want = alone(ops, q, k, v, t, starts, lens, exp_table, 800, qk_scale=65536 * 11)
+        assert ops.wit_status() == 2
+        got = ops.wit_window_attention(dev(q), k, v, dev(t), dev(starts), dev(np.array(lens)), 300, 800, dev(exp_table), qk_scale=65536 * 11)
+        assert ops.wit_status() == 2 and all(torch.equal(got[x], want[x]) for x in want)
+    want = alone(ops, q, k, v, table, starts, lens, exp_table, 800, 500, 3, qk_scale=65536 * 11)
+    s = starts.tolist()
+    for st, ln in ((s, [800, 801, 280]), (s, [800, -1, 280]), (s, [800, 259, 280]), (s, [800, (1 << 31) - 1, 280])):
+        out = {x: filled(*t.shape) for x, t in want.items()}
+        ops.wit_window_attention(dev(q), k, v, dev(table), dev(np.array(st)), dev(np.array(ln)), 300, 800, dev(exp_table), window=500, sinks=3, out=out, qk_scale=65536 * 11)
+        assert ops.wit_status() == 2
+        for x in ("qkv", "qkv_rem", "max", "exp_sum"):
+            expected = want[x].clone()
+            expected[s[1]:s[2]] = UNTOUCHED
+            assert torch.equal(out[x], expected), (ln, x)
+        for x in PROOF:
+            assert bool((out[x][s[1]:s[2]] == UNTOUCHED).all())
+    for st in ([0, -1, 300, 840], [-(1 << 31), 0, 1, 2], [0, 300, (1 << 31) - 1, 840], [840, 560, 300, 0], [0, 0, 0, 9999], [0, 301, 301, 301]):
+        out = {x: filled(*t.shape) for x, t in want.items()}
+        ops.wit_window_attention(dev(q), k, v, dev(table), dev(np.array(st)), dev(np.array(lens)), 300, 800, dev(exp_table), window=500, sinks=3, out=out, qk_scale=65536 * 11)
+        assert ops.wit_status() & 2, st
+
+
+@pytest.mark.parametrize("n,H,D", [(70, 2, 64), (720, 16, 128)])
+def test_window_attention_of_wide_sums(ops, exp_table, n, H, D):
+    """a table of large entries that is no exponential: sums beyond 2^28, probabilities of three digits"""
+    rng = np.random.default_rng(33)
+    table, kc, vc = paged(rng, [n], 16, 2, D)
+    q = gauss(rng, (n, H, D))
+    flat = np.full(1 << 20, 3 << 20, dtype=np.int32)
+    flat[::7] = 1 << 16
+    k, v = dev(kc), dev(vc)
+    for prob_scale in (1 << 16, 1 << 22, 1 << 24):
+        want = alone(ops, q, k, v, table, [0, n], [n], flat, n, qk_scale=65536 * 11, prob_scale=prob_scale, out_scale=prob_scale)
+        got = ops.wit_window_attention(dev(q), k, v, dev(table), dev(np.array([0, n])), dev(np.array([n])), n, n, dev(flat), qk_scale=65536 * 11, prob_scale=prob_scale, out_scale=prob_scale)
+        assert all(torch.equal(got[x], want[x]) for x in want)
+        ops.wit_status()                                # queries beyond 32 bits where the probabilities are many
+    run_window(ops, q[:40, :4], kc[:, :, :1], vc[:, :, :1], table, [0, 40], [n], flat, 40, n, 20, 2, qk_scale=65536 * 11)
+    assert ops.wit_status() == 0
+
+
+def test_window_attention_of_a_long_cache(ops):
+    """131072 positions of the same score and value, whose digits' products would leave 32 bits if all were added up there"""
+    n, new, H, D = 131072, 128, 16, 1024
+    prob_scale, out_scale, e, x = 8064 * n, 1 << 31, 1000, -128 * 65536 + 127 * 256 - 128
+    k = torch.zeros((n // 1024, 1024, 1, D), dtype=torch.int32, device="cuda")
+    v = torch.full_like(k, x)
+    table = torch.full((1 << 10,), e, dtype=torch.int32, device="cuda")
+    got = ops.wit_window_attention(dev(np.ones((new, H, D), dtype=np.int32)), k, v, dev(np.arange(n // 1024)[None]), dev(np.array([0, new])), dev(np.array([n])), new, n, table,
+                                   bit_shift=10, index_bits=10, prob_scale=prob_scale, out_scale=out_scale, proof=False)
+    for j in range(new):
+        seen = n - new + j + 1
+        y = seen * ((e * prob_scale + seen * e // 2) // (seen * e)) * x
+        want = (y + out_scale // 2) // out_scale
+        assert bool((got["qkv"][j] == want).all()) and bool((got["qkv_rem"][j] == y - want * out_scale).all()), j
+    assert ops.wit_status() == 0
+
+
+def test_window_attention_looks_a_table_up_that_is_off_by_one(ops, exp_table):
+    """wherever the entry stands that is not the exponential's"""
+    rng = np.random.default_rng(34)
+    n, H, D = 520, 16, 128
+    table, kc, vc = paged(rng, [n], 16, 2, D)
+    q, k, v = gauss(rng, (n, H, D)), dev(kc), dev(vc)
+    for at in (-1, -2, -3, -1025, -40000, -200000, -(1 << 19)):
+        other = exp_table.copy()
+        other[at] += 1
+        want = alone(ops, q, k, v, table, [0, n], [n], other, n, qk_scale=65536 * 11)
+        got = ops.wit_window_attention(dev(q), k, v, dev(table), dev(np.array([0, n])), dev(np.array([n])), n, n, dev(other), qk_scale=65536 * 11)
+        assert all(torch.equal(got[x], want[x]) for x in want), at
+    assert ops.wit_status() == 0
+
+
 # ------------------------------------------------------------------ the next token
 def next_case(rng, n, vocab, longest):
     logits = gauss(rng, (n, vocab), 200000.0)
