@@ -182,7 +182,8 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     };
     p.score_cols = chunk(p.dim64 > 8 ? 4096 : 768, 32);
     p.score_chunks = token::ceil_div(p.cols, p.score_cols);
-    p.exp_cols = std::max(4u, chunk(2048, 16));
+    // four tiles or more, which a wave reads at once (4 sequences of 4000: 20 us, and 25 and 40 by two and one), but where that leaves CUs idle (3 of 500: 19 and 11 by one)
+    p.exp_cols = std::max(std::min(4u, chunk(256, 16)), chunk(2048, 16));
     p.exp_chunks = token::ceil_div(p.cols, p.exp_cols);
     p.groups = token::ceil_div(dim, kValueDims);
     const uint64_t want = beside * p.groups >= 512 ? 1 : 512 / (beside * p.groups);
