@@ -845,7 +845,7 @@ int grape_wit_window_attention(const grape_wit_window_attention_args *args, cons
  *
  * A logit beyond int32 sets GRAPE_WIT_QUOTIENT and becomes the nearest one that is not excluded; a gap beyond int32 sets
  * GRAPE_WIT_SUM_WIDE, with its low 32 bits stored.  rep < 1 (taken as none), a history length outside 0..history (taken as the
- * nearest) and a token of the history outside the vocabulary (skipped) set GRAPE_WIT_INDEX.  1 <= scale <= 2^31; vocab <= 2^24.
+ * nearest) and a token of the history outside the vocabulary (skipped) set GRAPE_WIT_INDEX.  1 <= scale <= 2^31; vocab and history <= 2^24.
  * d_workspace (16-byte aligned): grape_wit_next_token_workspace(...) bytes, one for each of the calls that may run at the same time. */
 typedef struct {
     const int32_t *d_logits, *d_history, *d_history_lens, *d_repetition, *d_presence, *d_frequency, *d_bias, *d_mask;

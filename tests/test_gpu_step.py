@@ -516,6 +516,80 @@ def test_window_attention_looks_a_table_up_that_is_off_by_one(ops, exp_table):
     assert ops.wit_status() == 0
 
 
+def test_window_attention_of_many_sequences_with_long_heads(ops, exp_table):
+    """the largest workgroups of the scores: eight steps of the queries' digits and offsets of 32 tiles; pages that sequences share"""
+    rng = np.random.default_rng(35)
+    for seqs, H, D, window in ((100, 8, 512, 0), (100, 8, 450, 1900), (40, 16, 130, 0)):
+        kc, vc = gauss(rng, (130, 16, H, D)), gauss(rng, (130, 16, H, D))
+        table = rng.integers(0, 130, (seqs, 129)).astype(np.int32)
+        lens, starts = rng.integers(1900, 2060, seqs), np.arange(seqs + 1) * 2
+        q, k, v = gauss(rng, (2 * seqs, H, D)), dev(kc), dev(vc)
+        want = alone(ops, q, k, v, table, starts, lens, exp_table, 2060, window, 0, qk_scale=65536 * 22)
+        got = ops.wit_window_attention(dev(q), k, v, dev(table), dev(starts), dev(lens), 2, 2060, dev(exp_table), window=window, qk_scale=65536 * 22)
+        assert all(torch.equal(got[x], want[x]) for x in want) and ops.wit_status() == 0
+
+
+def test_window_attention_of_offsets_beyond_32_bits(ops, exp_table):
+    """pages 2^27 elements apart, and rows of a proof of more than 2^32 elements"""
+    rng = np.random.default_rng(36)
+    D, n = 512, 17 * 16
+    far = torch.empty((16 << 27) + 16 * D, dtype=torch.int32, device="cuda").as_strided((17, 16, 1, D), (1 << 27, D, D, 1))
+    near = dev(gauss(rng, (17, 16, 1, D)))
+    far.copy_(near)
+    table = rng.permutation(17)[None].astype(np.int32)
+    for new, H in ((1, 4), (9, 4), (272, 32)):
+        q = dev(gauss(rng, (new, H, D)))
+        args = (dev(table), dev(np.array([0, new])), dev(np.array([n])), new, n, dev(exp_table))
+        want, got = (ops.wit_window_attention(q, x, x, *args, qk_scale=65536 * 22) for x in (near, far))
+        assert all(torch.equal(got[x], want[x]) for x in want)
+    del far, want, got
+    new, L, H, HK, D = 2048, 70000, 32, 8, 64
+    kc, vc = gauss(rng, (9, 1000, HK, D)), gauss(rng, (9, 1000, HK, D))
+    table = rng.integers(0, 9, (1, 70)).astype(np.int32)
+    q, k, v = gauss(rng, (new, H, D)), dev(kc), dev(vc)
+    got = {"qkv": filled(new, H, D), "softmax_output": torch.zeros((new, H, L), dtype=torch.int32, device="cuda")}
+    ops.wit_window_attention(dev(q), k, v, dev(table), dev(np.array([0, new])), dev(np.array([L])), new, L, dev(exp_table), window=256, sinks=4, out=got, qk_scale=65536 * 8)
+    want = alone(ops, q[-40:], k, v, table, [0, 40], [L], exp_table, L, 256, 4, qk_scale=65536 * 8, out={x: torch.zeros_like(t[-40:]) for x, t in got.items()})
+    assert all(torch.equal(got[x][-40:], want[x]) for x in want) and ops.wit_status() == 0
+
+
+def test_calls_with_many_rows_on_two_streams_and_replayed(ops, exp_table):
+    rng = np.random.default_rng(37)
+    cases = []
+    for n, H, HK, D in ((520, 16, 2, 128), (300, 8, 1, 1024), (40, 4, 2, 64)):
+        table, kc, vc = paged(rng, [n + 160], 16, HK, D)
+        q = [dev(gauss(rng, (n, H, D))) for _ in range(3)]
+        rest = (dev(kc), dev(vc), dev(table), dev(np.array([0, n])), dev(np.array([n + 160])), n, n + 160, dev(exp_table))
+        cases.append((q, rest, [ops.wit_window_attention(x, *rest, qk_scale=65536 * 11) for x in q]))
+    # the scores of 1024 products over 11 have a deviation of 2.9, and the table's 2^20 entries end 16 below the maximum: some are looked for outside
+    status = ops.wit_status()
+    assert status == 2
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    results = []
+    for i in range(3):
+        for (q, rest, _), s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                results.append(ops.wit_window_attention(q[i], *rest, qk_scale=65536 * 11))
+    torch.cuda.synchronize()
+    for j, got in enumerate(results):
+        want = cases[j % 3][2][j // 3]
+        assert all(torch.equal(got[x], want[x]) for x in want)
+    for q, rest, want in cases:
+        x = q[0].clone()
+        out = {name: torch.zeros_like(t) for name, t in want[0].items()}
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.wit_window_attention(x, *rest, qk_scale=65536 * 11, out=out)
+        for i in (1, 0, 2, 1):
+            x.copy_(q[i])
+            graph.replay()
+            again = ops.wit_window_attention(q[i], *rest, qk_scale=65536 * 11)
+            torch.cuda.synchronize()
+            assert all(torch.equal(out[name], want[i][name]) and torch.equal(again[name], want[i][name]) for name in want[i])
+    assert ops.wit_status() == status
+
+
 # ------------------------------------------------------------------ the next token
 def next_case(rng, n, vocab, longest):
     logits = gauss(rng, (n, vocab), 200000.0)

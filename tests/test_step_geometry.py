@@ -255,7 +255,7 @@ def following(**kw):
     return ops._NEXT.pack(*{**NEXT, **kw}.values())
 
 
-@pytest.mark.parametrize("bad", [dict(n=65536), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(scale=0), dict(scale=-1), dict(scale=LARGE + 1), dict(history=LARGE), dict(xs=-1), dict(hs=-1), dict(bs=-1),
+@pytest.mark.parametrize("bad", [dict(n=65536), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(scale=0), dict(scale=-1), dict(scale=LARGE + 1), dict(history=LARGE), dict(history=(1 << 24) + 1), dict(xs=-1), dict(hs=-1), dict(bs=-1),
                                  dict(ms=-1), dict(xs=1 << 40), dict(hs=1 << 40), dict(bs=1 << 40), dict(ms=1 << 40), dict(x=0), dict(t=0), dict(h=0), dict(hl=0), dict(ws=0), dict(wb=10), dict(ws=0xc00008)])
 def test_bad_choices_are_refused(lib, bad):
     assert lib.refuse_next(following()) is None and lib.refuse_next(None)
@@ -264,7 +264,7 @@ def test_bad_choices_are_refused(lib, bad):
 
 def test_choices_that_are_taken(lib):
     for ok in (dict(n=0, x=0, t=0, ws=0, wb=0, h=0, hl=0), dict(history=0, h=0, hl=0), dict(b=0), dict(m=0), dict(o=0, r=0, c=0, g=0, mx=0), dict(scale=1), dict(scale=LARGE), dict(xs=0), dict(xs=5000),
-               dict(o=0x100000), dict(o=0x100000, n=1, xs=7)):
+               dict(o=0x100000), dict(o=0x100000, n=1, xs=7), dict(history=1 << 24)):
         assert lib.refuse_next(following(**ok)) is None, ok
 
 
