@@ -85,7 +85,8 @@ inline const char* refuse_pages(const grape_wit_page_step_args* a) {
 }
 
 // ---- the next token
-// A workgroup takes a chunk of a row's vocabulary, and counts the row's history for it.
+// A workgroup takes a chunk of a row's vocabulary, and counts the row's history for it: 8192 tokens, or half and a quarter where that leaves CUs
+// idle (one row of 32000: 5.5 us, by 8192 8.7; 64 rows 12.0 by 4096, 13.7 by 2048, 14.5 by 8192; 256 rows of 131072: 67, by 2048 110).
 struct NextPlan {
     uint32_t chunk, chunks;
     size_t bytes;
@@ -95,7 +96,7 @@ constexpr uint32_t kNextLeast = 2048, kNextMost = 8192;
 inline NextPlan next_plan(uint32_t seqs, uint32_t vocab) {
     NextPlan p;
     p.chunk = kNextMost;
-    while (p.chunk > kNextLeast && (uint64_t)seqs * token::ceil_div(vocab, p.chunk) < 512) p.chunk /= 2;
+    while (p.chunk > kNextLeast && (uint64_t)seqs * token::ceil_div(vocab, p.chunk) < 400) p.chunk /= 2;
     p.chunks = token::ceil_div(vocab, p.chunk);
     p.bytes = (size_t)8 * seqs * p.chunks;
     return p;

@@ -10,6 +10,8 @@ namespace grape {
 // itself, in LDS, and then takes its share of the rows, the new pages and the ones given back, each of which finds its sequence by
 // halving.  Nothing that a workgroup reads is written by another one: the lengths and the ring's span go to places of their own,
 // entries of the table are read below the pages held and written above, and the ring is written behind its last entry alone.
+// Bound by latency: 7.5 us for one more token of 64 sequences, 10 for a few prompts among running answers, 12.6 for 1023 sequences behind a window: two
+// rounds of loads with the scans between them.
 // ------------------------------------------------------------------------------------------------
 struct PageArgs {
     grape_wit_page_step_args a;
@@ -174,7 +176,9 @@ __global__ void __launch_bounds__(THREADS) wit_page_step_kernel(PageArgs p) {
 // ------------------------------------------------------------------------------------------------
 // The next token.  A workgroup counts a row's history for its chunk of the vocabulary in LDS, applies what the counts, biases and
 // mask ask for and keeps its largest logit; a second launch joins the chunks and writes how far each logit is below the row's largest.
-// Bound by memory: 4 bytes read a logit, up to 16 written, and 4 read again for the distances.
+// Bound by memory: 4 bytes read a logit, up to 16 written, and 4 read again for the distances.  256 rows of 131072: 67 + 5 us, 2 TB/s, held up by
+// the vector instructions of the counting and the adjusting (half of the time); one row of 32000: 5.5 + 3 us, two chains of loads.  Lists of the tokens
+// that occur, so that only these are divided, were slower than dividing where a count is not zero.
 // ------------------------------------------------------------------------------------------------
 constexpr int32_t kLowest = INT32_MIN;          // of a token that must not be chosen
 struct NextArgs {
@@ -415,8 +419,9 @@ int grape_wit_page_step(const grape_wit_page_step_args* args, grape_stream_t st)
     hipStream_t s = as_stream(st);
     const int rc = wit_status_word(&p.status);
     if (rc) return rc;
-    // every workgroup makes the sums, of a sequence a thread or up to four
-    const uint32_t threads = p.a.seqs <= 256 ? 256 : 1024, workgroups = std::min(256u, token::ceil_div(p.a.rows, threads) + token::ceil_div(p.a.seqs, 128));
+    // every workgroup makes the sums, of up to four sequences a thread; waves fewer meet sooner (64 sequences 7.5 us, and 8.8 by 1024 threads, 600 10.4 and 11.3,
+    // 1023 12.5 and 14.4, but 2048 16.4 and 15.3, 4096 25 and 17)
+    const uint32_t threads = p.a.seqs <= 1024 ? 256 : 1024, workgroups = std::min(256u, token::ceil_div(p.a.rows, threads) + token::ceil_div(p.a.seqs, 128));
     const size_t lds = (size_t)20 * p.a.seqs;
     if (threads == 256) wit_page_step_kernel<256><<<std::max(1u, workgroups), 256, lds, s>>>(p);
     else wit_page_step_kernel<1024><<<std::max(1u, workgroups), 1024, lds, s>>>(p);

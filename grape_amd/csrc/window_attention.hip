@@ -12,7 +12,13 @@ namespace grape {
 // Scores, softmax through the table, products with the values, for tiles of 32 rows: the query heads that read one cache head, token
 // after token, so that a key or a value that is read serves 32 rows.  The softmax is the table's, rounded: the row's maximum is
 // needed before the first exponential and the sum of all before the first probability, hence a launch for each of the three, and
-// a fourth that joins the values' partial sums where the positions are cut up.
+// a fourth that joins the values' partial sums where the positions are cut up.  Rows of 32 are two operands of a product for each key
+// that is loaded; 16 would read keys and values twice as often, 64 leave no registers for the five sums of the planes' products.
+//
+// 2048 new tokens, 32 heads of 128 over 8, with a proof (1.34 GB written, 0.54 GB of it read again): 46 us operands, 158 scores, 208
+// exponentials, 248 values, each of the last three near what it writes and reads at 3.3 to 4 TB/s.  One head of 4096: 63 + 130 + 18 + 139 us, of which 142
+// are the products' at the rate of a large int8 one.  5 drafted tokens of 8 sequences of up to 3000: 35 + 15 + 39 + 5 us, chains of
+// dependent loads in short workgroups; a fourth wave of registers (128 of them) or other chunks are no faster.
 //
 // Both products run on the int8 matrix cores, exactly.  An element of magnitude below 2^23 is three balanced digits of base 256, the bytes
 // of x + 0x808080 with their top bits turned over, nine products of planes for a pair of operands and six where the probabilities
@@ -301,7 +307,8 @@ __device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0
 // The operands of a call with many rows, made once: turning an element into digits costs as much as its products with 32 rows.  Keys of a
 // tile of 64 positions: [step][plane][16 positions][lane group][position], queries of a tile of rows: [step][plane][lane group][row], values of a
 // tile of 64 positions: [16 elements][plane][lane group][element] - 16 bytes each, what a lane of a product takes.  Positions that nobody sees and
-// pages outside the cache are zero.  A workgroup takes 256 elements.
+// pages outside the cache are zero.  A workgroup takes 256 elements.  2048 tokens, 40 + 8 heads of 128: 46 us for 64 MB, bound by the chain of
+// starts, lengths, pages and elements in one round of workgroups (queries alone 24); with it scores go from 239 to 158 us, values from 319 to 248.
 __global__ void __launch_bounds__(256) wit_window_pack_kernel(WindowArgs p) {
     __shared__ double factors[2 * kFactors];
     __shared__ int64_t off[kCols];
@@ -401,6 +408,8 @@ __global__ void __launch_bounds__(256) wit_window_pack_kernel(WindowArgs p) {
 // (PACKED), or from the cache into the operand (lane l the elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16); the queries' digits from LDS.
 // Five accumulators become a sum in double precision, exact below 2^53, and below 2^50 the quotient of (y + s/2 + 1/2) / s needs no
 // second look: it is no nearer than 1 / (2 s) to a whole number, and the product with 1 / s off by at most 2^-52 of itself.
+// Bound by vector instructions and stores together where a proof is made (100 us without them and 158 with, for the 2048 tokens above); by LDS
+// for heads of 4096: a wave reads 6 KB of the queries' digits for 18 products, 4 waves 170 bytes a clock of 128.
 template <bool PACKED, bool VEC, bool REM>
 __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
@@ -618,7 +627,8 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
 }
 
 // Exponentials of 32 rows and a chunk of the positions, and the rows' sums, to which the chunks add.  A wave takes 256 positions of a row
-// at a time.  The table's entries are 4 MB, of which a wave asks for 64 lines at a time: reading them is bound by L2.
+// at a time, two of them under way.  The table's entries are 4 MB, of which a wave asks for 64 lines at a time: reading them is bound by L2
+// (606 us for the 2048 tokens above, the factors' products 208: 0.8 GB at 3.9 TB/s).
 template <bool FACTORS, bool SHIFTED>
 __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
     __shared__ int32_t top[kRows];
@@ -765,7 +775,9 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
 // Probabilities of 32 rows and their products with 128 elements of the values, over a chunk of the positions.  Eight threads a row make
 // the digits of 64 positions in LDS; a wave takes 32 elements and all rows, and turns its values into operands in registers.  A
 // probability is floor((e P + floor(S/2)) / S) from one product in double precision, as the scores' quotients are, where S is below 2^28 and P
-// at most 2^22; the remainder of the division gives the lookup's query.
+// at most 2^22; the remainder of the division gives the lookup's query.  Four waves of 32 elements leave 256 registers each, of which the sums
+// take 80 to 112 and spill a few.  Heads of more than 128 elements are divided among workgroups that make the probabilities again (one head of
+// 4096: 139 us).
 constexpr uint32_t kValueThreads = 256;
 constexpr uint64_t kPlainSum = (uint64_t)1 << 28;
 enum Written { kNone, kBoth, kSome };          // of the probabilities and queries
@@ -1078,7 +1090,7 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     GRAPE_REQUIRE(initialised(), "grape_init has not been called");
     GRAPE_REFUSED_IF(step::refuse_window(args, cache));
     if (!args->seqs || !args->rows || !args->max_new) return GRAPE_OK;
-    if (args->max_new == 1) return attend_single(*args, *cache, st);          // heads by sixteen and not rows by 32, one launch for few positions
+    if (args->max_new == 1) return attend_single(*args, *cache, st);          // heads by sixteen and not rows by 32, one launch for few positions (24 sequences behind a window of 1024: 79 us, and 84 here)
     WindowArgs p;
     p.a = *args;
     p.c = *cache;
