@@ -240,7 +240,7 @@ struct Division {
 struct Penalty {
     Division up, down;                         // of logits above zero, and of the others
     Scaler wide_up, wide_down;
-    int64_t scale, repetition;
+    int64_t scale, repetition, whole_presence, whole_frequency;
     double presence, frequency;
     bool divides, plain;
     __device__ __forceinline__ void apply(int32_t x, uint32_t count, double& y, int32_t& rem) const {
@@ -257,7 +257,9 @@ struct Penalty {
                 uint32_t beyond = 0;          // a quotient beyond int32 is still one of 64 bits
                 if (x > 0) wide_up.apply(product, q, rem, beyond);
                 else wide_down.apply(product, q, rem, beyond);
-                y = beyond ? (double)((product - rem) / by) : (double)q;
+                // up to 2^62, which a penalty of up to 2^55 may bring back to where every bit counts
+                y = (double)((beyond ? (product - rem) / by : (int64_t)q) - (whole_frequency * (int64_t)count + whole_presence));
+                return;
             }
         }
         y -= __builtin_fma(frequency, (double)count, presence);
@@ -307,8 +309,10 @@ __global__ void __launch_bounds__(kNextThreads, 6) wit_next_adjust_kernel(NextAr
         penalty.wide_up = Scaler{penalty.repetition, penalty.up.inv, -1};
         penalty.wide_down = p.scale;
     }
-    penalty.presence = a.d_presence ? (double)a.d_presence[b] : 0.0;
-    penalty.frequency = a.d_frequency ? (double)a.d_frequency[b] : 0.0;
+    penalty.whole_presence = a.d_presence ? a.d_presence[b] : 0;
+    penalty.whole_frequency = a.d_frequency ? a.d_frequency[b] : 0;
+    penalty.presence = (double)penalty.whole_presence;
+    penalty.frequency = (double)penalty.whole_frequency;
     __syncthreads();
     for (uint32_t from = 0; from < (uint32_t)len; from += kNextAhead * kNextThreads) {
         if (from) fetch(from);

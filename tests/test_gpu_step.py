@@ -663,6 +663,23 @@ def test_next_token_of_the_largest_numbers(ops):
             run_next(ops, {**c, "presence": None, "frequency": None, "bias": None}, scale=scale)
 
 
+@pytest.mark.parametrize("x", [(1 << 31) - 1, -(1 << 31) + 1])
+def test_next_token_of_penalties_that_cancel(ops, x):
+    """a quotient beyond 2^53 that the penalty for 2^23 occurrences brings back into 32 bits: every bit of both counts"""
+    n = (1 << 23) + 1
+    for rep in (259, 275) if x > 0 else ((1 << 31) - 40, (1 << 31) - 33):
+        scale = 1 << 31 if x > 0 else 300
+        y, by = (x * scale, rep) if x > 0 else (x * rep, scale)
+        y, rem = (y + by // 2) // by, y - (y + by // 2) // by * by
+        assert abs(y) > 1 << 53 and y % 2
+        frequency = y // n
+        assert abs(frequency) < 1 << 31
+        got = ops.wit_next_token(dev(np.array([[x, -5, 3]])), torch.zeros((1, n), dtype=torch.int32, device="cuda"), dev(np.array([n])), repetition=dev(np.array([rep])),
+                                 presence=dev(np.array([77])), frequency=dev(np.array([frequency])), scale=scale)
+        assert host(got["logits"])[0].tolist() == [y - frequency * n - 77, -5, 3] and host(got["rem"])[0].tolist() == [rem, 0, 0] and host(got["count"])[0].tolist() == [n, 0, 0]
+    assert ops.wit_status() == 0
+
+
 def test_next_token_reports_what_is_out_of_range(ops):
     rng = np.random.default_rng(3)
     c = next_case(rng, 4, 100, 30)
