@@ -16,8 +16,8 @@ namespace grape {
 // that is loaded; 16 would read keys and values twice as often, 64 leave no registers for the five sums of the planes' products.
 //
 // 2048 new tokens, 32 heads of 128 over 8, with a proof (1.34 GB written, 0.54 GB of it read again): 46 us operands, 158 scores, 208
-// exponentials, 248 values, each of the last three near what it writes and reads at 3.3 to 4 TB/s.  One head of 4096: 63 + 130 + 18 + 139 us, of which 142
-// are the products' at the rate of a large int8 one.  5 drafted tokens of 8 sequences of up to 3000: 35 + 15 + 39 + 5 us, chains of
+// exponentials, 248 values, each of the last three near what it writes and reads at 3.3 to 4 TB/s.  One head of 4096: 63 + 112 + 18 + 139 us, of which 142
+// to 176 are the products' at the rate of a large int8 one.  5 drafted tokens of 8 sequences of up to 3000: 35 + 15 + 39 + 5 us, chains of
 // dependent loads in short workgroups; a fourth wave of registers (128 of them) or other chunks are no faster.
 //
 // Both products run on the int8 matrix cores, exactly.  An element of magnitude below 2^23 is three balanced digits of base 256, the bytes
@@ -145,7 +145,7 @@ __device__ __forceinline__ int64_t offset_of(const WindowArgs& p, uint32_t b, co
 }
 
 // The queries' digits of a block of 512 elements in LDS, [step of 64][plane][lane group][row], 16 bytes each.
-constexpr uint32_t kBlockSteps = 8;
+constexpr uint32_t kBlockSteps = 8, kHalfQuads = kBlockSteps / 2 * step::kQueryStepBytes / 16 / 256;
 __device__ __forceinline__ const int32_t* query_of(const WindowArgs& p, const RowTile& w, uint32_t r) {
     const uint32_t tok = w.token(p, r);
     return p.a.d_q + (int64_t)(w.first + tok) * p.a.q_stride + (size_t)(w.kv * p.plan.each + (w.at + r - tok * p.plan.each)) * p.c.dim;
@@ -408,8 +408,8 @@ __global__ void __launch_bounds__(256) wit_window_pack_kernel(WindowArgs p) {
 // (PACKED), or from the cache into the operand (lane l the elements 64 s + 16 c + 4 (l / 16) .. + 4 of position l % 16); the queries' digits from LDS.
 // Five accumulators become a sum in double precision, exact below 2^53, and below 2^50 the quotient of (y + s/2 + 1/2) / s needs no
 // second look: it is no nearer than 1 / (2 s) to a whole number, and the product with 1 / s off by at most 2^-52 of itself.
-// Bound by vector instructions and stores together where a proof is made (100 us without them and 158 with, for the 2048 tokens above); by LDS
-// for heads of 4096: a wave reads 6 KB of the queries' digits for 18 products, 4 waves 170 bytes a clock of 128.
+// Bound by vector instructions and stores together where a proof is made (the 2048 tokens above: 158 us, 3.7 TB/s); heads of 4096 reach 1.4 POP/s of
+// the 1.8 that a large int8 product does (112 us; 130 when a block of queries was loaded between two barriers and not beside the products).
 template <bool PACKED, bool VEC, bool REM>
 __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
@@ -454,8 +454,8 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
     uint32_t over = 0;
     auto stage = [&](uint32_t block) {
         if constexpr (PACKED) {
-            const uint32_t n = min(steps - kBlockSteps * block, kBlockSteps) * (uint32_t)(step::kQueryStepBytes / 16);
-            const v4i_t* from = reinterpret_cast<const v4i_t*>(p.queries + ((size_t)blockIdx.x * steps + kBlockSteps * block) * step::kQueryStepBytes);
+            const uint32_t n = steps * (uint32_t)(step::kQueryStepBytes / 16);
+            const v4i_t* from = reinterpret_cast<const v4i_t*>(p.queries + (size_t)blockIdx.x * steps * step::kQueryStepBytes);
 #pragma unroll 4
             for (uint32_t i = threadIdx.x; i < n; i += 256) reinterpret_cast<v4i_t*>(lds)[i] = from[i];
         } else {
@@ -468,6 +468,25 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
         __syncthreads();
     }
     const v4i_t* q_digits = reinterpret_cast<const v4i_t*>(lds) + w.kg * kRows + w.col;
+    // PACKED, of more steps than LDS holds: half of what it holds at a time, in turn; the next half is under way while one is used
+    v4i_t under_way[kHalfQuads];
+    uint32_t turn = 0;
+    auto request_half = [&](uint32_t s) {
+        const uint32_t n = min(steps - s, kBlockSteps / 2) * (uint32_t)(step::kQueryStepBytes / 16);
+        const v4i_t* from = reinterpret_cast<const v4i_t*>(p.queries + ((size_t)blockIdx.x * steps + s) * step::kQueryStepBytes);
+#pragma unroll
+        for (uint32_t i = 0; i < kHalfQuads; i++) under_way[i] = from[min(threadIdx.x + 256 * i, n - 1)];
+    };
+    auto store_half = [&](uint32_t half) {
+        v4i_t* to = reinterpret_cast<v4i_t*>(lds) + half * kHalfQuads * 256;
+#pragma unroll
+        for (uint32_t i = 0; i < kHalfQuads; i++) to[threadIdx.x + 256 * i] = under_way[i];
+    };
+    if (PACKED && blocks > 1) {
+        request_half(0);
+        store_half(0);
+        __syncthreads();
+    }
     // PACKED: operands of two steps, each next pair requested as the one before it has been used
     v4i_t x[4], keys[2][3];
     auto request = [&](int half, uint32_t tile, uint32_t s) {
@@ -532,14 +551,21 @@ __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p)
                 multiply(keys[0], 0);
                 request(0, next_tile, 0);
             } else {
+                const bool halves = blocks > 1;
 #pragma unroll 1
                 for (uint32_t s = 0; s < steps; s += 2) {
-                    next_block(s);
                     const bool more = s + 2 < steps;
-                    multiply(keys[0], s % kBlockSteps);
+                    const uint32_t in_half = s % (kBlockSteps / 2), at = halves ? turn * (kBlockSteps / 2) + in_half : s;
+                    if (halves && in_half == 0) request_half(s + kBlockSteps / 2 < steps ? s + kBlockSteps / 2 : 0);
+                    multiply(keys[0], at);
                     request(0, more ? tile : next_tile, more ? s + 2 : 0);
-                    multiply(keys[1], s % kBlockSteps + 1);
+                    multiply(keys[1], at + 1);
                     request(1, more ? tile : next_tile, more ? s + 3 : 1);
+                    if (halves && (!more || in_half + 2 == kBlockSteps / 2)) {
+                        turn ^= 1;
+                        store_half(turn);
+                        __syncthreads();
+                    }
                 }
             }
         } else {
