@@ -191,6 +191,9 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     p.value_cols = (uint32_t)std::min<uint64_t>((cols + want - 1) / want, kValueMost);
     p.value_chunks = token::ceil_div(p.cols, p.value_cols);
     if (p.score_chunks > 65535 || p.exp_chunks > 65535 || (uint64_t)p.value_chunks * p.groups > 65535) return false;
+    // workgroups without rows or positions, of many sequences that might be long, take their time too
+    const uint64_t most = std::max<uint64_t>(std::max(p.score_chunks, p.exp_chunks), (uint64_t)p.value_chunks * p.groups);
+    if (tiles * cache_heads * most >= (uint64_t)1 << 27) return false;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     // Operands are made beforehand where each key and value then serves eight tiles of rows or more (24 sequences of 2000 positions, 32 heads of 128
     // over 8: 32 new tokens 674 us from the cache and 706 so, 12 of 64 tokens 671 and 627), in calls of 2^30 products or more (one such sequence:

@@ -226,6 +226,18 @@ def test_plans_cover_what_is_seen_within_their_limits(lib):
     assert taken > 1500 and packed > 50
 
 
+def test_launches_of_workgroups_without_work_are_bounded(lib):
+    """many sequences, each of which might be long, and few rows: what is launched is not what is there"""
+    assert plan_of(lib, 2, 60000, 64, 64, 64, 2, 65000 * 16 * 64, 0, 0) is None and plan_of(lib, 2, 60000, 64, 64, 64, 2, 131072, 0, 0) is None
+    assert plan_of(lib, 2, 2, 64, 64, 64, 2, 65000 * 16 * 64, 0, 0) and plan_of(lib, 16384, 4096, 64, 8, 128, 4, 131072, 0, 0) and plan_of(lib, 1 << 20, 1, 1, 1, 64, 1 << 17, 1 << 17, 100, 0)
+    rng = np.random.default_rng(5)
+    for _ in range(2000):
+        hk, n = int(2 ** rng.uniform(0, 8)), int(2 ** rng.uniform(1, 30))
+        size = (int(2 ** rng.uniform(0, 16)), int(2 ** rng.uniform(0, 16)), hk, hk, int(2 ** rng.uniform(0, 13)), 2, n, 0, 0)
+        p = plan_of(lib, *size)
+        assert p is None or p["tiles"] * hk * max(p["score_chunks"], p["exp_chunks"], p["value_chunks"] * p["groups"]) < 1 << 27
+
+
 def test_tiles_of_rows_are_owned_by_one_sequence(lib):
     """numbered from starts[b] * each / 32 + b on: no number twice, none beyond the plan's"""
     rng = np.random.default_rng(4)
