@@ -228,7 +228,7 @@ GRAPE_HD uint32_t seen_most(uint32_t max_len, uint32_t window, uint32_t sinks) {
     return window && (uint64_t)window + sinks < max_len ? window + sinks : max_len;
 }
 inline bool single_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len, uint32_t window, uint32_t sinks, token::AttentionPlan& p) {
-    return rows && max_len && token::attention_plan(seqs, heads, cache_heads, dim, seen_most(max_len, window, sinks), p, max_len, rows);
+    return rows && max_len && token::attention_plan(seqs, heads, cache_heads, dim, seen_most(max_len, window, sinks), p, rows);
 }
 inline size_t window_workspace(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_new, uint32_t max_len, uint32_t window, uint32_t sinks) {
     if (max_new == 1) {

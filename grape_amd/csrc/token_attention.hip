@@ -30,6 +30,7 @@ struct AttendArgs {
     uint32_t* status;
     const int32_t* d_starts;     // of a call with a window, see Span
     uint32_t rows, window, sinks;
+    bool scores_held, exp_held;  // by the workspace, see Place
 };
 
 // The positions lo <= t < hi that a sequence attends to, and its row.  With a window (WINDOW) and first tokens that stay visible the
@@ -55,6 +56,24 @@ struct Span {
         }
     }
     __device__ __forceinline__ uint32_t at(uint32_t t) const { return WINDOW && t < first ? t - gap : t; }
+};
+
+// Where a row's entries of number lo <= t < hi stand: in a tensor of max_len entries a row at their positions, or (`held`, with a window) in
+// the workspace, whose rows are as long as what a token attends to and begin with number lo: 24 sequences behind a window of 1024 that may
+// be 131072 long then need 10 MB and not 0.81 GB.
+template <bool WINDOW>
+struct Place {
+    size_t base;
+    uint32_t first = 0, gap = 0;
+    __device__ __forceinline__ Place(const AttendArgs& p, const Span<WINDOW>& span, size_t row, bool held) {
+        base = row * p.a.max_len;
+        if constexpr (WINDOW) {
+            first = held ? 0 : span.first;
+            gap = span.gap;
+            if (held) base = row * p.plan.row_held - span.lo;
+        }
+    }
+    __device__ __forceinline__ size_t at(uint32_t t) const { return base + (WINDOW && t < first ? t - gap : t); }
 };
 
 // The sequence, the chunk of `size` positions and the positions that are number `index` when the sequences' chunks are counted, one
@@ -282,16 +301,15 @@ template <bool WINDOW, class F>
 __device__ __forceinline__ void score_rows(const AttendArgs& p, const Tile& w, const Span<WINDOW>& span, uint32_t t0, uint32_t n, const int64_t* off, const uint64_t* sums, uint32_t stride,
                                            const unsigned long long* q_sum, uint32_t& bad, F largest) {
     for (uint32_t r = w.wave; r < w.R; r += 4) {
-        const size_t o = (w.row0 + r) * p.a.max_len;
+        const Place<WINDOW> score(p, span, w.row0 + r, p.scores_held), dense(p, span, w.row0 + r, false);
         const uint64_t more = (uint64_t)kCacheOffset * q_sum[r];
         int32_t mx = INT32_MIN;
         for (uint32_t i = w.lane; i < n; i += 64) {
             const int64_t y = off[i] < 0 ? 0 : (int64_t)(sums[r * stride + i] + more);          // a page outside: zero
-            const size_t to = o + span.at(t0 + i);
             int32_t q, rem;
             p.qk.apply(y, q, rem, bad);
-            p.a.d_scores[to] = q;
-            if (p.a.d_scores_rem) p.a.d_scores_rem[to] = rem;
+            p.a.d_scores[score.at(t0 + i)] = q;
+            if (p.a.d_scores_rem) p.a.d_scores_rem[dense.at(t0 + i)] = rem;
             mx = max(mx, q);
         }
 #pragma unroll
@@ -305,12 +323,12 @@ __device__ __forceinline__ void score_rows(const AttendArgs& p, const Tile& w, c
 constexpr uint32_t kExpAhead = 8;
 template <bool WINDOW>
 __device__ __forceinline__ unsigned long long exponentials(const AttendArgs& p, size_t row, const Span<WINDOW>& span, uint32_t t0, uint32_t from, uint32_t step, uint32_t n, int32_t mx, uint32_t& bad) {
-    const size_t o = row * p.a.max_len;
+    const Place<WINDOW> score(p, span, row, p.scores_held), exp(p, span, row, p.exp_held), dense(p, span, row, false);
     unsigned long long sum = 0;
     for (uint32_t t = from; t < n; t += step * kExpAhead) {
         int32_t x[kExpAhead], e[kExpAhead];
 #pragma unroll
-        for (uint32_t j = 0; j < kExpAhead; j++) x[j] = t + j * step < n ? p.a.d_scores[o + span.at(t0 + t + j * step)] : mx;
+        for (uint32_t j = 0; j < kExpAhead; j++) x[j] = t + j * step < n ? p.a.d_scores[score.at(t0 + t + j * step)] : mx;
 #pragma unroll
         for (uint32_t j = 0; j < kExpAhead; j++) {
             const int64_t idx = (int64_t)x[j] - mx + (((int64_t)1 << p.a.bit_shift) - 1);
@@ -323,9 +341,8 @@ __device__ __forceinline__ unsigned long long exponentials(const AttendArgs& p, 
             const uint32_t i = t + j * step;
             if (i >= n) break;
             if (e[j] < 0) bad |= (uint32_t)kWitSum;
-            const size_t to = o + span.at(t0 + i);
-            p.a.d_exp[to] = e[j];
-            if (p.a.d_shifted) p.a.d_shifted[to] = (int32_t)((int64_t)x[j] - mx);
+            p.a.d_exp[exp.at(t0 + i)] = e[j];
+            if (p.a.d_shifted) p.a.d_shifted[dense.at(t0 + i)] = (int32_t)((int64_t)x[j] - mx);
             sum += (unsigned long long)(e[j] < 0 ? 0 : e[j]);
         }
     }
@@ -616,8 +633,8 @@ __global__ void __launch_bounds__(256, 4) wit_attend_values_kernel(AttendArgs p)
             sum = 1;
         }
         if (chunk == 0 && group == 0 && row.from == 0 && p.a.d_sum) store_sum(&p.a.d_sum[at], sum, bad);
-        const int32_t* exps = p.a.d_exp + at * p.a.max_len;
-        const unsigned long long mine = probabilities<PP, kProbAhead>(p, w, row, span, t0, n, off, sum, group == 0, lds, bad, [&](uint32_t i) { return (uint32_t)max(exps[span.at(t0 + i)], 0); });
+        const Place<WINDOW> exps(p, span, at, p.exp_held);
+        const unsigned long long mine = probabilities<PP, kProbAhead>(p, w, row, span, t0, n, off, sum, group == 0, lds, bad, [&](uint32_t i) { return (uint32_t)max(p.a.d_exp[exps.at(t0 + i)], 0); });
         if (row.leads) atomicAdd(&p_sum[row.r], mine);
     }
     __syncthreads();
@@ -811,6 +828,8 @@ static int attend(AttendArgs& p, grape_stream_t st) {
     grape_wit_attention_args& a = p.a;
     const token::AttentionPlan& pl = p.plan;
     uint8_t* ws = (uint8_t*)a.d_workspace;
+    p.scores_held = WINDOW && !a.d_scores;
+    p.exp_held = WINDOW && !a.d_exp;
     if (!pl.whole && !a.d_scores) a.d_scores = (int32_t*)(ws + pl.at_scores);
     if (!pl.whole && !a.d_exp) a.d_exp = (int32_t*)(ws + pl.at_exp);
     p.chunk_max = (int32_t*)(ws + pl.at_max);

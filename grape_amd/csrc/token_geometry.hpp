@@ -106,6 +106,7 @@ struct AttentionPlan {
     bool counted;                      // the scores' and the values' workgroups find their chunk by counting (see find_chunk)
     bool whole;                        // one launch, a workgroup for all positions
     size_t whole_lds;
+    uint32_t row_held;                 // entries of a row of scores or exponentials in the workspace
     size_t at_scores, at_exp, at_max, at_sum, at_part, bytes;      // offsets in the workspace
 };
 constexpr uint32_t kTokenLds = 60 * 1024;      // of a workgroup; of one that takes all positions:
@@ -116,8 +117,8 @@ constexpr uint32_t kCountedMost = 256;        // sequences whose chunks are coun
 
 inline uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
 
-// `row_len`, `rows`: entries of a row of scores, and rows, where they are other than max_len positions and one of each sequence
-inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len, AttentionPlan& p, uint32_t row_len = 0, uint32_t rows = 0) {
+// max_len: how many positions a row attends to at most; `rows`: how many rows there are where it is more than one of each sequence
+inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_len, AttentionPlan& p, uint32_t rows = 0) {
     if (!seqs || !heads || !cache_heads || !dim || heads > 65535 || seqs > 65535 || heads % cache_heads || dim > 8192 || max_len >= (uint32_t)1 << 31) return false;
     const uint64_t rows_all = (uint64_t)seqs * heads;
     if ((unsigned __int128)rows_all * max_len >= (uint64_t)1 << 38) return false;
@@ -177,9 +178,9 @@ inline bool attention_plan(uint32_t seqs, uint32_t heads, uint32_t cache_heads, 
     p.whole_lds = 8 * kWholeMost + (size_t)8 * p.rows * (dim > kWholeMost ? dim : kWholeMost) + (size_t)4 * kWholeMost * p.rows + (one > two ? one : two);
     p.whole = p.whole_lds <= kWholeLds && max_len <= kWholeMost && dim <= 256;
     const uint64_t rows_held = (uint64_t)std::max(seqs, rows) * heads;
-    const uint32_t row_held = std::max(max_len, row_len);
-    if ((unsigned __int128)rows_held * row_held >= (uint64_t)1 << 38) return false;
-    const size_t row = (size_t)rows_held * row_held * 4;
+    if ((unsigned __int128)rows_held * max_len >= (uint64_t)1 << 38) return false;
+    p.row_held = max_len;
+    const size_t row = (size_t)rows_held * max_len * 4;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     p.at_scores = 0;
     p.at_exp = up(row);

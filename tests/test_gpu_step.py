@@ -364,6 +364,34 @@ def test_window_attention_with_some_outputs_and_a_kept_workspace(ops, exp_table,
     assert ops.wit_status() == 0
 
 
+@pytest.mark.parametrize("lens,max_len,window,sinks", [([5000, 1, 1023, 1024, 1025, 1028, 1029, 3000, 0], 6000, 1024, 4), ([700, 300, 299, 257], 100000, 256, 0), ([900, 2000], 2000, 300, 900),
+                                                       ([20, 60, 0, 400], 500, 40, 3), ([100000, 3], 100000, 5000, 70)])
+def test_single_tokens_keep_what_they_see_and_no_more(ops, exp_table, lens, max_len, window, sinks):
+    """scores and exponentials in a workspace of exactly its size, whose rows are as long as the window and the sinks: the answer, with or
+    without some of a proof's rows, is that of the call for several tokens, and nothing stands behind the workspace"""
+    rng = np.random.default_rng(sum(lens))
+    H, HK, D, page = 8, 2, 64, 16
+    new = [min(n, 1) for n in lens]
+    table, kc, vc = paged(rng, lens, page, HK, D)
+    starts = starts_of(new) + 1
+    q = gauss(rng, (int(starts[-1]) + 1, H, D))
+    args = (dev(q), dev(kc), dev(vc), dev(table), dev(starts), dev(np.array(lens)))
+    kw = {"window": window, "sinks": sinks, "qk_scale": 1 << 19}
+    shapes = {"qkv": (len(q), H, D), "qkv_rem": (len(q), H, D), "scores": (len(q), H, max_len), "exp_output": (len(q), H, max_len), "softmax_output": (len(q), H, max_len),
+              "scores_rem": (len(q), H, max_len), "exp_sum": (len(q), H)}
+    want = ops.wit_window_attention(*args, 2, max_len, dev(exp_table), out={x: filled(*t) for x, t in shapes.items()}, **kw)
+    size = ops.wit_window_attention_workspace(len(q), len(lens), H, HK, D, 1, max_len, window, sinks)
+    assert size < 4 * len(q) * H * (window + sinks) * 4 + len(q) * H * D * 8 * 40 + 4096
+    for keep in (("qkv", "qkv_rem"), ("qkv", "scores"), ("qkv", "exp_output"), ("qkv", "softmax_output", "scores_rem", "exp_sum"), tuple(shapes)):
+        space = torch.randint(-128, 127, (size + 4096,), device="cuda", dtype=torch.int8).view(torch.uint8)
+        behind = space[size:].clone()
+        got = ops.wit_window_attention(*args, 1, max_len, dev(exp_table), out={x: filled(*shapes[x]) for x in keep}, workspace=space[:size] if size else None, **kw)
+        for x in keep:
+            assert torch.equal(got[x], want[x]), (keep, x)
+        assert torch.equal(space[size:], behind)
+    assert ops.wit_status() == 0
+
+
 # ---- calls with many rows, whose queries, keys and values are turned into digits once
 def alone(ops, q, kc, vc, table, starts, lens, exp_table, max_len, window=0, sinks=0, **kw):
     """each token as a sequence of its own, one new token long"""

@@ -258,6 +258,22 @@ def test_workspace_of_refused_sizes(lib):
         assert lib.window_workspace(*good[:i], x, *good[i + 1:]) == 0, (i, x)
 
 
+def test_workspace_of_single_tokens_is_of_what_they_see(lib):
+    """behind a window a row of scores is as long as the window and the sinks, whatever the sequences' lengths are"""
+    rng = np.random.default_rng(6)
+    for _ in range(2000):
+        seqs, hk, longest, w = int(2 ** rng.uniform(0, 11)), int(2 ** rng.uniform(0, 4)), int(2 ** rng.uniform(0, 20)), int(2 ** rng.uniform(0, 14))
+        sinks, h, d = int(rng.choice([0, 1, 4, 300])), hk * int(2 ** rng.uniform(0, 4)), int(2 ** rng.uniform(0, 9))
+        got = lib.window_workspace(seqs, seqs, h, hk, d, 1, longest, w, sinks)
+        assert got == lib.window_workspace(seqs, seqs, h, hk, d, 1, min(longest, w + sinks), 0, 0)
+    size = (24, 24, 32, 8, 128, 1, 131072)
+    row = 24 * 32 * 1028 * 4
+    assert 2 * row < lib.window_workspace(*size, 1024, 4) < 4 * row and lib.window_workspace(*size, 0, 0) > 24 * 32 * 131072 * 8
+    # a call that fits is not refused for the positions that nobody sees: 65535 sequences that may have 2^20
+    assert lib.window_workspace(65535, 65535, 32, 8, 128, 1, 1 << 20, 1024, 4) > 0
+    assert lib.refuse_window(window(n=65535, rows=65535, heads=32, new=1, max_len=1 << 20, window=1024, sinks=4, wb=1 << 50), cache(heads=8, dim=128)) is None
+
+
 # ------------------------------------------------------------------ the next token
 NEXT = dict(x=0x100000, h=0x200000, hl=0x300000, rep=0, pre=0, fre=0, b=0x400000, m=0x500000, o=0x600000, r=0x700000, c=0x800000, g=0x900000, t=0xa00000, mx=0xb00000, ws=0xc00000,
             wb=1 << 20, xs=1000, hs=50, bs=0, ms=0, scale=1 << 16, n=4, vocab=1000, history=50, res=0)
