@@ -248,6 +248,44 @@ GRAPE_HD bool new_tokens(int32_t s, int32_t e, int32_t len, uint32_t rows, uint3
     return ok;
 }
 
+// The sequence that tile of rows `ti` belongs to; any other where it belongs to none.  One search, ballot(f) asking 64 sequences at a time
+// what f says of lane 0 .. 63, for the last one whose tiles start at ti or before.  An entry that is no row of the call starts no tiles, so that the
+// others, which ascend, are searched as if it was not there; but where it was asked for its part of the sequences the search ends at one before it, whose
+// rows then have no end (not has_rows), and all are gone through.
+GRAPE_HD bool is_row(int32_t s, uint32_t rows) { return (uint32_t)s <= rows; }          // rows <= 2^24: no negative one is
+GRAPE_HD bool has_rows(int32_t s, int32_t e, uint32_t rows) { return is_row(s, rows) && is_row(e, rows) && s <= e; }
+GRAPE_HD uint64_t first_tile(int32_t s, uint32_t b, uint32_t each) { return (uint64_t)(uint32_t)s * each / kRows + b; }
+GRAPE_HD uint32_t last_lane(unsigned long long lanes) { return 63u - (uint32_t)__builtin_clzll(lanes); }
+template <class Ballot>
+GRAPE_HD uint32_t search_tile(const int32_t* starts, uint32_t seqs, uint32_t rows, uint32_t each, uint32_t ti, Ballot ballot) {
+    uint32_t lo = 0, left = seqs;
+    while (left > 1) {
+        const uint32_t step = (left + 63) / 64;
+        const unsigned long long before = ballot([&](uint32_t lane) {
+            const uint32_t at = lane * step < left ? lo + lane * step : lo + left - 1;
+            const int32_t s = starts[at];
+            return lane * step < left && is_row(s, rows) && first_tile(s, at, each) <= ti;
+        });
+        const uint32_t last = before ? last_lane(before) : 0;
+        lo += last * step;
+        left = left - last * step < step ? left - last * step : step;
+    }
+    return lo;
+}
+template <class Ballot>
+GRAPE_HD uint32_t scan_for_tile(const int32_t* starts, uint32_t seqs, uint32_t rows, uint32_t each, uint32_t ti, Ballot ballot) {
+    for (uint32_t base = 0; base < seqs; base += 64) {
+        const unsigned long long here = ballot([&](uint32_t lane) {
+            const uint32_t b = base + lane;
+            if (b >= seqs) return false;
+            const int32_t s = starts[b], e = starts[b + 1];
+            return has_rows(s, e, rows) && first_tile(s, b, each) <= ti && (ti - first_tile(s, b, each)) * kRows < (uint64_t)(uint32_t)(e - s) * each;
+        });
+        if (here) return base + last_lane(here);
+    }
+    return 0;
+}
+
 // The positions that a tile of rows with the tokens at pos0 .. pos1 sees, in tiles: `sink_tiles` from 0 on, then those from tile
 // `from` on, `tiles` in all.
 struct Seen {

@@ -97,21 +97,18 @@ struct RowTile {
         // the heads of one tile are neighbours, so that each die's L2 gets the keys of its own heads where there are eight; long rows first
         kv = index % p.c.heads;
         const uint32_t ti = p.plan.tiles - 1 - index / p.c.heads;
-        auto tile0 = [&](uint32_t s) { return (uint32_t)max(p.a.d_starts[s], 0) * (uint64_t)p.plan.each / kRows + s; };
-        // the last sequence whose tiles start at ti or before, 64 of them asked at a time
-        uint32_t lo = 0, left = p.a.seqs;
-        while (left > 1) {
-            const uint32_t step = (left + 63) / 64, probe = lane * step;
-            const unsigned long long before = __ballot(probe < left && tile0(lo + min(probe, left - 1)) <= ti);
-            const uint32_t last = before ? 63 - (uint32_t)__builtin_clzll(before) : 0;
-            lo += last * step;
-            left = min(step, left - last * step);
+        auto ballot = [&](auto f) { return __ballot(f(lane)); };
+        b = step::search_tile(p.a.d_starts, p.a.seqs, p.a.rows, p.plan.each, ti, ballot);
+        int32_t s = p.a.d_starts[b], e = p.a.d_starts[b + 1], len = p.a.d_lens[b];
+        if (!step::has_rows(s, e, p.a.rows)) {
+            b = step::scan_for_tile(p.a.d_starts, p.a.seqs, p.a.rows, p.plan.each, ti, ballot);
+            s = p.a.d_starts[b];
+            e = p.a.d_starts[b + 1];
+            len = p.a.d_lens[b];
         }
-        b = lo;
-        const int32_t s = p.a.d_starts[b];
-        if (!step::new_tokens(s, p.a.d_starts[b + 1], p.a.d_lens[b], p.a.rows, p.a.max_new, p.a.max_len, (uint64_t)p.a.table_stride * p.c.page_size, n, pos)) return false;
+        if (!step::new_tokens(s, e, len, p.a.rows, p.a.max_new, p.a.max_len, (uint64_t)p.a.table_stride * p.c.page_size, n, pos)) return false;
         first = (uint32_t)s;
-        const uint64_t base = tile0(b);
+        const uint64_t base = step::first_tile(s, b, p.plan.each);
         if (ti < base) return false;
         const uint64_t local = (uint64_t)(ti - base) * kRows, all = (uint64_t)n * p.plan.each;
         if (local >= all) return false;

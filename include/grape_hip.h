@@ -814,8 +814,9 @@ int grape_wit_page_step(const grape_wit_page_step_args *args, grape_stream_t str
  * [rows][heads][max_len], and positions that a token does not attend to, like rows of no sequence, are left as they were.
  *
  * max_new and max_len bound the sequences' new tokens and lengths.  A sequence outside these bounds, with fewer tokens than rows,
- * or with more than table_stride*page_size, sets GRAPE_WIT_INDEX, and its rows are left as they were.  Pages that no token of
- * the call sees are not read.  rows <= 2^24.  d_workspace as for grape_wit_paged_attention, grape_wit_window_attention_workspace(...)
+ * or with more than table_stride*page_size, sets GRAPE_WIT_INDEX, and its rows are left as they were: an entry of d_starts that is not in
+ * 0..rows does that to the two sequences that it bounds.  The other entries ascend; where one does not (GRAPE_WIT_INDEX again), rows of any
+ * sequence may be left as they were.  Pages that no token of the call sees are not read.  rows <= 2^24.  d_workspace as for grape_wit_paged_attention, grape_wit_window_attention_workspace(...)
  * bytes. */
 typedef struct {
     const int32_t *d_q;

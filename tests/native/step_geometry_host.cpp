@@ -36,6 +36,18 @@ int sequence(int32_t len, int32_t n, uint64_t most, uint32_t page, uint32_t wind
 int new_tokens(int32_t s, int32_t e, int32_t len, uint32_t rows, uint32_t max_new, uint32_t max_len, uint64_t most, uint32_t* o) {
     return step::new_tokens(s, e, len, rows, max_new, max_len, most, o[0], o[1]);
 }
+// the sequence that every tile of rows is given to
+void tile_owners(const int32_t* starts, uint32_t seqs, uint32_t rows, uint32_t each, uint32_t tiles, uint32_t* o) {
+    auto ballot = [](auto f) {
+        unsigned long long lanes = 0;
+        for (uint32_t lane = 0; lane < 64; lane++) lanes |= (unsigned long long)(f(lane) ? 1 : 0) << lane;
+        return lanes;
+    };
+    for (uint32_t t = 0; t < tiles; t++) {
+        o[t] = step::search_tile(starts, seqs, rows, each, t, ballot);
+        if (!step::has_rows(starts[o[t]], starts[o[t] + 1], rows)) o[t] = step::scan_for_tile(starts, seqs, rows, each, t, ballot);
+    }
+}
 int sees(uint32_t pos, uint32_t t, uint32_t window, uint32_t sinks) { return step::sees(pos, t, window, sinks); }
 // the tiles of positions that tokens pos0 .. pos1 see, and for n of them from v0 on those that all see
 uint32_t seen_tiles(uint32_t pos0, uint32_t pos1, uint32_t window, uint32_t sinks, uint32_t v0, uint32_t n, uint32_t* tiles, uint32_t* numbers, uint32_t* full) {

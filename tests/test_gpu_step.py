@@ -289,6 +289,29 @@ def test_window_attention_reports_bad_sequences_and_pages(ops, exp_table, max_ne
         assert ops.wit_status() & 2, st
 
 
+@pytest.mark.parametrize("new,H,HK,D", [([128, 20, 12, 30], 2, 2, 64), ([300, 280, 260, 290], 16, 2, 128), ([2, 1, 3] * 30, 4, 1, 32), ([1] * 199 + [2], 2, 1, 16), ([1] * 100, 2, 1, 64)])
+def test_window_attention_beside_starts_that_are_no_rows(ops, exp_table, new, H, HK, D):
+    """a start that is no row of the call leaves the rows of the two sequences that it bounds as they were, and all others get theirs"""
+    rng = np.random.default_rng(sum(new))
+    lens, page = [n + int(x) for n, x in zip(new, rng.integers(0, 40, len(new)))], 16
+    table, kc, vc = paged(rng, lens, page, HK, D)
+    starts, L, n = starts_of(new), max(lens), len(new)
+    q, k, v, lens = gauss(rng, (int(starts[-1]), H, D)), dev(kc), dev(vc), dev(np.array(lens))
+    call = lambda st, **kw: ops.wit_window_attention(dev(q), k, v, dev(table), dev(st), lens, max(new), L, dev(exp_table), qk_scale=65536 * 11, **kw)  # noqa: E731
+    shapes = {"qkv": q.shape, "qkv_rem": q.shape, "max": q.shape[:2], "exp_sum": q.shape[:2]} | {x: q.shape[:2] + (L,) for x in PROOF}
+    want = call(starts, out={x: filled(*t) for x, t in shapes.items()})
+    assert ops.wit_status() == 0
+    for bad in ([n // 2], [1], [0], [n], [n - 1, n], list(range(n // 3, n)), [1, n // 2, n - 1], list(range(0, n, 3)), list(range(0, n + 1, 64))):
+        st = starts.copy()
+        st[bad] = rng.choice([-1, len(q) + 1, (1 << 31) - 1, -(1 << 31)], len(bad))
+        out = call(st, out={x: filled(*t.shape) for x, t in want.items()})
+        assert ops.wit_status() == 2
+        gone = {b for i in bad for b in (i - 1, i)}
+        there = torch.tensor([b not in gone for b in range(n) for _ in range(new[b])], device="cuda")
+        for x in shapes:
+            assert torch.equal(out[x][there], want[x][there]) and bool((out[x][~there] == UNTOUCHED).all()), (bad, x)
+
+
 def test_window_attention_reports_its_table_and_sums(ops, exp_table):
     rng = np.random.default_rng(10)
     table, kc, vc = paged(rng, [200], 16, 1, 64)

@@ -28,7 +28,7 @@ def lib():
     for name, args, res in (("refuse_pages", [p], ctypes.c_char_p), ("refuse_window", [p, p], ctypes.c_char_p), ("refuse_next", [p], ctypes.c_char_p), ("struct_bytes", [ctypes.c_int], z),
                             ("window_workspace", [u] * 9, z), ("next_workspace", [u] * 2, z), ("next_of", [u, u, p], None), ("sequence", [i, i, q, u, u, u, p, u], ctypes.c_int),
                             ("new_tokens", [i, i, i, u, u, u, q, p], ctypes.c_int), ("sees", [u] * 4, ctypes.c_int), ("seen_tiles", [u] * 6 + [p] * 3, u), ("any", [u] * 5, ctypes.c_int),
-                            ("window_of", [u] * 9 + [p], ctypes.c_int), ("pages_fields", [p, p], None), ("window_fields", [p, p], None), ("next_fields", [p, p], None)):
+                            ("window_of", [u] * 9 + [p], ctypes.c_int), ("tile_owners", [p, u, u, u, u, p], None), ("pages_fields", [p, p], None), ("window_fields", [p, p], None), ("next_fields", [p, p], None)):
         getattr(l, name).argtypes, getattr(l, name).restype = args, res
     return l
 
@@ -249,6 +249,39 @@ def test_tiles_of_rows_are_owned_by_one_sequence(lib):
         p = plan_of(lib, max(rows, 1), seqs, each, 1, 64, 300, 300, 0, 0)
         numbers = [int(starts[b]) * each // 32 + b + i for b in range(seqs) for i in range(-(-int(new[b]) * each // 32))]
         assert len(set(numbers)) == len(numbers) and max(numbers, default=0) < p["tiles"]
+
+
+def owners_of(lib, starts, rows, each):
+    """the sequence that each tile of rows is given to, and of those whose rows are some the one that it should be"""
+    starts = np.asarray(starts, dtype=np.int32)
+    seqs = len(starts) - 1
+    tiles = rows * each // 32 + seqs
+    got = np.zeros(tiles, dtype=np.uint32)
+    lib.tile_owners(starts.ctypes.data, seqs, rows, each, tiles, got.ctypes.data)
+    want = np.full(tiles, -1, dtype=np.int64)
+    for b, (s, e) in enumerate(zip(starts.tolist(), starts[1:].tolist())):
+        if 0 <= s <= e <= rows:
+            want[s * each // 32 + b:s * each // 32 + b + -(-(e - s) * each // 32)] = b
+    return got, want
+
+
+def test_tiles_of_rows_find_their_sequence_beside_entries_that_are_no_rows(lib):
+    """an entry of the starts that is no row of the call takes the two sequences that it bounds with it, and no other"""
+    got, want = owners_of(lib, [0, 128, -1, 160], 160, 1)
+    assert got[:4].tolist() == [0] * 4 and want[:4].tolist() == [0] * 4
+    rng = np.random.default_rng(7)
+    for _ in range(400):
+        each, seqs = int(rng.integers(1, 40)), int(2 ** rng.uniform(0, 9))
+        if rng.random() < 0.05:
+            seqs = int(rng.integers(4000, 9000))
+        starts = np.concatenate(([0], np.cumsum(rng.integers(0, int(rng.choice([2, 3, 30])), seqs)))) + int(rng.integers(0, 5))
+        rows = int(starts[-1]) + int(rng.integers(0, 3))
+        at = rng.random(seqs + 1) < rng.choice([0, 0.01, 0.1, 0.7])
+        starts[at] = rng.choice([-1, -LARGE, LARGE - 1, rows + 1], int(at.sum()))
+        if rng.random() < 0.3:                             # entries behind the last sequence that are not made
+            starts[int(rng.integers(0, seqs + 1)):] = -1
+        got, want = owners_of(lib, starts, rows, each)
+        assert (got < seqs).all() and np.array_equal(got[want >= 0], want[want >= 0])
 
 
 def test_workspace_of_refused_sizes(lib):
