@@ -159,6 +159,7 @@ constexpr uint32_t kValueMost = 511;          // tiles of positions: four produc
 constexpr uint32_t kPackTiles = 8, kPackSteps = 4;          // tiles of rows that operands made beforehand serve at least; steps of a workgroup
 constexpr uint64_t kPackProducts = (uint64_t)1 << 30;
 constexpr size_t kKeyStepBytes = 3 * kCols * 64, kQueryStepBytes = 3 * kRows * 64, kValueStepBytes = 3 * kCols * 64;
+constexpr uint32_t kJoinRows = 4;              // of a workgroup that joins the values' chunks
 constexpr uint32_t kOffsetTiles = 16;          // tiles of positions whose offsets a values workgroup holds
 
 inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim, uint32_t max_new, uint32_t max_len, uint32_t window, uint32_t sinks,
@@ -191,8 +192,10 @@ inline bool window_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t c
     p.value_cols = (uint32_t)std::min<uint64_t>((cols + want - 1) / want, kValueMost);
     p.value_chunks = token::ceil_div(p.cols, p.value_cols);
     if (p.score_chunks > 65535 || p.exp_chunks > 65535 || (uint64_t)p.value_chunks * p.groups > 65535) return false;
-    // workgroups without rows or positions, of many sequences that might be long, take their time too
-    const uint64_t most = std::max<uint64_t>(std::max(p.score_chunks, p.exp_chunks), (uint64_t)p.value_chunks * p.groups);
+    // workgroups without rows or positions, of many sequences that might be long, take their time too; the join's are many where few rows of long
+    // heads stand beside many sequences without any
+    const uint64_t joins = p.value_chunks > 1 ? (uint64_t)p.dim64 * (kRows / kJoinRows) : 0;
+    const uint64_t most = std::max(std::max<uint64_t>(std::max(p.score_chunks, p.exp_chunks), (uint64_t)p.value_chunks * p.groups), joins);
     if (tiles * cache_heads * most >= (uint64_t)1 << 27) return false;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     // Operands are made beforehand where each key and value then serves eight tiles of rows or more (24 sequences of 2000 positions, 32 heads of 128

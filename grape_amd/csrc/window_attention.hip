@@ -1080,11 +1080,11 @@ __global__ void __launch_bounds__(kValueThreads, 2) wit_window_values_kernel(Win
 }
 
 // The chunks' partial sums of 64 elements of a row, a wave each.
-__global__ void __launch_bounds__(256) wit_window_join_kernel(WindowArgs p) {
+__global__ void __launch_bounds__(64 * step::kJoinRows) wit_window_join_kernel(WindowArgs p) {
     RowTile w;
     if (!w.find(p, blockIdx.x)) return;
     const step::Seen seen = w.seen(p);
-    const uint32_t r = blockIdx.z * 4 + w.wave, e = blockIdx.y * 64 + w.lane, dim = p.c.dim;
+    const uint32_t r = blockIdx.z * step::kJoinRows + w.wave, e = blockIdx.y * 64 + w.lane, dim = p.c.dim;
     if (seen.tiles <= p.plan.value_cols || r >= w.R || e >= dim) return;
     const uint32_t parts = (seen.tiles - 1) / p.plan.value_cols + 1;
     uint32_t bad = 0;
@@ -1189,7 +1189,7 @@ int grape_wit_window_attention(const grape_wit_window_attention_args* args, cons
     else values_by(integral_constant<int, 4>{});
     GRAPE_LAUNCH_CHECK();
     if (pl.value_chunks > 1) {
-        wit_window_join_kernel<<<dim3(p.along, pl.dim64, kRows / 4), 256, 0, s>>>(p);
+        wit_window_join_kernel<<<dim3(p.along, pl.dim64, kRows / step::kJoinRows), 64 * step::kJoinRows, 0, s>>>(p);
         GRAPE_LAUNCH_CHECK();
     }
     return GRAPE_OK;

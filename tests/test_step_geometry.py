@@ -238,6 +238,24 @@ def test_launches_of_workgroups_without_work_are_bounded(lib):
         assert p is None or p["tiles"] * hk * max(p["score_chunks"], p["exp_chunks"], p["value_chunks"] * p["groups"]) < 1 << 27
 
 
+def test_launches_that_join_are_bounded(lib):
+    """a workgroup for 64 elements of four rows of every tile, of sequences without rows too"""
+    assert plan_of(lib, 2, 65535, 8, 8, 8192, 2, 40000, 0, 0) is None
+    assert plan_of(lib, 2, 16383 - 1, 8, 8, 8192, 2, 40000, 0, 0)["value_chunks"] == 2 and plan_of(lib, 2, 16384, 8, 8, 8192, 2, 40000, 0, 0) is None
+    assert plan_of(lib, 2, 65535, 8, 8, 8192, 2, 30000, 0, 0)["value_chunks"] == 1          # nothing is joined
+    rng = np.random.default_rng(8)
+    joined = 0
+    for _ in range(4000):
+        hk, n, seqs = int(2 ** rng.uniform(0, 8)), int(2 ** rng.uniform(10, 20)), int(2 ** rng.uniform(0, 16))
+        rows = int(rng.choice([seqs, 1 + seqs // 4, 2 ** rng.uniform(0, 10)]))
+        size = (rows, seqs, hk, hk, int(2 ** rng.uniform(0, 13)), 2, n, 0, 0)
+        p = plan_of(lib, *size)
+        if p and p["value_chunks"] > 1:
+            joined += 1
+            assert p["tiles"] * hk * p["dim64"] * 8 < 1 << 27, size
+    assert joined > 500
+
+
 def test_tiles_of_rows_are_owned_by_one_sequence(lib):
     """numbered from starts[b] * each / 32 + b on: no number twice, none beyond the plan's"""
     rng = np.random.default_rng(4)
