@@ -812,6 +812,7 @@ struct ValueLds {
     int64_t off[2][step::kOffsetTiles * kCols];
     unsigned long long p_sum[kRows];
     uint32_t third[2], wide, outside;          // the last tile with digits in the third plane (and 1), of even and odd ones; whether a page is outside the cache
+    uint32_t large;                            // whether a row's sum is kPlainSum or more
 };
 
 template <int PP, bool WIDE, Written W, bool PACKED>
@@ -830,7 +831,9 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     }
     if (!WIDE && r < w.R && group == 0 && chunk == 0 && part == 0 && p.a.d_sum) store_sum(&p.a.d_sum[row], sum, bad);
     const double inv = 1.0 / (double)sum, scale = (double)p.a.prob_scale, half = (double)(sum >> 1) + 0.5, whole_sum = (double)sum, odd = (double)(sum & 1) - 1.0;
-    const bool plain = PP == 3 && __all(sum < kPlainSum);
+    // Both choose between loops that meet at barriers, so they are the workgroup's: read behind a barrier that follows what is written to them, and
+    // written again behind another one.
+    bool plain = false, outside = false;
     // of the values: elements e0 + 2 col, + 1; lanes behind the last element take it again
     const uint32_t e0 = group * step::kValueDims + 32 * w.wave, el = e0 + 2 * w.col;
     const bool pairs = dim % 2 == 0;
@@ -939,6 +942,7 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
                 if ((tile + 1) % K == 0) {
                     make_offsets(tile + 1);
                     __syncthreads();
+                    outside = __builtin_amdgcn_readfirstlane((int)lds.outside) != 0;
                 }
                 fetch_values(tile + 1);
             }
@@ -968,7 +972,7 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
                 d[j] = (there >> (4 * h + j)) & 1u ? pr[h][j] : 0;
-                if (!PACKED && !FULL && lds.outside && offset_of(p, w.b, seen, t + 4 * h + j) < 0) d[j] = 0;          // a page outside: no value
+                if (!PACKED && !FULL && outside && offset_of(p, w.b, seen, t + 4 * h + j) < 0) d[j] = 0;          // a page outside: no value
                 if constexpr (WIDE) all += (uint32_t)d[j];
             }
             if constexpr (PP == 3) {
@@ -1002,17 +1006,20 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
         if constexpr (PP > 3) multiply(std::integral_constant<int, 3>{});
         if constexpr (PACKED) request(FULL ? tile + 1 : min(tile + 1, tiles - 1));
     };
+    if constexpr (PACKED) request(0);
     __syncthreads();
     if (threadIdx.x < 2) lds.third[threadIdx.x] = 0;
     if (threadIdx.x == 0) lds.outside = 0;
+    if (sum >= kPlainSum) lds.large = 1;
     __syncthreads();
+    plain = PP == 3 && __builtin_amdgcn_readfirstlane((int)lds.large) == 0;
     if constexpr (PACKED) {
         for (uint32_t i = threadIdx.x; i < tiles * p.plan.splits; i += kValueThreads)
             if (p.over[p.tile_of(w.b, w.kv, made.number(seen.tile(v0 + i / p.plan.splits))) * p.plan.splits + i % p.plan.splits] & 2u) over = kOver;
-        request(0);
     } else {
         make_offsets(0);
         __syncthreads();
+        outside = __builtin_amdgcn_readfirstlane((int)lds.outside) != 0;
         fetch_values(0);
     }
     fetch_exps(0, std::false_type{});
@@ -1023,7 +1030,7 @@ __device__ __forceinline__ bool window_values(const WindowArgs& p, const RowTile
     for (; tile < full0; tile++) body(tile, std::false_type{});
     wait_for_memory();
 #pragma unroll 1
-    for (; plain && tile + 1 < full1 && !lds.outside; tile++) body(tile, std::true_type{});
+    for (; plain && tile + 1 < full1 && !outside; tile++) body(tile, std::true_type{});
 #pragma unroll 1
     for (; tile < tiles; tile++) body(tile, std::false_type{});
     if constexpr (WIDE) {
@@ -1071,7 +1078,7 @@ __global__ void __launch_bounds__(kValueThreads, 2) wit_window_values_kernel(Win
     const uint32_t group = GROUPS ? blockIdx.y % p.plan.groups : 0, chunk = GROUPS ? blockIdx.y / p.plan.groups : blockIdx.y;
     if (chunk * p.plan.value_cols >= seen.tiles) return;
     uint32_t bad = 0;
-    if (threadIdx.x == 0) lds.wide = 0;
+    if (threadIdx.x == 0) lds.wide = lds.large = 0;          // behind window_values' first barrier the others write them
     bool wide;
     if (W != kNone && GROUPS && group) wide = window_values<PP, false, kNone, PACKED>(p, w, seen, lds, group, chunk, bad);
     else wide = window_values<PP, false, W, PACKED>(p, w, seen, lds, group, chunk, bad);

@@ -535,6 +535,27 @@ def test_window_attention_of_wide_sums(ops, exp_table, n, H, D):
     assert ops.wit_status() == 0
 
 
+@pytest.mark.parametrize("prob_scale", [1 << 16, 1 << 22, 1 << 24])
+def test_window_attention_of_rows_that_go_different_ways(ops, exp_table, prob_scale):
+    """rows of one tile whose sums are below and above 2^28, and pages outside the cache that turn up between tiles that all rows see"""
+    rng = np.random.default_rng(38)
+    for new, n, H, HK, D in ((40, 2600, 4, 4, 64), (33, 2600, 2, 2, 33), (260, 2600, 16, 2, 128)):
+        table, kc, vc = paged(rng, [n], 16, HK, D)
+        q, k, v = gauss(rng, (new, H, D)), dev(kc), dev(vc)
+        # all entries the same, so that a row's sum says how many positions it sees: 2^28 in the middle of the new tokens
+        flat = np.full(1 << 20, (1 << 28) // (n - new // 2), dtype=np.int32)
+        for bad in ([], [120], [64, 70, 128, 161], [1, 162]):
+            t = table.copy()
+            t[0, bad] = -1
+            want = alone(ops, q, k, v, t, [0, new], [n], flat, n, qk_scale=65536 * 11, prob_scale=prob_scale, out_scale=prob_scale)
+            status = ops.wit_status()
+            assert (status & 2 != 0) == bool(bad) and int(want["exp_sum"].min()) < 1 << 28 <= int(want["exp_sum"].max())
+            got = ops.wit_window_attention(dev(q), k, v, dev(t), dev(np.array([0, new])), dev(np.array([n])), new, n, dev(flat), qk_scale=65536 * 11, prob_scale=prob_scale, out_scale=prob_scale)
+            assert ops.wit_status() == status
+            for x in want:
+                assert torch.equal(got[x], want[x]), (new, bad, x)
+
+
 def test_window_attention_of_a_long_cache(ops):
     """131072 positions of the same score and value, whose digits' products would leave 32 bits if all were added up there"""
     n, new, H, D = 131072, 128, 16, 1024
