@@ -132,6 +132,13 @@ inline const char* refuse_next(const grape_wit_next_token_args* a) {
         for (int o = 0; o < 7; o++)
             GRAPE_REFUSE(ranges_meet(in[i], 4 * ((size_t)(a->seqs - 1) * stride[i] + a->vocab), out[o], out_bytes[o]) &&
                              !(i == 0 && o == 0 && in[i] == out[o] && (a->seqs == 1 || stride[i] == (int64_t)a->vocab)), "an output overlaps an input");
+    // what the first launch reads beside them must not be what it writes (all but d_token and d_max); entries of the history behind its lengths are not used,
+    // so it is not looked at here
+    const size_t words = ((size_t)a->seqs - 1) * (size_t)a->mask_stride + (a->vocab + 31) / 32;
+    const void* beside[] = {a->d_history_lens, a->d_repetition, a->d_presence, a->d_frequency, a->d_mask};
+    const size_t beside_bytes[] = {a->history ? one : 0, one, one, one, 4 * words};
+    for (int i = 0; i < 5; i++)
+        for (int o = 0; o < 7; o++) GRAPE_REFUSE(o != 4 && o != 5 && ranges_meet(beside[i], beside_bytes[i], out[o], out_bytes[o]), "an output overlaps an input");
     return nullptr;
 }
 

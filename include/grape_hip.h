@@ -842,7 +842,8 @@ int grape_wit_window_attention(const grape_wit_window_attention_args *args, cons
  * d_token[b] is the token with the largest logit, the first of several, or -1 where all are excluded; d_max[b] that logit.  For a
  * proof, [seqs][vocab] each: d_out the logits, d_rem the division's remainders (0 where there was none), d_count, and d_gap, the
  * largest logit less each (0 where excluded), to be looked up in a range.  All but d_token may be NULL; d_out may be d_logits where
- * logits_stride = vocab, else outputs must not overlap each other or logits and biases.
+ * logits_stride = vocab, else outputs must not overlap each other or logits and biases, nor those of a proof and d_workspace any other input (d_token
+ * and d_max are written when these have been read).
  *
  * A logit beyond int32 sets GRAPE_WIT_QUOTIENT and becomes the nearest one that is not excluded; a gap beyond int32 sets
  * GRAPE_WIT_SUM_WIDE, with its low 32 bits stored.  rep < 1 (taken as none), a history length outside 0..history (taken as the

@@ -801,6 +801,21 @@ def test_next_token_of_strided_rows_in_place_and_with_some_outputs(ops):
     assert ops.wit_status() == 0
 
 
+def test_next_token_appends_to_its_history(ops):
+    """the token goes behind those it was chosen by, its logit where a penalty stood: both are written when all has been read"""
+    rng = np.random.default_rng(5)
+    for vocab in (50, 40000):
+        c = next_case(rng, 1, vocab, 3000)
+        history = dev(np.concatenate((c["history"], np.full((1, 50), -9, dtype=np.int32)), 1))
+        for n in range(2990, 3010):
+            d = {x: dev(np.asarray(t)) for x, t in c.items()} | {"history": history, "history_lens": dev(np.array([n]))}
+            want = ops.wit_next_token(**{**d, "history": history.clone()})
+            got = ops.wit_next_token(**d, out={"token": history[0, n:n + 1], "max": d["presence"]})
+            assert torch.equal(history[0, n:n + 1], want["token"]) and torch.equal(got["max"], want["max"])
+            c["logits"] = gauss(rng, (1, vocab), 200000.0)
+    assert ops.wit_status() == 0
+
+
 # ------------------------------------------------------------------ together
 def test_a_step_after_the_other(ops, exp_table):
     """requests with prompts, then their answers token by token: pages, rotation and append, attention, a projection as the head, the next token -

@@ -361,6 +361,25 @@ def test_choices_whose_outputs_overlap_are_refused(lib):
     assert lib.refuse_next(following(o=0x100000, xs=1001)) and lib.refuse_next(following(o=0x100000 + 4000)) and lib.refuse_next(following(o=0x100004))
 
 
+def test_choices_whose_rows_overlap_what_is_read_beside_the_logits_are_refused(lib):
+    """another workgroup may read lengths, penalties and masks when one has written its part of the rows; the tokens are written behind all"""
+    ins = dict(hl=16, rep=16, pre=16, fre=16, m=4 * (3 * 40 + 32))
+    base = dict(rep=0xd00000, pre=0xe00000, fre=0xf00000, ms=40)
+    at = {**NEXT, **base}
+    outs = dict(o=16000, r=16000, c=16000, g=16000, ws=lib.next_workspace(4, 1000))
+    assert lib.refuse_next(following(**base)) is None
+    for a, size in ins.items():
+        for b, n in outs.items():
+            first = at[a] - n + 16
+            for x in (at[a], at[a] + (size - 4) // 16 * 16, first - first % 16):
+                assert lib.refuse_next(following(**{**base, b: x})), (a, b)
+            assert lib.refuse_next(following(**{**base, b: at[a] + -(-size // 16) * 16})) is None and lib.refuse_next(following(**{**base, b: at[a] - -(-n // 16) * 16})) is None, (a, b)
+        assert lib.refuse_next(following(**{**base, "t": at[a]})) is None and lib.refuse_next(following(**{**base, "mx": at[a]})) is None
+    # rows of the mask that are the same, and lengths that are not read
+    assert lib.refuse_next(following(**{**base, "ms": 0, "c": at["m"] + 128})) is None and lib.refuse_next(following(**{**base, "ms": 0, "c": at["m"] + 124}))
+    assert lib.refuse_next(following(**{**base, "history": 0, "c": at["hl"]})) is None
+
+
 def test_chunks_of_the_vocabulary(lib):
     out = (ctypes.c_uint32 * 2)()
     for n in (1, 2, 7, 64, 256, 1000, 65535):
