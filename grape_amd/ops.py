@@ -946,7 +946,8 @@ def wit_page_step(lens, new, block_table, free_pages, free_span, page_size, rows
     a request has left, go to the ring's end.  All int32.  Returns a dict of new tensors, or `out`, such a dict to write to: "starts" (seqs + 1),
     "positions" (rows) and "slots" (rows, int64: -1 behind the last token) for wit_rope_append and wit_window_attention, "lens" and
     "free_span" for the next step.  `rows` bounds the step's tokens; where they, the free pages or the ring's room do not suffice, bit 32 of
-    wit_status is set and the sequences from the first that does not fit get no tokens."""
+    wit_status is set and the sequences from the first that does not fit get no tokens.  lens has to be what the step before returned (0 for a new request): behind a
+    window a sequence cannot be made shorter, and without one the pages that it then no longer holds go to the ring's end by the caller's hand."""
     lib = init()
     dev = _place()
     n = len(lens)
@@ -976,7 +977,8 @@ def wit_window_attention(q, k_cache, v_cache, block_table, starts, lens, max_new
     sequence b with lens[b] tokens (themselves among them).  Each attends to what stands before it and to itself, with `window` > 0 only to the last
     `window` of these and the first `sinks`.  max_new and max_len bound the sequences' new tokens and lengths.  Returns the dict of
     wit_paged_attention, with rows in the place of seqs; positions that a token does not attend to and rows of no sequence are not
-    written (0 where the call makes the tensors).  `out` and `workspace` as there (wit_window_attention_workspace(...) bytes)."""
+    written (0 where the call makes the tensors).  `out` and `workspace` as there (wit_window_attention_workspace(...) bytes, which grow with rows times the positions
+    that a row may see; long prompts go piece by piece)."""
     lib = init()
     dev = _place()
     cache, heads_kv, dim = _cache(k_cache, v_cache, dev)
@@ -1029,7 +1031,7 @@ _NEXT_ROWS = ("logits", "rem", "count", "gap")
 
 def wit_next_token(logits, history=None, history_lens=None, repetition=None, presence=None, frequency=None, bias=None, mask=None, scale=1 << 16, out=None,
                    proof=True, workspace=None):
-    """The choice of the next token from logits (seqs, vocab).  A token that occurs among the first history_lens[b] of history (seqs, tokens;
+    """The choice of the next token from logits (seqs, vocab): the one with the largest, nothing is drawn at random.  A token that occurs among the first history_lens[b] of history (seqs, tokens;
     negative ones are skipped) has its logit divided (if positive) or multiplied (else) by repetition[b] / scale and lowered by presence[b] + frequency[b] for
     each time; bias (vocab) or (seqs, vocab) is added; mask (seqs, ceil(vocab / 32)) or one row of it holds a bit for each token that may be
     chosen, the first in a word's lowest.  All int32.  Returns a dict: "token" (seqs), the first with the largest logit or -1 where none may be chosen,

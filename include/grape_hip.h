@@ -789,6 +789,10 @@ int grape_wit_matvec_q4(int32_t *d_q, int32_t *d_r, const int32_t *d_x, int64_t 
  * again.  window and sinks must be those of the sequences' earlier steps.  A ring of twice as many entries as there are pages has
  * room for everything.
  *
+ * d_lens[b] must be what the step before left in d_lens_out[b], 0 for a new request.  A shorter one - drafted tokens that were not accepted
+ * - leaves pages behind it in nobody's hands, which the caller then puts at the ring's end, and is not possible behind a window, where
+ * pages that the longer sequence had left would be given back a second time.
+ *
  * Writes d_starts[seqs + 1], the rows at which the sequences' tokens start (row after row, sequence after sequence);
  * d_positions[rows] and d_slots[rows] (page*page_size + offset) of the tokens, 0 and -1 in rows behind the last; d_lens_out[seqs],
  * the lengths after the step (0 where the request is over); d_span_out, the ring's head and count after it.  Outputs must
@@ -797,7 +801,7 @@ int grape_wit_matvec_q4(int32_t *d_q, int32_t *d_r, const int32_t *d_x, int64_t 
  * Where the rows or the free pages do not suffice, GRAPE_WIT_PAGES is set and no sequence from the first one on that does not fit
  * gets a token; the same bit says that the ring had no room for a page given back, which is lost then.  A negative length or one that leaves the table,
  * d_new below -1 and a negative page set GRAPE_WIT_INDEX: such a sequence gets no token and keeps its length, a token of such a page slot -1.
- * At most 4096 sequences; table_stride*page_size and seqs*table_stride below 2^31. */
+ * At most 4096 sequences, as each workgroup holds the sums of all in LDS (20 bytes each); table_stride*page_size and seqs*table_stride below 2^31. */
 typedef struct {
     const int32_t *d_lens, *d_new, *d_span;
     int32_t *d_block_table, *d_free, *d_starts, *d_positions;
@@ -816,8 +820,14 @@ int grape_wit_page_step(const grape_wit_page_step_args *args, grape_stream_t str
  * max_new and max_len bound the sequences' new tokens and lengths.  A sequence outside these bounds, with fewer tokens than rows,
  * or with more than table_stride*page_size, sets GRAPE_WIT_INDEX, and its rows are left as they were: an entry of d_starts that is not in
  * 0..rows does that to the two sequences that it bounds.  The other entries ascend; where one does not (GRAPE_WIT_INDEX again), rows of any
- * sequence may be left as they were.  Pages that no token of the call sees are not read.  rows <= 2^24.  d_workspace as for grape_wit_paged_attention, grape_wit_window_attention_workspace(...)
- * bytes. */
+ * sequence may be left as they were.  Pages that no token of the call sees are not read.  rows <= 2^24.  Nothing runs where rows, seqs or
+ * max_new is 0, and calls whose launches would hold 2^27 workgroups or more are refused.
+ *
+ * A table whose entry 2^bit_shift - 1 - d is round(S exp(-d/S)), with S the entry of d = 0 and bit_shift <= 20, is computed instead of looked up where
+ * several tokens are new (max_new > 1); any other gives its own entries, in up to three times the time.  d_workspace as for
+ * grape_wit_paged_attention, grape_wit_window_attention_workspace(...) bytes: 8 for each row, head and position that a row may see (with
+ * max_new > 1 in whole tiles of 64, whether or not d_scores and d_exp are there), and what the launches share beside them.  2048 tokens of
+ * 32 heads take 1.1 GB behind nothing, 70 GB behind 129024 others and 2.3 GB with a window of 4096: long prompts without one go piece by piece. */
 typedef struct {
     const int32_t *d_q;
     int64_t q_stride;
@@ -831,7 +841,7 @@ typedef struct {
 size_t grape_wit_window_attention_workspace(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t cache_heads, uint32_t dim,
                                             uint32_t max_new, uint32_t max_len, uint32_t window, uint32_t sinks);
 int grape_wit_window_attention(const grape_wit_window_attention_args *args, const grape_wit_cache *cache, grape_stream_t stream);
-/* The choice of the next token.  Row b's logits x stand at d_logits + b*logits_stride, and count[v] is how often v is among the
+/* The choice of the next token: the one with the largest logit, nothing is drawn at random.  Row b's logits x stand at d_logits + b*logits_stride, and count[v] is how often v is among the
  * first d_history_lens[b] tokens at d_history + b*history_stride (negative ones are skipped).  Where count > 0
  *     x becomes floor((x*scale + floor(rep/2)) / rep) if x > 0, else floor((x*rep + floor(scale/2)) / scale), with rep = d_repetition[b],
  *     and then loses d_presence[b] + d_frequency[b]*count;

@@ -136,6 +136,30 @@ def test_pages_of_a_conversation(ops):
     assert ops.wit_status() == 0
 
 
+def test_drafted_tokens_are_taken_back(ops):
+    """without a window: a shorter length, and the pages behind it at the ring's end by the caller's hand; every page stays in one place"""
+    rng = np.random.default_rng(6)
+    seqs, page, pages, width = 5, 4, 200, 40
+    ring = np.full(2 * pages, -1, dtype=np.int32)
+    ring[:pages] = rng.permutation(pages)
+    ring, span, table, lens = dev(ring), dev(np.array([0, pages])), filled(seqs, width), dev(rng.integers(0, 1, seqs))
+    at = torch.arange(width, device="cuda")
+    for step in range(30):
+        out = ops.wit_page_step(lens, dev(rng.integers(1, 12, seqs)), table, ring, span, page, 60)
+        shorter = torch.maximum(lens, out["lens"] - dev(rng.integers(0, 9, seqs)))
+        up = lambda n: ((n + page - 1) // page)[:, None]  # noqa: E731
+        back = table[(at >= up(shorter)) & (at < up(out["lens"]))]
+        head, count = host(out["free_span"]).tolist()
+        ring[(head + count + torch.arange(len(back), device="cuda")) % (2 * pages)] = back
+        span, lens = dev(np.array([head, count + len(back)])), shorter
+        held = table[at < up(lens)]
+        free = ring[(head + torch.arange(count + len(back), device="cuda")) % (2 * pages)]
+        assert sorted(host(torch.cat((held, free))).tolist()) == list(range(pages)), step
+        if bool((lens > 130).any()):
+            break
+    assert ops.wit_status() == 0
+
+
 # ------------------------------------------------------------------ attention
 def run_window(ops, q, kc, vc, table, starts, lens, exp_table, max_new, max_len, window=0, sinks=0, proof=True, keep=None, **kw):
     rows, H, D = q.shape
