@@ -111,7 +111,7 @@ inline const char* refuse_next(const grape_wit_next_token_args* a) {
     GRAPE_REFUSE(a->seqs > 65535, "at most 65535 sequences");
     GRAPE_REFUSE(a->vocab < 1 || a->vocab > (uint32_t)1 << 24, "the vocabulary must have 1 to 2^24 tokens");
     GRAPE_REFUSE(a->scale < 1 || a->scale > (int64_t)1 << 31, "scale must be in 1..2^31 (the remainder is stored as int32)");
-    GRAPE_REFUSE(a->history > (uint32_t)1 << 24, "at most 2^24 tokens of history");          // each of up to 8192 workgroups of a row reads it all
+    GRAPE_REFUSE(a->history > (uint32_t)1 << 24, "at most 2^24 tokens of history");          // each of up to 2048 workgroups of a row reads it all
     const int64_t most = (int64_t)1 << 40;
     GRAPE_REFUSE(a->logits_stride < 0 || a->history_stride < 0 || a->bias_stride < 0 || a->mask_stride < 0, "negative stride");
     GRAPE_REFUSE(a->logits_stride >= most || a->history_stride >= most || a->bias_stride >= most || a->mask_stride >= most, "stride of 2^40 or more");

@@ -15,16 +15,20 @@ namespace grape {
 // a fourth that joins the values' partial sums where the positions are cut up.  Rows of 32 are two operands of a product for each key
 // that is loaded; 16 would read keys and values twice as often, 64 leave no registers for the five sums of the planes' products.
 //
-// 2048 new tokens, 32 heads of 128 over 8, with a proof (1.34 GB written, 0.54 GB of it read again): 46 us operands, 158 scores, 208
-// exponentials, 248 values, each of the last three near what it writes and reads at 3.3 to 4 TB/s.  One head of 4096: 63 + 112 + 18 + 139 us, of which 142
-// to 176 are the products' at the rate of a large int8 one.  5 drafted tokens of 8 sequences of up to 3000: 35 + 15 + 39 + 5 us, chains of
+// 2048 new tokens, 32 heads of 128 over 8, with a proof (1.68 GB written, 0.54 GB of it read again): 47 us operands, 158 scores, 209
+// exponentials, 246 values, each of the last three near what it writes and reads at 3.4 to 3.9 TB/s.  One head of 4096: 63 + 113-117 + 18 + 139-144 us; its products alone
+// would take 103 at the 2.5 POP/s that the kernel of a large int8 product reaches.  5 drafted tokens of 8 sequences of up to 3000: 35 + 15 + 39 + 5 us, chains of
 // dependent loads in short workgroups; a fourth wave of registers (128 of them) or other chunks are no faster.
 //
 // Both products run on the int8 matrix cores, exactly.  An element of magnitude below 2^23 is three balanced digits of base 256, the bytes
 // of x + 0x808080 with their top bits turned over, nine products of planes for a pair of operands and six where the probabilities
 // are small; pairs with the same sum of exponents share an accumulator (3 * 2^14 * 8192 elements stay below 2^31).  Where a larger
-// element turns up, the wave (or, for the values, the workgroup) takes its positions again with x - c, c = 128 (1 + 2^8 + 2^16), whose four
-// digits are the bytes of x with the three lower top bits turned over: sum q k = sum (q-c)(k-c) + c (sum (q-c) + sum (k-c)) + c^2 dim.
+// element turns up, positions are taken again with x - c, c = 128 (1 + 2^8 + 2^16), whose four digits are the bytes of x with the
+// three lower top bits turned over: sum q k = sum (q-c)(k-c) + c (sum (q-c) + sum (k-c)) + c^2 dim.  For a large key these are the sixteen
+// positions that its wave takes of each tile of the chunk; with operands made beforehand, or for a large query, all of the chunk; for a large value the
+// workgroup's whole chunk.  That is meant to be right, not fast: its operands come element by element with nothing under way.  The 2048 tokens
+// above take 655 us without a large element, 2139 with one key, 2454 with one key in a hundred, 769 with one value and 804 with one in a hundred; one head of
+// 4096 311, 745, 1664, 440 and 503; five drafted tokens 76, 107, 178, 88 and 93 (each time with the same inputs again and again).
 // ------------------------------------------------------------------------------------------------
 using step::kCols;
 using step::kRows;
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(256) wit_window_pack_kernel(WindowArgs p) {
 // Five accumulators become a sum in double precision, exact below 2^53, and below 2^50 the quotient of (y + s/2 + 1/2) / s needs no
 // second look: it is no nearer than 1 / (2 s) to a whole number, and the product with 1 / s off by at most 2^-52 of itself.
 // Bound by vector instructions and stores together where a proof is made (the 2048 tokens above: 158 us, 3.7 TB/s); heads of 4096 reach 1.4 POP/s of
-// the 1.8 that a large int8 product does (112 us; 130 when a block of queries was loaded between two barriers and not beside the products).
+// the 2.5 that a large int8 product does, by 1.05e7 requests of L2, up to 1.3 GB (113 us; 130 when a block of queries was loaded between two barriers and not beside the products).
 template <bool PACKED, bool VEC, bool REM>
 __global__ void __launch_bounds__(256, 2) wit_window_scores_kernel(WindowArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
@@ -800,7 +804,7 @@ __global__ void __launch_bounds__(256) wit_window_exp_kernel(WindowArgs p) {
 // probability is floor((e P + floor(S/2)) / S) from one product in double precision, as the scores' quotients are, where S is below 2^28 and P
 // at most 2^22; the remainder of the division gives the lookup's query.  Four waves of 32 elements leave 256 registers each, of which the sums
 // take 80 to 112 and spill a few.  Heads of more than 128 elements are divided among workgroups that make the probabilities again (one head of
-// 4096: 139 us).
+// 4096: 140 us, 0.74 POP/s of six products of planes, 1.4e7 requests of L2).
 constexpr uint32_t kValueThreads = 256;
 constexpr uint64_t kPlainSum = (uint64_t)1 << 28;
 enum Written { kNone, kBoth, kSome };          // of the probabilities and queries
